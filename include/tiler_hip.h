@@ -765,6 +765,91 @@ tiler_hip_status tiler_hip_contract(tiler_hip_context *ctx, uint32_t dtype,
                                     const void *right, void *out, tiler_hip_stream stream);
 
 /* ------------------------------------------------------------------------
+ * The feed-forward sublayer of a language model: layer norm, the gated
+ * product, each with its gradients, and the 8-bit linear layer.  No
+ * counterpart in the reference, which has no backward pass, no mean-centred
+ * norm and no 8-bit product.  Tensors are dense row-major, at any alignment of
+ * their elements; outputs overlap neither the inputs nor one another.  Every
+ * call is deterministic, launches on `stream` and may be captured into a graph.
+ *
+ * Workspace: a call that needs device memory of its own takes it as
+ * (workspace, workspace_bytes), 16-byte aligned and at least what the matching
+ * *_workspace query answers; its contents need no clearing and mean nothing
+ * after the call.  Calls that may overlap (two streams, two captured graphs)
+ * need one each.  NULL: the context's call scratch, or an allocation on the
+ * stream, which refuses under graph capture (TILER_HIP_REFUSE_CAPACITY). */
+
+/* Layer normalization over the last axis, with mu the row's mean and
+ * r = 1 / sqrt(mean((x - mu)^2) + eps):
+ *   y = (x - mu) r w + b
+ * dtype TILER_HIP_F32 or TILER_HIP_BF16 (binary32 arithmetic on exactly
+ * widened operands, one narrowing of y).  w and b are one row of `extent`
+ * each; NULL reads as ones and as zeros.  mean and rstd (f32 [rows], both or
+ * neither) receive mu and r for the gradients.  eps positive and finite; rows
+ * up to 2^32 - 1 elements.  The variance is that of the differences from the
+ * mean, never a difference of squares.  A row holding a NaN or an infinity
+ * gives NaNs. */
+tiler_hip_status tiler_hip_layer_norm(tiler_hip_context *ctx, uint32_t dtype, const void *x,
+                                      const void *w, const void *b, uint64_t rows, uint64_t extent,
+                                      uint32_t eps_bits, void *y, float *mean, float *rstd,
+                                      tiler_hip_stream stream);
+/* Its gradients, with xh = (x - mu) r and g = dy w:
+ *   dx = r (g - mean(g) - xh mean(g xh)), dw = sum over rows of dy xh, db = of dy
+ * mean and rstd as the forward call wrote them.  Any of dx, dw and db may be
+ * NULL (not wanted).  With no rows dw and db are zeros.  Sums in binary32 or
+ * more, in a fixed order. */
+tiler_hip_status tiler_hip_layer_norm_backward(tiler_hip_context *ctx, uint32_t dtype, const void *dy,
+                                               const void *x, const void *w, const float *mean,
+                                               const float *rstd, uint64_t rows, uint64_t extent, void *dx,
+                                               void *dw, void *db, void *workspace,
+                                               uint64_t workspace_bytes, tiler_hip_stream stream);
+/* The largest workspace a backward call of these sizes takes.  ctx may be NULL
+ * (the declared profile's device). */
+tiler_hip_status tiler_hip_layer_norm_backward_workspace(const tiler_hip_context *ctx, uint32_t dtype,
+                                                         uint64_t rows, uint64_t extent, uint64_t *bytes);
+
+/* The gated feed-forward product, bf16 operands and results, f32 sums:
+ *   G = x Wg^T, U = x Wu^T, h = silu(G) * U
+ * x [m, k], wg and wu [n, k] (td,od->to), h [m, n].  h comes from the f32 sums,
+ * rounded once.  gate and up (bf16 [m, n], both or neither) receive G and U
+ * for the gradients.  k at least 1. */
+tiler_hip_status tiler_hip_gated_contract_bf16(tiler_hip_context *ctx, const uint16_t *x,
+                                               const uint16_t *wg, const uint16_t *wu, uint64_t m,
+                                               uint64_t n, uint64_t k, uint16_t *h, uint16_t *gate,
+                                               uint16_t *up, tiler_hip_stream stream);
+/* Its gradients from the kept G and U, with s = 1 / (1 + e^-G):
+ *   dU = dh G s, dG = dh U s (1 + G (1 - s))       rounded to bf16
+ *   dx = dG Wg + dU Wu, dwg = dG^T x, dwu = dU^T x
+ * dx may be NULL, dwg and dwu may both be NULL (not wanted).  With m = 0 the
+ * weights' gradients are zeros, with n = 0 dx is. */
+tiler_hip_status tiler_hip_gated_contract_bf16_backward(
+    tiler_hip_context *ctx, const uint16_t *x, const uint16_t *wg, const uint16_t *wu,
+    const uint16_t *gate, const uint16_t *up, const uint16_t *dh, uint64_t m, uint64_t n, uint64_t k,
+    uint16_t *dx, uint16_t *dwg, uint16_t *dwu, void *workspace, uint64_t workspace_bytes,
+    tiler_hip_stream stream);
+tiler_hip_status tiler_hip_gated_contract_bf16_backward_workspace(const tiler_hip_context *ctx, uint64_t m,
+                                                                  uint64_t n, uint64_t k, uint64_t *bytes);
+
+/* Rows in 8 bits with one scale each (dtype of x: TILER_HIP_F32 or
+ * TILER_HIP_BF16):
+ *   scales[i] = max(fl(max |x_i| / 127), 2^-126), q_ij = x_ij / scales[i] to the
+ *   nearest integer, ties to even, exactly (in -127 .. 127)
+ * A row holding a NaN or an infinity has the scale NaN and codes 0, so that
+ * what is computed from it is NaN. */
+tiler_hip_status tiler_hip_quantize_rows_i8(tiler_hip_context *ctx, uint32_t dtype, const void *x,
+                                            uint64_t rows, uint64_t extent, int8_t *q, float *scales,
+                                            tiler_hip_stream stream);
+/* Contraction td,od->to of int8 operands with a scale per row of each:
+ *   c[i, j] = fl(fl(fl(sum_k a_ik b_jk) a_scales[i]) b_scales[j])
+ * The sum is an exact integer (k at most 131071, any codes), fl rounds to
+ * binary32; dtype TILER_HIP_F32, or TILER_HIP_BF16 for one more narrowing.
+ * a [m, k], b [n, k], a_scales [m], b_scales [n], c [m, n]. */
+tiler_hip_status tiler_hip_contract_i8(tiler_hip_context *ctx, const int8_t *a, const int8_t *b,
+                                       const float *a_scales, const float *b_scales, uint64_t m,
+                                       uint64_t n, uint64_t k, uint32_t dtype, void *c,
+                                       tiler_hip_stream stream);
+
+/* ------------------------------------------------------------------------
  * Realization recognizer: one scheduled region -> the dispatches that realize
  * it on this library's entry points.  It takes the role of tiler-metal's
  * emit_entry_point (tiler-metal/src/emit.rs:647-840) for a backend whose code
@@ -803,6 +888,26 @@ tiler_hip_status tiler_hip_contract(tiler_hip_context *ctx, uint32_t dtype,
                                               scale, zero point, y, and a 4-byte scratch slot where the
                                               kernel records the operands' domain verdict (0 in domain,
                                               1 scale, 2 zero point); extents[0] = element count */
+
+/* The feed-forward sublayer's programs (families of this library, with no
+ * ScalarProgram in the reference).  `variant` says which optional operands and
+ * results the region has; slots only for those. */
+#define TILER_HIP_PROGRAM_LAYER_NORM 13          /* extents {rows, extent}, scalars {eps bits};
+                                                    TILER_HIP_NORM_{WEIGHT,BIAS,STATISTICS} */
+#define TILER_HIP_PROGRAM_LAYER_NORM_BACKWARD 14 /* extents {rows, extent}; TILER_HIP_NORM_{WEIGHT,DX,DW,DB} */
+#define TILER_HIP_PROGRAM_GATED_CONTRACTION 15   /* bf16, extents {m, n, k}; TILER_HIP_GATED_KEEP */
+#define TILER_HIP_PROGRAM_GATED_CONTRACTION_BACKWARD 16 /* bf16, extents {m, n, k}; TILER_HIP_GATED_{DX,DW} */
+#define TILER_HIP_PROGRAM_QUANTIZE_ROWS_I8 17    /* dtype: x's; extents {rows, extent}; variant 0 */
+#define TILER_HIP_PROGRAM_CONTRACTION_I8 18      /* dtype: the result's; extents {m, n, k}; variant 0 */
+#define TILER_HIP_NORM_WEIGHT 1u
+#define TILER_HIP_NORM_BIAS 2u
+#define TILER_HIP_NORM_STATISTICS 4u
+#define TILER_HIP_NORM_DX 8u
+#define TILER_HIP_NORM_DW 16u
+#define TILER_HIP_NORM_DB 32u
+#define TILER_HIP_GATED_KEEP 1u
+#define TILER_HIP_GATED_DX 2u
+#define TILER_HIP_GATED_DW 4u
 
 /* PROGRAM_FOLD variants.  The input is dense row-major with `rank` dims in
  * extents[]; grouping[0] is the reduced-axis mask (bit d: axis d reduced);
@@ -927,7 +1032,13 @@ typedef struct {
  *               out of range; then the lowest such position).  The program arms the
  *               record itself; validate host indices first (tiler_hip_validate_gather_index).
  *   broadcast   src, out
- *   convert     src, dst */
+ *   convert     src, dst
+ *   layer norm  x, [w,] [b,] y, [mean, rstd]
+ *   layer norm backward  dy, x, [w,] mean, rstd, [dx,] [dw,] [db,] then scratch slots
+ *   gated contraction    x, wg, wu, h, [gate, up]
+ *   gated contraction backward  x, wg, wu, gate, up, dh, [dx,] [dwg, dwu,] then scratch slots
+ *   quantize rows        x, q, scales
+ *   contraction i8       a, b, a_scales, b_scales, c */
 #define TILER_HIP_SLOT_INPUT 0
 #define TILER_HIP_SLOT_OUTPUT 1
 #define TILER_HIP_SLOT_SCRATCH 2

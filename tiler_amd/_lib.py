@@ -64,6 +64,22 @@ PROGRAM_EXPRESSION = 9
 PROGRAM_FOLD = 10
 PROGRAM_REINDEX = 11
 PROGRAM_DEQUANTIZE_U4 = 12
+PROGRAM_LAYER_NORM = 13
+PROGRAM_LAYER_NORM_BACKWARD = 14
+PROGRAM_GATED_CONTRACTION = 15
+PROGRAM_GATED_CONTRACTION_BACKWARD = 16
+PROGRAM_QUANTIZE_ROWS_I8 = 17
+PROGRAM_CONTRACTION_I8 = 18
+
+NORM_WEIGHT = 1
+NORM_BIAS = 2
+NORM_STATISTICS = 4
+NORM_DX = 8
+NORM_DW = 16
+NORM_DB = 32
+GATED_KEEP = 1
+GATED_DX = 2
+GATED_DW = 4
 
 FOLD_SUM = 0
 FOLD_SQUARED = 1
@@ -494,6 +510,15 @@ SIGNATURES = {
     "tiler_hip_contract_strict_f32": (_S, [_CTX, _P, _P, _U64, _U64, _U64, _P, _P]),
     "tiler_hip_contract_bf16": (_S, [_CTX, _P, _P, _U64, _U64, _U64, _P, _U32, _P]),
     "tiler_hip_contract": (_S, [_CTX, _U32, ctypes.POINTER(ContractionStructure), _U32, _U32, _P, _P, _P, _P]),
+    "tiler_hip_layer_norm": (_S, [_CTX, _U32, _P, _P, _P, _U64, _U64, _U32, _P, _P, _P, _P]),
+    "tiler_hip_layer_norm_backward": (_S, [_CTX, _U32, _P, _P, _P, _P, _P, _U64, _U64, _P, _P, _P, _P, _U64, _P]),
+    "tiler_hip_layer_norm_backward_workspace": (_S, [_CTX, _U32, _U64, _U64, ctypes.POINTER(_U64)]),
+    "tiler_hip_gated_contract_bf16": (_S, [_CTX, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _P]),
+    "tiler_hip_gated_contract_bf16_backward": (_S, [_CTX, _P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _P,
+                                                    _U64, _P]),
+    "tiler_hip_gated_contract_bf16_backward_workspace": (_S, [_CTX, _U64, _U64, _U64, ctypes.POINTER(_U64)]),
+    "tiler_hip_quantize_rows_i8": (_S, [_CTX, _U32, _P, _U64, _U64, _P, _P, _P]),
+    "tiler_hip_contract_i8": (_S, [_CTX, _P, _P, _P, _P, _U64, _U64, _U64, _U32, _P, _P]),
     "tiler_hip_realize": (_S, [_CTX, ctypes.POINTER(Region), ctypes.POINTER(Realization),
                                ctypes.c_char_p, _U64]),
     "tiler_hip_propose": (_S, [_CTX, ctypes.POINTER(Region), ctypes.POINTER(ProviderOffer),

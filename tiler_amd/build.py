@@ -76,6 +76,7 @@ def build(verbose: bool = False) -> str:
           "-o", tmp_lib,
           os.path.join(CSRC, "runtime", "tiler_hip.cpp"),
           os.path.join(CSRC, "runtime", "program.cpp"),
+          os.path.join(CSRC, "runtime", "feed_forward.cpp"),
           os.path.join(CSRC, "runtime", "digest.cpp"),
           os.path.join(CSRC, "runtime", "envelope.cpp"),
           os.path.join(CSRC, "runtime", "code_object.cpp"),

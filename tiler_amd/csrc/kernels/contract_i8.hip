@@ -1,0 +1,139 @@
+// The 8-bit linear layer for gfx950: rows quantized to int8 with one binary32
+// scale each, and the product of two such operands,
+//
+//   C[i, j] = (sum over k of a_ik b_jk) sa_i sb_j     (a [m, k], b [n, k])
+//
+// on v_mfma_i32_16x16x64_i8.  The integer sum is exact (k <= 131071 keeps
+// |sum| <= 2^31 - 2^14 for every pair of codes, -128 included); it is rounded
+// to binary32, multiplied by sa_i, then by sb_j, and narrowed to bf16 where C is bf16.
+#include "product.h"
+
+namespace {
+
+using tiler_product::I8;
+using tiler_product::Operand;
+using tiler_product::i32x4;
+using tiler_product::kSlice;
+
+// s = max(max |x| / 127, 2^-126), the quotient correctly rounded; q = x / s to
+// the nearest integer, ties to even, exactly: the candidate rint(x * (1 / s))
+// is at most one off, next to a tie; d = x - r s is exact in one FMA (a
+// multiple of s's last place below 2 s, or x itself when r = 0), so comparing
+// it with the exact s / 2 decides.  |x| <= 127 s (1 + 2^-24), so |q| <= 127.
+__device__ __forceinline__ float row_scale(float largest) {
+  const float s = largest / 127.0f;
+  return s < 0x1p-126f ? 0x1p-126f : s;
+}
+__device__ __forceinline__ int32_t code_of(float x, float s, float inverse) {
+  float r = __builtin_rintf(x * inverse);
+  const float d = __builtin_fmaf(-r, s, x), half = 0.5f * s;
+  const bool odd = ((int32_t)r) & 1;
+  if (d > half || (odd && d == half)) r += 1.0f;
+  else if (-d > half || (odd && -d == half)) r -= 1.0f;
+  return (int32_t)r;
+}
+
+// |x| and whether it is not finite, folded over a row: the magnitude's bits
+// order as the magnitudes do, infinity and NaN last.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// One workgroup per row, any extent and alignment: the row is read twice, the
+// second time from the caches.
+template <typename T>
+__device__ __forceinline__ void quantize_rows_body(const T* __restrict__ x, uint64_t rows, uint64_t extent,
+                                                   int8_t* __restrict__ q, float* __restrict__ scales) {
+  __shared__ uint32_t waves[4];
+  for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * extent;
+    int8_t* qr = q + row * extent;
+    auto value = [&](uint64_t i) {
+      if constexpr (sizeof(T) == 2) return tiler::bf16_widen(xr[i]);
+      else return xr[i];
+    };
+    uint32_t top = 0;
+    for (uint64_t i = threadIdx.x; i < extent; i += 256u) {
+      const uint32_t b = magnitude(value(i));
+      top = b > top ? b : top;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const uint32_t other = __shfl_xor(top, o, 64);
+      top = other > top ? other : top;
+    }
+    __syncthreads();  // the row before is done with the waves' words
+    if ((threadIdx.x & 63u) == 0) waves[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = waves[w] > top ? waves[w] : top;
+    const bool finite = top < 0x7f800000u;
+    const float s = finite ? row_scale(__uint_as_float(top)) : __uint_as_float(TILER_CANONICAL_F32_NAN);
+    const float inverse = 1.0f / s;
+    if (threadIdx.x == 0) scales[row] = s;
+    for (uint64_t i = threadIdx.x; i < extent; i += 256u)
+      qr[i] = finite ? (int8_t)code_of(value(i), s, inverse) : (int8_t)0;
+  }
+}
+
+}  // namespace
+
+extern "C" __global__ void __launch_bounds__(256)
+tiler_quantize_rows_i8_bf16(const uint16_t* __restrict__ x, uint64_t rows, uint64_t extent, int8_t* __restrict__ q,
+                            float* __restrict__ scales) {
+  quantize_rows_body<uint16_t>(x, rows, extent, q, scales);
+}
+extern "C" __global__ void __launch_bounds__(256)
+tiler_quantize_rows_i8_f32(const float* __restrict__ x, uint64_t rows, uint64_t extent, int8_t* __restrict__ q,
+                           float* __restrict__ scales) {
+  quantize_rows_body<float>(x, rows, extent, q, scales);
+}
+
+namespace {
+
+__device__ __forceinline__ float scaled(int32_t sum, float sa, float sb) { return tiler::canon((float)sum * sa * sb); }
+
+// Guarded form: 128 x 128 tiles, any sizes and alignments.
+template <bool kBf16>
+__device__ __forceinline__ void contract_i8_guarded(const int8_t* __restrict__ a, const int8_t* __restrict__ b,
+                                                    const float* __restrict__ sa, const float* __restrict__ sb,
+                                                    uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * 256u * kSlice];
+  const uint32_t m0 = blockIdx.y * 128u, n0 = blockIdx.x * 128u;
+  const Operand oa{reinterpret_cast<const uint8_t*>(a), k, m, k}, ob{reinterpret_cast<const uint8_t*>(b), k, n, k};
+  i32x4 acc[4][4];
+  tiler_product::guarded_product<I8, false, false, 2, 2, 4, 4>(
+      smem, (k + 127u) / 128u,
+      [&](uint32_t t, uint32_t r, uint32_t p) { return tiler_product::operand_piece<I8, false>(oa, m0, t * 128u, r, p); },
+      [&](uint32_t t, uint32_t r, uint32_t p) { return tiler_product::operand_piece<I8, false>(ob, n0, t * 128u, r, p); },
+      acc);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t col = n0 + (wave & 1u) * 64u + j * 16u + (lane & 15u);
+    if (col >= n) continue;
+    const float cs = sb[col];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t row = m0 + (wave >> 1) * 64u + i * 16u + (lane >> 4) * 4u + r;
+        if (row >= m) continue;
+        const float v = scaled(acc[i][j][r], sa[row], cs);
+        const uint64_t at = (uint64_t)row * n + col;
+        if constexpr (kBf16) static_cast<uint16_t*>(c)[at] = (uint16_t)tiler::bf16_narrow(v);
+        else static_cast<float*>(c)[at] = v;
+      }
+  }
+}
+
+}  // namespace
+
+extern "C" __global__ void __launch_bounds__(256)
+tiler_contract_i8_bf16_g(const int8_t* __restrict__ a, const int8_t* __restrict__ b, const float* __restrict__ sa,
+                         const float* __restrict__ sb, uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
+  contract_i8_guarded<true>(a, b, sa, sb, m, n, k, c);
+}
+extern "C" __global__ void __launch_bounds__(256)
+tiler_contract_i8_f32_g(const int8_t* __restrict__ a, const int8_t* __restrict__ b, const float* __restrict__ sa,
+                        const float* __restrict__ sb, uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
+  contract_i8_guarded<false>(a, b, sa, sb, m, n, k, c);
+}

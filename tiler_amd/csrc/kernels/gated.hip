@@ -1,0 +1,185 @@
+// The gated feed-forward product and its gradients for gfx950, bf16 on MFMA
+// with f32 accumulation:
+//
+//   G = x Wg^T, U = x Wu^T, h = silu(G) U          (x [m, k]; Wg, Wu [n, k])
+//   dU = dh silu(G), dG = dh U s (1 + G (1 - s))    s = 1 / (1 + e^-G)
+//   dx = dG Wg + dU Wu, dWg = dG^T x, dWu = dU^T x
+//
+// Forward: one kernel reads x once for both projections; a wave's columns are
+// half gate, half up (the same 32 of each), so both sums of an output meet in
+// one lane's registers and the activation and the product need no exchange.
+// h is taken from the f32 sums and rounded once; G and U, where kept, are the
+// same sums rounded once.
+//
+// Backward: dG and dU are formed once per element from the kept G and U and
+// rounded to bf16 (the matrix pipe's operand type; one rounding of each term
+// of a sum, as independent as the terms), then dx contracts them with the
+// weights as they lie (the weights' rows are its depth) and dWg, dWu with x
+// over the tokens (both operands in column layout).
+#include "product.h"
+
+namespace {
+
+using tiler_product::Bf16;
+using tiler_product::Operand;
+using tiler_product::kSlice;
+
+// e^-v by the hardware exponential; 1 / (1 + e) by the hardware reciprocal:
+// a few binary32 steps from the sigmoid, and the value is rounded to bf16 (or
+// multiplied into one) next.  +-inf and NaN as the formula gives them.
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -0x1.715476p+0f));
+}
+
+// Guarded form: 128 tokens x (64 gate + 64 up) columns, any sizes and
+// alignments.  Row r of the B tile: gate (r & 32 == 0) or up row
+// (r >> 6) * 32 + (r & 31) of the 64-column tile.
+constexpr int kW = 2, kMB = 4, kNB = 4;  // 2 x 2 waves of 4 x 4 blocks
+constexpr uint32_t kGuardedBytes = 2u * 256u * kSlice;
+
+}  // namespace
+
+extern "C" __global__ void __launch_bounds__(256)
+tiler_gated_bf16_g(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu,
+                   uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
+                   uint16_t* __restrict__ up) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
+  const uint32_t m0 = blockIdx.y * 128u, n0 = blockIdx.x * 64u;
+  const Operand a{reinterpret_cast<const uint8_t*>(x), k, m, k};
+  // (a distance, not a choice of two captured pointers, which the compiler keeps in memory)
+  const int64_t between = reinterpret_cast<const uint8_t*>(wu) - reinterpret_cast<const uint8_t*>(wg);
+  f32x4 acc[kMB][kNB];
+  tiler_product::guarded_product<Bf16, false, false, kW, kW, kMB, kNB>(
+      smem, (k + 63u) / 64u,
+      [=](uint32_t t, uint32_t r, uint32_t c) { return tiler_product::operand_piece<Bf16, false>(a, m0, t * 64u, r, c); },
+      [=](uint32_t t, uint32_t r, uint32_t c) {
+        const uint32_t col = (r >> 6) * 32u + (r & 31u);
+        const Operand b{reinterpret_cast<const uint8_t*>(wg) + ((r & 32u) ? between : 0), k, n, k};
+        return tiler_product::operand_piece<Bf16, false>(b, n0, t * 64u, col, c);
+      },
+      acc);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < kMB; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t row = m0 + (wave / kW) * 64u + i * 16u + (lane >> 4) * 4u + r;
+        const uint32_t col = n0 + (wave % kW) * 32u + j * 16u + (lane & 15u);
+        if (row >= m || col >= n) continue;
+        const float g = acc[i][j][r], u = acc[i][j + 2][r];
+        const uint64_t at = (uint64_t)row * n + col;
+        h[at] = (uint16_t)tiler::bf16_narrow(g * sigmoid(g) * u);
+        if (gate) {
+          gate[at] = (uint16_t)tiler::bf16_narrow(g);
+          up[at] = (uint16_t)tiler::bf16_narrow(u);
+        }
+      }
+}
+
+// dG and dU of one row's eight columns per thread, into rows of `ld` elements
+// (a multiple of 64; the columns past n are written as zeros).
+extern "C" __global__ void __launch_bounds__(256)
+tiler_gated_bf16_grad(const uint16_t* __restrict__ gate, const uint16_t* __restrict__ up,
+                      const uint16_t* __restrict__ dh, uint32_t m, uint32_t n, uint32_t ld, uint16_t* __restrict__ dg,
+                      uint16_t* __restrict__ du) {
+  const uint32_t per = ld / 8u;
+  const uint64_t total = (uint64_t)m * per;
+  for (uint64_t id = blockIdx.x * 256ull + threadIdx.x; id < total; id += gridDim.x * 256ull) {
+    const uint32_t row = (uint32_t)(id / per), col = (uint32_t)(id % per) * 8u;
+    const uint64_t at = (uint64_t)row * n + col;
+    const uint32_t valid = col >= n ? 0u : n - col < 8u ? (n - col) * 2u : 16u;
+    u32x4 vg = {0, 0, 0, 0}, vu = vg, vd = vg;
+    if (valid) {
+      auto piece = [&](const uint16_t* q) {
+        return tiler_product::guarded_piece(reinterpret_cast<const uint8_t*>(q + at), valid,
+                                            reinterpret_cast<const uint8_t*>(q));
+      };
+      vg = piece(gate);
+      vu = piece(up);
+      vd = piece(dh);
+    }
+    u32x4 og, ou;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float g2[2], u2[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const float g = tiler::bf16_widen((vg[e] >> (16 * p)) & 0xffffu), u = tiler::bf16_widen((vu[e] >> (16 * p)) & 0xffffu);
+        const float d = tiler::bf16_widen((vd[e] >> (16 * p)) & 0xffffu), s = sigmoid(g);
+        g2[p] = d * u * s * (1.0f + g * (1.0f - s));
+        u2[p] = d * g * s;
+      }
+      og[e] = tiler::bf16_pack2_rne(g2[0], g2[1]);
+      ou[e] = tiler::bf16_pack2_rne(u2[0], u2[1]);
+    }
+    const uint64_t to = (uint64_t)row * ld + col;
+    *reinterpret_cast<u32x4*>(dg + to) = og;
+    *reinterpret_cast<u32x4*>(du + to) = ou;
+  }
+}
+
+// dx [m, k] = dG Wg + dU Wu: depth n twice (dG with Wg, then dU with Wu), the
+// weights in column layout.  Guarded: 128 x 128 tiles, any sizes.
+extern "C" __global__ void __launch_bounds__(256)
+tiler_gated_bf16_dx_g(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,
+                      const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m, uint32_t n,
+                      uint32_t k, uint16_t* __restrict__ dx) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
+  const uint32_t m0 = blockIdx.y * 128u, c0 = blockIdx.x * 128u, per = (n + 63u) / 64u;
+  f32x4 acc[kMB][kNB];
+  tiler_product::guarded_product<Bf16, false, true, kW, kW, kMB, kNB>(
+      smem, 2u * per,
+      [=](uint32_t t, uint32_t r, uint32_t c) {
+        const Operand a{reinterpret_cast<const uint8_t*>(t < per ? dg : du), ld, m, n};
+        return tiler_product::operand_piece<Bf16, false>(a, m0, (t < per ? t : t - per) * 64u, r, c);
+      },
+      [=](uint32_t t, uint32_t r, uint32_t c) {
+        const Operand b{reinterpret_cast<const uint8_t*>(t < per ? wg : wu), k, k, n};
+        return tiler_product::operand_piece<Bf16, true>(b, c0, (t < per ? t : t - per) * 64u, r, c);
+      },
+      acc);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < kMB; ++i)
+#pragma unroll
+    for (int j = 0; j < kNB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t row = m0 + (wave / kW) * 64u + i * 16u + (lane >> 4) * 4u + r;
+        const uint32_t col = c0 + (wave % kW) * 64u + j * 16u + (lane & 15u);
+        if (row < m && col < k) dx[(uint64_t)row * k + col] = (uint16_t)tiler::bf16_narrow(acc[i][j][r]);
+      }
+}
+
+// dWg [n, k] = dG^T x and dWu = dU^T x (blockIdx.z): depth m, both operands in
+// column layout.  Guarded: 128 x 128 tiles, any sizes.  tiles_n row tiles each.
+extern "C" __global__ void __launch_bounds__(256)
+tiler_gated_bf16_dw_g(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,
+                      const uint16_t* __restrict__ x, uint32_t m, uint32_t n, uint32_t k, uint32_t tiles_n,
+                      uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
+  const bool second = blockIdx.y >= tiles_n;
+  const uint32_t j0 = (second ? blockIdx.y - tiles_n : blockIdx.y) * 128u, c0 = blockIdx.x * 128u;
+  const Operand a{reinterpret_cast<const uint8_t*>(second ? du : dg), ld, n, m};
+  const Operand b{reinterpret_cast<const uint8_t*>(x), k, k, m};
+  f32x4 acc[kMB][kNB];
+  tiler_product::guarded_product<Bf16, true, true, kW, kW, kMB, kNB>(
+      smem, (m + 63u) / 64u,
+      [=](uint32_t t, uint32_t r, uint32_t c) { return tiler_product::operand_piece<Bf16, true>(a, j0, t * 64u, r, c); },
+      [=](uint32_t t, uint32_t r, uint32_t c) { return tiler_product::operand_piece<Bf16, true>(b, c0, t * 64u, r, c); },
+      acc);
+  uint16_t* out = second ? dwu : dwg;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < kMB; ++i)
+#pragma unroll
+    for (int j = 0; j < kNB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t row = j0 + (wave / kW) * 64u + i * 16u + (lane >> 4) * 4u + r;
+        const uint32_t col = c0 + (wave % kW) * 64u + j * 16u + (lane & 15u);
+        if (row < n && col < k) out[(uint64_t)row * k + col] = (uint16_t)tiler::bf16_narrow(acc[i][j][r]);
+      }
+}

@@ -14,3 +14,6 @@
 #include "contract_ksplit.hip"
 #include "contract_general.hip"
 #include "dequantize.hip"
+#include "layer_norm.hip"
+#include "gated.hip"
+#include "contract_i8.hip"

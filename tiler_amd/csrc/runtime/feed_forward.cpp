@@ -1,0 +1,203 @@
+// Planners of the feed-forward sublayer's families: layer norm and its
+// gradients, the gated product and its gradients, the 8-bit linear layer.
+#include "program.h"
+
+#include <cmath>
+#include <cstdio>
+
+namespace tiler_rt {
+
+namespace {
+
+uint64_t mul_sat(uint64_t a, uint64_t b) { return a && b > UINT64_MAX / a ? UINT64_MAX : a * b; }
+uint64_t add_sat(uint64_t a, uint64_t b) { return a > UINT64_MAX - b ? UINT64_MAX : a + b; }
+uint64_t ceil_div(uint64_t a, uint64_t b) { return a / b + (a % b != 0); }
+
+// Whether one launch holds this many workgroups along x: the runtime takes
+// fewer than 2^32 work items.
+bool grid_holds(uint64_t workgroups, uint32_t threads) { return workgroups <= 0xffffffffull / threads; }
+
+const char* type_name(uint32_t dtype) { return dtype == TILER_HIP_BF16 ? "bf16" : "f32"; }
+
+void slot_or_null(Launch& l, bool present, uint32_t slot) {
+  if (present) l.ptr(slot);
+  else l.null_ptr();
+}
+
+constexpr uint32_t kNormRowWorkgroups = 1u << 20;  // rows beyond take further rounds of the row loops
+
+}  // namespace
+
+// Slots: x, [w,] [b,] y, [mean, rstd].
+tiler_hip_status plan_layer_norm(const Target&, uint32_t dtype, uint32_t parts, uint64_t rows, uint64_t extent,
+                                 uint32_t eps_bits, const uintptr_t*, Program& p) {
+  float eps;
+  std::memcpy(&eps, &eps_bits, 4);
+  if (!(eps > 0.0f) || !std::isfinite(eps))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "eps must be positive and finite");
+  if (dtype != TILER_HIP_F32 && dtype != TILER_HIP_BF16)
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "layer_norm dtype");
+  if (parts & ~(uint32_t)(TILER_HIP_NORM_WEIGHT | TILER_HIP_NORM_BIAS | TILER_HIP_NORM_STATISTICS))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "layer_norm parts");
+  const bool has_w = parts & TILER_HIP_NORM_WEIGHT, has_b = parts & TILER_HIP_NORM_BIAS,
+             stats = parts & TILER_HIP_NORM_STATISTICS;
+  const uint64_t elem = dtype == TILER_HIP_BF16 ? 2 : 4, bytes = mul_sat(mul_sat(rows, extent), elem);
+  const uint32_t x = p.slot(bytes, kSlotInput);
+  const uint32_t w = has_w ? p.slot(mul_sat(extent, elem), kSlotInput) : 0;
+  const uint32_t b = has_b ? p.slot(mul_sat(extent, elem), kSlotInput) : 0;
+  const uint32_t y = p.slot(bytes, kSlotOutput);
+  const uint32_t mean = stats ? p.slot(mul_sat(rows, 4), kSlotOutput) : 0;
+  const uint32_t rstd = stats ? p.slot(mul_sat(rows, 4), kSlotOutput) : 0;
+  if (rows == 0 || extent == 0) return TILER_HIP_OK;
+  if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
+  char name[64];
+  std::snprintf(name, sizeof(name), "tiler_layer_norm_%s_s", type_name(dtype));
+  Launch& l = p.add(name, (uint32_t)(rows < kNormRowWorkgroups ? rows : kNormRowWorkgroups), 1, 256).ptr(x);
+  slot_or_null(l, has_w, w);
+  slot_or_null(l, has_b, b);
+  l.u64(rows).u64(extent).f32(eps).ptr(y);
+  slot_or_null(l, stats, mean);
+  slot_or_null(l, stats, rstd);
+  return TILER_HIP_OK;
+}
+
+// Slots: dy, x, [w,] mean, rstd, [dx,] [dw,] [db,] [partials: scratch].
+tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint32_t parts, uint64_t rows,
+                                          uint64_t extent, const uintptr_t*, Program& p) {
+  if (dtype != TILER_HIP_F32 && dtype != TILER_HIP_BF16)
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "layer_norm dtype");
+  const uint32_t known = TILER_HIP_NORM_WEIGHT | TILER_HIP_NORM_DX | TILER_HIP_NORM_DW | TILER_HIP_NORM_DB;
+  if (parts & ~known) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "layer_norm_backward parts");
+  const bool has_w = parts & TILER_HIP_NORM_WEIGHT, has_dx = parts & TILER_HIP_NORM_DX,
+             has_dw = parts & TILER_HIP_NORM_DW, has_db = parts & TILER_HIP_NORM_DB;
+  const uint64_t elem = dtype == TILER_HIP_BF16 ? 2 : 4, bytes = mul_sat(mul_sat(rows, extent), elem);
+  const uint32_t dy = p.slot(bytes, kSlotInput), x = p.slot(bytes, kSlotInput);
+  const uint32_t w = has_w ? p.slot(mul_sat(extent, elem), kSlotInput) : 0;
+  const uint32_t mean = p.slot(mul_sat(rows, 4), kSlotInput), rstd = p.slot(mul_sat(rows, 4), kSlotInput);
+  const uint32_t dx = has_dx ? p.slot(bytes, kSlotOutput) : 0;
+  const uint32_t dw = has_dw ? p.slot(mul_sat(extent, elem), kSlotOutput) : 0;
+  const uint32_t db = has_db ? p.slot(mul_sat(extent, elem), kSlotOutput) : 0;
+  if (extent == 0) return TILER_HIP_OK;
+  if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
+  char name[64];
+  if (has_dx && rows) {
+    std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_s", type_name(dtype));
+    Launch& l = p.add(name, (uint32_t)(rows < kNormRowWorkgroups ? rows : kNormRowWorkgroups), 1, 256).ptr(dy).ptr(x);
+    slot_or_null(l, has_w, w);
+    l.ptr(mean).ptr(rstd).u64(rows).u64(extent).ptr(dx);
+  }
+  if (!has_dw && !has_db) return TILER_HIP_OK;
+  const uint64_t strips = rows < 4ull * t.compute_units ? ceil_div(rows, 16) : t.compute_units;
+  const uint64_t strip = rows ? ceil_div(rows, strips) : 0;
+  const uint32_t partials = p.slot(mul_sat(mul_sat(strips, extent), 8), kSlotScratch);
+  if (rows) {
+    std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_%s", type_name(dtype));
+    p.add(name, (uint32_t)ceil_div(extent, 256), (uint32_t)strips, 256)
+        .ptr(dy).ptr(x).ptr(mean).ptr(rstd).u64(rows).u64(extent).u64(strip).ptr(partials);
+  }
+  std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_final_%s", type_name(dtype));
+  Launch& l = p.add(name, (uint32_t)ceil_div(2 * extent, 256), 1, 256).ptr(partials).u32((uint32_t)strips).u64(extent);
+  slot_or_null(l, has_dw, dw);
+  slot_or_null(l, has_db, db);
+  return TILER_HIP_OK;
+}
+
+namespace {
+
+tiler_hip_status check_product(uint64_t m, uint64_t n, uint64_t k, Program& p) {
+  if (k == 0) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "empty contracted extent");
+  if (m > 0x7fffff00ull || n > 0x7fffff00ull || k > 0x7fffff00ull || ceil_div(m, 128) > 65535 ||
+      !grid_holds(ceil_div(n, 64), 256) || !grid_holds(ceil_div(k, 64), 256))
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
+  return TILER_HIP_OK;
+}
+
+}  // namespace
+
+// Slots: x, wg, wu, h, [gate, up].
+tiler_hip_status plan_gated_contract_bf16(const Target&, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
+                                          const uintptr_t*, Program& p) {
+  if (parts & ~(uint32_t)TILER_HIP_GATED_KEEP) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "gated_contract parts");
+  const bool keep = parts & TILER_HIP_GATED_KEEP;
+  const uint64_t out = mul_sat(mul_sat(m, n), 2), weight = mul_sat(mul_sat(n, k), 2);
+  const uint32_t x = p.slot(mul_sat(mul_sat(m, k), 2), kSlotInput);
+  const uint32_t wg = p.slot(weight, kSlotInput), wu = p.slot(weight, kSlotInput);
+  const uint32_t h = p.slot(out, kSlotOutput);
+  const uint32_t gate = keep ? p.slot(out, kSlotOutput) : 0, up = keep ? p.slot(out, kSlotOutput) : 0;
+  if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
+  if (m == 0 || n == 0) return TILER_HIP_OK;
+  Launch& l = p.add("tiler_gated_bf16_g", (uint32_t)ceil_div(n, 64), (uint32_t)ceil_div(m, 128), 256)
+                  .ptr(x).ptr(wg).ptr(wu).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(h);
+  slot_or_null(l, keep, gate);
+  slot_or_null(l, keep, up);
+  return TILER_HIP_OK;
+}
+
+// Slots: x, wg, wu, gate, up, dh, [dx,] [dwg, dwu,] dG, dU (scratch:
+// rows of n rounded up to 64 elements).
+tiler_hip_status plan_gated_contract_bf16_backward(const Target&, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
+                                                   const uintptr_t*, Program& p) {
+  if (parts & ~(uint32_t)(TILER_HIP_GATED_DX | TILER_HIP_GATED_DW))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "gated_contract_backward parts");
+  const bool has_dx = parts & TILER_HIP_GATED_DX, has_dw = parts & TILER_HIP_GATED_DW;
+  const uint64_t mid = mul_sat(mul_sat(m, n), 2), weight = mul_sat(mul_sat(n, k), 2), in = mul_sat(mul_sat(m, k), 2);
+  const uint32_t x = p.slot(in, kSlotInput), wg = p.slot(weight, kSlotInput), wu = p.slot(weight, kSlotInput);
+  const uint32_t gate = p.slot(mid, kSlotInput), up = p.slot(mid, kSlotInput), dh = p.slot(mid, kSlotInput);
+  const uint32_t dx = has_dx ? p.slot(in, kSlotOutput) : 0;
+  const uint32_t dwg = has_dw ? p.slot(weight, kSlotOutput) : 0, dwu = has_dw ? p.slot(weight, kSlotOutput) : 0;
+  if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
+  if (2 * ceil_div(n, 128) > 65535) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
+  if (!parts) return TILER_HIP_OK;
+  const uint64_t ld = ceil_div(n, 64) * 64, half = mul_sat(mul_sat(m, ld), 2);
+  const uint32_t dg = p.slot(half, kSlotScratch), du = p.slot(half, kSlotScratch);
+  const uint32_t m32 = (uint32_t)m, n32 = (uint32_t)n, k32 = (uint32_t)k, ld32 = (uint32_t)ld;
+  if (m && n) {
+    const uint64_t groups = ceil_div(m * (ld / 8), 256);
+    p.add("tiler_gated_bf16_grad", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
+        .ptr(gate).ptr(up).ptr(dh).u32(m32).u32(n32).u32(ld32).ptr(dg).ptr(du);
+  }
+  if (has_dx && m)
+    p.add("tiler_gated_bf16_dx_g", (uint32_t)ceil_div(k, 128), (uint32_t)ceil_div(m, 128), 256)
+        .ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx);
+  if (has_dw && n)
+    p.add("tiler_gated_bf16_dw_g", (uint32_t)ceil_div(k, 128), (uint32_t)(2 * ceil_div(n, 128)), 256)
+        .ptr(dg).ptr(du).u32(ld32).ptr(x).u32(m32).u32(n32).u32(k32).u32((uint32_t)ceil_div(n, 128)).ptr(dwg).ptr(dwu);
+  return TILER_HIP_OK;
+}
+
+// Slots: x, q, scales.
+tiler_hip_status plan_quantize_rows_i8(const Target&, uint32_t dtype, uint64_t rows, uint64_t extent, const uintptr_t*,
+                                       Program& p) {
+  if (dtype != TILER_HIP_F32 && dtype != TILER_HIP_BF16)
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "quantize_rows dtype");
+  const uint64_t n = mul_sat(rows, extent);
+  const uint32_t x = p.slot(mul_sat(n, dtype == TILER_HIP_BF16 ? 2 : 4), kSlotInput);
+  const uint32_t q = p.slot(n, kSlotOutput), scales = p.slot(mul_sat(rows, 4), kSlotOutput);
+  if (rows == 0 || extent == 0) return TILER_HIP_OK;
+  if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
+  char name[64];
+  std::snprintf(name, sizeof(name), "tiler_quantize_rows_i8_%s", type_name(dtype));
+  p.add(name, (uint32_t)(rows < kNormRowWorkgroups ? rows : kNormRowWorkgroups), 1, 256)
+      .ptr(x).u64(rows).u64(extent).ptr(q).ptr(scales);
+  return TILER_HIP_OK;
+}
+
+// Slots: a, b, a_scales, b_scales, c.
+tiler_hip_status plan_contract_i8(const Target&, uint32_t out_dtype, uint64_t m, uint64_t n, uint64_t k,
+                                  const uintptr_t*, Program& p) {
+  if (out_dtype != TILER_HIP_F32 && out_dtype != TILER_HIP_BF16)
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "contract_i8 result dtype");
+  const uint32_t a = p.slot(mul_sat(m, k), kSlotInput), b = p.slot(mul_sat(n, k), kSlotInput);
+  const uint32_t sa = p.slot(mul_sat(m, 4), kSlotInput), sb = p.slot(mul_sat(n, 4), kSlotInput);
+  const uint32_t c = p.slot(mul_sat(mul_sat(m, n), out_dtype == TILER_HIP_BF16 ? 2 : 4), kSlotOutput);
+  if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
+  if (k > 131071) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "a sum of more than 131071 products could leave 32 bits");
+  if (m == 0 || n == 0) return TILER_HIP_OK;
+  char name[64];
+  std::snprintf(name, sizeof(name), "tiler_contract_i8_%s_g", type_name(out_dtype));
+  p.add(name, (uint32_t)ceil_div(n, 128), (uint32_t)ceil_div(m, 128), 256)
+      .ptr(a).ptr(b).ptr(sa).ptr(sb).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(c);
+  return TILER_HIP_OK;
+}
+
+}  // namespace tiler_rt

@@ -228,4 +228,20 @@ tiler_hip_status plan_fold(uint32_t op, uint32_t rank, const uint64_t* dims, uin
 tiler_hip_status plan_reindex(uint64_t src_elements, uint32_t rank, const uint64_t* out_dims,
                               const int64_t* strides, int64_t base, uint32_t element_bytes, Program& p);
 
+// The feed-forward sublayer (feed_forward.cpp).  Optional operands have a slot
+// only where they are present (`parts`, TILER_HIP_NORM_* / TILER_HIP_GATED_*);
+// each planner documents its slot order.
+tiler_hip_status plan_layer_norm(const Target& t, uint32_t dtype, uint32_t parts, uint64_t rows, uint64_t extent,
+                                 uint32_t eps_bits, const uintptr_t* addr, Program& p);
+tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint32_t parts, uint64_t rows,
+                                          uint64_t extent, const uintptr_t* addr, Program& p);
+tiler_hip_status plan_gated_contract_bf16(const Target& t, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
+                                          const uintptr_t* addr, Program& p);
+tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
+                                                   const uintptr_t* addr, Program& p);
+tiler_hip_status plan_quantize_rows_i8(const Target& t, uint32_t dtype, uint64_t rows, uint64_t extent,
+                                       const uintptr_t* addr, Program& p);
+tiler_hip_status plan_contract_i8(const Target& t, uint32_t out_dtype, uint64_t m, uint64_t n, uint64_t k,
+                                  const uintptr_t* addr, Program& p);
+
 }  // namespace tiler_rt

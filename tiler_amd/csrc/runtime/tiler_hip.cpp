@@ -356,6 +356,23 @@ const EntryRow kEntries[] = {
     TILER_BATCHED_ROWS("k4x8"), TILER_BATCHED_ROWS("k6x8"), TILER_BATCHED_ROWS("skinny1_l"),
     TILER_BATCHED_ROWS("skinny2_l"), TILER_BATCHED_ROWS("skinny3_l"), TILER_BATCHED_ROWS("skinny4_l"),
 #undef TILER_BATCHED_ROWS
+    // the feed-forward sublayer
+    {"tiler_layer_norm_bf16_s", "layer-norm/bf16", 6},
+    {"tiler_layer_norm_f32_s", "layer-norm-f32", 6},
+    {"tiler_layer_norm_grad_bf16_s", "layer-norm-backward/bf16", 6},
+    {"tiler_layer_norm_grad_f32_s", "layer-norm-backward-f32", 6},
+    {"tiler_layer_norm_columns_bf16", "layer-norm-backward/bf16", 5},
+    {"tiler_layer_norm_columns_f32", "layer-norm-backward-f32", 5},
+    {"tiler_layer_norm_columns_final_bf16", "layer-norm-backward/bf16", 3},
+    {"tiler_layer_norm_columns_final_f32", "layer-norm-backward-f32", 3},
+    {"tiler_gated_bf16_g", "gated-contraction-bf16", 6},
+    {"tiler_gated_bf16_grad", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_dx_g", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_dw_g", "gated-contraction-bf16-backward", 5},
+    {"tiler_quantize_rows_i8_bf16", "quantize-rows-i8/bf16", 3},
+    {"tiler_quantize_rows_i8_f32", "quantize-rows-i8/f32", 3},
+    {"tiler_contract_i8_bf16_g", "tensor-contraction-i8/bf16", 5},
+    {"tiler_contract_i8_f32_g", "tensor-contraction-i8/f32", 5},
 };
 constexpr uint32_t kEntryCount = sizeof(kEntries) / sizeof(kEntries[0]);
 
@@ -1910,6 +1927,231 @@ tiler_hip_status tiler_hip_reindex(tiler_hip_context* ctx, const void* src, uint
 }
 
 // ---------------------------------------------------------------------------
+// The feed-forward sublayer.  Slots follow the planners' orders: an optional
+// operand has one only where it is given.
+namespace {
+
+struct SlotList {
+  void* at[tiler_rt::kMaxSlots] = {};
+  uintptr_t addr[tiler_rt::kMaxSlots] = {};
+  uint32_t count = 0;
+  bool missing = false;  // a required operand is NULL
+  void add(const void* p, bool required = true) {
+    missing = missing || (required && !p);
+    addr[count] = (uintptr_t)p;
+    at[count++] = const_cast<void*>(p);
+  }
+  void add_given(const void* p) {
+    if (p) add(p);
+  }
+};
+
+// Bytes of the workspace that holds a program's scratch slots, each from a
+// 256-byte boundary.
+uint64_t workspace_need(const tiler_rt::Program& p) {
+  uint64_t need = 0;
+  for (uint32_t i = 0; i < p.nslots; ++i)
+    if (p.slot_roles[i] == tiler_rt::kSlotScratch) need += (p.slot_bytes[i] + 255u) / 256u * 256u;
+  return need;
+}
+
+// Where a backward program's scratch slots (its last ones) live: the caller's
+// workspace, or call scratch.
+tiler_hip_status bind_workspace(tiler_hip_context* ctx, const tiler_rt::Program& p, SlotList& slots, void* workspace,
+                                uint64_t workspace_bytes, hipStream_t s, CallScratch& scratch) {
+  const uint64_t need = workspace_need(p);
+  if (!need) return TILER_HIP_OK;
+  void* at = workspace;
+  if (workspace) {
+    if (((uintptr_t)workspace & 15u) != 0)
+      return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "the workspace is not 16-byte aligned");
+    if (workspace_bytes < need)
+      return fail(ctx, TILER_HIP_REFUSE_CAPACITY, "the workspace holds " + std::to_string(workspace_bytes) + " of " +
+                                                      std::to_string(need) + " bytes");
+  } else {
+    if (capturing(s))
+      return fail(ctx, TILER_HIP_REFUSE_CAPACITY, "workspace allocation under graph capture: give the call a workspace");
+    if (!(at = scratch.get(need))) return fail(ctx, TILER_HIP_FAIL_ALLOCATION, "workspace allocation failed");
+  }
+  for (uint32_t i = slots.count; i < p.nslots; ++i) {
+    slots.add(at);
+    at = static_cast<char*>(at) + (p.slot_bytes[i] + 255u) / 256u * 256u;
+  }
+  return TILER_HIP_OK;
+}
+
+}  // namespace
+
+tiler_hip_status tiler_hip_layer_norm(tiler_hip_context* ctx, uint32_t dtype, const void* x, const void* w,
+                                      const void* b, uint64_t rows, uint64_t extent, uint32_t eps_bits, void* y,
+                                      float* mean, float* rstd, tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  if (!mean != !rstd) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "mean and rstd go together");
+  SlotList slots;
+  slots.add(x);
+  slots.add_given(w);
+  slots.add_given(b);
+  slots.add(y);
+  slots.add_given(mean);
+  slots.add_given(rstd);
+  const uint32_t parts = (w ? TILER_HIP_NORM_WEIGHT : 0u) | (b ? TILER_HIP_NORM_BIAS : 0u) |
+                         (mean ? TILER_HIP_NORM_STATISTICS : 0u);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_layer_norm(target_of(ctx), dtype, parts, rows, extent, eps_bits, slots.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (p.nlaunches && slots.missing) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "x or y is NULL");
+  return run_program(ctx, p, slots.at, pick(ctx, stream));
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_layer_norm_backward(tiler_hip_context* ctx, uint32_t dtype, const void* dy, const void* x,
+                                               const void* w, const float* mean, const float* rstd, uint64_t rows,
+                                               uint64_t extent, void* dx, void* dw, void* db, void* workspace,
+                                               uint64_t workspace_bytes, tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  SlotList slots;
+  slots.add(dy);
+  slots.add(x);
+  slots.add_given(w);
+  slots.add(mean);
+  slots.add(rstd);
+  slots.add_given(dx);
+  slots.add_given(dw);
+  slots.add_given(db);
+  const uint32_t parts = (w ? TILER_HIP_NORM_WEIGHT : 0u) | (dx ? TILER_HIP_NORM_DX : 0u) |
+                         (dw ? TILER_HIP_NORM_DW : 0u) | (db ? TILER_HIP_NORM_DB : 0u);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_layer_norm_backward(target_of(ctx), dtype, parts, rows, extent, slots.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (!p.nlaunches) return TILER_HIP_OK;
+  if (rows && slots.missing) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "dy, x, mean or rstd is NULL");
+  hipStream_t s = pick(ctx, stream);
+  CallScratch scratch(ctx, s);
+  if ((st = bind_workspace(ctx, p, slots, workspace, workspace_bytes, s, scratch)) != TILER_HIP_OK) return st;
+  return run_program(ctx, p, slots.at, s);
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_layer_norm_backward_workspace(const tiler_hip_context* ctx, uint32_t dtype, uint64_t rows,
+                                                         uint64_t extent, uint64_t* bytes) try {
+  if (!bytes) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  const uintptr_t addr[tiler_rt::kMaxSlots] = {};
+  tiler_rt::Program p;
+  const tiler_hip_status st = tiler_rt::plan_layer_norm_backward(
+      target_of(ctx), dtype, TILER_HIP_NORM_WEIGHT | TILER_HIP_NORM_DX | TILER_HIP_NORM_DW | TILER_HIP_NORM_DB, rows,
+      extent, addr, p);
+  *bytes = st == TILER_HIP_OK ? workspace_need(p) : 0;
+  return st;
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_gated_contract_bf16(tiler_hip_context* ctx, const uint16_t* x, const uint16_t* wg,
+                                               const uint16_t* wu, uint64_t m, uint64_t n, uint64_t k, uint16_t* h,
+                                               uint16_t* gate, uint16_t* up, tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  if (!gate != !up) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "gate and up go together");
+  SlotList slots;
+  slots.add(x);
+  slots.add(wg);
+  slots.add(wu);
+  slots.add(h);
+  slots.add_given(gate);
+  slots.add_given(up);
+  tiler_rt::Program p;
+  tiler_hip_status st =
+      tiler_rt::plan_gated_contract_bf16(target_of(ctx), gate ? TILER_HIP_GATED_KEEP : 0u, m, n, k, slots.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (p.nlaunches && slots.missing) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "x, wg, wu or h is NULL");
+  return run_program(ctx, p, slots.at, pick(ctx, stream));
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_gated_contract_bf16_backward(tiler_hip_context* ctx, const uint16_t* x, const uint16_t* wg,
+                                                        const uint16_t* wu, const uint16_t* gate, const uint16_t* up,
+                                                        const uint16_t* dh, uint64_t m, uint64_t n, uint64_t k,
+                                                        uint16_t* dx, uint16_t* dwg, uint16_t* dwu, void* workspace,
+                                                        uint64_t workspace_bytes, tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  if (!dwg != !dwu) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "dwg and dwu go together");
+  SlotList slots;
+  slots.add(x);
+  slots.add(wg);
+  slots.add(wu);
+  slots.add(gate);
+  slots.add(up);
+  slots.add(dh);
+  slots.add_given(dx);
+  slots.add_given(dwg);
+  slots.add_given(dwu);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_gated_contract_bf16_backward(
+      target_of(ctx), (dx ? TILER_HIP_GATED_DX : 0u) | (dwg ? TILER_HIP_GATED_DW : 0u), m, n, k, slots.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (!p.nlaunches) return TILER_HIP_OK;
+  if (m && n && slots.missing)
+    return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "x, wg, wu, gate, up or dh is NULL");
+  hipStream_t s = pick(ctx, stream);
+  CallScratch scratch(ctx, s);
+  if ((st = bind_workspace(ctx, p, slots, workspace, workspace_bytes, s, scratch)) != TILER_HIP_OK) return st;
+  return run_program(ctx, p, slots.at, s);
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_gated_contract_bf16_backward_workspace(const tiler_hip_context* ctx, uint64_t m, uint64_t n,
+                                                                  uint64_t k, uint64_t* bytes) try {
+  if (!bytes) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  const uintptr_t addr[tiler_rt::kMaxSlots] = {};
+  tiler_rt::Program p;
+  const tiler_hip_status st = tiler_rt::plan_gated_contract_bf16_backward(
+      target_of(ctx), TILER_HIP_GATED_DX | TILER_HIP_GATED_DW, m, n, k, addr, p);
+  *bytes = st == TILER_HIP_OK ? workspace_need(p) : 0;
+  return st;
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_quantize_rows_i8(tiler_hip_context* ctx, uint32_t dtype, const void* x, uint64_t rows,
+                                            uint64_t extent, int8_t* q, float* scales, tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  SlotList slots;
+  slots.add(x);
+  slots.add(q);
+  slots.add(scales);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_quantize_rows_i8(target_of(ctx), dtype, rows, extent, slots.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (p.nlaunches && slots.missing) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "x, q or scales is NULL");
+  return run_program(ctx, p, slots.at, pick(ctx, stream));
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_contract_i8(tiler_hip_context* ctx, const int8_t* a, const int8_t* b, const float* a_scales,
+                                       const float* b_scales, uint64_t m, uint64_t n, uint64_t k, uint32_t dtype,
+                                       void* c, tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  SlotList slots;
+  slots.add(a);
+  slots.add(b);
+  slots.add(a_scales);
+  slots.add(b_scales);
+  slots.add(c);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_contract_i8(target_of(ctx), dtype, m, n, k, slots.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (p.nlaunches && slots.missing)
+    return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "a, b, a_scales, b_scales or c is NULL");
+  return run_program(ctx, p, slots.at, pick(ctx, stream));
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+// ---------------------------------------------------------------------------
 // Target environment (adapter.rs:295-322; environment.rs:249-400).
 namespace {
 
@@ -2227,6 +2469,33 @@ static tiler_hip_status plan_region(const tiler_hip_context* ctx, const tiler_hi
       st = r->dtype == TILER_HIP_F32
                ? tiler_rt::plan_dequantize_u4(tiler_rt::Mode::Realized, e[0], 0, 0, addr, p)
                : p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "the strict-affine U4 decode produces f32");
+      break;
+    case TILER_HIP_PROGRAM_LAYER_NORM:
+      st = c.reassociate ? tiler_rt::plan_layer_norm(t, r->dtype, r->variant, e[0], e[1], r->scalars[0], addr, p)
+                         : needs_reassociation("layer norm");
+      break;
+    case TILER_HIP_PROGRAM_LAYER_NORM_BACKWARD:
+      st = c.reassociate ? tiler_rt::plan_layer_norm_backward(t, r->dtype, r->variant, e[0], e[1], addr, p)
+                         : needs_reassociation("layer norm's gradients");
+      break;
+    case TILER_HIP_PROGRAM_GATED_CONTRACTION:
+    case TILER_HIP_PROGRAM_GATED_CONTRACTION_BACKWARD:
+      if (r->dtype != TILER_HIP_BF16)
+        st = p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "the gated contraction is a bf16 family");
+      else if (!c.reassociate)
+        st = needs_reassociation("the gated contraction");
+      else if (r->program == TILER_HIP_PROGRAM_GATED_CONTRACTION)
+        st = tiler_rt::plan_gated_contract_bf16(t, r->variant, e[0], e[1], e[2], addr, p);
+      else
+        st = tiler_rt::plan_gated_contract_bf16_backward(t, r->variant, e[0], e[1], e[2], addr, p);
+      break;
+    case TILER_HIP_PROGRAM_QUANTIZE_ROWS_I8:  // a maximum and exact quotients: no order to permit
+      st = r->variant ? p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "quantize_rows variant")
+                      : tiler_rt::plan_quantize_rows_i8(t, r->dtype, e[0], e[1], addr, p);
+      break;
+    case TILER_HIP_PROGRAM_CONTRACTION_I8:  // an integer sum: no order to permit
+      st = r->variant ? p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "contract_i8 variant")
+                      : tiler_rt::plan_contract_i8(t, r->dtype, e[0], e[1], e[2], addr, p);
       break;
     default:
       st = p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "no realization for this scalar program");

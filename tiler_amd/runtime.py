@@ -298,6 +298,57 @@ class Context:
         self._check(L.lib().tiler_hip_contract(self.handle, dtype, ctypes.byref(structure), epilogue, permissions,
                                                _ptr(left), _ptr(right), _ptr(out), stream), "contract")
 
+    # -- the feed-forward sublayer ---------------------------------------------
+    def layer_norm(self, dtype: int, x, w, b, rows: int, extent: int, eps_bits: int, y, mean=None, rstd=None,
+                   stream=None):
+        """y = (x - mean) rstd w + b over the last axis; w or b None: ones,
+        zeros.  mean and rstd (f32 [rows]) are kept for the gradients."""
+        self._check(L.lib().tiler_hip_layer_norm(self.handle, dtype, _ptr(x), _ptr(w), _ptr(b), rows, extent, eps_bits,
+                                                 _ptr(y), _ptr(mean), _ptr(rstd), stream), "layer_norm")
+
+    def layer_norm_backward(self, dtype: int, dy, x, w, mean, rstd, rows: int, extent: int, dx=None, dw=None, db=None,
+                            workspace=None, workspace_bytes: int = 0, stream=None):
+        """dx, dw and db (those given) from dy and what the forward call kept."""
+        self._check(L.lib().tiler_hip_layer_norm_backward(self.handle, dtype, _ptr(dy), _ptr(x), _ptr(w), _ptr(mean),
+                                                          _ptr(rstd), rows, extent, _ptr(dx), _ptr(dw), _ptr(db),
+                                                          _ptr(workspace), workspace_bytes, stream),
+                    "layer_norm_backward")
+
+    def layer_norm_backward_workspace(self, dtype: int, rows: int, extent: int) -> int:
+        n = ctypes.c_uint64()
+        self._check(L.lib().tiler_hip_layer_norm_backward_workspace(self.handle, dtype, rows, extent, ctypes.byref(n)),
+                    "layer_norm_backward_workspace")
+        return n.value
+
+    def gated_contract_bf16(self, x, wg, wu, m: int, n: int, k: int, h, gate=None, up=None, stream=None):
+        """h = silu(x wg^T) * (x wu^T); gate and up keep the two products for
+        the gradients."""
+        self._check(L.lib().tiler_hip_gated_contract_bf16(self.handle, _ptr(x), _ptr(wg), _ptr(wu), m, n, k, _ptr(h),
+                                                          _ptr(gate), _ptr(up), stream), "gated_contract_bf16")
+
+    def gated_contract_bf16_backward(self, x, wg, wu, gate, up, dh, m: int, n: int, k: int, dx=None, dwg=None,
+                                     dwu=None, workspace=None, workspace_bytes: int = 0, stream=None):
+        """dx, and dwg with dwu (those given) from dh and the kept products."""
+        self._check(L.lib().tiler_hip_gated_contract_bf16_backward(
+            self.handle, _ptr(x), _ptr(wg), _ptr(wu), _ptr(gate), _ptr(up), _ptr(dh), m, n, k, _ptr(dx), _ptr(dwg),
+            _ptr(dwu), _ptr(workspace), workspace_bytes, stream), "gated_contract_bf16_backward")
+
+    def gated_contract_bf16_backward_workspace(self, m: int, n: int, k: int) -> int:
+        b = ctypes.c_uint64()
+        self._check(L.lib().tiler_hip_gated_contract_bf16_backward_workspace(self.handle, m, n, k, ctypes.byref(b)),
+                    "gated_contract_bf16_backward_workspace")
+        return b.value
+
+    def quantize_rows_i8(self, dtype: int, x, rows: int, extent: int, q, scales, stream=None):
+        """Rows in 8 bits with one f32 scale each (nearest, ties to even)."""
+        self._check(L.lib().tiler_hip_quantize_rows_i8(self.handle, dtype, _ptr(x), rows, extent, _ptr(q),
+                                                       _ptr(scales), stream), "quantize_rows_i8")
+
+    def contract_i8(self, a, b, a_scales, b_scales, m: int, n: int, k: int, dtype: int, c, stream=None):
+        """c[i, j] = (sum_k a_ik b_jk) a_scales[i] b_scales[j], in f32 or bf16."""
+        self._check(L.lib().tiler_hip_contract_i8(self.handle, _ptr(a), _ptr(b), _ptr(a_scales), _ptr(b_scales), m, n,
+                                                  k, dtype, _ptr(c), stream), "contract_i8")
+
     def expression(self, dtype: int, nodes, inputs, n: int, y, root: int | None = None,
                    input_subnormals: int = 0, result_subnormals: int = 0, stream=None):
         """A pointwise expression DAG: `nodes` are (op, a, b) triples (L.NODE_*),
