@@ -149,6 +149,6 @@ def quantize_rows(x):
 
 def contract_i8(a, b, sa, sb):
     """The f32 result, bit for bit."""
-    total = (a.astype(np.int64) @ b.astype(np.int64).T)
+    total = a.astype(np.float64) @ b.astype(np.float64).T  # whole numbers below 2^31: exact
     with np.errstate(over="ignore", invalid="ignore"):
         return (total.astype(np.float32) * sa[:, None].astype(np.float32)) * sb[None, :].astype(np.float32)

@@ -98,7 +98,8 @@ def check_product(ctx, mem, m, n, k, dtype, shift=0, codes=None):
 
 SHAPES = [(1, 1, 1), (1, 16, 64), (1, 1000, 4096), (3, 5, 7), (16, 128, 256), (17, 100, 128), (33, 64, 1000),
           (64, 512, 4096), (65, 200, 512), (128, 128, 128), (129, 257, 144), (200, 96, 2048), (256, 256, 640),
-          (300, 513, 1111), (511, 264, 784), (1024, 1024, 1024), (257, 5001, 1111)]
+          (300, 513, 1111), (511, 264, 784), (1024, 1024, 1024), (257, 5001, 1111),
+          (4100, 4104, 208)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

@@ -59,7 +59,8 @@ def backward(ctx, mem, x, wg, wu, gate, up, dh, shift=0, want=(True, True), work
 # (m, n, k): a token, decode batches, prompts, ragged and odd, tiles exact
 SHAPES = [(1, 1, 1), (1, 64, 64), (1, 1000, 520), (2, 37, 11), (5, 128, 4096), (16, 256, 512), (17, 72, 136),
           (48, 520, 1024), (64, 96, 200), (65, 96, 512), (100, 264, 72), (128, 128, 64), (129, 127, 65),
-          (200, 512, 1000), (256, 256, 128), (257, 200, 264), (300, 1365, 509), (520, 392, 328), (512, 1024, 256)]
+          (200, 512, 1000), (256, 256, 128), (257, 200, 264), (300, 1365, 509), (520, 392, 328), (512, 1024, 256),
+          (4104, 2056, 72), (520, 4104, 2312), (2056, 72, 8200)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)

@@ -137,3 +137,75 @@ tiler_contract_i8_f32_g(const int8_t* __restrict__ a, const int8_t* __restrict__
                         const float* __restrict__ sb, uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
   contract_i8_guarded<false>(a, b, sa, sb, m, n, k, c);
 }
+
+// ---------------------------------------------------------------------------
+// Staged form: k a multiple of 16 and 16-byte aligned operands.
+namespace {
+
+template <int WM, int WN, int MB, bool kBf16>
+__device__ __forceinline__ void contract_i8_staged(const int8_t* __restrict__ a, const int8_t* __restrict__ b,
+                                                   const float* __restrict__ sa, const float* __restrict__ sb,
+                                                   uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
+  constexpr uint32_t kRowsA = WM * MB * 16u, kRowsB = WN * 64u, kThreads = 64u * WM * WN;
+  constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kRowsB / 8 / (WM * WN);
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kRowsB) * kSlice];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t tm, tn;
+  tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (n + kRowsB - 1u) / kRowsB, tm, tn);
+  const uint32_t m0 = tm * kRowsA, n0 = tn * kRowsB;
+  const tiler_product::RowLoader<I8, kLoadsA> la(reinterpret_cast<const uint8_t*>(a + (uint64_t)m0 * k), k,
+                                                 m - m0 < kRowsA ? m - m0 : kRowsA, k, wave * kLoadsA * 8u,
+                                                 wave * kLoadsA * 8u, lane);
+  const tiler_product::RowLoader<I8, kLoadsB> lb(reinterpret_cast<const uint8_t*>(b + (uint64_t)n0 * k), k,
+                                                 n - n0 < kRowsB ? n - n0 : kRowsB, k, wave * kLoadsB * 8u,
+                                                 wave * kLoadsB * 8u, lane);
+  i32x4 acc[MB][4];
+  tiler_product::staged_product<I8, false, false, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+      smem, (k + 127u) / 128u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
+      [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
+  const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 64u;
+  float rows[MB][4], cols[4];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t row = m0 + row0 + i * 16u + (lane >> 4) * 4u + r;
+      rows[i][r] = sa[row < m ? row : m - 1u];
+    }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t col = n0 + col0 + j * 16u + (lane & 15u);
+    cols[j] = sb[col < n ? col : n - 1u];
+  }
+  if constexpr (kBf16) {
+    __syncthreads();
+    tiler_product::store_tile_bf16<kRowsA, kRowsB, kThreads, MB, 4>(
+        smem, row0, col0, static_cast<uint16_t*>(c), m, n, m0, n0,
+        [&](int i, int j, int r) { return (float)acc[i][j][r] * rows[i][r] * cols[j]; });
+  } else {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t row = m0 + row0 + i * 16u + (lane >> 4) * 4u + r, col = n0 + col0 + j * 16u + (lane & 15u);
+          if (row < m && col < n)
+            static_cast<float*>(c)[(uint64_t)row * n + col] = scaled(acc[i][j][r], rows[i][r], cols[j]);
+        }
+  }
+}
+
+}  // namespace
+
+#define TILER_CONTRACT_I8_STAGED(TY, BF16, TILE, WM, WN, MB)                                                       \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                          \
+      tiler_contract_i8_##TY##_t##TILE(const int8_t* __restrict__ a, const int8_t* __restrict__ b,                 \
+                                       const float* __restrict__ sa, const float* __restrict__ sb, uint32_t m,     \
+                                       uint32_t n, uint32_t k, void* __restrict__ c) {                             \
+    contract_i8_staged<WM, WN, MB, BF16>(a, b, sa, sb, m, n, k, c);                                                \
+  }
+TILER_CONTRACT_I8_STAGED(bf16, true, 256, 2, 4, 8)
+TILER_CONTRACT_I8_STAGED(f32, false, 256, 2, 4, 8)
+TILER_CONTRACT_I8_STAGED(bf16, true, 128, 2, 2, 4)
+TILER_CONTRACT_I8_STAGED(f32, false, 128, 2, 2, 4)

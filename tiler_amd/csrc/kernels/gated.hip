@@ -183,3 +183,130 @@ tiler_gated_bf16_dw_g(const uint16_t* __restrict__ dg, const uint16_t* __restric
         if (row < n && col < k) out[(uint64_t)row * k + col] = (uint16_t)tiler::bf16_narrow(acc[i][j][r]);
       }
 }
+
+// ---------------------------------------------------------------------------
+// Staged forms: k a multiple of 8 and 16-byte aligned operands.  WM x WN waves
+// of MB x 4 blocks.
+namespace {
+
+template <int WM, int WN, int MB>
+__device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
+                                             const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
+                                             uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
+                                             uint16_t* __restrict__ up) {
+  constexpr uint32_t kRowsA = WM * MB * 16u, kRowsB = WN * 64u, kCols = kRowsB / 2u, kThreads = 64u * WM * WN;
+  constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kRowsB / 8 / (WM * WN);
+  static_assert(kLoadsB == 4, "a wave's 32 rows of B lie in one of the two weights");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kRowsB) * kSlice];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t tm, tn;
+  tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (n + kCols - 1u) / kCols, tm, tn);
+  const uint32_t m0 = tm * kRowsA, n0 = tn * kCols;
+  const tiler_product::RowLoader<Bf16, kLoadsA> la(reinterpret_cast<const uint8_t*>(x + (uint64_t)m0 * k), k,
+                                                   m - m0 < kRowsA ? m - m0 : kRowsA, k, wave * kLoadsA * 8u,
+                                                   wave * kLoadsA * 8u, lane);
+  // LDS rows 32 w .. 32 w + 31 of B: columns 32 (w / 2) .. of the gate's (w even) or the up projection's weight
+  const tiler_product::RowLoader<Bf16, kLoadsB> lb(
+      reinterpret_cast<const uint8_t*>(((wave & 1u) ? wu : wg) + (uint64_t)n0 * k), k, n - n0 < kCols ? n - n0 : kCols,
+      k, (wave >> 1) * 32u, wave * 32u, lane);
+  f32x4 acc[MB][4];
+  tiler_product::staged_product<Bf16, false, false, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+      smem, (k + 63u) / 64u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
+      [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
+  const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 32u;
+  auto store = [&](uint16_t* out, auto value) {
+    __syncthreads();
+    tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 2>(smem, row0, col0, out, m, n, m0, n0, value);
+  };
+  store(h, [&](int i, int j, int r) { return acc[i][j][r] * sigmoid(acc[i][j][r]) * acc[i][j + 2][r]; });
+  if (gate) {
+    store(gate, [&](int i, int j, int r) { return acc[i][j][r]; });
+    store(up, [&](int i, int j, int r) { return acc[i][j + 2][r]; });
+  }
+}
+
+template <int WM, int WN, int MB>
+__device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du,
+                                                uint32_t ld, const uint16_t* __restrict__ wg,
+                                                const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
+                                                uint16_t* __restrict__ dx) {
+  constexpr uint32_t kRowsA = WM * MB * 16u, kCols = WN * 64u, kThreads = 64u * WM * WN;
+  constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kCols / 8 / (WM * WN);
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kCols) * kSlice];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t tm, tn;
+  tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (k + kCols - 1u) / kCols, tm, tn);
+  const uint32_t m0 = tm * kRowsA, c0 = tn * kCols, per = ld / 64u;
+  // dG's rows hold zeros from n to ld, the weights' depth rows load as zeros there
+  tiler_product::RowLoader<Bf16, kLoadsA> la(reinterpret_cast<const uint8_t*>(dg + (uint64_t)m0 * ld), ld,
+                                             m - m0 < kRowsA ? m - m0 : kRowsA, ld, wave * kLoadsA * 8u,
+                                             wave * kLoadsA * 8u, lane);
+  tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(wg + c0), k, c0, n, wave, lane);
+  const int64_t next_a = reinterpret_cast<const uint8_t*>(du) - reinterpret_cast<const uint8_t*>(dg);
+  const int64_t next_b = reinterpret_cast<const uint8_t*>(wu) - reinterpret_cast<const uint8_t*>(wg);
+  f32x4 acc[MB][4];
+  tiler_product::staged_product<Bf16, false, true, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+      smem, 2u * per,
+      [&](uint32_t t, uint8_t* at) {
+        if (t == per) la.base += next_a;
+        la.issue(t < per ? t : t - per, at);
+      },
+      [&](uint32_t t, uint8_t* at) {
+        if (t == per) lb.base += next_b;
+        lb.issue(t < per ? t : t - per, at);
+      },
+      acc);
+  __syncthreads();
+  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(
+      smem, (wave / WN) * MB * 16u, (wave % WN) * 64u, dx, m, k, m0, c0, [&](int i, int j, int r) { return acc[i][j][r]; });
+}
+
+template <int WM, int WN, int MB>
+__device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du,
+                                                uint32_t ld, const uint16_t* __restrict__ x, uint32_t m, uint32_t n,
+                                                uint32_t k, uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {
+  constexpr uint32_t kRowsA = WM * MB * 16u, kCols = WN * 64u, kThreads = 64u * WM * WN;
+  constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kCols / 8 / (WM * WN);
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kCols) * kSlice];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tiles = (n + kRowsA - 1u) / kRowsA;
+  uint32_t tm, tn;
+  tiler_product::tile_of(blockIdx.x, 2u * tiles, (k + kCols - 1u) / kCols, tm, tn);
+  const bool second = tm >= tiles;
+  const uint32_t j0 = (second ? tm - tiles : tm) * kRowsA, c0 = tn * kCols;
+  const tiler_product::ColumnLoader<kRowsA, kLoadsA> la(reinterpret_cast<const uint8_t*>((second ? du : dg) + j0), ld, j0,
+                                                        m, wave, lane);
+  const tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(x + c0), k, c0, m, wave, lane);
+  f32x4 acc[MB][4];
+  tiler_product::staged_product<Bf16, true, true, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+      smem, (m + 63u) / 64u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
+      [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
+  __syncthreads();
+  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(
+      smem, (wave / WN) * MB * 16u, (wave % WN) * 64u, second ? dwu : dwg, n, k, j0, c0,
+      [&](int i, int j, int r) { return acc[i][j][r]; });
+}
+
+}  // namespace
+
+#define TILER_GATED_STAGED(TILE, WM, WN, MB)                                                                        \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
+      tiler_gated_bf16_t##TILE(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,                     \
+                               const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,                 \
+                               uint16_t* __restrict__ h, uint16_t* __restrict__ gate, uint16_t* __restrict__ up) {  \
+    gated_staged<WM, WN, MB>(x, wg, wu, m, n, k, h, gate, up);                                                      \
+  }                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
+      tiler_gated_bf16_dx_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
+                                  const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m,     \
+                                  uint32_t n, uint32_t k, uint16_t* __restrict__ dx) {                              \
+    gated_dx_staged<WM, WN, MB>(dg, du, ld, wg, wu, m, n, k, dx);                                                   \
+  }                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
+      tiler_gated_bf16_dw_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
+                                  const uint16_t* __restrict__ x, uint32_t m, uint32_t n, uint32_t k,               \
+                                  uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {                         \
+    gated_dw_staged<WM, WN, MB>(dg, du, ld, x, m, n, k, dwg, dwu);                                                  \
+  }
+TILER_GATED_STAGED(256, 2, 4, 8)
+TILER_GATED_STAGED(128, 2, 2, 4)

@@ -211,4 +211,216 @@ __device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, 
   }
 }
 
+// ---------------------------------------------------------------------------
+// The staged product: pieces move global -> LDS with buffer_load_dwordx4 ...
+// lds, two slices in LDS, for operands whose rows (depth rows, in column
+// layout) start on 16 bytes.
+//
+// A loader issues its wave's share of one slice of one operand.  The buffer
+// resource starts at the slice (64-bit scalar arithmetic, so an operand may
+// have any size; a tile's own span stays below 2^31 bytes) and ends with the
+// operand, so what lies past the last row, or past the last depth row of a
+// column operand, loads as zeros; pieces past the depth of a row operand,
+// which lie in the next row, are sent past the resource's end instead.
+// Columns past the last of a column operand load whatever follows: they only
+// reach results that are not stored.
+constexpr uint32_t kPastEnd = 0x80000000u;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const uint8_t* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
+}
+
+// TILE rows from `base`, `rows` of them real; `wave_rows` where this wave's
+// LOADS * 8 rows start in memory and `wave_lds` where they go in the tile (the
+// gated product's weights interleave two matrices).
+template <typename E, int LOADS>
+struct RowLoader {
+  const uint8_t* base;
+  uint32_t span, depth_bytes, lds0;
+  uint32_t voff[LOADS], piece[2];
+  __device__ __forceinline__ RowLoader(const uint8_t* base_, uint64_t ld, uint32_t rows, uint32_t depth,
+                                       uint32_t wave_rows, uint32_t wave_lds, uint32_t lane)
+      : base(base_), span((uint32_t)(rows * ld * E::kBytes)), depth_bytes(depth * E::kBytes), lds0(wave_lds * kSlice) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const uint32_t in = (lane & 7u) ^ (((wave_lds + j * 8u + (lane >> 3)) >> 1) & 7u);
+      if (j < 2) piece[j] = in * 16u;
+      voff[j] = (wave_rows + j * 8u + (lane >> 3)) * (uint32_t)(ld * E::kBytes) + in * 16u;
+    }
+  }
+  __device__ __forceinline__ void issue(uint32_t t, uint8_t* tile) const {
+    const uint32_t at = t * kSlice, left = depth_bytes - at;
+    const __amdgpu_buffer_rsrc_t panel = resource(base + at, span - at);
+    if (left >= kSlice) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (lds_bytes*)(tile + lds0 + j * 1024u), 16, voff[j], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (lds_bytes*)(tile + lds0 + j * 1024u), 16,
+                                                 piece[j & 1] < left ? voff[j] : kPastEnd, 0, 0, 0);
+    }
+  }
+};
+
+// A slice of 64 depth rows of TILE columns (bf16) from `base`, which points at
+// the tile's first column of depth row 0; `before` columns of the row lie
+// before it.
+template <uint32_t TILE, int LOADS>
+struct ColumnLoader {
+  const uint8_t* base;
+  uint64_t row_bytes;
+  uint32_t depth, before_bytes, lds0;
+  uint32_t voff[LOADS];
+  __device__ __forceinline__ ColumnLoader(const uint8_t* base_, uint64_t ld, uint32_t before, uint32_t depth_,
+                                          uint32_t wave, uint32_t lane)
+      : base(base_), row_bytes(ld * 2u), depth(depth_), before_bytes(before * 2u), lds0(wave * LOADS * 1024u) {
+    constexpr uint32_t kPer = TILE / 8u;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const uint32_t id = (wave * LOADS + j) * 64u + lane, outer = id / kPer, slot = id % kPer;
+      const uint32_t block = (slot >> 1) ^ ((outer & 3u) | ((outer >> 1) & 4u));
+      voff[j] = outer * (uint32_t)row_bytes + block * 32u + (slot & 1u) * 16u;
+    }
+  }
+  __device__ __forceinline__ void issue(uint32_t t, uint8_t* tile) const {
+    const uint32_t left = depth - t * 64u, rows = left < 64u ? left : 64u;
+    const __amdgpu_buffer_rsrc_t panel =
+        resource(base + t * 64u * row_bytes, rows * (uint32_t)row_bytes - before_bytes);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (lds_bytes*)(tile + lds0 + j * 1024u), 16, voff[j], 0, 0, 0);
+  }
+};
+
+// vmcnt(n) alone (gfx9 layout: vmcnt [3:0] and [15:14], expcnt [6:4], lgkmcnt [11:8]).
+constexpr int wait_loads(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
+constexpr int kWaitLds = 0xC07F;  // lgkmcnt(0) alone
+
+// issue_a(t, tile) and issue_b request slice t, kLoads loads of a wave in all.
+// A slice is two depth steps; the fragments of the next step are read while
+// the products of the current one run, across slices too, so the only
+// wait a wave takes is the barrier in the middle of a slice: behind it every
+// wave's reads of the slice are done (its buffer takes the slice after the
+// next) and every wave's share of the next slice has landed.
+template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, int kLoads, typename IA, typename IB>
+__device__ __forceinline__ void staged_product(uint8_t* smem, uint32_t slices, IA issue_a, IB issue_b,
+                                               typename E::Acc (&acc)[MB][NB]) {
+  constexpr uint32_t kRowsA = WM * MB * 16u, kRowsB = WN * NB * 16u, kTileA = kRowsA * kSlice;
+  constexpr uint32_t kStage = (kRowsA + kRowsB) * kSlice;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Fragments<kRowsA, kACol, MB> ra((wave / WN) * MB * 16u, lane);
+  const Fragments<kRowsB, kBCol, NB> rb((wave % WN) * NB * 16u, lane);
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = E::zero();
+  auto issue = [&](uint32_t t) {
+    uint8_t* at = smem + (t & 1u) * kStage;
+    issue_a(t, at);
+    issue_b(t, at + kTileA);
+  };
+  u32x4 fa[2][MB], fb[2][NB];
+  auto read = [&](uint32_t t, int s) {
+    const uint8_t* at = smem + (t & 1u) * kStage;
+    ra.read(at, s, fa[s]);
+    rb.read(at + kTileA, s, fb[s]);
+  };
+  auto products = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(fa[s][i], fb[s][j], acc[i][j]);
+  };
+  if (slices == 0) return;
+  issue(0);
+  if (slices > 1) {
+    issue(1);
+    __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
+  } else {
+    __builtin_amdgcn_s_waitcnt(wait_loads(0));
+  }
+  asm volatile("s_barrier" ::: "memory");
+  read(0, 0);
+  for (uint32_t t = 0; t + 1 < slices; ++t) {
+    read(t, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    products(0);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(wait_loads(0));
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitLds);  // satisfied: tells the compiler so
+    if (t + 2 < slices) issue(t + 2);
+    read(t + 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    products(1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  read(slices - 1, 1);
+  products(0);
+  products(1);
+}
+
+// Tile `id` of a tiles_m x tiles_n grid.  Workgroups go round robin over the
+// 8 XCDs: each XCD takes a contiguous run of an order that walks groups of
+// 8 tile rows column by column, so the tiles an XCD runs together (32 CUs)
+// share 8 row panels and a few column panels in its L2.
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+  const uint32_t total = tiles_m * tiles_n, xcd = id & 7u, per = total >> 3, rest = total & 7u;
+  const uint32_t at = xcd * per + (xcd < rest ? xcd : rest) + (id >> 3);
+  const uint32_t group = at / (8u * tiles_n), in = at % (8u * tiles_n);
+  const uint32_t height = tiles_m - group * 8u < 8u ? tiles_m - group * 8u : 8u;
+  tm = group * 8u + in % height;
+  tn = in / height;
+}
+
+// A pair of adjacent result rows (v0: row r, v1: row r + 1) of this lane's
+// column, and the neighbouring lane's of its column: row r's two columns on
+// even lanes, row r + 1's on odd ones, narrowed to bf16 (NaN canonical).
+__device__ __forceinline__ uint32_t column_pair(float v0, float v1, bool odd) {
+  const uint32_t p = tiler::bf16_pack2_rne(v0, v1);
+  const uint32_t q = (uint32_t)__builtin_amdgcn_mov_dpp((int)p, 0xB1, 0xF, 0xF, true);  // quad_perm [1,0,3,2]
+  return __builtin_amdgcn_perm(q, p, odd ? 0x03020706u : 0x05040100u);
+}
+
+// Stores a tile of bf16 results through LDS: value(i, j, r) is this lane's
+// result of row 16 i + 4 (lane / 16) + r, column 16 j + lane % 16 of its wave's
+// (row0, col0) part of the ROWS x COLS tile; the tile is at (m0, n0) of the
+// m x n result.  16-byte stores of whole row pieces, at any alignment.  The
+// caller's waves are done with the LDS.
+template <uint32_t ROWS, uint32_t COLS, uint32_t THREADS, int MB, int NB, typename F>
+__device__ __forceinline__ void store_tile_bf16(uint8_t* smem, uint32_t row0, uint32_t col0, uint16_t* out, uint32_t m,
+                                                uint32_t n, uint32_t m0, uint32_t n0, F value) {
+  constexpr uint32_t kRow = COLS * 2u, kPer = COLS / 8u;
+  const uint32_t lane = threadIdx.x & 63u;
+  const bool odd = lane & 1u;
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const uint32_t row = row0 + i * 16u + (lane >> 4) * 4u + r + (odd ? 1u : 0u);
+        const uint32_t col = col0 + j * 16u + (lane & 14u);
+        *reinterpret_cast<uint32_t*>(smem + row * kRow + (((col >> 3) ^ (((row & 7u) << 1) & (kPer - 1u))) << 4) + ((col & 7u) << 1)) =
+            column_pair(value(i, j, r), value(i, j, r + 1), odd);
+      }
+  __syncthreads();
+#pragma unroll 4
+  for (uint32_t id = threadIdx.x; id < ROWS * kPer; id += THREADS) {
+    const uint32_t row = id / kPer, piece = id % kPer, col = n0 + piece * 8u;
+    if (m0 + row >= m || col >= n) continue;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(smem + row * kRow + ((piece ^ (((row & 7u) << 1) & (kPer - 1u))) << 4));
+    uint16_t* to = out + (uint64_t)(m0 + row) * n + col;
+    if (n - col >= 8u) {
+      *reinterpret_cast<u32x4_any*>(to) = v;
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 7u; ++e)
+        if (e < n - col) to[e] = (uint16_t)(v[e >> 1] >> (16u * (e & 1u)));
+    }
+  }
+}
+
 }  // namespace tiler_product

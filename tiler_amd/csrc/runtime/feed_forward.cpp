@@ -10,7 +10,7 @@ namespace tiler_rt {
 namespace {
 
 uint64_t mul_sat(uint64_t a, uint64_t b) { return a && b > UINT64_MAX / a ? UINT64_MAX : a * b; }
-uint64_t add_sat(uint64_t a, uint64_t b) { return a > UINT64_MAX - b ? UINT64_MAX : a + b; }
+bool aligned16(uintptr_t a) { return (a & 15u) == 0; }
 uint64_t ceil_div(uint64_t a, uint64_t b) { return a / b + (a % b != 0); }
 
 // Whether one launch holds this many workgroups along x: the runtime takes
@@ -112,11 +112,26 @@ tiler_hip_status check_product(uint64_t m, uint64_t n, uint64_t k, Program& p) {
   return TILER_HIP_OK;
 }
 
+// The staged forms move 16-byte pieces of rows `row_bytes` apart and address a
+// 256-row panel through one buffer resource (below 2^31 bytes).
+bool staged_rows(uint64_t row_bytes) { return row_bytes % 16 == 0 && row_bytes * 256 < (1ull << 31); }
+
+// 256-tiles when they go round the CUs at least once, else 128-tiles (four
+// times as many, two to a CU).
+uint32_t staged_tile(const Target& t, uint64_t m, uint64_t n256, uint64_t n) {
+  return mul_sat(ceil_div(m, 256), ceil_div(n, n256)) >= t.compute_units ? 256 : 128;
+}
+
+Launch& add_tiles(Program& p, const std::string& stem, uint32_t tile, uint64_t tiles) {
+  const std::string name = stem + "_t" + std::to_string(tile);
+  return p.add(name.c_str(), (uint32_t)tiles, 1, tile == 256 ? 512 : 256);
+}
+
 }  // namespace
 
 // Slots: x, wg, wu, h, [gate, up].
-tiler_hip_status plan_gated_contract_bf16(const Target&, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
-                                          const uintptr_t*, Program& p) {
+tiler_hip_status plan_gated_contract_bf16(const Target& t, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
+                                          const uintptr_t* addr, Program& p) {
   if (parts & ~(uint32_t)TILER_HIP_GATED_KEEP) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "gated_contract parts");
   const bool keep = parts & TILER_HIP_GATED_KEEP;
   const uint64_t out = mul_sat(mul_sat(m, n), 2), weight = mul_sat(mul_sat(n, k), 2);
@@ -126,6 +141,17 @@ tiler_hip_status plan_gated_contract_bf16(const Target&, uint32_t parts, uint64_
   const uint32_t gate = keep ? p.slot(out, kSlotOutput) : 0, up = keep ? p.slot(out, kSlotOutput) : 0;
   if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
   if (m == 0 || n == 0) return TILER_HIP_OK;
+  if (staged_rows(2 * k) && aligned16(addr[x]) && aligned16(addr[wg]) && aligned16(addr[wu])) {
+    const uint32_t tile = staged_tile(t, m, 128, n);
+    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(n, tile / 2));
+    if (grid_holds(tiles, 512)) {
+      Launch& l = add_tiles(p, "tiler_gated_bf16", tile, tiles)
+                      .ptr(x).ptr(wg).ptr(wu).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(h);
+      slot_or_null(l, keep, gate);
+      slot_or_null(l, keep, up);
+      return TILER_HIP_OK;
+    }
+  }
   Launch& l = p.add("tiler_gated_bf16_g", (uint32_t)ceil_div(n, 64), (uint32_t)ceil_div(m, 128), 256)
                   .ptr(x).ptr(wg).ptr(wu).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(h);
   slot_or_null(l, keep, gate);
@@ -135,8 +161,8 @@ tiler_hip_status plan_gated_contract_bf16(const Target&, uint32_t parts, uint64_
 
 // Slots: x, wg, wu, gate, up, dh, [dx,] [dwg, dwu,] dG, dU (scratch:
 // rows of n rounded up to 64 elements).
-tiler_hip_status plan_gated_contract_bf16_backward(const Target&, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
-                                                   const uintptr_t*, Program& p) {
+tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
+                                                   const uintptr_t* addr, Program& p) {
   if (parts & ~(uint32_t)(TILER_HIP_GATED_DX | TILER_HIP_GATED_DW))
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "gated_contract_backward parts");
   const bool has_dx = parts & TILER_HIP_GATED_DX, has_dw = parts & TILER_HIP_GATED_DW;
@@ -156,12 +182,28 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target&, uint32_t parts
     p.add("tiler_gated_bf16_grad", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
         .ptr(gate).ptr(up).ptr(dh).u32(m32).u32(n32).u32(ld32).ptr(dg).ptr(du);
   }
-  if (has_dx && m)
-    p.add("tiler_gated_bf16_dx_g", (uint32_t)ceil_div(k, 128), (uint32_t)ceil_div(m, 128), 256)
-        .ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx);
-  if (has_dw && n)
-    p.add("tiler_gated_bf16_dw_g", (uint32_t)ceil_div(k, 128), (uint32_t)(2 * ceil_div(n, 128)), 256)
-        .ptr(dg).ptr(du).u32(ld32).ptr(x).u32(m32).u32(n32).u32(k32).u32((uint32_t)ceil_div(n, 128)).ptr(dwg).ptr(dwu);
+  // Columns of the weights and of x (k of them a row) are read in 16-byte pieces.
+  const bool rows_ok = staged_rows(2 * k) && staged_rows(2 * ld);
+  if (has_dx && m) {
+    const uint32_t tile = staged_tile(t, m, 256, k);
+    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(k, tile));
+    if (rows_ok && aligned16(addr[wg]) && aligned16(addr[wu]) && grid_holds(tiles, 512))
+      add_tiles(p, "tiler_gated_bf16_dx", tile, tiles)
+          .ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx);
+    else
+      p.add("tiler_gated_bf16_dx_g", (uint32_t)ceil_div(k, 128), (uint32_t)ceil_div(m, 128), 256)
+          .ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx);
+  }
+  if (has_dw && n) {
+    const uint32_t tile = staged_tile(t, 2 * n, 256, k);
+    const uint64_t tiles = mul_sat(2 * ceil_div(n, tile), ceil_div(k, tile));
+    if (rows_ok && aligned16(addr[x]) && grid_holds(tiles, 512))
+      add_tiles(p, "tiler_gated_bf16_dw", tile, tiles)
+          .ptr(dg).ptr(du).u32(ld32).ptr(x).u32(m32).u32(n32).u32(k32).ptr(dwg).ptr(dwu);
+    else
+      p.add("tiler_gated_bf16_dw_g", (uint32_t)ceil_div(k, 128), (uint32_t)(2 * ceil_div(n, 128)), 256)
+          .ptr(dg).ptr(du).u32(ld32).ptr(x).u32(m32).u32(n32).u32(k32).u32((uint32_t)ceil_div(n, 128)).ptr(dwg).ptr(dwu);
+  }
   return TILER_HIP_OK;
 }
 
@@ -183,8 +225,8 @@ tiler_hip_status plan_quantize_rows_i8(const Target&, uint32_t dtype, uint64_t r
 }
 
 // Slots: a, b, a_scales, b_scales, c.
-tiler_hip_status plan_contract_i8(const Target&, uint32_t out_dtype, uint64_t m, uint64_t n, uint64_t k,
-                                  const uintptr_t*, Program& p) {
+tiler_hip_status plan_contract_i8(const Target& t, uint32_t out_dtype, uint64_t m, uint64_t n, uint64_t k,
+                                  const uintptr_t* addr, Program& p) {
   if (out_dtype != TILER_HIP_F32 && out_dtype != TILER_HIP_BF16)
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "contract_i8 result dtype");
   const uint32_t a = p.slot(mul_sat(m, k), kSlotInput), b = p.slot(mul_sat(n, k), kSlotInput);
@@ -194,6 +236,15 @@ tiler_hip_status plan_contract_i8(const Target&, uint32_t out_dtype, uint64_t m,
   if (k > 131071) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "a sum of more than 131071 products could leave 32 bits");
   if (m == 0 || n == 0) return TILER_HIP_OK;
   char name[64];
+  if (staged_rows(k) && aligned16(addr[a]) && aligned16(addr[b])) {
+    const uint32_t tile = staged_tile(t, m, 256, n);
+    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(n, tile));
+    if (grid_holds(tiles, 512)) {
+      add_tiles(p, std::string("tiler_contract_i8_") + type_name(out_dtype), tile, tiles)
+          .ptr(a).ptr(b).ptr(sa).ptr(sb).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(c);
+      return TILER_HIP_OK;
+    }
+  }
   std::snprintf(name, sizeof(name), "tiler_contract_i8_%s_g", type_name(out_dtype));
   p.add(name, (uint32_t)ceil_div(n, 128), (uint32_t)ceil_div(m, 128), 256)
       .ptr(a).ptr(b).ptr(sa).ptr(sb).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(c);

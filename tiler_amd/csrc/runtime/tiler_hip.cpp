@@ -373,6 +373,14 @@ const EntryRow kEntries[] = {
     {"tiler_quantize_rows_i8_f32", "quantize-rows-i8/f32", 3},
     {"tiler_contract_i8_bf16_g", "tensor-contraction-i8/bf16", 5},
     {"tiler_contract_i8_f32_g", "tensor-contraction-i8/f32", 5},
+#define TILER_STAGED_ROWS(TILE)                                                            \
+  {"tiler_gated_bf16_t" TILE, "gated-contraction-bf16", 6},                                 \
+      {"tiler_gated_bf16_dx_t" TILE, "gated-contraction-bf16-backward", 5},                 \
+      {"tiler_gated_bf16_dw_t" TILE, "gated-contraction-bf16-backward", 5},                 \
+      {"tiler_contract_i8_bf16_t" TILE, "tensor-contraction-i8/bf16", 5},                   \
+      {"tiler_contract_i8_f32_t" TILE, "tensor-contraction-i8/f32", 5}
+    TILER_STAGED_ROWS("256"), TILER_STAGED_ROWS("128"),
+#undef TILER_STAGED_ROWS
 };
 constexpr uint32_t kEntryCount = sizeof(kEntries) / sizeof(kEntries[0]);
 
