@@ -7,6 +7,7 @@
 // |sum| <= 2^31 - 2^14 for every pair of codes, -128 included); it is rounded
 // to binary32, multiplied by sa_i, then by sb_j, and narrowed to bf16 where C is bf16.
 #include "product.h"
+#include "row_pieces.h"
 
 namespace {
 
@@ -37,12 +38,85 @@ __device__ __forceinline__ int32_t code_of(float x, float s, float inverse) {
 // order as the magnitudes do, infinity and NaN last.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// One workgroup per row, any extent and alignment: the row is read twice, the
-// second time from the caches.
+// The largest magnitude of a group of WAVES waves, in every lane.
+template <int WAVES>
+__device__ __forceinline__ uint32_t group_top(uint32_t top, uint32_t* slots) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint32_t other = __shfl_xor(top, o, 64);
+    top = other > top ? other : top;
+  }
+  if constexpr (WAVES > 1) {
+    __syncthreads();  // a row before is done with the slots
+    if ((threadIdx.x & 63u) == 0) slots[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = slots[w] > top ? slots[w] : top;
+  }
+  return top;
+}
+
+// A group of WAVES waves per row, CH pieces a thread held in registers between
+// the maximum and the codes: x read once.  8 codes (bf16) or 4 (f32) leave in
+// one store.
+template <typename T, int WAVES, int CH>
+__device__ __forceinline__ void quantize_rows(const T* __restrict__ x, uint64_t rows, uint32_t extent,
+                                              int8_t* __restrict__ q, float* __restrict__ scales) {
+  using namespace tiler_rows;
+  constexpr int V = kVec<T>;
+  __shared__ uint32_t slots[WAVES];
+  const uint32_t t = threadIdx.x % (64u * WAVES);
+  const uint64_t row = (uint64_t)blockIdx.x * (WAVES == 1 ? 4 : 1) + threadIdx.x / (64u * WAVES);
+  if (row >= rows) return;  // whole groups
+  x += row * extent;
+  q += row * extent;
+  u32x4 v[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) v[c] = load_piece<T, true>(x, (c * 64u * WAVES + t) * V, extent);
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t b = magnitude(element<T>(v[c], i));
+      top = b > top ? b : top;
+    }
+  top = group_top<WAVES>(top, slots);
+#pragma unroll
+  for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(v[c]));  // widened again below, not kept widened
+  const bool finite = top < 0x7f800000u;
+  const float s = finite ? row_scale(__uint_as_float(top)) : __uint_as_float(TILER_CANONICAL_F32_NAN);
+  const float inverse = 1.0f / s;
+  if (t == 0) scales[row] = s;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t at = (c * 64u * WAVES + t) * V, valid = valid_from<T>(at, extent);
+    if (valid == 0) continue;
+    uint32_t words[V / 4];
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) word |= (uint32_t)(uint8_t)code_of(element<T>(v[c], 4 * h + e), s, inverse) << (8 * e);
+      words[h] = finite ? word : 0u;
+    }
+    if (valid == (uint32_t)V) {
+      if constexpr (V == 8) *reinterpret_cast<u32x2_any*>(q + at) = u32x2{words[0], words[1]};
+      else *reinterpret_cast<u32_any*>(q + at) = words[0];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V - 1; ++e)
+        if ((uint32_t)e < valid) q[at + e] = (int8_t)(words[e >> 2] >> (8 * (e & 3)));
+    }
+  }
+}
+
+// Any number of rows of any extent: one workgroup per row at a time, the row
+// read twice, the second time from the caches.
 template <typename T>
-__device__ __forceinline__ void quantize_rows_body(const T* __restrict__ x, uint64_t rows, uint64_t extent,
-                                                   int8_t* __restrict__ q, float* __restrict__ scales) {
-  __shared__ uint32_t waves[4];
+__device__ __forceinline__ void quantize_stream(const T* __restrict__ x, uint64_t rows, uint64_t extent,
+                                                int8_t* __restrict__ q, float* __restrict__ scales) {
+  __shared__ uint32_t slots[4];
   for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * extent;
     int8_t* qr = q + row * extent;
@@ -55,16 +129,7 @@ __device__ __forceinline__ void quantize_rows_body(const T* __restrict__ x, uint
       const uint32_t b = magnitude(value(i));
       top = b > top ? b : top;
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const uint32_t other = __shfl_xor(top, o, 64);
-      top = other > top ? other : top;
-    }
-    __syncthreads();  // the row before is done with the waves' words
-    if ((threadIdx.x & 63u) == 0) waves[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; ++w) top = waves[w] > top ? waves[w] : top;
+    top = group_top<4>(top, slots);
     const bool finite = top < 0x7f800000u;
     const float s = finite ? row_scale(__uint_as_float(top)) : __uint_as_float(TILER_CANONICAL_F32_NAN);
     const float inverse = 1.0f / s;
@@ -76,16 +141,31 @@ __device__ __forceinline__ void quantize_rows_body(const T* __restrict__ x, uint
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256)
-tiler_quantize_rows_i8_bf16(const uint16_t* __restrict__ x, uint64_t rows, uint64_t extent, int8_t* __restrict__ q,
-                            float* __restrict__ scales) {
-  quantize_rows_body<uint16_t>(x, rows, extent, q, scales);
-}
-extern "C" __global__ void __launch_bounds__(256)
-tiler_quantize_rows_i8_f32(const float* __restrict__ x, uint64_t rows, uint64_t extent, int8_t* __restrict__ q,
-                           float* __restrict__ scales) {
-  quantize_rows_body<float>(x, rows, extent, q, scales);
-}
+#define TILER_QUANTIZE_ROWS(TY, T, WAVES, CH)                                                              \
+  extern "C" __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)                              \
+      tiler_quantize_rows_i8_##TY##_w##WAVES##c##CH(const T* __restrict__ x, uint64_t rows, uint64_t extent, \
+                                                    int8_t* __restrict__ q, float* __restrict__ scales) {  \
+    quantize_rows<T, WAVES, CH>(x, rows, (uint32_t)extent, q, scales);                                     \
+  }
+#define TILER_QUANTIZE_FORMS(TY, T)                                                                        \
+  extern "C" __global__ void __launch_bounds__(256)                                                        \
+      tiler_quantize_rows_i8_##TY##_s(const T* __restrict__ x, uint64_t rows, uint64_t extent,             \
+                                      int8_t* __restrict__ q, float* __restrict__ scales) {                \
+    quantize_stream<T>(x, rows, extent, q, scales);                                                        \
+  }                                                                                                        \
+  TILER_QUANTIZE_ROWS(TY, T, 1, 1)                                                                         \
+  TILER_QUANTIZE_ROWS(TY, T, 1, 2)                                                                         \
+  TILER_QUANTIZE_ROWS(TY, T, 1, 4)                                                                         \
+  TILER_QUANTIZE_ROWS(TY, T, 1, 8)                                                                         \
+  TILER_QUANTIZE_ROWS(TY, T, 1, 16)                                                                        \
+  TILER_QUANTIZE_ROWS(TY, T, 4, 1)                                                                         \
+  TILER_QUANTIZE_ROWS(TY, T, 4, 2)                                                                         \
+  TILER_QUANTIZE_ROWS(TY, T, 4, 4)                                                                         \
+  TILER_QUANTIZE_ROWS(TY, T, 16, 1)                                                                        \
+  TILER_QUANTIZE_ROWS(TY, T, 16, 2)                                                                        \
+  TILER_QUANTIZE_ROWS(TY, T, 16, 4)
+TILER_QUANTIZE_FORMS(bf16, uint16_t)
+TILER_QUANTIZE_FORMS(f32, float)
 
 namespace {
 

@@ -4,7 +4,7 @@
 //   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) r w + b
 //   xh = (x - mu) r, g = dy w:
 //   dx = r (g - mean(g) - xh mean(g xh)), dw = sum over rows of dy xh, db = of dy
-#include "common.h"
+#include "row_pieces.h"
 
 namespace {
 
@@ -83,6 +83,238 @@ __device__ __forceinline__ void layer_norm_grad_stream(const T* __restrict__ dy,
   }
 }
 
+// ---------------------------------------------------------------------------
+// Rows in registers.
+
+// Forward: a group of WAVES waves per row, CH pieces a thread.  The mean is
+// taken first, then the differences' sum and squares: the first corrects the
+// mean's rounding, so that neither a large offset nor the grouping of the sum
+// reaches the variance.
+template <typename T, int WAVES, int CH>
+__device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T* __restrict__ w,
+                                                const T* __restrict__ b, uint64_t rows, uint32_t extent, float eps,
+                                                T* __restrict__ y, float* __restrict__ mean,
+                                                float* __restrict__ rstd) {
+  using namespace tiler_rows;
+  constexpr int V = kVec<T>;
+  constexpr uint32_t kGroups = WAVES == 1 ? 4 : 1;
+  __shared__ float slots[2][2 * (WAVES == 1 ? 1 : WAVES)];
+  const uint32_t t = threadIdx.x % (64u * WAVES);
+  const uint64_t row = (uint64_t)blockIdx.x * kGroups + threadIdx.x / (64u * WAVES);
+  if (row >= rows) return;  // whole groups
+  x += row * extent;
+  y += row * extent;
+  u32x4 v[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) v[c] = load_piece<T, true>(x, (c * 64u * WAVES + t) * V, extent);
+  float s = 0.0f, none = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    float e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = element<T>(v[c], i);
+    s += pairwise(e);
+  }
+  group_sums<WAVES>(s, none, slots[0]);
+  // opaque: widened again below, not kept widened across the sums
+#pragma unroll
+  for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(v[c]));
+  const float count = (float)extent, mu0 = s / count;
+  float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t valid = valid_from<T>((c * 64u * WAVES + t) * V, extent);
+    float d[V], q[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      d[i] = (uint32_t)i < valid ? element<T>(v[c], i) - mu0 : 0.0f;
+      q[i] = d[i] * d[i];
+    }
+    s1 += pairwise(d);
+    s2 += pairwise(q);
+  }
+  group_sums<WAVES>(s1, s2, slots[1]);
+#pragma unroll
+  for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(v[c]));
+  const float shift = s1 / count, var = s2 / count - shift * shift, mu = mu0 + shift;
+  const float r = 1.0f / __builtin_sqrtf((var < 0.0f ? 0.0f : var) + eps);
+  if (t == 0 && mean) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t at = (c * 64u * WAVES + t) * V;
+    if (at >= extent) continue;
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = ((element<T>(v[c], i) - mu0) - shift) * r;
+    if (w) {
+      const u32x4 wv = load_piece<T, false>(w, at, extent);
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = o[i] * element<T>(wv, i);
+    }
+    if (b) {
+      const u32x4 bv = load_piece<T, false>(b, at, extent);
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = o[i] + element<T>(bv, i);
+    }
+    store_piece<T>(y, at, extent, o);
+  }
+}
+
+// Gradients, one read of dy and x: a workgroup of 16 waves holds 16 / WAVES
+// rows at a time and walks the rows with a stride of the whole grid; a thread
+// keeps the column sums of its own pieces over all of its rows, the groups meet
+// in LDS, and each workgroup leaves one partial (dw's sums, then db's), or the
+// results themselves where it is the only one.  The next rows are loaded
+// before the current ones are reduced.
+template <typename T, int WAVES, int CH, bool kAhead, bool kWhole>
+__device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, const T* __restrict__ x,
+                                                     const T* __restrict__ w, const float* __restrict__ mean,
+                                                     const float* __restrict__ rstd, uint64_t rows, uint32_t extent,
+                                                     T* __restrict__ dx, float* __restrict__ partials,
+                                                     T* __restrict__ dw, T* __restrict__ db) {
+  using namespace tiler_rows;
+  constexpr int V = kVec<T>;
+  constexpr uint32_t kGroups = 16 / WAVES, kSpan = CH * 64u * WAVES * V;  // elements a group's pieces cover
+  __shared__ float slots[2][32];
+  __shared__ float columns[kGroups > 1 ? 2 * kSpan : 1];
+  const uint32_t t = threadIdx.x % (64u * WAVES), group = threadIdx.x / (64u * WAVES);
+  const bool sums = partials || dw || db;
+  float aw[CH][V], ab[CH][V];
+  u32x4 wv[CH], xv[CH], dv[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t at = (c * 64u * WAVES + t) * V;
+    wv[c] = w ? load_piece<T, false, kWhole>(w, at, extent) : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < V; ++i) aw[c][i] = ab[c][i] = 0.0f;
+  }
+  const uint64_t step = (uint64_t)gridDim.x * kGroups;
+  uint64_t row = (uint64_t)blockIdx.x * kGroups + group;
+  const uint64_t rounds = (rows - (uint64_t)blockIdx.x * kGroups + step - 1) / step;  // the first group's: the same for all
+  float mu = 0.0f, r = 0.0f;
+  auto load = [&](uint64_t at_row, u32x4(&xo)[CH], u32x4(&dyo)[CH], float& muo, float& ro) {
+    const bool real = at_row < rows;
+    muo = real ? mean[at_row] : 0.0f;
+    ro = real ? rstd[at_row] : 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const uint32_t at = (c * 64u * WAVES + t) * V;
+      // a group past the last row holds zeros: its sums and stores drop out
+      xo[c] = real ? load_piece<T, true, kWhole>(x + at_row * extent, at, extent) : u32x4{0, 0, 0, 0};
+      dyo[c] = real ? load_piece<T, true, kWhole>(dy + at_row * extent, at, extent) : u32x4{0, 0, 0, 0};
+    }
+  };
+  load(row, xv, dv, mu, r);
+#pragma unroll 1
+  for (uint64_t k = 0; k < rounds; ++k) {
+    u32x4 xn[CH], dn[CH];
+    float mun = 0.0f, rn = 0.0f;
+    if (kAhead && k + 1 < rounds) load(row + step, xn, dn, mun, rn);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float g[V], q[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        // past the row's end dy is zero, and so are the terms
+        const float d = element<T>(dv[c], i), xh = (element<T>(xv[c], i) - mu) * r;
+        g[i] = w ? d * element<T>(wv[c], i) : d;
+        q[i] = g[i] * xh;
+        aw[c][i] += d * xh;
+        ab[c][i] += d;
+        asm volatile("" : "+v"(aw[c][i]), "+v"(ab[c][i]));  // added here, not past the barrier with its terms kept
+      }
+      s1 += pairwise(g);
+      s2 += pairwise(q);
+      __builtin_amdgcn_sched_barrier(0);  // one piece's temporaries at a time
+    }
+    // opaque: widened again below, not kept widened across the sums
+#pragma unroll
+    for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(xv[c]), "+v"(dv[c]), "+v"(wv[c]));
+    if (dx) {  // uniform: every wave takes the same barriers
+      group_sums<WAVES>(s1, s2, slots[k & 1u]);
+      const float c1 = s1 / (float)extent, c2 = s2 / (float)extent;
+      if (row < rows) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const uint32_t at = (c * 64u * WAVES + t) * V;
+          if (at >= extent) continue;
+          float o[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = element<T>(dv[c], i), g = w ? d * element<T>(wv[c], i) : d;
+            o[i] = r * (g - c1 - (element<T>(xv[c], i) - mu) * r * c2);
+          }
+          store_piece<T, kWhole>(dx + row * extent, at, extent, o);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    row += step;
+    if (k + 1 < rounds) {
+      if (kAhead) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          xv[c] = xn[c];
+          dv[c] = dn[c];
+        }
+        mu = mun;
+        r = rn;
+      } else {
+        load(row, xv, dv, mu, r);
+      }
+    }
+  }
+  if (!sums) return;
+  // The groups' columns, added in ascending order of the groups.
+  if constexpr (kGroups > 1) {
+    for (uint32_t q = 1; q < kGroups; ++q) {
+      __syncthreads();
+      if (group == q) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            columns[(c * V + i) * 64u * WAVES + t] = aw[c][i];
+            columns[kSpan + (c * V + i) * 64u * WAVES + t] = ab[c][i];
+          }
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            aw[c][i] += columns[(c * V + i) * 64u * WAVES + t];
+            ab[c][i] += columns[kSpan + (c * V + i) * 64u * WAVES + t];
+          }
+      }
+    }
+    if (group != 0) return;
+  }
+  const bool alone = gridDim.x == 1;
+  float* out = alone ? nullptr : partials + (uint64_t)blockIdx.x * 2u * extent;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t at = (c * 64u * WAVES + t) * V;
+    if (at >= extent) continue;
+    if (alone) {
+      if (dw) store_piece<T, kWhole>(dw, at, extent, aw[c]);
+      if (db) store_piece<T, kWhole>(db, at, extent, ab[c]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (at + i < extent) {
+          out[at + i] = aw[c][i];
+          out[extent + at + i] = ab[c][i];
+        }
+    }
+  }
+}
+
 // Column sums over a strip of rows: blockIdx.x takes 256 columns, blockIdx.y
 // rows [y * strip, ...); partial y holds dw's sums, then db's.
 template <typename T>
@@ -104,14 +336,24 @@ __device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, con
   out[extent + col] = sb;
 }
 
-// dw and db from `count` partials, in ascending order of the strips.
+// dw and db from `count` partials: 64 columns a workgroup, wave q the partials
+// q, q + 16, ... in ascending order, the waves' sums in ascending order.
 template <typename T>
 __device__ __forceinline__ void layer_norm_columns_final(const float* __restrict__ partials, uint32_t count,
                                                          uint64_t extent, T* __restrict__ dw, T* __restrict__ db) {
-  const uint64_t i = blockIdx.x * 256ull + threadIdx.x;
-  if (i >= 2u * extent) return;
+  __shared__ float waves[16][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint64_t i = blockIdx.x * 64ull + lane;
   float s = 0.0f;
-  for (uint32_t p = 0; p < count; ++p) s += partials[(uint64_t)p * 2u * extent + i];
+  if (i < 2u * extent) {
+#pragma unroll 8
+    for (uint32_t p = wave; p < count; p += 16u) s += partials[(uint64_t)p * 2u * extent + i];
+  }
+  waves[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || i >= 2u * extent) return;
+#pragma unroll
+  for (int q = 1; q < 16; ++q) s += waves[q][lane];
   T* out = i < extent ? dw : db;
   if (out) norm_store(out, i < extent ? i : i - extent, s);
 }
@@ -139,10 +381,54 @@ __device__ __forceinline__ void layer_norm_columns_final(const float* __restrict
                                     float* __restrict__ partials) {                                       \
     layer_norm_columns<T>(dy, x, mean, rstd, rows, extent, strip, partials);                              \
   }                                                                                                       \
-  extern "C" __global__ void __launch_bounds__(256)                                                       \
+  extern "C" __global__ void __launch_bounds__(1024)                                                      \
       tiler_layer_norm_columns_final_##TY(const float* __restrict__ partials, uint32_t count,             \
                                           uint64_t extent, T* __restrict__ dw, T* __restrict__ db) {      \
     layer_norm_columns_final<T>(partials, count, extent, dw, db);                                         \
   }
 TILER_LAYER_NORM(bf16, uint16_t)
 TILER_LAYER_NORM(f32, float)
+
+#define TILER_LAYER_NORM_ROWS(TY, T, WAVES, CH)                                                            \
+  extern "C" __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)                              \
+      tiler_layer_norm_##TY##_w##WAVES##c##CH(const T* __restrict__ x, const T* __restrict__ w,            \
+                                              const T* __restrict__ b, uint64_t rows, uint64_t extent,     \
+                                              float eps, T* __restrict__ y, float* __restrict__ mean,      \
+                                              float* __restrict__ rstd) {                                  \
+    layer_norm_rows<T, WAVES, CH>(x, w, b, rows, (uint32_t)extent, eps, y, mean, rstd);                    \
+  }
+#define TILER_LAYER_NORM_GRAD_ROWS(TY, T, WAVES, CH, NAME, AHEAD, WHOLE)                                   \
+  extern "C" __global__ void __launch_bounds__(1024)                                                       \
+      tiler_layer_norm_grad_##TY##_w##WAVES##c##CH##NAME(                                                  \
+          const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ w,                      \
+          const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint64_t extent,  \
+          T* __restrict__ dx, float* __restrict__ partials, T* __restrict__ dw, T* __restrict__ db) {      \
+    layer_norm_grad_rows<T, WAVES, CH, AHEAD, WHOLE>(dy, x, w, mean, rstd, rows, (uint32_t)extent, dx,     \
+                                                     partials, dw, db);                                    \
+  }
+#define TILER_LAYER_NORM_FORMS(TY, T)      \
+  TILER_LAYER_NORM_ROWS(TY, T, 1, 1)       \
+  TILER_LAYER_NORM_ROWS(TY, T, 1, 2)       \
+  TILER_LAYER_NORM_ROWS(TY, T, 1, 4)       \
+  TILER_LAYER_NORM_ROWS(TY, T, 1, 8)       \
+  TILER_LAYER_NORM_ROWS(TY, T, 1, 16)      \
+  TILER_LAYER_NORM_ROWS(TY, T, 4, 1)       \
+  TILER_LAYER_NORM_ROWS(TY, T, 4, 2)       \
+  TILER_LAYER_NORM_ROWS(TY, T, 4, 4)       \
+  TILER_LAYER_NORM_ROWS(TY, T, 16, 1)      \
+  TILER_LAYER_NORM_ROWS(TY, T, 16, 2)      \
+  TILER_LAYER_NORM_ROWS(TY, T, 16, 4)      \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 1, 1, , true, true) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 2, 1, , true, true) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 4, 1, , true, true) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 8, 1, , true, true) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 1, , true, true) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 2, , true, true) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 1, 1, r, false, false) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 2, 1, r, false, false) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 4, 1, r, false, false) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 8, 1, r, false, false) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 1, r, false, false) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 2, r, false, false)
+TILER_LAYER_NORM_FORMS(bf16, uint16_t)
+TILER_LAYER_NORM_FORMS(f32, float)

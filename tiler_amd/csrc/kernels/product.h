@@ -18,7 +18,7 @@
 // Both layouts deal a lane the same depth elements, so they mix freely.
 #pragma once
 
-#include "common.h"
+#include "pieces.h"
 
 namespace tiler_product {
 
@@ -27,8 +27,8 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_bytes;
-// 16 bytes at any byte address (global memory takes unaligned vector accesses)
-typedef u32x4 u32x4_any __attribute__((aligned(1)));
+using tiler_pieces::guarded_piece;
+using tiler_pieces::u32x4_any;
 
 constexpr uint32_t kSlice = 128;  // bytes of depth per tile
 
@@ -96,34 +96,6 @@ struct Fragments {
     }
   }
 };
-
-// Sixteen bytes from `p` of which the first `valid` (at least 1) exist; the
-// rest zero.  `start` is where the operand starts: a short piece is the end of
-// the 16 bytes before its end, or, next to the operand's start, read by bytes.
-__device__ __forceinline__ u32x4 guarded_piece(const uint8_t* p, uint32_t valid, const uint8_t* start) {
-  if (valid >= 16u) return *reinterpret_cast<const u32x4_any*>(p);
-  uint64_t lo = 0, hi = 0;
-  const uint32_t missing = 16u - valid;
-  if ((uint64_t)(p - start) >= missing) {
-    const u32x4 v = *reinterpret_cast<const u32x4_any*>(p - missing);
-    lo = (uint64_t)v.y << 32 | v.x;
-    hi = (uint64_t)v.w << 32 | v.z;
-    if (missing >= 8u) {
-      lo = hi >> (8u * (missing - 8u));
-      hi = 0;
-    } else {
-      lo = lo >> (8u * missing) | hi << (64u - 8u * missing);
-      hi >>= 8u * missing;
-    }
-  } else {
-#pragma unroll 1
-    for (uint32_t e = valid; e-- > 0;) {
-      hi = hi << 8 | lo >> 56;
-      lo = lo << 8 | p[e];
-    }
-  }
-  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
-}
 
 // An operand in memory: `rows` indices of the result, `depth` contracted ones,
 // `ld` elements between consecutive rows (row layout) or depth rows (column).

@@ -1,0 +1,115 @@
+// Rows held in registers by a group of WAVES waves, 16-byte pieces at any
+// alignment: piece c of thread t of the group starts at element
+// (c 64 WAVES + t) kVec of its row (kVec = 8 bf16 or 4 f32), so each load
+// instruction of a wave covers 1 KiB of contiguous row.
+#pragma once
+
+#include "pieces.h"
+
+namespace tiler_rows {
+
+using tiler_pieces::u32_any;
+using tiler_pieces::u32x2_any;
+using tiler_pieces::u32x4_any;
+
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+// Element e of a piece, widened.
+template <typename T>
+__device__ __forceinline__ float element(const u32x4& v, int e) {
+  if constexpr (sizeof(T) == 2) return __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
+  else return __uint_as_float(v[e]);
+}
+
+// How many of the elements from `at` lie in the row.
+template <typename T>
+__device__ __forceinline__ uint32_t valid_from(uint32_t at, uint32_t extent) {
+  return at >= extent ? 0u : extent - at < (uint32_t)kVec<T> ? extent - at : (uint32_t)kVec<T>;
+}
+
+// The piece at `at`, zeros past the row's end.  kStream: read once, past the
+// caches.  kWhole: the extent is a multiple of kVec, so no piece is cut.
+template <typename T, bool kStream, bool kWhole = false>
+__device__ __forceinline__ u32x4 load_piece(const T* row, uint32_t at, uint32_t extent) {
+  if constexpr (kWhole) {
+    if (at >= extent) return u32x4{0, 0, 0, 0};
+    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + at);
+    return kStream ? __builtin_nontemporal_load(p) : *p;
+  }
+  const uint32_t valid = valid_from<T>(at, extent);
+  if (valid == (uint32_t)kVec<T>) {
+    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + at);
+    return kStream ? __builtin_nontemporal_load(p) : *p;
+  }
+  if (valid == 0) return u32x4{0, 0, 0, 0};
+  return tiler_pieces::guarded_piece(reinterpret_cast<const uint8_t*>(row + at), valid * (uint32_t)sizeof(T),
+                                     reinterpret_cast<const uint8_t*>(row));
+}
+
+// Narrows and stores the piece's elements inside the row.
+template <typename T, bool kWhole = false>
+__device__ __forceinline__ void store_piece(T* row, uint32_t at, uint32_t extent, const float (&o)[kVec<T>]) {
+  const uint32_t valid = valid_from<T>(at, extent);
+  u32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 2) v[e] = tiler::bf16_pack2_rne(o[2 * e], o[2 * e + 1]);
+    else v[e] = __float_as_uint(tiler::canon(o[e]));
+  }
+  if (kWhole || valid == (uint32_t)kVec<T>) {
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(row + at));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kVec<T> - 1; ++e)
+    if ((uint32_t)e < valid) {
+      if constexpr (sizeof(T) == 2) row[at + e] = (T)(v[e >> 1] >> (16 * (e & 1)));
+      else row[at + e] = __uint_as_float(v[e]);
+    }
+}
+
+// Sum of a kVec run, in pairs.
+template <int N>
+__device__ __forceinline__ float pairwise(const float (&v)[N]) {
+  if constexpr (N == 8) return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+  else return (v[0] + v[1]) + (v[2] + v[3]);
+}
+
+// Two sums over a group of WAVES waves, the same values in every lane.  The
+// waves of one workgroup all call it; `slots` holds 2 floats per wave, and a
+// caller alternates between two such arrays from call to call, so that one
+// barrier a call is enough.
+template <int WAVES>
+__device__ __forceinline__ void group_sums(float& a, float& b, float* slots) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    a += __shfl_xor(a, o, 64);
+    b += __shfl_xor(b, o, 64);
+  }
+  if constexpr (WAVES > 1) {
+    const uint32_t wave = threadIdx.x >> 6, first = wave / WAVES * WAVES;
+    if ((threadIdx.x & 63u) == 0) {
+      slots[2u * wave] = a;
+      slots[2u * wave + 1u] = b;
+    }
+    __syncthreads();
+    float sa[WAVES], sb[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      sa[w] = slots[2u * (first + w)];
+      sb[w] = slots[2u * (first + w) + 1u];
+    }
+#pragma unroll
+    for (int s = 1; s < WAVES; s *= 2)
+#pragma unroll
+      for (int w = 0; w + s < WAVES; w += 2 * s) {
+        sa[w] += sa[w + s];
+        sb[w] += sb[w + s];
+      }
+    a = sa[0];
+    b = sb[0];
+  }
+}
+
+}  // namespace tiler_rows

@@ -24,12 +24,45 @@ void slot_or_null(Launch& l, bool present, uint32_t slot) {
   else l.null_ptr();
 }
 
-constexpr uint32_t kNormRowWorkgroups = 1u << 20;  // rows beyond take further rounds of the row loops
+constexpr uint32_t kRowWorkgroups = 1u << 20;  // rows beyond take further rounds of the streamed forms' row loops
+
+// The register form of a row kernel (row_pieces.h) for rows of `extent`
+// elements, kVec = `vec` to a 16-byte piece: WAVES waves per row and CH pieces
+// a thread, "w{WAVES}c{CH}", or "s" (streamed) beyond what registers hold.
+// One wave a row (four rows a workgroup, no barrier) where that gives every
+// SIMD a wave and a thread at most 16 pieces; fewer rows than that, or longer
+// ones, take four waves a row, then sixteen.
+struct RowForm {
+  char name[16];
+  uint32_t block;
+  uint64_t grid;
+};
+RowForm row_form(const Target& t, uint64_t rows, uint64_t extent, uint64_t vec) {
+  const uint64_t pieces = ceil_div(extent, vec);
+  RowForm f{"s", 256, rows < kRowWorkgroups ? rows : kRowWorkgroups};
+  uint32_t waves = 0, ch = 0;
+  auto pow2 = [](uint64_t v) {
+    uint32_t p = 1;
+    while (p < v) p <<= 1;
+    return p;
+  };
+  if (pieces <= 64 || (pieces <= 64 * 16 && rows >= 4ull * t.compute_units)) waves = 1, ch = pow2(ceil_div(pieces, 64));
+  else if (pieces <= 256 * 4) waves = 4, ch = pow2(ceil_div(pieces, 256));
+  else if (pieces <= 1024 * 4) waves = 16, ch = pow2(ceil_div(pieces, 1024));
+  const uint32_t block = waves == 1 ? 256 : 64 * waves;
+  const uint64_t grid = waves == 1 ? ceil_div(rows, 4) : rows;
+  if (waves && grid_holds(grid, block)) {
+    std::snprintf(f.name, sizeof(f.name), "w%uc%u", waves, ch);
+    f.block = block;
+    f.grid = grid;
+  }
+  return f;
+}
 
 }  // namespace
 
 // Slots: x, [w,] [b,] y, [mean, rstd].
-tiler_hip_status plan_layer_norm(const Target&, uint32_t dtype, uint32_t parts, uint64_t rows, uint64_t extent,
+tiler_hip_status plan_layer_norm(const Target& t, uint32_t dtype, uint32_t parts, uint64_t rows, uint64_t extent,
                                  uint32_t eps_bits, const uintptr_t*, Program& p) {
   float eps;
   std::memcpy(&eps, &eps_bits, 4);
@@ -51,8 +84,9 @@ tiler_hip_status plan_layer_norm(const Target&, uint32_t dtype, uint32_t parts, 
   if (rows == 0 || extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
-  std::snprintf(name, sizeof(name), "tiler_layer_norm_%s_s", type_name(dtype));
-  Launch& l = p.add(name, (uint32_t)(rows < kNormRowWorkgroups ? rows : kNormRowWorkgroups), 1, 256).ptr(x);
+  const RowForm f = row_form(t, rows, extent, 16 / elem);
+  std::snprintf(name, sizeof(name), "tiler_layer_norm_%s_%s", type_name(dtype), f.name);
+  Launch& l = p.add(name, (uint32_t)f.grid, 1, f.block).ptr(x);
   slot_or_null(l, has_w, w);
   slot_or_null(l, has_b, b);
   l.u64(rows).u64(extent).f32(eps).ptr(y);
@@ -80,23 +114,49 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
   if (extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
-  if (has_dx && rows) {
-    std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_s", type_name(dtype));
-    Launch& l = p.add(name, (uint32_t)(rows < kNormRowWorkgroups ? rows : kNormRowWorkgroups), 1, 256).ptr(dy).ptr(x);
+  const bool sums = has_dw || has_db;
+  if (!has_dx && !sums) return TILER_HIP_OK;
+  const uint64_t vec = 16 / elem, pieces = ceil_div(extent, vec);
+  const uint32_t waves = pieces <= 64 ? 1 : pieces <= 128 ? 2 : pieces <= 256 ? 4 : pieces <= 512 ? 8 : 16;
+  uint64_t count = 0;  // partials of dw's and db's sums
+  uint32_t partials = 0;
+  if (rows && pieces <= 2048) {
+    // Rows in registers, 16 / WAVES of them per workgroup at a time: at most
+    // one workgroup per CU, so that there are few partials.  "r": the last
+    // piece of a row is cut.
+    const uint64_t groups = ceil_div(rows, 16 / waves);
+    count = groups < t.compute_units ? groups : t.compute_units;
+    if (sums && count > 1) partials = p.slot(mul_sat(mul_sat(count, extent), 8), kSlotScratch);
+    std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_w%uc%u%s", type_name(dtype), waves,
+                  pieces <= 1024 ? 1u : 2u, extent % vec ? "r" : "");
+    Launch& l = p.add(name, (uint32_t)count, 1, 1024).ptr(dy).ptr(x);
     slot_or_null(l, has_w, w);
-    l.ptr(mean).ptr(rstd).u64(rows).u64(extent).ptr(dx);
-  }
-  if (!has_dw && !has_db) return TILER_HIP_OK;
-  const uint64_t strips = rows < 4ull * t.compute_units ? ceil_div(rows, 16) : t.compute_units;
-  const uint64_t strip = rows ? ceil_div(rows, strips) : 0;
-  const uint32_t partials = p.slot(mul_sat(mul_sat(strips, extent), 8), kSlotScratch);
-  if (rows) {
+    l.ptr(mean).ptr(rstd).u64(rows).u64(extent);
+    slot_or_null(l, has_dx, dx);
+    slot_or_null(l, sums && count > 1, partials);
+    slot_or_null(l, has_dw, dw);
+    slot_or_null(l, has_db, db);
+    if (!sums || count == 1) return TILER_HIP_OK;
+  } else if (rows) {
+    if (has_dx) {
+      std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_s", type_name(dtype));
+      Launch& l = p.add(name, (uint32_t)(rows < kRowWorkgroups ? rows : kRowWorkgroups), 1, 256).ptr(dy).ptr(x);
+      slot_or_null(l, has_w, w);
+      l.ptr(mean).ptr(rstd).u64(rows).u64(extent).ptr(dx);
+    }
+    if (!sums) return TILER_HIP_OK;
+    count = ceil_div(rows, 16) < t.compute_units ? ceil_div(rows, 16) : t.compute_units;
+    partials = p.slot(mul_sat(mul_sat(count, extent), 8), kSlotScratch);
     std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_%s", type_name(dtype));
-    p.add(name, (uint32_t)ceil_div(extent, 256), (uint32_t)strips, 256)
-        .ptr(dy).ptr(x).ptr(mean).ptr(rstd).u64(rows).u64(extent).u64(strip).ptr(partials);
+    p.add(name, (uint32_t)ceil_div(extent, 256), (uint32_t)count, 256)
+        .ptr(dy).ptr(x).ptr(mean).ptr(rstd).u64(rows).u64(extent).u64(ceil_div(rows, count)).ptr(partials);
+  } else if (!sums) {
+    return TILER_HIP_OK;
   }
   std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_final_%s", type_name(dtype));
-  Launch& l = p.add(name, (uint32_t)ceil_div(2 * extent, 256), 1, 256).ptr(partials).u32((uint32_t)strips).u64(extent);
+  Launch& l = p.add(name, (uint32_t)ceil_div(2 * extent, 64), 1, 1024);
+  slot_or_null(l, count > 0, partials);  // no rows: zeros
+  l.u32((uint32_t)count).u64(extent);
   slot_or_null(l, has_dw, dw);
   slot_or_null(l, has_db, db);
   return TILER_HIP_OK;
@@ -208,7 +268,7 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
 }
 
 // Slots: x, q, scales.
-tiler_hip_status plan_quantize_rows_i8(const Target&, uint32_t dtype, uint64_t rows, uint64_t extent, const uintptr_t*,
+tiler_hip_status plan_quantize_rows_i8(const Target& t, uint32_t dtype, uint64_t rows, uint64_t extent, const uintptr_t*,
                                        Program& p) {
   if (dtype != TILER_HIP_F32 && dtype != TILER_HIP_BF16)
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "quantize_rows dtype");
@@ -218,8 +278,9 @@ tiler_hip_status plan_quantize_rows_i8(const Target&, uint32_t dtype, uint64_t r
   if (rows == 0 || extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
-  std::snprintf(name, sizeof(name), "tiler_quantize_rows_i8_%s", type_name(dtype));
-  p.add(name, (uint32_t)(rows < kNormRowWorkgroups ? rows : kNormRowWorkgroups), 1, 256)
+  const RowForm f = row_form(t, rows, extent, dtype == TILER_HIP_BF16 ? 8 : 4);
+  std::snprintf(name, sizeof(name), "tiler_quantize_rows_i8_%s_%s", type_name(dtype), f.name);
+  p.add(name, (uint32_t)f.grid, 1, f.block)
       .ptr(x).u64(rows).u64(extent).ptr(q).ptr(scales);
   return TILER_HIP_OK;
 }

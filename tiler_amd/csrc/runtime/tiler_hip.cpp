@@ -357,8 +357,6 @@ const EntryRow kEntries[] = {
     TILER_BATCHED_ROWS("skinny2_l"), TILER_BATCHED_ROWS("skinny3_l"), TILER_BATCHED_ROWS("skinny4_l"),
 #undef TILER_BATCHED_ROWS
     // the feed-forward sublayer
-    {"tiler_layer_norm_bf16_s", "layer-norm/bf16", 6},
-    {"tiler_layer_norm_f32_s", "layer-norm-f32", 6},
     {"tiler_layer_norm_grad_bf16_s", "layer-norm-backward/bf16", 6},
     {"tiler_layer_norm_grad_f32_s", "layer-norm-backward-f32", 6},
     {"tiler_layer_norm_columns_bf16", "layer-norm-backward/bf16", 5},
@@ -369,8 +367,23 @@ const EntryRow kEntries[] = {
     {"tiler_gated_bf16_grad", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dx_g", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dw_g", "gated-contraction-bf16-backward", 5},
-    {"tiler_quantize_rows_i8_bf16", "quantize-rows-i8/bf16", 3},
-    {"tiler_quantize_rows_i8_f32", "quantize-rows-i8/f32", 3},
+#define TILER_ROW_FORM(FORM)                                                   \
+  {"tiler_layer_norm_bf16_" FORM, "layer-norm/bf16", 6},                        \
+      {"tiler_layer_norm_f32_" FORM, "layer-norm-f32", 6},                      \
+      {"tiler_quantize_rows_i8_bf16_" FORM, "quantize-rows-i8/bf16", 3},        \
+      {"tiler_quantize_rows_i8_f32_" FORM, "quantize-rows-i8/f32", 3}
+    TILER_ROW_FORM("s"), TILER_ROW_FORM("w1c1"), TILER_ROW_FORM("w1c2"), TILER_ROW_FORM("w1c4"),
+    TILER_ROW_FORM("w1c8"), TILER_ROW_FORM("w1c16"), TILER_ROW_FORM("w4c1"), TILER_ROW_FORM("w4c2"),
+    TILER_ROW_FORM("w4c4"), TILER_ROW_FORM("w16c1"), TILER_ROW_FORM("w16c2"), TILER_ROW_FORM("w16c4"),
+#undef TILER_ROW_FORM
+#define TILER_GRAD_FORM(FORM)                                                  \
+  {"tiler_layer_norm_grad_bf16_" FORM, "layer-norm-backward/bf16", 9},          \
+      {"tiler_layer_norm_grad_f32_" FORM, "layer-norm-backward-f32", 9},        \
+      {"tiler_layer_norm_grad_bf16_" FORM "r", "layer-norm-backward/bf16", 9},  \
+      {"tiler_layer_norm_grad_f32_" FORM "r", "layer-norm-backward-f32", 9}
+    TILER_GRAD_FORM("w1c1"), TILER_GRAD_FORM("w2c1"), TILER_GRAD_FORM("w4c1"), TILER_GRAD_FORM("w8c1"),
+    TILER_GRAD_FORM("w16c1"), TILER_GRAD_FORM("w16c2"),
+#undef TILER_GRAD_FORM
     {"tiler_contract_i8_bf16_g", "tensor-contraction-i8/bf16", 5},
     {"tiler_contract_i8_f32_g", "tensor-contraction-i8/f32", 5},
 #define TILER_STAGED_ROWS(TILE)                                                            \
