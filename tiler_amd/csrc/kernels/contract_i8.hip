@@ -178,13 +178,14 @@ __device__ __forceinline__ void contract_i8_guarded(const int8_t* __restrict__ a
                                                     uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * 256u * kSlice];
   const uint32_t m0 = blockIdx.y * 128u, n0 = blockIdx.x * 128u;
-  const Operand oa{reinterpret_cast<const uint8_t*>(a), k, m, k}, ob{reinterpret_cast<const uint8_t*>(b), k, n, k};
+  const tiler_product::GuardedLoader<I8, false, 128, 256> la(Operand{reinterpret_cast<const uint8_t*>(a), k, m, k}, m0);
+  const tiler_product::GuardedLoader<I8, false, 128, 256> lb(Operand{reinterpret_cast<const uint8_t*>(b), k, n, k}, n0);
   i32x4 acc[4][4];
   tiler_product::guarded_product<I8, false, false, 2, 2, 4, 4>(
-      smem, (k + 127u) / 128u,
-      [&](uint32_t t, uint32_t r, uint32_t p) { return tiler_product::operand_piece<I8, false>(oa, m0, t * 128u, r, p); },
-      [&](uint32_t t, uint32_t r, uint32_t p) { return tiler_product::operand_piece<I8, false>(ob, n0, t * 128u, r, p); },
-      acc);
+      smem, (k + 127u) / 128u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
+      [&](uint32_t t, u32x4(&v)[4]) { lb.load(lb.o.base, t, v); },
+      [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
+      [&](uint8_t* tile, const u32x4(&v)[4]) { lb.store(tile, v); }, acc);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -207,12 +208,12 @@ __device__ __forceinline__ void contract_i8_guarded(const int8_t* __restrict__ a
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256)
+extern "C" __global__ void __launch_bounds__(256, 2)
 tiler_contract_i8_bf16_g(const int8_t* __restrict__ a, const int8_t* __restrict__ b, const float* __restrict__ sa,
                          const float* __restrict__ sb, uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
   contract_i8_guarded<true>(a, b, sa, sb, m, n, k, c);
 }
-extern "C" __global__ void __launch_bounds__(256)
+extern "C" __global__ void __launch_bounds__(256, 2)
 tiler_contract_i8_f32_g(const int8_t* __restrict__ a, const int8_t* __restrict__ b, const float* __restrict__ sa,
                         const float* __restrict__ sb, uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
   contract_i8_guarded<false>(a, b, sa, sb, m, n, k, c);
@@ -289,3 +290,59 @@ TILER_CONTRACT_I8_STAGED(bf16, true, 256, 2, 4, 8)
 TILER_CONTRACT_I8_STAGED(f32, false, 256, 2, 4, 8)
 TILER_CONTRACT_I8_STAGED(bf16, true, 128, 2, 2, 4)
 TILER_CONTRACT_I8_STAGED(f32, false, 128, 2, 2, 4)
+
+// ---------------------------------------------------------------------------
+// Few rows (m <= 64): the bytes of b.  A workgroup takes 16 columns, its 8
+// waves the depth in turn.
+namespace {
+
+template <int MB, bool kBf16>
+__device__ __forceinline__ void contract_i8_few(const int8_t* __restrict__ a, const int8_t* __restrict__ b,
+                                                const float* __restrict__ sa, const float* __restrict__ sb, uint32_t m,
+                                                uint32_t n, uint32_t k, void* __restrict__ c) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[tiler_product::few_rows_lds<MB, 1, 8>()];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16u;
+  const tiler_product::RowLoader<I8, 2 * MB> la(reinterpret_cast<const uint8_t*>(a), k, m, k, 0, 0, lane);
+  const tiler_product::RowLoader<I8, 2> lb(reinterpret_cast<const uint8_t*>(b + (uint64_t)n0 * k), k,
+                                           n - n0 < 16u ? n - n0 : 16u, k, 0, 0, lane);
+  tiler_product::few_rows_product<I8, MB, 1, 8>(
+      smem, (k + 127u) / 128u,
+      [&](uint32_t t, uint8_t* slot) {
+        lb.issue(t, slot + MB * 16u * kSlice);
+        la.issue(t, slot);
+      },
+      [&](auto total) {
+        if (wave >= (uint32_t)MB) return;
+        const i32x4 v = total(wave);
+        const uint32_t col = n0 + (lane & 15u);
+        if (col >= n) return;
+        const float cs = sb[col];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t row = wave * 16u + (lane >> 4) * 4u + r;
+          if (row >= m) continue;
+          const float f = scaled(v[r], sa[row], cs);
+          const uint64_t at = (uint64_t)row * n + col;
+          if constexpr (kBf16) static_cast<uint16_t*>(c)[at] = (uint16_t)tiler::bf16_narrow(f);
+          else static_cast<float*>(c)[at] = f;
+        }
+      });
+}
+
+}  // namespace
+
+#define TILER_CONTRACT_I8_FEW(TY, BF16, MB)                                                                        \
+  extern "C" __global__ void __launch_bounds__(512)                                                                \
+      tiler_contract_i8_##TY##_few##MB(const int8_t* __restrict__ a, const int8_t* __restrict__ b,                 \
+                                       const float* __restrict__ sa, const float* __restrict__ sb, uint32_t m,     \
+                                       uint32_t n, uint32_t k, void* __restrict__ c) {                             \
+    contract_i8_few<MB, BF16>(a, b, sa, sb, m, n, k, c);                                                           \
+  }
+TILER_CONTRACT_I8_FEW(bf16, true, 1)
+TILER_CONTRACT_I8_FEW(bf16, true, 2)
+TILER_CONTRACT_I8_FEW(bf16, true, 3)
+TILER_CONTRACT_I8_FEW(bf16, true, 4)
+TILER_CONTRACT_I8_FEW(f32, false, 1)
+TILER_CONTRACT_I8_FEW(f32, false, 2)
+TILER_CONTRACT_I8_FEW(f32, false, 3)
+TILER_CONTRACT_I8_FEW(f32, false, 4)

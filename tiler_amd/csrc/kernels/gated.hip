@@ -39,23 +39,30 @@ constexpr uint32_t kGuardedBytes = 2u * 256u * kSlice;
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256)
+extern "C" __global__ void __launch_bounds__(256, 2)
 tiler_gated_bf16_g(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu,
                    uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
                    uint16_t* __restrict__ up) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
   const uint32_t m0 = blockIdx.y * 128u, n0 = blockIdx.x * 64u;
-  const Operand a{reinterpret_cast<const uint8_t*>(x), k, m, k};
-  // (a distance, not a choice of two captured pointers, which the compiler keeps in memory)
-  const int64_t between = reinterpret_cast<const uint8_t*>(wu) - reinterpret_cast<const uint8_t*>(wg);
+  // thread t's pieces of B are rows t / 8 + 32 q of its tile: gate rows for even q, up rows for odd
+  const tiler_product::GuardedLoader<Bf16, false, 128, 256> la(Operand{reinterpret_cast<const uint8_t*>(x), k, m, k}, m0);
+  const tiler_product::GuardedLoader<Bf16, false, 64, 256> lb(Operand{reinterpret_cast<const uint8_t*>(wg), k, n, k}, n0);
   f32x4 acc[kMB][kNB];
   tiler_product::guarded_product<Bf16, false, false, kW, kW, kMB, kNB>(
-      smem, (k + 63u) / 64u,
-      [=](uint32_t t, uint32_t r, uint32_t c) { return tiler_product::operand_piece<Bf16, false>(a, m0, t * 64u, r, c); },
-      [=](uint32_t t, uint32_t r, uint32_t c) {
-        const uint32_t col = (r >> 6) * 32u + (r & 31u);
-        const Operand b{reinterpret_cast<const uint8_t*>(wg) + ((r & 32u) ? between : 0), k, n, k};
-        return tiler_product::operand_piece<Bf16, false>(b, n0, t * 64u, col, c);
+      smem, (k + 63u) / 64u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
+      [&](uint32_t t, u32x4(&v)[4]) {
+        u32x4 g[2], u[2];
+        lb.load(reinterpret_cast<const uint8_t*>(wg), t, g);
+        lb.load(reinterpret_cast<const uint8_t*>(wu), t, u);
+        v[0] = g[0], v[1] = u[0], v[2] = g[1], v[3] = u[1];
+      },
+      [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
+      [&](uint8_t* tile, const u32x4(&v)[4]) {
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q)
+          *reinterpret_cast<u32x4*>(tile + tiler_product::piece_offset<128, false>(threadIdx.x / 8u + 32u * q,
+                                                                                  threadIdx.x % 8u)) = v[q];
       },
       acc);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -120,68 +127,108 @@ tiler_gated_bf16_grad(const uint16_t* __restrict__ gate, const uint16_t* __restr
   }
 }
 
-// dx [m, k] = dG Wg + dU Wu: depth n twice (dG with Wg, then dU with Wu), the
-// weights in column layout.  Guarded: 128 x 128 tiles, any sizes.
-extern "C" __global__ void __launch_bounds__(256)
-tiler_gated_bf16_dx_g(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,
-                      const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m, uint32_t n,
-                      uint32_t k, uint16_t* __restrict__ dx) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
-  const uint32_t m0 = blockIdx.y * 128u, c0 = blockIdx.x * 128u, per = (n + 63u) / 64u;
-  f32x4 acc[kMB][kNB];
-  tiler_product::guarded_product<Bf16, false, true, kW, kW, kMB, kNB>(
-      smem, 2u * per,
-      [=](uint32_t t, uint32_t r, uint32_t c) {
-        const Operand a{reinterpret_cast<const uint8_t*>(t < per ? dg : du), ld, m, n};
-        return tiler_product::operand_piece<Bf16, false>(a, m0, (t < per ? t : t - per) * 64u, r, c);
-      },
-      [=](uint32_t t, uint32_t r, uint32_t c) {
-        const Operand b{reinterpret_cast<const uint8_t*>(t < per ? wg : wu), k, k, n};
-        return tiler_product::operand_piece<Bf16, true>(b, c0, (t < per ? t : t - per) * 64u, r, c);
-      },
-      acc);
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+// Where the depth of dx is split over `splits` workgroups a tile (blockIdx.y):
+// this one's slices of the 2 per in all.
+__device__ __forceinline__ void split_range(uint32_t slices, uint32_t splits, uint32_t s, uint32_t& t0, uint32_t& t1) {
+  t0 = (uint32_t)((uint64_t)slices * s / splits);
+  t1 = (uint32_t)((uint64_t)slices * (s + 1u) / splits);
+}
+
+// A wave's blocks as binary32 partials of the m x n result.
+template <int MB, int NB>
+__device__ __forceinline__ void store_partial(const f32x4 (&acc)[MB][NB], float* out, uint32_t m, uint32_t n, uint32_t row0,
+                                              uint32_t col0) {
+  const uint32_t lane = threadIdx.x & 63u;
 #pragma unroll
-  for (int i = 0; i < kMB; ++i)
+  for (int i = 0; i < MB; ++i)
 #pragma unroll
-    for (int j = 0; j < kNB; ++j)
+    for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t row = m0 + (wave / kW) * 64u + i * 16u + (lane >> 4) * 4u + r;
-        const uint32_t col = c0 + (wave % kW) * 64u + j * 16u + (lane & 15u);
-        if (row < m && col < k) dx[(uint64_t)row * k + col] = (uint16_t)tiler::bf16_narrow(acc[i][j][r]);
+        const uint32_t row = row0 + i * 16u + (lane >> 4) * 4u + r, col = col0 + j * 16u + (lane & 15u);
+        if (row < m && col < n) out[(uint64_t)row * n + col] = acc[i][j][r];
       }
 }
 
-// dWg [n, k] = dG^T x and dWu = dU^T x (blockIdx.z): depth m, both operands in
-// column layout.  Guarded: 128 x 128 tiles, any sizes.  tiles_n row tiles each.
+// dx [m, k] = dG Wg + dU Wu: depth n twice (dG with Wg, then dU with Wu), the
+// weights in column layout.  Guarded: 128 x 128 tiles, any sizes.  With splits
+// > 1 each split's sums go to partials[split], binary32 [m, k].
+extern "C" __global__ void __launch_bounds__(256, 2)
+tiler_gated_bf16_dx_g(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,
+                      const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m, uint32_t n,
+                      uint32_t k, uint16_t* __restrict__ dx, uint32_t splits, float* __restrict__ partials) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
+  const uint32_t tiles_k = (k + 127u) / 128u;
+  const uint32_t m0 = blockIdx.x / tiles_k * 128u, c0 = blockIdx.x % tiles_k * 128u, per = ld / 64u;
+  uint32_t t0, t1;
+  split_range(2u * per, splits, blockIdx.y, t0, t1);
+  f32x4 acc[kMB][kNB];
+  if (n == 0) {
+#pragma unroll
+    for (int i = 0; i < kMB; ++i)
+#pragma unroll
+      for (int j = 0; j < kNB; ++j) acc[i][j] = Bf16::zero();
+  } else {
+    // dG's rows hold zeros from n to ld
+    const tiler_product::GuardedLoader<Bf16, false, 128, 256> la(
+        Operand{reinterpret_cast<const uint8_t*>(dg), ld, m, ld}, m0);
+    const tiler_product::GuardedLoader<Bf16, true, 128, 256> lb(Operand{reinterpret_cast<const uint8_t*>(wg), k, k, n},
+                                                                c0);
+    tiler_product::guarded_product<Bf16, false, true, kW, kW, kMB, kNB>(
+        smem, t1 - t0,
+        [&](uint32_t t, u32x4(&v)[4]) {
+          const bool first = t + t0 < per;
+          la.load(reinterpret_cast<const uint8_t*>(first ? dg : du), first ? t + t0 : t + t0 - per, v);
+        },
+        [&](uint32_t t, u32x4(&v)[4]) {
+          const bool first = t + t0 < per;
+          lb.load(reinterpret_cast<const uint8_t*>(first ? wg : wu), first ? t + t0 : t + t0 - per, v);
+        },
+        [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
+        [&](uint8_t* tile, const u32x4(&v)[4]) { lb.store(tile, v); }, acc);
+  }
+  const uint32_t wave = threadIdx.x >> 6, row0 = m0 + (wave / kW) * 64u, col0 = c0 + (wave % kW) * 64u;
+  if (splits > 1) {
+    store_partial(acc, partials + (uint64_t)blockIdx.y * m * k, m, k, row0, col0);
+    return;
+  }
+  tiler_product::store_tile_bf16<128, 128, 256, kMB, kNB>(smem, (wave / kW) * 64u, (wave % kW) * 64u, dx, m, k, m0, c0,
+                                                          [&](int i, int j, int r) { return acc[i][j][r]; });
+}
+
+// dx from its splits' partials, in ascending order.
 extern "C" __global__ void __launch_bounds__(256)
+tiler_gated_bf16_dx_sum(const float* __restrict__ partials, uint32_t splits, uint64_t count, uint16_t* __restrict__ dx) {
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < count; i += gridDim.x * 256ull) {
+    float s = partials[i];
+#pragma unroll 4
+    for (uint32_t p = 1; p < splits; ++p) s += partials[p * count + i];
+    dx[i] = (uint16_t)tiler::bf16_narrow(s);
+  }
+}
+
+// dWg [n, k] = dG^T x and dWu = dU^T x: depth m, both operands in column
+// layout.  Guarded: 128 x 128 tiles, any sizes; tiles_n row tiles of each.
+extern "C" __global__ void __launch_bounds__(256, 2)
 tiler_gated_bf16_dw_g(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,
                       const uint16_t* __restrict__ x, uint32_t m, uint32_t n, uint32_t k, uint32_t tiles_n,
                       uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
   const bool second = blockIdx.y >= tiles_n;
   const uint32_t j0 = (second ? blockIdx.y - tiles_n : blockIdx.y) * 128u, c0 = blockIdx.x * 128u;
-  const Operand a{reinterpret_cast<const uint8_t*>(second ? du : dg), ld, n, m};
-  const Operand b{reinterpret_cast<const uint8_t*>(x), k, k, m};
+  const tiler_product::GuardedLoader<Bf16, true, 128, 256> la(
+      Operand{reinterpret_cast<const uint8_t*>(second ? du : dg), ld, n, m}, j0);
+  const tiler_product::GuardedLoader<Bf16, true, 128, 256> lb(Operand{reinterpret_cast<const uint8_t*>(x), k, k, m}, c0);
   f32x4 acc[kMB][kNB];
   tiler_product::guarded_product<Bf16, true, true, kW, kW, kMB, kNB>(
-      smem, (m + 63u) / 64u,
-      [=](uint32_t t, uint32_t r, uint32_t c) { return tiler_product::operand_piece<Bf16, true>(a, j0, t * 64u, r, c); },
-      [=](uint32_t t, uint32_t r, uint32_t c) { return tiler_product::operand_piece<Bf16, true>(b, c0, t * 64u, r, c); },
-      acc);
-  uint16_t* out = second ? dwu : dwg;
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < kMB; ++i)
-#pragma unroll
-    for (int j = 0; j < kNB; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t row = j0 + (wave / kW) * 64u + i * 16u + (lane >> 4) * 4u + r;
-        const uint32_t col = c0 + (wave % kW) * 64u + j * 16u + (lane & 15u);
-        if (row < n && col < k) out[(uint64_t)row * k + col] = (uint16_t)tiler::bf16_narrow(acc[i][j][r]);
-      }
+      smem, (m + 63u) / 64u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
+      [&](uint32_t t, u32x4(&v)[4]) { lb.load(lb.o.base, t, v); },
+      [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
+      [&](uint8_t* tile, const u32x4(&v)[4]) { lb.store(tile, v); }, acc);
+  const uint32_t wave = threadIdx.x >> 6;
+  tiler_product::store_tile_bf16<128, 128, 256, kMB, kNB>(smem, (wave / kW) * 64u, (wave % kW) * 64u,
+                                                          second ? dwu : dwg, n, k, j0, c0,
+                                                          [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 
 // ---------------------------------------------------------------------------
@@ -229,36 +276,43 @@ template <int WM, int WN, int MB>
 __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du,
                                                 uint32_t ld, const uint16_t* __restrict__ wg,
                                                 const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
-                                                uint16_t* __restrict__ dx) {
+                                                uint16_t* __restrict__ dx, uint32_t splits,
+                                                float* __restrict__ partials) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kCols = WN * 64u, kThreads = 64u * WM * WN;
   constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kCols / 8 / (WM * WN);
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kCols) * kSlice];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t tm, tn;
+  uint32_t tm, tn, t0, t1;
   tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (k + kCols - 1u) / kCols, tm, tn);
   const uint32_t m0 = tm * kRowsA, c0 = tn * kCols, per = ld / 64u;
+  split_range(2u * per, splits, blockIdx.y, t0, t1);
   // dG's rows hold zeros from n to ld, the weights' depth rows load as zeros there
-  tiler_product::RowLoader<Bf16, kLoadsA> la(reinterpret_cast<const uint8_t*>(dg + (uint64_t)m0 * ld), ld,
-                                             m - m0 < kRowsA ? m - m0 : kRowsA, ld, wave * kLoadsA * 8u,
-                                             wave * kLoadsA * 8u, lane);
-  tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(wg + c0), k, c0, n, wave, lane);
-  const int64_t next_a = reinterpret_cast<const uint8_t*>(du) - reinterpret_cast<const uint8_t*>(dg);
-  const int64_t next_b = reinterpret_cast<const uint8_t*>(wu) - reinterpret_cast<const uint8_t*>(wg);
+  const tiler_product::RowLoader<Bf16, kLoadsA> la(reinterpret_cast<const uint8_t*>(dg + (uint64_t)m0 * ld), ld,
+                                                   m - m0 < kRowsA ? m - m0 : kRowsA, ld, wave * kLoadsA * 8u,
+                                                   wave * kLoadsA * 8u, lane);
+  const tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(wg + c0), k, c0, n, wave, lane);
+  const uint8_t* const a2 = reinterpret_cast<const uint8_t*>(du + (uint64_t)m0 * ld);
+  const uint8_t* const b2 = reinterpret_cast<const uint8_t*>(wu + c0);
   f32x4 acc[MB][4];
   tiler_product::staged_product<Bf16, false, true, WM, WN, MB, 4, kLoadsA + kLoadsB>(
-      smem, 2u * per,
+      smem, t1 - t0,
       [&](uint32_t t, uint8_t* at) {
-        if (t == per) la.base += next_a;
-        la.issue(t < per ? t : t - per, at);
+        const bool first = t + t0 < per;
+        la.issue(first ? la.base : a2, first ? t + t0 : t + t0 - per, at);
       },
       [&](uint32_t t, uint8_t* at) {
-        if (t == per) lb.base += next_b;
-        lb.issue(t < per ? t : t - per, at);
+        const bool first = t + t0 < per;
+        lb.issue(first ? lb.base : b2, first ? t + t0 : t + t0 - per, at);
       },
       acc);
+  const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 64u;
+  if (splits > 1) {
+    store_partial(acc, partials + (uint64_t)blockIdx.y * m * k, m, k, m0 + row0, c0 + col0);
+    return;
+  }
   __syncthreads();
-  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(
-      smem, (wave / WN) * MB * 16u, (wave % WN) * 64u, dx, m, k, m0, c0, [&](int i, int j, int r) { return acc[i][j][r]; });
+  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(smem, row0, col0, dx, m, k, m0, c0,
+                                                                 [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 
 template <int WM, int WN, int MB>
@@ -299,8 +353,9 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
   extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
       tiler_gated_bf16_dx_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
                                   const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m,     \
-                                  uint32_t n, uint32_t k, uint16_t* __restrict__ dx) {                              \
-    gated_dx_staged<WM, WN, MB>(dg, du, ld, wg, wu, m, n, k, dx);                                                   \
+                                  uint32_t n, uint32_t k, uint16_t* __restrict__ dx, uint32_t splits,               \
+                                  float* __restrict__ partials) {                                                   \
+    gated_dx_staged<WM, WN, MB>(dg, du, ld, wg, wu, m, n, k, dx, splits, partials);                                 \
   }                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
       tiler_gated_bf16_dw_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
@@ -310,3 +365,58 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
   }
 TILER_GATED_STAGED(256, 2, 4, 8)
 TILER_GATED_STAGED(128, 2, 2, 4)
+
+// ---------------------------------------------------------------------------
+// Few tokens (m <= 64): the weights' bytes.  A workgroup takes 16 columns of
+// both projections, its 8 waves the depth in turn.
+namespace {
+
+template <int MB>
+__device__ __forceinline__ void gated_few(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
+                                          const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
+                                          uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
+                                          uint16_t* __restrict__ up) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[tiler_product::few_rows_lds<MB, 2, 8>()];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16u;
+  const uint32_t cols = n - n0 < 16u ? n - n0 : 16u;
+  const tiler_product::RowLoader<Bf16, 2 * MB> la(reinterpret_cast<const uint8_t*>(x), k, m, k, 0, 0, lane);
+  const tiler_product::RowLoader<Bf16, 2> lg(reinterpret_cast<const uint8_t*>(wg + (uint64_t)n0 * k), k, cols, k, 0, 0, lane);
+  const uint8_t* const u0 = reinterpret_cast<const uint8_t*>(wu + (uint64_t)n0 * k);
+  tiler_product::few_rows_product<Bf16, MB, 2, 8>(
+      smem, (k + 63u) / 64u,
+      [&](uint32_t t, uint8_t* slot) {
+        lg.issue(t, slot + MB * 16u * kSlice);
+        lg.issue(u0, t, slot + (MB + 1) * 16u * kSlice);
+        la.issue(t, slot);
+      },
+      [&](auto total) {
+        if (wave >= (uint32_t)MB) return;
+        const f32x4 g = total(2u * wave), u = total(2u * wave + 1u);
+        const uint32_t col = n0 + (lane & 15u);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t row = wave * 16u + (lane >> 4) * 4u + r;
+          if (row >= m || col >= n) continue;
+          const uint64_t at = (uint64_t)row * n + col;
+          h[at] = (uint16_t)tiler::bf16_narrow(g[r] * sigmoid(g[r]) * u[r]);
+          if (gate) {
+            gate[at] = (uint16_t)tiler::bf16_narrow(g[r]);
+            up[at] = (uint16_t)tiler::bf16_narrow(u[r]);
+          }
+        }
+      });
+}
+
+}  // namespace
+
+#define TILER_GATED_FEW(MB)                                                                                        \
+  extern "C" __global__ void __launch_bounds__(512)                                                                \
+      tiler_gated_bf16_few##MB(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,                    \
+                               const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,                \
+                               uint16_t* __restrict__ h, uint16_t* __restrict__ gate, uint16_t* __restrict__ up) { \
+    gated_few<MB>(x, wg, wu, m, n, k, h, gate, up);                                                                \
+  }
+TILER_GATED_FEW(1)
+TILER_GATED_FEW(2)
+TILER_GATED_FEW(3)
+TILER_GATED_FEW(4)

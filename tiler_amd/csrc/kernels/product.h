@@ -118,16 +118,69 @@ __device__ __forceinline__ u32x4 operand_piece(const Operand& o, uint32_t row0, 
 }
 
 // The guarded product, for any sizes and alignments: pieces come through
-// registers (zero outside the operand), one slice ahead of the products.
-// WM x WN waves of MB x NB blocks of 16 x 16; piece_a(t, outer, inner) and
-// piece_b fetch a piece of slice t.
-template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, typename FA, typename FB>
-__device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, FA piece_a, FB piece_b,
-                                                typename E::Acc (&acc)[MB][NB]) {
+// registers, two slices ahead of the products.  A loader's pieces of a slice
+// lie at fixed offsets from a base that moves along the depth; only the last
+// slice of an operand is checked piece by piece (zero past the depth).  In the
+// others a row past the last reads the last one, and a column piece past the
+// row's end reads on into the next depth row: both only reach results that are
+// not stored.  (The reading on needs rows of at least a piece; narrower ones
+// are checked throughout.)
+template <typename E, bool kCol, uint32_t TILE, uint32_t THREADS>
+struct GuardedLoader {
+  static constexpr uint32_t kLoads = TILE * 8u / THREADS, kOuter = kCol ? TILE / 8u : 8u, kPer = 16u / E::kBytes;
+  static constexpr uint32_t kDepth = kCol ? 64u : kSlice / E::kBytes;  // depth elements per slice
+  static_assert(TILE * 8u % THREADS == 0, "whole pieces per thread");
+  Operand o;
+  uint32_t row0;
+  uint32_t voff[kLoads];
+  __device__ __forceinline__ GuardedLoader(const Operand& o_, uint32_t row0_) : o(o_), row0(row0_) {
+#pragma unroll
+    for (uint32_t q = 0; q < kLoads; ++q) {
+      const uint32_t id = threadIdx.x + q * THREADS, outer = id / kOuter, inner = id % kOuter;
+      if constexpr (kCol) {
+        const uint32_t last = (o.rows - 1u - row0) / kPer;
+        voff[q] = outer * (uint32_t)(o.ld * E::kBytes) + (inner < last ? inner : last) * 16u;
+      } else {
+        const uint32_t last = o.rows - 1u - row0;
+        voff[q] = (outer < last ? outer : last) * (uint32_t)(o.ld * E::kBytes) + inner * 16u;
+      }
+    }
+  }
+  // `base`: the operand's storage (one of two, in the products over two segments of depth).
+  __device__ __forceinline__ void load(const uint8_t* base, uint32_t t, u32x4 (&v)[kLoads]) const {
+    const bool whole = kCol ? (t + 1u) * kDepth < o.depth && o.ld >= kPer : (t + 1u) * kDepth <= o.depth;
+    if (whole) {
+      const uint8_t* at = base + (kCol ? t * 64u * o.ld * E::kBytes + row0 * (uint64_t)E::kBytes
+                                       : row0 * o.ld * E::kBytes + (uint64_t)t * kSlice);
+#pragma unroll
+      for (uint32_t q = 0; q < kLoads; ++q) v[q] = *reinterpret_cast<const u32x4_any*>(at + voff[q]);
+    } else {
+      const Operand here{base, o.ld, o.rows, o.depth};
+#pragma unroll
+      for (uint32_t q = 0; q < kLoads; ++q) {
+        const uint32_t id = threadIdx.x + q * THREADS;
+        v[q] = operand_piece<E, kCol>(here, row0, t * kDepth, id / kOuter, id % kOuter);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* tile, const u32x4 (&v)[kLoads]) const {
+#pragma unroll
+    for (uint32_t q = 0; q < kLoads; ++q) {
+      const uint32_t id = threadIdx.x + q * THREADS;
+      *reinterpret_cast<u32x4*>(tile + piece_offset<TILE, kCol>(id / kOuter, id % kOuter)) = v[q];
+    }
+  }
+};
+
+// load_a(t, pieces) and load_b fetch a slice, store_a(tile, pieces) and store_b
+// put it into LDS; WM x WN waves of MB x NB blocks of 16 x 16.
+template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, typename LA, typename LB, typename SA,
+          typename SB>
+__device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, LA load_a, LB load_b, SA store_a,
+                                                SB store_b, typename E::Acc (&acc)[MB][NB]) {
   constexpr uint32_t kThreads = 64u * WM * WN, kRowsA = WM * MB * 16u, kRowsB = WN * NB * 16u;
   constexpr uint32_t kLoadsA = kRowsA * 8u / kThreads, kLoadsB = kRowsB * 8u / kThreads;
   constexpr uint32_t kStage = (kRowsA + kRowsB) * kSlice;
-  static_assert(kRowsA * 8u % kThreads == 0 && kRowsB * 8u % kThreads == 0, "whole pieces per thread");
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const Fragments<kRowsA, kACol, MB> ra((wave / WN) * MB * 16u, lane);
   const Fragments<kRowsB, kBCol, NB> rb((wave % WN) * NB * 16u, lane);
@@ -135,38 +188,21 @@ __device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, 
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = E::zero();
-  u32x4 pa[kLoadsA], pb[kLoadsB];
-  constexpr uint32_t kOuterA = Pieces<kRowsA, kACol>::kPerOuter, kOuterB = Pieces<kRowsB, kBCol>::kPerOuter;
-  auto load = [&](uint32_t t) {
-#pragma unroll
-    for (uint32_t q = 0; q < kLoadsA; ++q) {
-      const uint32_t id = threadIdx.x + q * kThreads;
-      pa[q] = piece_a(t, id / kOuterA, id % kOuterA);
-    }
-#pragma unroll
-    for (uint32_t q = 0; q < kLoadsB; ++q) {
-      const uint32_t id = threadIdx.x + q * kThreads;
-      pb[q] = piece_b(t, id / kOuterB, id % kOuterB);
-    }
+  if (slices == 0) return;
+  u32x4 pa[2][kLoadsA], pb[2][kLoadsB];
+  auto load = [&](uint32_t t, auto slot) {
+    load_a(t, pa[decltype(slot)::value]);
+    load_b(t, pb[decltype(slot)::value]);
   };
-  auto store = [&](uint32_t stage) {
-    uint8_t* at = smem + stage * kStage;
-#pragma unroll
-    for (uint32_t q = 0; q < kLoadsA; ++q) {
-      const uint32_t id = threadIdx.x + q * kThreads;
-      *reinterpret_cast<u32x4*>(at + piece_offset<kRowsA, kACol>(id / kOuterA, id % kOuterA)) = pa[q];
-    }
-#pragma unroll
-    for (uint32_t q = 0; q < kLoadsB; ++q) {
-      const uint32_t id = threadIdx.x + q * kThreads;
-      *reinterpret_cast<u32x4*>(at + kRowsA * kSlice + piece_offset<kRowsB, kBCol>(id / kOuterB, id % kOuterB)) = pb[q];
-    }
+  auto store = [&](uint32_t t, auto slot) {
+    uint8_t* at = smem + (t & 1u) * kStage;
+    store_a(at, pa[decltype(slot)::value]);
+    store_b(at + kRowsA * kSlice, pb[decltype(slot)::value]);
   };
-  load(0);
-  store(0);
-  __syncthreads();
-  for (uint32_t t = 0; t < slices; ++t) {
-    if (t + 1 < slices) load(t + 1);
+  // slice t in LDS, slice t + 1 in registers (slot (t + 1) % 2): requests slice
+  // t + 2, multiplies slice t, puts slice t + 1 into LDS
+  auto turn = [&](uint32_t t, auto next, auto after) {
+    if (t + 2 < slices) load(t + 2, after);
     const uint8_t* at = smem + (t & 1u) * kStage;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -178,8 +214,18 @@ __device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, 
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(fa[i], fb[j], acc[i][j]);
     }
-    if (t + 1 < slices) store((t & 1u) ^ 1u);
+    if (t + 1 < slices) store(t + 1, next);
     __syncthreads();
+  };
+  constexpr tiler::Step<0> even{};
+  constexpr tiler::Step<1> odd{};
+  load(0, even);
+  if (slices > 1) load(1, odd);
+  store(0, even);
+  __syncthreads();
+  for (uint32_t t = 0; t < slices; t += 2) {
+    turn(t, odd, even);
+    if (t + 1 < slices) turn(t + 1, even, odd);
   }
 }
 
@@ -220,9 +266,10 @@ struct RowLoader {
       voff[j] = (wave_rows + j * 8u + (lane >> 3)) * (uint32_t)(ld * E::kBytes) + in * 16u;
     }
   }
-  __device__ __forceinline__ void issue(uint32_t t, uint8_t* tile) const {
+  __device__ __forceinline__ void issue(uint32_t t, uint8_t* tile) const { issue(base, t, tile); }
+  __device__ __forceinline__ void issue(const uint8_t* from, uint32_t t, uint8_t* tile) const {
     const uint32_t at = t * kSlice, left = depth_bytes - at;
-    const __amdgpu_buffer_rsrc_t panel = resource(base + at, span - at);
+    const __amdgpu_buffer_rsrc_t panel = resource(from + at, span - at);
     if (left >= kSlice) {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j)
@@ -256,10 +303,11 @@ struct ColumnLoader {
       voff[j] = outer * (uint32_t)row_bytes + block * 32u + (slot & 1u) * 16u;
     }
   }
-  __device__ __forceinline__ void issue(uint32_t t, uint8_t* tile) const {
+  __device__ __forceinline__ void issue(uint32_t t, uint8_t* tile) const { issue(base, t, tile); }
+  __device__ __forceinline__ void issue(const uint8_t* from, uint32_t t, uint8_t* tile) const {
     const uint32_t left = depth - t * 64u, rows = left < 64u ? left : 64u;
     const __amdgpu_buffer_rsrc_t panel =
-        resource(base + t * 64u * row_bytes, rows * (uint32_t)row_bytes - before_bytes);
+        resource(from + t * 64u * row_bytes, rows * (uint32_t)row_bytes - before_bytes);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (lds_bytes*)(tile + lds0 + j * 1024u), 16, voff[j], 0, 0, 0);
@@ -332,6 +380,68 @@ __device__ __forceinline__ void staged_product(uint8_t* smem, uint32_t slices, I
   read(slices - 1, 1);
   products(0);
   products(1);
+}
+
+// The product for few rows: a workgroup of W waves owns MB x NB blocks of
+// 16 x 16 results, and wave w the depth slices w, w + W, ...: it moves a slice's
+// rows into a slot of its own (issue(t, slot)), reads its fragments, requests
+// its next slice into the same slot and multiplies while that lands.  No barrier
+// until the end, so nearly W slots a workgroup stay in flight; then every wave
+// leaves its partial tile in LDS, and finish(total) takes the blocks' sums:
+// total(q) is block q's (row block q / NB, column block q % NB), the waves'
+// parts added in ascending order.
+template <typename E, int MB, int NB, int W, typename I, typename F>
+__device__ __forceinline__ void few_rows_product(uint8_t* smem, uint32_t slices, I issue, F finish) {
+  constexpr uint32_t kSlot = (MB + NB) * 16u * kSlice;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Fragments<MB * 16u, false, MB> ra(0, lane);
+  const Fragments<NB * 16u, false, NB> rb(0, lane);
+  typename E::Acc acc[MB][NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = E::zero();
+  uint8_t* const slot = smem + wave * kSlot;
+  if (wave < slices) issue(wave, slot);
+  for (uint32_t t = wave; t < slices; t += W) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    u32x4 fa[2][MB], fb[2][NB];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      ra.read(slot, s, fa[s]);
+      rb.read(slot + MB * 16u * kSlice, s, fb[s]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + W < slices) issue(t + W, slot);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(fa[s][i], fb[s][j], acc[i][j]);
+  }
+  __syncthreads();
+  typename E::Acc* const part = reinterpret_cast<typename E::Acc*>(smem);
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) part[(wave * MB * NB + i * NB + j) * 64u + lane] = acc[i][j];
+  __syncthreads();
+  auto total = [&](uint32_t q) {
+    typename E::Acc v = part[q * 64u + lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const typename E::Acc o = part[(w * MB * NB + q) * 64u + lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += o[r];
+    }
+    return v;
+  };
+  finish(total);
+}
+template <int MB, int NB, int W>
+constexpr uint32_t few_rows_lds() {
+  return W * (MB + NB) * 16u * kSlice > W * MB * NB * 1024u ? W * (MB + NB) * 16u * kSlice : W * MB * NB * 1024u;
 }
 
 // Tile `id` of a tiles_m x tiles_n grid.  Workgroups go round robin over the

@@ -166,8 +166,9 @@ namespace {
 
 tiler_hip_status check_product(uint64_t m, uint64_t n, uint64_t k, Program& p) {
   if (k == 0) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "empty contracted extent");
-  if (m > 0x7fffff00ull || n > 0x7fffff00ull || k > 0x7fffff00ull || ceil_div(m, 128) > 65535 ||
-      !grid_holds(ceil_div(n, 64), 256) || !grid_holds(ceil_div(k, 64), 256))
+  // a tile's rows lie within 32-bit offsets of its first: k below 2^24 elements
+  if (m > 0x7fffff00ull || n > 0x7fffff00ull || k >= (1ull << 24) || ceil_div(m, 128) > 65535 ||
+      !grid_holds(ceil_div(n, 64), 256))
     return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
   return TILER_HIP_OK;
 }
@@ -201,7 +202,16 @@ tiler_hip_status plan_gated_contract_bf16(const Target& t, uint32_t parts, uint6
   const uint32_t gate = keep ? p.slot(out, kSlotOutput) : 0, up = keep ? p.slot(out, kSlotOutput) : 0;
   if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
   if (m == 0 || n == 0) return TILER_HIP_OK;
-  if (staged_rows(2 * k) && aligned16(addr[x]) && aligned16(addr[wg]) && aligned16(addr[wu])) {
+  const bool al = staged_rows(2 * k) && aligned16(addr[x]) && aligned16(addr[wg]) && aligned16(addr[wu]);
+  if (al && m <= 64 && grid_holds(ceil_div(n, 16), 512)) {
+    const std::string name = "tiler_gated_bf16_few" + std::to_string(ceil_div(m, 16));
+    Launch& l = p.add(name.c_str(), (uint32_t)ceil_div(n, 16), 1, 512)
+                    .ptr(x).ptr(wg).ptr(wu).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(h);
+    slot_or_null(l, keep, gate);
+    slot_or_null(l, keep, up);
+    return TILER_HIP_OK;
+  }
+  if (al) {
     const uint32_t tile = staged_tile(t, m, 128, n);
     const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(n, tile / 2));
     if (grid_holds(tiles, 512)) {
@@ -232,7 +242,7 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
   const uint32_t dx = has_dx ? p.slot(in, kSlotOutput) : 0;
   const uint32_t dwg = has_dw ? p.slot(weight, kSlotOutput) : 0, dwu = has_dw ? p.slot(weight, kSlotOutput) : 0;
   if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
-  if (2 * ceil_div(n, 128) > 65535) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
+  if (n >= (1ull << 22)) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
   if (!parts) return TILER_HIP_OK;
   const uint64_t ld = ceil_div(n, 64) * 64, half = mul_sat(mul_sat(m, ld), 2);
   const uint32_t dg = p.slot(half, kSlotScratch), du = p.slot(half, kSlotScratch);
@@ -245,14 +255,30 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
   // Columns of the weights and of x (k of them a row) are read in 16-byte pieces.
   const bool rows_ok = staged_rows(2 * k) && staged_rows(2 * ld);
   if (has_dx && m) {
-    const uint32_t tile = staged_tile(t, m, 256, k);
-    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(k, tile));
-    if (rows_ok && aligned16(addr[wg]) && aligned16(addr[wu]) && grid_holds(tiles, 512))
-      add_tiles(p, "tiler_gated_bf16_dx", tile, tiles)
-          .ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx);
-    else
-      p.add("tiler_gated_bf16_dx_g", (uint32_t)ceil_div(k, 128), (uint32_t)ceil_div(m, 128), 256)
-          .ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx);
+    // The depth 2 n of dx is split over as many workgroups as fill the chip
+    // twice (two 128-tiles to a CU) where the tiles alone do not: at least
+    // four slices each, the binary32 partials added by one more launch.
+    const bool staged = rows_ok && aligned16(addr[wg]) && aligned16(addr[wu]);
+    const uint32_t tile = staged ? staged_tile(t, m, 256, k) : 128;
+    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(k, tile)), slices = 2 * (ld / 64);
+    uint64_t splits = 1;
+    if (tile == 128 && tiles < 2ull * t.compute_units) {
+      splits = 2ull * t.compute_units / tiles;
+      if (splits > slices / 4) splits = slices / 4;
+      if (splits > 32) splits = 32;
+      if (splits == 0) splits = 1;
+    }
+    if (!grid_holds(tiles, 512)) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
+    const uint32_t partials = splits > 1 ? p.slot(mul_sat(mul_sat(splits, m * k), 4), kSlotScratch) : 0;
+    Launch& l = staged ? add_tiles(p, "tiler_gated_bf16_dx", tile, tiles) : p.add("tiler_gated_bf16_dx_g", (uint32_t)tiles, 1, 256);
+    l.grid[1] = (uint32_t)splits;
+    l.ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx).u32((uint32_t)splits);
+    slot_or_null(l, splits > 1, partials);
+    if (splits > 1) {
+      const uint64_t groups = ceil_div(m * k, 256);
+      p.add("tiler_gated_bf16_dx_sum", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
+          .ptr(partials).u32((uint32_t)splits).u64(m * k).ptr(dx);
+    }
   }
   if (has_dw && n) {
     const uint32_t tile = staged_tile(t, 2 * n, 256, k);
@@ -297,7 +323,14 @@ tiler_hip_status plan_contract_i8(const Target& t, uint32_t out_dtype, uint64_t 
   if (k > 131071) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "a sum of more than 131071 products could leave 32 bits");
   if (m == 0 || n == 0) return TILER_HIP_OK;
   char name[64];
-  if (staged_rows(k) && aligned16(addr[a]) && aligned16(addr[b])) {
+  const bool al = staged_rows(k) && aligned16(addr[a]) && aligned16(addr[b]);
+  if (al && m <= 64 && grid_holds(ceil_div(n, 16), 512)) {
+    std::snprintf(name, sizeof(name), "tiler_contract_i8_%s_few%u", type_name(out_dtype), (uint32_t)ceil_div(m, 16));
+    p.add(name, (uint32_t)ceil_div(n, 16), 1, 512)
+        .ptr(a).ptr(b).ptr(sa).ptr(sb).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(c);
+    return TILER_HIP_OK;
+  }
+  if (al) {
     const uint32_t tile = staged_tile(t, m, 256, n);
     const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(n, tile));
     if (grid_holds(tiles, 512)) {

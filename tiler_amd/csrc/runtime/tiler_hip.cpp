@@ -365,7 +365,7 @@ const EntryRow kEntries[] = {
     {"tiler_layer_norm_columns_final_f32", "layer-norm-backward-f32", 3},
     {"tiler_gated_bf16_g", "gated-contraction-bf16", 6},
     {"tiler_gated_bf16_grad", "gated-contraction-bf16-backward", 5},
-    {"tiler_gated_bf16_dx_g", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_dx_g", "gated-contraction-bf16-backward", 6},
     {"tiler_gated_bf16_dw_g", "gated-contraction-bf16-backward", 5},
 #define TILER_ROW_FORM(FORM)                                                   \
   {"tiler_layer_norm_bf16_" FORM, "layer-norm/bf16", 6},                        \
@@ -388,12 +388,19 @@ const EntryRow kEntries[] = {
     {"tiler_contract_i8_f32_g", "tensor-contraction-i8/f32", 5},
 #define TILER_STAGED_ROWS(TILE)                                                            \
   {"tiler_gated_bf16_t" TILE, "gated-contraction-bf16", 6},                                 \
-      {"tiler_gated_bf16_dx_t" TILE, "gated-contraction-bf16-backward", 5},                 \
+      {"tiler_gated_bf16_dx_t" TILE, "gated-contraction-bf16-backward", 6},                 \
       {"tiler_gated_bf16_dw_t" TILE, "gated-contraction-bf16-backward", 5},                 \
       {"tiler_contract_i8_bf16_t" TILE, "tensor-contraction-i8/bf16", 5},                   \
       {"tiler_contract_i8_f32_t" TILE, "tensor-contraction-i8/f32", 5}
     TILER_STAGED_ROWS("256"), TILER_STAGED_ROWS("128"),
 #undef TILER_STAGED_ROWS
+    {"tiler_gated_bf16_dx_sum", "gated-contraction-bf16-backward", 2},
+#define TILER_FEW_ROWS(MB)                                                          \
+  {"tiler_gated_bf16_few" MB, "gated-contraction-bf16", 6},                         \
+      {"tiler_contract_i8_bf16_few" MB, "tensor-contraction-i8/bf16", 5},           \
+      {"tiler_contract_i8_f32_few" MB, "tensor-contraction-i8/f32", 5}
+    TILER_FEW_ROWS("1"), TILER_FEW_ROWS("2"), TILER_FEW_ROWS("3"), TILER_FEW_ROWS("4"),
+#undef TILER_FEW_ROWS
 };
 constexpr uint32_t kEntryCount = sizeof(kEntries) / sizeof(kEntries[0]);
 
@@ -2126,12 +2133,19 @@ tiler_hip_status tiler_hip_gated_contract_bf16_backward(tiler_hip_context* ctx, 
 tiler_hip_status tiler_hip_gated_contract_bf16_backward_workspace(const tiler_hip_context* ctx, uint64_t m, uint64_t n,
                                                                   uint64_t k, uint64_t* bytes) try {
   if (!bytes) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
-  const uintptr_t addr[tiler_rt::kMaxSlots] = {};
-  tiler_rt::Program p;
-  const tiler_hip_status st = tiler_rt::plan_gated_contract_bf16_backward(
-      target_of(ctx), TILER_HIP_GATED_DX | TILER_HIP_GATED_DW, m, n, k, addr, p);
-  *bytes = st == TILER_HIP_OK ? workspace_need(p) : 0;
-  return st;
+  // the larger of what aligned and unaligned operands take
+  *bytes = 0;
+  for (const uintptr_t at : {(uintptr_t)0, (uintptr_t)2}) {
+    uintptr_t addr[tiler_rt::kMaxSlots];
+    for (uintptr_t& a : addr) a = at;
+    tiler_rt::Program p;
+    const tiler_hip_status st = tiler_rt::plan_gated_contract_bf16_backward(
+        target_of(ctx), TILER_HIP_GATED_DX | TILER_HIP_GATED_DW, m, n, k, addr, p);
+    if (st != TILER_HIP_OK) return st;
+    const uint64_t need = workspace_need(p);
+    if (need > *bytes) *bytes = need;
+  }
+  return TILER_HIP_OK;
 } catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
   return TILER_HIP_REFUSE_CAPACITY;
 }
