@@ -71,8 +71,8 @@ __device__ __forceinline__ void quantize_rows(const T* __restrict__ x, uint64_t 
   x += row * extent;
   q += row * extent;
   u32x4 v[CH];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) v[c] = load_piece<T, true>(x, (c * 64u * WAVES + t) * V, extent);
+  load_row<T, WAVES, CH, true>(x, t, extent, v);
+  settle_row<T, WAVES, CH>(t, extent, v);
   uint32_t top = 0;
 #pragma unroll
   for (int c = 0; c < CH; ++c)
@@ -108,6 +108,7 @@ __device__ __forceinline__ void quantize_rows(const T* __restrict__ x, uint64_t 
       for (int e = 0; e < V - 1; ++e)
         if ((uint32_t)e < valid) q[at + e] = (int8_t)(words[e >> 2] >> (8 * (e & 3)));
     }
+    __builtin_amdgcn_sched_barrier(0);  // one piece's temporaries at a time
   }
 }
 

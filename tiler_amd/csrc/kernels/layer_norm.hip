@@ -105,8 +105,8 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
   x += row * extent;
   y += row * extent;
   u32x4 v[CH];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) v[c] = load_piece<T, true>(x, (c * 64u * WAVES + t) * V, extent);
+  load_row<T, WAVES, CH, true>(x, t, extent, v);
+  settle_row<T, WAVES, CH>(t, extent, v);
   float s = 0.0f, none = 0.0f;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -142,24 +142,33 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
     mean[row] = mu;
     rstd[row] = r;
   }
+  // w and b a few pieces at a time: they come from the caches
+  constexpr int kBatch = CH < 4 ? CH : 4;
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const uint32_t at = (c * 64u * WAVES + t) * V;
-    if (at >= extent) continue;
-    float o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = ((element<T>(v[c], i) - mu0) - shift) * r;
+  for (int c0 = 0; c0 < CH; c0 += kBatch) {
+    const uint32_t t0 = c0 * 64u * WAVES + t;  // as pieces 0.. of a thread further on
+    u32x4 wv[kBatch], bv[kBatch];
     if (w) {
-      const u32x4 wv = load_piece<T, false>(w, at, extent);
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = o[i] * element<T>(wv, i);
+      load_row<T, WAVES, kBatch, false>(w, t0, extent, wv);
+      settle_row<T, WAVES, kBatch>(t0, extent, wv);
     }
     if (b) {
-      const u32x4 bv = load_piece<T, false>(b, at, extent);
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = o[i] + element<T>(bv, i);
+      load_row<T, WAVES, kBatch, false>(b, t0, extent, bv);
+      settle_row<T, WAVES, kBatch>(t0, extent, bv);
     }
-    store_piece<T>(y, at, extent, o);
+#pragma unroll
+    for (int c = 0; c < kBatch; ++c) {
+      const uint32_t at = (c * 64u * WAVES + t0) * V;
+      if (at >= extent) continue;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        o[i] = ((element<T>(v[c0 + c], i) - mu0) - shift) * r;
+        if (w) o[i] = o[i] * element<T>(wv[c], i);
+        if (b) o[i] = o[i] + element<T>(bv[c], i);
+      }
+      store_piece<T>(y, at, extent, o);
+    }
   }
 }
 
@@ -169,7 +178,7 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
 // in LDS, and each workgroup leaves one partial (dw's sums, then db's), or the
 // results themselves where it is the only one.  The next rows are loaded
 // before the current ones are reduced.
-template <typename T, int WAVES, int CH, bool kAhead, bool kWhole>
+template <typename T, int WAVES, int CH>
 __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, const T* __restrict__ x,
                                                      const T* __restrict__ w, const float* __restrict__ mean,
                                                      const float* __restrict__ rstd, uint64_t rows, uint32_t extent,
@@ -177,6 +186,7 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
                                                      T* __restrict__ dw, T* __restrict__ db) {
   using namespace tiler_rows;
   constexpr int V = kVec<T>;
+  constexpr bool kAhead = CH * V <= 8;  // beyond, the next rows' pieces do not fit the registers
   constexpr uint32_t kGroups = 16 / WAVES, kSpan = CH * 64u * WAVES * V;  // elements a group's pieces cover
   __shared__ float slots[2][32];
   __shared__ float columns[kGroups > 1 ? 2 * kSpan : 1];
@@ -186,26 +196,25 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
   u32x4 wv[CH], xv[CH], dv[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const uint32_t at = (c * 64u * WAVES + t) * V;
-    wv[c] = w ? load_piece<T, false, kWhole>(w, at, extent) : u32x4{0, 0, 0, 0};
+    wv[c] = u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < V; ++i) aw[c][i] = ab[c][i] = 0.0f;
+  }
+  if (w) {
+    load_row<T, WAVES, CH, false>(w, t, extent, wv);
+    settle_row<T, WAVES, CH>(t, extent, wv);
   }
   const uint64_t step = (uint64_t)gridDim.x * kGroups;
   uint64_t row = (uint64_t)blockIdx.x * kGroups + group;
   const uint64_t rounds = (rows - (uint64_t)blockIdx.x * kGroups + step - 1) / step;  // the first group's: the same for all
   float mu = 0.0f, r = 0.0f;
+  // A group past the last row reads the last one; its terms are dropped.
   auto load = [&](uint64_t at_row, u32x4(&xo)[CH], u32x4(&dyo)[CH], float& muo, float& ro) {
-    const bool real = at_row < rows;
-    muo = real ? mean[at_row] : 0.0f;
-    ro = real ? rstd[at_row] : 0.0f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const uint32_t at = (c * 64u * WAVES + t) * V;
-      // a group past the last row holds zeros: its sums and stores drop out
-      xo[c] = real ? load_piece<T, true, kWhole>(x + at_row * extent, at, extent) : u32x4{0, 0, 0, 0};
-      dyo[c] = real ? load_piece<T, true, kWhole>(dy + at_row * extent, at, extent) : u32x4{0, 0, 0, 0};
-    }
+    const uint64_t here = at_row < rows ? at_row : rows - 1u;
+    muo = mean[here];
+    ro = rstd[here];
+    load_row<T, WAVES, CH, true>(x + here * extent, t, extent, xo);
+    load_row<T, WAVES, CH, true>(dy + here * extent, t, extent, dyo);
   };
   load(row, xv, dv, mu, r);
 #pragma unroll 1
@@ -213,6 +222,13 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
     u32x4 xn[CH], dn[CH];
     float mun = 0.0f, rn = 0.0f;
     if (kAhead && k + 1 < rounds) load(row + step, xn, dn, mun, rn);
+    settle_row<T, WAVES, CH>(t, extent, xv);
+    settle_row<T, WAVES, CH>(t, extent, dv);
+    if (row >= rows) {  // whole groups, in the last round
+#pragma unroll
+      for (int c = 0; c < CH; ++c) xv[c] = dv[c] = u32x4{0, 0, 0, 0};
+      mu = r = 0.0f;
+    }
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -248,14 +264,14 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
             const float d = element<T>(dv[c], i), g = w ? d * element<T>(wv[c], i) : d;
             o[i] = r * (g - c1 - (element<T>(xv[c], i) - mu) * r * c2);
           }
-          store_piece<T, kWhole>(dx + row * extent, at, extent, o);
+          store_piece<T>(dx + row * extent, at, extent, o);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
     row += step;
     if (k + 1 < rounds) {
-      if (kAhead) {
+      if constexpr (kAhead) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           xv[c] = xn[c];
@@ -302,8 +318,8 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
     const uint32_t at = (c * 64u * WAVES + t) * V;
     if (at >= extent) continue;
     if (alone) {
-      if (dw) store_piece<T, kWhole>(dw, at, extent, aw[c]);
-      if (db) store_piece<T, kWhole>(db, at, extent, ab[c]);
+      if (dw) store_piece<T>(dw, at, extent, aw[c]);
+      if (db) store_piece<T>(db, at, extent, ab[c]);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i)
@@ -397,14 +413,13 @@ TILER_LAYER_NORM(f32, float)
                                               float* __restrict__ rstd) {                                  \
     layer_norm_rows<T, WAVES, CH>(x, w, b, rows, (uint32_t)extent, eps, y, mean, rstd);                    \
   }
-#define TILER_LAYER_NORM_GRAD_ROWS(TY, T, WAVES, CH, NAME, AHEAD, WHOLE)                                   \
+#define TILER_LAYER_NORM_GRAD_ROWS(TY, T, WAVES, CH)                                                        \
   extern "C" __global__ void __launch_bounds__(1024)                                                       \
-      tiler_layer_norm_grad_##TY##_w##WAVES##c##CH##NAME(                                                  \
+      tiler_layer_norm_grad_##TY##_w##WAVES##c##CH(                                                        \
           const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ w,                      \
           const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint64_t extent,  \
           T* __restrict__ dx, float* __restrict__ partials, T* __restrict__ dw, T* __restrict__ db) {      \
-    layer_norm_grad_rows<T, WAVES, CH, AHEAD, WHOLE>(dy, x, w, mean, rstd, rows, (uint32_t)extent, dx,     \
-                                                     partials, dw, db);                                    \
+    layer_norm_grad_rows<T, WAVES, CH>(dy, x, w, mean, rstd, rows, (uint32_t)extent, dx, partials, dw, db); \
   }
 #define TILER_LAYER_NORM_FORMS(TY, T)      \
   TILER_LAYER_NORM_ROWS(TY, T, 1, 1)       \
@@ -418,17 +433,11 @@ TILER_LAYER_NORM(f32, float)
   TILER_LAYER_NORM_ROWS(TY, T, 16, 1)      \
   TILER_LAYER_NORM_ROWS(TY, T, 16, 2)      \
   TILER_LAYER_NORM_ROWS(TY, T, 16, 4)      \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 1, 1, , true, true) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 2, 1, , true, true) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 4, 1, , true, true) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 8, 1, , true, true) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 1, , true, true) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 2, , true, true) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 1, 1, r, false, false) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 2, 1, r, false, false) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 4, 1, r, false, false) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 8, 1, r, false, false) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 1, r, false, false) \
-  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 2, r, false, false)
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 1, 1) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 2, 1) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 4, 1) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 8, 1) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 1) \
+  TILER_LAYER_NORM_GRAD_ROWS(TY, T, 16, 2)
 TILER_LAYER_NORM_FORMS(bf16, uint16_t)
 TILER_LAYER_NORM_FORMS(f32, float)

@@ -28,27 +28,45 @@ __device__ __forceinline__ uint32_t valid_from(uint32_t at, uint32_t extent) {
   return at >= extent ? 0u : extent - at < (uint32_t)kVec<T> ? extent - at : (uint32_t)kVec<T>;
 }
 
-// The piece at `at`, zeros past the row's end.  kStream: read once, past the
-// caches.  kWhole: the extent is a multiple of kVec, so no piece is cut.
-template <typename T, bool kStream, bool kWhole = false>
-__device__ __forceinline__ u32x4 load_piece(const T* row, uint32_t at, uint32_t extent) {
-  if constexpr (kWhole) {
-    if (at >= extent) return u32x4{0, 0, 0, 0};
-    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + at);
-    return kStream ? __builtin_nontemporal_load(p) : *p;
+// A thread's CH pieces of a row in two steps, so that nothing stands between
+// the loads: load_row reads a whole piece each, those that would pass the
+// row's end the last one inside it; settle_row moves their elements into place
+// and clears what lies past the end.  kStream: read once, past the caches.
+template <typename T, int WAVES, int CH, bool kStream>
+__device__ __forceinline__ void load_row(const T* row, uint32_t t, uint32_t extent, u32x4 (&v)[CH]) {
+  constexpr uint32_t V = kVec<T>;
+  if (extent >= V) {  // uniform
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const uint32_t at = (c * 64u * WAVES + t) * V;
+      const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + (at + V <= extent ? at : extent - V));
+      v[c] = kStream ? __builtin_nontemporal_load(p) : *p;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) v[c] = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t e = 0; e + 1 < V; ++e)
+      if (t == 0 && e < extent) {
+        if constexpr (sizeof(T) == 2) v[0][e >> 1] |= (uint32_t)row[e] << (16u * (e & 1u));
+        else v[0][e] = __float_as_uint(row[e]);
+      }
   }
-  const uint32_t valid = valid_from<T>(at, extent);
-  if (valid == (uint32_t)kVec<T>) {
-    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + at);
-    return kStream ? __builtin_nontemporal_load(p) : *p;
+}
+template <typename T, int WAVES, int CH>
+__device__ __forceinline__ void settle_row(uint32_t t, uint32_t extent, u32x4 (&v)[CH]) {
+  constexpr uint32_t V = kVec<T>;
+  if (extent < V) return;  // uniform: in place already
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t at = (c * 64u * WAVES + t) * V;
+    if (at + V > extent) v[c] = at >= extent ? u32x4{0, 0, 0, 0}
+                                             : tiler_pieces::drop_bytes(v[c], (at + V - extent) * (uint32_t)sizeof(T));
   }
-  if (valid == 0) return u32x4{0, 0, 0, 0};
-  return tiler_pieces::guarded_piece(reinterpret_cast<const uint8_t*>(row + at), valid * (uint32_t)sizeof(T),
-                                     reinterpret_cast<const uint8_t*>(row));
 }
 
 // Narrows and stores the piece's elements inside the row.
-template <typename T, bool kWhole = false>
+template <typename T>
 __device__ __forceinline__ void store_piece(T* row, uint32_t at, uint32_t extent, const float (&o)[kVec<T>]) {
   const uint32_t valid = valid_from<T>(at, extent);
   u32x4 v;
@@ -57,7 +75,7 @@ __device__ __forceinline__ void store_piece(T* row, uint32_t at, uint32_t extent
     if constexpr (sizeof(T) == 2) v[e] = tiler::bf16_pack2_rne(o[2 * e], o[2 * e + 1]);
     else v[e] = __float_as_uint(tiler::canon(o[e]));
   }
-  if (kWhole || valid == (uint32_t)kVec<T>) {
+  if (valid == (uint32_t)kVec<T>) {
     __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(row + at));
     return;
   }

@@ -122,13 +122,12 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
   uint32_t partials = 0;
   if (rows && pieces <= 2048) {
     // Rows in registers, 16 / WAVES of them per workgroup at a time: at most
-    // one workgroup per CU, so that there are few partials.  "r": the last
-    // piece of a row is cut.
+    // one workgroup per CU, so that there are few partials.
     const uint64_t groups = ceil_div(rows, 16 / waves);
     count = groups < t.compute_units ? groups : t.compute_units;
     if (sums && count > 1) partials = p.slot(mul_sat(mul_sat(count, extent), 8), kSlotScratch);
-    std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_w%uc%u%s", type_name(dtype), waves,
-                  pieces <= 1024 ? 1u : 2u, extent % vec ? "r" : "");
+    std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_w%uc%u", type_name(dtype), waves,
+                  pieces <= 1024 ? 1u : 2u);
     Launch& l = p.add(name, (uint32_t)count, 1, 1024).ptr(dy).ptr(x);
     slot_or_null(l, has_w, w);
     l.ptr(mean).ptr(rstd).u64(rows).u64(extent);

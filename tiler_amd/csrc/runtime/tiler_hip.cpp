@@ -378,9 +378,7 @@ const EntryRow kEntries[] = {
 #undef TILER_ROW_FORM
 #define TILER_GRAD_FORM(FORM)                                                  \
   {"tiler_layer_norm_grad_bf16_" FORM, "layer-norm-backward/bf16", 9},          \
-      {"tiler_layer_norm_grad_f32_" FORM, "layer-norm-backward-f32", 9},        \
-      {"tiler_layer_norm_grad_bf16_" FORM "r", "layer-norm-backward/bf16", 9},  \
-      {"tiler_layer_norm_grad_f32_" FORM "r", "layer-norm-backward-f32", 9}
+      {"tiler_layer_norm_grad_f32_" FORM, "layer-norm-backward-f32", 9}
     TILER_GRAD_FORM("w1c1"), TILER_GRAD_FORM("w2c1"), TILER_GRAD_FORM("w4c1"), TILER_GRAD_FORM("w8c1"),
     TILER_GRAD_FORM("w16c1"), TILER_GRAD_FORM("w16c2"),
 #undef TILER_GRAD_FORM
