@@ -17,7 +17,7 @@ using tiler_product::i32x4;
 using tiler_product::kSlice;
 
 // s = max(max |x| / 127, 2^-126), the quotient correctly rounded; q = x / s to
-// the nearest integer, ties to even, exactly: the candidate rint(x * (1 / s))
+// the nearest integer, ties to even, exactly: the candidate r = rint(x (1 / s))
 // is at most one off, next to a tie; d = x - r s is exact in one FMA (a
 // multiple of s's last place below 2 s, or x itself when r = 0), so comparing
 // it with the exact s / 2 decides.  |x| <= 127 s (1 + 2^-24), so |q| <= 127.
@@ -32,6 +32,27 @@ __device__ __forceinline__ int32_t code_of(float x, float s, float inverse) {
   if (d > half || (odd && d == half)) r += 1.0f;
   else if (-d > half || (odd && -d == half)) r -= 1.0f;
   return (int32_t)r;
+}
+
+// Four codes, a byte each.  The candidates come as the low bits of
+// x (1 / s) + 1.5 2^23 (one FMA, rounded to an integer by the sum); where some
+// |x - r s| reaches s / 2, a tie or a candidate that is off, the exact rule.
+constexpr float kRound = 12582912.0f;
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float s, float inverse) {
+  uint32_t bits[4];
+  bool check = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float m = __builtin_fmaf(x[e], inverse, kRound);
+    bits[e] = __float_as_uint(m);
+    check |= __builtin_fabsf(__builtin_fmaf(-(m - kRound), s, x[e])) >= 0.5f * s;
+  }
+  if (check) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bits[e] = (uint32_t)code_of(x[e], s, inverse);
+  }
+  const uint32_t lo = __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(bits[3], bits[2], 0x04000c0cu);
+  return lo | hi;
 }
 
 // |x| and whether it is not finite, folded over a row: the magnitude's bits
@@ -95,9 +116,10 @@ __device__ __forceinline__ void quantize_rows(const T* __restrict__ x, uint64_t 
     uint32_t words[V / 4];
 #pragma unroll
     for (int h = 0; h < V / 4; ++h) {
-      uint32_t word = 0;
+      float four[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) word |= (uint32_t)(uint8_t)code_of(element<T>(v[c], 4 * h + e), s, inverse) << (8 * e);
+      for (int e = 0; e < 4; ++e) four[e] = element<T>(v[c], 4 * h + e);
+      const uint32_t word = codes_of(four, s, inverse);
       words[h] = finite ? word : 0u;
     }
     if (valid == (uint32_t)V) {

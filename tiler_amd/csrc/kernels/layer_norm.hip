@@ -86,10 +86,11 @@ __device__ __forceinline__ void layer_norm_grad_stream(const T* __restrict__ dy,
 // ---------------------------------------------------------------------------
 // Rows in registers.
 
-// Forward: a group of WAVES waves per row, CH pieces a thread.  The mean is
-// taken first, then the differences' sum and squares: the first corrects the
-// mean's rounding, so that neither a large offset nor the grouping of the sum
-// reaches the variance.
+// Forward: a group of WAVES waves per row, CH pieces a thread.  The mean first,
+// then the squares of the differences from it.  For f32 rows the differences
+// are summed too: that corrects the mean's rounding, which a row far from zero
+// would otherwise carry into its results (bf16 results round far more coarsely,
+// and the sum would cost a tenth of the kernel).
 template <typename T, int WAVES, int CH>
 __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T* __restrict__ w,
                                                 const T* __restrict__ b, uint64_t rows, uint32_t extent, float eps,
@@ -97,7 +98,8 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
                                                 float* __restrict__ rstd) {
   using namespace tiler_rows;
   constexpr int V = kVec<T>;
-  constexpr uint32_t kGroups = WAVES == 1 ? 4 : 1;
+  constexpr bool kCorrect = sizeof(T) == 4;
+  constexpr uint32_t kGroups = WAVES == 1 ? 4 : 1, kSpan = 64u * WAVES * V;
   __shared__ float slots[2][2 * (WAVES == 1 ? 1 : WAVES)];
   const uint32_t t = threadIdx.x % (64u * WAVES);
   const uint64_t row = (uint64_t)blockIdx.x * kGroups + threadIdx.x / (64u * WAVES);
@@ -119,25 +121,35 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
   // opaque: widened again below, not kept widened across the sums
 #pragma unroll
   for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(v[c]));
-  const float count = (float)extent, mu0 = s / count;
-  float s1 = 0.0f, s2 = 0.0f;
+  const float count = (float)extent;
+  float mu = s / count, s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const uint32_t valid = valid_from<T>((c * 64u * WAVES + t) * V, extent);
-    float d[V], q[V];
+    float d[V], q = 0.0f;
+    if ((c + 1u) * kSpan <= extent) {  // uniform: every thread's piece is whole
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      d[i] = (uint32_t)i < valid ? element<T>(v[c], i) - mu0 : 0.0f;
-      q[i] = d[i] * d[i];
+      for (int i = 0; i < V; ++i) d[i] = element<T>(v[c], i) - mu;
+    } else {
+      const uint32_t valid = valid_from<T>((c * 64u * WAVES + t) * V, extent);
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = (uint32_t)i < valid ? element<T>(v[c], i) - mu : 0.0f;
     }
-    s1 += pairwise(d);
-    s2 += pairwise(q);
+#pragma unroll
+    for (int i = 0; i < V; ++i) q = __builtin_fmaf(d[i], d[i], q);
+    if constexpr (kCorrect) s1 += pairwise(d);
+    s2 += q;
   }
-  group_sums<WAVES>(s1, s2, slots[1]);
+  group_sums<WAVES>(s2, s1, slots[1]);
 #pragma unroll
   for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(v[c]));
-  const float shift = s1 / count, var = s2 / count - shift * shift, mu = mu0 + shift;
-  const float r = 1.0f / __builtin_sqrtf((var < 0.0f ? 0.0f : var) + eps);
+  float var = s2 / count;
+  if constexpr (kCorrect) {
+    const float shift = s1 / count;
+    var = __builtin_fmaf(-shift, shift, var);
+    var = var < 0.0f ? 0.0f : var;
+    mu = mu + shift;
+  }
+  const float r = 1.0f / __builtin_sqrtf(var + eps);
   if (t == 0 && mean) {
     mean[row] = mu;
     rstd[row] = r;
@@ -163,9 +175,10 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
       float o[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        o[i] = ((element<T>(v[c0 + c], i) - mu0) - shift) * r;
-        if (w) o[i] = o[i] * element<T>(wv[c], i);
-        if (b) o[i] = o[i] + element<T>(bv[c], i);
+        o[i] = (element<T>(v[c0 + c], i) - mu) * r;
+        if (w && b) o[i] = __builtin_fmaf(o[i], element<T>(wv[c], i), element<T>(bv[c], i));
+        else if (w) o[i] = o[i] * element<T>(wv[c], i);
+        else if (b) o[i] = o[i] + element<T>(bv[c], i);
       }
       store_piece<T>(y, at, extent, o);
     }
@@ -232,19 +245,19 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float g[V], q[V];
+      float g[V], q = 0.0f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         // past the row's end dy is zero, and so are the terms
         const float d = element<T>(dv[c], i), xh = (element<T>(xv[c], i) - mu) * r;
         g[i] = w ? d * element<T>(wv[c], i) : d;
-        q[i] = g[i] * xh;
-        aw[c][i] += d * xh;
+        q = __builtin_fmaf(g[i], xh, q);
+        aw[c][i] = __builtin_fmaf(d, xh, aw[c][i]);
         ab[c][i] += d;
         asm volatile("" : "+v"(aw[c][i]), "+v"(ab[c][i]));  // added here, not past the barrier with its terms kept
       }
       s1 += pairwise(g);
-      s2 += pairwise(q);
+      s2 += q;
       __builtin_amdgcn_sched_barrier(0);  // one piece's temporaries at a time
     }
     // opaque: widened again below, not kept widened across the sums
@@ -252,7 +265,9 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
     for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(xv[c]), "+v"(dv[c]), "+v"(wv[c]));
     if (dx) {  // uniform: every wave takes the same barriers
       group_sums<WAVES>(s1, s2, slots[k & 1u]);
-      const float c1 = s1 / (float)extent, c2 = s2 / (float)extent;
+      // dx = r g + (x - mu) (-r^2 c2) - r c1: x's share as one FMA of x
+      const float c1 = s1 / (float)extent, c2 = s2 / (float)extent, a = -(r * r) * c2;
+      const float z = __builtin_fmaf(-mu, a, -(r * c1));
       if (row < rows) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -262,7 +277,7 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             const float d = element<T>(dv[c], i), g = w ? d * element<T>(wv[c], i) : d;
-            o[i] = r * (g - c1 - (element<T>(xv[c], i) - mu) * r * c2);
+            o[i] = __builtin_fmaf(g, r, __builtin_fmaf(element<T>(xv[c], i), a, z));
           }
           store_piece<T>(dx + row * extent, at, extent, o);
           __builtin_amdgcn_sched_barrier(0);

@@ -65,15 +65,25 @@ __device__ __forceinline__ void settle_row(uint32_t t, uint32_t extent, u32x4 (&
   }
 }
 
-// Narrows and stores the piece's elements inside the row.
+// Narrows and stores the piece's elements inside the row.  A NaN is looked for
+// two values at a time (an unordered comparison) and made canonical where there
+// is one.
 template <typename T>
-__device__ __forceinline__ void store_piece(T* row, uint32_t at, uint32_t extent, const float (&o)[kVec<T>]) {
+__device__ __forceinline__ void store_piece(T* row, uint32_t at, uint32_t extent, float (&o)[kVec<T>]) {
   const uint32_t valid = valid_from<T>(at, extent);
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < kVec<T>; e += 2) nan |= __builtin_isunordered(o[e], o[e + 1]);
+  if (nan) {
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) o[e] = tiler::canon(o[e]);
+  }
   u32x4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if constexpr (sizeof(T) == 2) v[e] = tiler::bf16_pack2_rne(o[2 * e], o[2 * e + 1]);
-    else v[e] = __float_as_uint(tiler::canon(o[e]));
+    if constexpr (sizeof(T) == 2)
+      v[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((tiler::f32x2_pair{o[2 * e], o[2 * e + 1]}), tiler::bf16x2_pair));
+    else v[e] = __float_as_uint(o[e]);
   }
   if (valid == (uint32_t)kVec<T>) {
     __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(row + at));
