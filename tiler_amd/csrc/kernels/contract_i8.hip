@@ -62,11 +62,7 @@ __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(
 // The largest magnitude of a group of WAVES waves, in every lane.
 template <int WAVES>
 __device__ __forceinline__ uint32_t group_top(uint32_t top, uint32_t* slots) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const uint32_t other = __shfl_xor(top, o, 64);
-    top = other > top ? other : top;
-  }
+  top = tiler_rows::wave_fold(top, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
   if constexpr (WAVES > 1) {
     __syncthreads();  // a row before is done with the slots
     if ((threadIdx.x & 63u) == 0) slots[threadIdx.x >> 6] = top;
@@ -165,7 +161,7 @@ __device__ __forceinline__ void quantize_stream(const T* __restrict__ x, uint64_
 }  // namespace
 
 #define TILER_QUANTIZE_ROWS(TY, T, WAVES, CH)                                                              \
-  extern "C" __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)                              \
+  extern "C" __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 4)                            \
       tiler_quantize_rows_i8_##TY##_w##WAVES##c##CH(const T* __restrict__ x, uint64_t rows, uint64_t extent, \
                                                     int8_t* __restrict__ q, float* __restrict__ scales) {  \
     quantize_rows<T, WAVES, CH>(x, rows, (uint32_t)extent, q, scales);                                     \
@@ -179,8 +175,6 @@ __device__ __forceinline__ void quantize_stream(const T* __restrict__ x, uint64_
   TILER_QUANTIZE_ROWS(TY, T, 1, 1)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 1, 2)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 1, 4)                                                                         \
-  TILER_QUANTIZE_ROWS(TY, T, 1, 8)                                                                         \
-  TILER_QUANTIZE_ROWS(TY, T, 1, 16)                                                                        \
   TILER_QUANTIZE_ROWS(TY, T, 4, 1)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 4, 2)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 4, 4)                                                                         \

@@ -185,7 +185,12 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
   }
 }
 
-// Gradients, one read of dy and x: a workgroup of 16 waves holds 16 / WAVES
+// Waves of a gradient workgroup: 8, two workgroups to a CU (each waits at its
+// own barriers); 16 where a row takes them all.
+template <int WAVES>
+constexpr int kGradWaves = WAVES == 16 ? 16 : 8;
+
+// Gradients, one read of dy and x: a workgroup holds kGradWaves / WAVES
 // rows at a time and walks the rows with a stride of the whole grid; a thread
 // keeps the column sums of its own pieces over all of its rows, the groups meet
 // in LDS, and each workgroup leaves one partial (dw's sums, then db's), or the
@@ -200,8 +205,8 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
   using namespace tiler_rows;
   constexpr int V = kVec<T>;
   constexpr bool kAhead = CH * V <= 8;  // beyond, the next rows' pieces do not fit the registers
-  constexpr uint32_t kGroups = 16 / WAVES, kSpan = CH * 64u * WAVES * V;  // elements a group's pieces cover
-  __shared__ float slots[2][32];
+  constexpr uint32_t kGroups = kGradWaves<WAVES> / WAVES, kSpan = CH * 64u * WAVES * V;  // elements a group's pieces cover
+  __shared__ float slots[2][2 * kGradWaves<WAVES>];
   __shared__ float columns[kGroups > 1 ? 2 * kSpan : 1];
   const uint32_t t = threadIdx.x % (64u * WAVES), group = threadIdx.x / (64u * WAVES);
   const bool sums = partials || dw || db;
@@ -229,17 +234,16 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
     load_row<T, WAVES, CH, true>(x + here * extent, t, extent, xo);
     load_row<T, WAVES, CH, true>(dy + here * extent, t, extent, dyo);
   };
-  load(row, xv, dv, mu, r);
-#pragma unroll 1
-  for (uint64_t k = 0; k < rounds; ++k) {
-    u32x4 xn[CH], dn[CH];
-    float mun = 0.0f, rn = 0.0f;
-    if (kAhead && k + 1 < rounds) load(row + step, xn, dn, mun, rn);
-    settle_row<T, WAVES, CH>(t, extent, xv);
-    settle_row<T, WAVES, CH>(t, extent, dv);
+  // One round: the next rows' pieces are requested (past the last rows, the
+  // last one again), then the current ones are reduced and stored.
+  auto turn = [&](uint64_t k, u32x4(&xc)[CH], u32x4(&dc)[CH], float mu, float r, u32x4(&xn)[CH], u32x4(&dn)[CH],
+                  float& mun, float& rn) {
+    if constexpr (kAhead) load(row + step, xn, dn, mun, rn);
+    settle_row<T, WAVES, CH>(t, extent, xc);
+    settle_row<T, WAVES, CH>(t, extent, dc);
     if (row >= rows) {  // whole groups, in the last round
 #pragma unroll
-      for (int c = 0; c < CH; ++c) xv[c] = dv[c] = u32x4{0, 0, 0, 0};
+      for (int c = 0; c < CH; ++c) xc[c] = dc[c] = u32x4{0, 0, 0, 0};
       mu = r = 0.0f;
     }
     float s1 = 0.0f, s2 = 0.0f;
@@ -249,7 +253,7 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         // past the row's end dy is zero, and so are the terms
-        const float d = element<T>(dv[c], i), xh = (element<T>(xv[c], i) - mu) * r;
+        const float d = element<T>(dc[c], i), xh = (element<T>(xc[c], i) - mu) * r;
         g[i] = w ? d * element<T>(wv[c], i) : d;
         q = __builtin_fmaf(g[i], xh, q);
         aw[c][i] = __builtin_fmaf(d, xh, aw[c][i]);
@@ -262,7 +266,7 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
     }
     // opaque: widened again below, not kept widened across the sums
 #pragma unroll
-    for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(xv[c]), "+v"(dv[c]), "+v"(wv[c]));
+    for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(xc[c]), "+v"(dc[c]), "+v"(wv[c]));
     if (dx) {  // uniform: every wave takes the same barriers
       group_sums<WAVES>(s1, s2, slots[k & 1u]);
       // dx = r g + (x - mu) (-r^2 c2) - r c1: x's share as one FMA of x
@@ -276,8 +280,8 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
           float o[V];
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float d = element<T>(dv[c], i), g = w ? d * element<T>(wv[c], i) : d;
-            o[i] = __builtin_fmaf(g, r, __builtin_fmaf(element<T>(xv[c], i), a, z));
+            const float d = element<T>(dc[c], i), g = w ? d * element<T>(wv[c], i) : d;
+            o[i] = __builtin_fmaf(g, r, __builtin_fmaf(element<T>(xc[c], i), a, z));
           }
           store_piece<T>(dx + row * extent, at, extent, o);
           __builtin_amdgcn_sched_barrier(0);
@@ -285,19 +289,17 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
       }
     }
     row += step;
-    if (k + 1 < rounds) {
-      if constexpr (kAhead) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          xv[c] = xn[c];
-          dv[c] = dn[c];
-        }
-        mu = mun;
-        r = rn;
-      } else {
-        load(row, xv, dv, mu, r);
-      }
+    if constexpr (!kAhead) {
+      if (k + 1 < rounds) load(row, xn, dn, mun, rn);
     }
+  };
+  load(row, xv, dv, mu, r);
+  u32x4 xo[CH], dyo[CH];
+  float muo = 0.0f, ro = 0.0f;
+#pragma unroll 1
+  for (uint64_t k = 0; k < rounds; k += 2) {  // two rounds, so that no piece moves between registers
+    turn(k, xv, dv, mu, r, xo, dyo, muo, ro);
+    if (k + 1 < rounds) turn(k + 1, xo, dyo, muo, ro, xv, dv, mu, r);
   }
   if (!sums) return;
   // The groups' columns, added in ascending order of the groups.
@@ -421,7 +423,7 @@ TILER_LAYER_NORM(bf16, uint16_t)
 TILER_LAYER_NORM(f32, float)
 
 #define TILER_LAYER_NORM_ROWS(TY, T, WAVES, CH)                                                            \
-  extern "C" __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)                              \
+  extern "C" __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 4)                            \
       tiler_layer_norm_##TY##_w##WAVES##c##CH(const T* __restrict__ x, const T* __restrict__ w,            \
                                               const T* __restrict__ b, uint64_t rows, uint64_t extent,     \
                                               float eps, T* __restrict__ y, float* __restrict__ mean,      \
@@ -429,7 +431,7 @@ TILER_LAYER_NORM(f32, float)
     layer_norm_rows<T, WAVES, CH>(x, w, b, rows, (uint32_t)extent, eps, y, mean, rstd);                    \
   }
 #define TILER_LAYER_NORM_GRAD_ROWS(TY, T, WAVES, CH)                                                        \
-  extern "C" __global__ void __launch_bounds__(1024)                                                       \
+  extern "C" __global__ void __launch_bounds__(64 * kGradWaves<WAVES>)                                     \
       tiler_layer_norm_grad_##TY##_w##WAVES##c##CH(                                                        \
           const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ w,                      \
           const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint64_t extent,  \
@@ -441,7 +443,6 @@ TILER_LAYER_NORM(f32, float)
   TILER_LAYER_NORM_ROWS(TY, T, 1, 2)       \
   TILER_LAYER_NORM_ROWS(TY, T, 1, 4)       \
   TILER_LAYER_NORM_ROWS(TY, T, 1, 8)       \
-  TILER_LAYER_NORM_ROWS(TY, T, 1, 16)      \
   TILER_LAYER_NORM_ROWS(TY, T, 4, 1)       \
   TILER_LAYER_NORM_ROWS(TY, T, 4, 2)       \
   TILER_LAYER_NORM_ROWS(TY, T, 4, 4)       \

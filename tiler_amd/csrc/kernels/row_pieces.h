@@ -28,35 +28,24 @@ __device__ __forceinline__ uint32_t valid_from(uint32_t at, uint32_t extent) {
   return at >= extent ? 0u : extent - at < (uint32_t)kVec<T> ? extent - at : (uint32_t)kVec<T>;
 }
 
-// A thread's CH pieces of a row in two steps, so that nothing stands between
-// the loads: load_row reads a whole piece each, those that would pass the
-// row's end the last one inside it; settle_row moves their elements into place
-// and clears what lies past the end.  kStream: read once, past the caches.
+// A thread's CH pieces of a row (of at least kVec elements) in two steps, so
+// that no branch stands between the loads: load_row reads a whole piece each,
+// those that would pass the row's end the last one inside it; settle_row moves
+// their elements into place and clears what lies past the end.  kStream: read
+// once, past the caches.
 template <typename T, int WAVES, int CH, bool kStream>
 __device__ __forceinline__ void load_row(const T* row, uint32_t t, uint32_t extent, u32x4 (&v)[CH]) {
   constexpr uint32_t V = kVec<T>;
-  if (extent >= V) {  // uniform
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const uint32_t at = (c * 64u * WAVES + t) * V;
-      const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + (at + V <= extent ? at : extent - V));
-      v[c] = kStream ? __builtin_nontemporal_load(p) : *p;
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) v[c] = u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (uint32_t e = 0; e + 1 < V; ++e)
-      if (t == 0 && e < extent) {
-        if constexpr (sizeof(T) == 2) v[0][e >> 1] |= (uint32_t)row[e] << (16u * (e & 1u));
-        else v[0][e] = __float_as_uint(row[e]);
-      }
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t at = (c * 64u * WAVES + t) * V;
+    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + (at + V <= extent ? at : extent - V));
+    v[c] = kStream ? __builtin_nontemporal_load(p) : *p;
   }
 }
 template <typename T, int WAVES, int CH>
 __device__ __forceinline__ void settle_row(uint32_t t, uint32_t extent, u32x4 (&v)[CH]) {
   constexpr uint32_t V = kVec<T>;
-  if (extent < V) return;  // uniform: in place already
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const uint32_t at = (c * 64u * WAVES + t) * V;
@@ -104,17 +93,31 @@ __device__ __forceinline__ float pairwise(const float (&v)[N]) {
   else return (v[0] + v[1]) + (v[2] + v[3]);
 }
 
+// A wave's fold of v under f, the same value in every lane: within each row of
+// 16 lanes by four data-parallel moves (lanes i ^ 1, i ^ 2, 7 - i, 15 - i), then
+// the four rows' values, read through scalar registers.  No LDS round trips.
+template <typename V, typename F>
+__device__ __forceinline__ V wave_fold(V v, F f) {
+  auto moved = [](V x, auto ctrl) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  v = f(v, moved(v, tiler::Step<0xB1>{}));   // quad_perm [1,0,3,2]
+  v = f(v, moved(v, tiler::Step<0x4E>{}));   // quad_perm [2,3,0,1]
+  v = f(v, moved(v, tiler::Step<0x141>{}));  // row_half_mirror
+  v = f(v, moved(v, tiler::Step<0x140>{}));  // row_mirror
+  auto lane = [&](int l) { return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
+  return f(f(lane(0), lane(16)), f(lane(32), lane(48)));
+}
+
 // Two sums over a group of WAVES waves, the same values in every lane.  The
 // waves of one workgroup all call it; `slots` holds 2 floats per wave, and a
 // caller alternates between two such arrays from call to call, so that one
 // barrier a call is enough.
 template <int WAVES>
 __device__ __forceinline__ void group_sums(float& a, float& b, float* slots) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    a += __shfl_xor(a, o, 64);
-    b += __shfl_xor(b, o, 64);
-  }
+  auto add = [](float p, float q) { return p + q; };
+  a = wave_fold(a, add);
+  b = wave_fold(b, add);
   if constexpr (WAVES > 1) {
     const uint32_t wave = threadIdx.x >> 6, first = wave / WAVES * WAVES;
     if ((threadIdx.x & 63u) == 0) {

@@ -30,14 +30,17 @@ constexpr uint32_t kRowWorkgroups = 1u << 20;  // rows beyond take further round
 // elements, kVec = `vec` to a 16-byte piece: WAVES waves per row and CH pieces
 // a thread, "w{WAVES}c{CH}", or "s" (streamed) beyond what registers hold.
 // One wave a row (four rows a workgroup, no barrier) where that gives every
-// SIMD a wave and a thread at most 16 pieces; fewer rows than that, or longer
-// ones, take four waves a row, then sixteen.
+// SIMD a wave and a thread at most `one_wave` pieces; fewer rows than that, or
+// longer ones, take four waves a row, then sixteen.  Rows shorter than a piece
+// are streamed.  us, one wave and four: norm of 8192 x 4096 bf16 31.8 / 65, of
+// 4096 x 4096 f32 (16 pieces) 31.6 / 27.6, of 2048 x 8192 bf16 (16) 20.4 / 17.9;
+// quantization of 4096 x 4096 bf16 (8) 17.7 / 13.4, of 8192 x 2048 (4) 15.2 / 14.3.
 struct RowForm {
   char name[16];
   uint32_t block;
   uint64_t grid;
 };
-RowForm row_form(const Target& t, uint64_t rows, uint64_t extent, uint64_t vec) {
+RowForm row_form(const Target& t, uint64_t rows, uint64_t extent, uint64_t vec, uint64_t one_wave) {
   const uint64_t pieces = ceil_div(extent, vec);
   RowForm f{"s", 256, rows < kRowWorkgroups ? rows : kRowWorkgroups};
   uint32_t waves = 0, ch = 0;
@@ -46,7 +49,8 @@ RowForm row_form(const Target& t, uint64_t rows, uint64_t extent, uint64_t vec) 
     while (p < v) p <<= 1;
     return p;
   };
-  if (pieces <= 64 || (pieces <= 64 * 16 && rows >= 4ull * t.compute_units)) waves = 1, ch = pow2(ceil_div(pieces, 64));
+  if (extent < vec) waves = 0;
+  else if (pieces <= 64 || (pieces <= 64 * one_wave && rows >= 4ull * t.compute_units)) waves = 1, ch = pow2(ceil_div(pieces, 64));
   else if (pieces <= 256 * 4) waves = 4, ch = pow2(ceil_div(pieces, 256));
   else if (pieces <= 1024 * 4) waves = 16, ch = pow2(ceil_div(pieces, 1024));
   const uint32_t block = waves == 1 ? 256 : 64 * waves;
@@ -84,7 +88,7 @@ tiler_hip_status plan_layer_norm(const Target& t, uint32_t dtype, uint32_t parts
   if (rows == 0 || extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
-  const RowForm f = row_form(t, rows, extent, 16 / elem);
+  const RowForm f = row_form(t, rows, extent, 16 / elem, 8);
   std::snprintf(name, sizeof(name), "tiler_layer_norm_%s_%s", type_name(dtype), f.name);
   Launch& l = p.add(name, (uint32_t)f.grid, 1, f.block).ptr(x);
   slot_or_null(l, has_w, w);
@@ -120,15 +124,17 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
   const uint32_t waves = pieces <= 64 ? 1 : pieces <= 128 ? 2 : pieces <= 256 ? 4 : pieces <= 512 ? 8 : 16;
   uint64_t count = 0;  // partials of dw's and db's sums
   uint32_t partials = 0;
-  if (rows && pieces <= 2048) {
-    // Rows in registers, 16 / WAVES of them per workgroup at a time: at most
-    // one workgroup per CU, so that there are few partials.
-    const uint64_t groups = ceil_div(rows, 16 / waves);
-    count = groups < t.compute_units ? groups : t.compute_units;
+  if (rows && extent >= vec && pieces <= 2048) {
+    // Rows in registers, 8 / WAVES of them (or one of 16 waves) per workgroup at
+    // a time, at most as many workgroups as run at once, so that there are few
+    // partials.
+    const uint64_t groups = waves == 16 ? rows : ceil_div(rows, 8 / waves);
+    const uint64_t most = (waves == 16 ? 1ull : 2ull) * t.compute_units;
+    count = groups < most ? groups : most;
     if (sums && count > 1) partials = p.slot(mul_sat(mul_sat(count, extent), 8), kSlotScratch);
     std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_w%uc%u", type_name(dtype), waves,
                   pieces <= 1024 ? 1u : 2u);
-    Launch& l = p.add(name, (uint32_t)count, 1, 1024).ptr(dy).ptr(x);
+    Launch& l = p.add(name, (uint32_t)count, 1, waves == 16 ? 1024 : 512).ptr(dy).ptr(x);
     slot_or_null(l, has_w, w);
     l.ptr(mean).ptr(rstd).u64(rows).u64(extent);
     slot_or_null(l, has_dx, dx);
@@ -303,7 +309,7 @@ tiler_hip_status plan_quantize_rows_i8(const Target& t, uint32_t dtype, uint64_t
   if (rows == 0 || extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
-  const RowForm f = row_form(t, rows, extent, dtype == TILER_HIP_BF16 ? 8 : 4);
+  const RowForm f = row_form(t, rows, extent, dtype == TILER_HIP_BF16 ? 8 : 4, 4);
   std::snprintf(name, sizeof(name), "tiler_quantize_rows_i8_%s_%s", type_name(dtype), f.name);
   p.add(name, (uint32_t)f.grid, 1, f.block)
       .ptr(x).u64(rows).u64(extent).ptr(q).ptr(scales);
