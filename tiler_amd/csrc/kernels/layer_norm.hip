@@ -19,6 +19,9 @@ __device__ __forceinline__ void norm_store(T* p, uint64_t i, float v) {
   else p[i] = tiler::canon(v);
 }
 
+// Columns of a partial: dw's sums, then db's, each from a 32-byte boundary.
+__device__ __forceinline__ uint64_t partial_ld(uint64_t extent) { return (extent + 7u) / 8u * 8u; }
+
 // Sum over a 256-thread workgroup, the same value in every thread.
 __device__ __forceinline__ double block_sum(double v, double* waves) {
 #pragma unroll
@@ -329,7 +332,8 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
     if (group != 0) return;
   }
   const bool alone = gridDim.x == 1;
-  float* out = alone ? nullptr : partials + (uint64_t)blockIdx.x * 2u * extent;
+  const uint32_t ld = partial_ld(extent);
+  float* out = alone ? nullptr : partials + (uint64_t)blockIdx.x * 2u * ld;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const uint32_t at = (c * 64u * WAVES + t) * V;
@@ -339,11 +343,10 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
       if (db) store_piece<T>(db, at, extent, ab[c]);
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (at + i < extent) {
-          out[at + i] = aw[c][i];
-          out[extent + at + i] = ab[c][i];
-        }
+      for (int i = 0; i < V; i += 4) {
+        *reinterpret_cast<f32x4*>(out + at + i) = f32x4{aw[c][i], aw[c][i + 1], aw[c][i + 2], aw[c][i + 3]};
+        *reinterpret_cast<f32x4*>(out + ld + at + i) = f32x4{ab[c][i], ab[c][i + 1], ab[c][i + 2], ab[c][i + 3]};
+      }
     }
   }
 }
@@ -364,31 +367,35 @@ __device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, con
     sw += d * ((norm_load(x, r * extent + col) - mean[r]) * rstd[r]);
     sb += d;
   }
-  float* out = partials + (uint64_t)blockIdx.y * 2u * extent;
+  const uint64_t ld = partial_ld(extent);
+  float* out = partials + (uint64_t)blockIdx.y * 2u * ld;
   out[col] = sw;
-  out[extent + col] = sb;
+  out[ld + col] = sb;
 }
 
-// dw and db from `count` partials: 64 columns a workgroup, wave q the partials
-// q, q + 16, ... in ascending order, the waves' sums in ascending order.
+// dw (blockIdx.y 0) and db (1) from `count` partials: 64 columns a workgroup,
+// wave q the partials q, q + 16, ... in ascending order, the waves' sums in
+// ascending order.
 template <typename T>
 __device__ __forceinline__ void layer_norm_columns_final(const float* __restrict__ partials, uint32_t count,
                                                          uint64_t extent, T* __restrict__ dw, T* __restrict__ db) {
   __shared__ float waves[16][64];
+  T* const out = blockIdx.y ? db : dw;
+  if (!out) return;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint64_t i = blockIdx.x * 64ull + lane;
+  const uint64_t col = blockIdx.x * 64ull + lane, ld = partial_ld(extent);
   float s = 0.0f;
-  if (i < 2u * extent) {
+  if (col < extent) {
+    const float* at = partials + blockIdx.y * ld + col;
 #pragma unroll 8
-    for (uint32_t p = wave; p < count; p += 16u) s += partials[(uint64_t)p * 2u * extent + i];
+    for (uint32_t p = wave; p < count; p += 16u) s += at[(uint64_t)p * 2u * ld];
   }
   waves[wave][lane] = s;
   __syncthreads();
-  if (wave != 0 || i >= 2u * extent) return;
+  if (wave != 0 || col >= extent) return;
 #pragma unroll
   for (int q = 1; q < 16; ++q) s += waves[q][lane];
-  T* out = i < extent ? dw : db;
-  if (out) norm_store(out, i < extent ? i : i - extent, s);
+  norm_store(out, col, s);
 }
 
 }  // namespace

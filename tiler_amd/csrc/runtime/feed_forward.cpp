@@ -131,7 +131,7 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
     const uint64_t groups = waves == 16 ? rows : ceil_div(rows, 8 / waves);
     const uint64_t most = (waves == 16 ? 1ull : 2ull) * t.compute_units;
     count = groups < most ? groups : most;
-    if (sums && count > 1) partials = p.slot(mul_sat(mul_sat(count, extent), 8), kSlotScratch);
+    if (sums && count > 1) partials = p.slot(mul_sat(mul_sat(count, ceil_div(extent, 8) * 8), 8), kSlotScratch);
     std::snprintf(name, sizeof(name), "tiler_layer_norm_grad_%s_w%uc%u", type_name(dtype), waves,
                   pieces <= 1024 ? 1u : 2u);
     Launch& l = p.add(name, (uint32_t)count, 1, waves == 16 ? 1024 : 512).ptr(dy).ptr(x);
@@ -151,7 +151,7 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
     }
     if (!sums) return TILER_HIP_OK;
     count = ceil_div(rows, 16) < t.compute_units ? ceil_div(rows, 16) : t.compute_units;
-    partials = p.slot(mul_sat(mul_sat(count, extent), 8), kSlotScratch);
+    partials = p.slot(mul_sat(mul_sat(count, ceil_div(extent, 8) * 8), 8), kSlotScratch);
     std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_%s", type_name(dtype));
     p.add(name, (uint32_t)ceil_div(extent, 256), (uint32_t)count, 256)
         .ptr(dy).ptr(x).ptr(mean).ptr(rstd).u64(rows).u64(extent).u64(ceil_div(rows, count)).ptr(partials);
@@ -159,7 +159,7 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
     return TILER_HIP_OK;
   }
   std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_final_%s", type_name(dtype));
-  Launch& l = p.add(name, (uint32_t)ceil_div(2 * extent, 64), 1, 1024);
+  Launch& l = p.add(name, (uint32_t)ceil_div(extent, 64), 2, 1024);
   slot_or_null(l, count > 0, partials);  // no rows: zeros
   l.u32((uint32_t)count).u64(extent);
   slot_or_null(l, has_dw, dw);
