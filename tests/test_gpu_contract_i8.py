@@ -8,6 +8,7 @@ import pytest
 import feed_forward_reference as ref
 import oracle
 from tiler_amd import _lib as L
+from tiler_amd.realize import realize
 from test_gpu_layer_norm import CODE, Buffers, storage
 
 pytestmark = pytest.mark.gpu
@@ -106,6 +107,23 @@ SHAPES = [(1, 1, 1), (1, 16, 64), (1, 1000, 4096), (3, 5, 7), (16, 128, 256), (1
 @pytest.mark.parametrize("m,n,k", SHAPES)
 def test_product(ctx, mem, dtype, m, n, k):
     check_product(ctx, mem, m, n, k, dtype)
+
+
+# Every form of the product, shallower and deeper than the slices it keeps in LDS
+FORMS = [("few1x1", 3, 24, 1040), ("few2x1", 17, 2056, 1040), ("few2x2", 17, 4104, 1040), ("few4x2", 33, 4104, 1040),
+         ("few4x4", 33, 8200, 2064), ("t64_d", 33, 8200, 528), ("t64_d", 3, 20008, 1040), ("t96_d", 130, 12008, 2064),
+         ("t96", 3, 8200, 80), ("t96", 130, 12008, 1040), ("t128", 301, 8200, 16), ("t128", 200, 12008, 1040),
+         ("t192", 520, 14344, 16), ("t192", 400, 20008, 1040), ("t256", 1000, 12008, 16), ("t256", 1500, 8200, 1040),
+         ("g64", 70, 200, 333), ("g128", 600, 9000, 65)]
+
+
+@pytest.mark.parametrize("form,m,n,k", FORMS)
+def test_product_forms(ctx, mem, form, m, n, k):
+    for dtype in ("bf16", "f32"):
+        rz = realize(L.PROGRAM_CONTRACTION_I8, (m, n, k), dtype=CODE[dtype], permissions=L.PERMITS_REASSOCIATION,
+                     flags=L.REGION_ALIGNED16)
+        assert rz.symbols == [f"tiler_contract_i8_{dtype}_{form}"]
+        check_product(ctx, mem, m, n, k, dtype)
 
 
 @pytest.mark.parametrize("m,n,k", [(16, 128, 256), (100, 96, 512), (300, 264, 1024)])

@@ -7,6 +7,7 @@ import pytest
 import feed_forward_reference as ref
 import oracle
 from tiler_amd import _lib as L
+from tiler_amd.realize import realize
 from test_gpu_layer_norm import Buffers, within
 
 pytestmark = pytest.mark.gpu
@@ -96,6 +97,22 @@ def test_forward_whole_numbers(ctx, mem, m, n, k):
     got = forward(ctx, mem, bf(x), bf(wg), bf(wu), keep=True)
     for a, v in zip(got, (g * u, g, u)):
         assert np.array_equal(a, bf(v)), np.argwhere(a != bf(v))[:4]
+
+
+# Every form of the product, shallower and deeper than the slices it keeps in LDS
+FORMS = [("few1x1", 3, 24, 528), ("few2x1", 17, 2056, 1040), ("few4x1", 33, 2056, 1040), ("few4x2", 33, 4104, 1040),
+         ("t64_d", 33, 4104, 528), ("t64_d", 3, 14344, 528), ("t96_d", 70, 8200, 1040), ("t128_d", 100, 8200, 528),
+         ("t96", 17, 24, 16), ("t96", 17, 20008, 1040), ("t128", 301, 4104, 16), ("t128", 100, 20008, 1040),
+         ("t160", 400, 8200, 16), ("t160", 130, 8200, 1040), ("t192", 333, 12008, 16), ("t192", 333, 12008, 1040),
+         ("t256", 400, 12008, 16), ("t256", 400, 12008, 1040), ("g64", 70, 200, 333), ("g128", 300, 4099, 65)]
+
+
+@pytest.mark.parametrize("form,m,n,k", FORMS)
+def test_forward_forms(ctx, mem, form, m, n, k):
+    rz = realize(L.PROGRAM_GATED_CONTRACTION, (m, n, k), dtype=L.BF16, permissions=L.PERMITS_REASSOCIATION,
+                 flags=L.REGION_ALIGNED16)
+    assert rz.symbols == ["tiler_gated_bf16_" + form]
+    test_forward_whole_numbers(ctx, mem, m, n, k)
 
 
 def operands(rng, m, n, k):

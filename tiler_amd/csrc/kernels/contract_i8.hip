@@ -188,21 +188,25 @@ namespace {
 
 __device__ __forceinline__ float scaled(int32_t sum, float sa, float sb) { return tiler::canon((float)sum * sa * sb); }
 
-// Guarded form: 128 x 128 tiles, any sizes and alignments.
-template <bool kBf16>
+// Guarded form: 128 x 128 (or 64 x 128) tiles, any sizes and alignments.
+template <int MB, bool kBf16>
 __device__ __forceinline__ void contract_i8_guarded(const int8_t* __restrict__ a, const int8_t* __restrict__ b,
                                                     const float* __restrict__ sa, const float* __restrict__ sb,
                                                     uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * 256u * kSlice];
-  const uint32_t m0 = blockIdx.y * 128u, n0 = blockIdx.x * 128u;
-  const tiler_product::GuardedLoader<I8, false, 128, 256> la(Operand{reinterpret_cast<const uint8_t*>(a), k, m, k}, m0);
-  const tiler_product::GuardedLoader<I8, false, 128, 256> lb(Operand{reinterpret_cast<const uint8_t*>(b), k, n, k}, n0);
-  i32x4 acc[4][4];
-  tiler_product::guarded_product<I8, false, false, 2, 2, 4, 4>(
-      smem, (k + 127u) / 128u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
-      [&](uint32_t t, u32x4(&v)[4]) { lb.load(lb.o.base, t, v); },
-      [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
-      [&](uint8_t* tile, const u32x4(&v)[4]) { lb.store(tile, v); }, acc);
+  constexpr uint32_t kRows = 2u * MB * 16u;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRows + 128u) * kSlice];
+  const uint32_t m0 = blockIdx.y * kRows, n0 = blockIdx.x * 128u;
+  const Operand oa{reinterpret_cast<const uint8_t*>(a), k, m, k}, ob{reinterpret_cast<const uint8_t*>(b), k, n, k};
+  i32x4 acc[MB][4];
+  auto product = [&](const auto& la, const auto& lb) {
+    tiler_product::guarded_product<I8, false, false, 2, 2, MB, 4>(
+        smem, (k + 127u) / 128u, [&](uint32_t t, u32x4(&v)[MB]) { la.load(oa.base, t, v); },
+        [&](uint32_t t, u32x4(&v)[4]) { lb.load(ob.base, t, v); },
+        [&](uint32_t t, uint8_t* tile, u32x4(&v)[MB]) { la.store(t, tile, v); },
+        [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { lb.store(t, tile, v); }, acc);
+  };
+  if (k >= 16u) product(tiler_product::GuardedLoader<I8, false, kRows, 256>(oa, m0), tiler_product::GuardedLoader<I8, false, 128, 256>(ob, n0));
+  else product(tiler_product::TinyLoader<I8, false, kRows, 256>(oa, m0), tiler_product::TinyLoader<I8, false, 128, 256>(ob, n0));
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -210,10 +214,10 @@ __device__ __forceinline__ void contract_i8_guarded(const int8_t* __restrict__ a
     if (col >= n) continue;
     const float cs = sb[col];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t row = m0 + (wave >> 1) * 64u + i * 16u + (lane >> 4) * 4u + r;
+        const uint32_t row = m0 + (wave >> 1) * MB * 16u + i * 16u + (lane >> 4) * 4u + r;
         if (row >= m) continue;
         const float v = scaled(acc[i][j][r], sa[row], cs);
         const uint64_t at = (uint64_t)row * n + col;
@@ -225,28 +229,29 @@ __device__ __forceinline__ void contract_i8_guarded(const int8_t* __restrict__ a
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256, 2)
-tiler_contract_i8_bf16_g(const int8_t* __restrict__ a, const int8_t* __restrict__ b, const float* __restrict__ sa,
-                         const float* __restrict__ sb, uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
-  contract_i8_guarded<true>(a, b, sa, sb, m, n, k, c);
-}
-extern "C" __global__ void __launch_bounds__(256, 2)
-tiler_contract_i8_f32_g(const int8_t* __restrict__ a, const int8_t* __restrict__ b, const float* __restrict__ sa,
-                        const float* __restrict__ sb, uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
-  contract_i8_guarded<false>(a, b, sa, sb, m, n, k, c);
-}
+#define TILER_CONTRACT_I8_GUARDED(TY, BF16, TILE, MB)                                                              \
+  extern "C" __global__ void __launch_bounds__(256, 2)                                                             \
+      tiler_contract_i8_##TY##_g##TILE(const int8_t* __restrict__ a, const int8_t* __restrict__ b,                 \
+                                       const float* __restrict__ sa, const float* __restrict__ sb, uint32_t m,     \
+                                       uint32_t n, uint32_t k, void* __restrict__ c) {                             \
+    contract_i8_guarded<MB, BF16>(a, b, sa, sb, m, n, k, c);                                                       \
+  }
+TILER_CONTRACT_I8_GUARDED(bf16, true, 128, 4)
+TILER_CONTRACT_I8_GUARDED(f32, false, 128, 4)
+TILER_CONTRACT_I8_GUARDED(bf16, true, 64, 2)
+TILER_CONTRACT_I8_GUARDED(f32, false, 64, 2)
 
 // ---------------------------------------------------------------------------
 // Staged form: k a multiple of 16 and 16-byte aligned operands.
 namespace {
 
-template <int WM, int WN, int MB, bool kBf16>
+template <int WM, int WN, int MB, int S, bool kBf16>
 __device__ __forceinline__ void contract_i8_staged(const int8_t* __restrict__ a, const int8_t* __restrict__ b,
                                                    const float* __restrict__ sa, const float* __restrict__ sb,
                                                    uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kRowsB = WN * 64u, kThreads = 64u * WM * WN;
   constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kRowsB / 8 / (WM * WN);
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kRowsB) * kSlice];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * (kRowsA + kRowsB) * kSlice];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t tm, tn;
   tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (n + kRowsB - 1u) / kRowsB, tm, tn);
@@ -258,7 +263,7 @@ __device__ __forceinline__ void contract_i8_staged(const int8_t* __restrict__ a,
                                                  n - n0 < kRowsB ? n - n0 : kRowsB, k, wave * kLoadsB * 8u,
                                                  wave * kLoadsB * 8u, lane);
   i32x4 acc[MB][4];
-  tiler_product::staged_product<I8, false, false, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+  tiler_product::staged_product<I8, false, false, WM, WN, MB, 4, kLoadsA + kLoadsB, S>(
       smem, (k + 127u) / 128u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
       [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
   const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 64u;
@@ -296,70 +301,91 @@ __device__ __forceinline__ void contract_i8_staged(const int8_t* __restrict__ a,
 
 }  // namespace
 
-#define TILER_CONTRACT_I8_STAGED(TY, BF16, TILE, WM, WN, MB)                                                       \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                          \
-      tiler_contract_i8_##TY##_t##TILE(const int8_t* __restrict__ a, const int8_t* __restrict__ b,                 \
+// Four waves: two workgroups to a CU; eight: one.  Two waves a SIMD in either.
+// The deep forms (_d) keep as many slices in LDS as it holds, for the grids that
+// give a CU one workgroup.
+#define TILER_CONTRACT_I8_STAGED(TY, BF16, NAME, WN, MB, S)                                                        \
+  extern "C" __global__ void __launch_bounds__(S > 2 ? 512 : 128 * WN, 2)                                       \
+      tiler_contract_i8_##TY##_t##NAME(const int8_t* __restrict__ a, const int8_t* __restrict__ b,                 \
                                        const float* __restrict__ sa, const float* __restrict__ sb, uint32_t m,     \
                                        uint32_t n, uint32_t k, void* __restrict__ c) {                             \
-    contract_i8_staged<WM, WN, MB, BF16>(a, b, sa, sb, m, n, k, c);                                                \
+    contract_i8_staged<2, WN, MB, S, BF16>(a, b, sa, sb, m, n, k, c);                                              \
   }
-TILER_CONTRACT_I8_STAGED(bf16, true, 256, 2, 4, 8)
-TILER_CONTRACT_I8_STAGED(f32, false, 256, 2, 4, 8)
-TILER_CONTRACT_I8_STAGED(bf16, true, 128, 2, 2, 4)
-TILER_CONTRACT_I8_STAGED(f32, false, 128, 2, 2, 4)
+#define TILER_CONTRACT_I8_TILES(TY, BF16)             \
+  TILER_CONTRACT_I8_STAGED(TY, BF16, 96, 2, 3, 2)     \
+  TILER_CONTRACT_I8_STAGED(TY, BF16, 128, 2, 4, 2)    \
+  TILER_CONTRACT_I8_STAGED(TY, BF16, 192, 4, 6, 2)    \
+  TILER_CONTRACT_I8_STAGED(TY, BF16, 256, 4, 8, 2)    \
+  TILER_CONTRACT_I8_STAGED(TY, BF16, 64_d, 2, 2, 6)   \
+  TILER_CONTRACT_I8_STAGED(TY, BF16, 96_d, 2, 3, 5)
+TILER_CONTRACT_I8_TILES(bf16, true)
+TILER_CONTRACT_I8_TILES(f32, false)
 
 // ---------------------------------------------------------------------------
-// Few rows (m <= 64): the bytes of b.  A workgroup takes 16 columns, its 8
-// waves the depth in turn.
+// Few rows: the bytes of b.  A workgroup takes 16 MB rows and 16 NB columns, its
+// 8 waves the depth in turn.
 namespace {
 
-template <int MB, bool kBf16>
+// The results of MB x NB blocks from their sums.
+template <int MB, int NB, bool kBf16, typename T>
+__device__ __forceinline__ void contract_i8_finish(T total, const float* __restrict__ sa, const float* __restrict__ sb,
+                                                   uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
+                                                   void* __restrict__ c) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  for (uint32_t q = wave; q < (uint32_t)(MB * NB); q += 8u) {
+    const i32x4 v = total(q);
+    const uint32_t col = n0 + q % NB * 16u + (lane & 15u);
+    if (col >= n) continue;
+    const float cs = sb[col];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t row = m0 + q / NB * 16u + (lane >> 4) * 4u + r;
+      if (row >= m) continue;
+      const float f = scaled(v[r], sa[row], cs);
+      const uint64_t at = (uint64_t)row * n + col;
+      if constexpr (kBf16) static_cast<uint16_t*>(c)[at] = (uint16_t)tiler::bf16_narrow(f);
+      else static_cast<float*>(c)[at] = f;
+    }
+  }
+}
+
+template <int MB, int NB, bool kBf16>
 __device__ __forceinline__ void contract_i8_few(const int8_t* __restrict__ a, const int8_t* __restrict__ b,
                                                 const float* __restrict__ sa, const float* __restrict__ sb, uint32_t m,
                                                 uint32_t n, uint32_t k, void* __restrict__ c) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[tiler_product::few_rows_lds<MB, 1, 8>()];
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16u;
-  const tiler_product::RowLoader<I8, 2 * MB> la(reinterpret_cast<const uint8_t*>(a), k, m, k, 0, 0, lane);
-  const tiler_product::RowLoader<I8, 2> lb(reinterpret_cast<const uint8_t*>(b + (uint64_t)n0 * k), k,
-                                           n - n0 < 16u ? n - n0 : 16u, k, 0, 0, lane);
-  tiler_product::few_rows_product<I8, MB, 1, 8>(
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[tiler_product::few_rows_lds<MB, NB, 8>()];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  uint32_t tm, tn;
+  tiler_product::panel_of(blockIdx.x, (m + MB * 16u - 1u) / (MB * 16u), (n + NB * 16u - 1u) / (NB * 16u), tm, tn);
+  if (tn * NB * 16u >= n) return;
+  const uint32_t m0 = tm * MB * 16u, n0 = tn * NB * 16u;
+  const tiler_product::RowLoader<I8, 2 * MB> la(reinterpret_cast<const uint8_t*>(a + (uint64_t)m0 * k), k,
+                                                m - m0 < MB * 16u ? m - m0 : MB * 16u, k, 0, 0, lane);
+  const tiler_product::RowLoader<I8, 2 * NB> lb(reinterpret_cast<const uint8_t*>(b + (uint64_t)n0 * k), k,
+                                                n - n0 < NB * 16u ? n - n0 : NB * 16u, k, 0, 0, lane);
+  tiler_product::few_rows_product<I8, MB, NB, 8>(
       smem, (k + 127u) / 128u,
       [&](uint32_t t, uint8_t* slot) {
         lb.issue(t, slot + MB * 16u * kSlice);
         la.issue(t, slot);
       },
-      [&](auto total) {
-        if (wave >= (uint32_t)MB) return;
-        const i32x4 v = total(wave);
-        const uint32_t col = n0 + (lane & 15u);
-        if (col >= n) return;
-        const float cs = sb[col];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t row = wave * 16u + (lane >> 4) * 4u + r;
-          if (row >= m) continue;
-          const float f = scaled(v[r], sa[row], cs);
-          const uint64_t at = (uint64_t)row * n + col;
-          if constexpr (kBf16) static_cast<uint16_t*>(c)[at] = (uint16_t)tiler::bf16_narrow(f);
-          else static_cast<float*>(c)[at] = f;
-        }
-      });
+      [&](auto total) { contract_i8_finish<MB, NB, kBf16>(total, sa, sb, m, n, m0, n0, c); });
 }
 
 }  // namespace
 
-#define TILER_CONTRACT_I8_FEW(TY, BF16, MB)                                                                        \
+#define TILER_CONTRACT_I8_FEW(TY, BF16, MB, NB)                                                                    \
   extern "C" __global__ void __launch_bounds__(512)                                                                \
-      tiler_contract_i8_##TY##_few##MB(const int8_t* __restrict__ a, const int8_t* __restrict__ b,                 \
-                                       const float* __restrict__ sa, const float* __restrict__ sb, uint32_t m,     \
-                                       uint32_t n, uint32_t k, void* __restrict__ c) {                             \
-    contract_i8_few<MB, BF16>(a, b, sa, sb, m, n, k, c);                                                           \
+      tiler_contract_i8_##TY##_few##MB##x##NB(const int8_t* __restrict__ a, const int8_t* __restrict__ b,          \
+                                              const float* __restrict__ sa, const float* __restrict__ sb,          \
+                                              uint32_t m, uint32_t n, uint32_t k, void* __restrict__ c) {          \
+    contract_i8_few<MB, NB, BF16>(a, b, sa, sb, m, n, k, c);                                                       \
   }
-TILER_CONTRACT_I8_FEW(bf16, true, 1)
-TILER_CONTRACT_I8_FEW(bf16, true, 2)
-TILER_CONTRACT_I8_FEW(bf16, true, 3)
-TILER_CONTRACT_I8_FEW(bf16, true, 4)
-TILER_CONTRACT_I8_FEW(f32, false, 1)
-TILER_CONTRACT_I8_FEW(f32, false, 2)
-TILER_CONTRACT_I8_FEW(f32, false, 3)
-TILER_CONTRACT_I8_FEW(f32, false, 4)
+#define TILER_CONTRACT_I8_FEW_FORMS(TY, BF16) \
+  TILER_CONTRACT_I8_FEW(TY, BF16, 1, 1)       \
+  TILER_CONTRACT_I8_FEW(TY, BF16, 2, 1)       \
+  TILER_CONTRACT_I8_FEW(TY, BF16, 2, 2)       \
+  TILER_CONTRACT_I8_FEW(TY, BF16, 4, 2)       \
+  TILER_CONTRACT_I8_FEW(TY, BF16, 4, 4)
+TILER_CONTRACT_I8_FEW_FORMS(bf16, true)
+TILER_CONTRACT_I8_FEW_FORMS(f32, false)

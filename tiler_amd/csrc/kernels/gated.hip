@@ -31,48 +31,53 @@ __device__ __forceinline__ float sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -0x1.715476p+0f));
 }
 
-// Guarded form: 128 tokens x (64 gate + 64 up) columns, any sizes and
+// Guarded form: 128 (or 64) tokens x (64 gate + 64 up) columns, any sizes and
 // alignments.  Row r of the B tile: gate (r & 32 == 0) or up row
 // (r >> 6) * 32 + (r & 31) of the 64-column tile.
 constexpr int kW = 2, kMB = 4, kNB = 4;  // 2 x 2 waves of 4 x 4 blocks
 constexpr uint32_t kGuardedBytes = 2u * 256u * kSlice;
 
-}  // namespace
-
-extern "C" __global__ void __launch_bounds__(256, 2)
-tiler_gated_bf16_g(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu,
-                   uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
-                   uint16_t* __restrict__ up) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
-  const uint32_t m0 = blockIdx.y * 128u, n0 = blockIdx.x * 64u;
+template <int MB>
+__device__ __forceinline__ void gated_guarded(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
+                                              const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
+                                              uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
+                                              uint16_t* __restrict__ up) {
+  constexpr uint32_t kRows = kW * MB * 16u;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRows + 128u) * kSlice];
+  const uint32_t m0 = blockIdx.y * kRows, n0 = blockIdx.x * 64u;
   // thread t's pieces of B are rows t / 8 + 32 q of its tile: gate rows for even q, up rows for odd
-  const tiler_product::GuardedLoader<Bf16, false, 128, 256> la(Operand{reinterpret_cast<const uint8_t*>(x), k, m, k}, m0);
-  const tiler_product::GuardedLoader<Bf16, false, 64, 256> lb(Operand{reinterpret_cast<const uint8_t*>(wg), k, n, k}, n0);
-  f32x4 acc[kMB][kNB];
-  tiler_product::guarded_product<Bf16, false, false, kW, kW, kMB, kNB>(
-      smem, (k + 63u) / 64u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
-      [&](uint32_t t, u32x4(&v)[4]) {
-        u32x4 g[2], u[2];
-        lb.load(reinterpret_cast<const uint8_t*>(wg), t, g);
-        lb.load(reinterpret_cast<const uint8_t*>(wu), t, u);
-        v[0] = g[0], v[1] = u[0], v[2] = g[1], v[3] = u[1];
-      },
-      [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
-      [&](uint8_t* tile, const u32x4(&v)[4]) {
-#pragma unroll
-        for (uint32_t q = 0; q < 4; ++q)
-          *reinterpret_cast<u32x4*>(tile + tiler_product::piece_offset<128, false>(threadIdx.x / 8u + 32u * q,
-                                                                                  threadIdx.x % 8u)) = v[q];
-      },
-      acc);
+  const Operand a{reinterpret_cast<const uint8_t*>(x), k, m, k}, b{reinterpret_cast<const uint8_t*>(wg), k, n, k};
+  f32x4 acc[MB][kNB];
+  // (lb fetches 64 rows of either weight, whole lays the 128 of the tile out)
+  auto product = [&](const auto& la, const auto& lb, const auto& whole) {
+    tiler_product::guarded_product<Bf16, false, false, kW, kW, MB, kNB>(
+        smem, (k + 63u) / 64u, [&](uint32_t t, u32x4(&v)[MB]) { la.load(a.base, t, v); },
+        [&](uint32_t t, u32x4(&v)[4]) {
+          u32x4 g[2], u[2];
+          lb.load(reinterpret_cast<const uint8_t*>(wg), t, g);
+          lb.load(reinterpret_cast<const uint8_t*>(wu), t, u);
+          v[0] = g[0], v[1] = u[0], v[2] = g[1], v[3] = u[1];
+        },
+        [&](uint32_t t, uint8_t* tile, u32x4(&v)[MB]) { la.store(t, tile, v); },
+        [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { whole.store(t, tile, v); },
+        acc);
+  };
+  using tiler_product::GuardedLoader;
+  using tiler_product::TinyLoader;
+  if (k >= 8u)
+    product(GuardedLoader<Bf16, false, kRows, 256>(a, m0), GuardedLoader<Bf16, false, 64, 256>(b, n0),
+            GuardedLoader<Bf16, false, 128, 256>(b, n0));
+  else
+    product(TinyLoader<Bf16, false, kRows, 256>(a, m0), TinyLoader<Bf16, false, 64, 256>(b, n0),
+            TinyLoader<Bf16, false, 128, 256>(b, n0));
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int i = 0; i < kMB; ++i)
+  for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t row = m0 + (wave / kW) * 64u + i * 16u + (lane >> 4) * 4u + r;
+        const uint32_t row = m0 + (wave / kW) * MB * 16u + i * 16u + (lane >> 4) * 4u + r;
         const uint32_t col = n0 + (wave % kW) * 32u + j * 16u + (lane & 15u);
         if (row >= m || col >= n) continue;
         const float g = acc[i][j][r], u = acc[i][j + 2][r];
@@ -83,6 +88,22 @@ tiler_gated_bf16_g(const uint16_t* __restrict__ x, const uint16_t* __restrict__ 
           up[at] = (uint16_t)tiler::bf16_narrow(u);
         }
       }
+}
+
+}  // namespace
+
+// Tiles of 128 and of 64 tokens.
+extern "C" __global__ void __launch_bounds__(256, 2)
+tiler_gated_bf16_g128(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu,
+                      uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
+                      uint16_t* __restrict__ up) {
+  gated_guarded<4>(x, wg, wu, m, n, k, h, gate, up);
+}
+extern "C" __global__ void __launch_bounds__(256, 2)
+tiler_gated_bf16_g64(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu,
+                     uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
+                     uint16_t* __restrict__ up) {
+  gated_guarded<2>(x, wg, wu, m, n, k, h, gate, up);
 }
 
 // dG and dU of one row's eight columns per thread, into rows of `ld` elements
@@ -172,20 +193,23 @@ tiler_gated_bf16_dx_g(const uint16_t* __restrict__ dg, const uint16_t* __restric
     // dG's rows hold zeros from n to ld
     const tiler_product::GuardedLoader<Bf16, false, 128, 256> la(
         Operand{reinterpret_cast<const uint8_t*>(dg), ld, m, ld}, m0);
-    const tiler_product::GuardedLoader<Bf16, true, 128, 256> lb(Operand{reinterpret_cast<const uint8_t*>(wg), k, k, n},
-                                                                c0);
-    tiler_product::guarded_product<Bf16, false, true, kW, kW, kMB, kNB>(
-        smem, t1 - t0,
-        [&](uint32_t t, u32x4(&v)[4]) {
-          const bool first = t + t0 < per;
-          la.load(reinterpret_cast<const uint8_t*>(first ? dg : du), first ? t + t0 : t + t0 - per, v);
-        },
-        [&](uint32_t t, u32x4(&v)[4]) {
-          const bool first = t + t0 < per;
-          lb.load(reinterpret_cast<const uint8_t*>(first ? wg : wu), first ? t + t0 : t + t0 - per, v);
-        },
-        [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
-        [&](uint8_t* tile, const u32x4(&v)[4]) { lb.store(tile, v); }, acc);
+    const Operand b{reinterpret_cast<const uint8_t*>(wg), k, k, n};
+    auto product = [&](const auto& lb) {
+      tiler_product::guarded_product<Bf16, false, true, kW, kW, kMB, kNB>(
+          smem, t1 - t0,
+          [&](uint32_t t, u32x4(&v)[4]) {
+            const bool first = t + t0 < per;
+            la.load(reinterpret_cast<const uint8_t*>(first ? dg : du), first ? t + t0 : t + t0 - per, v);
+          },
+          [&](uint32_t t, u32x4(&v)[4]) {
+            const bool first = t + t0 < per;
+            lb.load(reinterpret_cast<const uint8_t*>(first ? wg : wu), first ? t + t0 : t + t0 - per, v);
+          },
+          [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { la.store(t + t0 < per ? t + t0 : t + t0 - per, tile, v); },
+          [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { lb.store(t + t0 < per ? t + t0 : t + t0 - per, tile, v); }, acc);
+    };
+    if (k >= 8u) product(tiler_product::GuardedLoader<Bf16, true, 128, 256>(b, c0));
+    else product(tiler_product::TinyLoader<Bf16, true, 128, 256>(b, c0));
   }
   const uint32_t wave = threadIdx.x >> 6, row0 = m0 + (wave / kW) * 64u, col0 = c0 + (wave % kW) * 64u;
   if (splits > 1) {
@@ -216,15 +240,20 @@ tiler_gated_bf16_dw_g(const uint16_t* __restrict__ dg, const uint16_t* __restric
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
   const bool second = blockIdx.y >= tiles_n;
   const uint32_t j0 = (second ? blockIdx.y - tiles_n : blockIdx.y) * 128u, c0 = blockIdx.x * 128u;
+  // dG's and dU's rows are ld long: whole pieces
   const tiler_product::GuardedLoader<Bf16, true, 128, 256> la(
-      Operand{reinterpret_cast<const uint8_t*>(second ? du : dg), ld, n, m}, j0);
-  const tiler_product::GuardedLoader<Bf16, true, 128, 256> lb(Operand{reinterpret_cast<const uint8_t*>(x), k, k, m}, c0);
+      Operand{reinterpret_cast<const uint8_t*>(second ? du : dg), ld, ld, m}, j0);
+  const Operand b{reinterpret_cast<const uint8_t*>(x), k, k, m};
   f32x4 acc[kMB][kNB];
-  tiler_product::guarded_product<Bf16, true, true, kW, kW, kMB, kNB>(
-      smem, (m + 63u) / 64u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
-      [&](uint32_t t, u32x4(&v)[4]) { lb.load(lb.o.base, t, v); },
-      [&](uint8_t* tile, const u32x4(&v)[4]) { la.store(tile, v); },
-      [&](uint8_t* tile, const u32x4(&v)[4]) { lb.store(tile, v); }, acc);
+  auto product = [&](const auto& lb) {
+    tiler_product::guarded_product<Bf16, true, true, kW, kW, kMB, kNB>(
+        smem, (m + 63u) / 64u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
+        [&](uint32_t t, u32x4(&v)[4]) { lb.load(b.base, t, v); },
+        [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { la.store(t, tile, v); },
+        [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { lb.store(t, tile, v); }, acc);
+  };
+  if (k >= 8u) product(tiler_product::GuardedLoader<Bf16, true, 128, 256>(b, c0));
+  else product(tiler_product::TinyLoader<Bf16, true, 128, 256>(b, c0));
   const uint32_t wave = threadIdx.x >> 6;
   tiler_product::store_tile_bf16<128, 128, 256, kMB, kNB>(smem, (wave / kW) * 64u, (wave % kW) * 64u,
                                                           second ? dwu : dwg, n, k, j0, c0,
@@ -236,7 +265,7 @@ tiler_gated_bf16_dw_g(const uint16_t* __restrict__ dg, const uint16_t* __restric
 // of MB x 4 blocks.
 namespace {
 
-template <int WM, int WN, int MB>
+template <int WM, int WN, int MB, int S>
 __device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
                                              const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
                                              uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
@@ -244,7 +273,7 @@ __device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, con
   constexpr uint32_t kRowsA = WM * MB * 16u, kRowsB = WN * 64u, kCols = kRowsB / 2u, kThreads = 64u * WM * WN;
   constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kRowsB / 8 / (WM * WN);
   static_assert(kLoadsB == 4, "a wave's 32 rows of B lie in one of the two weights");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kRowsB) * kSlice];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * (kRowsA + kRowsB) * kSlice];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t tm, tn;
   tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (n + kCols - 1u) / kCols, tm, tn);
@@ -257,7 +286,7 @@ __device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, con
       reinterpret_cast<const uint8_t*>(((wave & 1u) ? wu : wg) + (uint64_t)n0 * k), k, n - n0 < kCols ? n - n0 : kCols,
       k, (wave >> 1) * 32u, wave * 32u, lane);
   f32x4 acc[MB][4];
-  tiler_product::staged_product<Bf16, false, false, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+  tiler_product::staged_product<Bf16, false, false, WM, WN, MB, 4, kLoadsA + kLoadsB, S>(
       smem, (k + 63u) / 64u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
       [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
   const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 32u;
@@ -294,7 +323,7 @@ __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg,
   const uint8_t* const a2 = reinterpret_cast<const uint8_t*>(du + (uint64_t)m0 * ld);
   const uint8_t* const b2 = reinterpret_cast<const uint8_t*>(wu + c0);
   f32x4 acc[MB][4];
-  tiler_product::staged_product<Bf16, false, true, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+  tiler_product::staged_product<Bf16, false, true, WM, WN, MB, 4, kLoadsA + kLoadsB, 2>(
       smem, t1 - t0,
       [&](uint32_t t, uint8_t* at) {
         const bool first = t + t0 < per;
@@ -332,7 +361,7 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
                                                         m, wave, lane);
   const tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(x + c0), k, c0, m, wave, lane);
   f32x4 acc[MB][4];
-  tiler_product::staged_product<Bf16, true, true, WM, WN, MB, 4, kLoadsA + kLoadsB>(
+  tiler_product::staged_product<Bf16, true, true, WM, WN, MB, 4, kLoadsA + kLoadsB, 2>(
       smem, (m + 63u) / 64u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
       [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
   __syncthreads();
@@ -343,80 +372,114 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
 
 }  // namespace
 
-#define TILER_GATED_STAGED(TILE, WM, WN, MB)                                                                        \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
-      tiler_gated_bf16_t##TILE(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,                     \
+// Four waves: two workgroups to a CU; eight: one.  Two waves a SIMD in either.
+// The deep forms (_d) keep as many slices in LDS as it holds, for the grids that
+// give a CU one workgroup: there a slice's time is its loads' latency over the
+// slices in flight.  (Their bound of 512 threads, of which 256 run, keeps the
+// compiler to 256 registers: given 512, it spreads them over the accumulation
+// registers and copies them back and forth.)
+#define TILER_GATED_TILES(NAME, WN, MB, S)                                                                          \
+  extern "C" __global__ void __launch_bounds__(S > 2 ? 512 : 128 * WN, 2)                                       \
+      tiler_gated_bf16_t##NAME(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,                     \
                                const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,                 \
                                uint16_t* __restrict__ h, uint16_t* __restrict__ gate, uint16_t* __restrict__ up) {  \
-    gated_staged<WM, WN, MB>(x, wg, wu, m, n, k, h, gate, up);                                                      \
-  }                                                                                                                 \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
+    gated_staged<2, WN, MB, S>(x, wg, wu, m, n, k, h, gate, up);                                                    \
+  }
+#define TILER_GATED_DX_STAGED(TILE, WN, MB)                                                                         \
+  extern "C" __global__ void __launch_bounds__(128 * WN, 2)                                                         \
       tiler_gated_bf16_dx_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
                                   const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m,     \
                                   uint32_t n, uint32_t k, uint16_t* __restrict__ dx, uint32_t splits,               \
                                   float* __restrict__ partials) {                                                   \
-    gated_dx_staged<WM, WN, MB>(dg, du, ld, wg, wu, m, n, k, dx, splits, partials);                                 \
-  }                                                                                                                 \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4)                                           \
+    gated_dx_staged<2, WN, MB>(dg, du, ld, wg, wu, m, n, k, dx, splits, partials);                                  \
+  }
+#define TILER_GATED_DW_STAGED(TILE, WN, MB)                                                                         \
+  extern "C" __global__ void __launch_bounds__(128 * WN, 2)                                                         \
       tiler_gated_bf16_dw_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
                                   const uint16_t* __restrict__ x, uint32_t m, uint32_t n, uint32_t k,               \
                                   uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {                         \
-    gated_dw_staged<WM, WN, MB>(dg, du, ld, x, m, n, k, dwg, dwu);                                                  \
+    gated_dw_staged<2, WN, MB>(dg, du, ld, x, m, n, k, dwg, dwu);                                                   \
   }
-TILER_GATED_STAGED(256, 2, 4, 8)
-TILER_GATED_STAGED(128, 2, 2, 4)
+TILER_GATED_TILES(96, 2, 3, 2)
+TILER_GATED_TILES(128, 2, 4, 2)
+TILER_GATED_TILES(160, 2, 5, 2)
+TILER_GATED_TILES(192, 4, 6, 2)
+TILER_GATED_TILES(256, 4, 8, 2)
+TILER_GATED_TILES(64_d, 2, 2, 6)
+TILER_GATED_TILES(96_d, 2, 3, 5)
+TILER_GATED_TILES(128_d, 2, 4, 4)
+TILER_GATED_DX_STAGED(128, 2, 4)
+TILER_GATED_DX_STAGED(256, 4, 8)
+TILER_GATED_DW_STAGED(128, 2, 4)
+TILER_GATED_DW_STAGED(256, 4, 8)
 
 // ---------------------------------------------------------------------------
-// Few tokens (m <= 64): the weights' bytes.  A workgroup takes 16 columns of
-// both projections, its 8 waves the depth in turn.
+// Few tokens: the weights' bytes.  A workgroup takes 16 MB tokens and 16 P
+// columns of both projections, its 8 waves the depth in turn.
 namespace {
 
-template <int MB>
+// The results of MB x P blocks from their gate and up sums (a row of blocks: P
+// gate blocks, then P up blocks).
+template <int MB, int P, typename T>
+__device__ __forceinline__ void gated_finish(T total, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
+                                             uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
+                                             uint16_t* __restrict__ up) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  for (uint32_t q = wave; q < (uint32_t)(MB * P); q += 8u) {
+    const uint32_t i = q / P, j = q % P;
+    const f32x4 g = total(i * 2u * P + j), u = total(i * 2u * P + P + j);
+    const uint32_t col = n0 + j * 16u + (lane & 15u);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t row = m0 + i * 16u + (lane >> 4) * 4u + r;
+      if (row >= m || col >= n) continue;
+      const uint64_t at = (uint64_t)row * n + col;
+      h[at] = (uint16_t)tiler::bf16_narrow(g[r] * sigmoid(g[r]) * u[r]);
+      if (gate) {
+        gate[at] = (uint16_t)tiler::bf16_narrow(g[r]);
+        up[at] = (uint16_t)tiler::bf16_narrow(u[r]);
+      }
+    }
+  }
+}
+
+template <int MB, int P>
 __device__ __forceinline__ void gated_few(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
                                           const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
                                           uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
                                           uint16_t* __restrict__ up) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[tiler_product::few_rows_lds<MB, 2, 8>()];
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16u;
-  const uint32_t cols = n - n0 < 16u ? n - n0 : 16u;
-  const tiler_product::RowLoader<Bf16, 2 * MB> la(reinterpret_cast<const uint8_t*>(x), k, m, k, 0, 0, lane);
-  const tiler_product::RowLoader<Bf16, 2> lg(reinterpret_cast<const uint8_t*>(wg + (uint64_t)n0 * k), k, cols, k, 0, 0, lane);
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[tiler_product::few_rows_lds<MB, 2 * P, 8>()];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  uint32_t tm, tn;
+  tiler_product::panel_of(blockIdx.x, (m + MB * 16u - 1u) / (MB * 16u), (n + P * 16u - 1u) / (P * 16u), tm, tn);
+  if (tn * P * 16u >= n) return;
+  const uint32_t m0 = tm * MB * 16u, n0 = tn * P * 16u, cols = n - n0 < P * 16u ? n - n0 : P * 16u;
+  const tiler_product::RowLoader<Bf16, 2 * MB> la(reinterpret_cast<const uint8_t*>(x + (uint64_t)m0 * k), k,
+                                                  m - m0 < MB * 16u ? m - m0 : MB * 16u, k, 0, 0, lane);
+  const tiler_product::RowLoader<Bf16, 2 * P> lg(reinterpret_cast<const uint8_t*>(wg + (uint64_t)n0 * k), k, cols, k, 0, 0,
+                                                 lane);
   const uint8_t* const u0 = reinterpret_cast<const uint8_t*>(wu + (uint64_t)n0 * k);
-  tiler_product::few_rows_product<Bf16, MB, 2, 8>(
+  tiler_product::few_rows_product<Bf16, MB, 2 * P, 8>(
       smem, (k + 63u) / 64u,
       [&](uint32_t t, uint8_t* slot) {
         lg.issue(t, slot + MB * 16u * kSlice);
-        lg.issue(u0, t, slot + (MB + 1) * 16u * kSlice);
+        lg.issue(u0, t, slot + (MB + P) * 16u * kSlice);
         la.issue(t, slot);
       },
-      [&](auto total) {
-        if (wave >= (uint32_t)MB) return;
-        const f32x4 g = total(2u * wave), u = total(2u * wave + 1u);
-        const uint32_t col = n0 + (lane & 15u);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t row = wave * 16u + (lane >> 4) * 4u + r;
-          if (row >= m || col >= n) continue;
-          const uint64_t at = (uint64_t)row * n + col;
-          h[at] = (uint16_t)tiler::bf16_narrow(g[r] * sigmoid(g[r]) * u[r]);
-          if (gate) {
-            gate[at] = (uint16_t)tiler::bf16_narrow(g[r]);
-            up[at] = (uint16_t)tiler::bf16_narrow(u[r]);
-          }
-        }
-      });
+      [&](auto total) { gated_finish<MB, P>(total, m, n, m0, n0, h, gate, up); });
 }
 
 }  // namespace
 
-#define TILER_GATED_FEW(MB)                                                                                        \
+#define TILER_GATED_FEW(MB, P)                                                                                     \
   extern "C" __global__ void __launch_bounds__(512)                                                                \
-      tiler_gated_bf16_few##MB(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,                    \
-                               const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,                \
-                               uint16_t* __restrict__ h, uint16_t* __restrict__ gate, uint16_t* __restrict__ up) { \
-    gated_few<MB>(x, wg, wu, m, n, k, h, gate, up);                                                                \
+      tiler_gated_bf16_few##MB##x##P(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,              \
+                                     const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,          \
+                                     uint16_t* __restrict__ h, uint16_t* __restrict__ gate,                        \
+                                     uint16_t* __restrict__ up) {                                                  \
+    gated_few<MB, P>(x, wg, wu, m, n, k, h, gate, up);                                                             \
   }
-TILER_GATED_FEW(1)
-TILER_GATED_FEW(2)
-TILER_GATED_FEW(3)
-TILER_GATED_FEW(4)
+TILER_GATED_FEW(1, 1)
+TILER_GATED_FEW(2, 1)
+TILER_GATED_FEW(4, 1)
+TILER_GATED_FEW(4, 2)

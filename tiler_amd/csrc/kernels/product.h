@@ -118,52 +118,69 @@ __device__ __forceinline__ u32x4 operand_piece(const Operand& o, uint32_t row0, 
 }
 
 // The guarded product, for any sizes and alignments: pieces come through
-// registers, two slices ahead of the products.  A loader's pieces of a slice
-// lie at fixed offsets from a base that moves along the depth; only the last
-// slice of an operand is checked piece by piece (zero past the depth).  In the
-// others a row past the last reads the last one, and a column piece past the
-// row's end reads on into the next depth row: both only reach results that are
-// not stored.  (The reading on needs rows of at least a piece; narrower ones
-// are checked throughout.)
+// registers, two slices ahead of the products.  A loader's load is free of
+// branches, so that nothing waits between the loads: a piece that would pass
+// its row's end (or its depth row's) is the last whole one inside it, a row or
+// depth row past the last is the last one again.  store puts the pieces into
+// LDS and, in the slices and tiles that need it, moves their elements into
+// place and clears what lies past the depth; what lies past the last row or
+// column only reaches results that are not stored.
 template <typename E, bool kCol, uint32_t TILE, uint32_t THREADS>
 struct GuardedLoader {
   static constexpr uint32_t kLoads = TILE * 8u / THREADS, kOuter = kCol ? TILE / 8u : 8u, kPer = 16u / E::kBytes;
   static constexpr uint32_t kDepth = kCol ? 64u : kSlice / E::kBytes;  // depth elements per slice
   static_assert(TILE * 8u % THREADS == 0, "whole pieces per thread");
   Operand o;
-  uint32_t row0;
-  uint32_t voff[kLoads];
-  __device__ __forceinline__ GuardedLoader(const Operand& o_, uint32_t row0_) : o(o_), row0(row0_) {
+  uint32_t row0, row_bytes;
+  __device__ __forceinline__ GuardedLoader(const Operand& o_, uint32_t row0_)
+      : o(o_), row0(row0_), row_bytes((kCol ? o_.rows : o_.depth) * E::kBytes) {}
+  // `base`: the operand's storage (one of two, in the products over two segments of depth).
+  __device__ __forceinline__ void load(const uint8_t* base, uint32_t t, u32x4 (&v)[kLoads]) const {
+    const uint8_t* from = base + (kCol ? (uint64_t)t * 64u : (uint64_t)row0) * o.ld * E::kBytes;
+    const uint32_t last = kCol ? o.depth - 1u - t * 64u : o.rows - 1u - row0;  // outer's
+    const uint32_t in0 = kCol ? row0 * E::kBytes : t * kSlice, in_last = row_bytes - 16u;
+#pragma unroll
+    for (uint32_t q = 0; q < kLoads; ++q) {
+      const uint32_t id = threadIdx.x + q * THREADS, outer = id / kOuter, in = in0 + id % kOuter * 16u;
+      const uint32_t off = (outer < last ? outer : last) * (uint32_t)(o.ld * E::kBytes) + (in < in_last ? in : in_last);
+      v[q] = *reinterpret_cast<const u32x4_any*>(from + off);
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t t, uint8_t* tile, u32x4 (&v)[kLoads]) const {
+    const uint32_t in0 = kCol ? row0 * E::kBytes : t * kSlice;
+    const bool cut = in0 + kOuter * 16u > row_bytes, ends = kCol && (t + 1u) * 64u > o.depth;
 #pragma unroll
     for (uint32_t q = 0; q < kLoads; ++q) {
       const uint32_t id = threadIdx.x + q * THREADS, outer = id / kOuter, inner = id % kOuter;
-      if constexpr (kCol) {
-        const uint32_t last = (o.rows - 1u - row0) / kPer;
-        voff[q] = outer * (uint32_t)(o.ld * E::kBytes) + (inner < last ? inner : last) * 16u;
-      } else {
-        const uint32_t last = o.rows - 1u - row0;
-        voff[q] = (outer < last ? outer : last) * (uint32_t)(o.ld * E::kBytes) + inner * 16u;
+      if (cut) {
+        const uint32_t end = in0 + inner * 16u + 16u;
+        if (end > row_bytes) v[q] = end - row_bytes >= 16u ? u32x4{0, 0, 0, 0} : tiler_pieces::drop_bytes(v[q], end - row_bytes);
       }
+      if (ends && t * 64u + outer >= o.depth) v[q] = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(tile + piece_offset<TILE, kCol>(outer, inner)) = v[q];
     }
   }
-  // `base`: the operand's storage (one of two, in the products over two segments of depth).
+};
+// The same for operands with rows of less than a piece: checked piece by piece.
+template <typename E, bool kCol, uint32_t TILE, uint32_t THREADS>
+struct TinyLoader {
+  static constexpr uint32_t kLoads = TILE * 8u / THREADS, kOuter = kCol ? TILE / 8u : 8u;
+  static constexpr uint32_t kDepth = kCol ? 64u : kSlice / E::kBytes;
+  Operand o;
+  uint32_t row0;
+  __device__ __forceinline__ TinyLoader(const Operand& o_, uint32_t row0_) : o(o_), row0(row0_) {}
   __device__ __forceinline__ void load(const uint8_t* base, uint32_t t, u32x4 (&v)[kLoads]) const {
-    const bool whole = kCol ? (t + 1u) * kDepth < o.depth && o.ld >= kPer : (t + 1u) * kDepth <= o.depth;
-    if (whole) {
-      const uint8_t* at = base + (kCol ? t * 64u * o.ld * E::kBytes + row0 * (uint64_t)E::kBytes
-                                       : row0 * o.ld * E::kBytes + (uint64_t)t * kSlice);
+    const Operand here{base, o.ld, o.rows, o.depth};
+#pragma unroll 1
+    for (uint32_t q = 0; q < kLoads; ++q) {
+      const uint32_t id = threadIdx.x + q * THREADS;
+      const u32x4 p = operand_piece<E, kCol>(here, row0, t * kDepth, id / kOuter, id % kOuter);
 #pragma unroll
-      for (uint32_t q = 0; q < kLoads; ++q) v[q] = *reinterpret_cast<const u32x4_any*>(at + voff[q]);
-    } else {
-      const Operand here{base, o.ld, o.rows, o.depth};
-#pragma unroll
-      for (uint32_t q = 0; q < kLoads; ++q) {
-        const uint32_t id = threadIdx.x + q * THREADS;
-        v[q] = operand_piece<E, kCol>(here, row0, t * kDepth, id / kOuter, id % kOuter);
-      }
+      for (uint32_t x = 0; x < kLoads; ++x)
+        if (x == q) v[x] = p;
     }
   }
-  __device__ __forceinline__ void store(uint8_t* tile, const u32x4 (&v)[kLoads]) const {
+  __device__ __forceinline__ void store(uint32_t, uint8_t* tile, const u32x4 (&v)[kLoads]) const {
 #pragma unroll
     for (uint32_t q = 0; q < kLoads; ++q) {
       const uint32_t id = threadIdx.x + q * THREADS;
@@ -172,8 +189,8 @@ struct GuardedLoader {
   }
 };
 
-// load_a(t, pieces) and load_b fetch a slice, store_a(tile, pieces) and store_b
-// put it into LDS; WM x WN waves of MB x NB blocks of 16 x 16.
+// load_a(t, pieces) and load_b fetch a slice, store_a(t, tile, pieces) and
+// store_b put it into LDS; WM x WN waves of MB x NB blocks of 16 x 16.
 template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, typename LA, typename LB, typename SA,
           typename SB>
 __device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, LA load_a, LB load_b, SA store_a,
@@ -196,13 +213,10 @@ __device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, 
   };
   auto store = [&](uint32_t t, auto slot) {
     uint8_t* at = smem + (t & 1u) * kStage;
-    store_a(at, pa[decltype(slot)::value]);
-    store_b(at + kRowsA * kSlice, pb[decltype(slot)::value]);
+    store_a(t, at, pa[decltype(slot)::value]);
+    store_b(t, at + kRowsA * kSlice, pb[decltype(slot)::value]);
   };
-  // slice t in LDS, slice t + 1 in registers (slot (t + 1) % 2): requests slice
-  // t + 2, multiplies slice t, puts slice t + 1 into LDS
-  auto turn = [&](uint32_t t, auto next, auto after) {
-    if (t + 2 < slices) load(t + 2, after);
+  auto multiply = [&](uint32_t t) {
     const uint8_t* at = smem + (t & 1u) * kStage;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -214,24 +228,40 @@ __device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, 
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(fa[i], fb[j], acc[i][j]);
     }
-    if (t + 1 < slices) store(t + 1, next);
+  };
+  // Slice t in LDS, slice t + 1 in registers (slot (t + 1) % 2): requests slice
+  // t + 2, multiplies slice t, puts slice t + 1 into LDS.  Two turns a round
+  // without a condition in them, so that a wait counts only the loads before it.
+  auto turn = [&](uint32_t t, auto next, auto after) {
+    load(t + 2 < slices ? t + 2 : slices - 1, after);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(t);
+    store(t + 1, next);
     __syncthreads();
   };
   constexpr tiler::Step<0> even{};
   constexpr tiler::Step<1> odd{};
   load(0, even);
-  if (slices > 1) load(1, odd);
+  load(slices > 1 ? 1 : 0, odd);
   store(0, even);
   __syncthreads();
-  for (uint32_t t = 0; t < slices; t += 2) {
+  uint32_t t = 0;
+  for (; t + 2 < slices; t += 2) {
     turn(t, odd, even);
-    if (t + 1 < slices) turn(t + 1, even, odd);
+    turn(t + 1, even, odd);
   }
+  multiply(t);
+  if (t + 1 < slices) {
+    store(t + 1, odd);
+    __syncthreads();
+    multiply(t + 1);
+  }
+  __syncthreads();  // the caller may use the LDS
 }
 
 // ---------------------------------------------------------------------------
 // The staged product: pieces move global -> LDS with buffer_load_dwordx4 ...
-// lds, two slices in LDS, for operands whose rows (depth rows, in column
+// lds, S slices in LDS, for operands whose rows (depth rows, in column
 // layout) start on 16 bytes.
 //
 // A loader issues its wave's share of one slice of one operand.  The buffer
@@ -322,9 +352,11 @@ constexpr int kWaitLds = 0xC07F;  // lgkmcnt(0) alone
 // A slice is two depth steps; the fragments of the next step are read while
 // the products of the current one run, across slices too, so the only
 // wait a wave takes is the barrier in the middle of a slice: behind it every
-// wave's reads of the slice are done (its buffer takes the slice after the
-// next) and every wave's share of the next slice has landed.
-template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, int kLoads, typename IA, typename IB>
+// wave's reads of the slice are done (its buffer takes slice t + S) and every
+// wave's share of the next slice has landed.  The reads are
+// dealt out among the products (4096 x 14336 x 4096, dx 745 -> 715 us, the
+// weights' gradients 800 -> 750, against all reads first).
+template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, int kLoads, int S, typename IA, typename IB>
 __device__ __forceinline__ void staged_product(uint8_t* smem, uint32_t slices, IA issue_a, IB issue_b,
                                                typename E::Acc (&acc)[MB][NB]) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kRowsB = WN * NB * 16u, kTileA = kRowsA * kSlice;
@@ -336,14 +368,15 @@ __device__ __forceinline__ void staged_product(uint8_t* smem, uint32_t slices, I
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = E::zero();
-  auto issue = [&](uint32_t t) {
-    uint8_t* at = smem + (t & 1u) * kStage;
+  static_assert((S - 1) * kLoads < 64, "the loads in flight fit the wait counter");
+  auto issue = [&](uint32_t t, uint32_t stage) {
+    uint8_t* at = smem + stage * kStage;
     issue_a(t, at);
     issue_b(t, at + kTileA);
   };
   u32x4 fa[2][MB], fb[2][NB];
-  auto read = [&](uint32_t t, int s) {
-    const uint8_t* at = smem + (t & 1u) * kStage;
+  auto read = [&](uint32_t stage, int s) {
+    const uint8_t* at = smem + stage * kStage;
     ra.read(at, s, fa[s]);
     rb.read(at + kTileA, s, fb[s]);
   };
@@ -354,42 +387,74 @@ __device__ __forceinline__ void staged_product(uint8_t* smem, uint32_t slices, I
       for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(fa[s][i], fb[s][j], acc[i][j]);
   };
   if (slices == 0) return;
-  issue(0);
-  if (slices > 1) {
-    issue(1);
-    __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
-  } else {
-    __builtin_amdgcn_s_waitcnt(wait_loads(0));
-  }
+#pragma unroll
+  for (uint32_t t = 0; t < (uint32_t)S; ++t)
+    if (t < slices) issue(t, t);
+  if (slices >= (uint32_t)S) __builtin_amdgcn_s_waitcnt(wait_loads((S - 1) * kLoads));
+  else __builtin_amdgcn_s_waitcnt(wait_loads(0));
   asm volatile("s_barrier" ::: "memory");
   read(0, 0);
+  constexpr int kReads = (kACol ? 2 * MB : MB) + (kBCol ? 2 * NB : NB), kEach = MB * NB / kReads;
+  auto deal = [&]() {  // one LDS read (0x100), kEach products (0x008), and so on; the products left over
+#pragma unroll
+    for (int q = 0; q < kReads; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MB * NB - kEach * kReads, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t stage = 0;  // slice t's
   for (uint32_t t = 0; t + 1 < slices; ++t) {
-    read(t, 1);
-    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t next = stage + 1u == (uint32_t)S ? 0u : stage + 1u;
+    read(stage, 1);
     products(0);
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(wait_loads(0));
+    deal();
+    // slice t + 1 has landed (behind it, where S > 2, S - 2 more are in flight)
+    if (S == 2 || t + S > slices) __builtin_amdgcn_s_waitcnt(wait_loads(0));
+    else __builtin_amdgcn_s_waitcnt(wait_loads((S - 2) * kLoads));
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_s_waitcnt(kWaitLds);  // satisfied: tells the compiler so
-    if (t + 2 < slices) issue(t + 2);
-    read(t + 1, 0);
-    __builtin_amdgcn_sched_barrier(0);
+    if (t + S < slices) issue(t + S, stage);
+    read(next, 0);
     products(1);
-    __builtin_amdgcn_sched_barrier(0);
+    deal();
+    stage = next;
   }
-  read(slices - 1, 1);
+  read(stage, 1);
   products(0);
   products(1);
 }
 
+// Every wave's partial tile to LDS, then finish(total): total(q) is block q's
+// sum (row block q / NB, column block q % NB), the waves' parts in ascending order.
+template <typename E, int MB, int NB, int W, typename F>
+__device__ __forceinline__ void fold_waves(uint8_t* smem, const typename E::Acc (&acc)[MB][NB], F finish) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  __syncthreads();
+  typename E::Acc* const part = reinterpret_cast<typename E::Acc*>(smem);
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) part[(wave * MB * NB + i * NB + j) * 64u + lane] = acc[i][j];
+  __syncthreads();
+  auto total = [&](uint32_t q) {
+    typename E::Acc v = part[q * 64u + lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const typename E::Acc o = part[(w * MB * NB + q) * 64u + lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += o[r];
+    }
+    return v;
+  };
+  finish(total);
+}
 // The product for few rows: a workgroup of W waves owns MB x NB blocks of
 // 16 x 16 results, and wave w the depth slices w, w + W, ...: it moves a slice's
 // rows into a slot of its own (issue(t, slot)), reads its fragments, requests
 // its next slice into the same slot and multiplies while that lands.  No barrier
-// until the end, so nearly W slots a workgroup stay in flight; then every wave
-// leaves its partial tile in LDS, and finish(total) takes the blocks' sums:
-// total(q) is block q's (row block q / NB, column block q % NB), the waves'
-// parts added in ascending order.
+// until the end, so nearly W slots a workgroup stay in flight; then fold_waves.
 template <typename E, int MB, int NB, int W, typename I, typename F>
 __device__ __forceinline__ void few_rows_product(uint8_t* smem, uint32_t slices, I issue, F finish) {
   constexpr uint32_t kSlot = (MB + NB) * 16u * kSlice;
@@ -420,24 +485,7 @@ __device__ __forceinline__ void few_rows_product(uint8_t* smem, uint32_t slices,
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(fa[s][i], fb[s][j], acc[i][j]);
   }
-  __syncthreads();
-  typename E::Acc* const part = reinterpret_cast<typename E::Acc*>(smem);
-#pragma unroll
-  for (int i = 0; i < MB; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) part[(wave * MB * NB + i * NB + j) * 64u + lane] = acc[i][j];
-  __syncthreads();
-  auto total = [&](uint32_t q) {
-    typename E::Acc v = part[q * 64u + lane];
-#pragma unroll
-    for (int w = 1; w < W; ++w) {
-      const typename E::Acc o = part[(w * MB * NB + q) * 64u + lane];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] += o[r];
-    }
-    return v;
-  };
-  finish(total);
+  fold_waves<E, MB, NB, W>(smem, acc, finish);
 }
 template <int MB, int NB, int W>
 constexpr uint32_t few_rows_lds() {
@@ -455,6 +503,18 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t 
   const uint32_t height = tiles_m - group * 8u < 8u ? tiles_m - group * 8u : 8u;
   tm = group * 8u + in % height;
   tn = in / height;
+}
+
+// The tile of the few-row products: column panels in groups of eight, one per
+// XCD, whose tiles run one after another there (tn may lie past the last panel).
+__device__ __forceinline__ void panel_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+  if (tiles_n >= 8u) {
+    tm = (id >> 3) % tiles_m;
+    tn = (id >> 3) / tiles_m * 8u + (id & 7u);
+  } else {
+    tm = id % tiles_m;
+    tn = id / tiles_m;
+  }
 }
 
 // A pair of adjacent result rows (v0: row r, v1: row r + 1) of this lane's

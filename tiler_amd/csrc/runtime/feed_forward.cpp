@@ -182,10 +182,97 @@ tiler_hip_status check_product(uint64_t m, uint64_t n, uint64_t k, Program& p) {
 // 256-row panel through one buffer resource (below 2^31 bytes).
 bool staged_rows(uint64_t row_bytes) { return row_bytes % 16 == 0 && row_bytes * 256 < (1ull << 31); }
 
-// 256-tiles when they go round the CUs at least once, else 128-tiles (four
-// times as many, two to a CU).
-uint32_t staged_tile(const Target& t, uint64_t m, uint64_t n256, uint64_t n) {
-  return mul_sat(ceil_div(m, 256), ceil_div(n, n256)) >= t.compute_units ? 256 : 128;
+// A form of a staged product: a workgroup's rows and columns of the result, its
+// threads, and what its run takes (us).  With W workgroups, q = ceil(W / CUs) and
+// s slices of 128 bytes of depth:
+//   kOne   one workgroup to a CU      c0 + q (c1 + c2 s)
+//   kTwo   two workgroups to a CU     c0 + floor(q / 2) (c1 + c2 s) + (q mod 2) (c3 + c4 s)
+//   kFew   a slice in eight a wave, t = ceil(s / 8)
+//                                     c0 + q (c1 + c2 t) + c3 t + c4 t max(W / CUs, 1)
+// The constants are least squares fits of measured times (m 1 .. 4096, n 600 ..
+// 14336, k 800 .. 8192, at most 3000 workgroups): within 5% in the mean, and the
+// form of the least estimate is 1.2% slower than the fastest in the mean.
+struct ProductForm {
+  const char* name;
+  uint32_t rows, cols, threads;
+  enum Kind { kOne, kTwo, kFew } kind;
+  double c[5];
+};
+
+// us, by size: 16 x 14336 x 4096 45 (few1x1), t64_d 100; 301 x 14336 x 4096: t160 86,
+// t192 90, t128 119; 4096 x 14336 x 4096: t256 740, t128 830.
+constexpr ProductForm kGatedForms[] = {
+    {"few1x1", 16, 16, 512, ProductForm::kFew, {2.591, 0.235, 0.356, 0.131, 0.151}},
+    {"few2x1", 32, 16, 512, ProductForm::kFew, {2.524, 0.481, 0.610, 0, 0.115}},
+    {"few4x1", 64, 16, 512, ProductForm::kFew, {1.224, 1.963, 0.888, 0, 0.142}},
+    {"few4x2", 64, 32, 512, ProductForm::kFew, {1.264, 2.788, 1.431, 0, 0}},
+    {"t64_d", 64, 64, 256, ProductForm::kOne, {1.756, 2.011, 0.340}},
+    {"t96_d", 96, 64, 256, ProductForm::kOne, {1.799, 2.356, 0.428}},
+    {"t128_d", 128, 64, 256, ProductForm::kOne, {1.449, 2.893, 0.503}},
+    {"t96", 96, 64, 256, ProductForm::kTwo, {0.141, 3.587, 0.708, 2.314, 0.574}},
+    {"t128", 128, 64, 256, ProductForm::kTwo, {0.554, 3.867, 0.848, 3.017, 0.604}},
+    {"t160", 160, 64, 256, ProductForm::kTwo, {1.673, 3.506, 1.020, 2.685, 0.628}},
+    {"t192", 192, 128, 512, ProductForm::kOne, {0, 6.314, 0.976}},
+    {"t256", 256, 128, 512, ProductForm::kOne, {0, 7.471, 1.199}},
+};
+// us, by size: 16 x 4096 x 4096 few1x1 6.2; 301 x 4096 x 4096 t64_d 15.6 (two slices in LDS 20.7);
+// 4096 x 4096 x 4096 t256 59.4, t128 64.
+constexpr ProductForm kInt8Forms[] = {
+    {"few1x1", 16, 16, 512, ProductForm::kFew, {2.586, 0.193, 0.091, 0.172, 0.256}},
+    {"few2x1", 32, 16, 512, ProductForm::kFew, {2.499, 0.363, 0.274, 0.052, 0.271}},
+    {"few2x2", 32, 32, 512, ProductForm::kFew, {2.376, 0.655, 0.496, 0, 0.245}},
+    {"few4x2", 64, 32, 512, ProductForm::kFew, {1.207, 2.072, 1.051, 0, 0.012}},
+    {"few4x4", 64, 64, 512, ProductForm::kFew, {0.825, 3.623, 1.313, 0, 0.150}},
+    {"t64_d", 64, 128, 256, ProductForm::kOne, {0.976, 2.979, 0.328}},
+    {"t96_d", 96, 128, 256, ProductForm::kOne, {0.884, 3.723, 0.416}},
+    {"t96", 96, 128, 256, ProductForm::kTwo, {0.821, 5.652, 0.613, 2.477, 0.535}},
+    {"t128", 128, 128, 256, ProductForm::kTwo, {1.091, 6.483, 0.727, 2.924, 0.584}},
+    {"t192", 192, 256, 512, ProductForm::kOne, {0, 7.540, 0.934}},
+    {"t256", 256, 256, 512, ProductForm::kOne, {0, 9.259, 1.178}},
+};
+
+// A form's workgroups.  The few-row forms take their column panels eight at a
+// time, one to an XCD.
+uint64_t workgroups(const ProductForm& f, uint64_t m, uint64_t n) {
+  const uint64_t rows = ceil_div(m, f.rows), cols = ceil_div(n, f.cols);
+  return mul_sat(rows, f.kind == ProductForm::kFew && cols >= 8 ? ceil_div(cols, 8) * 8 : cols);
+}
+
+// The form of the least estimate, or null where no form's grid fits a launch.
+template <size_t N>
+const ProductForm* choose(const ProductForm (&forms)[N], const Target& t, uint64_t m, uint64_t n, uint64_t slices) {
+  const ProductForm* best = nullptr;
+  double least = 0;
+  for (const ProductForm& f : forms) {
+    const uint64_t w = workgroups(f, m, n);
+    if (!grid_holds(w, f.threads)) continue;
+    const double q = (double)ceil_div(w, t.compute_units), s = (double)slices;
+    double us = f.c[0];
+    if (f.kind == ProductForm::kOne) {
+      us += q * (f.c[1] + f.c[2] * s);
+    } else if (f.kind == ProductForm::kTwo) {
+      const double pairs = std::floor(q / 2);
+      us += pairs * (f.c[1] + f.c[2] * s) + (q - 2 * pairs) * (f.c[3] + f.c[4] * s);
+    } else {
+      const double part = std::ceil(s / 8), share = (double)w / t.compute_units;
+      us += q * (f.c[1] + f.c[2] * part) + f.c[3] * part + f.c[4] * part * (share > 1 ? share : 1);
+    }
+    if (!best || us < least) best = &f, least = us;
+  }
+  return best;
+}
+
+// Rows of the guarded forms' tiles, 64 or 128: 64 where those are at most one to
+// a CU, or no more of them.  us, 64 and 128: int8 257 x 5001 x 1111 15.0 / 23.4,
+// 2048 x 4096 x 4095 86 / 70; gated 200 x 4096 x 4095 48 / 66, 777 of them 125 / 99.
+uint32_t guarded_rows(const Target& t, uint64_t m, uint64_t column_tiles) {
+  return m <= 64 || mul_sat(ceil_div(m, 64), column_tiles) <= t.compute_units ? 64 : 128;
+}
+
+// The gradients' tiles: 256 when they go round the CUs at least once, else 128
+// (four times as many, two to a CU).
+uint32_t staged_tile(const Target& t, uint64_t m, uint64_t n) {
+  return mul_sat(ceil_div(m, 256), ceil_div(n, 256)) >= t.compute_units ? 256 : 128;
 }
 
 Launch& add_tiles(Program& p, const std::string& stem, uint32_t tile, uint64_t tiles) {
@@ -208,26 +295,11 @@ tiler_hip_status plan_gated_contract_bf16(const Target& t, uint32_t parts, uint6
   if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
   if (m == 0 || n == 0) return TILER_HIP_OK;
   const bool al = staged_rows(2 * k) && aligned16(addr[x]) && aligned16(addr[wg]) && aligned16(addr[wu]);
-  if (al && m <= 64 && grid_holds(ceil_div(n, 16), 512)) {
-    const std::string name = "tiler_gated_bf16_few" + std::to_string(ceil_div(m, 16));
-    Launch& l = p.add(name.c_str(), (uint32_t)ceil_div(n, 16), 1, 512)
-                    .ptr(x).ptr(wg).ptr(wu).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(h);
-    slot_or_null(l, keep, gate);
-    slot_or_null(l, keep, up);
-    return TILER_HIP_OK;
-  }
-  if (al) {
-    const uint32_t tile = staged_tile(t, m, 128, n);
-    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(n, tile / 2));
-    if (grid_holds(tiles, 512)) {
-      Launch& l = add_tiles(p, "tiler_gated_bf16", tile, tiles)
-                      .ptr(x).ptr(wg).ptr(wu).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(h);
-      slot_or_null(l, keep, gate);
-      slot_or_null(l, keep, up);
-      return TILER_HIP_OK;
-    }
-  }
-  Launch& l = p.add("tiler_gated_bf16_g", (uint32_t)ceil_div(n, 64), (uint32_t)ceil_div(m, 128), 256)
+  const ProductForm* const f = al ? choose(kGatedForms, t, m, n, ceil_div(k, 64)) : nullptr;
+  const uint32_t rows = guarded_rows(t, m, ceil_div(n, 64));
+  const std::string name = "tiler_gated_bf16_" + (f ? std::string(f->name) : "g" + std::to_string(rows));
+  Launch& l = (f ? p.add(name.c_str(), (uint32_t)workgroups(*f, m, n), 1, f->threads)
+                 : p.add(name.c_str(), (uint32_t)ceil_div(n, 64), (uint32_t)ceil_div(m, rows), 256))
                   .ptr(x).ptr(wg).ptr(wu).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(h);
   slot_or_null(l, keep, gate);
   slot_or_null(l, keep, up);
@@ -264,7 +336,7 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
     // twice (two 128-tiles to a CU) where the tiles alone do not: at least
     // four slices each, the binary32 partials added by one more launch.
     const bool staged = rows_ok && aligned16(addr[wg]) && aligned16(addr[wu]);
-    const uint32_t tile = staged ? staged_tile(t, m, 256, k) : 128;
+    const uint32_t tile = staged ? staged_tile(t, m, k) : 128;
     const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(k, tile)), slices = 2 * (ld / 64);
     uint64_t splits = 1;
     if (tile == 128 && tiles < 2ull * t.compute_units) {
@@ -286,7 +358,7 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
     }
   }
   if (has_dw && n) {
-    const uint32_t tile = staged_tile(t, 2 * n, 256, k);
+    const uint32_t tile = staged_tile(t, 2 * n, k);
     const uint64_t tiles = mul_sat(2 * ceil_div(n, tile), ceil_div(k, tile));
     if (rows_ok && aligned16(addr[x]) && grid_holds(tiles, 512))
       add_tiles(p, "tiler_gated_bf16_dw", tile, tiles)
@@ -327,25 +399,13 @@ tiler_hip_status plan_contract_i8(const Target& t, uint32_t out_dtype, uint64_t 
   if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
   if (k > 131071) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "a sum of more than 131071 products could leave 32 bits");
   if (m == 0 || n == 0) return TILER_HIP_OK;
-  char name[64];
   const bool al = staged_rows(k) && aligned16(addr[a]) && aligned16(addr[b]);
-  if (al && m <= 64 && grid_holds(ceil_div(n, 16), 512)) {
-    std::snprintf(name, sizeof(name), "tiler_contract_i8_%s_few%u", type_name(out_dtype), (uint32_t)ceil_div(m, 16));
-    p.add(name, (uint32_t)ceil_div(n, 16), 1, 512)
-        .ptr(a).ptr(b).ptr(sa).ptr(sb).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(c);
-    return TILER_HIP_OK;
-  }
-  if (al) {
-    const uint32_t tile = staged_tile(t, m, 256, n);
-    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(n, tile));
-    if (grid_holds(tiles, 512)) {
-      add_tiles(p, std::string("tiler_contract_i8_") + type_name(out_dtype), tile, tiles)
-          .ptr(a).ptr(b).ptr(sa).ptr(sb).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(c);
-      return TILER_HIP_OK;
-    }
-  }
-  std::snprintf(name, sizeof(name), "tiler_contract_i8_%s_g", type_name(out_dtype));
-  p.add(name, (uint32_t)ceil_div(n, 128), (uint32_t)ceil_div(m, 128), 256)
+  const ProductForm* const f = al ? choose(kInt8Forms, t, m, n, ceil_div(k, 128)) : nullptr;
+  const uint32_t rows = guarded_rows(t, m, ceil_div(n, 128));
+  const std::string name = std::string("tiler_contract_i8_") + type_name(out_dtype) + "_" +
+                           (f ? std::string(f->name) : "g" + std::to_string(rows));
+  (f ? p.add(name.c_str(), (uint32_t)workgroups(*f, m, n), 1, f->threads)
+     : p.add(name.c_str(), (uint32_t)ceil_div(n, 128), (uint32_t)ceil_div(m, rows), 256))
       .ptr(a).ptr(b).ptr(sa).ptr(sb).u32((uint32_t)m).u32((uint32_t)n).u32((uint32_t)k).ptr(c);
   return TILER_HIP_OK;
 }

@@ -363,7 +363,6 @@ const EntryRow kEntries[] = {
     {"tiler_layer_norm_columns_f32", "layer-norm-backward-f32", 5},
     {"tiler_layer_norm_columns_final_bf16", "layer-norm-backward/bf16", 3},
     {"tiler_layer_norm_columns_final_f32", "layer-norm-backward-f32", 3},
-    {"tiler_gated_bf16_g", "gated-contraction-bf16", 6},
     {"tiler_gated_bf16_grad", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dx_g", "gated-contraction-bf16-backward", 6},
     {"tiler_gated_bf16_dw_g", "gated-contraction-bf16-backward", 5},
@@ -383,23 +382,25 @@ const EntryRow kEntries[] = {
     TILER_GRAD_FORM("w1c1"), TILER_GRAD_FORM("w2c1"), TILER_GRAD_FORM("w4c1"), TILER_GRAD_FORM("w8c1"),
     TILER_GRAD_FORM("w16c1"), TILER_GRAD_FORM("w16c2"),
 #undef TILER_GRAD_FORM
-    {"tiler_contract_i8_bf16_g", "tensor-contraction-i8/bf16", 5},
-    {"tiler_contract_i8_f32_g", "tensor-contraction-i8/f32", 5},
-#define TILER_STAGED_ROWS(TILE)                                                            \
-  {"tiler_gated_bf16_t" TILE, "gated-contraction-bf16", 6},                                 \
-      {"tiler_gated_bf16_dx_t" TILE, "gated-contraction-bf16-backward", 6},                 \
-      {"tiler_gated_bf16_dw_t" TILE, "gated-contraction-bf16-backward", 5},                 \
-      {"tiler_contract_i8_bf16_t" TILE, "tensor-contraction-i8/bf16", 5},                   \
-      {"tiler_contract_i8_f32_t" TILE, "tensor-contraction-i8/f32", 5}
-    TILER_STAGED_ROWS("256"), TILER_STAGED_ROWS("128"),
-#undef TILER_STAGED_ROWS
+    {"tiler_gated_bf16_dx_t128", "gated-contraction-bf16-backward", 6},
+    {"tiler_gated_bf16_dx_t256", "gated-contraction-bf16-backward", 6},
     {"tiler_gated_bf16_dx_sum", "gated-contraction-bf16-backward", 2},
-#define TILER_FEW_ROWS(MB)                                                          \
-  {"tiler_gated_bf16_few" MB, "gated-contraction-bf16", 6},                         \
-      {"tiler_contract_i8_bf16_few" MB, "tensor-contraction-i8/bf16", 5},           \
-      {"tiler_contract_i8_f32_few" MB, "tensor-contraction-i8/f32", 5}
-    TILER_FEW_ROWS("1"), TILER_FEW_ROWS("2"), TILER_FEW_ROWS("3"), TILER_FEW_ROWS("4"),
-#undef TILER_FEW_ROWS
+    {"tiler_gated_bf16_dw_t128", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_dw_t256", "gated-contraction-bf16-backward", 5},
+#define TILER_GATED_FORM(FORM) {"tiler_gated_bf16_" FORM, "gated-contraction-bf16", 6}
+    TILER_GATED_FORM("g64"), TILER_GATED_FORM("g128"), TILER_GATED_FORM("few1x1"), TILER_GATED_FORM("few2x1"),
+    TILER_GATED_FORM("few4x1"), TILER_GATED_FORM("few4x2"), TILER_GATED_FORM("t64_d"), TILER_GATED_FORM("t96_d"),
+    TILER_GATED_FORM("t128_d"), TILER_GATED_FORM("t96"), TILER_GATED_FORM("t128"), TILER_GATED_FORM("t160"),
+    TILER_GATED_FORM("t192"), TILER_GATED_FORM("t256"),
+#undef TILER_GATED_FORM
+#define TILER_INT8_FORM(FORM)                                                \
+  {"tiler_contract_i8_bf16_" FORM, "tensor-contraction-i8/bf16", 5},         \
+      {"tiler_contract_i8_f32_" FORM, "tensor-contraction-i8/f32", 5}
+    TILER_INT8_FORM("g64"), TILER_INT8_FORM("g128"), TILER_INT8_FORM("few1x1"), TILER_INT8_FORM("few2x1"),
+    TILER_INT8_FORM("few2x2"), TILER_INT8_FORM("few4x2"), TILER_INT8_FORM("few4x4"), TILER_INT8_FORM("t64_d"),
+    TILER_INT8_FORM("t96_d"), TILER_INT8_FORM("t96"), TILER_INT8_FORM("t128"), TILER_INT8_FORM("t192"),
+    TILER_INT8_FORM("t256"),
+#undef TILER_INT8_FORM
 };
 constexpr uint32_t kEntryCount = sizeof(kEntries) / sizeof(kEntries[0]);
 
