@@ -196,17 +196,17 @@ __device__ __forceinline__ void contract_i8_guarded(const int8_t* __restrict__ a
   constexpr uint32_t kRows = 2u * MB * 16u;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRows + 128u) * kSlice];
   const uint32_t m0 = blockIdx.y * kRows, n0 = blockIdx.x * 128u;
-  const Operand oa{reinterpret_cast<const uint8_t*>(a), k, m, k}, ob{reinterpret_cast<const uint8_t*>(b), k, n, k};
+  const Operand oa{reinterpret_cast<const uint8_t*>(a), m, k}, ob{reinterpret_cast<const uint8_t*>(b), n, k};
   i32x4 acc[MB][4];
   auto product = [&](const auto& la, const auto& lb) {
-    tiler_product::guarded_product<I8, false, false, 2, 2, MB, 4>(
+    tiler_product::guarded_product<I8, 2, 2, MB, 4>(
         smem, (k + 127u) / 128u, [&](uint32_t t, u32x4(&v)[MB]) { la.load(oa.base, t, v); },
         [&](uint32_t t, u32x4(&v)[4]) { lb.load(ob.base, t, v); },
         [&](uint32_t t, uint8_t* tile, u32x4(&v)[MB]) { la.store(t, tile, v); },
         [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { lb.store(t, tile, v); }, acc);
   };
-  if (k >= 16u) product(tiler_product::GuardedLoader<I8, false, kRows, 256>(oa, m0), tiler_product::GuardedLoader<I8, false, 128, 256>(ob, n0));
-  else product(tiler_product::TinyLoader<I8, false, kRows, 256>(oa, m0), tiler_product::TinyLoader<I8, false, 128, 256>(ob, n0));
+  if (k >= 16u) product(tiler_product::GuardedLoader<I8, kRows, 256>(oa, m0), tiler_product::GuardedLoader<I8, 128, 256>(ob, n0));
+  else product(tiler_product::TinyLoader<I8, kRows, 256>(oa, m0), tiler_product::TinyLoader<I8, 128, 256>(ob, n0));
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {

@@ -34,8 +34,11 @@ __device__ __forceinline__ float sigmoid(float v) {
 // Guarded form: 128 (or 64) tokens x (64 gate + 64 up) columns, any sizes and
 // alignments.  Row r of the B tile: gate (r & 32 == 0) or up row
 // (r >> 6) * 32 + (r & 31) of the 64-column tile.
-constexpr int kW = 2, kMB = 4, kNB = 4;  // 2 x 2 waves of 4 x 4 blocks
-constexpr uint32_t kGuardedBytes = 2u * 256u * kSlice;
+constexpr int kW = 2, kNB = 4;  // 2 x 2 waves of MB x 4 blocks, MB 4 or 2
+
+// Rows of dG and dU, and of the copies of x and the weights in the backward pass.
+__device__ __forceinline__ uint32_t row_of_mid(uint32_t n) { return (n + 63u) & ~63u; }
+__device__ __forceinline__ uint32_t row_of_copy(uint32_t k) { return (k + 7u) & ~7u; }
 
 template <int MB>
 __device__ __forceinline__ void gated_guarded(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
@@ -46,11 +49,11 @@ __device__ __forceinline__ void gated_guarded(const uint16_t* __restrict__ x, co
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRows + 128u) * kSlice];
   const uint32_t m0 = blockIdx.y * kRows, n0 = blockIdx.x * 64u;
   // thread t's pieces of B are rows t / 8 + 32 q of its tile: gate rows for even q, up rows for odd
-  const Operand a{reinterpret_cast<const uint8_t*>(x), k, m, k}, b{reinterpret_cast<const uint8_t*>(wg), k, n, k};
+  const Operand a{reinterpret_cast<const uint8_t*>(x), m, k}, b{reinterpret_cast<const uint8_t*>(wg), n, k};
   f32x4 acc[MB][kNB];
   // (lb fetches 64 rows of either weight, whole lays the 128 of the tile out)
   auto product = [&](const auto& la, const auto& lb, const auto& whole) {
-    tiler_product::guarded_product<Bf16, false, false, kW, kW, MB, kNB>(
+    tiler_product::guarded_product<Bf16, kW, kW, MB, kNB>(
         smem, (k + 63u) / 64u, [&](uint32_t t, u32x4(&v)[MB]) { la.load(a.base, t, v); },
         [&](uint32_t t, u32x4(&v)[4]) {
           u32x4 g[2], u[2];
@@ -65,11 +68,11 @@ __device__ __forceinline__ void gated_guarded(const uint16_t* __restrict__ x, co
   using tiler_product::GuardedLoader;
   using tiler_product::TinyLoader;
   if (k >= 8u)
-    product(GuardedLoader<Bf16, false, kRows, 256>(a, m0), GuardedLoader<Bf16, false, 64, 256>(b, n0),
-            GuardedLoader<Bf16, false, 128, 256>(b, n0));
+    product(GuardedLoader<Bf16, kRows, 256>(a, m0), GuardedLoader<Bf16, 64, 256>(b, n0),
+            GuardedLoader<Bf16, 128, 256>(b, n0));
   else
-    product(TinyLoader<Bf16, false, kRows, 256>(a, m0), TinyLoader<Bf16, false, 64, 256>(b, n0),
-            TinyLoader<Bf16, false, 128, 256>(b, n0));
+    product(TinyLoader<Bf16, kRows, 256>(a, m0), TinyLoader<Bf16, 64, 256>(b, n0),
+            TinyLoader<Bf16, 128, 256>(b, n0));
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < MB; ++i)
@@ -106,23 +109,50 @@ tiler_gated_bf16_g64(const uint16_t* __restrict__ x, const uint16_t* __restrict_
   gated_guarded<2>(x, wg, wu, m, n, k, h, gate, up);
 }
 
-// dG and dU of one row's eight columns per thread, into rows of `ld` elements
-// (a multiple of 64; the columns past n are written as zeros).
+// dG and dU (behind dG) of one row's eight columns per item, into rows of n
+// rounded up to 64 (the columns past n are written as zeros).  Where the rows of
+// x or of the weights do not start on 16 bytes, they are copied to rows that do,
+// of k rounded up to 8, so that the products always run staged: gradients of
+// 4096 x 14336 x 4095, us, 226 + 712 + 741; with the products' operands through
+// registers instead (as the forward pass's guarded form) 112 + 1395 + 1349.
 extern "C" __global__ void __launch_bounds__(256)
 tiler_gated_bf16_grad(const uint16_t* __restrict__ gate, const uint16_t* __restrict__ up,
-                      const uint16_t* __restrict__ dh, uint32_t m, uint32_t n, uint32_t ld, uint16_t* __restrict__ dg,
-                      uint16_t* __restrict__ du) {
-  const uint32_t per = ld / 8u;
-  const uint64_t total = (uint64_t)m * per;
-  for (uint64_t id = blockIdx.x * 256ull + threadIdx.x; id < total; id += gridDim.x * 256ull) {
+                      const uint16_t* __restrict__ dh, const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
+                      const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ dg,
+                      uint16_t* __restrict__ to_x, uint16_t* __restrict__ to_w) {
+  using tiler_pieces::guarded_piece;
+  using tiler_pieces::u32x4_any;
+  const uint32_t ld = row_of_mid(n), per = ld / 8u, ldk = row_of_copy(k), per_k = ldk / 8u;
+  const uint64_t first = blockIdx.x * 256ull + threadIdx.x, step = gridDim.x * 256ull;
+  const uint64_t copies = ((to_x ? (uint64_t)m : 0u) + (to_w ? 2ull * n : 0u)) * per_k;
+  for (uint64_t id = first; id < copies; id += step) {
+    uint64_t row = id / per_k;
+    const uint32_t col = (uint32_t)(id % per_k) * 8u;
+    const uint16_t* from = x;
+    uint16_t* to = to_x;
+    if (!to_x || row >= m) {
+      if (to_x) row -= m;
+      from = row >= n ? wu : wg;
+      to = to_w + (row >= n ? (uint64_t)n * ldk : 0u);
+      if (row >= n) row -= n;
+    }
+    const uint32_t valid = k - col < 8u ? (k - col) * 2u : 16u;
+    *reinterpret_cast<u32x4*>(to + row * ldk + col) = guarded_piece(
+        reinterpret_cast<const uint8_t*>(from + row * k + col), valid, reinterpret_cast<const uint8_t*>(from));
+  }
+  const uint64_t mids = (uint64_t)m * per;
+  for (uint64_t id = first; id < mids; id += step) {
     const uint32_t row = (uint32_t)(id / per), col = (uint32_t)(id % per) * 8u;
     const uint64_t at = (uint64_t)row * n + col;
     const uint32_t valid = col >= n ? 0u : n - col < 8u ? (n - col) * 2u : 16u;
     u32x4 vg = {0, 0, 0, 0}, vu = vg, vd = vg;
-    if (valid) {
+    if (valid == 16u) {
+      vg = *reinterpret_cast<const u32x4_any*>(gate + at);
+      vu = *reinterpret_cast<const u32x4_any*>(up + at);
+      vd = *reinterpret_cast<const u32x4_any*>(dh + at);
+    } else if (valid) {
       auto piece = [&](const uint16_t* q) {
-        return tiler_product::guarded_piece(reinterpret_cast<const uint8_t*>(q + at), valid,
-                                            reinterpret_cast<const uint8_t*>(q));
+        return guarded_piece(reinterpret_cast<const uint8_t*>(q + at), valid, reinterpret_cast<const uint8_t*>(q));
       };
       vg = piece(gate);
       vu = piece(up);
@@ -144,12 +174,12 @@ tiler_gated_bf16_grad(const uint16_t* __restrict__ gate, const uint16_t* __restr
     }
     const uint64_t to = (uint64_t)row * ld + col;
     *reinterpret_cast<u32x4*>(dg + to) = og;
-    *reinterpret_cast<u32x4*>(du + to) = ou;
+    *reinterpret_cast<u32x4*>(dg + (uint64_t)m * ld + to) = ou;
   }
 }
 
-// Where the depth of dx is split over `splits` workgroups a tile (blockIdx.y):
-// this one's slices of the 2 per in all.
+// Where the depth is split over `splits` workgroups a tile (blockIdx.y): this
+// one's slices.
 __device__ __forceinline__ void split_range(uint32_t slices, uint32_t splits, uint32_t s, uint32_t& t0, uint32_t& t1) {
   t0 = (uint32_t)((uint64_t)slices * s / splits);
   t1 = (uint32_t)((uint64_t)slices * (s + 1u) / splits);
@@ -171,97 +201,42 @@ __device__ __forceinline__ void store_partial(const f32x4 (&acc)[MB][NB], float*
       }
 }
 
-// dx [m, k] = dG Wg + dU Wu: depth n twice (dG with Wg, then dU with Wu), the
-// weights in column layout.  Guarded: 128 x 128 tiles, any sizes.  With splits
-// > 1 each split's sums go to partials[split], binary32 [m, k].
-extern "C" __global__ void __launch_bounds__(256, 2)
-tiler_gated_bf16_dx_g(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,
-                      const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m, uint32_t n,
-                      uint32_t k, uint16_t* __restrict__ dx, uint32_t splits, float* __restrict__ partials) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
-  const uint32_t tiles_k = (k + 127u) / 128u;
-  const uint32_t m0 = blockIdx.x / tiles_k * 128u, c0 = blockIdx.x % tiles_k * 128u, per = ld / 64u;
-  uint32_t t0, t1;
-  split_range(2u * per, splits, blockIdx.y, t0, t1);
-  f32x4 acc[kMB][kNB];
-  if (n == 0) {
-#pragma unroll
-    for (int i = 0; i < kMB; ++i)
-#pragma unroll
-      for (int j = 0; j < kNB; ++j) acc[i][j] = Bf16::zero();
-  } else {
-    // dG's rows hold zeros from n to ld
-    const tiler_product::GuardedLoader<Bf16, false, 128, 256> la(
-        Operand{reinterpret_cast<const uint8_t*>(dg), ld, m, ld}, m0);
-    const Operand b{reinterpret_cast<const uint8_t*>(wg), k, k, n};
-    auto product = [&](const auto& lb) {
-      tiler_product::guarded_product<Bf16, false, true, kW, kW, kMB, kNB>(
-          smem, t1 - t0,
-          [&](uint32_t t, u32x4(&v)[4]) {
-            const bool first = t + t0 < per;
-            la.load(reinterpret_cast<const uint8_t*>(first ? dg : du), first ? t + t0 : t + t0 - per, v);
-          },
-          [&](uint32_t t, u32x4(&v)[4]) {
-            const bool first = t + t0 < per;
-            lb.load(reinterpret_cast<const uint8_t*>(first ? wg : wu), first ? t + t0 : t + t0 - per, v);
-          },
-          [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { la.store(t + t0 < per ? t + t0 : t + t0 - per, tile, v); },
-          [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { lb.store(t + t0 < per ? t + t0 : t + t0 - per, tile, v); }, acc);
-    };
-    if (k >= 8u) product(tiler_product::GuardedLoader<Bf16, true, 128, 256>(b, c0));
-    else product(tiler_product::TinyLoader<Bf16, true, 128, 256>(b, c0));
-  }
-  const uint32_t wave = threadIdx.x >> 6, row0 = m0 + (wave / kW) * 64u, col0 = c0 + (wave % kW) * 64u;
-  if (splits > 1) {
-    store_partial(acc, partials + (uint64_t)blockIdx.y * m * k, m, k, row0, col0);
-    return;
-  }
-  tiler_product::store_tile_bf16<128, 128, 256, kMB, kNB>(smem, (wave / kW) * 64u, (wave % kW) * 64u, dx, m, k, m0, c0,
-                                                          [&](int i, int j, int r) { return acc[i][j][r]; });
-}
-
-// dx from its splits' partials, in ascending order.
+// Gradients from the partials of the products whose depth is split, each in
+// ascending order: `count_x` elements of dx, `count_w` of either weight's
+// gradient (0: not split).  Four to a thread.
 extern "C" __global__ void __launch_bounds__(256)
-tiler_gated_bf16_dx_sum(const float* __restrict__ partials, uint32_t splits, uint64_t count, uint16_t* __restrict__ dx) {
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < count; i += gridDim.x * 256ull) {
-    float s = partials[i];
+tiler_gated_bf16_sum(const float* __restrict__ of_x, uint32_t splits_x, uint64_t count_x, uint16_t* __restrict__ dx,
+                     const float* __restrict__ of_w, uint32_t splits_w, uint64_t count_w, uint16_t* __restrict__ dwg,
+                     uint16_t* __restrict__ dwu) {
+  const uint64_t pieces_x = (count_x + 3u) / 4u, pieces_w = (count_w + 3u) / 4u, total = pieces_x + 2u * pieces_w;
+  for (uint64_t id = blockIdx.x * 256ull + threadIdx.x; id < total; id += gridDim.x * 256ull) {
+    const bool is_x = id < pieces_x, second = !is_x && id - pieces_x >= pieces_w;
+    const uint64_t at = (is_x ? id : id - pieces_x - (second ? pieces_w : 0u)) * 4u, count = is_x ? count_x : count_w;
+    const uint64_t stride = is_x ? count_x : 2u * count_w;
+    const uint32_t splits = is_x ? splits_x : splits_w;
+    const float* from = (is_x ? of_x : of_w + (second ? count_w : 0u)) + at;
+    uint16_t* to = (is_x ? dx : second ? dwu : dwg) + at;
+    if (count - at >= 4u) {
+      f32x4 s = __builtin_bit_cast(f32x4, *reinterpret_cast<const tiler_pieces::u32x4_any*>(from));
 #pragma unroll 4
-    for (uint32_t p = 1; p < splits; ++p) s += partials[p * count + i];
-    dx[i] = (uint16_t)tiler::bf16_narrow(s);
+      for (uint32_t p = 1; p < splits; ++p) {
+        const f32x4 v = __builtin_bit_cast(f32x4, *reinterpret_cast<const tiler_pieces::u32x4_any*>(from + p * stride));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+      }
+      *reinterpret_cast<tiler_pieces::u32x2_any*>(to) = u32x2{tiler::bf16_pack2_rne(s[0], s[1]), tiler::bf16_pack2_rne(s[2], s[3])};
+    } else {
+      for (uint64_t e = 0; e < count - at; ++e) {
+        float s = from[e];
+        for (uint32_t p = 1; p < splits; ++p) s += from[p * stride + e];
+        to[e] = (uint16_t)tiler::bf16_narrow(s);
+      }
+    }
   }
-}
-
-// dWg [n, k] = dG^T x and dWu = dU^T x: depth m, both operands in column
-// layout.  Guarded: 128 x 128 tiles, any sizes; tiles_n row tiles of each.
-extern "C" __global__ void __launch_bounds__(256, 2)
-tiler_gated_bf16_dw_g(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,
-                      const uint16_t* __restrict__ x, uint32_t m, uint32_t n, uint32_t k, uint32_t tiles_n,
-                      uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kGuardedBytes];
-  const bool second = blockIdx.y >= tiles_n;
-  const uint32_t j0 = (second ? blockIdx.y - tiles_n : blockIdx.y) * 128u, c0 = blockIdx.x * 128u;
-  // dG's and dU's rows are ld long: whole pieces
-  const tiler_product::GuardedLoader<Bf16, true, 128, 256> la(
-      Operand{reinterpret_cast<const uint8_t*>(second ? du : dg), ld, ld, m}, j0);
-  const Operand b{reinterpret_cast<const uint8_t*>(x), k, k, m};
-  f32x4 acc[kMB][kNB];
-  auto product = [&](const auto& lb) {
-    tiler_product::guarded_product<Bf16, true, true, kW, kW, kMB, kNB>(
-        smem, (m + 63u) / 64u, [&](uint32_t t, u32x4(&v)[4]) { la.load(la.o.base, t, v); },
-        [&](uint32_t t, u32x4(&v)[4]) { lb.load(b.base, t, v); },
-        [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { la.store(t, tile, v); },
-        [&](uint32_t t, uint8_t* tile, u32x4(&v)[4]) { lb.store(t, tile, v); }, acc);
-  };
-  if (k >= 8u) product(tiler_product::GuardedLoader<Bf16, true, 128, 256>(b, c0));
-  else product(tiler_product::TinyLoader<Bf16, true, 128, 256>(b, c0));
-  const uint32_t wave = threadIdx.x >> 6;
-  tiler_product::store_tile_bf16<128, 128, 256, kMB, kNB>(smem, (wave / kW) * 64u, (wave % kW) * 64u,
-                                                          second ? dwu : dwg, n, k, j0, c0,
-                                                          [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 
 // ---------------------------------------------------------------------------
-// Staged forms: k a multiple of 8 and 16-byte aligned operands.  WM x WN waves
+// Staged forms: rows that start on 16 bytes.  WM x WN waves
 // of MB x 4 blocks.
 namespace {
 
@@ -301,11 +276,13 @@ __device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, con
   }
 }
 
+// dx [m, k] = dG Wg + dU Wu: depth n twice (dG with Wg, then dU with Wu), the
+// weights in column layout, their rows ldk long (wu null: Wu is behind Wg).  With
+// splits > 1 each split's sums go to partials[split], binary32 [m, k].
 template <int WM, int WN, int MB>
-__device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du,
-                                                uint32_t ld, const uint16_t* __restrict__ wg,
-                                                const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,
-                                                uint16_t* __restrict__ dx, uint32_t splits,
+__device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ wg,
+                                                const uint16_t* __restrict__ wu, uint32_t ldk, uint32_t m, uint32_t n,
+                                                uint32_t k, uint16_t* __restrict__ dx, uint32_t splits,
                                                 float* __restrict__ partials) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kCols = WN * 64u, kThreads = 64u * WM * WN;
   constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kCols / 8 / (WM * WN);
@@ -313,15 +290,15 @@ __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg,
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t tm, tn, t0, t1;
   tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (k + kCols - 1u) / kCols, tm, tn);
-  const uint32_t m0 = tm * kRowsA, c0 = tn * kCols, per = ld / 64u;
+  const uint32_t m0 = tm * kRowsA, c0 = tn * kCols, ld = row_of_mid(n), per = ld / 64u;
   split_range(2u * per, splits, blockIdx.y, t0, t1);
   // dG's rows hold zeros from n to ld, the weights' depth rows load as zeros there
   const tiler_product::RowLoader<Bf16, kLoadsA> la(reinterpret_cast<const uint8_t*>(dg + (uint64_t)m0 * ld), ld,
                                                    m - m0 < kRowsA ? m - m0 : kRowsA, ld, wave * kLoadsA * 8u,
                                                    wave * kLoadsA * 8u, lane);
-  const tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(wg + c0), k, c0, n, wave, lane);
-  const uint8_t* const a2 = reinterpret_cast<const uint8_t*>(du + (uint64_t)m0 * ld);
-  const uint8_t* const b2 = reinterpret_cast<const uint8_t*>(wu + c0);
+  const tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(wg + c0), ldk, c0, n, wave, lane);
+  const uint8_t* const a2 = reinterpret_cast<const uint8_t*>(dg + ((uint64_t)m + m0) * ld);
+  const uint8_t* const b2 = reinterpret_cast<const uint8_t*>((wu ? wu : wg + (uint64_t)n * ldk) + c0);
   f32x4 acc[MB][4];
   tiler_product::staged_product<Bf16, false, true, WM, WN, MB, 4, kLoadsA + kLoadsB, 2>(
       smem, t1 - t0,
@@ -344,10 +321,14 @@ __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg,
                                                                  [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 
+// dWg [n, k] = dG^T x and dWu = dU^T x: depth m, both operands in column
+// layout, x's rows ldk long.  With splits > 1 each split's sums go to
+// partials[split], binary32 [2, n, k].
 template <int WM, int WN, int MB>
-__device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du,
-                                                uint32_t ld, const uint16_t* __restrict__ x, uint32_t m, uint32_t n,
-                                                uint32_t k, uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {
+__device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ x,
+                                                uint32_t ldk, uint32_t m, uint32_t n, uint32_t k,
+                                                uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu, uint32_t splits,
+                                                float* __restrict__ partials) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kCols = WN * 64u, kThreads = 64u * WM * WN;
   constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kCols / 8 / (WM * WN);
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kCols) * kSlice];
@@ -356,18 +337,24 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
   uint32_t tm, tn;
   tiler_product::tile_of(blockIdx.x, 2u * tiles, (k + kCols - 1u) / kCols, tm, tn);
   const bool second = tm >= tiles;
-  const uint32_t j0 = (second ? tm - tiles : tm) * kRowsA, c0 = tn * kCols;
-  const tiler_product::ColumnLoader<kRowsA, kLoadsA> la(reinterpret_cast<const uint8_t*>((second ? du : dg) + j0), ld, j0,
+  const uint32_t j0 = (second ? tm - tiles : tm) * kRowsA, c0 = tn * kCols, ld = row_of_mid(n);
+  const tiler_product::ColumnLoader<kRowsA, kLoadsA> la(reinterpret_cast<const uint8_t*>(dg + (second ? (uint64_t)m * ld : 0u) + j0), ld, j0,
                                                         m, wave, lane);
-  const tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(x + c0), k, c0, m, wave, lane);
+  const tiler_product::ColumnLoader<kCols, kLoadsB> lb(reinterpret_cast<const uint8_t*>(x + c0), ldk, c0, m, wave, lane);
   f32x4 acc[MB][4];
+  uint32_t t0, t1;
+  split_range((m + 63u) / 64u, splits, blockIdx.y, t0, t1);
   tiler_product::staged_product<Bf16, true, true, WM, WN, MB, 4, kLoadsA + kLoadsB, 2>(
-      smem, (m + 63u) / 64u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
-      [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
+      smem, t1 - t0, [&](uint32_t t, uint8_t* at) { la.issue(t0 + t, at); },
+      [&](uint32_t t, uint8_t* at) { lb.issue(t0 + t, at); }, acc);
+  const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 64u;
+  if (splits > 1) {
+    store_partial(acc, partials + ((uint64_t)blockIdx.y * 2u + (second ? 1u : 0u)) * n * k, n, k, j0 + row0, c0 + col0);
+    return;
+  }
   __syncthreads();
-  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(
-      smem, (wave / WN) * MB * 16u, (wave % WN) * 64u, second ? dwu : dwg, n, k, j0, c0,
-      [&](int i, int j, int r) { return acc[i][j][r]; });
+  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(smem, row0, col0, second ? dwu : dwg, n, k, j0, c0,
+                                                                 [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 
 }  // namespace
@@ -387,18 +374,18 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
   }
 #define TILER_GATED_DX_STAGED(TILE, WN, MB)                                                                         \
   extern "C" __global__ void __launch_bounds__(128 * WN, 2)                                                         \
-      tiler_gated_bf16_dx_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
-                                  const uint16_t* __restrict__ wg, const uint16_t* __restrict__ wu, uint32_t m,     \
-                                  uint32_t n, uint32_t k, uint16_t* __restrict__ dx, uint32_t splits,               \
+      tiler_gated_bf16_dx_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ wg,                 \
+                                  const uint16_t* __restrict__ wu, uint32_t ldk, uint32_t m, uint32_t n,            \
+                                  uint32_t k, uint16_t* __restrict__ dx, uint32_t splits,                           \
                                   float* __restrict__ partials) {                                                   \
-    gated_dx_staged<2, WN, MB>(dg, du, ld, wg, wu, m, n, k, dx, splits, partials);                                  \
+    gated_dx_staged<2, WN, MB>(dg, wg, wu, ldk, m, n, k, dx, splits, partials);                                     \
   }
 #define TILER_GATED_DW_STAGED(TILE, WN, MB)                                                                         \
   extern "C" __global__ void __launch_bounds__(128 * WN, 2)                                                         \
-      tiler_gated_bf16_dw_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ du, uint32_t ld,    \
-                                  const uint16_t* __restrict__ x, uint32_t m, uint32_t n, uint32_t k,               \
-                                  uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu) {                         \
-    gated_dw_staged<2, WN, MB>(dg, du, ld, x, m, n, k, dwg, dwu);                                                   \
+      tiler_gated_bf16_dw_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ x, uint32_t ldk,    \
+                                  uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ dwg,                   \
+                                  uint16_t* __restrict__ dwu, uint32_t splits, float* __restrict__ partials) {      \
+    gated_dw_staged<2, WN, MB>(dg, x, ldk, m, n, k, dwg, dwu, splits, partials);                                    \
   }
 TILER_GATED_TILES(96, 2, 3, 2)
 TILER_GATED_TILES(128, 2, 4, 2)

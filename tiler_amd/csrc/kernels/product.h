@@ -50,19 +50,10 @@ struct I8 {
   }
 };
 
-// Byte offset of 16-byte piece `id` of an operand tile in LDS, and which
-// piece of the operand it is: (row, piece along the depth) in row layout,
-// (depth row, 8-column piece) in column layout.
-template <uint32_t TILE, bool kCol>
-__device__ __forceinline__ uint32_t piece_offset(uint32_t outer, uint32_t inner) {
-  if constexpr (kCol) return outer * (TILE * 2u) + (((inner >> 1) ^ ((outer & 3u) | ((outer >> 1) & 4u))) << 5) + ((inner & 1u) << 4);
-  else return outer * kSlice + ((inner ^ ((outer >> 1) & 7u)) << 4);
+// Byte offset of a row's 16-byte piece in a row-layout tile.
+__device__ __forceinline__ uint32_t piece_offset(uint32_t row, uint32_t piece) {
+  return row * kSlice + ((piece ^ ((row >> 1) & 7u)) << 4);
 }
-template <uint32_t TILE, bool kCol>
-struct Pieces {
-  static constexpr uint32_t kPerOuter = kCol ? TILE / 8u : 8u;  // pieces of one row / depth row
-  static constexpr uint32_t kCount = TILE * 8u;
-};
 
 // A lane's fragments of BLOCKS 16-row blocks starting at row `row0` of a tile.
 template <uint32_t TILE, bool kCol, int BLOCKS>
@@ -97,84 +88,65 @@ struct Fragments {
   }
 };
 
-// An operand in memory: `rows` indices of the result, `depth` contracted ones,
-// `ld` elements between consecutive rows (row layout) or depth rows (column).
+// A row-layout operand in memory: `rows` rows of `depth` elements, one after
+// another.
 struct Operand {
   const uint8_t* base;
-  uint64_t ld;
   uint32_t rows, depth;
 };
-
-// Piece (outer, inner) of the tile at (row0, depth0), zero outside the operand.
-template <typename E, bool kCol>
-__device__ __forceinline__ u32x4 operand_piece(const Operand& o, uint32_t row0, uint32_t depth0, uint32_t outer,
-                                               uint32_t inner) {
-  constexpr uint32_t kPer = 16u / E::kBytes;
-  const uint32_t major = (kCol ? depth0 : row0) + outer, major_end = kCol ? o.depth : o.rows;
-  const uint32_t minor = (kCol ? row0 : depth0) + inner * kPer, minor_end = kCol ? o.rows : o.depth;
-  if (major >= major_end || minor >= minor_end) return u32x4{0, 0, 0, 0};
-  const uint64_t left = (uint64_t)(minor_end - minor) * E::kBytes;
-  return guarded_piece(o.base + (major * o.ld + minor) * E::kBytes, left < 16u ? (uint32_t)left : 16u, o.base);
-}
 
 // The guarded product, for any sizes and alignments: pieces come through
 // registers, two slices ahead of the products.  A loader's load is free of
 // branches, so that nothing waits between the loads: a piece that would pass
-// its row's end (or its depth row's) is the last whole one inside it, a row or
-// depth row past the last is the last one again.  store puts the pieces into
-// LDS and, in the slices and tiles that need it, moves their elements into
-// place and clears what lies past the depth; what lies past the last row or
-// column only reaches results that are not stored.
-template <typename E, bool kCol, uint32_t TILE, uint32_t THREADS>
+// its row's end is the last whole one inside it, a row past the last is the last
+// one again.  store puts the pieces into LDS and, in the last slice, moves their
+// elements into place and clears what lies past the depth; rows past the last
+// only reach results that are not stored.
+template <typename E, uint32_t TILE, uint32_t THREADS>
 struct GuardedLoader {
-  static constexpr uint32_t kLoads = TILE * 8u / THREADS, kOuter = kCol ? TILE / 8u : 8u, kPer = 16u / E::kBytes;
-  static constexpr uint32_t kDepth = kCol ? 64u : kSlice / E::kBytes;  // depth elements per slice
+  static constexpr uint32_t kLoads = TILE * 8u / THREADS;
   static_assert(TILE * 8u % THREADS == 0, "whole pieces per thread");
   Operand o;
   uint32_t row0, row_bytes;
   __device__ __forceinline__ GuardedLoader(const Operand& o_, uint32_t row0_)
-      : o(o_), row0(row0_), row_bytes((kCol ? o_.rows : o_.depth) * E::kBytes) {}
-  // `base`: the operand's storage (one of two, in the products over two segments of depth).
+      : o(o_), row0(row0_), row_bytes(o_.depth * E::kBytes) {}
+  // `base`: the operand's storage (either weight's, in the gated product).
   __device__ __forceinline__ void load(const uint8_t* base, uint32_t t, u32x4 (&v)[kLoads]) const {
-    const uint8_t* from = base + (kCol ? (uint64_t)t * 64u : (uint64_t)row0) * o.ld * E::kBytes;
-    const uint32_t last = kCol ? o.depth - 1u - t * 64u : o.rows - 1u - row0;  // outer's
-    const uint32_t in0 = kCol ? row0 * E::kBytes : t * kSlice, in_last = row_bytes - 16u;
+    const uint8_t* from = base + (uint64_t)row0 * row_bytes;
+    const uint32_t last = o.rows - 1u - row0, in_last = row_bytes - 16u;
 #pragma unroll
     for (uint32_t q = 0; q < kLoads; ++q) {
-      const uint32_t id = threadIdx.x + q * THREADS, outer = id / kOuter, in = in0 + id % kOuter * 16u;
-      const uint32_t off = (outer < last ? outer : last) * (uint32_t)(o.ld * E::kBytes) + (in < in_last ? in : in_last);
-      v[q] = *reinterpret_cast<const u32x4_any*>(from + off);
+      const uint32_t id = threadIdx.x + q * THREADS, row = id / 8u, in = t * kSlice + id % 8u * 16u;
+      v[q] = *reinterpret_cast<const u32x4_any*>(from + (row < last ? row : last) * row_bytes + (in < in_last ? in : in_last));
     }
   }
   __device__ __forceinline__ void store(uint32_t t, uint8_t* tile, u32x4 (&v)[kLoads]) const {
-    const uint32_t in0 = kCol ? row0 * E::kBytes : t * kSlice;
-    const bool cut = in0 + kOuter * 16u > row_bytes, ends = kCol && (t + 1u) * 64u > o.depth;
+    const bool cut = (t + 1u) * kSlice > row_bytes;
 #pragma unroll
     for (uint32_t q = 0; q < kLoads; ++q) {
-      const uint32_t id = threadIdx.x + q * THREADS, outer = id / kOuter, inner = id % kOuter;
+      const uint32_t id = threadIdx.x + q * THREADS;
       if (cut) {
-        const uint32_t end = in0 + inner * 16u + 16u;
+        const uint32_t end = t * kSlice + id % 8u * 16u + 16u;
         if (end > row_bytes) v[q] = end - row_bytes >= 16u ? u32x4{0, 0, 0, 0} : tiler_pieces::drop_bytes(v[q], end - row_bytes);
       }
-      if (ends && t * 64u + outer >= o.depth) v[q] = u32x4{0, 0, 0, 0};
-      *reinterpret_cast<u32x4*>(tile + piece_offset<TILE, kCol>(outer, inner)) = v[q];
+      *reinterpret_cast<u32x4*>(tile + piece_offset(id / 8u, id % 8u)) = v[q];
     }
   }
 };
-// The same for operands with rows of less than a piece: checked piece by piece.
-template <typename E, bool kCol, uint32_t TILE, uint32_t THREADS>
+// The same for rows of less than a piece (one slice): checked piece by piece.
+template <typename E, uint32_t TILE, uint32_t THREADS>
 struct TinyLoader {
-  static constexpr uint32_t kLoads = TILE * 8u / THREADS, kOuter = kCol ? TILE / 8u : 8u;
-  static constexpr uint32_t kDepth = kCol ? 64u : kSlice / E::kBytes;
+  static constexpr uint32_t kLoads = TILE * 8u / THREADS;
   Operand o;
   uint32_t row0;
   __device__ __forceinline__ TinyLoader(const Operand& o_, uint32_t row0_) : o(o_), row0(row0_) {}
-  __device__ __forceinline__ void load(const uint8_t* base, uint32_t t, u32x4 (&v)[kLoads]) const {
-    const Operand here{base, o.ld, o.rows, o.depth};
+  __device__ __forceinline__ void load(const uint8_t* base, uint32_t, u32x4 (&v)[kLoads]) const {
+    const uint32_t bytes = o.depth * E::kBytes;
 #pragma unroll 1
     for (uint32_t q = 0; q < kLoads; ++q) {
-      const uint32_t id = threadIdx.x + q * THREADS;
-      const u32x4 p = operand_piece<E, kCol>(here, row0, t * kDepth, id / kOuter, id % kOuter);
+      const uint32_t id = threadIdx.x + q * THREADS, row = row0 + id / 8u;
+      u32x4 p = {0, 0, 0, 0};
+      if (row < o.rows && id % 8u == 0) p = guarded_piece(base + (uint64_t)row * bytes, bytes, base);
 #pragma unroll
       for (uint32_t x = 0; x < kLoads; ++x)
         if (x == q) v[x] = p;
@@ -184,28 +156,26 @@ struct TinyLoader {
 #pragma unroll
     for (uint32_t q = 0; q < kLoads; ++q) {
       const uint32_t id = threadIdx.x + q * THREADS;
-      *reinterpret_cast<u32x4*>(tile + piece_offset<TILE, kCol>(id / kOuter, id % kOuter)) = v[q];
+      *reinterpret_cast<u32x4*>(tile + piece_offset(id / 8u, id % 8u)) = v[q];
     }
   }
 };
 
 // load_a(t, pieces) and load_b fetch a slice, store_a(t, tile, pieces) and
 // store_b put it into LDS; WM x WN waves of MB x NB blocks of 16 x 16.
-template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, typename LA, typename LB, typename SA,
-          typename SB>
+template <typename E, int WM, int WN, int MB, int NB, typename LA, typename LB, typename SA, typename SB>
 __device__ __forceinline__ void guarded_product(uint8_t* smem, uint32_t slices, LA load_a, LB load_b, SA store_a,
                                                 SB store_b, typename E::Acc (&acc)[MB][NB]) {
   constexpr uint32_t kThreads = 64u * WM * WN, kRowsA = WM * MB * 16u, kRowsB = WN * NB * 16u;
   constexpr uint32_t kLoadsA = kRowsA * 8u / kThreads, kLoadsB = kRowsB * 8u / kThreads;
   constexpr uint32_t kStage = (kRowsA + kRowsB) * kSlice;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const Fragments<kRowsA, kACol, MB> ra((wave / WN) * MB * 16u, lane);
-  const Fragments<kRowsB, kBCol, NB> rb((wave % WN) * NB * 16u, lane);
+  const Fragments<kRowsA, false, MB> ra((wave / WN) * MB * 16u, lane);
+  const Fragments<kRowsB, false, NB> rb((wave % WN) * NB * 16u, lane);
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = E::zero();
-  if (slices == 0) return;
   u32x4 pa[2][kLoadsA], pb[2][kLoadsB];
   auto load = [&](uint32_t t, auto slot) {
     load_a(t, pa[decltype(slot)::value]);
@@ -326,6 +296,7 @@ struct ColumnLoader {
                                           uint32_t wave, uint32_t lane)
       : base(base_), row_bytes(ld * 2u), depth(depth_), before_bytes(before * 2u), lds0(wave * LOADS * 1024u) {
     constexpr uint32_t kPer = TILE / 8u;
+    static_assert(TILE >= 128 && (TILE & (TILE - 1u)) == 0, "eight blocks of a row change places");
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const uint32_t id = (wave * LOADS + j) * 64u + lane, outer = id / kPer, slot = id % kPer;

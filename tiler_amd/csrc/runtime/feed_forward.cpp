@@ -269,15 +269,34 @@ uint32_t guarded_rows(const Target& t, uint64_t m, uint64_t column_tiles) {
   return m <= 64 || mul_sat(ceil_div(m, 64), column_tiles) <= t.compute_units ? 64 : 128;
 }
 
-// The gradients' tiles: 256 when they go round the CUs at least once, else 128
-// (four times as many, two to a CU).
-uint32_t staged_tile(const Target& t, uint64_t m, uint64_t n) {
-  return mul_sat(ceil_div(m, 256), ceil_div(n, 256)) >= t.compute_units ? 256 : 128;
+// The gradients' products: tiles of 256 (one to a CU) or 128 (two to a CU), their
+// depth split over `splits` workgroups a tile where the tiles alone leave CUs
+// idle, the binary32 partials added by one more launch.  The least of the same
+// estimates, the partials' passes at 4.5 bytes a ns.
+struct GradientForm {
+  uint32_t tile, splits;
+  uint64_t tiles;
+};
+GradientForm gradient_form(const Target& t, uint64_t halves, uint64_t rows, uint64_t cols, uint64_t slices) {
+  GradientForm best{0, 1, 0};
+  double least = 0;
+  for (const uint32_t tile : {256u, 128u}) {
+    const uint64_t tiles = mul_sat(halves * ceil_div(rows, tile), ceil_div(cols, tile));
+    if (!grid_holds(tiles, 512)) continue;
+    for (uint32_t splits = 1; splits <= 32 && (splits == 1 || splits * 2 <= slices); ++splits) {
+      const double q = std::ceil((double)tiles * splits / t.compute_units), s = (double)ceil_div(slices, splits);
+      const double pairs = std::floor(q / 2);
+      double us = tile == 256 ? q * (7.5 + 1.2 * s) : pairs * (3.9 + 0.85 * s) + (q - 2 * pairs) * (3.0 + 0.6 * s);
+      if (splits > 1) us += 3 + (double)splits * halves * rows * cols * 8 / 4.5e6;
+      if (!best.tile || us < least) best = {tile, splits, tiles}, least = us;
+    }
+  }
+  return best;
 }
 
-Launch& add_tiles(Program& p, const std::string& stem, uint32_t tile, uint64_t tiles) {
-  const std::string name = stem + "_t" + std::to_string(tile);
-  return p.add(name.c_str(), (uint32_t)tiles, 1, tile == 256 ? 512 : 256);
+Launch& add_gradient(Program& p, const char* stem, const GradientForm& f) {
+  const std::string name = std::string(stem) + "_t" + std::to_string(f.tile);
+  return p.add(name.c_str(), (uint32_t)f.tiles, f.splits, f.tile == 256 ? 512 : 256);
 }
 
 }  // namespace
@@ -306,8 +325,9 @@ tiler_hip_status plan_gated_contract_bf16(const Target& t, uint32_t parts, uint6
   return TILER_HIP_OK;
 }
 
-// Slots: x, wg, wu, gate, up, dh, [dx,] [dwg, dwu,] dG, dU (scratch:
-// rows of n rounded up to 64 elements).
+// Slots: x, wg, wu, gate, up, dh, [dx,] [dwg, dwu,] and scratch: dG with dU
+// behind it, copies of x and of the weights where their rows do not start on 16
+// bytes, partial sums of dx.
 tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t parts, uint64_t m, uint64_t n, uint64_t k,
                                                    const uintptr_t* addr, Program& p) {
   if (parts & ~(uint32_t)(TILER_HIP_GATED_DX | TILER_HIP_GATED_DW))
@@ -319,53 +339,54 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
   const uint32_t dx = has_dx ? p.slot(in, kSlotOutput) : 0;
   const uint32_t dwg = has_dw ? p.slot(weight, kSlotOutput) : 0, dwu = has_dw ? p.slot(weight, kSlotOutput) : 0;
   if (tiler_hip_status st = check_product(m, n, k, p); st != TILER_HIP_OK) return st;
-  if (n >= (1ull << 22)) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
+  if (n > (1ull << 22) - 64 || k > (1ull << 22) - 64)  // 256 of their rows lie within one buffer resource
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
   if (!parts) return TILER_HIP_OK;
-  const uint64_t ld = ceil_div(n, 64) * 64, half = mul_sat(mul_sat(m, ld), 2);
-  const uint32_t dg = p.slot(half, kSlotScratch), du = p.slot(half, kSlotScratch);
-  const uint32_t m32 = (uint32_t)m, n32 = (uint32_t)n, k32 = (uint32_t)k, ld32 = (uint32_t)ld;
+  const uint64_t ld = ceil_div(n, 64) * 64, ldk = ceil_div(k, 8) * 8;
+  const uint32_t dg = p.slot(mul_sat(mul_sat(m, ld), 4), kSlotScratch);
+  const uint32_t m32 = (uint32_t)m, n32 = (uint32_t)n, k32 = (uint32_t)k;
+  // The products run over n and over m: nothing of the operands is read where either is 0.
+  const bool copy_w = has_dx && m && n && !(k % 8 == 0 && aligned16(addr[wg]) && aligned16(addr[wu]));
+  const bool copy_x = has_dw && m && n && !(k % 8 == 0 && aligned16(addr[x]));
+  const uint32_t to_x = copy_x ? p.slot(mul_sat(mul_sat(m, ldk), 2), kSlotScratch) : 0;
+  const uint32_t to_w = copy_w ? p.slot(mul_sat(mul_sat(n, ldk), 4), kSlotScratch) : 0;
   if (m && n) {
-    const uint64_t groups = ceil_div(m * (ld / 8), 256);
-    p.add("tiler_gated_bf16_grad", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
-        .ptr(gate).ptr(up).ptr(dh).u32(m32).u32(n32).u32(ld32).ptr(dg).ptr(du);
+    const uint64_t mids = m * (ld / 8), copies = ((copy_x ? m : 0) + (copy_w ? 2 * n : 0)) * (ldk / 8);
+    const uint64_t groups = ceil_div(mids > copies ? mids : copies, 256);
+    Launch& l = p.add("tiler_gated_bf16_grad", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
+                    .ptr(gate).ptr(up).ptr(dh).ptr(x).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dg);
+    slot_or_null(l, copy_x, to_x);
+    slot_or_null(l, copy_w, to_w);
   }
-  // Columns of the weights and of x (k of them a row) are read in 16-byte pieces.
-  const bool rows_ok = staged_rows(2 * k) && staged_rows(2 * ld);
+  const GradientForm fx = gradient_form(t, 1, m, k, n ? 2 * (ld / 64) : 0), fw = gradient_form(t, 2, n, k, ceil_div(m, 64));
+  if ((has_dx && m && !fx.tile) || (has_dw && n && !fw.tile))
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
+  const bool sum_x = has_dx && m && fx.splits > 1, sum_w = has_dw && n && fw.splits > 1;
+  const uint32_t of_x = sum_x ? p.slot(mul_sat(mul_sat(fx.splits, m * k), 4), kSlotScratch) : 0;
+  const uint32_t of_w = sum_w ? p.slot(mul_sat(mul_sat(fw.splits, n * k), 8), kSlotScratch) : 0;
   if (has_dx && m) {
-    // The depth 2 n of dx is split over as many workgroups as fill the chip
-    // twice (two 128-tiles to a CU) where the tiles alone do not: at least
-    // four slices each, the binary32 partials added by one more launch.
-    const bool staged = rows_ok && aligned16(addr[wg]) && aligned16(addr[wu]);
-    const uint32_t tile = staged ? staged_tile(t, m, k) : 128;
-    const uint64_t tiles = mul_sat(ceil_div(m, tile), ceil_div(k, tile)), slices = 2 * (ld / 64);
-    uint64_t splits = 1;
-    if (tile == 128 && tiles < 2ull * t.compute_units) {
-      splits = 2ull * t.compute_units / tiles;
-      if (splits > slices / 4) splits = slices / 4;
-      if (splits > 32) splits = 32;
-      if (splits == 0) splits = 1;
-    }
-    if (!grid_holds(tiles, 512)) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
-    const uint32_t partials = splits > 1 ? p.slot(mul_sat(mul_sat(splits, m * k), 4), kSlotScratch) : 0;
-    Launch& l = staged ? add_tiles(p, "tiler_gated_bf16_dx", tile, tiles) : p.add("tiler_gated_bf16_dx_g", (uint32_t)tiles, 1, 256);
-    l.grid[1] = (uint32_t)splits;
-    l.ptr(dg).ptr(du).u32(ld32).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dx).u32((uint32_t)splits);
-    slot_or_null(l, splits > 1, partials);
-    if (splits > 1) {
-      const uint64_t groups = ceil_div(m * k, 256);
-      p.add("tiler_gated_bf16_dx_sum", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
-          .ptr(partials).u32((uint32_t)splits).u64(m * k).ptr(dx);
-    }
+    Launch& l = add_gradient(p, "tiler_gated_bf16_dx", fx).ptr(dg).ptr(copy_w ? to_w : wg);
+    slot_or_null(l, !copy_w, wu);
+    l.u32((uint32_t)(copy_w ? ldk : k)).u32(m32).u32(n32).u32(k32).ptr(dx).u32(fx.splits);
+    slot_or_null(l, sum_x, of_x);
   }
   if (has_dw && n) {
-    const uint32_t tile = staged_tile(t, 2 * n, k);
-    const uint64_t tiles = mul_sat(2 * ceil_div(n, tile), ceil_div(k, tile));
-    if (rows_ok && aligned16(addr[x]) && grid_holds(tiles, 512))
-      add_tiles(p, "tiler_gated_bf16_dw", tile, tiles)
-          .ptr(dg).ptr(du).u32(ld32).ptr(x).u32(m32).u32(n32).u32(k32).ptr(dwg).ptr(dwu);
-    else
-      p.add("tiler_gated_bf16_dw_g", (uint32_t)ceil_div(k, 128), (uint32_t)(2 * ceil_div(n, 128)), 256)
-          .ptr(dg).ptr(du).u32(ld32).ptr(x).u32(m32).u32(n32).u32(k32).u32((uint32_t)ceil_div(n, 128)).ptr(dwg).ptr(dwu);
+    Launch& l = add_gradient(p, "tiler_gated_bf16_dw", fw)
+                    .ptr(dg).ptr(copy_x ? to_x : x).u32((uint32_t)(copy_x ? ldk : k)).u32(m32).u32(n32).u32(k32)
+                    .ptr(dwg).ptr(dwu).u32(fw.splits);
+    slot_or_null(l, sum_w, of_w);
+  }
+  if (sum_x || sum_w) {
+    const uint64_t pieces = (sum_x ? ceil_div(m * k, 4) : 0) + (sum_w ? 2 * ceil_div(n * k, 4) : 0);
+    const uint64_t groups = ceil_div(pieces, 256);
+    Launch& l = p.add("tiler_gated_bf16_sum", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256);
+    slot_or_null(l, sum_x, of_x);
+    l.u32(fx.splits).u64(sum_x ? m * k : 0);
+    slot_or_null(l, sum_x, dx);
+    slot_or_null(l, sum_w, of_w);
+    l.u32(fw.splits).u64(sum_w ? n * k : 0);
+    slot_or_null(l, sum_w, dwg);
+    slot_or_null(l, sum_w, dwu);
   }
   return TILER_HIP_OK;
 }

@@ -363,9 +363,7 @@ const EntryRow kEntries[] = {
     {"tiler_layer_norm_columns_f32", "layer-norm-backward-f32", 5},
     {"tiler_layer_norm_columns_final_bf16", "layer-norm-backward/bf16", 3},
     {"tiler_layer_norm_columns_final_f32", "layer-norm-backward-f32", 3},
-    {"tiler_gated_bf16_grad", "gated-contraction-bf16-backward", 5},
-    {"tiler_gated_bf16_dx_g", "gated-contraction-bf16-backward", 6},
-    {"tiler_gated_bf16_dw_g", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_grad", "gated-contraction-bf16-backward", 9},
 #define TILER_ROW_FORM(FORM)                                                   \
   {"tiler_layer_norm_bf16_" FORM, "layer-norm/bf16", 6},                        \
       {"tiler_layer_norm_f32_" FORM, "layer-norm-f32", 6},                      \
@@ -382,9 +380,9 @@ const EntryRow kEntries[] = {
     TILER_GRAD_FORM("w1c1"), TILER_GRAD_FORM("w2c1"), TILER_GRAD_FORM("w4c1"), TILER_GRAD_FORM("w8c1"),
     TILER_GRAD_FORM("w16c1"), TILER_GRAD_FORM("w16c2"),
 #undef TILER_GRAD_FORM
-    {"tiler_gated_bf16_dx_t128", "gated-contraction-bf16-backward", 6},
-    {"tiler_gated_bf16_dx_t256", "gated-contraction-bf16-backward", 6},
-    {"tiler_gated_bf16_dx_sum", "gated-contraction-bf16-backward", 2},
+    {"tiler_gated_bf16_dx_t128", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_dx_t256", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_sum", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dw_t128", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dw_t256", "gated-contraction-bf16-backward", 5},
 #define TILER_GATED_FORM(FORM) {"tiler_gated_bf16_" FORM, "gated-contraction-bf16", 6}
