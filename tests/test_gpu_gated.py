@@ -146,6 +146,24 @@ def test_backward_whole_numbers(ctx, mem, m, n, k):
         assert np.array_equal(g, bf(v)), np.argwhere(g != bf(v))[:4]
 
 
+# (dx's tile and whether its depth is split, the weights' gradients'), odd k: copied operands
+GRADIENT_FORMS = [(128, False, 128, False, 100, 72, 72), (128, True, 128, False, 300, 264, 265),
+                  (128, True, 256, False, 300, 1000, 4104), (128, False, 128, True, 520, 72, 72),
+                  (128, True, 128, True, 777, 264, 71), (256, True, 128, False, 1000, 2056, 4104),
+                  (256, True, 256, False, 2050, 2056, 2055), (256, False, 128, True, 2050, 72, 4104),
+                  (256, False, 256, False, 2050, 1000, 4104)]
+
+
+@pytest.mark.parametrize("tile_x,split_x,tile_w,split_w,m,n,k", GRADIENT_FORMS)
+def test_backward_forms(ctx, mem, tile_x, split_x, tile_w, split_w, m, n, k):
+    rz = realize(L.PROGRAM_GATED_CONTRACTION_BACKWARD, (m, n, k), dtype=L.BF16, variant=L.GATED_DX | L.GATED_DW,
+                 permissions=L.PERMITS_REASSOCIATION, flags=L.REGION_ALIGNED16)
+    names = ["tiler_gated_bf16_grad", f"tiler_gated_bf16_dx_t{tile_x}", f"tiler_gated_bf16_dw_t{tile_w}"]
+    assert rz.symbols == names + ["tiler_gated_bf16_sum"] * (split_x or split_w)
+    assert [d.grid[1] > 1 for d in rz.dispatches[1:3]] == [split_x, split_w]
+    test_backward_whole_numbers(ctx, mem, m, n, k)
+
+
 @pytest.mark.parametrize("want", [(True, False), (False, True), (False, False)])
 def test_backward_parts(ctx, mem, want):
     rng = np.random.default_rng(9)
