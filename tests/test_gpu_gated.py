@@ -102,9 +102,10 @@ def test_forward_whole_numbers(ctx, mem, m, n, k):
 # Every form of the product, shallower and deeper than the slices it keeps in LDS
 FORMS = [("few1x1", 3, 24, 528), ("few2x1", 17, 2056, 1040), ("few4x1", 33, 2056, 1040), ("few4x2", 33, 4104, 1040),
          ("t64_d", 33, 4104, 528), ("t64_d", 3, 14344, 528), ("t96_d", 70, 8200, 1040), ("t128_d", 100, 8200, 528),
-         ("t96", 17, 24, 16), ("t96", 17, 20008, 1040), ("t128", 301, 4104, 16), ("t128", 100, 20008, 1040),
-         ("t160", 400, 8200, 16), ("t160", 130, 8200, 1040), ("t192", 333, 12008, 16), ("t192", 333, 12008, 1040),
-         ("t256", 400, 12008, 16), ("t256", 400, 12008, 1040), ("g64", 70, 200, 333), ("g128", 300, 4099, 65)]
+         ("t64_d", 3, 14344, 272), ("t96", 17, 24, 16), ("t96", 33, 20008, 1040), ("t128", 301, 8200, 16),
+         ("t128", 100, 20008, 1040), ("t160_w", 400, 8200, 1040), ("t192_n", 130, 8200, 1040),
+         ("t256_n", 200, 12008, 1040), ("t192", 520, 8200, 16), ("t192", 333, 12008, 1040), ("t256", 400, 14344, 80),
+         ("t256", 400, 12008, 1040), ("g64", 70, 200, 333), ("g128", 300, 4099, 65)]
 
 
 @pytest.mark.parametrize("form,m,n,k", FORMS)

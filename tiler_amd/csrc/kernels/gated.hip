@@ -246,20 +246,22 @@ __device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, con
                                              uint16_t* __restrict__ h, uint16_t* __restrict__ gate,
                                              uint16_t* __restrict__ up) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kRowsB = WN * 64u, kCols = kRowsB / 2u, kThreads = 64u * WM * WN;
-  constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kRowsB / 8 / (WM * WN);
-  static_assert(kLoadsB == 4, "a wave's 32 rows of B lie in one of the two weights");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * (kRowsA + kRowsB) * kSlice];
+  constexpr int kLoadsA = (kRowsA / 8 + WM * WN - 1) / (WM * WN), kLoadsB = kRowsB / 8 / (WM * WN);
+  static_assert(kLoadsB == 4 || kLoadsB == 2, "a wave's rows of B lie in one of the two weights");
+  constexpr bool kUneven = kRowsA % (8 * WM * WN) != 0;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * (kRowsA + kRowsB) * kSlice + (kUneven ? 1024u : 0u)];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t tm, tn;
   tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (n + kCols - 1u) / kCols, tm, tn);
   const uint32_t m0 = tm * kRowsA, n0 = tn * kCols;
-  const tiler_product::RowLoader<Bf16, kLoadsA> la(reinterpret_cast<const uint8_t*>(x + (uint64_t)m0 * k), k,
-                                                   m - m0 < kRowsA ? m - m0 : kRowsA, k, wave * kLoadsA * 8u,
-                                                   wave * kLoadsA * 8u, lane);
-  // LDS rows 32 w .. 32 w + 31 of B: columns 32 (w / 2) .. of the gate's (w even) or the up projection's weight
+  const tiler_product::RowLoader<Bf16, kLoadsA, kUneven ? kRowsA : ~0u> la(
+      reinterpret_cast<const uint8_t*>(x + (uint64_t)m0 * k), k, m - m0 < kRowsA ? m - m0 : kRowsA, k, wave * kLoadsA * 8u,
+                                                   wave * kLoadsA * 8u, lane, smem + S * (kRowsA + kRowsB) * kSlice);
+  // B's LDS rows 64 c .. 64 c + 31 are columns 32 c .. of the gate's weight, the next 32 of the up projection's
+  const uint32_t b0 = wave * kLoadsB * 8u;
   const tiler_product::RowLoader<Bf16, kLoadsB> lb(
-      reinterpret_cast<const uint8_t*>(((wave & 1u) ? wu : wg) + (uint64_t)n0 * k), k, n - n0 < kCols ? n - n0 : kCols,
-      k, (wave >> 1) * 32u, wave * 32u, lane);
+      reinterpret_cast<const uint8_t*>(((b0 & 32u) ? wu : wg) + (uint64_t)n0 * k), k, n - n0 < kCols ? n - n0 : kCols,
+      k, (b0 >> 6) * 32u + (b0 & 31u), b0, lane);
   f32x4 acc[MB][4];
   tiler_product::staged_product<Bf16, false, false, WM, WN, MB, 4, kLoadsA + kLoadsB, S>(
       smem, (k + 63u) / 64u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
@@ -360,17 +362,20 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
 }  // namespace
 
 // Four waves: two workgroups to a CU; eight: one.  Two waves a SIMD in either.
-// The deep forms (_d) keep as many slices in LDS as it holds, for the grids that
-// give a CU one workgroup: there a slice's time is its loads' latency over the
-// slices in flight.  (Their bound of 512 threads, of which 256 run, keeps the
-// compiler to 256 registers: given 512, it spreads them over the accumulation
-// registers and copies them back and forth.)
-#define TILER_GATED_TILES(NAME, WN, MB, S)                                                                          \
-  extern "C" __global__ void __launch_bounds__(S > 2 ? 512 : 128 * WN, 2)                                       \
+// What LDS holds decides what is in flight, and that a slice's time where the
+// weights come from memory: eight waves with three slices of a smaller tile (_n:
+// 64 columns of each projection, _w: 128) against two of a larger, us, 256 x
+// 14336 x 4096: 66 (256_n; with two slices 89) / 104 (256); 301 of them: 80
+// (160_w) / 90 (192).  The deep forms (_d), four waves and one workgroup to a
+// CU, are for grids that give a CU one workgroup in any case.  (Their bound of 512
+// threads, of which 256 run, keeps the compiler to 256 registers: given 512, it
+// spreads them over the accumulation registers and copies them back and forth.)
+#define TILER_GATED_TILES(NAME, WM, WN, MB, S)                                                                          \
+  extern "C" __global__ void __launch_bounds__(S > 2 ? 512 : 64 * WM * WN, 2)                                       \
       tiler_gated_bf16_t##NAME(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,                     \
                                const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k,                 \
                                uint16_t* __restrict__ h, uint16_t* __restrict__ gate, uint16_t* __restrict__ up) {  \
-    gated_staged<2, WN, MB, S>(x, wg, wu, m, n, k, h, gate, up);                                                    \
+    gated_staged<WM, WN, MB, S>(x, wg, wu, m, n, k, h, gate, up);                                                    \
   }
 #define TILER_GATED_DX_STAGED(TILE, WN, MB)                                                                         \
   extern "C" __global__ void __launch_bounds__(128 * WN, 2)                                                         \
@@ -387,14 +392,16 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
                                   uint16_t* __restrict__ dwu, uint32_t splits, float* __restrict__ partials) {      \
     gated_dw_staged<2, WN, MB>(dg, x, ldk, m, n, k, dwg, dwu, splits, partials);                                    \
   }
-TILER_GATED_TILES(96, 2, 3, 2)
-TILER_GATED_TILES(128, 2, 4, 2)
-TILER_GATED_TILES(160, 2, 5, 2)
-TILER_GATED_TILES(192, 4, 6, 2)
-TILER_GATED_TILES(256, 4, 8, 2)
-TILER_GATED_TILES(64_d, 2, 2, 6)
-TILER_GATED_TILES(96_d, 2, 3, 5)
-TILER_GATED_TILES(128_d, 2, 4, 4)
+TILER_GATED_TILES(96, 2, 2, 3, 2)
+TILER_GATED_TILES(128, 2, 2, 4, 2)
+TILER_GATED_TILES(192, 2, 4, 6, 2)
+TILER_GATED_TILES(256, 2, 4, 8, 2)
+TILER_GATED_TILES(192_n, 4, 2, 3, 3)
+TILER_GATED_TILES(256_n, 4, 2, 4, 3)
+TILER_GATED_TILES(160_w, 2, 4, 5, 3)
+TILER_GATED_TILES(64_d, 2, 2, 2, 6)
+TILER_GATED_TILES(96_d, 2, 2, 3, 5)
+TILER_GATED_TILES(128_d, 2, 2, 4, 4)
 TILER_GATED_DX_STAGED(128, 2, 4)
 TILER_GATED_DX_STAGED(256, 4, 8)
 TILER_GATED_DW_STAGED(128, 2, 4)

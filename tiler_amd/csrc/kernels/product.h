@@ -250,21 +250,29 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const uint8_t* base, 
 
 // TILE rows from `base`, `rows` of them real; `wave_rows` where this wave's
 // LOADS * 8 rows start in memory and `wave_lds` where they go in the tile (the
-// gated product's weights interleave two matrices).
-template <typename E, int LOADS>
+// gated product's weights interleave two matrices).  Where the waves' rows are
+// more than the tile's, the loads past it bring zeros to `spare` (1024 bytes),
+// so that every wave counts the same loads.
+template <typename E, int LOADS, uint32_t TILE = ~0u>
 struct RowLoader {
   const uint8_t* base;
   uint32_t span, depth_bytes, lds0;
+  uint8_t* spare;
   uint32_t voff[LOADS], piece[2];
   __device__ __forceinline__ RowLoader(const uint8_t* base_, uint64_t ld, uint32_t rows, uint32_t depth,
-                                       uint32_t wave_rows, uint32_t wave_lds, uint32_t lane)
-      : base(base_), span((uint32_t)(rows * ld * E::kBytes)), depth_bytes(depth * E::kBytes), lds0(wave_lds * kSlice) {
+                                       uint32_t wave_rows, uint32_t wave_lds, uint32_t lane, uint8_t* spare_ = nullptr)
+      : base(base_), span((uint32_t)(rows * ld * E::kBytes)), depth_bytes(depth * E::kBytes), lds0(wave_lds * kSlice),
+        spare(spare_) {
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const uint32_t in = (lane & 7u) ^ (((wave_lds + j * 8u + (lane >> 3)) >> 1) & 7u);
       if (j < 2) piece[j] = in * 16u;
-      voff[j] = (wave_rows + j * 8u + (lane >> 3)) * (uint32_t)(ld * E::kBytes) + in * 16u;
+      voff[j] = past(j) ? kPastEnd : (wave_rows + j * 8u + (lane >> 3)) * (uint32_t)(ld * E::kBytes) + in * 16u;
     }
+  }
+  __device__ __forceinline__ bool past(int j) const { return TILE != ~0u && lds0 + j * 1024u >= TILE * kSlice; }
+  __device__ __forceinline__ lds_bytes* place(uint8_t* tile, int j) const {
+    return (lds_bytes*)(past(j) ? spare : tile + lds0 + j * 1024u);
   }
   __device__ __forceinline__ void issue(uint32_t t, uint8_t* tile) const { issue(base, t, tile); }
   __device__ __forceinline__ void issue(const uint8_t* from, uint32_t t, uint8_t* tile) const {
@@ -273,11 +281,11 @@ struct RowLoader {
     if (left >= kSlice) {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (lds_bytes*)(tile + lds0 + j * 1024u), 16, voff[j], 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, place(tile, j), 16, voff[j], 0, 0, 0);
     } else {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (lds_bytes*)(tile + lds0 + j * 1024u), 16,
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, place(tile, j), 16,
                                                  piece[j & 1] < left ? voff[j] : kPastEnd, 0, 0, 0);
     }
   }

@@ -190,8 +190,8 @@ bool staged_rows(uint64_t row_bytes) { return row_bytes % 16 == 0 && row_bytes *
 //   kFew   a slice in eight a wave, t = ceil(s / 8)
 //                                     c0 + q (c1 + c2 t) + c3 t + c4 t max(W / CUs, 1)
 // The constants are least squares fits of measured times (m 1 .. 4096, n 600 ..
-// 14336, k 800 .. 8192, at most 3000 workgroups): within 5% in the mean, and the
-// form of the least estimate is 1.2% slower than the fastest in the mean.
+// 28672, k 800 .. 8192, at most 3000 workgroups): the form of the least estimate
+// is 1% slower than the fastest in the mean.
 struct ProductForm {
   const char* name;
   uint32_t rows, cols, threads;
@@ -199,21 +199,23 @@ struct ProductForm {
   double c[5];
 };
 
-// us, by size: 16 x 14336 x 4096 45 (few1x1), t64_d 100; 301 x 14336 x 4096: t160 86,
-// t192 90, t128 119; 4096 x 14336 x 4096: t256 740, t128 830.
+// us, by size: 16 x 14336 x 4096 few1x1 45, t64_d 100; 301 of them t160_w 80, t192 90,
+// t128 124; 4096 of them t256 740, t128 830; 512 x 4096 x 4096 t128_d 39, t256_n 52.
 constexpr ProductForm kGatedForms[] = {
     {"few1x1", 16, 16, 512, ProductForm::kFew, {2.591, 0.235, 0.356, 0.131, 0.151}},
     {"few2x1", 32, 16, 512, ProductForm::kFew, {2.524, 0.481, 0.610, 0, 0.115}},
     {"few4x1", 64, 16, 512, ProductForm::kFew, {1.224, 1.963, 0.888, 0, 0.142}},
     {"few4x2", 64, 32, 512, ProductForm::kFew, {1.264, 2.788, 1.431, 0, 0}},
-    {"t64_d", 64, 64, 256, ProductForm::kOne, {1.756, 2.011, 0.340}},
-    {"t96_d", 96, 64, 256, ProductForm::kOne, {1.799, 2.356, 0.428}},
-    {"t128_d", 128, 64, 256, ProductForm::kOne, {1.449, 2.893, 0.503}},
-    {"t96", 96, 64, 256, ProductForm::kTwo, {0.141, 3.587, 0.708, 2.314, 0.574}},
-    {"t128", 128, 64, 256, ProductForm::kTwo, {0.554, 3.867, 0.848, 3.017, 0.604}},
-    {"t160", 160, 64, 256, ProductForm::kTwo, {1.673, 3.506, 1.020, 2.685, 0.628}},
-    {"t192", 192, 128, 512, ProductForm::kOne, {0, 6.314, 0.976}},
-    {"t256", 256, 128, 512, ProductForm::kOne, {0, 7.471, 1.199}},
+    {"t64_d", 64, 64, 256, ProductForm::kOne, {1.747, 1.993, 0.351}},
+    {"t96_d", 96, 64, 256, ProductForm::kOne, {1.914, 2.338, 0.435}},
+    {"t128_d", 128, 64, 256, ProductForm::kOne, {1.567, 2.883, 0.511}},
+    {"t96", 96, 64, 256, ProductForm::kTwo, {0.826, 2.393, 0.767, 1.920, 0.581}},
+    {"t128", 128, 64, 256, ProductForm::kTwo, {1.502, 2.597, 0.915, 2.333, 0.611}},
+    {"t192_n", 192, 64, 512, ProductForm::kOne, {1.186, 4.003, 0.623}},
+    {"t256_n", 256, 64, 512, ProductForm::kOne, {0, 6.050, 0.756}},
+    {"t160_w", 160, 128, 512, ProductForm::kOne, {0.029, 7.031, 0.923}},
+    {"t192", 192, 128, 512, ProductForm::kOne, {0, 6.068, 1.019}},
+    {"t256", 256, 128, 512, ProductForm::kOne, {0, 7.392, 1.237}},
 };
 // us, by size: 16 x 4096 x 4096 few1x1 6.2; 301 x 4096 x 4096 t64_d 15.6 (two slices in LDS 20.7);
 // 4096 x 4096 x 4096 t256 59.4, t128 64.

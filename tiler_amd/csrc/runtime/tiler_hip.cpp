@@ -388,8 +388,8 @@ const EntryRow kEntries[] = {
 #define TILER_GATED_FORM(FORM) {"tiler_gated_bf16_" FORM, "gated-contraction-bf16", 6}
     TILER_GATED_FORM("g64"), TILER_GATED_FORM("g128"), TILER_GATED_FORM("few1x1"), TILER_GATED_FORM("few2x1"),
     TILER_GATED_FORM("few4x1"), TILER_GATED_FORM("few4x2"), TILER_GATED_FORM("t64_d"), TILER_GATED_FORM("t96_d"),
-    TILER_GATED_FORM("t128_d"), TILER_GATED_FORM("t96"), TILER_GATED_FORM("t128"), TILER_GATED_FORM("t160"),
-    TILER_GATED_FORM("t192"), TILER_GATED_FORM("t256"),
+    TILER_GATED_FORM("t128_d"), TILER_GATED_FORM("t96"), TILER_GATED_FORM("t128"), TILER_GATED_FORM("t160_w"),
+    TILER_GATED_FORM("t192_n"), TILER_GATED_FORM("t256_n"), TILER_GATED_FORM("t192"), TILER_GATED_FORM("t256"),
 #undef TILER_GATED_FORM
 #define TILER_INT8_FORM(FORM)                                                \
   {"tiler_contract_i8_bf16_" FORM, "tensor-contraction-i8/bf16", 5},         \
