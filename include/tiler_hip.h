@@ -812,7 +812,7 @@ tiler_hip_status tiler_hip_layer_norm_backward_workspace(const tiler_hip_context
  *   G = x Wg^T, U = x Wu^T, h = silu(G) * U
  * x [m, k], wg and wu [n, k] (td,od->to), h [m, n].  h comes from the f32 sums,
  * rounded once.  gate and up (bf16 [m, n], both or neither) receive G and U
- * for the gradients.  k at least 1. */
+ * for the gradients.  k at least 1, below 2^24; m up to 65535 * 128. */
 tiler_hip_status tiler_hip_gated_contract_bf16(tiler_hip_context *ctx, const uint16_t *x,
                                                const uint16_t *wg, const uint16_t *wu, uint64_t m,
                                                uint64_t n, uint64_t k, uint16_t *h, uint16_t *gate,
@@ -821,7 +821,7 @@ tiler_hip_status tiler_hip_gated_contract_bf16(tiler_hip_context *ctx, const uin
  *   dU = dh G s, dG = dh U s (1 + G (1 - s))       rounded to bf16
  *   dx = dG Wg + dU Wu, dwg = dG^T x, dwu = dU^T x
  * dx may be NULL, dwg and dwu may both be NULL (not wanted).  With m = 0 the
- * weights' gradients are zeros, with n = 0 dx is. */
+ * weights' gradients are zeros, with n = 0 dx is.  n and k up to 2^22 - 64. */
 tiler_hip_status tiler_hip_gated_contract_bf16_backward(
     tiler_hip_context *ctx, const uint16_t *x, const uint16_t *wg, const uint16_t *wu,
     const uint16_t *gate, const uint16_t *up, const uint16_t *dh, uint64_t m, uint64_t n, uint64_t k,

@@ -185,8 +185,9 @@ def kept(dtype, x):
     return mu.astype(np.float32), r.astype(np.float32)
 
 
-def check_backward(ctx, mem, dtype, rows, extent, rng, shift=0, with_w=True, want=(True, True, True), workspace="given"):
-    x = rows_of(rng, rows, extent, dtype)
+def check_backward(ctx, mem, dtype, rows, extent, rng, shift=0, with_w=True, want=(True, True, True), workspace="given",
+                   offset=0.0):
+    x = ref.store(dtype, ref.wide(dtype, rows_of(rng, rows, extent, dtype)) + offset)
     dy = ref.store(dtype, rng.standard_normal((rows, extent)))
     w = ref.store(dtype, rng.normal(1, 0.2, extent)) if with_w else None
     mean, rstd = kept(dtype, x)
@@ -212,6 +213,13 @@ def test_backward(ctx, mem, dtype, extent):
 @pytest.mark.parametrize("rows,extent", [(2049, 128), (5003, 1000), (1100, 4096), (33, 16385)])
 def test_backward_many_rows(ctx, mem, dtype, rows, extent):
     check_backward(ctx, mem, dtype, rows, extent, np.random.default_rng(rows), workspace=None)
+
+
+@pytest.mark.parametrize("dtype,offset", [("f32", 3000.0), ("f32", -1e5), ("bf16", 40.0)])
+@pytest.mark.parametrize("extent", [100, 4096, 20001])
+def test_backward_far_from_zero(ctx, mem, dtype, offset, extent):
+    """Rows whose mean is many deviations from zero."""
+    check_backward(ctx, mem, dtype, 70, extent, np.random.default_rng(extent), offset=offset)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

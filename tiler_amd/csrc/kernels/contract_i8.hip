@@ -6,6 +6,11 @@
 // on v_mfma_i32_16x16x64_i8.  The integer sum is exact (k <= 131071 keeps
 // |sum| <= 2^31 - 2^14 for every pair of codes, -128 included); it is rounded
 // to binary32, multiplied by sa_i, then by sb_j, and narrowed to bf16 where C is bf16.
+//
+// us: rows of 4096 x 4096 bf16 quantized 11 (50 MB, 4.6 TB/s: read once), the
+// product 4096 x 4096 x 4096 58 (2.4 P operations/s, the matrix pipe; the forms of
+// few rows and small grids are bound by what LDS keeps in flight): 16 x 4096 x
+// 4096 5.3, 301 rows 15.6; 257 x 5001 x 1111 (rows off 16 bytes) 15.
 #include "product.h"
 #include "row_pieces.h"
 

@@ -16,6 +16,11 @@
 // of a sum, as independent as the terms), then dx contracts them with the
 // weights as they lie (the weights' rows are its depth) and dWg, dWu with x
 // over the tokens (both operands in column layout).
+//
+// us, 4096 x 14336 x 4096: forward 740 (1.3 PFLOP/s: the matrix pipe under the
+// card's power limit, as a plain library product of the size), dG and dU 98
+// (587 MB, 6 TB/s), dx 725, the weights' gradients 755.  16 tokens 45: the
+// weights' 235 MB.
 #include "product.h"
 
 namespace {

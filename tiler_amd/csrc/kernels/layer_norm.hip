@@ -4,6 +4,12 @@
 //   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) r w + b
 //   xh = (x - mu) r, g = dy w:
 //   dx = r (g - mean(g) - xh mean(g xh)), dw = sum over rows of dy xh, db = of dy
+//
+// Memory bounds all of it, so a row is read once and held in registers between
+// its sums and its results, and the gradients' workgroups keep dw's and db's sums
+// over their rows in registers.  us, and a copy of the same bytes: 8192 x 4096
+// bf16 with statistics 29 / 26, its gradients 46 and 4.6 for the partials' sum /
+// 39; 16 x 4096, a launch, 6; gradients of 1237 x 1023 f32 6.9 and 4.2 / 3.
 #include "row_pieces.h"
 
 namespace {
