@@ -100,3 +100,23 @@ def test_empty_requests_launch_nothing_or_zeros():
     assert len(region(L.PROGRAM_GATED_CONTRACTION_BACKWARD, (5, 0, 32), variant=L.GATED_DX | L.GATED_DW).symbols) == 1
     assert region(L.PROGRAM_QUANTIZE_ROWS_I8, (0, 64)).symbols == []
     assert region(L.PROGRAM_CONTRACTION_I8, (5, 0, 32)).symbols == []
+
+
+def test_host_functions_refuse_before_any_device_work():
+    """Shapes and dtypes are checked on the host: no context is ever asked for."""
+    import numpy as np
+    from tiler_amd import families as f
+    x, w, i8, s = np.zeros((3, 8), np.uint16), np.zeros((5, 8), np.uint16), np.zeros((3, 8), np.int8), np.ones(3, np.float32)
+    mid = np.zeros((3, 5), np.uint16)
+    for call in (lambda: f.layer_norm(np.zeros((3, 8)), ctx=0), lambda: f.layer_norm(x[0], ctx=0),
+                 lambda: f.layer_norm(x, weights=np.zeros(7, np.uint16), ctx=0),
+                 lambda: f.layer_norm(x, bias=np.zeros(8, np.float32), ctx=0),
+                 lambda: f.layer_norm_backward(x[:2], x, None, s, s, ctx=0),
+                 lambda: f.layer_norm_backward(x, x, None, s[:2], s, ctx=0),
+                 lambda: f.gated_contract_bf16(x, w, w[:4], ctx=0), lambda: f.gated_contract_bf16(x, w[:, :7], w, ctx=0),
+                 lambda: f.gated_contract_bf16(x.astype(np.float32), w, w, ctx=0),
+                 lambda: f.gated_contract_bf16_backward(x, w, w, mid, mid[:2], mid, ctx=0),
+                 lambda: f.quantize_rows_i8(i8, ctx=0), lambda: f.contract_i8(i8, i8[:, :7], s, s, ctx=0),
+                 lambda: f.contract_i8(i8, i8, s, s[:2], ctx=0), lambda: f.contract_i8(i8, i8, s, s, np.float64, ctx=0)):
+        with pytest.raises(Refusal):
+            call()

@@ -7,6 +7,7 @@ import pytest
 
 import feed_forward_reference as ref
 from tiler_amd import _lib as L
+from tiler_amd import families
 from tiler_amd.realize import propose, realize, route
 from tiler_amd.runtime import Refusal
 from test_gpu_layer_norm import Buffers, rows_of, within
@@ -203,6 +204,39 @@ def test_quantized_layer_behind_a_norm(ctx, mem):
             assert np.array_equal(mem.get(c, BF, (t, n)), got)
     finally:
         ctx.graph_destroy(graph)
+
+
+def test_host_functions(ctx):
+    rng = np.random.default_rng(8)
+    t, d, i = 33, 100, 72
+    for dtype in ("bf16", "f32"):
+        x, w, b = rows_of(rng, t, d, dtype), ref.store(dtype, rng.uniform(0.5, 1.5, d)), ref.store(dtype, rng.normal(0, 1, d))
+        y, mean, rstd = families.layer_norm(x, w, b, EPS, ctx=ctx)
+        args = [ref.wide(dtype, v) for v in (x, w, b)]
+        within(ref.wide(dtype, y), ref.layer_norm(*args)[0], ref.layer_norm_bounds(dtype, *args)[0], "y")
+        dy = ref.store(dtype, rng.standard_normal((t, d)))
+        args = (ref.wide(dtype, dy), args[0], args[1], mean.astype(np.float64), rstd.astype(np.float64))
+        for g, v, e in zip(families.layer_norm_backward(dy, x, w, mean, rstd, ctx=ctx), ref.layer_norm_backward(*args),
+                           ref.layer_norm_backward_bounds(dtype, *args)):
+            within(ref.wide(dtype, g), v, e, dtype)
+        q, s = families.quantize_rows_i8(x, ctx=ctx)
+        eq, es = ref.quantize_rows(ref.wide(dtype, x))
+        assert np.array_equal(q, eq) and np.array_equal(s, es)
+        for out in (np.float32, np.uint16):
+            want = ref.contract_i8(eq, eq, es, es)
+            got = families.contract_i8(q, q, s, s, out, ctx=ctx)
+            assert np.array_equal(got, want if out == np.float32 else bf(want))
+    x, wg, wu = bf(rng.standard_normal((t, d))), bf(rng.standard_normal((i, d)) / 10), bf(rng.standard_normal((i, d)) / 10)
+    args = [w64(v) for v in (x, wg, wu)]
+    h, gate, up = families.gated_contract_bf16(x, wg, wu, ctx=ctx)
+    for g, v, e in zip((h, gate, up), ref.gated(*args), ref.gated_bounds(*args)):
+        within(w64(g), v, e, "gated")
+    dh = bf(rng.standard_normal((t, i)))
+    args += [w64(v) for v in (gate, up, dh)]
+    for g, v, e in zip(families.gated_contract_bf16_backward(x, wg, wu, gate, up, dh, ctx=ctx), ref.gated_backward(*args),
+                       ref.gated_backward_bounds(*args)):
+        within(w64(g), v, e, "gradients")
+    assert families.layer_norm(np.zeros((0, 8), np.uint16), ctx=ctx)[0].shape == (0, 8)
 
 
 # -- the adapter --------------------------------------------------------------

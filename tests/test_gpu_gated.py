@@ -147,19 +147,21 @@ def test_backward_whole_numbers(ctx, mem, m, n, k):
         assert np.array_equal(g, bf(v)), np.argwhere(g != bf(v))[:4]
 
 
-# (dx's tile and whether its depth is split, the weights' gradients'), odd k: copied operands
-GRADIENT_FORMS = [(128, False, 128, False, 100, 72, 72), (128, True, 128, False, 300, 264, 265),
-                  (128, True, 256, False, 300, 1000, 4104), (128, False, 128, True, 520, 72, 72),
-                  (128, True, 128, True, 777, 264, 71), (256, True, 128, False, 1000, 2056, 4104),
-                  (256, True, 256, False, 2050, 2056, 2055), (256, False, 128, True, 2050, 72, 4104),
-                  (256, False, 256, False, 2050, 1000, 4104)]
+# dx's form and whether its depth is split, the weights' gradients'; odd k: copied operands
+GRADIENT_FORMS = [("t64_d", False, "t64_d", False, 520, 264, 265), ("t64_d", False, "t64_d", True, 1500, 264, 1000),
+                  ("t64_d", True, "t64_d", False, 520, 1000, 1000), ("t64_d", False, "t128", True, 2050, 264, 71),
+                  ("t128", True, "t64_d", False, 520, 264, 71),
+                  ("t128", True, "t128", False, 100, 1000, 265), ("t128", False, "t128", False, 520, 264, 4104),
+                  ("t128", True, "t128", True, 4100, 2056, 71), ("t256", True, "t128", False, 1000, 2056, 4104),
+                  ("t256", True, "t256", False, 2050, 2056, 2055), ("t256", False, "t128", True, 4100, 72, 2055),
+                  ("t256", False, "t256", True, 4100, 1000, 2055)]
 
 
-@pytest.mark.parametrize("tile_x,split_x,tile_w,split_w,m,n,k", GRADIENT_FORMS)
-def test_backward_forms(ctx, mem, tile_x, split_x, tile_w, split_w, m, n, k):
+@pytest.mark.parametrize("form_x,split_x,form_w,split_w,m,n,k", GRADIENT_FORMS)
+def test_backward_forms(ctx, mem, form_x, split_x, form_w, split_w, m, n, k):
     rz = realize(L.PROGRAM_GATED_CONTRACTION_BACKWARD, (m, n, k), dtype=L.BF16, variant=L.GATED_DX | L.GATED_DW,
                  permissions=L.PERMITS_REASSOCIATION, flags=L.REGION_ALIGNED16)
-    names = ["tiler_gated_bf16_grad", f"tiler_gated_bf16_dx_t{tile_x}", f"tiler_gated_bf16_dw_t{tile_w}"]
+    names = ["tiler_gated_bf16_grad", f"tiler_gated_bf16_dx_{form_x}", f"tiler_gated_bf16_dw_{form_w}"]
     assert rz.symbols == names + ["tiler_gated_bf16_sum"] * (split_x or split_w)
     assert [d.grid[1] > 1 for d in rz.dispatches[1:3]] == [split_x, split_w]
     test_backward_whole_numbers(ctx, mem, m, n, k)

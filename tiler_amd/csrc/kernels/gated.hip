@@ -44,6 +44,10 @@ constexpr int kW = 2, kNB = 4;  // 2 x 2 waves of MB x 4 blocks, MB 4 or 2
 // Rows of dG and dU, and of the copies of x and the weights in the backward pass.
 __device__ __forceinline__ uint32_t row_of_mid(uint32_t n) { return (n + 63u) & ~63u; }
 __device__ __forceinline__ uint32_t row_of_copy(uint32_t k) { return (k + 7u) & ~7u; }
+__device__ __forceinline__ uint64_t quotient(uint64_t v, uint32_t by) {  // a 64-bit division costs five of 32
+  return v >> 32 ? v / by : (uint32_t)v / by;
+}
+constexpr uint32_t kGradGroups = 8192;  // workgroups that form dG and dU, at most
 
 template <int MB>
 __device__ __forceinline__ void gated_guarded(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
@@ -128,26 +132,29 @@ tiler_gated_bf16_grad(const uint16_t* __restrict__ gate, const uint16_t* __restr
   using tiler_pieces::guarded_piece;
   using tiler_pieces::u32x4_any;
   const uint32_t ld = row_of_mid(n), per = ld / 8u, ldk = row_of_copy(k), per_k = ldk / 8u;
-  const uint64_t first = blockIdx.x * 256ull + threadIdx.x, step = gridDim.x * 256ull;
-  const uint64_t copies = ((to_x ? (uint64_t)m : 0u) + (to_w ? 2ull * n : 0u)) * per_k;
-  for (uint64_t id = first; id < copies; id += step) {
-    uint64_t row = id / per_k;
-    const uint32_t col = (uint32_t)(id % per_k) * 8u;
-    const uint16_t* from = x;
-    uint16_t* to = to_x;
-    if (!to_x || row >= m) {
-      if (to_x) row -= m;
-      from = row >= n ? wu : wg;
-      to = to_w + (row >= n ? (uint64_t)n * ldk : 0u);
-      if (row >= n) row -= n;
+  const uint64_t mids = (uint64_t)m * per, copies = ((to_x ? (uint64_t)m : 0u) + (to_w ? 2ull * n : 0u)) * per_k;
+  // The first workgroups form dG and dU, the others copy.
+  const uint32_t forming = (uint32_t)(mids < kGradGroups * 256ull ? (mids + 255u) / 256u : kGradGroups);
+  if (blockIdx.x >= forming) {
+    for (uint64_t id = (blockIdx.x - forming) * 256ull + threadIdx.x; id < copies; id += (gridDim.x - forming) * 256ull) {
+      uint64_t row = quotient(id, per_k);
+      const uint32_t col = (uint32_t)(id - row * per_k) * 8u;
+      const uint16_t* from = x;
+      uint16_t* to = to_x;
+      if (!to_x || row >= m) {
+        if (to_x) row -= m;
+        from = row >= n ? wu : wg;
+        to = to_w + (row >= n ? (uint64_t)n * ldk : 0u);
+        if (row >= n) row -= n;
+      }
+      const uint32_t valid = k - col < 8u ? (k - col) * 2u : 16u;
+      *reinterpret_cast<u32x4*>(to + row * ldk + col) = guarded_piece(
+          reinterpret_cast<const uint8_t*>(from + row * k + col), valid, reinterpret_cast<const uint8_t*>(from));
     }
-    const uint32_t valid = k - col < 8u ? (k - col) * 2u : 16u;
-    *reinterpret_cast<u32x4*>(to + row * ldk + col) = guarded_piece(
-        reinterpret_cast<const uint8_t*>(from + row * k + col), valid, reinterpret_cast<const uint8_t*>(from));
+    return;
   }
-  const uint64_t mids = (uint64_t)m * per;
-  for (uint64_t id = first; id < mids; id += step) {
-    const uint32_t row = (uint32_t)(id / per), col = (uint32_t)(id % per) * 8u;
+  for (uint64_t id = blockIdx.x * 256ull + threadIdx.x; id < mids; id += forming * 256ull) {
+    const uint32_t row = (uint32_t)quotient(id, per), col = (uint32_t)(id - (uint64_t)row * per) * 8u;
     const uint64_t at = (uint64_t)row * n + col;
     const uint32_t valid = col >= n ? 0u : n - col < 8u ? (n - col) * 2u : 16u;
     u32x4 vg = {0, 0, 0, 0}, vu = vg, vd = vg;
@@ -286,14 +293,14 @@ __device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, con
 // dx [m, k] = dG Wg + dU Wu: depth n twice (dG with Wg, then dU with Wu), the
 // weights in column layout, their rows ldk long (wu null: Wu is behind Wg).  With
 // splits > 1 each split's sums go to partials[split], binary32 [m, k].
-template <int WM, int WN, int MB>
+template <int WM, int WN, int MB, int S>
 __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ wg,
                                                 const uint16_t* __restrict__ wu, uint32_t ldk, uint32_t m, uint32_t n,
                                                 uint32_t k, uint16_t* __restrict__ dx, uint32_t splits,
                                                 float* __restrict__ partials) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kCols = WN * 64u, kThreads = 64u * WM * WN;
   constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kCols / 8 / (WM * WN);
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kCols) * kSlice];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * (kRowsA + kCols) * kSlice];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t tm, tn, t0, t1;
   tiler_product::tile_of(blockIdx.x, (m + kRowsA - 1u) / kRowsA, (k + kCols - 1u) / kCols, tm, tn);
@@ -307,7 +314,7 @@ __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg,
   const uint8_t* const a2 = reinterpret_cast<const uint8_t*>(dg + ((uint64_t)m + m0) * ld);
   const uint8_t* const b2 = reinterpret_cast<const uint8_t*>((wu ? wu : wg + (uint64_t)n * ldk) + c0);
   f32x4 acc[MB][4];
-  tiler_product::staged_product<Bf16, false, true, WM, WN, MB, 4, kLoadsA + kLoadsB, 2>(
+  tiler_product::staged_product<Bf16, false, true, WM, WN, MB, 4, kLoadsA + kLoadsB, S>(
       smem, t1 - t0,
       [&](uint32_t t, uint8_t* at) {
         const bool first = t + t0 < per;
@@ -331,14 +338,14 @@ __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg,
 // dWg [n, k] = dG^T x and dWu = dU^T x: depth m, both operands in column
 // layout, x's rows ldk long.  With splits > 1 each split's sums go to
 // partials[split], binary32 [2, n, k].
-template <int WM, int WN, int MB>
+template <int WM, int WN, int MB, int S>
 __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ x,
                                                 uint32_t ldk, uint32_t m, uint32_t n, uint32_t k,
                                                 uint16_t* __restrict__ dwg, uint16_t* __restrict__ dwu, uint32_t splits,
                                                 float* __restrict__ partials) {
   constexpr uint32_t kRowsA = WM * MB * 16u, kCols = WN * 64u, kThreads = 64u * WM * WN;
   constexpr int kLoadsA = kRowsA / 8 / (WM * WN), kLoadsB = kCols / 8 / (WM * WN);
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2u * (kRowsA + kCols) * kSlice];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * (kRowsA + kCols) * kSlice];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles = (n + kRowsA - 1u) / kRowsA;
   uint32_t tm, tn;
@@ -351,7 +358,7 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
   f32x4 acc[MB][4];
   uint32_t t0, t1;
   split_range((m + 63u) / 64u, splits, blockIdx.y, t0, t1);
-  tiler_product::staged_product<Bf16, true, true, WM, WN, MB, 4, kLoadsA + kLoadsB, 2>(
+  tiler_product::staged_product<Bf16, true, true, WM, WN, MB, 4, kLoadsA + kLoadsB, S>(
       smem, t1 - t0, [&](uint32_t t, uint8_t* at) { la.issue(t0 + t, at); },
       [&](uint32_t t, uint8_t* at) { lb.issue(t0 + t, at); }, acc);
   const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 64u;
@@ -382,20 +389,20 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
                                uint16_t* __restrict__ h, uint16_t* __restrict__ gate, uint16_t* __restrict__ up) {  \
     gated_staged<WM, WN, MB, S>(x, wg, wu, m, n, k, h, gate, up);                                                    \
   }
-#define TILER_GATED_DX_STAGED(TILE, WN, MB)                                                                         \
-  extern "C" __global__ void __launch_bounds__(128 * WN, 2)                                                         \
-      tiler_gated_bf16_dx_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ wg,                 \
+#define TILER_GATED_DX_STAGED(NAME, WN, MB, S)                                                                        \
+  extern "C" __global__ void __launch_bounds__(S > 2 ? 512 : 128 * WN, 2)                                                         \
+      tiler_gated_bf16_dx_t##NAME(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ wg,                 \
                                   const uint16_t* __restrict__ wu, uint32_t ldk, uint32_t m, uint32_t n,            \
                                   uint32_t k, uint16_t* __restrict__ dx, uint32_t splits,                           \
                                   float* __restrict__ partials) {                                                   \
-    gated_dx_staged<2, WN, MB>(dg, wg, wu, ldk, m, n, k, dx, splits, partials);                                     \
+    gated_dx_staged<2, WN, MB, S>(dg, wg, wu, ldk, m, n, k, dx, splits, partials);                                     \
   }
-#define TILER_GATED_DW_STAGED(TILE, WN, MB)                                                                         \
-  extern "C" __global__ void __launch_bounds__(128 * WN, 2)                                                         \
-      tiler_gated_bf16_dw_t##TILE(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ x, uint32_t ldk,    \
+#define TILER_GATED_DW_STAGED(NAME, WN, MB, S)                                                                        \
+  extern "C" __global__ void __launch_bounds__(S > 2 ? 512 : 128 * WN, 2)                                                         \
+      tiler_gated_bf16_dw_t##NAME(const uint16_t* __restrict__ dg, const uint16_t* __restrict__ x, uint32_t ldk,    \
                                   uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ dwg,                   \
                                   uint16_t* __restrict__ dwu, uint32_t splits, float* __restrict__ partials) {      \
-    gated_dw_staged<2, WN, MB>(dg, x, ldk, m, n, k, dwg, dwu, splits, partials);                                    \
+    gated_dw_staged<2, WN, MB, S>(dg, x, ldk, m, n, k, dwg, dwu, splits, partials);                                    \
   }
 TILER_GATED_TILES(96, 2, 2, 3, 2)
 TILER_GATED_TILES(128, 2, 2, 4, 2)
@@ -407,10 +414,12 @@ TILER_GATED_TILES(160_w, 2, 4, 5, 3)
 TILER_GATED_TILES(64_d, 2, 2, 2, 6)
 TILER_GATED_TILES(96_d, 2, 2, 3, 5)
 TILER_GATED_TILES(128_d, 2, 2, 4, 4)
-TILER_GATED_DX_STAGED(128, 2, 4)
-TILER_GATED_DX_STAGED(256, 4, 8)
-TILER_GATED_DW_STAGED(128, 2, 4)
-TILER_GATED_DW_STAGED(256, 4, 8)
+TILER_GATED_DX_STAGED(64_d, 2, 2, 6)
+TILER_GATED_DX_STAGED(128, 2, 4, 2)
+TILER_GATED_DX_STAGED(256, 4, 8, 2)
+TILER_GATED_DW_STAGED(64_d, 2, 2, 6)
+TILER_GATED_DW_STAGED(128, 2, 4, 2)
+TILER_GATED_DW_STAGED(256, 4, 8, 2)
 
 // ---------------------------------------------------------------------------
 // Few tokens: the weights' bytes.  A workgroup takes 16 MB tokens and 16 P

@@ -55,6 +55,10 @@ __device__ __forceinline__ uint32_t piece_offset(uint32_t row, uint32_t piece) {
   return row * kSlice + ((piece ^ ((row >> 1) & 7u)) << 4);
 }
 
+// f(d) changes the places of at most eight blocks, four in a tile of 64.
+template <uint32_t TILE>
+constexpr uint32_t kBlockMask = TILE / 16u < 8u ? TILE / 16u - 1u : 7u;
+
 // A lane's fragments of BLOCKS 16-row blocks starting at row `row0` of a tile.
 template <uint32_t TILE, bool kCol, int BLOCKS>
 struct Fragments {
@@ -62,7 +66,7 @@ struct Fragments {
   __device__ __forceinline__ Fragments(uint32_t row0, uint32_t lane) {
     const uint32_t i = lane & 15u, g = lane >> 4;
     if constexpr (kCol) {
-      const uint32_t f = (i >> 2) | ((g & 1u) << 2);
+      const uint32_t f = ((i >> 2) | ((g & 1u) << 2)) & kBlockMask<TILE>;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b)
         at[b] = (8u * g + (i >> 2)) * (TILE * 2u) + (((row0 / 16u + b) ^ f) << 5) + ((i & 3u) << 3);
@@ -304,11 +308,11 @@ struct ColumnLoader {
                                           uint32_t wave, uint32_t lane)
       : base(base_), row_bytes(ld * 2u), depth(depth_), before_bytes(before * 2u), lds0(wave * LOADS * 1024u) {
     constexpr uint32_t kPer = TILE / 8u;
-    static_assert(TILE >= 128 && (TILE & (TILE - 1u)) == 0, "eight blocks of a row change places");
+    static_assert(TILE >= 64 && (TILE & (TILE - 1u)) == 0, "blocks of a row change places");
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const uint32_t id = (wave * LOADS + j) * 64u + lane, outer = id / kPer, slot = id % kPer;
-      const uint32_t block = (slot >> 1) ^ ((outer & 3u) | ((outer >> 1) & 4u));
+      const uint32_t block = (slot >> 1) ^ (((outer & 3u) | ((outer >> 1) & 4u)) & kBlockMask<TILE>);
       voff[j] = outer * (uint32_t)row_bytes + block * 32u + (slot & 1u) * 16u;
     }
   }

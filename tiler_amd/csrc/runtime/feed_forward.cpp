@@ -240,6 +240,17 @@ uint64_t workgroups(const ProductForm& f, uint64_t m, uint64_t n) {
   return mul_sat(rows, f.kind == ProductForm::kFew && cols >= 8 ? ceil_div(cols, 8) * 8 : cols);
 }
 
+// q rounds of workgroups (`share` of the CUs, kFew's) with s slices each.
+double estimate(const ProductForm& f, double q, double s, double share) {
+  if (f.kind == ProductForm::kOne) return f.c[0] + q * (f.c[1] + f.c[2] * s);
+  if (f.kind == ProductForm::kTwo) {
+    const double pairs = std::floor(q / 2);
+    return f.c[0] + pairs * (f.c[1] + f.c[2] * s) + (q - 2 * pairs) * (f.c[3] + f.c[4] * s);
+  }
+  const double part = std::ceil(s / 8);
+  return f.c[0] + q * (f.c[1] + f.c[2] * part) + f.c[3] * part + f.c[4] * part * (share > 1 ? share : 1);
+}
+
 // The form of the least estimate, or null where no form's grid fits a launch.
 template <size_t N>
 const ProductForm* choose(const ProductForm (&forms)[N], const Target& t, uint64_t m, uint64_t n, uint64_t slices) {
@@ -248,17 +259,7 @@ const ProductForm* choose(const ProductForm (&forms)[N], const Target& t, uint64
   for (const ProductForm& f : forms) {
     const uint64_t w = workgroups(f, m, n);
     if (!grid_holds(w, f.threads)) continue;
-    const double q = (double)ceil_div(w, t.compute_units), s = (double)slices;
-    double us = f.c[0];
-    if (f.kind == ProductForm::kOne) {
-      us += q * (f.c[1] + f.c[2] * s);
-    } else if (f.kind == ProductForm::kTwo) {
-      const double pairs = std::floor(q / 2);
-      us += pairs * (f.c[1] + f.c[2] * s) + (q - 2 * pairs) * (f.c[3] + f.c[4] * s);
-    } else {
-      const double part = std::ceil(s / 8), share = (double)w / t.compute_units;
-      us += q * (f.c[1] + f.c[2] * part) + f.c[3] * part + f.c[4] * part * (share > 1 ? share : 1);
-    }
+    const double us = estimate(f, (double)ceil_div(w, t.compute_units), (double)slices, (double)w / t.compute_units);
     if (!best || us < least) best = &f, least = us;
   }
   return best;
@@ -271,34 +272,41 @@ uint32_t guarded_rows(const Target& t, uint64_t m, uint64_t column_tiles) {
   return m <= 64 || mul_sat(ceil_div(m, 64), column_tiles) <= t.compute_units ? 64 : 128;
 }
 
-// The gradients' products: tiles of 256 (one to a CU) or 128 (two to a CU), their
-// depth split over `splits` workgroups a tile where the tiles alone leave CUs
-// idle, the binary32 partials added by one more launch.  The least of the same
-// estimates, the partials' passes at 4.5 bytes a ns.
-struct GradientForm {
-  uint32_t tile, splits;
-  uint64_t tiles;
+// The gradients' products: a form's tile, the depth split over `splits` workgroups a
+// tile where the tiles alone leave CUs idle, the binary32 partials added by one
+// more launch.  The least of the same estimates, the partials' passes at 4.5 bytes a
+// ns.  us, dx of 2048 x 8192 x 2048: t256 in four 135, t128 in two 159, t256 whole
+// 316; the weights' gradients of 8192 x 512 x 512: t128 in eight 25, whole 78; of
+// 777 x 1365 x 509: t64_d 10.9, t128 13.1.
+constexpr ProductForm kGradientForms[] = {
+    {"t64_d", 64, 128, 256, ProductForm::kOne, {1.7, 2.4, 0.41}},
+    {"t128", 128, 128, 256, ProductForm::kTwo, {0, 3.9, 0.85, 3.0, 0.6}},
+    {"t256", 256, 256, 512, ProductForm::kOne, {0, 7.5, 1.2}},
 };
-GradientForm gradient_form(const Target& t, uint64_t halves, uint64_t rows, uint64_t cols, uint64_t slices) {
-  GradientForm best{0, 1, 0};
+struct GradientChoice {
+  const ProductForm* form = nullptr;
+  uint32_t splits = 1;
+  uint64_t tiles = 0;
+};
+GradientChoice choose_gradient(const Target& t, uint64_t halves, uint64_t rows, uint64_t cols, uint64_t slices) {
+  GradientChoice best;
   double least = 0;
-  for (const uint32_t tile : {256u, 128u}) {
-    const uint64_t tiles = mul_sat(halves * ceil_div(rows, tile), ceil_div(cols, tile));
+  for (const ProductForm& f : kGradientForms) {
+    const uint64_t tiles = mul_sat(halves * ceil_div(rows, f.rows), ceil_div(cols, f.cols));
     if (!grid_holds(tiles, 512)) continue;
     for (uint32_t splits = 1; splits <= 32 && (splits == 1 || splits * 2 <= slices); ++splits) {
-      const double q = std::ceil((double)tiles * splits / t.compute_units), s = (double)ceil_div(slices, splits);
-      const double pairs = std::floor(q / 2);
-      double us = tile == 256 ? q * (7.5 + 1.2 * s) : pairs * (3.9 + 0.85 * s) + (q - 2 * pairs) * (3.0 + 0.6 * s);
+      const double q = std::ceil((double)tiles * splits / t.compute_units);
+      double us = estimate(f, q, (double)ceil_div(slices, splits), 0);
       if (splits > 1) us += 3 + (double)splits * halves * rows * cols * 8 / 4.5e6;
-      if (!best.tile || us < least) best = {tile, splits, tiles}, least = us;
+      if (!best.form || us < least) best = {&f, splits, tiles}, least = us;
     }
   }
   return best;
 }
 
-Launch& add_gradient(Program& p, const char* stem, const GradientForm& f) {
-  const std::string name = std::string(stem) + "_t" + std::to_string(f.tile);
-  return p.add(name.c_str(), (uint32_t)f.tiles, f.splits, f.tile == 256 ? 512 : 256);
+Launch& add_gradient(Program& p, const char* stem, const GradientChoice& c) {
+  const std::string name = std::string(stem) + "_" + c.form->name;
+  return p.add(name.c_str(), (uint32_t)c.tiles, c.splits, c.form->threads);
 }
 
 }  // namespace
@@ -353,15 +361,16 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
   const uint32_t to_x = copy_x ? p.slot(mul_sat(mul_sat(m, ldk), 2), kSlotScratch) : 0;
   const uint32_t to_w = copy_w ? p.slot(mul_sat(mul_sat(n, ldk), 4), kSlotScratch) : 0;
   if (m && n) {
-    const uint64_t mids = m * (ld / 8), copies = ((copy_x ? m : 0) + (copy_w ? 2 * n : 0)) * (ldk / 8);
-    const uint64_t groups = ceil_div(mids > copies ? mids : copies, 256);
-    Launch& l = p.add("tiler_gated_bf16_grad", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
+    // workgroups that form dG and dU, then those that copy: at most 8192 of each
+    auto groups = [](uint64_t pieces) { return pieces < 8192 * 256ull ? ceil_div(pieces, 256) : 8192; };
+    const uint64_t copies = ((copy_x ? m : 0) + (copy_w ? 2 * n : 0)) * (ldk / 8);
+    Launch& l = p.add("tiler_gated_bf16_grad", (uint32_t)(groups(m * (ld / 8)) + groups(copies)), 1, 256)
                     .ptr(gate).ptr(up).ptr(dh).ptr(x).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dg);
     slot_or_null(l, copy_x, to_x);
     slot_or_null(l, copy_w, to_w);
   }
-  const GradientForm fx = gradient_form(t, 1, m, k, n ? 2 * (ld / 64) : 0), fw = gradient_form(t, 2, n, k, ceil_div(m, 64));
-  if ((has_dx && m && !fx.tile) || (has_dw && n && !fw.tile))
+  const GradientChoice fx = choose_gradient(t, 1, m, k, n ? 2 * (ld / 64) : 0), fw = choose_gradient(t, 2, n, k, ceil_div(m, 64));
+  if ((has_dx && m && !fx.form) || (has_dw && n && !fw.form))
     return p.refuse(TILER_HIP_REFUSE_CAPACITY, "contraction extents beyond the launch profile");
   const bool sum_x = has_dx && m && fx.splits > 1, sum_w = has_dw && n && fw.splits > 1;
   const uint32_t of_x = sum_x ? p.slot(mul_sat(mul_sat(fx.splits, m * k), 4), kSlotScratch) : 0;

@@ -380,9 +380,11 @@ const EntryRow kEntries[] = {
     TILER_GRAD_FORM("w1c1"), TILER_GRAD_FORM("w2c1"), TILER_GRAD_FORM("w4c1"), TILER_GRAD_FORM("w8c1"),
     TILER_GRAD_FORM("w16c1"), TILER_GRAD_FORM("w16c2"),
 #undef TILER_GRAD_FORM
+    {"tiler_gated_bf16_dx_t64_d", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dx_t128", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dx_t256", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_sum", "gated-contraction-bf16-backward", 5},
+    {"tiler_gated_bf16_dw_t64_d", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dw_t128", "gated-contraction-bf16-backward", 5},
     {"tiler_gated_bf16_dw_t256", "gated-contraction-bf16-backward", 5},
 #define TILER_GATED_FORM(FORM) {"tiler_gated_bf16_" FORM, "gated-contraction-bf16", 6}

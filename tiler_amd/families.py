@@ -257,8 +257,112 @@ def dequantize_u4(packed: np.ndarray, n: int, scale_bits: int, zero_point: int, 
         dy.free()
 
 
+# --- the feed-forward sublayer (no reference counterpart) ----------------------
+# Storage by numpy dtype: float32, or uint16 holding bf16 patterns.
+
+def _storage(values, what: str):
+    a = np.ascontiguousarray(values)
+    if a.ndim != 2 or a.dtype not in (np.float32, np.uint16):
+        raise Refusal(L.REFUSE_UNSUPPORTED, what, "rows in two dimensions, float32 or uint16 (bf16 patterns)")
+    return a, L.F32 if a.dtype == np.float32 else L.BF16
+
+
+def _operand(values, dtype, shape, what: str):
+    a = np.ascontiguousarray(values)
+    if a.dtype != dtype or a.shape != tuple(shape):
+        raise Refusal(L.REFUSE_INVALID_ARGUMENT, what, f"an operand is {a.dtype}{list(a.shape)}, not {np.dtype(dtype)}{list(shape)}")
+    return a
+
+
+def _run(ctx, inputs, outputs, launch):
+    """launch(context, device inputs, device outputs); the outputs, (dtype, shape) each, on the host."""
+    ctx = _ctx(ctx)
+    bufs = []
+    try:
+        for a in inputs:
+            bufs.append(None if a is None else ctx.to_device(a))
+        for dtype, shape in outputs:
+            bufs.append(ctx.alloc(max(int(np.prod(shape, dtype=np.int64)) * np.dtype(dtype).itemsize, 1)))
+        out = bufs[len(inputs):]
+        launch(ctx, bufs[:len(inputs)], out)
+        ctx.synchronize()
+        return [b.download(dtype, shape) for b, (dtype, shape) in zip(out, outputs)]
+    finally:
+        for b in bufs:
+            if b is not None:
+                b.free()
+
+
+def layer_norm(values, weights=None, bias=None, eps_bits: int = 0x3727C5AC, ctx=None):
+    """(y, mean, rstd) of the rows of `values` [rows, extent]; weights and bias
+    [extent] or None (ones, zeros)."""
+    x, code = _storage(values, "layer_norm")
+    rows, extent = x.shape
+    wb = [None if v is None else _operand(v, x.dtype, (extent,), "layer_norm") for v in (weights, bias)]
+    return tuple(_run(ctx, [x, *wb], [(x.dtype, x.shape), (np.float32, (rows,)), (np.float32, (rows,))],
+                      lambda c, i, o: c.layer_norm(code, *i, rows, extent, eps_bits, *o)))
+
+
+def layer_norm_backward(dy, values, weights, mean, rstd, ctx=None):
+    """(dx, dw, db) from dy and what layer_norm returned."""
+    x, code = _storage(values, "layer_norm_backward")
+    rows, extent = x.shape
+    dy = _operand(dy, x.dtype, x.shape, "layer_norm_backward")
+    w = None if weights is None else _operand(weights, x.dtype, (extent,), "layer_norm_backward")
+    stats = [_operand(v, np.float32, (rows,), "layer_norm_backward") for v in (mean, rstd)]
+    return tuple(_run(ctx, [dy, x, w, *stats], [(x.dtype, x.shape), (x.dtype, (extent,)), (x.dtype, (extent,))],
+                      lambda c, i, o: c.layer_norm_backward(code, *i, rows, extent, *o)))
+
+
+def _gated_operands(x, wg, wu, what: str):
+    x = np.ascontiguousarray(x)
+    wg = np.ascontiguousarray(wg)
+    if x.ndim != 2 or wg.ndim != 2 or x.dtype != np.uint16:
+        raise Refusal(L.REFUSE_UNSUPPORTED, what, "rows in two dimensions, uint16 (bf16 patterns)")
+    (m, k), n = x.shape, wg.shape[0]
+    return m, n, k, [x, _operand(wg, np.uint16, (n, k), what), _operand(wu, np.uint16, (n, k), what)]
+
+
+def gated_contract_bf16(x, wg, wu, ctx=None):
+    """(h, gate, up): h = silu(x wg^T) * (x wu^T) of bf16 patterns, x [m, k],
+    wg and wu [n, k]; gate and up are the two products."""
+    m, n, k, operands = _gated_operands(x, wg, wu, "gated_contract_bf16")
+    return tuple(_run(ctx, operands, [(np.uint16, (m, n))] * 3, lambda c, i, o: c.gated_contract_bf16(*i, m, n, k, *o)))
+
+
+def gated_contract_bf16_backward(x, wg, wu, gate, up, dh, ctx=None):
+    """(dx, dwg, dwu) from dh and what gated_contract_bf16 returned."""
+    what = "gated_contract_bf16_backward"
+    m, n, k, operands = _gated_operands(x, wg, wu, what)
+    operands += [_operand(v, np.uint16, (m, n), what) for v in (gate, up, dh)]
+    return tuple(_run(ctx, operands, [(np.uint16, (m, k)), (np.uint16, (n, k)), (np.uint16, (n, k))],
+                      lambda c, i, o: c.gated_contract_bf16_backward(*i, m, n, k, *o)))
+
+
+def quantize_rows_i8(values, ctx=None):
+    """(codes int8, scales float32) of the rows of `values` [rows, extent]."""
+    x, code = _storage(values, "quantize_rows_i8")
+    rows, extent = x.shape
+    return tuple(_run(ctx, [x], [(np.int8, x.shape), (np.float32, (rows,))],
+                      lambda c, i, o: c.quantize_rows_i8(code, *i, rows, extent, *o)))
+
+
+def contract_i8(a, b, a_scales, b_scales, out_dtype=np.float32, ctx=None):
+    """int8 a [m, k], b [n, k] with a scale a row each -> [m, n], float32 or
+    uint16 (bf16 patterns)."""
+    a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
+    if a.ndim != 2 or b.ndim != 2 or out_dtype not in (np.float32, np.uint16):
+        raise Refusal(L.REFUSE_UNSUPPORTED, "contract_i8", "operands in two dimensions, a float32 or uint16 result")
+    (m, k), n = a.shape, b.shape[0]
+    operands = [_operand(a, np.int8, (m, k), "contract_i8"), _operand(b, np.int8, (n, k), "contract_i8"),
+                _operand(a_scales, np.float32, (m,), "contract_i8"), _operand(b_scales, np.float32, (n,), "contract_i8")]
+    code = L.F32 if out_dtype == np.float32 else L.BF16
+    return _run(ctx, operands, [(out_dtype, (m, n))], lambda c, i, o: c.contract_i8(*i, m, n, k, code, *o))[0]
+
+
 __all__ = [
     "strict_sum", "strict_partitioned_sum", "cooperative_grouped_sum", "tree_sum",
     "rms_norm_f32", "rms_norm_bf16", "softmax_f32", "silu_f32", "gather",
-    "contract_strict_f32", "contract_bf16", "dequantize_u4", "default_context", "GatherIndexOutOfBounds",
+    "contract_strict_f32", "contract_bf16", "dequantize_u4", "layer_norm", "layer_norm_backward", "gated_contract_bf16",
+    "gated_contract_bf16_backward", "quantize_rows_i8", "contract_i8", "default_context", "GatherIndexOutOfBounds",
 ]
