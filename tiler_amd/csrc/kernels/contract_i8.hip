@@ -287,7 +287,7 @@ __device__ __forceinline__ void contract_i8_staged(const int8_t* __restrict__ a,
   }
   if constexpr (kBf16) {
     __syncthreads();
-    tiler_product::store_tile_bf16<kRowsA, kRowsB, kThreads, MB, 4>(
+    tiler_product::store_tile_bf16<kRowsA, kRowsB, kThreads, MB, 4, false>(
         smem, row0, col0, static_cast<uint16_t*>(c), m, n, m0, n0,
         [&](int i, int j, int r) { return (float)acc[i][j][r] * rows[i][r] * cols[j]; });
   } else {

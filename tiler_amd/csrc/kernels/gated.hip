@@ -17,10 +17,10 @@
 // weights as they lie (the weights' rows are its depth) and dWg, dWu with x
 // over the tokens (both operands in column layout).
 //
-// us, 4096 x 14336 x 4096: forward 740 (1.3 PFLOP/s: the matrix pipe under the
-// card's power limit, as a plain library product of the size), dG and dU 98
-// (587 MB, 6 TB/s), dx 725, the weights' gradients 755.  16 tokens 45: the
-// weights' 235 MB.
+// us, 4096 x 14336 x 4096: forward with G and U kept 735 (1.3 PFLOP/s: the matrix
+// pipe under the card's power limit, as a plain library product of the size), dG
+// and dU 98 (587 MB, 6 TB/s), dx 710, the weights' gradients 710.  16 tokens 45:
+// the weights' 235 MB.
 #include "product.h"
 
 namespace {
@@ -279,14 +279,18 @@ __device__ __forceinline__ void gated_staged(const uint16_t* __restrict__ x, con
       smem, (k + 63u) / 64u, [&](uint32_t t, uint8_t* at) { la.issue(t, at); },
       [&](uint32_t t, uint8_t* at) { lb.issue(t, at); }, acc);
   const uint32_t row0 = (wave / WN) * MB * 16u, col0 = (wave % WN) * 32u;
-  auto store = [&](uint16_t* out, auto value) {
+  // h for the next product, from the caches; G and U, as the weights' gradients, past
+  // them: too large to be kept until they are read (4096 x 14336 x 4096: 746 -> 735
+  // us, the weights' gradients 735 -> 710)
+  auto store = [&](auto stream, uint16_t* out, auto value) {
     __syncthreads();
-    tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 2>(smem, row0, col0, out, m, n, m0, n0, value);
+    tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 2, decltype(stream)::value != 0>(smem, row0, col0, out, m, n,
+                                                                                            m0, n0, value);
   };
-  store(h, [&](int i, int j, int r) { return acc[i][j][r] * sigmoid(acc[i][j][r]) * acc[i][j + 2][r]; });
+  store(tiler::Step<0>{}, h, [&](int i, int j, int r) { return acc[i][j][r] * sigmoid(acc[i][j][r]) * acc[i][j + 2][r]; });
   if (gate) {
-    store(gate, [&](int i, int j, int r) { return acc[i][j][r]; });
-    store(up, [&](int i, int j, int r) { return acc[i][j + 2][r]; });
+    store(tiler::Step<1>{}, gate, [&](int i, int j, int r) { return acc[i][j][r]; });
+    store(tiler::Step<1>{}, up, [&](int i, int j, int r) { return acc[i][j + 2][r]; });
   }
 }
 
@@ -331,7 +335,7 @@ __device__ __forceinline__ void gated_dx_staged(const uint16_t* __restrict__ dg,
     return;
   }
   __syncthreads();
-  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(smem, row0, col0, dx, m, k, m0, c0,
+  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4, false>(smem, row0, col0, dx, m, k, m0, c0,
                                                                  [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 
@@ -367,7 +371,7 @@ __device__ __forceinline__ void gated_dw_staged(const uint16_t* __restrict__ dg,
     return;
   }
   __syncthreads();
-  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4>(smem, row0, col0, second ? dwu : dwg, n, k, j0, c0,
+  tiler_product::store_tile_bf16<kRowsA, kCols, kThreads, MB, 4, true>(smem, row0, col0, second ? dwu : dwg, n, k, j0, c0,
                                                                  [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 

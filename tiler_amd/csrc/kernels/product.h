@@ -338,7 +338,7 @@ constexpr int kWaitLds = 0xC07F;  // lgkmcnt(0) alone
 // wave's reads of the slice are done (its buffer takes slice t + S) and every
 // wave's share of the next slice has landed.  The reads are
 // dealt out among the products (4096 x 14336 x 4096, dx 745 -> 715 us, the
-// weights' gradients 800 -> 750, against all reads first).
+// weights' gradients 800 -> 750, against all reads of a step first).
 template <typename E, bool kACol, bool kBCol, int WM, int WN, int MB, int NB, int kLoads, int S, typename IA, typename IB>
 __device__ __forceinline__ void staged_product(uint8_t* smem, uint32_t slices, IA issue_a, IB issue_b,
                                                typename E::Acc (&acc)[MB][NB]) {
@@ -512,9 +512,10 @@ __device__ __forceinline__ uint32_t column_pair(float v0, float v1, bool odd) {
 // Stores a tile of bf16 results through LDS: value(i, j, r) is this lane's
 // result of row 16 i + 4 (lane / 16) + r, column 16 j + lane % 16 of its wave's
 // (row0, col0) part of the ROWS x COLS tile; the tile is at (m0, n0) of the
-// m x n result.  16-byte stores of whole row pieces, at any alignment.  The
-// caller's waves are done with the LDS.
-template <uint32_t ROWS, uint32_t COLS, uint32_t THREADS, int MB, int NB, typename F>
+// m x n result.  16-byte stores of whole row pieces, at any alignment; kStream:
+// past the caches, for results that wait for another pass.  The caller's waves are
+// done with the LDS.
+template <uint32_t ROWS, uint32_t COLS, uint32_t THREADS, int MB, int NB, bool kStream, typename F>
 __device__ __forceinline__ void store_tile_bf16(uint8_t* smem, uint32_t row0, uint32_t col0, uint16_t* out, uint32_t m,
                                                 uint32_t n, uint32_t m0, uint32_t n0, F value) {
   constexpr uint32_t kRow = COLS * 2u, kPer = COLS / 8u;
@@ -539,7 +540,8 @@ __device__ __forceinline__ void store_tile_bf16(uint8_t* smem, uint32_t row0, ui
     const u32x4 v = *reinterpret_cast<const u32x4*>(smem + row * kRow + ((piece ^ (((row & 7u) << 1) & (kPer - 1u))) << 4));
     uint16_t* to = out + (uint64_t)(m0 + row) * n + col;
     if (n - col >= 8u) {
-      *reinterpret_cast<u32x4_any*>(to) = v;
+      if constexpr (kStream) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(to));
+      else *reinterpret_cast<u32x4_any*>(to) = v;
     } else {
 #pragma unroll
       for (uint32_t e = 0; e < 7u; ++e)
