@@ -149,11 +149,11 @@ def test_backward_whole_numbers(ctx, mem, m, n, k):
 
 # dx's form and whether its depth is split, the weights' gradients'; odd k: copied operands
 GRADIENT_FORMS = [("t64_d", False, "t64_d", False, 520, 264, 265), ("t64_d", False, "t64_d", True, 1500, 264, 1000),
-                  ("t64_d", True, "t64_d", False, 520, 1000, 1000), ("t64_d", False, "t128", True, 2050, 264, 71),
-                  ("t128", True, "t64_d", False, 520, 264, 71),
-                  ("t128", True, "t128", False, 100, 1000, 265), ("t128", False, "t128", False, 520, 264, 4104),
+                  ("t64_d", True, "t64_d", False, 520, 1000, 1000), ("t64_d", False, "t128", True, 4100, 1000, 265),
+                  ("t128", True, "t64_d", False, 2050, 2056, 265),
+                  ("t128", True, "t128", False, 520, 1000, 1800), ("t128", False, "t128", False, 520, 264, 4104),
                   ("t128", True, "t128", True, 4100, 2056, 71), ("t256", True, "t128", False, 1000, 2056, 4104),
-                  ("t256", True, "t256", False, 2050, 2056, 2055), ("t256", False, "t128", True, 4100, 72, 2055),
+                  ("t256", True, "t256", False, 2050, 2056, 2055), ("t256", False, "t128", True, 4100, 264, 2055),
                   ("t256", False, "t256", True, 4100, 1000, 2055)]
 
 

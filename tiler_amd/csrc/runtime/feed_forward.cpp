@@ -274,14 +274,17 @@ uint32_t guarded_rows(const Target& t, uint64_t m, uint64_t column_tiles) {
 
 // The gradients' products: a form's tile, the depth split over `splits` workgroups a
 // tile where the tiles alone leave CUs idle, the binary32 partials added by one
-// more launch.  The least of the same estimates, the partials' passes at 4.5 bytes a
-// ns.  us, dx of 2048 x 8192 x 2048: t256 in four 135, t128 in two 159, t256 whole
-// 316; the weights' gradients of 8192 x 512 x 512: t128 in eight 25, whole 78; of
-// 777 x 1365 x 509: t64_d 10.9, t128 13.1.
+// more launch.  The least of the same estimates, with the results' stores (a
+// million elements: 0.39 us) or the partials' (1.31 a part, 1.55 and 0.29 a part
+// besides): fits of 1031 times of sizes spread over m 1 .. 4096, n to 10424, k to
+// 4096, 1.6% slower than the fastest form in the mean.  us, dx of 2048 x 8192 x
+// 2048: t256 in four 135, t128 in two 159, t256 whole 316; of 7 x 2048 x 872 t64_d
+// in eight 11.3, t128 in 32 16.3; the weights' gradients of 8192 x 512 x 512: t64_d
+// in four 24, t128 whole 78; of 777 x 1365 x 509: t64_d 10.9, t128 13.1.
 constexpr ProductForm kGradientForms[] = {
-    {"t64_d", 64, 128, 256, ProductForm::kOne, {1.7, 2.4, 0.41}},
-    {"t128", 128, 128, 256, ProductForm::kTwo, {0, 3.9, 0.85, 3.0, 0.6}},
-    {"t256", 256, 256, 512, ProductForm::kOne, {0, 7.5, 1.2}},
+    {"t64_d", 64, 128, 256, ProductForm::kOne, {2.974, 1.401, 0.395}},
+    {"t128", 128, 128, 256, ProductForm::kTwo, {4.210, 0, 0.900, 0.225, 0.588}},
+    {"t256", 256, 256, 512, ProductForm::kOne, {6.412, 0.164, 1.179}},
 };
 struct GradientChoice {
   const ProductForm* form = nullptr;
@@ -291,13 +294,14 @@ struct GradientChoice {
 GradientChoice choose_gradient(const Target& t, uint64_t halves, uint64_t rows, uint64_t cols, uint64_t slices) {
   GradientChoice best;
   double least = 0;
+  const double results = (double)halves * (double)rows * (double)cols * 1e-6;
   for (const ProductForm& f : kGradientForms) {
     const uint64_t tiles = mul_sat(halves * ceil_div(rows, f.rows), ceil_div(cols, f.cols));
     if (!grid_holds(tiles, 512)) continue;
     for (uint32_t splits = 1; splits <= 32 && (splits == 1 || splits * 2 <= slices); ++splits) {
       const double q = std::ceil((double)tiles * splits / t.compute_units);
       double us = estimate(f, q, (double)ceil_div(slices, splits), 0);
-      if (splits > 1) us += 3 + (double)splits * halves * rows * cols * 8 / 4.5e6;
+      us += splits > 1 ? 1.546 + splits * (0.294 + 1.309 * results) : 0.386 * results;
       if (!best.form || us < least) best = {&f, splits, tiles}, least = us;
     }
   }
