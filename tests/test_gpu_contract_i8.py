@@ -9,7 +9,7 @@ import feed_forward_reference as ref
 import oracle
 from tiler_amd import _lib as L
 from tiler_amd.realize import realize
-from test_gpu_layer_norm import CODE, Buffers, storage
+from test_gpu_layer_norm import CODE, ROW_FORMS, Buffers, storage
 
 pytestmark = pytest.mark.gpu
 
@@ -44,6 +44,17 @@ def test_quantize(ctx, mem, dtype, extent):
         x = rng.standard_normal((rows, extent)) * np.exp(rng.normal(0, 3, (rows, 1)))
         for shift in (0, 1):
             check_quantize(ctx, mem, dtype, ref.store(dtype, x), shift)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("form,rows,extent", ROW_FORMS)
+def test_quantize_forms(ctx, mem, dtype, form, rows, extent):
+    extent = extent if dtype == "bf16" else extent // 2
+    if dtype == "bf16" and form == "w1c4":
+        form = "w4c1"  # more than two pieces a thread
+    rz = realize(L.PROGRAM_QUANTIZE_ROWS_I8, (rows, extent), dtype=CODE[dtype], permissions=L.PERMITS_REASSOCIATION)
+    assert rz.symbols == [f"tiler_quantize_rows_i8_{dtype}_{form}"]
+    check_quantize(ctx, mem, dtype, ref.store(dtype, np.random.default_rng(extent).standard_normal((rows, extent))))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

@@ -6,6 +6,7 @@ import pytest
 
 import feed_forward_reference as ref
 from tiler_amd import _lib as L
+from tiler_amd.realize import realize
 from tiler_amd.runtime import Refusal
 
 pytestmark = pytest.mark.gpu
@@ -106,6 +107,27 @@ def test_forward(ctx, mem, dtype, extent):
         within(mean, wmean, emean, "mean")
         within(rstd, wrstd, erstd, "rstd")
         within(ref.wide(dtype, y), wy, ey, "y")
+
+
+# Every form of the rows (extents of bf16; of f32 half as long): a ragged last piece, ragged last workgroups
+ROW_FORMS = [("s", 5, 7), ("w1c1", 1030, 510), ("w1c2", 1030, 1022), ("w1c4", 2051, 2046), ("w4c1", 40, 2046),
+             ("w4c2", 40, 4094), ("w4c4", 300, 8190), ("w16c1", 40, 8190), ("w16c2", 9, 16382), ("w16c4", 9, 32766),
+             ("s", 9, 32770)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("form,rows,extent", ROW_FORMS)
+def test_forward_forms(ctx, mem, dtype, form, rows, extent):
+    extent = extent if dtype == "bf16" else extent // 2
+    rz = realize(L.PROGRAM_LAYER_NORM, (rows, extent), dtype=CODE[dtype], scalars=(ref.EPS_BITS, 0),
+                 permissions=L.PERMITS_REASSOCIATION)
+    assert rz.symbols == [f"tiler_layer_norm_{dtype}_{form}"]
+    rng = np.random.default_rng(extent)
+    x = rows_of(rng, rows, extent, dtype)
+    w, b = ref.store(dtype, rng.normal(1, 0.2, extent)), ref.store(dtype, rng.normal(0, 0.2, extent))
+    args = (ref.wide(dtype, x), ref.wide(dtype, w), ref.wide(dtype, b))
+    for got, want, bound in zip(forward(ctx, mem, dtype, x, w, b), ref.layer_norm(*args), ref.layer_norm_bounds(dtype, *args)):
+        within(ref.wide(dtype, got) if got.ndim == 2 else got, want, bound, (form, dtype))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

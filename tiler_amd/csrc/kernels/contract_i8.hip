@@ -8,7 +8,7 @@
 // to binary32, multiplied by sa_i, then by sb_j, and narrowed to bf16 where C is bf16.
 //
 // us: rows of 4096 x 4096 bf16 quantized 11 (50 MB, 4.6 TB/s: read once), the
-// product 4096 x 4096 x 4096 58 (2.4 P operations/s, the matrix pipe; the forms of
+// product 4096 x 4096 x 4096 59 (2.3 P operations/s, the matrix pipe; the forms of
 // few rows and small grids are bound by what LDS keeps in flight): 16 x 4096 x
 // 4096 5.3, 301 rows 15.6; 257 x 5001 x 1111 (rows off 16 bytes) 15.
 #include "product.h"
@@ -179,7 +179,6 @@ __device__ __forceinline__ void quantize_stream(const T* __restrict__ x, uint64_
   }                                                                                                        \
   TILER_QUANTIZE_ROWS(TY, T, 1, 1)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 1, 2)                                                                         \
-  TILER_QUANTIZE_ROWS(TY, T, 1, 4)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 4, 1)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 4, 2)                                                                         \
   TILER_QUANTIZE_ROWS(TY, T, 4, 4)                                                                         \
@@ -188,6 +187,7 @@ __device__ __forceinline__ void quantize_stream(const T* __restrict__ x, uint64_
   TILER_QUANTIZE_ROWS(TY, T, 16, 4)
 TILER_QUANTIZE_FORMS(bf16, uint16_t)
 TILER_QUANTIZE_FORMS(f32, float)
+TILER_QUANTIZE_ROWS(f32, float, 1, 4)
 
 namespace {
 

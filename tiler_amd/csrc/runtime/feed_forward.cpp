@@ -28,13 +28,14 @@ constexpr uint32_t kRowWorkgroups = 1u << 20;  // rows beyond take further round
 
 // The register form of a row kernel (row_pieces.h) for rows of `extent`
 // elements, kVec = `vec` to a 16-byte piece: WAVES waves per row and CH pieces
-// a thread, "w{WAVES}c{CH}", or "s" (streamed) beyond what registers hold.
-// One wave a row (four rows a workgroup, no barrier) where that gives every
-// SIMD a wave and a thread at most `one_wave` pieces; fewer rows than that, or
-// longer ones, take four waves a row, then sixteen.  Rows shorter than a piece
-// are streamed.  us, one wave and four: norm of 8192 x 4096 bf16 31.8 / 65, of
-// 4096 x 4096 f32 (16 pieces) 31.6 / 27.6, of 2048 x 8192 bf16 (16) 20.4 / 17.9;
-// quantization of 4096 x 4096 bf16 (8) 17.7 / 13.4, of 8192 x 2048 (4) 15.2 / 14.3.
+// a thread, "w{WAVES}c{CH}", or "s" (streamed) beyond what registers hold and for
+// rows shorter than a piece.  One wave a row (four rows a workgroup, no barrier)
+// where a thread has at most `one_wave` pieces and the rows fill the CUs twice over
+// for each; else four waves a row, and sixteen beyond 1024 pieces or for up to a
+// row a CU.  us, norm bf16, one wave / four / sixteen: 4096 x 2048 (4 pieces) 8.7 /
+// 10.9 / 27, 1024 x 2048 6.5 / 5.4 / 9.3, 8192 x 4096 (8) 31 / 28 / 56; four /
+// sixteen: 128 x 8192 6.1 / 4.9, 1024 x 8192 9.6 / 11.4; quantization of bf16 rows,
+// 4096 x 2048 (4) 9.5 / 8.4.
 struct RowForm {
   char name[16];
   uint32_t block;
@@ -49,9 +50,10 @@ RowForm row_form(const Target& t, uint64_t rows, uint64_t extent, uint64_t vec, 
     while (p < v) p <<= 1;
     return p;
   };
+  const uint32_t alone = pow2(ceil_div(pieces, 64));  // pieces a thread of a row's only wave
   if (extent < vec) waves = 0;
-  else if (pieces <= 64 || (pieces <= 64 * one_wave && rows >= 4ull * t.compute_units)) waves = 1, ch = pow2(ceil_div(pieces, 64));
-  else if (pieces <= 256 * 4) waves = 4, ch = pow2(ceil_div(pieces, 256));
+  else if (alone == 1 || (alone <= one_wave && rows >= 2ull * alone * t.compute_units)) waves = 1, ch = alone;
+  else if (pieces <= 512 || (pieces <= 1024 && rows > t.compute_units)) waves = 4, ch = pow2(ceil_div(pieces, 256));
   else if (pieces <= 1024 * 4) waves = 16, ch = pow2(ceil_div(pieces, 1024));
   const uint32_t block = waves == 1 ? 256 : 64 * waves;
   const uint64_t grid = waves == 1 ? ceil_div(rows, 4) : rows;
@@ -88,7 +90,7 @@ tiler_hip_status plan_layer_norm(const Target& t, uint32_t dtype, uint32_t parts
   if (rows == 0 || extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
-  const RowForm f = row_form(t, rows, extent, 16 / elem, 8);
+  const RowForm f = row_form(t, rows, extent, 16 / elem, 4);
   std::snprintf(name, sizeof(name), "tiler_layer_norm_%s_%s", type_name(dtype), f.name);
   Launch& l = p.add(name, (uint32_t)f.grid, 1, f.block).ptr(x);
   slot_or_null(l, has_w, w);
@@ -417,7 +419,7 @@ tiler_hip_status plan_quantize_rows_i8(const Target& t, uint32_t dtype, uint64_t
   if (rows == 0 || extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
-  const RowForm f = row_form(t, rows, extent, dtype == TILER_HIP_BF16 ? 8 : 4, 4);
+  const RowForm f = row_form(t, rows, extent, dtype == TILER_HIP_BF16 ? 8 : 4, dtype == TILER_HIP_BF16 ? 2 : 4);
   std::snprintf(name, sizeof(name), "tiler_quantize_rows_i8_%s_%s", type_name(dtype), f.name);
   p.add(name, (uint32_t)f.grid, 1, f.block)
       .ptr(x).u64(rows).u64(extent).ptr(q).ptr(scales);

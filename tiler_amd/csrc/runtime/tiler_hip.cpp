@@ -369,8 +369,9 @@ const EntryRow kEntries[] = {
       {"tiler_layer_norm_f32_" FORM, "layer-norm-f32", 6},                      \
       {"tiler_quantize_rows_i8_bf16_" FORM, "quantize-rows-i8/bf16", 3},        \
       {"tiler_quantize_rows_i8_f32_" FORM, "quantize-rows-i8/f32", 3}
-    TILER_ROW_FORM("s"), TILER_ROW_FORM("w1c1"), TILER_ROW_FORM("w1c2"), TILER_ROW_FORM("w1c4"),
-    {"tiler_layer_norm_bf16_w1c8", "layer-norm/bf16", 6}, {"tiler_layer_norm_f32_w1c8", "layer-norm-f32", 6},
+    TILER_ROW_FORM("s"), TILER_ROW_FORM("w1c1"), TILER_ROW_FORM("w1c2"),
+    {"tiler_layer_norm_bf16_w1c4", "layer-norm/bf16", 6}, {"tiler_layer_norm_f32_w1c4", "layer-norm-f32", 6},
+    {"tiler_quantize_rows_i8_f32_w1c4", "quantize-rows-i8/f32", 3},
     TILER_ROW_FORM("w4c1"), TILER_ROW_FORM("w4c2"),
     TILER_ROW_FORM("w4c4"), TILER_ROW_FORM("w16c1"), TILER_ROW_FORM("w16c2"), TILER_ROW_FORM("w16c4"),
 #undef TILER_ROW_FORM
