@@ -1,0 +1,83 @@
+"""The feed-forward sublayer's calls at the ends of their ranges."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import feed_forward_reference as ref
+from test_gpu_layer_norm import Buffers, backward, kept, rows_of, within
+
+pytestmark = pytest.mark.gpu
+
+U = ref.U
+
+
+@pytest.fixture
+def mem(ctx):
+    m = Buffers(ctx)
+    yield m
+    m.free()
+
+
+def bf(values):
+    return ref.store("bf16", values)
+
+
+def w64(stored):
+    return ref.wide("bf16", stored)
+
+
+# -- the norm's gradients far from zero ------------------------------------------
+
+def backward_bounds(dtype, dy, x, w, mean, rstd):
+    """mean and rstd are operands, so x - mean rounds by U |x - mean| and xh, one
+    more product, by 2 U |xh|, wherever the row lies.  The rest as in
+    ref.layer_norm_backward_bounds: the row means 52 U of their magnitudes, the
+    terms of dx at most 6 roundings, the column sums rows + 600 additions."""
+    dx, dw, db = ref.layer_norm_backward(dy, x, w, mean, rstd)
+    xh = np.abs((x - mean[:, None]) * rstd[:, None])
+    g = np.abs(dy if w is None else dy * w)
+    m1, m2 = g.mean(-1, keepdims=True), (g * xh).mean(-1, keepdims=True)
+    e_dx = rstd[:, None] * (4 * U * g + (52 + 4) * U * m1 + xh * (56 + 2 + 2 + 6) * U * m2)
+    n = min(x.shape[0], 1200) + 600
+    e_dw, e_db = (n + 2) * U * (np.abs(dy) * xh).sum(0), n * U * np.abs(dy).sum(0)
+    h = ref.half(dtype)
+    return e_dx + h * (np.abs(dx) + e_dx), e_dw + h * (np.abs(dw) + e_dw), e_db + h * (np.abs(db) + e_db)
+
+
+def check_backward(ctx, mem, dtype, dy, x, w, mean, rstd):
+    args = (ref.wide(dtype, dy), ref.wide(dtype, x), None if w is None else ref.wide(dtype, w), mean.astype(np.float64),
+            rstd.astype(np.float64))
+    got = backward(ctx, mem, dtype, dy, x, w, mean, rstd)
+    for g, v, e, what in zip(got, ref.layer_norm_backward(*args), backward_bounds(dtype, *args), ("dx", "dw", "db")):
+        within(ref.wide(dtype, g), v, e, what)
+
+
+# the forms of one to sixteen waves a row, two pieces a thread, and streamed rows
+@pytest.mark.parametrize("extent", [100, 256, 509, 1023, 2048, 4096, 8190, 20001])
+@pytest.mark.parametrize("offset", [3000.0, -1e5])
+def test_gradients_do_not_lose_a_row_far_from_zero(ctx, mem, offset, extent):
+    rng = np.random.default_rng(extent)
+    x = (rows_of(rng, 70, extent, "f32") + np.float32(offset)).astype(np.float32)
+    dy, w = rng.standard_normal((70, extent)).astype(np.float32), rng.normal(1, 0.2, extent).astype(np.float32)
+    for weight in (w, None):
+        check_backward(ctx, mem, "f32", dy, x, weight, *kept("f32", x))
+
+
+@pytest.mark.parametrize("extent", [100, 1024, 4096, 16384])
+def test_gradients_of_nearly_constant_bf16_rows(ctx, mem, extent):
+    rng = np.random.default_rng(extent)
+    x = np.full((40, extent), 200.0)
+    x[np.arange(40), rng.integers(0, extent, 40)] += 1
+    x, dy, w = bf(x), bf(rng.standard_normal((40, extent))), bf(rng.normal(1, 0.2, extent))
+    check_backward(ctx, mem, "bf16", dy, x, w, *kept("bf16", x))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("extent", [100, 4096, 20001])
+def test_gradients_of_constant_rows_with_a_tiny_eps(ctx, mem, dtype, extent):
+    """rstd = 1 / sqrt(eps) whose square passes binary32's range."""
+    rng = np.random.default_rng(extent)
+    x, dy = ref.store(dtype, np.full((6, extent), 3.0)), ref.store(dtype, rng.standard_normal((6, extent)))
+    mean, rstd = np.full(6, 3, np.float32), np.full(6, 2e20, np.float32)
+    check_backward(ctx, mem, dtype, dy, x, None, mean, rstd)
