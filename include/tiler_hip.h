@@ -796,8 +796,8 @@ tiler_hip_status tiler_hip_layer_norm(tiler_hip_context *ctx, uint32_t dtype, co
 /* Its gradients, with xh = (x - mu) r and g = dy w:
  *   dx = r (g - mean(g) - xh mean(g xh)), dw = sum over rows of dy xh, db = of dy
  * mean and rstd as the forward call wrote them.  Any of dx, dw and db may be
- * NULL (not wanted).  With no rows dw and db are zeros.  Sums in binary32 or
- * more, in a fixed order. */
+ * NULL (not wanted).  With no rows dw and db are zeros.  Rows up to 2^32 - 1
+ * elements.  Sums in binary32 or more, in a fixed order. */
 tiler_hip_status tiler_hip_layer_norm_backward(tiler_hip_context *ctx, uint32_t dtype, const void *dy,
                                                const void *x, const void *w, const float *mean,
                                                const float *rstd, uint64_t rows, uint64_t extent, void *dx,

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import feed_forward_reference as ref
+from tiler_amd import _lib as L
 from test_gpu_layer_norm import Buffers, backward, kept, rows_of, within
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +82,25 @@ def test_gradients_of_constant_rows_with_a_tiny_eps(ctx, mem, dtype, extent):
     x, dy = ref.store(dtype, np.full((6, extent), 3.0)), ref.store(dtype, rng.standard_normal((6, extent)))
     mean, rstd = np.full(6, 3, np.float32), np.full(6, 2e20, np.float32)
     check_backward(ctx, mem, dtype, dy, x, None, mean, rstd)
+
+
+# -- very long rows ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("extent", [(1 << 26) + 70, (1 << 28) + 5])
+def test_column_sums_of_very_long_rows(ctx, mem, extent):
+    """More columns than the column kernels have threads: each takes further ones.
+    Whole numbers, mean 0 and rstd 1: dw is the sum of dy x, exactly."""
+    pattern = np.arange(1021) % 13 - 6  # prime: no period of the columns' groups
+    dy, x = np.resize(bf(pattern), extent), np.resize(bf(pattern % 5 + 1), extent)
+    mean, rstd = mem.put(np.zeros(1, np.float32)), mem.put(np.ones(1, np.float32))
+    ws = ctx.alloc(ctx.layer_norm_backward_workspace(L.BF16, 1, extent))
+    bufs = [ctx.to_device(dy), ctx.to_device(x), ctx.alloc(2 * extent), ctx.alloc(2 * extent)]
+    try:
+        ctx.layer_norm_backward(L.BF16, bufs[0], bufs[1], None, mean, rstd, 1, extent, None, bufs[2], bufs[3],
+                                workspace=ws, workspace_bytes=ws.nbytes)
+        ctx.synchronize()
+        assert np.array_equal(bufs[3].download(np.uint16, (extent,)), np.resize(bf(pattern + 0.0), extent))
+        assert np.array_equal(bufs[2].download(np.uint16, (extent,)), np.resize(bf(pattern * (pattern % 5 + 1)), extent))
+    finally:
+        for b in [*bufs, ws]:
+            b.free()

@@ -361,31 +361,31 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
   }
 }
 
-// Column sums over a strip of rows: blockIdx.x takes 256 columns, blockIdx.y
-// rows [y * strip, ...); partial y holds dw's sums, then db's.
+// Column sums over a strip of rows: blockIdx.x takes 256 columns at a time,
+// blockIdx.y rows [y * strip, ...); partial y holds dw's sums, then db's.
 template <typename T>
 __device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, const T* __restrict__ x,
                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
                                                    uint64_t rows, uint64_t extent, uint64_t strip,
                                                    float* __restrict__ partials) {
-  const uint64_t col = blockIdx.x * 256ull + threadIdx.x;
-  if (col >= extent) return;
   const uint64_t r0 = blockIdx.y * strip, r1 = r0 + strip < rows ? r0 + strip : rows;
-  float sw = 0.0f, sb = 0.0f;
-  for (uint64_t r = r0; r < r1; ++r) {
-    const float d = norm_load(dy, r * extent + col);
-    sw += d * ((norm_load(x, r * extent + col) - mean[r]) * rstd[r]);
-    sb += d;
-  }
   const uint64_t ld = partial_ld(extent);
   float* out = partials + (uint64_t)blockIdx.y * 2u * ld;
-  out[col] = sw;
-  out[ld + col] = sb;
+  for (uint64_t col = blockIdx.x * 256ull + threadIdx.x; col < extent; col += gridDim.x * 256ull) {
+    float sw = 0.0f, sb = 0.0f;
+    for (uint64_t r = r0; r < r1; ++r) {
+      const float d = norm_load(dy, r * extent + col);
+      sw += d * ((norm_load(x, r * extent + col) - mean[r]) * rstd[r]);
+      sb += d;
+    }
+    out[col] = sw;
+    out[ld + col] = sb;
+  }
 }
 
-// dw (blockIdx.y 0) and db (1) from `count` partials: 64 columns a workgroup,
-// wave q the partials q, q + 16, ... in ascending order, the waves' sums in
-// ascending order.
+// dw (blockIdx.y 0) and db (1) from `count` partials: 64 columns a workgroup at
+// a time, wave q the partials q, q + 16, ... in ascending order, the waves' sums
+// in ascending order.
 template <typename T>
 __device__ __forceinline__ void layer_norm_columns_final(const float* __restrict__ partials, uint32_t count,
                                                          uint64_t extent, T* __restrict__ dw, T* __restrict__ db) {
@@ -393,19 +393,24 @@ __device__ __forceinline__ void layer_norm_columns_final(const float* __restrict
   T* const out = blockIdx.y ? db : dw;
   if (!out) return;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint64_t col = blockIdx.x * 64ull + lane, ld = partial_ld(extent);
-  float s = 0.0f;
-  if (col < extent) {
-    const float* at = partials + blockIdx.y * ld + col;
+  const uint64_t ld = partial_ld(extent);
+  for (uint64_t first = blockIdx.x * 64ull; first < extent; first += gridDim.x * 64ull) {  // the same for every wave
+    const uint64_t col = first + lane;
+    float s = 0.0f;
+    if (col < extent) {
+      const float* at = partials + blockIdx.y * ld + col;
 #pragma unroll 8
-    for (uint32_t p = wave; p < count; p += 16u) s += at[(uint64_t)p * 2u * ld];
-  }
-  waves[wave][lane] = s;
-  __syncthreads();
-  if (wave != 0 || col >= extent) return;
+      for (uint32_t p = wave; p < count; p += 16u) s += at[(uint64_t)p * 2u * ld];
+    }
+    if (first != blockIdx.x * 64ull) __syncthreads();  // the columns before are read
+    waves[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < extent) {
 #pragma unroll
-  for (int q = 1; q < 16; ++q) s += waves[q][lane];
-  norm_store(out, col, s);
+      for (int q = 1; q < 16; ++q) s += waves[q][lane];
+      norm_store(out, col, s);
+    }
+  }
 }
 
 }  // namespace

@@ -25,6 +25,11 @@ void slot_or_null(Launch& l, bool present, uint32_t slot) {
 }
 
 constexpr uint32_t kRowWorkgroups = 1u << 20;  // rows beyond take further rounds of the streamed forms' row loops
+constexpr uint32_t kColumnWorkgroups = 1u << 20;  // and groups of columns of the column sums' loops
+uint32_t column_groups(uint64_t extent, uint64_t columns) {
+  const uint64_t groups = ceil_div(extent, columns);
+  return (uint32_t)(groups < kColumnWorkgroups ? groups : kColumnWorkgroups);
+}
 
 // The register form of a row kernel (row_pieces.h) for rows of `extent`
 // elements, kVec = `vec` to a 16-byte piece: WAVES waves per row and CH pieces
@@ -155,13 +160,13 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
     count = ceil_div(rows, 16) < t.compute_units ? ceil_div(rows, 16) : t.compute_units;
     partials = p.slot(mul_sat(mul_sat(count, ceil_div(extent, 8) * 8), 8), kSlotScratch);
     std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_%s", type_name(dtype));
-    p.add(name, (uint32_t)ceil_div(extent, 256), (uint32_t)count, 256)
+    p.add(name, column_groups(extent, 256), (uint32_t)count, 256)
         .ptr(dy).ptr(x).ptr(mean).ptr(rstd).u64(rows).u64(extent).u64(ceil_div(rows, count)).ptr(partials);
   } else if (!sums) {
     return TILER_HIP_OK;
   }
   std::snprintf(name, sizeof(name), "tiler_layer_norm_columns_final_%s", type_name(dtype));
-  Launch& l = p.add(name, (uint32_t)ceil_div(extent, 64), 2, 1024);
+  Launch& l = p.add(name, column_groups(extent, 64), 2, 1024);
   slot_or_null(l, count > 0, partials);  // no rows: zeros
   l.u32((uint32_t)count).u64(extent);
   slot_or_null(l, has_dw, dw);
