@@ -1064,7 +1064,8 @@ typedef struct {
     uint32_t slot_count;
     uint32_t slot_roles[18];    /* TILER_HIP_SLOT_* */
     uint64_t slot_bytes[18];
-    uint32_t slot_alignment;    /* precondition on every slot base: 16 with ALIGNED16, else 1 */
+    uint32_t slot_alignment;    /* precondition on every slot base: 16 with ALIGNED16, else 1 (the
+                                   scratch slots of the two backward programs: 16 in any case) */
     uint32_t entry_count;       /* 0: zero work, nothing to dispatch */
     tiler_hip_realized_entry entries[4]; /* in execution order */
     uint32_t constant_slot;     /* the CONSTANT slot (slot_count when there is none) */

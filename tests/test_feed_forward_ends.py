@@ -4,7 +4,8 @@ from __future__ import annotations
 import pytest
 
 from tiler_amd import _lib as L
-from tiler_amd.realize import realize
+from tiler_amd.realize import prepare_route, realize
+from tiler_amd.runtime import Refusal
 
 RE = L.PERMITS_REASSOCIATION
 ALL_NORM = L.NORM_WEIGHT | L.NORM_DX | L.NORM_DW | L.NORM_DB
@@ -21,3 +22,23 @@ def test_norm_gradients_fit_a_launch(dtype, rows, extent):
         assert rz.dispatches
         for d in rz.dispatches:
             assert all(g * b < 1 << 32 for g, b in zip(d.grid, d.block)), (d.symbol, d.grid, d.block)
+
+
+@pytest.mark.parametrize("program,extents,variant", [
+    (L.PROGRAM_LAYER_NORM_BACKWARD, (600, 512), ALL_NORM),
+    (L.PROGRAM_LAYER_NORM_BACKWARD, (600, 40000), ALL_NORM),
+    (L.PROGRAM_GATED_CONTRACTION_BACKWARD, (300, 520, 264), L.GATED_DX | L.GATED_DW),
+    (L.PROGRAM_GATED_CONTRACTION_BACKWARD, (300, 520, 333), L.GATED_DX | L.GATED_DW)])
+def test_routed_scratch_is_aligned(program, extents, variant):
+    """Operands at any address; a caller's scratch from a 16-byte boundary, as the
+    direct call's workspace.  Refused before the context is asked for anything."""
+    rz = realize(program, extents, dtype=L.BF16, variant=variant, permissions=RE, flags=0)
+    assert rz.alignment == 1
+    scratch = [i for i, (role, _) in enumerate(rz.slots) if role == L.SLOT_SCRATCH]
+    assert scratch
+    for slot in scratch:
+        for off in (2, 8):
+            storage = [(4096 if i in scratch else 4098) + (off if i == slot else 0) for i in range(len(rz.slots))]
+            with pytest.raises(Refusal) as e:
+                prepare_route(None, rz, storage)
+            assert e.value.status == L.REFUSE_BINDING_MISMATCH and f"slot {slot} " in str(e.value)

@@ -6,6 +6,7 @@ import pytest
 
 import feed_forward_reference as ref
 from tiler_amd import _lib as L
+from tiler_amd.realize import realize, route
 from test_gpu_layer_norm import Buffers, backward, kept, rows_of, within
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +105,31 @@ def test_column_sums_of_very_long_rows(ctx, mem, extent):
     finally:
         for b in [*bufs, ws]:
             b.free()
+
+
+# -- routed with the caller's scratch -----------------------------------------------------
+
+@pytest.mark.parametrize("m,n,k", [(300, 520, 264), (300, 520, 333)])
+def test_routed_gradients_in_the_callers_scratch(ctx, mem, m, n, k):
+    """Operands at odd elements, scratch a 16-byte step past its allocations: the
+    direct call's bits, and nothing written past the slots."""
+    rng = np.random.default_rng(k)
+    shapes = [(m, k), (n, k), (n, k), (m, n), (m, n), (m, n)]
+    operands = [mem.put(bf(rng.standard_normal(s)), 1) for s in shapes]
+    want = [mem.out(np.uint16, c) for c in (m * k, n * k, n * k)]
+    ctx.gated_contract_bf16_backward(*operands, m, n, k, *want)
+    rz = realize(L.PROGRAM_GATED_CONTRACTION_BACKWARD, (m, n, k), dtype=L.BF16, variant=L.GATED_DX | L.GATED_DW,
+                 permissions=L.PERMITS_REASSOCIATION, flags=0, ctx=ctx)
+    got, scratch = [mem.out(np.uint16, c, 1) for c in (m * k, n * k, n * k)], []
+    given = iter(operands + got)
+    storage = []
+    for role, nbytes in rz.slots:
+        if role == L.SLOT_SCRATCH:
+            scratch.append((mem.out(np.uint8, nbytes, 16), nbytes))
+        storage.append(scratch[-1][0] if role == L.SLOT_SCRATCH else next(given))
+    assert scratch
+    route(ctx, rz, storage)
+    for w, g, c in zip(want, got, (m * k, n * k, n * k)):
+        assert np.array_equal(mem.get(w, np.uint16, (c,)), mem.get(g, np.uint16, (c,)))
+    for v, nbytes in scratch:
+        mem.get(v, np.uint8, (nbytes,))

@@ -58,6 +58,17 @@ class Realization:
     def symbols(self) -> list:
         return [d.symbol for d in self.dispatches]
 
+    def slot_alignment(self, slot: int) -> int:
+        """What slot `slot`'s address has to be a multiple of.  The scratch of
+        the feed-forward sublayer's gradients is moved in aligned 16-byte
+        pieces, however the operands lie."""
+        if self.slots[slot][0] == L.SLOT_SCRATCH and self.program in _ALIGNED_SCRATCH:
+            return 16
+        return self.alignment
+
+
+_ALIGNED_SCRATCH = (L.PROGRAM_LAYER_NORM_BACKWARD, L.PROGRAM_GATED_CONTRACTION_BACKWARD)
+
 
 def _entry_info(index: int):
     info = L.EntryInfo()
@@ -304,9 +315,10 @@ def prepare_route(ctx, realization: Realization, storage, payload=None, extents=
         cap = _capacity(buf)
         if cap is not None and cap < nbytes:
             raise Refusal(L.REFUSE_BINDING_MISMATCH, "route", f"slot {i} holds {cap} of {nbytes} bytes")
-        if _address(buf) % rz.alignment:
+        alignment = rz.slot_alignment(i)
+        if _address(buf) % alignment:
             raise Refusal(L.REFUSE_BINDING_MISMATCH, "route",
-                          f"slot {i} is not {rz.alignment}-byte aligned as the realization assumed")
+                          f"slot {i} is not {alignment}-byte aligned as the realization assumed")
     n = rz.raw.entry_count
     entries = (L.DispatchEntry * n)()
     keep = []
