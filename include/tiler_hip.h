@@ -785,8 +785,9 @@ tiler_hip_status tiler_hip_contract(tiler_hip_context *ctx, uint32_t dtype,
  * dtype TILER_HIP_F32 or TILER_HIP_BF16 (binary32 arithmetic on exactly
  * widened operands, one narrowing of y).  w and b are one row of `extent`
  * each; NULL reads as ones and as zeros.  mean and rstd (f32 [rows], both or
- * neither) receive mu and r for the gradients.  eps positive and finite; rows
- * up to 2^32 - 1 elements.  The variance is that of the differences from the
+ * neither) receive mu and r for the gradients; rows without elements have
+ * none and are refused with them.  eps positive and finite; rows up to
+ * 2^32 - 1 elements.  The variance is that of the differences from the
  * mean, never a difference of squares.  A row holding a NaN or an infinity
  * gives NaNs. */
 tiler_hip_status tiler_hip_layer_norm(tiler_hip_context *ctx, uint32_t dtype, const void *x,
@@ -835,7 +836,8 @@ tiler_hip_status tiler_hip_gated_contract_bf16_backward_workspace(const tiler_hi
  *   scales[i] = max(fl(max |x_i| / 127), 2^-126), q_ij = x_ij / scales[i] to the
  *   nearest integer, ties to even, exactly (in -127 .. 127)
  * A row holding a NaN or an infinity has the scale NaN and codes 0, so that
- * what is computed from it is NaN. */
+ * what is computed from it is NaN.  Rows without elements have no scale and are
+ * refused. */
 tiler_hip_status tiler_hip_quantize_rows_i8(tiler_hip_context *ctx, uint32_t dtype, const void *x,
                                             uint64_t rows, uint64_t extent, int8_t *q, float *scales,
                                             tiler_hip_stream stream);

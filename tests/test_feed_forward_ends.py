@@ -42,3 +42,17 @@ def test_routed_scratch_is_aligned(program, extents, variant):
             with pytest.raises(Refusal) as e:
                 prepare_route(None, rz, storage)
             assert e.value.status == L.REFUSE_BINDING_MISMATCH and f"slot {slot} " in str(e.value)
+
+
+def test_empty_rows():
+    """No element, no mean and no scale: refused where one is asked for."""
+    eps = (0x3727C5AC, 0)
+    for rows in (1, 100):
+        for program, kw in ((L.PROGRAM_LAYER_NORM, dict(variant=L.NORM_STATISTICS, scalars=eps)),
+                            (L.PROGRAM_LAYER_NORM, dict(variant=L.NORM_WEIGHT | L.NORM_BIAS | L.NORM_STATISTICS, scalars=eps)),
+                            (L.PROGRAM_QUANTIZE_ROWS_I8, {})):
+            with pytest.raises(Refusal) as e:
+                realize(program, (rows, 0), dtype=L.BF16, permissions=RE, **kw)
+            assert e.value.status == L.REFUSE_INVALID_ARGUMENT
+            assert realize(program, (0, 0), dtype=L.BF16, permissions=RE, **kw).symbols == []
+    assert realize(L.PROGRAM_LAYER_NORM, (100, 0), dtype=L.BF16, permissions=RE, scalars=eps).symbols == []

@@ -6,7 +6,9 @@ import pytest
 
 import feed_forward_reference as ref
 from tiler_amd import _lib as L
+from tiler_amd import families
 from tiler_amd.realize import realize, route
+from tiler_amd.runtime import Refusal
 from test_gpu_layer_norm import Buffers, backward, kept, rows_of, within
 
 pytestmark = pytest.mark.gpu
@@ -133,3 +135,25 @@ def test_routed_gradients_in_the_callers_scratch(ctx, mem, m, n, k):
         assert np.array_equal(mem.get(w, np.uint16, (c,)), mem.get(g, np.uint16, (c,)))
     for v, nbytes in scratch:
         mem.get(v, np.uint8, (nbytes,))
+
+
+# -- rows without elements ----------------------------------------------------------
+
+def test_empty_rows(ctx, mem):
+    """No element, no mean and no scale: refused where one is asked for, and
+    nothing is written."""
+    mean, rstd, y = mem.out(np.float32, 3), mem.out(np.float32, 3), mem.out(np.uint16, 8)
+    x = mem.put(np.zeros(8, np.uint16))
+    for call in (lambda: ctx.layer_norm(L.BF16, x, None, None, 3, 0, ref.EPS_BITS, y, mean, rstd),
+                 lambda: ctx.quantize_rows_i8(L.BF16, x, 3, 0, y, mean),
+                 lambda: families.layer_norm(np.zeros((3, 0), np.uint16), ctx=ctx),
+                 lambda: families.quantize_rows_i8(np.zeros((3, 0), np.float32), ctx=ctx)):
+        with pytest.raises(Refusal) as e:
+            call()
+        assert e.value.status == L.REFUSE_INVALID_ARGUMENT
+    ctx.layer_norm(L.BF16, x, None, None, 3, 0, ref.EPS_BITS, y)
+    ctx.layer_norm(L.BF16, x, None, None, 0, 0, ref.EPS_BITS, y, mean, rstd)
+    ctx.quantize_rows_i8(L.BF16, x, 0, 0, y, mean)
+    ctx.synchronize()
+    for v, t, c in ((mean, np.float32, 3), (rstd, np.float32, 3), (y, np.uint16, 8)):
+        assert (mem.get(v, t, (c,)).view(np.uint8) == 0xA5).all()

@@ -92,6 +92,8 @@ tiler_hip_status plan_layer_norm(const Target& t, uint32_t dtype, uint32_t parts
   const uint32_t y = p.slot(bytes, kSlotOutput);
   const uint32_t mean = stats ? p.slot(mul_sat(rows, 4), kSlotOutput) : 0;
   const uint32_t rstd = stats ? p.slot(mul_sat(rows, 4), kSlotOutput) : 0;
+  if (rows && extent == 0 && stats)
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows without elements have no mean");
   if (rows == 0 || extent == 0) return TILER_HIP_OK;
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
@@ -421,7 +423,8 @@ tiler_hip_status plan_quantize_rows_i8(const Target& t, uint32_t dtype, uint64_t
   const uint64_t n = mul_sat(rows, extent);
   const uint32_t x = p.slot(mul_sat(n, dtype == TILER_HIP_BF16 ? 2 : 4), kSlotInput);
   const uint32_t q = p.slot(n, kSlotOutput), scales = p.slot(mul_sat(rows, 4), kSlotOutput);
-  if (rows == 0 || extent == 0) return TILER_HIP_OK;
+  if (rows == 0) return TILER_HIP_OK;
+  if (extent == 0) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows without elements have no scale");
   if (extent > 0xffffffffull) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "row longer than 2^32 - 1 elements");
   char name[64];
   const RowForm f = row_form(t, rows, extent, dtype == TILER_HIP_BF16 ? 8 : 4, dtype == TILER_HIP_BF16 ? 2 : 4);
