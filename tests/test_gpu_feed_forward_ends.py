@@ -9,7 +9,7 @@ from tiler_amd import _lib as L
 from tiler_amd import families
 from tiler_amd.realize import realize, route
 from tiler_amd.runtime import Refusal
-from test_gpu_layer_norm import Buffers, backward, kept, rows_of, within
+from test_gpu_layer_norm import Buffers, backward, forward, kept, rows_of, within
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +157,53 @@ def test_empty_rows(ctx, mem):
     ctx.synchronize()
     for v, t, c in ((mean, np.float32, 3), (rstd, np.float32, 3), (y, np.uint16, 8)):
         assert (mem.get(v, t, (c,)).view(np.uint8) == 0xA5).all()
+
+
+# -- the norm far from zero -------------------------------------------------------
+
+def forward_bounds(dtype, x, w, b, e_mean):
+    """`e_mean`: how far the row's first, binary32 mean may be off.  The
+    differences from it round by U of themselves; their mean (52 U of their
+    magnitudes) is taken off again, so that y carries rounding of the differences'
+    size, not of the row's.  rstd: the variance's 60 U, of its sum of squares
+    around the first mean, and 4 U."""
+    y, mu, r = ref.layer_norm(x, w, b)
+    d, r = np.abs(x - mu[:, None]), r[:, None]
+    off = 54 * U * (d.mean(-1, keepdims=True) + e_mean) + 2 * U * e_mean
+    e_r = 60 * U * (1 + (e_mean * r) ** 2) + (off * r) * (e_mean * r) + 4 * U
+    e_xh = (U * (d + e_mean) + off) * r + d * r * (e_r + 4 * U)
+    scale = 1.0 if w is None else np.abs(w)
+    e_y = e_xh * scale + 2 * U * (d * r * scale + (0.0 if b is None else np.abs(b)))
+    return e_y + ref.half(dtype) * (np.abs(y) + e_y), U * np.abs(mu) + off[:, 0], (e_r * r)[:, 0]
+
+
+def check_forward(ctx, mem, dtype, x, w, b, e_mean):
+    args = (ref.wide(dtype, x), None if w is None else ref.wide(dtype, w), None if b is None else ref.wide(dtype, b))
+    bounds = forward_bounds(dtype, *args, e_mean)
+    for got, want, bound, what in zip(forward(ctx, mem, dtype, x, w, b), ref.layer_norm(*args), bounds, ("y", "mean", "rstd")):
+        within(ref.wide(dtype, got) if what == "y" else got, want, bound, what)
+
+
+@pytest.mark.parametrize("extent", [100, 509, 1023, 4096, 8190, 16380, 20001])
+@pytest.mark.parametrize("offset", [3000.0, -1e5])
+def test_norm_of_rows_far_from_zero(ctx, mem, offset, extent):
+    rng = np.random.default_rng(extent)
+    x = (rows_of(rng, 37, extent, "f32") + np.float32(offset)).astype(np.float32)
+    w, b = rng.normal(1, 0.2, extent).astype(np.float32), rng.normal(0, 0.2, extent).astype(np.float32)
+    e_mean = 52 * U * np.abs(x.astype(np.float64)).mean(-1, keepdims=True)
+    for weight, bias in ((w, b), (w, None), (None, b), (None, None)):
+        check_forward(ctx, mem, "f32", x, weight, bias, e_mean)
+
+
+@pytest.mark.parametrize("extent", [100, 509, 2046, 4096, 8190, 16382, 32766, 40000])
+def test_norm_of_nearly_constant_bf16_rows(ctx, mem, extent):
+    """Whole numbers: their sum is below 2^24 and exact, so the first mean is off by
+    its rounding alone."""
+    rng = np.random.default_rng(extent)
+    x = np.full((37, extent), 200.0)
+    for i in range(37):
+        x[i, rng.integers(0, extent, 1 + i % 4)] += rng.integers(1, 4)
+    w, b = bf(rng.normal(1, 0.2, extent)), bf(rng.normal(0, 0.2, extent))
+    assert x.sum(-1).max() < 1 << 24
+    for weight, bias in ((w, b), (None, None)):
+        check_forward(ctx, mem, "bf16", bf(x), weight, bias, 256 * U)

@@ -96,10 +96,15 @@ __device__ __forceinline__ void layer_norm_grad_stream(const T* __restrict__ dy,
 // Rows in registers.
 
 // Forward: a group of WAVES waves per row, CH pieces a thread.  The mean first,
-// then the squares of the differences from it.  For f32 rows the differences
-// are summed too: that corrects the mean's rounding, which a row far from zero
-// would otherwise carry into its results (bf16 results round far more coarsely,
-// and the sum would cost a tenth of the kernel).
+// then the squares of the differences from it.  The binary32 mean is off by its
+// roundings, |mu| 2^-24 and more, which a row far from zero or nearly constant
+// would carry into its results, so what it is off by (`shift`) is taken off the
+// differences too, in the FMA that scales them.  f32 rows: the mean of the
+// differences.  bf16 rows: the remainder of the division; their sum is all but
+// exact (8 bits a value, where the values are of one size) and the sum of the
+// differences would cost a tenth of the kernel.  With a row 10^5 deviations from
+// zero y is off by 1e-6 of a deviation, by 1e-2 with the mean alone; 8192 x 4096
+// bf16 27.2 us, with the mean alone 27.05.
 template <typename T, int WAVES, int CH>
 __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T* __restrict__ w,
                                                 const T* __restrict__ b, uint64_t rows, uint32_t extent, float eps,
@@ -118,6 +123,7 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
   u32x4 v[CH];
   load_row<T, WAVES, CH, true>(x, t, extent, v);
   settle_row<T, WAVES, CH>(t, extent, v);
+  const float count = (float)extent, inverse = 1.0f / count;
   float s = 0.0f, none = 0.0f;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -130,8 +136,8 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
   // opaque: widened again below, not kept widened across the sums
 #pragma unroll
   for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(v[c]));
-  const float count = (float)extent;
-  float mu = s / count, s1 = 0.0f, s2 = 0.0f;
+  const float mu = s / count;  // divided: a constant row's is exact
+  float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     float d[V], q = 0.0f;
@@ -151,16 +157,12 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
   group_sums<WAVES>(s2, s1, slots[1]);
 #pragma unroll
   for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(v[c]));
-  float var = s2 / count;
-  if constexpr (kCorrect) {
-    const float shift = s1 / count;
-    var = __builtin_fmaf(-shift, shift, var);
-    var = var < 0.0f ? 0.0f : var;
-    mu = mu + shift;
-  }
-  const float r = 1.0f / __builtin_sqrtf(var + eps);
+  const float shift = (kCorrect ? s1 : __builtin_fmaf(-mu, count, s)) * inverse;
+  float var = __builtin_fmaf(-shift, shift, s2 * inverse);
+  var = var < 0.0f ? 0.0f : var;
+  const float r = 1.0f / __builtin_sqrtf(var + eps), off = -(shift * r);
   if (t == 0 && mean) {
-    mean[row] = mu;
+    mean[row] = mu + shift;
     rstd[row] = r;
   }
   // w and b a few pieces at a time: they come from the caches
@@ -184,7 +186,7 @@ __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T
       float o[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        o[i] = (element<T>(v[c0 + c], i) - mu) * r;
+        o[i] = __builtin_fmaf(element<T>(v[c0 + c], i) - mu, r, off);
         if (w && b) o[i] = __builtin_fmaf(o[i], element<T>(wv[c], i), element<T>(bv[c], i));
         else if (w) o[i] = o[i] * element<T>(wv[c], i);
         else if (b) o[i] = o[i] + element<T>(bv[c], i);
