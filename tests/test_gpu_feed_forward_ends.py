@@ -207,3 +207,59 @@ def test_norm_of_nearly_constant_bf16_rows(ctx, mem, extent):
     assert x.sum(-1).max() < 1 << 24
     for weight, bias in ((w, b), (None, None)):
         check_forward(ctx, mem, "bf16", bf(x), weight, bias, 256 * U)
+
+
+# -- far gates --------------------------------------------------------------------
+
+FAR = np.array([-174.0, -160.0, -140.0, -120.0, -100.0, -95.0, -92.0, -90.0, -89.0, -88.5, -88.0, -87.5, -87.0, -85.0,
+                -80.0, -60.0, -30.0, -8.0, -1.28125, -0.0, 0.5, 8.0, 30.0, 80.0, 88.0, 90.0, 120.0, 200.0])
+
+
+def sigmoid(g):
+    """s and 1 - s, neither of them a difference."""
+    t = np.exp(-np.abs(g))
+    return np.where(g < 0, t, 1) / (1 + t), np.where(g < 0, 1, t) / (1 + t)
+
+
+def gate_bound(value, g, terms=None):
+    """The exponent of e^(-|G| / 2) rounds twice, |G| U of relative error in all, and
+    the factor enters twice; two exponentials of 2 U, a reciprocal, the products
+    and slope's sum 16 U.  Then bf16's rounding, at least half its least step."""
+    e = (20 + 2 * np.abs(g)) * U * (np.abs(value) if terms is None else terms)
+    return e + np.maximum(ref.half("bf16") * (np.abs(value) + e), 2.0 ** -134)
+
+
+@pytest.mark.parametrize("m,k", [(3, 64), (40, 333), (70, 5), (200, 1024), (700, 2048)])
+def test_far_gates(ctx, mem, m, k):
+    """silu(G) down to where bf16 holds nothing of the result: e^-G itself passes
+    binary32's range below G = -88.7, silu(G) U need not."""
+    n, rng = 2 * len(FAR), np.random.default_rng(m)
+    x, wg, wu = np.zeros((m, k)), np.zeros((n, k)), np.zeros((n, k))
+    x[:, 0] = x[:, 1] = 1  # one product each of G and U: exact
+    wg[:, 0] = np.tile(FAR, 2)
+    wu[:, 1] = np.repeat([1.5, -2.0 ** 100], len(FAR))
+    args = [bf(v) for v in (x, wg, wu)]
+    h, gate, up = (mem.out(np.uint16, m * n) for _ in range(3))
+    ctx.gated_contract_bf16(*(mem.put(v) for v in args), m, n, k, h, gate, up)
+    ctx.synchronize()
+    g, u = (np.broadcast_to(v, (m, n)) for v in (wg[:, 0], wu[:, 1]))
+    assert np.array_equal(w64(mem.get(gate, np.uint16, (m, n))), g) and np.array_equal(w64(mem.get(up, np.uint16, (m, n))), u)
+    want = g * sigmoid(g)[0] * u
+    within(w64(mem.get(h, np.uint16, (m, n))), want, gate_bound(want, g), "h")
+
+
+def test_slopes_of_far_gates(ctx, mem):
+    """dG and dU by themselves: one token, x = 1, and a depth of one."""
+    n = 2 * len(FAR)
+    g, u = np.tile(FAR, 2)[None, :], np.repeat([1.5, -2.0 ** 100], len(FAR))[None, :]
+    d = np.repeat([-3.0, 2.0 ** 10], len(FAR))[None, :]
+    one = np.ones((1, 1))
+    dwg, dwu = mem.out(np.uint16, n), mem.out(np.uint16, n)
+    w = mem.put(bf(np.ones((n, 1))))
+    ctx.gated_contract_bf16_backward(mem.put(bf(one)), w, w, *(mem.put(bf(v)) for v in (g, u, d)), 1, n, 1, None, dwg, dwu)
+    ctx.synchronize()
+    s, t = sigmoid(g)
+    want_u, want_g = d * g * s, d * u * s * (1 + g * t)
+    terms = np.abs(d * u * s) * (1 + np.abs(g) * t)
+    within(w64(mem.get(dwu, np.uint16, (1, n))), want_u, gate_bound(want_u, g), "dU")
+    within(w64(mem.get(dwg, np.uint16, (1, n))), want_g, gate_bound(want_g, g, terms), "dG")

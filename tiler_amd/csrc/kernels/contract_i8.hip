@@ -289,7 +289,12 @@ __device__ __forceinline__ void contract_i8_staged(const int8_t* __restrict__ a,
     __syncthreads();
     tiler_product::store_tile_bf16<kRowsA, kRowsB, kThreads, MB, 4, false>(
         smem, row0, col0, static_cast<uint16_t*>(c), m, n, m0, n0,
-        [&](int i, int j, int r) { return (float)acc[i][j][r] * rows[i][r] * cols[j]; });
+        [&](int i, int j) {
+          f32x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][j][r] * rows[i][r] * cols[j];
+          return v;
+        });
   } else {
 #pragma unroll
     for (int i = 0; i < MB; ++i)

@@ -509,7 +509,7 @@ __device__ __forceinline__ uint32_t column_pair(float v0, float v1, bool odd) {
   return __builtin_amdgcn_perm(q, p, odd ? 0x03020706u : 0x05040100u);
 }
 
-// Stores a tile of bf16 results through LDS: value(i, j, r) is this lane's
+// Stores a tile of bf16 results through LDS: value(i, j)[r] is this lane's
 // result of row 16 i + 4 (lane / 16) + r, column 16 j + lane % 16 of its wave's
 // (row0, col0) part of the ROWS x COLS tile; the tile is at (m0, n0) of the
 // m x n result.  16-byte stores of whole row pieces, at any alignment; kStream:
@@ -524,14 +524,16 @@ __device__ __forceinline__ void store_tile_bf16(uint8_t* smem, uint32_t row0, ui
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int j = 0; j < NB; ++j) {
+      const f32x4 v = value(i, j);
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
         const uint32_t row = row0 + i * 16u + (lane >> 4) * 4u + r + (odd ? 1u : 0u);
         const uint32_t col = col0 + j * 16u + (lane & 14u);
         *reinterpret_cast<uint32_t*>(smem + row * kRow + (((col >> 3) ^ (((row & 7u) << 1) & (kPer - 1u))) << 4) + ((col & 7u) << 1)) =
-            column_pair(value(i, j, r), value(i, j, r + 1), odd);
+            column_pair(v[r], v[r + 1], odd);
       }
+    }
   __syncthreads();
 #pragma unroll 4
   for (uint32_t id = threadIdx.x; id < ROWS * kPer; id += THREADS) {
