@@ -56,3 +56,16 @@ def test_empty_rows():
             assert e.value.status == L.REFUSE_INVALID_ARGUMENT
             assert realize(program, (0, 0), dtype=L.BF16, permissions=RE, **kw).symbols == []
     assert realize(L.PROGRAM_LAYER_NORM, (100, 0), dtype=L.BF16, permissions=RE, scalars=eps).symbols == []
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 64, 64), (300, 520, 264), (300, 520, 333), (4096, 14336, 4096), (4096, 14336, 4095)])
+def test_the_workgroups_that_form_the_middle_gradients(m, n, k):
+    """One launch forms dG and dU and copies operands: the kernel is told how many of
+    its workgroups do the former (behind six addresses and m, n, k), and the others
+    are those of the copies."""
+    rz = realize(L.PROGRAM_GATED_CONTRACTION_BACKWARD, (m, n, k), dtype=L.BF16, variant=L.GATED_DX | L.GATED_DW, permissions=RE)
+    d, e = rz.dispatches[0], rz.raw.entries[0]
+    told = [int.from_bytes(bytes(e.kernargs[o:o + 4]), "little") for o in (48, 52, 56, 60)]
+    groups = lambda pieces: min(-(-pieces // 256), 8192)
+    assert d.symbol == "tiler_gated_bf16_grad" and told == [m, n, k, groups(m * (-(-n // 64) * 8))]
+    assert d.grid[0] - told[3] == (groups((m + 2 * n) * -(-k // 8)) if k % 8 else 0)

@@ -78,7 +78,6 @@ __device__ __forceinline__ uint32_t row_of_copy(uint32_t k) { return (k + 7u) & 
 __device__ __forceinline__ uint64_t quotient(uint64_t v, uint32_t by) {  // a 64-bit division costs five of 32
   return v >> 32 ? v / by : (uint32_t)v / by;
 }
-constexpr uint32_t kGradGroups = 8192;  // workgroups that form dG and dU, at most
 
 template <int MB>
 __device__ __forceinline__ void gated_guarded(const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
@@ -150,7 +149,8 @@ tiler_gated_bf16_g64(const uint16_t* __restrict__ x, const uint16_t* __restrict_
 }
 
 // dG and dU (behind dG) of one row's eight columns per item, into rows of n
-// rounded up to 64 (the columns past n are written as zeros).  Where the rows of
+// rounded up to 64 (the columns past n are written as zeros): the first `forming`
+// workgroups; the others copy.  Where the rows of
 // x or of the weights do not start on 16 bytes, they are copied to rows that do,
 // of k rounded up to 8, so that the products always run staged: gradients of
 // 4096 x 14336 x 4095, us, 226 + 712 + 741; with the products' operands through
@@ -158,14 +158,12 @@ tiler_gated_bf16_g64(const uint16_t* __restrict__ x, const uint16_t* __restrict_
 extern "C" __global__ void __launch_bounds__(256)
 tiler_gated_bf16_grad(const uint16_t* __restrict__ gate, const uint16_t* __restrict__ up,
                       const uint16_t* __restrict__ dh, const uint16_t* __restrict__ x, const uint16_t* __restrict__ wg,
-                      const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k, uint16_t* __restrict__ dg,
-                      uint16_t* __restrict__ to_x, uint16_t* __restrict__ to_w) {
+                      const uint16_t* __restrict__ wu, uint32_t m, uint32_t n, uint32_t k, uint32_t forming,
+                      uint16_t* __restrict__ dg, uint16_t* __restrict__ to_x, uint16_t* __restrict__ to_w) {
   using tiler_pieces::guarded_piece;
   using tiler_pieces::u32x4_any;
   const uint32_t ld = row_of_mid(n), per = ld / 8u, ldk = row_of_copy(k), per_k = ldk / 8u;
   const uint64_t mids = (uint64_t)m * per, copies = ((to_x ? (uint64_t)m : 0u) + (to_w ? 2ull * n : 0u)) * per_k;
-  // The first workgroups form dG and dU, the others copy.
-  const uint32_t forming = (uint32_t)(mids < kGradGroups * 256ull ? (mids + 255u) / 256u : kGradGroups);
   if (blockIdx.x >= forming) {
     for (uint64_t id = (blockIdx.x - forming) * 256ull + threadIdx.x; id < copies; id += (gridDim.x - forming) * 256ull) {
       uint64_t row = quotient(id, per_k);

@@ -377,8 +377,9 @@ tiler_hip_status plan_gated_contract_bf16_backward(const Target& t, uint32_t par
     // workgroups that form dG and dU, then those that copy: at most 8192 of each
     auto groups = [](uint64_t pieces) { return pieces < 8192 * 256ull ? ceil_div(pieces, 256) : 8192; };
     const uint64_t copies = ((copy_x ? m : 0) + (copy_w ? 2 * n : 0)) * (ldk / 8);
-    Launch& l = p.add("tiler_gated_bf16_grad", (uint32_t)(groups(m * (ld / 8)) + groups(copies)), 1, 256)
-                    .ptr(gate).ptr(up).ptr(dh).ptr(x).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).ptr(dg);
+    const uint32_t forming = (uint32_t)groups(m * (ld / 8));
+    Launch& l = p.add("tiler_gated_bf16_grad", forming + (uint32_t)groups(copies), 1, 256)
+                    .ptr(gate).ptr(up).ptr(dh).ptr(x).ptr(wg).ptr(wu).u32(m32).u32(n32).u32(k32).u32(forming).ptr(dg);
     slot_or_null(l, copy_x, to_x);
     slot_or_null(l, copy_w, to_w);
   }

@@ -21,7 +21,7 @@
 namespace tiler_rt {
 
 constexpr uint32_t kMaxKernargBytes = 256;
-constexpr uint32_t kMaxArgs = 12;
+constexpr uint32_t kMaxArgs = 13;
 constexpr uint32_t kMaxBindings = 18;
 constexpr uint32_t kMaxSlots = 18;
 // Pointwise expressions: at most this many distinct inputs (one pointer each
