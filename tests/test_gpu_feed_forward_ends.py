@@ -1,4 +1,6 @@
-"""The feed-forward sublayer's calls at the ends of their ranges."""
+"""The feed-forward sublayer's calls at the ends of their ranges: rows far from
+zero, far gates, values that are not finite, empty rows, very many and very
+long rows."""
 from __future__ import annotations
 
 import numpy as np
@@ -9,7 +11,7 @@ from tiler_amd import _lib as L
 from tiler_amd import families
 from tiler_amd.realize import realize, route
 from tiler_amd.runtime import Refusal
-from test_gpu_layer_norm import Buffers, backward, forward, kept, rows_of, within
+from test_gpu_layer_norm import CODE, Buffers, backward, forward, kept, rows_of, within
 
 pytestmark = pytest.mark.gpu
 
@@ -263,3 +265,124 @@ def test_slopes_of_far_gates(ctx, mem):
     terms = np.abs(d * u * s) * (1 + np.abs(g) * t)
     within(w64(mem.get(dwu, np.uint16, (1, n))), want_u, gate_bound(want_u, g), "dU")
     within(w64(mem.get(dwg, np.uint16, (1, n))), want_g, gate_bound(want_g, g, terms), "dG")
+
+
+# -- very many short rows -------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_more_rows_than_workgroups(ctx, mem, dtype):
+    """Streamed rows past the 2^20 workgroups of a launch: each takes further rows."""
+    rows, extent = (1 << 20) + 5, 3
+    for program, variant, symbol in ((L.PROGRAM_LAYER_NORM, L.NORM_STATISTICS, "tiler_layer_norm_%s_s"),
+                                     (L.PROGRAM_LAYER_NORM_BACKWARD, L.NORM_DX, "tiler_layer_norm_grad_%s_s"),
+                                     (L.PROGRAM_QUANTIZE_ROWS_I8, 0, "tiler_quantize_rows_i8_%s_s")):
+        rz = realize(program, (rows, extent), dtype=CODE[dtype], variant=variant, scalars=(ref.EPS_BITS, 0),
+                     permissions=L.PERMITS_REASSOCIATION)
+        assert rz.symbols == [symbol % dtype] and rz.dispatches[0].grid[0] < rows
+    rng = np.random.default_rng(3)
+    x, dy = rows_of(rng, rows, extent, dtype), ref.store(dtype, rng.standard_normal((rows, extent)))
+    args = (ref.wide(dtype, x), None, None)
+    y, mean, rstd = forward(ctx, mem, dtype, x, None, None)
+    for got, want, bound in zip((ref.wide(dtype, y), mean, rstd), ref.layer_norm(*args), ref.layer_norm_bounds(dtype, *args)):
+        within(got, want, bound, "forward")
+    back = (ref.wide(dtype, dy), args[0], None, mean.astype(np.float64), rstd.astype(np.float64))
+    dx, _, _ = backward(ctx, mem, dtype, dy, x, None, mean, rstd, want=(True, False, False))
+    within(ref.wide(dtype, dx), ref.layer_norm_backward(*back)[0], ref.layer_norm_backward_bounds(dtype, *back)[0], "dx")
+    q, s = mem.out(np.int8, rows * extent), mem.out(np.float32, rows)
+    ctx.quantize_rows_i8(CODE[dtype], mem.put(x), rows, extent, q, s)
+    ctx.synchronize()
+    codes, scales = ref.quantize_rows(ref.wide(dtype, x))
+    assert np.array_equal(mem.get(q, np.int8, codes.shape), codes) and np.array_equal(mem.get(s, np.float32, (rows,)), scales)
+
+
+# -- values that are not finite -----------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("extent", [5, 100, 1023, 4096, 8190, 20001])
+def test_norm_of_poisoned_rows(ctx, mem, dtype, extent):
+    """A NaN or an infinity takes its own row, and no other."""
+    rng = np.random.default_rng(extent)
+    v = ref.wide(dtype, rows_of(rng, 9, extent, dtype))
+    v[2, extent - 1], v[4, 0], v[7, extent // 2] = np.nan, np.inf, -np.inf
+    x, bad = ref.store(dtype, v), [2, 4, 7]
+    good = np.delete(np.arange(9), bad)
+    y, mean, rstd = forward(ctx, mem, dtype, x, None, None)
+    assert np.isnan(ref.wide(dtype, y)[bad]).all() and np.isnan(rstd[bad]).all() and not np.isfinite(mean[bad]).any()
+    args = (v[good], None, None)
+    within(ref.wide(dtype, y)[good], ref.layer_norm(*args)[0], ref.layer_norm_bounds(dtype, *args)[0], "y")
+    # the gradients: NaN in those rows of dx and, as a sum over the rows, all over dw; db is dy's alone
+    dy = ref.store(dtype, rng.standard_normal((9, extent)))
+    dx, dw, db = (ref.wide(dtype, t) for t in backward(ctx, mem, dtype, dy, x, None, mean, rstd))
+    assert np.isnan(dx[bad]).all() and np.isnan(dw).all()
+    back = (ref.wide(dtype, dy)[good], v[good], None, mean[good].astype(np.float64), rstd[good].astype(np.float64))
+    within(dx[good], ref.layer_norm_backward(*back)[0], ref.layer_norm_backward_bounds(dtype, *back)[0], "dx")
+    wide_dy = ref.wide(dtype, dy)
+    e = 700 * U * np.abs(wide_dy).sum(0)
+    within(db, wide_dy.sum(0), e + ref.half(dtype) * (np.abs(wide_dy.sum(0)) + e), "db")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("extent", [5, 100, 1023, 4096, 8190, 20001])
+def test_poisoned_gradients_of_the_norm(ctx, mem, dtype, extent):
+    """A NaN or an infinity in dy takes its row of dx and its column of dw and db (dx of
+    the infinite row: both row means are infinite, so NaN or an infinity by the signs
+    of xh)."""
+    rng = np.random.default_rng(extent + 1)
+    x, v = rows_of(rng, 300, extent, dtype), ref.wide(dtype, ref.store(dtype, rng.standard_normal((300, extent))))
+    v[3, 0], v[299, extent - 1] = np.inf, np.nan
+    dy, (mean, rstd) = ref.store(dtype, v), kept(dtype, x)
+    dx, dw, db = (ref.wide(dtype, t) for t in backward(ctx, mem, dtype, dy, x, None, mean, rstd))
+    rows = np.zeros(300, bool)
+    rows[[3, 299]] = True
+    cols = np.zeros(extent, bool)
+    cols[[0, extent - 1]] = True
+    assert np.isnan(dx[299]).all() and not np.isfinite(dx[rows]).any() and np.isfinite(dx[~rows]).all()
+    for t in (dw, db):
+        assert not np.isfinite(t[cols]).any() and np.isfinite(t[~cols]).all()
+
+
+# a form of each kind: few tiles and many, whole and split depths, copied operands
+@pytest.mark.parametrize("m,n,k", [(40, 72, 72), (130, 136, 203), (520, 264, 264), (1500, 264, 1000), (2050, 2056, 2056)])
+def test_poisoned_gradients_of_the_gated_product(ctx, mem, m, n, k):
+    """In dh a NaN or an infinity takes a token's row of dx, a channel's row of dWg and
+    dWu; in x a column of both; in a weight a column of dx: nothing else."""
+    rng = np.random.default_rng(m)
+
+    def grads(poison):
+        v = {"x": (m, k), "wg": (n, k), "wu": (n, k), "gate": (m, n), "up": (m, n), "dh": (m, n)}
+        v = {name: w64(bf(rng.standard_normal(s))) for name, s in v.items()}
+        for name, at, value in poison:
+            v[name][at] = value
+        dx, dwg, dwu = mem.out(np.uint16, m * k), mem.out(np.uint16, n * k), mem.out(np.uint16, n * k)
+        ctx.gated_contract_bf16_backward(*(mem.put(bf(t)) for t in v.values()), m, n, k, dx, dwg, dwu)
+        ctx.synchronize()
+        return [w64(mem.get(t, np.uint16, s)) for t, s in ((dx, (m, k)), (dwg, (n, k)), (dwu, (n, k)))]
+
+    def only(t, rows=(), cols=()):
+        bad = np.zeros(t.shape, bool)
+        bad[list(rows)] = True
+        bad[:, list(cols)] = True
+        assert not np.isfinite(t[bad]).any() and np.isfinite(t[~bad]).all(), (np.argwhere(np.isfinite(t) == bad)[:4])
+
+    dx, dwg, dwu = grads([("dh", (m - 1, 0), np.nan), ("dh", (3, n - 1), np.inf)])
+    only(dx, rows=(3, m - 1)), only(dwg, rows=(0, n - 1)), only(dwu, rows=(0, n - 1))
+    dx, dwg, dwu = grads([("x", (m - 1, k - 1), np.inf), ("x", (0, 0), np.nan)])
+    only(dx), only(dwg, cols=(0, k - 1)), only(dwu, cols=(0, k - 1))
+    dx, dwg, dwu = grads([("wg", (n - 1, k - 1), np.nan), ("wu", (0, 1), -np.inf)])
+    only(dx, cols=(1, k - 1)), only(dwg), only(dwu)
+
+
+# -- calls that meet nothing, routed --------------------------------------------------
+
+def test_routed_without_tokens(ctx, mem):
+    """No token or no channel, through the recognizer: zeros, as the direct call."""
+    k = 40
+    for m, n in ((0, 72), (20, 0)):
+        rz = realize(L.PROGRAM_GATED_CONTRACTION_BACKWARD, (m, n, k), dtype=L.BF16, variant=L.GATED_DX | L.GATED_DW,
+                     permissions=L.PERMITS_REASSOCIATION)
+        some = mem.put(np.zeros(64, np.uint16))
+        outs = [mem.out(np.uint16, c) for c in (m * k, n * k, n * k)]
+        storage = iter([some] * 6 + outs)
+        route(ctx, rz, [None if role == L.SLOT_SCRATCH else int(next(storage).ptr) for role, _ in rz.slots])
+        for v, c in zip(outs, (m * k, n * k, n * k)):
+            assert (mem.get(v, np.uint16, (c,)) == 0).all()
