@@ -788,8 +788,11 @@ tiler_hip_status tiler_hip_contract(tiler_hip_context *ctx, uint32_t dtype,
  * neither) receive mu and r for the gradients; rows without elements have
  * none and are refused with them.  eps positive and finite; rows up to
  * 2^32 - 1 elements.  The variance is that of the differences from the
- * mean, never a difference of squares.  A row holding a NaN or an infinity
- * gives NaNs. */
+ * mean, never a difference of squares, and the binary32 mean's rounding is
+ * taken off the differences again (f32, and bf16 rows whose sum is exact in
+ * binary32).  A row holding a NaN or an infinity gives NaNs.  A finite row whose
+ * sum, or whose sum of squared differences, passes binary32's range is not
+ * normalized (NaNs, or r = 0). */
 tiler_hip_status tiler_hip_layer_norm(tiler_hip_context *ctx, uint32_t dtype, const void *x,
                                       const void *w, const void *b, uint64_t rows, uint64_t extent,
                                       uint32_t eps_bits, void *y, float *mean, float *rstd,
@@ -812,8 +815,9 @@ tiler_hip_status tiler_hip_layer_norm_backward_workspace(const tiler_hip_context
 /* The gated feed-forward product, bf16 operands and results, f32 sums:
  *   G = x Wg^T, U = x Wu^T, h = silu(G) * U
  * x [m, k], wg and wu [n, k] (td,od->to), h [m, n].  h comes from the f32 sums,
- * rounded once.  gate and up (bf16 [m, n], both or neither) receive G and U
- * for the gradients.  k at least 1, below 2^24; m up to 65535 * 128. */
+ * rounded once; its relative error before that grows as |G| 2^-23, and silu(G)
+ * is zero below G = -174.7.  gate and up (bf16 [m, n], both or neither) receive
+ * G and U for the gradients.  k at least 1, below 2^24; m up to 65535 * 128. */
 tiler_hip_status tiler_hip_gated_contract_bf16(tiler_hip_context *ctx, const uint16_t *x,
                                                const uint16_t *wg, const uint16_t *wu, uint64_t m,
                                                uint64_t n, uint64_t k, uint16_t *h, uint16_t *gate,
@@ -843,8 +847,8 @@ tiler_hip_status tiler_hip_quantize_rows_i8(tiler_hip_context *ctx, uint32_t dty
                                             tiler_hip_stream stream);
 /* Contraction td,od->to of int8 operands with a scale per row of each:
  *   c[i, j] = fl(fl(fl(sum_k a_ik b_jk) a_scales[i]) b_scales[j])
- * The sum is an exact integer (k at most 131071, any codes), fl rounds to
- * binary32; dtype TILER_HIP_F32, or TILER_HIP_BF16 for one more narrowing.
+ * The sum is an exact integer (k from 1 to 131071, any codes; m up to
+ * 65535 * 128), fl rounds to binary32; dtype TILER_HIP_F32, or TILER_HIP_BF16 for one more narrowing.
  * a [m, k], b [n, k], a_scales [m], b_scales [n], c [m, n]. */
 tiler_hip_status tiler_hip_contract_i8(tiler_hip_context *ctx, const int8_t *a, const int8_t *b,
                                        const float *a_scales, const float *b_scales, uint64_t m,

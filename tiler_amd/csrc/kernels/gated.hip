@@ -17,10 +17,11 @@
 // weights as they lie (the weights' rows are its depth) and dWg, dWu with x
 // over the tokens (both operands in column layout).
 //
-// us, 4096 x 14336 x 4096: forward with G and U kept 735 (1.3 PFLOP/s: the matrix
-// pipe under the card's power limit, as a plain library product of the size), dG
-// and dU 98 (587 MB, 6 TB/s), dx 710, the weights' gradients 710.  16 tokens 45:
-// the weights' 235 MB.
+// us, 4096 x 14336 x 4096, by the card: forward with G and U kept 750 .. 767 (1.26
+// .. 1.28 PFLOP/s: the matrix pipe under the power limit, as a plain library product
+// of the size), its gradients 1515 .. 1552, of them dG and dU 96 (587 MB, 6 TB/s),
+// dx and the weights' gradients half the rest each.  16 tokens 45: the weights'
+// 235 MB.
 #include "product.h"
 
 namespace {

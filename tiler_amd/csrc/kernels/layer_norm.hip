@@ -8,8 +8,10 @@
 // Memory bounds all of it, so a row is read once and held in registers between
 // its sums and its results, and the gradients' workgroups keep dw's and db's sums
 // over their rows in registers.  us, and a copy of the same bytes: 8192 x 4096
-// bf16 with statistics 26 / 26, its gradients 46 and 4.6 for the partials' sum /
-// 39; 16 x 4096, a launch, 6; gradients of 1237 x 1023 f32 6.9 and 4.2 / 3.
+// bf16 with statistics 27 / 26, its gradients 46 and 4.6 for the partials' sum /
+// 39; the same in f32 48 / 52 and 79 / 78; 16 x 4096, a launch, 6; gradients of
+// 1237 x 1023 f32 6.9 and 4.2 / 3.  Gradients of rows longer than registers hold
+// read dy and x twice, an element a load: 4096 x 12288 f32 341 / 117.
 #include "row_pieces.h"
 
 namespace {
@@ -102,9 +104,9 @@ __device__ __forceinline__ void layer_norm_grad_stream(const T* __restrict__ dy,
 // differences too, in the FMA that scales them.  f32 rows: the mean of the
 // differences.  bf16 rows: the remainder of the division; their sum is all but
 // exact (8 bits a value, where the values are of one size) and the sum of the
-// differences would cost a tenth of the kernel.  With a row 10^5 deviations from
-// zero y is off by 1e-6 of a deviation, by 1e-2 with the mean alone; 8192 x 4096
-// bf16 27.2 us, with the mean alone 27.05.
+// differences would cost a tenth of the kernel.  Of f32 rows 10^5 deviations
+// from zero y is off by 5e-7, by 1e-2 with the mean alone; 8192 x 4096 bf16 27.2
+// us, with the mean alone 27.05.
 template <typename T, int WAVES, int CH>
 __device__ __forceinline__ void layer_norm_rows(const T* __restrict__ x, const T* __restrict__ w,
                                                 const T* __restrict__ b, uint64_t rows, uint32_t extent, float eps,
@@ -284,7 +286,7 @@ __device__ __forceinline__ void layer_norm_grad_rows(const T* __restrict__ dy, c
       // dx = r g - (xh (r c2) + r c1), xh kept where the registers hold it (8192 x
       // 4096 bf16 48.7 us, formed again 50.0).  As an FMA of x with mu in the constant
       // (49.3) the row's distance from zero would round into dx: f32 rows 10^5
-      // deviations from zero 4e-4 of the largest dx instead of 1e-7; and r^2 leaves
+      // deviations from zero 4e-4 of the largest dx instead of 5e-8; and r^2 leaves
       // binary32 where a row's deviation is below 10^-19.
       const float c1 = s1 / (float)extent, c2 = s2 / (float)extent, a = -(r * c2), z = -(r * c1);
       if (row < rows) {

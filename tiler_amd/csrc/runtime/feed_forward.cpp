@@ -136,7 +136,8 @@ tiler_hip_status plan_layer_norm_backward(const Target& t, uint32_t dtype, uint3
   if (rows && extent >= vec && pieces <= 2048) {
     // Rows in registers, 8 / WAVES of them (or one of 16 waves) per workgroup at
     // a time, at most as many workgroups as run at once, so that there are few
-    // partials.
+    // partials.  Longer rows are streamed: 4096 x 12288 f32 341 us, 2048 x 18432
+    // bf16 226.
     const uint64_t groups = waves == 16 ? rows : ceil_div(rows, 8 / waves);
     const uint64_t most = (waves == 16 ? 1ull : 2ull) * t.compute_units;
     count = groups < most ? groups : most;
@@ -200,7 +201,9 @@ bool staged_rows(uint64_t row_bytes) { return row_bytes % 16 == 0 && row_bytes *
 //                                     c0 + q (c1 + c2 t) + c3 t + c4 t max(W / CUs, 1)
 // The constants are least squares fits of measured times (m 1 .. 4096, n 600 ..
 // 28672, k 800 .. 8192, at most 3000 workgroups): the form of the least estimate
-// is 1% slower than the fastest in the mean.
+// is 1% slower than the fastest in the mean.  Beyond those sizes they go on in
+// rounds and slices as they are (int8 k = 14336 with its rows' quantization: 16 x
+// 4096 14.7 us, 4.0 TB/s; 4096 x 4096 215, 2.2 P operations/s).
 struct ProductForm {
   const char* name;
   uint32_t rows, cols, threads;
@@ -209,7 +212,7 @@ struct ProductForm {
 };
 
 // us, by size: 16 x 14336 x 4096 few1x1 45, t64_d 100; 301 of them t160_w 80, t192 90,
-// t128 124; 4096 of them t256 740, t128 830; 512 x 4096 x 4096 t128_d 39, t256_n 52.
+// t128 124; 4096 of them t256 740 (750 .. 767 on other cards), t128 830; 512 x 4096 x 4096 t128_d 39, t256_n 52.
 constexpr ProductForm kGatedForms[] = {
     {"few1x1", 16, 16, 512, ProductForm::kFew, {2.591, 0.235, 0.356, 0.131, 0.151}},
     {"few2x1", 32, 16, 512, ProductForm::kFew, {2.524, 0.481, 0.610, 0, 0.115}},
