@@ -856,6 +856,163 @@ tiler_hip_status tiler_hip_contract_i8(tiler_hip_context *ctx, const int8_t *a, 
                                        tiler_hip_stream stream);
 
 /* ------------------------------------------------------------------------
+ * The attention sublayer of a language model, for serving (and, for the head
+ * norms with the rotation, for training).  The reference has no cache, no
+ * rotation and no masked attention.  A batch is `tokens` rows, the new tokens of
+ * `sequences` sequences one after another: sequence s has the rows starts[s] up
+ * to starts[s + 1].  Rows behind starts[sequences] pad the batch (to a captured
+ * graph's size, say) and belong to none.
+ *
+ * A serving step calls, on one stream,
+ *   tiler_hip_page_slots            where each new token goes
+ *   tiler_hip_norm_rotate           queries and keys normed and rotated, keys and
+ *                                   values stored there
+ *   tiler_hip_paged_attention_bf16  the new tokens' attention over the cache
+ * Every call is deterministic, launches on `stream` and may be captured into a
+ * graph; lengths and tables are read on the device, so that a graph replays with
+ * other ones.  Workspaces as for the feed-forward sublayer.  Outputs overlap
+ * neither the inputs nor one another, except that a cache is updated in place. */
+
+/* A cache of keys and values in pages of `page` tokens each: token t of page n,
+ * head h starts at element n * page_stride + t * token_stride + h * head_stride
+ * of k and of v (bf16, head_dim elements).  Slot n * page + t names the token; at
+ * most 2^31 - 1 slots.  Any strides under which no two rows overlap: [pages, page,
+ * heads, head_dim] and [pages, heads, page, head_dim] are the usual ones. */
+typedef struct {
+    void *k;
+    void *v;
+    uint64_t pages;
+    uint32_t page;
+    uint32_t heads;        /* key/value heads */
+    uint32_t head_dim;
+    uint32_t reserved;     /* 0 */
+    uint64_t page_stride;  /* elements */
+    uint64_t token_stride;
+    uint64_t head_stride;
+} tiler_hip_paged_cache;
+
+/* Page tables, positions and slots of a batch's new tokens.  Sequence s holds
+ * kept[s] tokens and gets fresh[s] more (below zero reads as zero); its row of
+ * `table` [sequences, table_width] names the pages of the kept ones.  The pages
+ * that the new ones open are taken from free_pages in order, sequence by sequence,
+ * and entered into the table (-1 for pages past the list's end; none beyond
+ * table_width); its other entries are left.
+ *   starts [sequences + 1]  first row of each sequence, and the rows of all
+ *   lengths [sequences]     kept + fresh
+ *   positions [tokens]      of each row's token in its sequence
+ *   slots [tokens]          page * table[s][position / page] + position % page; -1
+ *                           for a token without a page
+ *   taken [1]               pages wanted of the list (more than free_count: the
+ *                           last ones were not there)
+ * Rows behind the last sequence get position 0 and slot -1.  `tokens` is at least
+ * the sum of fresh: tokens past it get no row and the pages that they open no
+ * entry.  Results past 2^31 - 1 saturate (a slot becomes -1). */
+tiler_hip_status tiler_hip_page_slots(tiler_hip_context *ctx, const int32_t *kept, const int32_t *fresh,
+                                      uint64_t sequences, uint64_t page, const int32_t *free_pages,
+                                      uint64_t free_count, int32_t *table, uint64_t table_width,
+                                      uint64_t tokens, int32_t *starts, int32_t *lengths,
+                                      int32_t *positions, int32_t *slots, int32_t *taken,
+                                      tiler_hip_stream stream);
+
+/* Rows of heads: a token's q_heads query heads lie one after another, and its
+ * kv_heads key (and value) heads; each operand has a stride of its own from token
+ * to token (elements), so that the three may be slices of one projection. */
+typedef struct {
+    uint64_t tokens;
+    uint32_t q_heads;       /* either may be 0: queries or keys alone */
+    uint32_t kv_heads;
+    uint32_t head_dim;      /* 1 .. 1024 */
+    uint32_t rotary;        /* elements of a head that are rotated, its first ones: even, 0 .. head_dim */
+    uint32_t pairing;       /* TILER_HIP_ROTATE_HALVES or _NEIGHBOURS */
+    uint32_t eps_bits;      /* of the norm; 0: no norm (and no weights) */
+    uint64_t q_stride;      /* of q (and dq) */
+    uint64_t k_stride;      /* of k (and dk) */
+    uint64_t v_stride;
+    uint64_t q_out_stride;  /* of q_out (and dq_out) */
+    uint64_t k_out_stride;  /* of k_out (and dk_out) */
+    uint64_t reserved;      /* 0 */
+} tiler_hip_head_layout;
+#define TILER_HIP_ROTATE_HALVES 0u     /* pair p is elements p and p + rotary / 2 */
+#define TILER_HIP_ROTATE_NEIGHBOURS 1u /* pair p is elements 2 p and 2 p + 1 */
+
+/* The norm of each query and key head with the position rotation, in one pass:
+ *   u = x w / sqrt(mean(x^2) + eps)
+ *   y_i = u_i cos a - u_j sin a, y_j = u_j cos a + u_i sin a   for each pair (i, j)
+ * with a = positions[token] * frequencies[pair], a product in 64 bits (frequencies
+ * are f64 [rotary / 2], radians a position), cos and sin to binary32; elements
+ * behind `rotary` are u.  dtype TILER_HIP_F32 or TILER_HIP_BF16 (binary32
+ * arithmetic on exactly widened operands, one narrowing of y).  wq and wk [head_dim]
+ * or NULL (ones).  A head whose sum of squares passes binary32's range is not
+ * normed (zeros); a NaN or an infinity in a head gives NaNs there.
+ * The queries go to q_out; the keys to k_out, and with a cache (bf16) the keys and
+ * the values of v to the slots that slots[token] names: a slot outside the cache
+ * (-1) stores nothing, two tokens with one slot leave either.  v, cache and slots
+ * go together; k_out may be NULL with them. */
+tiler_hip_status tiler_hip_norm_rotate(tiler_hip_context *ctx, uint32_t dtype,
+                                       const tiler_hip_head_layout *heads, const void *q, const void *k,
+                                       const void *v, const void *wq, const void *wk,
+                                       const int32_t *positions, const double *frequencies, void *q_out,
+                                       void *k_out, const tiler_hip_paged_cache *cache,
+                                       const int32_t *slots, tiler_hip_stream stream);
+/* Its gradients, with g = dy turned back, r = 1 / sqrt(mean(x^2) + eps), xh = x r:
+ *   dx = r (g w - xh mean(g w xh)), dw = sum over tokens and heads of g xh
+ * (dx = g without a norm).  Any of dq, dk, dwq and dwk may be NULL (not wanted);
+ * q and k are read where there is a norm.  Without tokens dwq and dwk are zeros.
+ * Sums in binary32, in a fixed order. */
+tiler_hip_status tiler_hip_norm_rotate_backward(tiler_hip_context *ctx, uint32_t dtype,
+                                                const tiler_hip_head_layout *heads, const void *dq_out,
+                                                const void *dk_out, const void *q, const void *k,
+                                                const void *wq, const void *wk, const int32_t *positions,
+                                                const double *frequencies, void *dq, void *dk, void *dwq,
+                                                void *dwk, void *workspace, uint64_t workspace_bytes,
+                                                tiler_hip_stream stream);
+tiler_hip_status tiler_hip_norm_rotate_backward_workspace(const tiler_hip_context *ctx, uint32_t dtype,
+                                                          const tiler_hip_head_layout *heads,
+                                                          uint64_t *bytes);
+
+typedef struct {
+    uint64_t tokens;
+    uint64_t sequences;
+    uint32_t q_heads;       /* a multiple of the cache's heads: q head n reads key/value head n / (q_heads / heads) */
+    float scale;            /* of the logits; positive and finite */
+    uint64_t q_stride;      /* from token to token of q and of out, elements; heads one after another */
+    uint64_t out_stride;
+    uint64_t table_width;   /* pages a row of the table */
+    uint32_t window;        /* keys a query sees, its own among them; 0: all before it */
+    uint32_t sinks;         /* first tokens of a sequence that stay visible under a window */
+    uint64_t max_fresh;     /* the most new tokens of a sequence, and the most tokens of one with them: */
+    uint64_t max_length;    /* what the work is cut by (0: unknown); results do not depend on their being right */
+    uint64_t reserved;      /* 0 */
+} tiler_hip_attention_shape;
+
+/* Attention of the new tokens over the paged cache, in which they are stored
+ * already.  Row i of sequence s has position p = lengths[s] - (starts[s + 1] -
+ * starts[s]) + i and sees the keys j <= p with j > p - window (or window 0) or
+ * j < sinks:
+ *   out = sum_j e^(scale q k_j) v_j / sum_j e^(scale q k_j)
+ * q, out bf16 [tokens, q_heads, head_dim]; sums, maxima and the softmax in binary32,
+ * its weights rounded to bf16 for the product with v.  Token j of sequence s lies
+ * in page table[s][j / page]; an entry that names no page of the cache reads as
+ * zeros, and keys past the table's width are not seen.  A row that sees no key, or
+ * none with a logit above -infinity, is zeros.  Rows behind starts[sequences] are
+ * left as they are.  A NaN or an infinity in a key or value reaches the rows that
+ * see it; in a value also rows of its sequence that share a tile with one of those
+ * (no row reads what none of its tile's sees).  starts and lengths out of order or
+ * range touch nothing outside the operands.
+ * head_dim a multiple of 8 up to 256; the cache's rows start on 16 bytes
+ * (TILER_HIP_REFUSE_UNSUPPORTED else); q and out at any alignment. */
+tiler_hip_status tiler_hip_paged_attention_bf16(tiler_hip_context *ctx,
+                                                const tiler_hip_attention_shape *shape, const uint16_t *q,
+                                                const tiler_hip_paged_cache *cache, const int32_t *table,
+                                                const int32_t *starts, const int32_t *lengths,
+                                                uint16_t *out, void *workspace, uint64_t workspace_bytes,
+                                                tiler_hip_stream stream);
+tiler_hip_status tiler_hip_paged_attention_bf16_workspace(const tiler_hip_context *ctx,
+                                                          const tiler_hip_attention_shape *shape,
+                                                          const tiler_hip_paged_cache *cache,
+                                                          uint64_t *bytes);
+
+/* ------------------------------------------------------------------------
  * Realization recognizer: one scheduled region -> the dispatches that realize
  * it on this library's entry points.  It takes the role of tiler-metal's
  * emit_entry_point (tiler-metal/src/emit.rs:647-840) for a backend whose code
@@ -914,6 +1071,13 @@ tiler_hip_status tiler_hip_contract_i8(tiler_hip_context *ctx, const int8_t *a, 
 #define TILER_HIP_GATED_KEEP 1u
 #define TILER_HIP_GATED_DX 2u
 #define TILER_HIP_GATED_DW 4u
+#define TILER_HIP_ROTATE_WQ 1u
+#define TILER_HIP_ROTATE_WK 2u
+#define TILER_HIP_ROTATE_K_OUT 4u
+#define TILER_HIP_ROTATE_DQ 8u
+#define TILER_HIP_ROTATE_DK 16u
+#define TILER_HIP_ROTATE_DWQ 32u
+#define TILER_HIP_ROTATE_DWK 64u
 
 /* PROGRAM_FOLD variants.  The input is dense row-major with `rank` dims in
  * extents[]; grouping[0] is the reduced-axis mask (bit d: axis d reduced);

@@ -80,6 +80,15 @@ NORM_DB = 32
 GATED_KEEP = 1
 GATED_DX = 2
 GATED_DW = 4
+ROTATE_WQ = 1
+ROTATE_WK = 2
+ROTATE_K_OUT = 4
+ROTATE_DQ = 8
+ROTATE_DK = 16
+ROTATE_DWQ = 32
+ROTATE_DWK = 64
+ROTATE_HALVES = 0
+ROTATE_NEIGHBOURS = 1
 
 FOLD_SUM = 0
 FOLD_SQUARED = 1
@@ -234,6 +243,56 @@ class LiveExtent(ctypes.Structure):
         ("axis", ctypes.c_uint32),
         ("minimum", ctypes.c_uint64),
         ("bound", ctypes.c_uint64),
+    ]
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("pages", ctypes.c_uint64),
+        ("page", ctypes.c_uint32),
+        ("heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("page_stride", ctypes.c_uint64),
+        ("token_stride", ctypes.c_uint64),
+        ("head_stride", ctypes.c_uint64),
+    ]
+
+
+class HeadLayout(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_uint64),
+        ("q_heads", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("rotary", ctypes.c_uint32),
+        ("pairing", ctypes.c_uint32),
+        ("eps_bits", ctypes.c_uint32),
+        ("q_stride", ctypes.c_uint64),
+        ("k_stride", ctypes.c_uint64),
+        ("v_stride", ctypes.c_uint64),
+        ("q_out_stride", ctypes.c_uint64),
+        ("k_out_stride", ctypes.c_uint64),
+        ("reserved", ctypes.c_uint64),
+    ]
+
+
+class AttentionShape(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_uint64),
+        ("sequences", ctypes.c_uint64),
+        ("q_heads", ctypes.c_uint32),
+        ("scale", ctypes.c_float),
+        ("q_stride", ctypes.c_uint64),
+        ("out_stride", ctypes.c_uint64),
+        ("table_width", ctypes.c_uint64),
+        ("window", ctypes.c_uint32),
+        ("sinks", ctypes.c_uint32),
+        ("max_fresh", ctypes.c_uint64),
+        ("max_length", ctypes.c_uint64),
+        ("reserved", ctypes.c_uint64),
     ]
 
 
@@ -517,6 +576,16 @@ SIGNATURES = {
     "tiler_hip_gated_contract_bf16_backward": (_S, [_CTX, _P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _P,
                                                     _U64, _P]),
     "tiler_hip_gated_contract_bf16_backward_workspace": (_S, [_CTX, _U64, _U64, _U64, ctypes.POINTER(_U64)]),
+    "tiler_hip_page_slots": (_S, [_CTX, _P, _P, _U64, _U64, _P, _U64, _P, _U64, _U64, _P, _P, _P, _P, _P, _P]),
+    "tiler_hip_norm_rotate": (_S, [_CTX, _U32, ctypes.POINTER(HeadLayout), _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                   ctypes.POINTER(PagedCache), _P, _P]),
+    "tiler_hip_norm_rotate_backward": (_S, [_CTX, _U32, ctypes.POINTER(HeadLayout), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                            _P, _P, _P, _U64, _P]),
+    "tiler_hip_norm_rotate_backward_workspace": (_S, [_CTX, _U32, ctypes.POINTER(HeadLayout), ctypes.POINTER(_U64)]),
+    "tiler_hip_paged_attention_bf16": (_S, [_CTX, ctypes.POINTER(AttentionShape), _P, ctypes.POINTER(PagedCache), _P, _P, _P,
+                                            _P, _P, _U64, _P]),
+    "tiler_hip_paged_attention_bf16_workspace": (_S, [_CTX, ctypes.POINTER(AttentionShape), ctypes.POINTER(PagedCache),
+                                                      ctypes.POINTER(_U64)]),
     "tiler_hip_quantize_rows_i8": (_S, [_CTX, _U32, _P, _U64, _U64, _P, _P, _P]),
     "tiler_hip_contract_i8": (_S, [_CTX, _P, _P, _P, _P, _U64, _U64, _U64, _U32, _P, _P]),
     "tiler_hip_realize": (_S, [_CTX, ctypes.POINTER(Region), ctypes.POINTER(Realization),

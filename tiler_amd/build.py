@@ -77,6 +77,7 @@ def build(verbose: bool = False) -> str:
           os.path.join(CSRC, "runtime", "tiler_hip.cpp"),
           os.path.join(CSRC, "runtime", "program.cpp"),
           os.path.join(CSRC, "runtime", "feed_forward.cpp"),
+          os.path.join(CSRC, "runtime", "attention.cpp"),
           os.path.join(CSRC, "runtime", "digest.cpp"),
           os.path.join(CSRC, "runtime", "envelope.cpp"),
           os.path.join(CSRC, "runtime", "code_object.cpp"),

@@ -1,0 +1,342 @@
+// Planners of the attention sublayer's families: page tables and cache slots,
+// the head norms with the rotation and their gradients, attention over a paged
+// cache.
+#include "../kernels/attention.h"
+
+#include <cmath>
+#include <cstdio>
+
+#include "../kernels/head_rotate.h"
+#include "../kernels/page_slots.h"
+#include "program.h"
+
+namespace tiler_rt {
+
+namespace {
+
+uint64_t mul_sat(uint64_t a, uint64_t b) { return a && b > UINT64_MAX / a ? UINT64_MAX : a * b; }
+uint64_t add_sat(uint64_t a, uint64_t b) { return b > UINT64_MAX - a ? UINT64_MAX : a + b; }
+bool aligned16(uintptr_t a) { return (a & 15u) == 0; }
+uint64_t ceil_div(uint64_t a, uint64_t b) { return a / b + (a % b != 0); }
+constexpr uint64_t kMostPositions = 0x7fffffff;  // positions and slots are int32
+
+const char* type_name(uint32_t dtype) { return dtype == TILER_HIP_BF16 ? "bf16" : "f32"; }
+
+void slot_or_null(Launch& l, bool present, uint32_t slot) {
+  if (present) l.ptr(slot);
+  else l.null_ptr();
+}
+
+// Elements from the first to past the last of `rows` rows of `row` elements.
+uint64_t span(uint64_t rows, uint64_t stride, uint64_t row) {
+  return rows ? add_sat(mul_sat(rows - 1, stride), row) : 0;
+}
+
+TilerDivisor divisor_of(uint32_t d) {
+  TilerDivisor v{d, 1, 0};
+  while ((1ull << v.shift) < d) ++v.shift;
+  v.multiplier = (uint32_t)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+  return v;
+}
+
+// A cache's elements from the first to past the last, or a refusal.
+tiler_hip_status check_cache(const tiler_hip_paged_cache& c, Program& p, uint64_t& elements) {
+  if (c.reserved) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "paged cache: reserved is not 0");
+  if (c.page == 0 || c.heads == 0 || c.head_dim == 0)
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "paged cache: empty pages or heads");
+  if (mul_sat(c.pages, c.page) > kMostPositions)
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged cache: more than 2^31 - 1 tokens");
+  // no two rows overlap: each stride passes what the smaller ones span
+  struct Axis {
+    uint64_t count, stride;
+  } axes[3] = {{c.pages, c.page_stride}, {c.page, c.token_stride}, {c.heads, c.head_stride}};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (axes[j].count <= 1 ? false : axes[j + 1].count <= 1 || axes[j].stride > axes[j + 1].stride)
+        std::swap(axes[j], axes[j + 1]);
+  elements = c.head_dim;
+  for (const Axis& a : axes) {
+    if (a.count <= 1) continue;
+    if (a.stride < elements) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "paged cache: rows overlap");
+    elements = add_sat(mul_sat(a.count - 1, a.stride), elements);
+  }
+  if (elements > (1ull << 60)) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged cache: strides beyond 64-bit offsets");
+  if (c.pages == 0) elements = 0;
+  return TILER_HIP_OK;
+}
+
+tiler_hip_status check_heads(uint32_t dtype, uint32_t parts, const tiler_hip_head_layout& h, TilerHeads& k, Program& p) {
+  if (dtype != TILER_HIP_F32 && dtype != TILER_HIP_BF16)
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "norm_rotate dtype");
+  if (h.head_dim == 0) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "heads without elements");
+  if (h.head_dim > 1024) return p.refuse(TILER_HIP_REFUSE_CAPACITY, "heads of more than 1024 elements");
+  if (h.rotary > h.head_dim || h.rotary % 2)
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rotary: an even number of a head's elements");
+  if (h.pairing > TILER_HIP_ROTATE_NEIGHBOURS) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rotation pairing");
+  if (h.reserved) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "head layout: reserved is not 0");
+  float eps;
+  std::memcpy(&eps, &h.eps_bits, 4);
+  if (h.eps_bits && (!(eps > 0.0f) || !std::isfinite(eps)))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "eps must be positive and finite, or 0 for no norm");
+  if (!h.eps_bits && (parts & (TILER_HIP_ROTATE_WQ | TILER_HIP_ROTATE_WK | TILER_HIP_ROTATE_DWQ | TILER_HIP_ROTATE_DWK)))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "weights without a norm");
+  if (h.q_heads > (1u << 20) || h.kv_heads > (1u << 20))
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "more than 2^20 heads");
+  const uint64_t q_row = (uint64_t)h.q_heads * h.head_dim, k_row = (uint64_t)h.kv_heads * h.head_dim;
+  if (h.tokens > 1 && (h.q_stride < q_row || h.k_stride < k_row))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
+  if (h.tokens > (1ull << 40) || h.q_stride > (1ull << 40) || h.k_stride > (1ull << 40) || h.v_stride > (1ull << 40) ||
+      h.q_out_stride > (1ull << 40) || h.k_out_stride > (1ull << 40) ||
+      mul_sat(h.tokens, h.q_stride + h.k_stride + h.v_stride + h.q_out_stride + h.k_out_stride) > (1ull << 60))
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "rows of heads beyond 64-bit offsets");
+  k = TilerHeads{};
+  k.tokens = h.tokens;
+  k.q_heads = h.q_heads;
+  k.kv_heads = h.kv_heads;
+  k.head_dim = h.head_dim;
+  k.rotary = h.rotary;
+  k.neighbours = h.pairing == TILER_HIP_ROTATE_NEIGHBOURS;
+  k.norm = h.eps_bits != 0;
+  k.eps = eps;
+  k.q_stride = h.q_stride;
+  k.k_stride = h.k_stride;
+  k.v_stride = h.v_stride;
+  k.q_out_stride = h.q_out_stride;
+  k.k_out_stride = h.k_out_stride;
+  return TILER_HIP_OK;
+}
+
+}  // namespace
+
+// Slots: [kept, fresh,] [free,] [table,] starts, [lengths,] [positions, slots,]
+// taken: those of no elements have none.
+tiler_hip_status plan_page_slots(uint64_t sequences, uint64_t tokens, uint64_t page, uint64_t free_count,
+                                 uint64_t table_width, Program& p) {
+  if (page == 0) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "page_slots: pages without tokens");
+  if (page > kMostPositions || sequences >= kMostPositions || tokens > kMostPositions || free_count > kMostPositions ||
+      table_width > kMostPositions)
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "page_slots: counts of 2^31 and more");
+  const bool table = sequences && table_width;
+  const uint32_t kept = sequences ? p.slot(4 * sequences, kSlotInput) : 0;
+  const uint32_t fresh = sequences ? p.slot(4 * sequences, kSlotInput) : 0;
+  const uint32_t free = free_count ? p.slot(4 * free_count, kSlotInput) : 0;
+  const uint32_t at = table ? p.slot(4 * sequences * table_width, kSlotOutput) : 0;
+  const uint32_t starts = p.slot(4 * (sequences + 1), kSlotOutput);
+  const uint32_t lengths = sequences ? p.slot(4 * sequences, kSlotOutput) : 0;
+  const uint32_t positions = tokens ? p.slot(4 * tokens, kSlotOutput) : 0;
+  const uint32_t slots = tokens ? p.slot(4 * tokens, kSlotOutput) : 0;
+  const uint32_t taken = p.slot(4, kSlotOutput);
+  TilerPageSlots a{sequences, tokens, free_count, table ? table_width : 0, (uint32_t)page, 0};
+  const uint64_t groups = tokens ? ceil_div(tokens, 1024) : 1;
+  Launch& l = p.add("tiler_page_slots", (uint32_t)groups, 1, 1024).blob(&a, sizeof(a), 8);
+  slot_or_null(l, sequences, kept);
+  slot_or_null(l, sequences, fresh);
+  slot_or_null(l, free_count, free);
+  slot_or_null(l, table, at);
+  l.ptr(starts);
+  slot_or_null(l, sequences, lengths);
+  slot_or_null(l, tokens, positions);
+  slot_or_null(l, tokens, slots);
+  l.ptr(taken);
+  return TILER_HIP_OK;
+}
+
+// Slots: [q,] [k,] [v,] [wq,] [wk,] [positions, frequencies,] [q_out,] [k_out,]
+// [k_cache, v_cache, slots]: q and k where there are heads, positions and
+// frequencies where something is rotated.
+tiler_hip_status plan_norm_rotate(const Target& t, uint32_t dtype, uint32_t parts, const tiler_hip_head_layout& h,
+                                  const tiler_hip_paged_cache* cache, const uintptr_t*, Program& p) {
+  if (parts & ~(uint32_t)(TILER_HIP_ROTATE_WQ | TILER_HIP_ROTATE_WK | TILER_HIP_ROTATE_K_OUT))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "norm_rotate parts");
+  TilerHeads a;
+  if (tiler_hip_status st = check_heads(dtype, parts, h, a, p); st != TILER_HIP_OK) return st;
+  const bool has_q = h.q_heads, has_k = h.kv_heads, k_out = parts & TILER_HIP_ROTATE_K_OUT;
+  const uint64_t elem = dtype == TILER_HIP_BF16 ? 2 : 4;
+  const uint64_t q_row = (uint64_t)h.q_heads * h.head_dim, k_row = (uint64_t)h.kv_heads * h.head_dim;
+  if (h.tokens > 1 && (h.q_out_stride < q_row || (k_out && h.k_out_stride < k_row) || (cache && h.v_stride < k_row)))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
+  if (has_k && !k_out && !cache) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "the keys go nowhere");
+  uint64_t cached = 0;
+  if (cache) {
+    if (dtype != TILER_HIP_BF16) return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "the paged cache is bf16");
+    if (tiler_hip_status st = check_cache(*cache, p, cached); st != TILER_HIP_OK) return st;
+    if (cache->heads != h.kv_heads || cache->head_dim != h.head_dim)
+      return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "the cache has other heads");
+    a.page = cache->page;
+    a.slots = cache->pages * cache->page;
+    a.page_stride = cache->page_stride;
+    a.token_stride = cache->token_stride;
+    a.head_stride = cache->head_stride;
+  }
+  auto given = [&](bool there, uint64_t bytes, uint32_t role) { return there ? p.slot(bytes, role) : 0; };
+  const bool wq = parts & TILER_HIP_ROTATE_WQ, wk = parts & TILER_HIP_ROTATE_WK;
+  const uint32_t q = given(has_q, mul_sat(span(h.tokens, h.q_stride, q_row), elem), kSlotInput);
+  const uint32_t k = given(has_k, mul_sat(span(h.tokens, h.k_stride, k_row), elem), kSlotInput);
+  const uint32_t v = given(cache, mul_sat(span(h.tokens, h.v_stride, k_row), elem), kSlotInput);
+  const uint32_t at_wq = given(wq, elem * h.head_dim, kSlotInput), at_wk = given(wk, elem * h.head_dim, kSlotInput);
+  const uint32_t positions = given(h.rotary, mul_sat(h.tokens, 4), kSlotInput);
+  const uint32_t frequencies = given(h.rotary, 4ull * h.rotary, kSlotInput);
+  const uint32_t q_out = given(has_q, mul_sat(span(h.tokens, h.q_out_stride, q_row), elem), kSlotOutput);
+  const uint32_t to_k = given(k_out, mul_sat(span(h.tokens, h.k_out_stride, k_row), elem), kSlotOutput);
+  const uint32_t k_cache = given(cache, cached * 2, kSlotOutput), v_cache = given(cache, cached * 2, kSlotOutput);
+  const uint32_t slots = given(cache, mul_sat(h.tokens, 4), kSlotInput);
+  if (h.tokens == 0 || (!has_q && !has_k)) return TILER_HIP_OK;
+  const uint32_t groups = (uint32_t)(h.tokens < (1u << 20) ? h.tokens : 1u << 20);
+  char name[64];
+  std::snprintf(name, sizeof(name), "tiler_norm_rotate_%s_any", type_name(dtype));
+  Launch& l = p.add(name, groups, 1, 256).blob(&a, sizeof(a), 8);
+  slot_or_null(l, has_q, q);
+  slot_or_null(l, has_k, k);
+  slot_or_null(l, cache, v);
+  slot_or_null(l, wq, at_wq);
+  slot_or_null(l, wk, at_wk);
+  slot_or_null(l, h.rotary, positions);
+  slot_or_null(l, h.rotary, frequencies);
+  slot_or_null(l, has_q, q_out);
+  slot_or_null(l, k_out, to_k);
+  slot_or_null(l, cache, k_cache);
+  slot_or_null(l, cache, v_cache);
+  slot_or_null(l, cache, slots);
+  return TILER_HIP_OK;
+}
+
+// Slots: [dq_out,] [dk_out,] [q, k,] [wq,] [wk,] [positions, frequencies,] [dq,]
+// [dk,] [dwq,] [dwk,] [partials: scratch]: q and k where there is a norm.
+tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint32_t parts,
+                                           const tiler_hip_head_layout& h, const uintptr_t*, Program& p) {
+  const uint32_t known = TILER_HIP_ROTATE_WQ | TILER_HIP_ROTATE_WK | TILER_HIP_ROTATE_DQ | TILER_HIP_ROTATE_DK |
+                         TILER_HIP_ROTATE_DWQ | TILER_HIP_ROTATE_DWK;
+  if (parts & ~known) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "norm_rotate_backward parts");
+  TilerHeads a;
+  if (tiler_hip_status st = check_heads(dtype, parts, h, a, p); st != TILER_HIP_OK) return st;
+  const bool wq = parts & TILER_HIP_ROTATE_WQ, wk = parts & TILER_HIP_ROTATE_WK;
+  const bool dwq = parts & TILER_HIP_ROTATE_DWQ, dwk = parts & TILER_HIP_ROTATE_DWK;
+  const bool dq = (parts & TILER_HIP_ROTATE_DQ) && h.q_heads, dk = (parts & TILER_HIP_ROTATE_DK) && h.kv_heads;
+  const bool of_q = (dq || dwq) && h.q_heads, of_k = (dk || dwk) && h.kv_heads;
+  const uint64_t elem = dtype == TILER_HIP_BF16 ? 2 : 4;
+  const uint64_t q_row = (uint64_t)h.q_heads * h.head_dim, k_row = (uint64_t)h.kv_heads * h.head_dim;
+  if (h.tokens > 1 && ((of_q && h.q_out_stride < q_row) || (of_k && h.k_out_stride < k_row)))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
+  auto given = [&](bool there, uint64_t bytes, uint32_t role) { return there ? p.slot(bytes, role) : 0; };
+  const uint32_t dq_out = given(of_q, mul_sat(span(h.tokens, h.q_out_stride, q_row), elem), kSlotInput);
+  const uint32_t dk_out = given(of_k, mul_sat(span(h.tokens, h.k_out_stride, k_row), elem), kSlotInput);
+  const uint32_t q = given(of_q && a.norm, mul_sat(span(h.tokens, h.q_stride, q_row), elem), kSlotInput);
+  const uint32_t k = given(of_k && a.norm, mul_sat(span(h.tokens, h.k_stride, k_row), elem), kSlotInput);
+  const uint32_t at_wq = given(wq, elem * h.head_dim, kSlotInput), at_wk = given(wk, elem * h.head_dim, kSlotInput);
+  const uint32_t positions = given(h.rotary, mul_sat(h.tokens, 4), kSlotInput);
+  const uint32_t frequencies = given(h.rotary, 4ull * h.rotary, kSlotInput);
+  const uint32_t at_dq = given(dq, mul_sat(span(h.tokens, h.q_stride, q_row), elem), kSlotOutput);
+  const uint32_t at_dk = given(dk, mul_sat(span(h.tokens, h.k_stride, k_row), elem), kSlotOutput);
+  const uint32_t at_dwq = given(dwq, elem * h.head_dim, kSlotOutput), at_dwk = given(dwk, elem * h.head_dim, kSlotOutput);
+  char name[64];
+  const bool sum_q = of_q && dwq && h.tokens, sum_k = of_k && dwk && h.tokens;
+  uint32_t partials_q = 0, partials_k = 0;
+  // each workgroup leaves one row of partial sums
+  const uint64_t most = 2ull * t.compute_units;
+  const uint32_t count = (uint32_t)(h.tokens < most ? h.tokens : most);
+  if (sum_q) partials_q = p.slot(4ull * count * h.head_dim, kSlotScratch);
+  if (sum_k) partials_k = p.slot(4ull * count * h.head_dim, kSlotScratch);
+  if (h.tokens && (of_q || of_k)) {
+    std::snprintf(name, sizeof(name), "tiler_norm_rotate_grad_%s_any", type_name(dtype));
+    Launch& l = p.add(name, count, 2, 256).blob(&a, sizeof(a), 8);
+    slot_or_null(l, of_q, dq_out);
+    slot_or_null(l, of_k, dk_out);
+    slot_or_null(l, of_q && a.norm, q);
+    slot_or_null(l, of_k && a.norm, k);
+    slot_or_null(l, wq, at_wq);
+    slot_or_null(l, wk, at_wk);
+    slot_or_null(l, h.rotary, positions);
+    slot_or_null(l, h.rotary, frequencies);
+    slot_or_null(l, dq, at_dq);
+    slot_or_null(l, dk, at_dk);
+    slot_or_null(l, sum_q, partials_q);
+    slot_or_null(l, sum_k, partials_k);
+  }
+  if (dwq || dwk) {  // no tokens or no heads: zeros
+    std::snprintf(name, sizeof(name), "tiler_norm_rotate_sum_%s", type_name(dtype));
+    Launch& l = p.add(name, (uint32_t)ceil_div(h.head_dim, 64), 2, 1024);
+    slot_or_null(l, sum_q, partials_q);
+    slot_or_null(l, sum_k, partials_k);
+    l.u32(sum_q ? count : 0).u32(sum_k ? count : 0).u32(h.head_dim);
+    slot_or_null(l, dwq, at_dwq);
+    slot_or_null(l, dwk, at_dwk);
+  }
+  return TILER_HIP_OK;
+}
+
+// Slots: q, k, v, [table,] starts, lengths, out, [partial results, their maxima
+// and sums: scratch].
+tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_attention_shape& a,
+                                           const tiler_hip_paged_cache& cache, const uintptr_t* addr, Program& p) {
+  uint64_t cached = 0;
+  if (tiler_hip_status st = check_cache(cache, p, cached); st != TILER_HIP_OK) return st;
+  if (a.reserved) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "attention shape: reserved is not 0");
+  if (a.q_heads == 0 || a.q_heads % cache.heads)
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "query heads: a multiple of the cache's heads");
+  if (cache.head_dim % 8 || cache.head_dim > 256)
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "heads of 8 to 256 elements, a multiple of 8");
+  if (!(a.scale > 0.0f) || !std::isfinite(a.scale))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "scale must be positive and finite");
+  const uint64_t row = (uint64_t)a.q_heads * cache.head_dim;
+  if (a.tokens > 1 && (a.q_stride < row || a.out_stride < row))
+    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
+  if (a.sequences >= kMostPositions || mul_sat(a.tokens, a.q_heads) > kMostPositions ||
+      mul_sat(a.table_width, cache.page) > kMostPositions || a.q_stride > (1ull << 32) || a.out_stride > (1ull << 32))
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: counts of 2^31 and more");
+  const bool table = a.sequences && a.table_width;
+  const uint32_t q = p.slot(2 * span(a.tokens, a.q_stride, row), kSlotInput);
+  const uint32_t k = p.slot(2 * cached, kSlotInput), v = p.slot(2 * cached, kSlotInput);
+  const uint32_t at = table ? p.slot(4 * a.sequences * a.table_width, kSlotInput) : 0;
+  const uint32_t starts = p.slot(4 * (a.sequences + 1), kSlotInput), lengths = p.slot(4 * a.sequences, kSlotInput);
+  const uint32_t out = p.slot(2 * span(a.tokens, a.out_stride, row), kSlotOutput);
+  if (a.sequences == 0 || a.tokens == 0) return TILER_HIP_OK;
+  if ((cache.page_stride | cache.token_stride | cache.head_stride) % 8 || !aligned16(addr[k]) || !aligned16(addr[v]))
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "the cache's rows start on 16 bytes");
+  TilerAttentionShape s{};
+  s.tokens = (uint32_t)a.tokens;
+  s.sequences = (uint32_t)a.sequences;
+  s.kv_heads = cache.heads;
+  s.group = a.q_heads / cache.heads;
+  s.head_dim = cache.head_dim;
+  s.pages = (uint32_t)cache.pages;
+  s.width = (uint32_t)a.table_width;
+  s.window = a.window;
+  s.sinks = a.sinks;
+  s.scale = (float)((double)a.scale * 1.4426950408889634074);
+  s.page = divisor_of(cache.page);
+  s.groups = divisor_of(s.group);
+  s.q_stride = a.q_stride;
+  s.out_stride = a.out_stride;
+  s.page_stride = cache.page_stride;
+  s.token_stride = cache.token_stride;
+  s.head_stride = cache.head_stride;
+  const uint64_t room = a.table_width * cache.page;
+  uint64_t longest = a.max_length && a.max_length < room ? a.max_length : room;
+  if (a.window && longest > (uint64_t)a.window + a.sinks) longest = (uint64_t)a.window + a.sinks;
+  // split a sequence's keys where its workgroups would leave CUs idle, 512 keys at least to a part
+  const uint64_t alone = mul_sat(a.sequences, s.kv_heads);
+  uint64_t splits = ceil_div(2ull * t.compute_units, alone);
+  if (splits > ceil_div(longest, 512)) splits = ceil_div(longest, 512);
+  if (splits < 1) splits = 1;
+  s.splits = (uint32_t)splits;
+  if (mul_sat(alone, splits) > 0xffffffffull / 256)
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: more workgroups than a launch holds");
+  const uint64_t rows = a.tokens * a.q_heads;
+  const uint32_t part = splits > 1 ? p.slot(4 * mul_sat(rows * splits, s.head_dim), kSlotScratch) : 0;
+  const uint32_t ml = splits > 1 ? p.slot(8 * rows * splits, kSlotScratch) : 0;
+  char name[64];
+  std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_few%u", s.head_dim <= 64 ? 64 : s.head_dim <= 128 ? 128 : 256);
+  Launch& l = p.add(name, (uint32_t)(alone * splits), 1, 256).blob(&s, sizeof(s), 8).ptr(q).ptr(k).ptr(v);
+  slot_or_null(l, table, at);
+  l.ptr(starts).ptr(lengths).ptr(out);
+  slot_or_null(l, splits > 1, part);
+  slot_or_null(l, splits > 1, ml);
+  if (splits > 1) {
+    const uint64_t groups = ceil_div(rows, 4);
+    p.add("tiler_paged_attention_bf16_join", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
+        .blob(&s, sizeof(s), 8).ptr(starts).ptr(part).ptr(ml).ptr(out);
+  }
+  return TILER_HIP_OK;
+}
+
+}  // namespace tiler_rt

@@ -244,4 +244,15 @@ tiler_hip_status plan_quantize_rows_i8(const Target& t, uint32_t dtype, uint64_t
 tiler_hip_status plan_contract_i8(const Target& t, uint32_t out_dtype, uint64_t m, uint64_t n, uint64_t k,
                                   const uintptr_t* addr, Program& p);
 
+// The attention sublayer (attention.cpp).  `parts`: TILER_HIP_ROTATE_*, the
+// optional operands and results that are present.
+tiler_hip_status plan_page_slots(uint64_t sequences, uint64_t tokens, uint64_t page, uint64_t free_count,
+                                 uint64_t table_width, Program& p);
+tiler_hip_status plan_norm_rotate(const Target& t, uint32_t dtype, uint32_t parts, const tiler_hip_head_layout& h,
+                                  const tiler_hip_paged_cache* cache, const uintptr_t* addr, Program& p);
+tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint32_t parts,
+                                           const tiler_hip_head_layout& h, const uintptr_t* addr, Program& p);
+tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_attention_shape& a,
+                                           const tiler_hip_paged_cache& cache, const uintptr_t* addr, Program& p);
+
 }  // namespace tiler_rt

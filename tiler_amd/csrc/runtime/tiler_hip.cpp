@@ -402,6 +402,18 @@ const EntryRow kEntries[] = {
     TILER_INT8_FORM("t96_d"), TILER_INT8_FORM("t96"), TILER_INT8_FORM("t128"), TILER_INT8_FORM("t192"),
     TILER_INT8_FORM("t256"),
 #undef TILER_INT8_FORM
+    // the attention sublayer
+    {"tiler_page_slots", "page-slots", 9},
+    {"tiler_norm_rotate_bf16_any", "norm-rotate/bf16", 12},
+    {"tiler_norm_rotate_f32_any", "norm-rotate-f32", 12},
+    {"tiler_norm_rotate_grad_bf16_any", "norm-rotate-backward/bf16", 12},
+    {"tiler_norm_rotate_grad_f32_any", "norm-rotate-backward-f32", 12},
+    {"tiler_norm_rotate_sum_bf16", "norm-rotate-backward/bf16", 4},
+    {"tiler_norm_rotate_sum_f32", "norm-rotate-backward-f32", 4},
+    {"tiler_paged_attention_bf16_few64", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_few128", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_few256", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_join", "paged-attention-bf16", 4},
 };
 constexpr uint32_t kEntryCount = sizeof(kEntries) / sizeof(kEntries[0]);
 
@@ -2183,6 +2195,171 @@ tiler_hip_status tiler_hip_contract_i8(tiler_hip_context* ctx, const int8_t* a, 
   if (p.nlaunches && slots.missing)
     return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "a, b, a_scales, b_scales or c is NULL");
   return run_program(ctx, p, slots.at, pick(ctx, stream));
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+// ---------------------------------------------------------------------------
+// The attention sublayer.
+tiler_hip_status tiler_hip_page_slots(tiler_hip_context* ctx, const int32_t* kept, const int32_t* fresh,
+                                      uint64_t sequences, uint64_t page, const int32_t* free_pages, uint64_t free_count,
+                                      int32_t* table, uint64_t table_width, uint64_t tokens, int32_t* starts,
+                                      int32_t* lengths, int32_t* positions, int32_t* slots, int32_t* taken,
+                                      tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  SlotList list;
+  if (sequences) {
+    list.add(kept);
+    list.add(fresh);
+  }
+  if (free_count) list.add(free_pages);
+  if (sequences && table_width) list.add(table);
+  list.add(starts);
+  if (sequences) list.add(lengths);
+  if (tokens) {
+    list.add(positions);
+    list.add(slots);
+  }
+  list.add(taken);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_page_slots(sequences, tokens, page, free_count, table_width, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (list.missing) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "page_slots: an operand is NULL");
+  return run_program(ctx, p, list.at, pick(ctx, stream));
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_norm_rotate(tiler_hip_context* ctx, uint32_t dtype, const tiler_hip_head_layout* heads,
+                                       const void* q, const void* k, const void* v, const void* wq, const void* wk,
+                                       const int32_t* positions, const double* frequencies, void* q_out, void* k_out,
+                                       const tiler_hip_paged_cache* cache, const int32_t* slots,
+                                       tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  if (!heads) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "no head layout");
+  if (!v != !cache || !slots != !cache)
+    return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "v, cache and slots go together");
+  SlotList list;
+  if (heads->q_heads) list.add(q);
+  if (heads->kv_heads) list.add(k);
+  list.add_given(v);
+  list.add_given(wq);
+  list.add_given(wk);
+  if (heads->rotary) {
+    list.add(positions);
+    list.add(frequencies);
+  }
+  if (heads->q_heads) list.add(q_out);
+  list.add_given(k_out);
+  if (cache) {
+    list.add(cache->k);
+    list.add(cache->v);
+    list.add(slots);
+  }
+  const uint32_t parts = (wq ? TILER_HIP_ROTATE_WQ : 0u) | (wk ? TILER_HIP_ROTATE_WK : 0u) |
+                         (k_out ? TILER_HIP_ROTATE_K_OUT : 0u);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_norm_rotate(target_of(ctx), dtype, parts, *heads, cache, list.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (p.nlaunches && list.missing) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "norm_rotate: an operand is NULL");
+  return run_program(ctx, p, list.at, pick(ctx, stream));
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_norm_rotate_backward(tiler_hip_context* ctx, uint32_t dtype,
+                                                const tiler_hip_head_layout* heads, const void* dq_out,
+                                                const void* dk_out, const void* q, const void* k, const void* wq,
+                                                const void* wk, const int32_t* positions, const double* frequencies,
+                                                void* dq, void* dk, void* dwq, void* dwk, void* workspace,
+                                                uint64_t workspace_bytes, tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  if (!heads) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "no head layout");
+  // the planner's slots: what is wanted decides what is read
+  const bool of_q = (dq || dwq) && heads->q_heads, of_k = (dk || dwk) && heads->kv_heads;
+  SlotList list;
+  if (of_q) list.add(dq_out);
+  if (of_k) list.add(dk_out);
+  if (of_q && heads->eps_bits) list.add(q);
+  if (of_k && heads->eps_bits) list.add(k);
+  list.add_given(wq);
+  list.add_given(wk);
+  if (heads->rotary) {
+    list.add(positions);
+    list.add(frequencies);
+  }
+  if (heads->q_heads) list.add_given(dq);
+  if (heads->kv_heads) list.add_given(dk);
+  list.add_given(dwq);
+  list.add_given(dwk);
+  const uint32_t parts = (wq ? TILER_HIP_ROTATE_WQ : 0u) | (wk ? TILER_HIP_ROTATE_WK : 0u) |
+                         (dq ? TILER_HIP_ROTATE_DQ : 0u) | (dk ? TILER_HIP_ROTATE_DK : 0u) |
+                         (dwq ? TILER_HIP_ROTATE_DWQ : 0u) | (dwk ? TILER_HIP_ROTATE_DWK : 0u);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_norm_rotate_backward(target_of(ctx), dtype, parts, *heads, list.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (!p.nlaunches) return TILER_HIP_OK;
+  if (heads->tokens && list.missing)
+    return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "norm_rotate_backward: an operand is NULL");
+  hipStream_t s = pick(ctx, stream);
+  CallScratch scratch(ctx, s);
+  if ((st = bind_workspace(ctx, p, list, workspace, workspace_bytes, s, scratch)) != TILER_HIP_OK) return st;
+  return run_program(ctx, p, list.at, s);
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_norm_rotate_backward_workspace(const tiler_hip_context* ctx, uint32_t dtype,
+                                                          const tiler_hip_head_layout* heads, uint64_t* bytes) try {
+  if (!heads || !bytes) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  const uintptr_t addr[tiler_rt::kMaxSlots] = {};
+  tiler_rt::Program p;
+  const uint32_t sums = heads->eps_bits ? TILER_HIP_ROTATE_DWQ | TILER_HIP_ROTATE_DWK : 0u;
+  const tiler_hip_status st = tiler_rt::plan_norm_rotate_backward(
+      target_of(ctx), dtype, TILER_HIP_ROTATE_DQ | TILER_HIP_ROTATE_DK | sums, *heads, addr, p);
+  *bytes = st == TILER_HIP_OK ? workspace_need(p) : 0;
+  return st;
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_paged_attention_bf16(tiler_hip_context* ctx, const tiler_hip_attention_shape* shape,
+                                                const uint16_t* q, const tiler_hip_paged_cache* cache,
+                                                const int32_t* table, const int32_t* starts, const int32_t* lengths,
+                                                uint16_t* out, void* workspace, uint64_t workspace_bytes,
+                                                tiler_hip_stream stream) try {
+  if (!ctx) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  if (!shape || !cache) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "no shape or no cache");
+  SlotList list;
+  list.add(q);
+  list.add(cache->k, cache->pages != 0);
+  list.add(cache->v, cache->pages != 0);
+  if (shape->sequences && shape->table_width) list.add(table);
+  list.add(starts);
+  list.add(lengths);
+  list.add(out);
+  tiler_rt::Program p;
+  tiler_hip_status st = tiler_rt::plan_paged_attention_bf16(target_of(ctx), *shape, *cache, list.addr, p);
+  if (st != TILER_HIP_OK) return fail(ctx, st, p.diag);
+  if (!p.nlaunches) return TILER_HIP_OK;
+  if (list.missing) return fail(ctx, TILER_HIP_REFUSE_INVALID_ARGUMENT, "paged_attention: an operand is NULL");
+  hipStream_t s = pick(ctx, stream);
+  CallScratch scratch(ctx, s);
+  if ((st = bind_workspace(ctx, p, list, workspace, workspace_bytes, s, scratch)) != TILER_HIP_OK) return st;
+  return run_program(ctx, p, list.at, s);
+} catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
+  return TILER_HIP_REFUSE_CAPACITY;
+}
+
+tiler_hip_status tiler_hip_paged_attention_bf16_workspace(const tiler_hip_context* ctx,
+                                                          const tiler_hip_attention_shape* shape,
+                                                          const tiler_hip_paged_cache* cache, uint64_t* bytes) try {
+  if (!shape || !cache || !bytes) return TILER_HIP_REFUSE_INVALID_ARGUMENT;
+  const uintptr_t addr[tiler_rt::kMaxSlots] = {};
+  tiler_rt::Program p;
+  const tiler_hip_status st = tiler_rt::plan_paged_attention_bf16(target_of(ctx), *shape, *cache, addr, p);
+  *bytes = st == TILER_HIP_OK ? workspace_need(p) : 0;
+  return st;
 } catch (...) {  // host memory exhausted: nothing unwinds through the C ABI
   return TILER_HIP_REFUSE_CAPACITY;
 }

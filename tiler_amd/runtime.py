@@ -349,6 +349,52 @@ class Context:
         self._check(L.lib().tiler_hip_contract_i8(self.handle, _ptr(a), _ptr(b), _ptr(a_scales), _ptr(b_scales), m, n,
                                                   k, dtype, _ptr(c), stream), "contract_i8")
 
+    # -- the attention sublayer --------------------------------------------------
+    def page_slots(self, kept, fresh, sequences: int, page: int, free_pages, free_count: int, table, table_width: int,
+                   tokens: int, starts, lengths, positions, slots, taken, stream=None):
+        """The page table, positions and cache slots of a batch's new tokens
+        from the sequences' kept and fresh lengths (i32 throughout)."""
+        self._check(L.lib().tiler_hip_page_slots(self.handle, _ptr(kept), _ptr(fresh), sequences, page, _ptr(free_pages),
+                                                 free_count, _ptr(table), table_width, tokens, _ptr(starts),
+                                                 _ptr(lengths), _ptr(positions), _ptr(slots), _ptr(taken), stream),
+                    "page_slots")
+
+    def norm_rotate(self, dtype: int, heads: L.HeadLayout, q, k, v, wq, wk, positions, frequencies, q_out, k_out,
+                    cache: L.PagedCache | None = None, slots=None, stream=None):
+        """Query and key heads normed and rotated; with a cache, keys and
+        values stored at their slots."""
+        self._check(L.lib().tiler_hip_norm_rotate(self.handle, dtype, ctypes.byref(heads), _ptr(q), _ptr(k), _ptr(v),
+                                                  _ptr(wq), _ptr(wk), _ptr(positions), _ptr(frequencies), _ptr(q_out),
+                                                  _ptr(k_out), None if cache is None else ctypes.byref(cache),
+                                                  _ptr(slots), stream), "norm_rotate")
+
+    def norm_rotate_backward(self, dtype: int, heads: L.HeadLayout, dq_out, dk_out, q, k, wq, wk, positions, frequencies,
+                             dq=None, dk=None, dwq=None, dwk=None, workspace=None, workspace_bytes: int = 0, stream=None):
+        """dq, dk, dwq and dwk (those given) from dq_out and dk_out."""
+        self._check(L.lib().tiler_hip_norm_rotate_backward(
+            self.handle, dtype, ctypes.byref(heads), _ptr(dq_out), _ptr(dk_out), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk),
+            _ptr(positions), _ptr(frequencies), _ptr(dq), _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(workspace),
+            workspace_bytes, stream), "norm_rotate_backward")
+
+    def norm_rotate_backward_workspace(self, dtype: int, heads: L.HeadLayout) -> int:
+        n = ctypes.c_uint64()
+        self._check(L.lib().tiler_hip_norm_rotate_backward_workspace(self.handle, dtype, ctypes.byref(heads),
+                                                                     ctypes.byref(n)), "norm_rotate_backward_workspace")
+        return n.value
+
+    def paged_attention_bf16(self, shape: L.AttentionShape, q, cache: L.PagedCache, table, starts, lengths, out,
+                             workspace=None, workspace_bytes: int = 0, stream=None):
+        """The new tokens' attention over the paged cache that holds them."""
+        self._check(L.lib().tiler_hip_paged_attention_bf16(
+            self.handle, ctypes.byref(shape), _ptr(q), ctypes.byref(cache), _ptr(table), _ptr(starts), _ptr(lengths),
+            _ptr(out), _ptr(workspace), workspace_bytes, stream), "paged_attention_bf16")
+
+    def paged_attention_bf16_workspace(self, shape: L.AttentionShape, cache: L.PagedCache) -> int:
+        n = ctypes.c_uint64()
+        self._check(L.lib().tiler_hip_paged_attention_bf16_workspace(self.handle, ctypes.byref(shape), ctypes.byref(cache),
+                                                                     ctypes.byref(n)), "paged_attention_bf16_workspace")
+        return n.value
+
     def expression(self, dtype: int, nodes, inputs, n: int, y, root: int | None = None,
                    input_subnormals: int = 0, result_subnormals: int = 0, stream=None):
         """A pointwise expression DAG: `nodes` are (op, a, b) triples (L.NODE_*),
