@@ -16,7 +16,8 @@ struct TilerAttentionShape {
   uint32_t window, sinks;
   float scale;                                  // of the logits, times log2(e)
   TilerDivisor page, groups;
+  uint32_t page_stride, token_stride;           // of the cache, elements; a page's tokens span less than 2^32
   uint32_t reserved;
   uint64_t q_stride, out_stride;                // elements from token to token
-  uint64_t page_stride, token_stride, head_stride;
+  uint64_t head_stride;
 };

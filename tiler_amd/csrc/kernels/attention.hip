@@ -36,7 +36,22 @@ using tiler_pieces::u32x2_any;
 using tiler_pieces::u32x4_any;
 
 constexpr float kHidden = -__builtin_huge_valf();
-__device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
+// What is read in place of a key's or value's row that is not there.
+__device__ const u32x4 kZeroRow[32] = {};
+__device__ __forceinline__ uint64_t zero_row() {
+  uint64_t at = (uint64_t)(const void*)kZeroRow;
+  asm("" : "+v"(at));  // an address like the others: no branch around their loads
+  return at;
+}
+// 16 bytes a lane from `from` + kFrom, one after another to `to` (the instruction's
+// own offset counts on both sides).
+template <int kFrom = 0>
+__device__ __forceinline__ void load_to_lds(uint64_t from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((global_bytes*)from, (lds_bytes*)(to - kFrom), 16, kFrom, 0);
+}
+constexpr int kWaitAll = 0x0070;    // s_waitcnt vmcnt(0) lgkmcnt(0)
+constexpr int kWaitLds = 0xC07F;    // lgkmcnt(0)
+constexpr int kWaitLoads = 0x0F70;  // vmcnt(0)
 
 __device__ __forceinline__ uint32_t divide(const TilerDivisor& d, uint32_t n) {
   return (__umulhi(n, d.multiplier) + n) >> d.shift;
@@ -44,6 +59,15 @@ __device__ __forceinline__ uint32_t divide(const TilerDivisor& d, uint32_t n) {
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ uint32_t narrow2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((tiler::f32x2_pair{a, b}), tiler::bf16x2_pair));
+}
+// sum + the two weights of a packed pair, as the values' product takes them.
+__device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
+  const tiler::bf16x2_pair ones = {(__bf16)1.0f, (__bf16)1.0f};
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(tiler::bf16x2_pair, pair), ones, sum, false);
+}
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -85,14 +109,24 @@ struct Keys {
     steps = (high + kStep - 1u) / kStep - skip;
   }
   __device__ __forceinline__ uint32_t base(uint32_t t) const { return (t < sink_steps ? t : t + skip) * kStep; }
-  __device__ __forceinline__ bool read(uint32_t key) const { return key < high && (key >= low || key < sinks); }
+  __device__ __forceinline__ bool read(uint32_t key) const { return (key < high) & ((key >= low) | (key < sinks)); }
 };
 
-// Byte offset of a key's row in the cache, or all ones where none is read.
-__device__ __forceinline__ uint64_t row_offset(const TilerAttentionShape& a, bool read, int32_t entry, uint32_t key, uint32_t head) {
+// The keys that one row sees: key <= limit and (key > floor or key < sinks).
+struct Sight {
+  int32_t limit, floor;
+  __device__ __forceinline__ Sight(const TilerAttentionShape& a, uint32_t high, int32_t p) {
+    limit = p < (int32_t)high - 1 ? p : (int32_t)high - 1;
+    limit = limit > -1 ? limit : -1;
+    const int64_t behind = (int64_t)p - (int64_t)a.window;
+    floor = a.window && behind > -1 ? (int32_t)behind : -1;
+  }
+};
+// Byte offset of a key's row in the cache, or -1 where none is read.
+__device__ __forceinline__ int64_t row_offset(const TilerAttentionShape& a, bool read, int32_t entry, uint32_t key, uint32_t head) {
   const uint32_t in = key - divide(a.page, key) * a.page.divisor;
   const uint64_t at = (uint64_t)(uint32_t)entry * a.page_stride + (uint64_t)in * a.token_stride + (uint64_t)head * a.head_stride;
-  return read && (uint32_t)entry < a.pages ? at * 2u : ~0ull;
+  return (read & ((uint32_t)entry < a.pages)) ? (int64_t)(at * 2u) : -1;
 }
 
 // Place of a 16-byte piece in a value row of D elements in LDS.  The transposing
@@ -121,9 +155,9 @@ struct FewSpace {
 };
 
 template <int NC>
-__device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t* q, const uint8_t* k, const uint8_t* v,
-                                    const int32_t* table, const int32_t* starts, const int32_t* lengths, uint16_t* out,
-                                    float* part_o, tiler::f32x2_pair* part_ml, FewSpace<NC>& space) {
+__device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t* __restrict__ q, const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
+                                    const int32_t* __restrict__ table, const int32_t* __restrict__ starts, const int32_t* __restrict__ lengths, uint16_t* __restrict__ out,
+                                    float* __restrict__ part_o, tiler::f32x2_pair* __restrict__ part_ml, FewSpace<NC>& space) {
   using Space = FewSpace<NC>;
   constexpr int D = Space::D, NB = 2 * NC;  // blocks of 16 elements
   constexpr uint32_t kPieces = D / 8;
@@ -156,43 +190,46 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
     for (int i = 0; i < NB; ++i) o[i] = f32x4{0, 0, 0, 0};
     float m = kHidden, l = 0.0f;
     u32x4 kf[2][NC];
+    const Sight sight(a, keys.high, p);
+    const int32_t sinks = a.sinks < 0x7fffffffu ? (int32_t)a.sinks : 0x7fffffff;
+    const uint64_t zero = zero_row();
     int32_t entry = -1;
     auto look_up = [&](uint32_t t) {
       const uint32_t key = keys.base(t) + (lane & 31u);
-      entry = t < end && keys.read(key) ? pages[divide(a.page, key)] : -1;
+      entry = pages[((t < end) & keys.read(key)) ? divide(a.page, key) : 0u];
     };
     // Step t's keys into kf, its values on their way to the stage.
     auto request = [&](uint32_t t, uint32_t stage) {
       const uint32_t key = keys.base(t) + (lane & 31u);
-      const uint64_t off = row_offset(a, keys.read(key), entry, key, head);
+      const int64_t off = row_offset(a, keys.read(key), entry, key, head);
       auto of = [&](uint32_t r) {  // row r's offset
         const uint32_t lo = __builtin_amdgcn_ds_bpermute((int)(r * 4u), (int)(uint32_t)off);
         const uint32_t hi = __builtin_amdgcn_ds_bpermute((int)(r * 4u), (int)(uint32_t)(off >> 32));
-        return (uint64_t)hi << 32 | lo;
+        return (int64_t)((uint64_t)hi << 32 | lo);
       };
 #pragma unroll
       for (uint32_t i = 0; i < Space::kStage / 1024u; ++i) {
         const uint32_t id = i * 64u + lane, r = id / kPieces, piece = value_piece<D>(r, id % kPieces);
-        const uint64_t at = of(r);
-        const uint8_t* from = at != ~0ull && piece < real_pieces ? v + at + piece * 16u : (const uint8_t*)&kZeroPiece;
-        __builtin_amdgcn_global_load_lds((global_bytes*)from, (lds_bytes*)(space.stage[wave][stage] + i * 1024u), 16, 0, 0);
+        const int64_t at = of(r);
+        load_to_lds(at >= 0 && piece < real_pieces ? (uint64_t)v + at + piece * 16u : zero, space.stage[wave][stage] + i * 1024u);
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const uint64_t at = of(16u * b + col);
+        const int64_t at = of(16u * b + col);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const uint32_t piece = 4u * c + g;
-          const uint8_t* from = at != ~0ull && piece < real_pieces ? k + at + piece * 16u : (const uint8_t*)&kZeroPiece;
-          kf[b][c] = *reinterpret_cast<const u32x4*>(from);
+          kf[b][c] = *reinterpret_cast<const u32x4*>(at >= 0 && piece < real_pieces ? (uint64_t)k + at + piece * 16u : zero);
         }
       }
     };
     for (uint32_t t = begin + wave; t < end; t += Space::kWaves) {
       look_up(t);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(kWaitLds);  // the stage is read
+      asm volatile("" ::: "memory");
       request(t, 0);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(kWaitLoads);
+      asm volatile("" ::: "memory");
       f32x4 sc[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -205,10 +242,9 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const uint32_t key = base + 16u * b + 4u * g + r;
-          const bool seen = key < keys.high && (int32_t)key <= p &&
-                            (!a.window || (int64_t)key > (int64_t)p - (int64_t)a.window || key < a.sinks);
-          if (!seen) sc[b][r] = kHidden;
+          const int32_t key = (int32_t)(base + 16u * b + 4u * g + r);
+          const bool seen = (key <= sight.limit) & ((key > sight.floor) | (key < sinks));
+          sc[b][r] = seen ? sc[b][r] : kHidden;
         }
       float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                         fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
@@ -282,6 +318,350 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: four or eight waves of 32 rows each over steps of 64 keys, two steps
+// of keys and values in LDS, brought there directly, one while the other is worked
+// on.  Four waves bring a step; of eight, four take turns with the other four.
+//
+// LDS holds a step as 4 groups of 16 keys, each as NS segments of 32 elements, each
+// as 16 keys of 64 bytes: a wave brings one group, each lane a piece of one key for
+// every segment, so that it looks up one page a step.  Of the keys, piece c of a
+// segment sits at c ^ (key / 4 & 3): the 16 keys of a fragment read then cover all
+// banks.  A transposing read of the values takes 8 keys of one segment, 512 bytes
+// in a row.
+//
+// The running maximum moves only where a logit passes it by kSlack (a factor of
+// 2^8 in the weights, far inside binary32 and bf16): most steps rescale nothing.
+constexpr float kSlack = 8.0f;
+
+template <int I, int N, typename F>
+__device__ __forceinline__ void unroll(F f) {
+  if constexpr (I < N) {
+    f(tiler::Step<I>{});
+    unroll<I + 1, N>(f);
+  }
+}
+
+template <int NS>
+struct TileSpace {
+  static constexpr uint32_t kOperand = 64u * NS * 64u;
+  uint8_t keys[2][kOperand], values[2][kOperand];
+};
+
+template <int NS, int WAVES>
+__device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_t* __restrict__ q, const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
+                                     const int32_t* __restrict__ table, const int32_t* __restrict__ starts, const int32_t* __restrict__ lengths, uint16_t* __restrict__ out,
+                                     float* __restrict__ part_o, tiler::f32x2_pair* __restrict__ part_ml, TileSpace<NS>& space) {
+  constexpr uint32_t kRows = 32u * WAVES, kTurns = WAVES / 4;
+  constexpr int NC = 2 * NS;  // depth steps of 16 elements
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t col = lane & 31u, h = lane >> 5;
+  const uint32_t head = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads % a.splits;
+  const uint32_t at_tile = gridDim.x / (a.kv_heads * a.splits) - 1u - blockIdx.x / (a.kv_heads * a.splits);
+  // Sequence s has the tiles from starts[s] * group / kRows + s on: as many as its
+  // rows need, or one more.
+  uint32_t s = 0, tile_in = 0;
+  {
+    uint32_t before = 0, at = 0;
+    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64u) {
+      const uint32_t n = s0 + lane;
+      int32_t start = n < a.sequences ? starts[n] : 0;
+      start = start < 0 ? 0 : start > (int32_t)a.tokens ? (int32_t)a.tokens : start;
+      const uint32_t from = (uint32_t)start * a.group / kRows + n;
+      const uint64_t mask = __ballot(n < a.sequences && from <= at_tile);
+      if (mask) at = __builtin_amdgcn_readlane(from, 63 - __builtin_clzll(mask));
+      before += __popcll(mask);
+      if (mask != ~0ull) break;
+    }
+    if (before == 0) return;
+    s = before - 1u;
+    tile_in = at_tile - at;
+  }
+  const Sequence seq(a, starts, lengths, s);
+  const uint32_t rows = seq.fresh * a.group, row0 = tile_in * kRows;
+  if (row0 >= rows) return;
+  const int32_t* const pages = table + (uint64_t)s * a.width;
+  const uint32_t real_pieces = a.head_dim / 8u;
+  auto position = [&](uint32_t row) { return seq.kept + (int32_t)divide(a.groups, row < rows ? row : rows - 1u); };
+  const Keys<64> keys(a, position(row0), position(row0 + kRows - 1u));
+  const uint32_t begin = (uint32_t)((uint64_t)keys.steps * split / a.splits);
+  const uint32_t end = (uint32_t)((uint64_t)keys.steps * (split + 1u) / a.splits);
+  const uint32_t wave_row = row0 + wave * 32u;
+  const bool works = wave_row < rows;
+  const int32_t p_first = position(wave_row), p_last = position(wave_row + 31u);
+  const uint32_t row = wave_row + col, real = row < rows ? row : rows - 1u;
+  const uint32_t token = divide(a.groups, real), hq = head * a.group + (real - token * a.group);
+  const int32_t p = seq.kept + (int32_t)token;
+  u32x4 qf[NC];
+  {
+    const uint16_t* at = q + (uint64_t)(seq.first + token) * a.q_stride + (uint64_t)hq * a.head_dim;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      qf[c] = 2u * c + h < real_pieces ? *reinterpret_cast<const u32x4_any*>(at + 16 * c + 8 * h) : u32x4{0, 0, 0, 0};
+  }
+  // This lane's key of a step, and the piece of a segment that it brings; pieces
+  // past the head's end are zeros.
+  const uint32_t key_in = wave % 4u * 16u + (lane >> 2), turn = wave / 4u, value_in = lane & 3u, key_piece = value_in ^ ((lane >> 4) & 3u);
+  const bool cut = real_pieces != 4u * NS;
+  const uint64_t zero = zero_row();
+  const uint64_t keys_from = (uint64_t)k + head * a.head_stride * 2u + key_piece * 16u;
+  const uint64_t values_from = (uint64_t)v + head * a.head_stride * 2u + value_in * 16u;
+  // The page of this lane's key, the key's place in it (elements) and the entry of
+  // the table: looked up a step ahead, and stepped without a division.
+  const uint32_t page_span = a.page.divisor * a.token_stride;
+  const uint32_t step_pages = divide(a.page, 64u * kTurns), step_span = (64u * kTurns - step_pages * a.page.divisor) * a.token_stride;
+  uint32_t index = 0, in_page = 0, in_found = 0;
+  int32_t entry = -1;
+  uint64_t found = 0;  // a bit a lane
+  auto go_to = [&](uint32_t t) {
+    const uint32_t key = keys.base(t) + key_in;
+    index = divide(a.page, key);
+    in_page = (key - index * a.page.divisor) * a.token_stride;
+  };
+  auto look_up = [&](uint32_t t) {  // of step t, and on to this wave's next
+    const uint32_t base = keys.base(t), key = base + key_in;
+    found = t < end ? ~0ull : 0ull;
+    if (base < keys.low || base + 63u >= keys.high) found &= __ballot(keys.read(key));
+    entry = pages[found >> lane & 1u ? index : 0u];
+    in_found = in_page;
+    if (t < keys.sink_steps && t + kTurns >= keys.sink_steps) {
+      go_to(t + kTurns);
+    } else {
+      in_page += step_span;
+      const bool wraps = in_page >= page_span || in_page < step_span;
+      index += step_pages + (wraps ? 1u : 0u);
+      in_page -= wraps ? page_span : 0u;
+    }
+  };
+  struct Row {
+    uint64_t at, there;  // elements; a bit a lane
+  };
+  auto row_found = [&] {
+    return Row{(uint64_t)(uint32_t)entry * a.page_stride + in_found, found & __ballot((uint32_t)entry < a.pages)};
+  };
+  uint8_t* const to = space.keys[0] + wave % 4u * (NS * 1024u);
+  auto request = [&](const Row& r, uint64_t from, uint32_t piece, uint8_t* at) {
+    uint64_t src = from + r.at * 2u;
+    if (r.there != ~0ull) src = r.there >> lane & 1u ? src : zero;
+    unroll<0, NS>([&](auto n) {
+      if (cut) load_to_lds<n.value * 64>(4u * n.value + piece < real_pieces ? src : zero, at + n.value * 1024);
+      else load_to_lds<n.value * 64>(src, at + n.value * 1024);
+    });
+  };
+  auto request_keys = [&](const Row& r, uint32_t buffer) { request(r, keys_from, key_piece, to + buffer * TileSpace<NS>::kOperand); };
+  auto request_values = [&](const Row& r, uint32_t buffer) {
+    request(r, values_from, value_in, to + (2u + buffer) * TileSpace<NS>::kOperand);
+  };
+  auto landed = [&] {  // everything this wave requested; behind the barrier, every wave's
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    asm volatile("s_barrier" ::: "memory");
+  };
+  f32x16 o[NS], sc[2];
+  float m = kHidden, l = 0.0f, most = kHidden;  // most: of this lane's first 16 logits of a step
+  u32x4 pf[4];  // the last step's weights
+#pragma unroll
+  for (int n = 0; n < NS; ++n) o[n] = f32x16{};
+  // Byte offsets of this lane's fragments: keys 32 kb + col, piece 2 c + h; values
+  // of keys 16 kc + 4 h + (lane / 4 & 3) (and 8 on), elements 32 n + 16 (lane / 16 & 1) + 4 (lane & 3).
+  const uint32_t key_at = (col >> 4) * (NS * 1024u) + (col & 15u) * 64u, key_swap = (col >> 2) & 3u;
+  const uint32_t value_at = (4u * h + ((lane >> 2) & 3u)) * 64u + ((lane >> 4) & 1u) * 32u + (lane & 3u) * 8u;
+  const Sight first(a, keys.high, p_first), last(a, keys.high, p_last), sight(a, keys.high, p);
+  const int32_t sinks = a.sinks < 0x7fffffffu ? (int32_t)a.sinks : 0x7fffffff;
+  auto read_key = [&](uint32_t buffer, int kb, int c) {
+    return *reinterpret_cast<const u32x4*>(space.keys[buffer] + key_at + kb * (2u * NS * 1024u) + (c >> 1) * 1024u +
+                                           ((((c & 1u) * 2u + h) ^ key_swap) << 4));
+  };
+  auto read_value = [&](uint32_t buffer, int kc, int n) {
+    const uint8_t* at = space.values[buffer] + value_at + kc * (NS * 1024u) + n * 1024u;
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 512)));
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
+  // What the last step's maximum made of the results before that step's values.
+  bool moved = false;
+  float alpha = 1.0f;
+  auto rescale = [&] {
+    if (moved) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) o[n] *= alpha;
+    }
+  };
+  Row rows_of[3 - kTurns] = {};  // whose values are still to come: of this wave's steps before t + 2
+  // Step t, of which sc holds the logits: its weights to pf, while the matrix unit
+  // takes in the values of step t - 1 (unless t is the first) and makes the logits of
+  // step t + 1 in the place of these (unless t is the last).
+  auto step = [&](uint32_t t, auto is_first, auto is_last) {
+    const uint32_t buffer = (t - begin) & 1u;
+    const int32_t base = (int32_t)keys.base(t), top_key = base > 0x7fffffff - 63 ? 0x7fffffff : base + 63;
+    if (top_key > first.limit || (base <= last.floor && top_key >= sinks)) {  // not every row sees every key
+      const int32_t from = base + 4 * (int32_t)h, limit = sight.limit - from, floor = sight.floor - from, sink = sinks - from;
+      most = kHidden;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int32_t key = 8 * (i >> 2) + (i & 3);
+        const bool seen = (key <= limit) & ((key > floor) | (key < sink));
+        sc[i >> 4][i & 15] = seen ? sc[i >> 4][i & 15] : kHidden;
+        if (i < 16) most = fmaxf(most, sc[0][i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(most, sc[1][i]), sc[1][i + 1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+    const float top = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+    rescale();
+    moved = __any((top - m) * a.scale > kSlack);  // also at the first key: m is -infinity
+    if (moved) {
+      const float to = fmaxf(top, m);
+      alpha = to == kHidden ? 1.0f : exp2_fast((m - to) * a.scale);
+      m = to;
+      l *= alpha;
+    }
+    const float shift = m == kHidden ? 0.0f : -m * a.scale;
+    most = kHidden;
+    u32x4 weights[4];
+    float sums[2] = {0.0f, 0.0f}, one = 0.0f;
+    auto weigh = [&](int i) {  // logit i of the step's 32
+      const float w = exp2_fast(__builtin_fmaf(sc[i >> 4][i & 15], a.scale, shift));
+      if (i % 2 == 0) {
+        one = w;
+        asm volatile("" : "+v"(one));  // made here, not where it is used
+        return;
+      }
+      uint32_t both = narrow2(one, w);
+      float sum = add_pair(both, sums[(i >> 1) & 1]);
+      asm volatile("" : "+v"(both), "+v"(sum));
+      sums[(i >> 1) & 1] = sum;
+      weights[i >> 3][(i >> 1) & 3] = both;
+    };
+    // The products one by one: three quarters of the values' with the weights of the
+    // first 32 keys, whose logits' place the next first 32 take then, with the rest
+    // of the values' beside the other weights; then the next other 32 keys'.  With
+    // each product go its share of the weights (at the end, of the next maximum) and
+    // the fragment of a later product.  Nothing moves from one such group to another:
+    // left to itself the compiler puts all weights before the products.
+    constexpr int kA = is_first.value ? 0 : 3 * NS, kB = kA + (is_last.value ? 0 : 2 * NS), kC = kB + (is_first.value ? 0 : NS);
+    constexpr int kProducts = kC + (is_last.value ? 0 : 2 * NS), kAhead = NS > 4 ? 2 : 4;
+    auto fragment = [&](int u) {
+      const int p = u < kA ? u : u - (kB - kA);  // of the values
+      return u < kA || (u >= kB && u < kC) ? read_value(buffer ^ 1u, p / NS, p % NS)
+                                           : read_key(buffer ^ 1u, u >= kC, u < kB ? u - kA : u - kC);
+    };
+    auto weighed = [&](int u) {  // logits before product u
+      if (is_last.value) return kProducts ? 32 * u / (kProducts ? kProducts : 1) : 32;
+      return u < kA ? 16 * u / (kA ? kA : 1) : u < kC ? 16 + 16 * (u - kA) / (kC - kA) : 32;
+    };
+#pragma unroll
+    for (int i = 0; i < weighed(0); ++i) weigh(i);
+    u32x4 f[kAhead + 1];
+#pragma unroll
+    for (int u = 0; u < kAhead && u < kProducts; ++u) f[u] = fragment(u);
+#pragma unroll
+    for (int u = 0; u < kProducts; ++u) {
+      if (u + kAhead < kProducts) f[(u + kAhead) % (kAhead + 1)] = fragment(u + kAhead);
+      const u32x4 at = f[u % (kAhead + 1)];
+      const int p = u < kA ? u : u - (kB - kA);
+      if (u < kA || (u >= kB && u < kC)) o[p % NS] = mfma32(at, pf[p / NS], o[p % NS]);
+      else if (u < kB) sc[0] = mfma32(at, qf[u - kA], u == kA ? f32x16{} : sc[0]);
+      else sc[1] = mfma32(at, qf[u - kC], u == kC ? f32x16{} : sc[1]);
+#pragma unroll
+      for (int i = weighed(u); i < weighed(u + 1); ++i) weigh(i);
+      if (u >= kC) {
+#pragma unroll
+        for (int i = (u - kC) * 8 / (2 * NS); i < (u - kC + 1) * 8 / (2 * NS); ++i) {
+          most = fmaxf(fmaxf(most, sc[0][2 * i]), sc[0][2 * i + 1]);
+          asm volatile("" : "+v"(most));
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l += sums[0] + sums[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pf[i] = weights[i];
+  };
+  if (begin < end) {
+    using No = tiler::Step<0>;
+    using Yes = tiler::Step<1>;
+    go_to(begin + turn);
+    look_up(begin + turn);
+    for (uint32_t i = 0; i < 3u - kTurns; ++i) {
+      rows_of[i] = row_found();
+      look_up(begin + turn + (i + 1u) * kTurns);
+    }
+    if (turn == 0) request_keys(rows_of[0], 0);
+    landed();
+    if (kTurns == 1) request_keys(rows_of[2 - kTurns], 1);
+    else if (turn == 1) request_keys(rows_of[0], 1);
+    if (works) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) sc[kb] = mfma32(read_key(0, kb, c), qf[c], c == 0 ? f32x16{} : sc[kb]);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(most, sc[0][i]), sc[0][i + 1]);
+    }
+    // Before step t: the keys of step t + 1 and the values of step t - 1 have landed,
+    // and every wave has read those of steps t and t - 2, whose places the next ones take.
+    auto advance = [&](uint32_t t) {
+      landed();
+      const uint32_t buffer = (t - begin) & 1u;
+      if (kTurns > 1 && buffer != turn) return;
+      const Row r = row_found();
+      look_up(t + 2u + kTurns);
+      if (t + 2u < end) request_keys(r, buffer);
+      request_values(rows_of[0], buffer);
+      if (kTurns == 1) rows_of[0] = rows_of[2 - kTurns];
+      rows_of[2 - kTurns] = r;
+    };
+    uint32_t t = begin;
+    advance(t);
+    if (end - begin == 1u) {
+      if (works) step(t, Yes{}, Yes{});
+    } else {
+      if (works) step(t, Yes{}, No{});
+      for (++t; t + 1u < end; ++t) {
+        advance(t);
+        if (works) step(t, No{}, No{});
+      }
+      advance(t);
+      if (works) step(t, No{}, Yes{});
+    }
+    landed();  // the last values
+    if (works) {
+      rescale();
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+        for (int n = 0; n < NS; ++n) o[n] = mfma32(read_value((end - 1u - begin) & 1u, kc, n), pf[kc], o[n]);
+    }
+  }
+  if (row >= rows) return;
+  const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+  const float total = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+  const uint64_t token_row = seq.first + token;
+  if (a.splits > 1u) {
+    const uint64_t at = (token_row * (a.kv_heads * a.group) + hq) * a.splits + split;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const uint32_t d = 32u * n + 2u * i + 4u * h;
+        if (d < a.head_dim) *reinterpret_cast<f32x4*>(part_o + at * a.head_dim + d) = f32x4{o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]};
+      }
+    if (h == 0) part_ml[at] = tiler::f32x2_pair{m, total};
+  } else {
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t* const at = out + token_row * a.out_stride + (uint64_t)hq * a.head_dim;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const uint32_t d = 32u * n + 2u * i + 4u * h;
+        if (d < a.head_dim)
+          *reinterpret_cast<u32x2_any*>(at + d) = u32x2{narrow2(o[n][i] * by, o[n][i + 1] * by), narrow2(o[n][i + 2] * by, o[n][i + 3] * by)};
+      }
+  }
+}
+
 // A row's splits joined, in order: a wave a row.
 __device__ __forceinline__ void join(const TilerAttentionShape& a, const int32_t* starts, const float* part_o,
                                      const tiler::f32x2_pair* part_ml, uint16_t* out) {
@@ -321,6 +701,23 @@ TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few64, 2)
 TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few128, 4)
 TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few256, 8)
 #undef TILER_ATTENTION_FEW
+
+#define TILER_ATTENTION_TILE(NAME, NS, WAVES, EACH)                                                                 \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, EACH) NAME(                                                    \
+      TilerAttentionShape a, const uint16_t* q, const uint8_t* k, const uint8_t* v, const int32_t* table,           \
+      const int32_t* starts, const int32_t* lengths, uint16_t* out, float* part_o, tiler::f32x2_pair* part_ml) {    \
+    __shared__ __attribute__((aligned(16))) tiler_attention::TileSpace<NS> space;                                   \
+    tiler_attention::tile<NS, WAVES>(a, q, k, v, table, starts, lengths, out, part_o, part_ml, space);                 \
+  }
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t128_d64, 2, 4, 2)
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t128_d96, 3, 4, 2)
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t128_d128, 4, 4, 2)
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t128_d192, 6, 4, 1)
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t128_d256, 8, 4, 1)
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t256_d64, 2, 8, 2)
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t256_d96, 3, 8, 2)
+TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t256_d128, 4, 8, 2)
+#undef TILER_ATTENTION_TILE
 
 extern "C" __global__ void __launch_bounds__(256)
     tiler_paged_attention_bf16_join(TilerAttentionShape a, const int32_t* starts, const float* part_o,

@@ -290,6 +290,9 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   const uint32_t starts = p.slot(4 * (a.sequences + 1), kSlotInput), lengths = p.slot(4 * a.sequences, kSlotInput);
   const uint32_t out = p.slot(2 * span(a.tokens, a.out_stride, row), kSlotOutput);
   if (a.sequences == 0 || a.tokens == 0) return TILER_HIP_OK;
+  // the kernels' offsets inside the cache: 32 bits times 32 bits, and 32 inside a page
+  if ((cache.pages > 1 && cache.page_stride > 0xffffffffull) || mul_sat(cache.page, cache.token_stride) > 0xffffffffull)
+    return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: a page of 2^32 elements and more");
   if ((cache.page_stride | cache.token_stride | cache.head_stride) % 8 || !aligned16(addr[k]) || !aligned16(addr[v]))
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "the cache's rows start on 16 bytes");
   TilerAttentionShape s{};
@@ -307,26 +310,40 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   s.groups = divisor_of(s.group);
   s.q_stride = a.q_stride;
   s.out_stride = a.out_stride;
-  s.page_stride = cache.page_stride;
-  s.token_stride = cache.token_stride;
+  s.page_stride = (uint32_t)cache.page_stride;
+  s.token_stride = (uint32_t)cache.token_stride;
   s.head_stride = cache.head_stride;
   const uint64_t room = a.table_width * cache.page;
   uint64_t longest = a.max_length && a.max_length < room ? a.max_length : room;
   if (a.window && longest > (uint64_t)a.window + a.sinks) longest = (uint64_t)a.window + a.sinks;
-  // split a sequence's keys where its workgroups would leave CUs idle, 512 keys at least to a part
-  const uint64_t alone = mul_sat(a.sequences, s.kv_heads);
+  const uint64_t fresh = a.max_fresh && a.max_fresh < a.tokens ? a.max_fresh : a.tokens;
+  const uint32_t dim = s.head_dim;
+  uint64_t tile_rows = 16;
+  if (fresh * s.group > 16) {
+    tile_rows = 128;
+    // 256 rows (eight waves share the keys) where such tiles are two to a CU
+    if (dim <= 128 && mul_sat(a.tokens * s.group / 256, s.kv_heads) >= 2ull * t.compute_units) tile_rows = 256;
+  }
+  // split the keys where the tiles would leave CUs idle, 512 keys at least to a part
+  const uint64_t tiles = tile_rows == 16 ? a.sequences : a.tokens * s.group / tile_rows + a.sequences;
+  const uint64_t alone = mul_sat(tiles, s.kv_heads);
   uint64_t splits = ceil_div(2ull * t.compute_units, alone);
   if (splits > ceil_div(longest, 512)) splits = ceil_div(longest, 512);
   if (splits < 1) splits = 1;
   s.splits = (uint32_t)splits;
-  if (mul_sat(alone, splits) > 0xffffffffull / 256)
+  if (mul_sat(alone, splits) > 0xffffffffull / 512)
     return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: more workgroups than a launch holds");
   const uint64_t rows = a.tokens * a.q_heads;
   const uint32_t part = splits > 1 ? p.slot(4 * mul_sat(rows * splits, s.head_dim), kSlotScratch) : 0;
   const uint32_t ml = splits > 1 ? p.slot(8 * rows * splits, kSlotScratch) : 0;
   char name[64];
-  std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_few%u", s.head_dim <= 64 ? 64 : s.head_dim <= 128 ? 128 : 256);
-  Launch& l = p.add(name, (uint32_t)(alone * splits), 1, 256).blob(&s, sizeof(s), 8).ptr(q).ptr(k).ptr(v);
+  if (tile_rows == 16)
+    std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_few%u", dim <= 64 ? 64 : dim <= 128 ? 128 : 256);
+  else
+    std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_t%u_d%u", (uint32_t)tile_rows,
+                  dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256);
+  const uint32_t block = tile_rows == 256 ? 512 : 256;
+  Launch& l = p.add(name, (uint32_t)(alone * splits), 1, block).blob(&s, sizeof(s), 8).ptr(q).ptr(k).ptr(v);
   slot_or_null(l, table, at);
   l.ptr(starts).ptr(lengths).ptr(out);
   slot_or_null(l, splits > 1, part);

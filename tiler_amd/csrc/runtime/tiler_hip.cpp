@@ -413,6 +413,14 @@ const EntryRow kEntries[] = {
     {"tiler_paged_attention_bf16_few64", "paged-attention-bf16", 9},
     {"tiler_paged_attention_bf16_few128", "paged-attention-bf16", 9},
     {"tiler_paged_attention_bf16_few256", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t128_d64", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t128_d96", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t128_d128", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t128_d192", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t128_d256", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t256_d64", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t256_d96", "paged-attention-bf16", 9},
+    {"tiler_paged_attention_bf16_t256_d128", "paged-attention-bf16", 9},
     {"tiler_paged_attention_bf16_join", "paged-attention-bf16", 4},
 };
 constexpr uint32_t kEntryCount = sizeof(kEntries) / sizeof(kEntries[0]);
