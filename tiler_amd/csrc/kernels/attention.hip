@@ -120,6 +120,7 @@ struct Sight {
     limit = limit > -1 ? limit : -1;
     const int64_t behind = (int64_t)p - (int64_t)a.window;
     floor = a.window && behind > -1 ? (int32_t)behind : -1;
+    floor = floor < limit ? floor : limit;
   }
 };
 // Byte offset of a key's row in the cache, or -1 where none is read.
@@ -402,7 +403,6 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   // This lane's key of a step, and the piece of a segment that it brings; pieces
   // past the head's end are zeros.
   const uint32_t key_in = wave % 4u * 16u + (lane >> 2), turn = wave / 4u, value_in = lane & 3u, key_piece = value_in ^ ((lane >> 4) & 3u);
-  const bool cut = real_pieces != 4u * NS;
   const uint64_t zero = zero_row();
   const uint64_t keys_from = (uint64_t)k + head * a.head_stride * 2u + key_piece * 16u;
   const uint64_t values_from = (uint64_t)v + head * a.head_stride * 2u + value_in * 16u;
@@ -420,9 +420,14 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   };
   auto look_up = [&](uint32_t t) {  // of step t, and on to this wave's next
     const uint32_t base = keys.base(t), key = base + key_in;
-    found = t < end ? ~0ull : 0ull;
-    if (base < keys.low || base + 63u >= keys.high) found &= __ballot(keys.read(key));
-    entry = pages[found >> lane & 1u ? index : 0u];
+    uint32_t at = index;
+    found = ~0ull;
+    if (t >= end || base < keys.low || base + 63u >= keys.high) {
+      found = t < end ? __ballot(keys.read(key)) : 0ull;
+      at = found >> lane & 1u ? index : 0u;
+      asm volatile("" : "+v"(at));
+    }
+    entry = pages[at];
     in_found = in_page;
     if (t < keys.sink_steps && t + kTurns >= keys.sink_steps) {
       go_to(t + kTurns);
@@ -441,11 +446,20 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   };
   uint8_t* const to = space.keys[0] + wave % 4u * (NS * 1024u);
   auto request = [&](const Row& r, uint64_t from, uint32_t piece, uint8_t* at) {
+    // Branches, not selections: the asm keeps the usual case free of them.
     uint64_t src = from + r.at * 2u;
-    if (r.there != ~0ull) src = r.there >> lane & 1u ? src : zero;
+    if (r.there != ~0ull) {
+      src = r.there >> lane & 1u ? src : zero;
+      asm volatile("" : "+v"(src));
+    }
     unroll<0, NS>([&](auto n) {
-      if (cut) load_to_lds<n.value * 64>(4u * n.value + piece < real_pieces ? src : zero, at + n.value * 1024);
-      else load_to_lds<n.value * 64>(src, at + n.value * 1024);
+      if (4u * n.value + 4u > real_pieces) {
+        uint64_t some = 4u * n.value + piece < real_pieces ? src : zero;
+        asm volatile("" : "+v"(some));
+        load_to_lds<n.value * 64>(some, at + n.value * 1024);
+      } else {
+        load_to_lds<n.value * 64>(src, at + n.value * 1024);
+      }
     });
   };
   auto request_keys = [&](const Row& r, uint32_t buffer) { request(r, keys_from, key_piece, to + buffer * TileSpace<NS>::kOperand); };
@@ -493,15 +507,26 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   auto step = [&](uint32_t t, auto is_first, auto is_last) {
     const uint32_t buffer = (t - begin) & 1u;
     const int32_t base = (int32_t)keys.base(t), top_key = base > 0x7fffffff - 63 ? 0x7fffffff : base + 63;
-    if (top_key > first.limit || (base <= last.floor && top_key >= sinks)) {  // not every row sees every key
-      const int32_t from = base + 4 * (int32_t)h, limit = sight.limit - from, floor = sight.floor - from, sink = sinks - from;
-      most = kHidden;
+    const bool cut_above = top_key > first.limit, cut_below = base <= last.floor && top_key >= sinks;
+    if (cut_above || cut_below) {  // not every row sees every key
+      const int32_t from = base + 4 * (int32_t)h;
+      auto show = [&](auto seen) {
+        most = kHidden;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int32_t key = 8 * (i >> 2) + (i & 3);
-        const bool seen = (key <= limit) & ((key > floor) | (key < sink));
-        sc[i >> 4][i & 15] = seen ? sc[i >> 4][i & 15] : kHidden;
-        if (i < 16) most = fmaxf(most, sc[0][i]);
+        for (int i = 0; i < 32; ++i) {
+          sc[i >> 4][i & 15] = seen(8 * (i >> 2) + (i & 3)) ? sc[i >> 4][i & 15] : kHidden;
+          if (i < 16) most = fmaxf(most, sc[0][i]);
+        }
+      };
+      if (!cut_below || top_key < (int32_t)keys.low) {  // one bound: the row's own key, or the sinks before every window
+        const int32_t limit = (cut_below ? sinks - 1 : sight.limit) - from;
+        show([&](int32_t key) { return key <= limit; });
+      } else if (base >= sinks) {  // a window: one comparison of what lies above its floor
+        const uint32_t below = (uint32_t)(from - 1 - sight.floor), count = (uint32_t)(sight.limit - sight.floor);
+        show([&](int32_t key) { return below + (uint32_t)key < count; });
+      } else {
+        const int32_t limit = sight.limit - from, floor = sight.floor - from, sink = sinks - from;
+        show([&](int32_t key) { return (key <= limit) & ((key > floor) | (key < sink)); });
       }
     }
 #pragma unroll
@@ -540,7 +565,7 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
     // the fragment of a later product.  Nothing moves from one such group to another:
     // left to itself the compiler puts all weights before the products.
     constexpr int kA = is_first.value ? 0 : 3 * NS, kB = kA + (is_last.value ? 0 : 2 * NS), kC = kB + (is_first.value ? 0 : NS);
-    constexpr int kProducts = kC + (is_last.value ? 0 : 2 * NS), kAhead = NS > 4 ? 2 : 4;
+    constexpr int kProducts = kC + (is_last.value ? 0 : 2 * NS), kBatch = 2;
     auto fragment = [&](int u) {
       const int p = u < kA ? u : u - (kB - kA);  // of the values
       return u < kA || (u >= kB && u < kC) ? read_value(buffer ^ 1u, p / NS, p % NS)
@@ -552,17 +577,21 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
     };
 #pragma unroll
     for (int i = 0; i < weighed(0); ++i) weigh(i);
-    u32x4 f[kAhead + 1];
+    u32x4 f[2][kBatch];
 #pragma unroll
-    for (int u = 0; u < kAhead && u < kProducts; ++u) f[u] = fragment(u);
-#pragma unroll
-    for (int u = 0; u < kProducts; ++u) {
-      if (u + kAhead < kProducts) f[(u + kAhead) % (kAhead + 1)] = fragment(u + kAhead);
-      const u32x4 at = f[u % (kAhead + 1)];
+    for (int u = 0; u < kBatch && u < kProducts; ++u) f[0][u] = fragment(u);
+    unroll<0, kProducts>([&](auto product) {
+      constexpr int u = product.value;
+      const u32x4 at = f[u / kBatch % 2][u % kBatch];
       const int p = u < kA ? u : u - (kB - kA);
       if (u < kA || (u >= kB && u < kC)) o[p % NS] = mfma32(at, pf[p / NS], o[p % NS]);
       else if (u < kB) sc[0] = mfma32(at, qf[u - kA], u == kA ? f32x16{} : sc[0]);
       else sc[1] = mfma32(at, qf[u - kC], u == kC ? f32x16{} : sc[1]);
+      if (u % kBatch == 0) {  // this batch's fragments are there: the next one's
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = u + kBatch; j < u + 2 * kBatch && j < kProducts; ++j) f[j / kBatch % 2][j % kBatch] = fragment(j);
+      }
 #pragma unroll
       for (int i = weighed(u); i < weighed(u + 1); ++i) weigh(i);
       if (u >= kC) {
@@ -573,7 +602,7 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-    }
+    });
     l += sums[0] + sums[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) pf[i] = weights[i];

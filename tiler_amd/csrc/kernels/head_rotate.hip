@@ -186,6 +186,261 @@ __device__ __forceinline__ void rotate_grad_any(const TilerHeads& a, const T* dq
     partials[(uint64_t)blockIdx.x * a.head_dim + i] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 }
 
+// Heads in registers: a unit is two 16-byte pieces of a head, a lane's, and L lanes
+// hold a head (2 L pieces at least; lanes past its end idle).  In the rotated part a
+// unit is kVec pairs whichever way they lie: pieces u and u + rotary / (2 kVec), or 2 u
+// and 2 u + 1; behind it, the next two pieces.  Any alignment: memory takes unaligned
+// vectors.  A token's angles are made once, by the workgroup, into LDS.
+template <typename T, bool kNeighbours>
+struct Unit {
+  static constexpr uint32_t V = tiler_rows::kVec<T>;
+  uint32_t first, second;  // elements; second past the head where there is no second piece
+  uint32_t pair;           // the unit's first pair
+  bool rotated, there, both;
+  __device__ __forceinline__ Unit(const TilerHeads& a, uint32_t u) {
+    const uint32_t turned = a.rotary / (2u * V);
+    rotated = u < turned;
+    pair = u * V;
+    first = !rotated ? a.rotary + (u - turned) * 2u * V : kNeighbours ? 2u * u * V : u * V;
+    second = rotated && !kNeighbours ? first + a.rotary / 2u : first + V;
+    there = first < a.head_dim;
+    both = there && second < a.head_dim;
+  }
+};
+
+template <typename T>
+struct Pieces {
+  static constexpr int V = tiler_rows::kVec<T>;
+  u32x4 a, b;
+  template <typename U>
+  __device__ __forceinline__ void load(const T* head, const U& u) {
+    a = b = u32x4{0, 0, 0, 0};
+    if (u.there) a = *reinterpret_cast<const tiler_rows::u32x4_any*>(head + u.first);
+    if (u.both) b = *reinterpret_cast<const tiler_rows::u32x4_any*>(head + u.second);
+  }
+  template <typename U>
+  __device__ __forceinline__ void store(T* head, const U& u) const {
+    if (u.there) *reinterpret_cast<tiler_rows::u32x4_any*>(head + u.first) = a;
+    if (u.both) *reinterpret_cast<tiler_rows::u32x4_any*>(head + u.second) = b;
+  }
+  __device__ __forceinline__ void widen(float (&x)[2 * V]) const {
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = tiler_rows::element<T>(a, e), x[V + e] = tiler_rows::element<T>(b, e);
+  }
+  __device__ __forceinline__ void narrow(const float (&x)[2 * V]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(T) == 2) {
+        a[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((tiler::f32x2_pair{x[2 * e], x[2 * e + 1]}), tiler::bf16x2_pair));
+        b[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((tiler::f32x2_pair{x[V + 2 * e], x[V + 2 * e + 1]}), tiler::bf16x2_pair));
+      } else {
+        a[e] = __float_as_uint(x[e]);
+        b[e] = __float_as_uint(x[V + e]);
+      }
+    }
+  }
+};
+
+// The unit's pairs turned, by the angle or back.
+template <int V, bool kNeighbours>
+__device__ __forceinline__ void turn(float (&x)[2 * V], const tiler::f32x2_pair* turns, bool back) {
+  tiler::f32x2_pair cs[V];
+#pragma unroll
+  for (int e = 0; e < V; e += 2) {
+    const f32x4 two = *reinterpret_cast<const f32x4*>(turns + e);
+    cs[e] = tiler::f32x2_pair{two.x, back ? -two.y : two.y};
+    cs[e + 1] = tiler::f32x2_pair{two.z, back ? -two.w : two.w};
+  }
+  if constexpr (kNeighbours) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float i = x[2 * e], j = x[2 * e + 1];
+      x[2 * e] = __builtin_fmaf(i, cs[e].x, -(j * cs[e].y));
+      x[2 * e + 1] = __builtin_fmaf(j, cs[e].x, i * cs[e].y);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float i = x[e], j = x[V + e];
+      x[e] = __builtin_fmaf(i, cs[e].x, -(j * cs[e].y));
+      x[V + e] = __builtin_fmaf(j, cs[e].x, i * cs[e].y);
+    }
+  }
+}
+
+// Sum over groups of L lanes, in every lane of the group.
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+  auto moved = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  v += moved(v, tiler::Step<0xB1>{});                         // quad_perm [1,0,3,2]
+  v += moved(v, tiler::Step<0x4E>{});                         // quad_perm [2,3,0,1]
+  if constexpr (L >= 8) v += moved(v, tiler::Step<0x141>{});  // row_half_mirror
+  if constexpr (L >= 16) v += moved(v, tiler::Step<0x140>{}); // row_mirror
+  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  if constexpr (L >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+
+constexpr uint32_t kTurnPairs = 2048;  // angles a workgroup holds: of 8 tokens of 256 pairs, say
+
+// The workgroup's tokens are `each` at a time; its tasks, heads of them, go round the
+// groups of L lanes.  HBM bounds it: 8192 tokens of 32 and 8 heads of 128 bf16 take 28 us
+// traced (6.0 TB/s), 173 in the form of any size; their gradients 46 (5.5 TB/s) and 5 for
+// the sum of the partials, 334 in the form of any size.
+template <typename T, int L, bool kNeighbours>
+__device__ __forceinline__ void rotate_units(const TilerHeads& a, const T* __restrict__ q, const T* __restrict__ k,
+                                             const T* __restrict__ v, const T* __restrict__ wq, const T* __restrict__ wk,
+                                             const int32_t* __restrict__ positions, const double* __restrict__ frequencies,
+                                             T* __restrict__ q_out, T* __restrict__ k_out, T* __restrict__ k_cache,
+                                             T* __restrict__ v_cache, const int32_t* __restrict__ slots) {
+  constexpr int V = tiler_rows::kVec<T>;
+  constexpr uint32_t kGroups = 256 / L;
+  __shared__ __attribute__((aligned(16))) tiler::f32x2_pair turns[kTurnPairs];
+  const uint32_t group = threadIdx.x / L, pairs = a.rotary / 2u, each = a.each;
+  const uint32_t heads = a.q_heads + a.kv_heads + (v ? a.kv_heads : 0u);
+  const Unit<T, kNeighbours> unit(a, threadIdx.x % L);
+  Pieces<T> of_q, of_k;
+  if (wq) of_q.load(wq, unit);
+  if (wk) of_k.load(wk, unit);
+  for (uint64_t token0 = (uint64_t)blockIdx.x * each; token0 < a.tokens; token0 += (uint64_t)gridDim.x * each) {
+    const uint32_t count = a.tokens - token0 < each ? (uint32_t)(a.tokens - token0) : each;
+    if (token0 != (uint64_t)blockIdx.x * each) __syncthreads();  // the turns before are read
+    for (uint32_t i = threadIdx.x; i < count * pairs; i += 256u) {
+      const uint32_t t = i / pairs;
+      turns[i] = turn_of((double)positions[token0 + t] * frequencies[i - t * pairs]);
+    }
+    __syncthreads();
+    uint32_t in = group / heads, n = group - in * heads;  // the task's token, and its head
+    while (in < count) {
+      const uint64_t token = token0 + in;
+      const bool is_q = n < a.q_heads, is_k = !is_q && n < a.q_heads + a.kv_heads;
+      const uint32_t head = is_q ? n : is_k ? n - a.q_heads : n - a.q_heads - a.kv_heads;
+      Pieces<T> x;
+      x.load((is_q ? q + token * a.q_stride : is_k ? k + token * a.k_stride : v + token * a.v_stride) + (uint64_t)head * a.head_dim, unit);
+      if (is_q || is_k) {
+        float u[2 * V];
+        x.widen(u);
+        if (a.norm) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) sum = __builtin_fmaf(u[e], u[e], sum);
+          const float r = 1.0f / __builtin_sqrtf(group_sum<L>(sum) / (float)a.head_dim + a.eps);
+          const bool weighted = is_q ? wq != nullptr : wk != nullptr;
+          float w[2 * V];
+          Pieces<T> wp;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) wp.a[e] = is_q ? of_q.a[e] : of_k.a[e], wp.b[e] = is_q ? of_q.b[e] : of_k.b[e];
+          wp.widen(w);
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) u[e] = weighted ? u[e] * r * w[e] : u[e] * r;
+        }
+        if (unit.rotated) turn<V, kNeighbours>(u, turns + in * pairs + unit.pair, false);
+        x.narrow(u);
+      }
+      if (is_q) x.store(q_out + token * a.q_out_stride + (uint64_t)head * a.head_dim, unit);
+      if (is_k && k_out) x.store(k_out + token * a.k_out_stride + (uint64_t)head * a.head_dim, unit);
+      if (!is_q && slots) {
+        const int64_t slot = slots[token];
+        if (slot >= 0 && (uint64_t)slot < a.slots) {
+          const uint32_t page = (uint32_t)slot / a.page, place = (uint32_t)slot - page * a.page;
+          x.store((is_k ? k_cache : v_cache) + (uint64_t)page * a.page_stride + (uint64_t)place * a.token_stride + (uint64_t)head * a.head_stride, unit);
+        }
+      }
+      n += kGroups;
+      while (n >= heads) n -= heads, ++in;
+    }
+  }
+}
+
+// Its gradients.  The first a.q_groups workgroups have the queries' heads, the others
+// the keys'.
+template <typename T, int L, bool kNeighbours>
+__device__ __forceinline__ void rotate_grad_units(const TilerHeads& a, const T* __restrict__ dq_out, const T* __restrict__ dk_out,
+                                                  const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ wq,
+                                                  const T* __restrict__ wk, const int32_t* __restrict__ positions,
+                                                  const double* __restrict__ frequencies, T* __restrict__ dq, T* __restrict__ dk,
+                                                  float* __restrict__ partials_q, float* __restrict__ partials_k) {
+  constexpr int V = tiler_rows::kVec<T>;
+  constexpr uint32_t kGroups = 256 / L;
+  __shared__ __attribute__((aligned(16))) union {
+    tiler::f32x2_pair turns[kTurnPairs];
+    float sums[kGroups][2 * V * L];
+  } space;
+  const bool is_q = blockIdx.x < a.q_groups;
+  const uint32_t block = is_q ? blockIdx.x : blockIdx.x - a.q_groups, blocks = is_q ? a.q_groups : gridDim.x - a.q_groups;
+  const uint32_t group = threadIdx.x / L, pairs = a.rotary / 2u, each = a.each, heads = is_q ? a.q_heads : a.kv_heads;
+  const uint64_t x_stride = is_q ? a.q_stride : a.k_stride, dy_stride = is_q ? a.q_out_stride : a.k_out_stride;
+  const T *const xs = is_q ? q : k, *const dys = is_q ? dq_out : dk_out, *const w = is_q ? wq : wk;
+  T* const dxs = is_q ? dq : dk;
+  float* const partials = is_q ? partials_q : partials_k;
+  const Unit<T, kNeighbours> unit(a, threadIdx.x % L);
+  float weight[2 * V], dw[2 * V];
+  {
+    Pieces<T> of;
+    if (w) of.load(w, unit);
+    of.widen(weight);
+#pragma unroll
+    for (int e = 0; e < 2 * V; ++e) weight[e] = w ? weight[e] : 1.0f, dw[e] = 0.0f;
+  }
+  for (uint64_t token0 = (uint64_t)block * each; token0 < a.tokens; token0 += (uint64_t)blocks * each) {
+    const uint32_t count = a.tokens - token0 < each ? (uint32_t)(a.tokens - token0) : each;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count * pairs; i += 256u) {
+      const uint32_t t = i / pairs;
+      space.turns[i] = turn_of((double)positions[token0 + t] * frequencies[i - t * pairs]);
+    }
+    __syncthreads();
+    uint32_t in = group / heads, n = group - in * heads;
+    while (in < count) {
+      const uint64_t token = token0 + in;
+      Pieces<T> dy, x;
+      dy.load(dys + token * dy_stride + (uint64_t)n * a.head_dim, unit);
+      if (a.norm) x.load(xs + token * x_stride + (uint64_t)n * a.head_dim, unit);
+      float g[2 * V];
+      dy.widen(g);
+      if (unit.rotated) turn<V, kNeighbours>(g, space.turns + in * pairs + unit.pair, true);
+      if (a.norm) {
+        float e_x[2 * V], squares = 0.0f, along = 0.0f;
+        x.widen(e_x);
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) {
+          squares = __builtin_fmaf(e_x[e], e_x[e], squares);
+          along = __builtin_fmaf(g[e] * weight[e], e_x[e], along);
+        }
+        const float r = 1.0f / __builtin_sqrtf(group_sum<L>(squares) / (float)a.head_dim + a.eps);
+        const float mean = group_sum<L>(along) * r / (float)a.head_dim;
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) {
+          const float xh = e_x[e] * r;
+          dw[e] = __builtin_fmaf(g[e], xh, dw[e]);
+          g[e] = r * __builtin_fmaf(-xh, mean, g[e] * weight[e]);
+        }
+      }
+      if (dxs) {
+        dy.narrow(g);
+        dy.store(dxs + token * x_stride + (uint64_t)n * a.head_dim, unit);
+      }
+      n += kGroups;
+      while (n >= heads) n -= heads, ++in;
+    }
+  }
+  if (!partials) return;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if (unit.there) space.sums[group][unit.first + e] = dw[e];
+    if (unit.both) space.sums[group][unit.second + e] = dw[V + e];
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < a.head_dim; i += 256u) {
+    float s = 0.0f;
+    for (uint32_t n = 0; n < kGroups; ++n) s += space.sums[n][i];
+    partials[(uint64_t)block * a.head_dim + i] = s;
+  }
+}
+
 // dw from the rows of partial sums: 64 elements a workgroup, sixteen waves that
 // each add every sixteenth row.  blockIdx.y: the queries' (0) or the keys'.
 template <typename T>
@@ -232,3 +487,31 @@ __device__ __forceinline__ void rotate_sums(const float* partials_q, const float
 TILER_NORM_ROTATE(bf16, uint16_t)
 TILER_NORM_ROTATE(f32, float)
 #undef TILER_NORM_ROTATE
+
+#define TILER_NORM_ROTATE_UNITS(TY, T, L, FORM, NEIGHBOURS)                                                           \
+  extern "C" __global__ void __launch_bounds__(256) tiler_norm_rotate_##TY##_##FORM(                                  \
+      TilerHeads a, const T* q, const T* k, const T* v, const T* wq, const T* wk, const int32_t* positions,           \
+      const double* frequencies, T* q_out, T* k_out, T* k_cache, T* v_cache, const int32_t* slots) {                  \
+    tiler_heads::rotate_units<T, L, NEIGHBOURS>(a, q, k, v, wq, wk, positions, frequencies, q_out, k_out, k_cache,    \
+                                                v_cache, slots);                                                      \
+  }                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(256) tiler_norm_rotate_grad_##TY##_##FORM(                             \
+      TilerHeads a, const T* dq_out, const T* dk_out, const T* q, const T* k, const T* wq, const T* wk,               \
+      const int32_t* positions, const double* frequencies, T* dq, T* dk, float* partials_q, float* partials_k) {      \
+    tiler_heads::rotate_grad_units<T, L, NEIGHBOURS>(a, dq_out, dk_out, q, k, wq, wk, positions, frequencies, dq, dk, \
+                                                     partials_q, partials_k);                                         \
+  }
+#define TILER_NORM_ROTATE_FORMS(TY, T, L)             \
+  TILER_NORM_ROTATE_UNITS(TY, T, L, h##L, false)      \
+  TILER_NORM_ROTATE_UNITS(TY, T, L, n##L, true)
+#define TILER_NORM_ROTATE_LANES(L)          \
+  TILER_NORM_ROTATE_FORMS(bf16, uint16_t, L) \
+  TILER_NORM_ROTATE_FORMS(f32, float, L)
+TILER_NORM_ROTATE_LANES(4)
+TILER_NORM_ROTATE_LANES(8)
+TILER_NORM_ROTATE_LANES(16)
+TILER_NORM_ROTATE_LANES(32)
+TILER_NORM_ROTATE_LANES(64)
+#undef TILER_NORM_ROTATE_LANES
+#undef TILER_NORM_ROTATE_FORMS
+#undef TILER_NORM_ROTATE_UNITS

@@ -106,6 +106,23 @@ tiler_hip_status check_heads(uint32_t dtype, uint32_t parts, const tiler_hip_hea
   return TILER_HIP_OK;
 }
 
+// Lanes that hold a head in units of two 16-byte pieces (head_rotate.hip), or 0 for
+// the form of any size: where a piece would be cut, or the head passes a wave.
+uint32_t unit_lanes(uint32_t dtype, const tiler_hip_head_layout& h) {
+  const uint32_t vec = dtype == TILER_HIP_BF16 ? 8 : 4;
+  if (h.head_dim % vec || h.rotary % (2 * vec) || h.rotary / 2 > 512) return 0;
+  uint32_t lanes = 4;
+  while (lanes * 2 * vec < h.head_dim) lanes *= 2;
+  return lanes <= 64 ? lanes : 0;
+}
+
+// Tokens a workgroup takes at a time: up to four, whose angles are a good share of
+// its threads' first work, once every CU has two workgroups of them.
+uint32_t tokens_each(const Target& t, const tiler_hip_head_layout& h) {
+  const uint64_t share = h.tokens / (2ull * t.compute_units);
+  return share >= 4 ? 4 : share >= 2 ? 2 : 1;
+}
+
 }  // namespace
 
 // Slots: [kept, fresh,] [free,] [table,] starts, [lengths,] [positions, slots,]
@@ -181,9 +198,13 @@ tiler_hip_status plan_norm_rotate(const Target& t, uint32_t dtype, uint32_t part
   const uint32_t k_cache = given(cache, cached * 2, kSlotOutput), v_cache = given(cache, cached * 2, kSlotOutput);
   const uint32_t slots = given(cache, mul_sat(h.tokens, 4), kSlotInput);
   if (h.tokens == 0 || (!has_q && !has_k)) return TILER_HIP_OK;
-  const uint32_t groups = (uint32_t)(h.tokens < (1u << 20) ? h.tokens : 1u << 20);
   char name[64];
-  std::snprintf(name, sizeof(name), "tiler_norm_rotate_%s_any", type_name(dtype));
+  const uint32_t lanes = unit_lanes(dtype, h);
+  a.each = lanes ? tokens_each(t, h) : 1;
+  const uint64_t all = ceil_div(h.tokens, a.each);
+  const uint32_t groups = (uint32_t)(all < (1u << 20) ? all : 1u << 20);
+  if (lanes) std::snprintf(name, sizeof(name), "tiler_norm_rotate_%s_%c%u", type_name(dtype), a.neighbours ? 'n' : 'h', lanes);
+  else std::snprintf(name, sizeof(name), "tiler_norm_rotate_%s_any", type_name(dtype));
   Launch& l = p.add(name, groups, 1, 256).blob(&a, sizeof(a), 8);
   slot_or_null(l, has_q, q);
   slot_or_null(l, has_k, k);
@@ -232,13 +253,23 @@ tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint
   const bool sum_q = of_q && dwq && h.tokens, sum_k = of_k && dwk && h.tokens;
   uint32_t partials_q = 0, partials_k = 0;
   // each workgroup leaves one row of partial sums
-  const uint64_t most = 2ull * t.compute_units;
-  const uint32_t count = (uint32_t)(h.tokens < most ? h.tokens : most);
-  if (sum_q) partials_q = p.slot(4ull * count * h.head_dim, kSlotScratch);
-  if (sum_k) partials_k = p.slot(4ull * count * h.head_dim, kSlotScratch);
+  const uint32_t lanes = unit_lanes(dtype, h);
+  a.each = lanes ? tokens_each(t, h) : 1;
+  const uint64_t most = 4ull * t.compute_units, all = ceil_div(h.tokens, a.each);
+  uint32_t count_q = (uint32_t)(all < most / 2 ? all : most / 2), count_k = count_q;
+  if (lanes) {  // the workgroups by the heads' shares
+    const double share = of_q && of_k ? (double)h.q_heads / ((double)h.q_heads + h.kv_heads) : 1.0;
+    const uint64_t q_most = (uint64_t)(share * (double)most), k_most = of_q ? most - q_most : most;
+    count_q = of_q ? (uint32_t)(all < q_most ? all : q_most ? q_most : 1) : 0;
+    count_k = of_k ? (uint32_t)(all < k_most ? all : k_most ? k_most : 1) : 0;
+    a.q_groups = count_q;
+  }
+  if (sum_q) partials_q = p.slot(4ull * count_q * h.head_dim, kSlotScratch);
+  if (sum_k) partials_k = p.slot(4ull * count_k * h.head_dim, kSlotScratch);
   if (h.tokens && (of_q || of_k)) {
-    std::snprintf(name, sizeof(name), "tiler_norm_rotate_grad_%s_any", type_name(dtype));
-    Launch& l = p.add(name, count, 2, 256).blob(&a, sizeof(a), 8);
+    if (lanes) std::snprintf(name, sizeof(name), "tiler_norm_rotate_grad_%s_%c%u", type_name(dtype), a.neighbours ? 'n' : 'h', lanes);
+    else std::snprintf(name, sizeof(name), "tiler_norm_rotate_grad_%s_any", type_name(dtype));
+    Launch& l = (lanes ? p.add(name, count_q + count_k, 1, 256) : p.add(name, count_q, 2, 256)).blob(&a, sizeof(a), 8);
     slot_or_null(l, of_q, dq_out);
     slot_or_null(l, of_k, dk_out);
     slot_or_null(l, of_q && a.norm, q);
@@ -257,7 +288,7 @@ tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint
     Launch& l = p.add(name, (uint32_t)ceil_div(h.head_dim, 64), 2, 1024);
     slot_or_null(l, sum_q, partials_q);
     slot_or_null(l, sum_k, partials_k);
-    l.u32(sum_q ? count : 0).u32(sum_k ? count : 0).u32(h.head_dim);
+    l.u32(sum_q ? count_q : 0).u32(sum_k ? count_k : 0).u32(h.head_dim);
     slot_or_null(l, dwq, at_dwq);
     slot_or_null(l, dwk, at_dwk);
   }

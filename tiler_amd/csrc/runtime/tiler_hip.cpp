@@ -410,6 +410,15 @@ const EntryRow kEntries[] = {
     {"tiler_norm_rotate_grad_f32_any", "norm-rotate-backward-f32", 12},
     {"tiler_norm_rotate_sum_bf16", "norm-rotate-backward/bf16", 4},
     {"tiler_norm_rotate_sum_f32", "norm-rotate-backward-f32", 4},
+#define TILER_ROTATE_FORM(FORM)                                          \
+  {"tiler_norm_rotate_bf16_" FORM, "norm-rotate/bf16", 12},               \
+      {"tiler_norm_rotate_f32_" FORM, "norm-rotate-f32", 12},             \
+      {"tiler_norm_rotate_grad_bf16_" FORM, "norm-rotate-backward/bf16", 12}, \
+      {"tiler_norm_rotate_grad_f32_" FORM, "norm-rotate-backward-f32", 12}
+    TILER_ROTATE_FORM("h4"), TILER_ROTATE_FORM("h8"), TILER_ROTATE_FORM("h16"), TILER_ROTATE_FORM("h32"),
+    TILER_ROTATE_FORM("h64"), TILER_ROTATE_FORM("n4"), TILER_ROTATE_FORM("n8"), TILER_ROTATE_FORM("n16"),
+    TILER_ROTATE_FORM("n32"), TILER_ROTATE_FORM("n64"),
+#undef TILER_ROTATE_FORM
     {"tiler_paged_attention_bf16_few64", "paged-attention-bf16", 9},
     {"tiler_paged_attention_bf16_few128", "paged-attention-bf16", 9},
     {"tiler_paged_attention_bf16_few256", "paged-attention-bf16", 9},
