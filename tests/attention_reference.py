@@ -104,38 +104,52 @@ def paged_attention(q, k, v, table, starts, lengths, scale, window, sinks, out):
     """(out, bound): q [tokens, heads, dim], k and v [pages, page, kv_heads, dim] in
     64 bits; rows of no sequence keep what `out` holds, with a bound of 0.
 
-    bound: the weights are rounded to bf16 for the product with v (U16 of sum w |v|),
-    the result to bf16 (U16 of itself); a logit of dim products is off by dim / 16
-    + 16 roundings at most in each of the matrix unit's running sums, taken as dim,
-    on scale * sum |q k|, twice that where it enters the weight and the weights'
-    sum; the sums over the keys (chains of at most keys / 16 + 32 steps, with their
-    rescaling) and the exponential add the rest."""
+    bound: the weights w_j are rounded to bf16, for the product with v and for their
+    sum alike: sum w_j (1 + e_j) v_j / sum w_j (1 + e_j) is off by sum w_j e_j (v_j -
+    out) / (1 - U16), at most U16 (1 + 2 U16) sum w |v - out|; the result to bf16 (U16
+    of itself); a logit of dim products is off by dim / 16 + 16 roundings at most in
+    each of the matrix unit's running sums, taken as dim, on scale * sum |q k|, twice
+    that where it enters the weight and the weights' sum; the sums over the keys
+    (chains of at most keys / 16 + 32 steps, with their rescaling) and the exponential
+    add the rest."""
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
     out, bound = np.array(out, np.float64), np.zeros(np.shape(out))
     pages, page, kv_heads, dim = k.shape
     group = q.shape[1] // kv_heads
     for s in range(len(lengths)):
-        fresh = starts[s + 1] - starts[s]
-        for i in range(fresh):
-            p, row = lengths[s] - fresh + i, starts[s] + i
-            j = np.arange(max(min(p + 1, table.shape[1] * page), 0))
-            if window:
-                j = j[(j > p - window) | (j < sinks)]
-            entry = table[s, j // page] if len(j) else j
-            there = (entry >= 0) & (entry < pages)
-            at = np.where(there, entry, 0)
-            for h in range(q.shape[1]):
-                kk = np.where(there[:, None], k[at, j % page, h // group], 0.0) if len(j) else np.zeros((0, dim))
-                vv = np.where(there[:, None], v[at, j % page, h // group], 0.0) if len(j) else np.zeros((0, dim))
-                logits = scale * (kk @ q[row, h])
-                if not len(j) or logits.max() == -np.inf:
-                    out[row, h] = 0.0
+        fresh = int(starts[s + 1] - starts[s])
+        most = max(min(int(lengths[s]), table.shape[1] * page), 0)
+        keys = np.arange(most)
+        entry = table[s, keys // page] if most else keys
+        there = (entry >= 0) & (entry < pages)
+        at = np.where(there, entry, 0)
+        for h in range(kv_heads):
+            kk = np.where(there[:, None], k[at, keys % page, h], 0.0) if most else np.zeros((0, dim))
+            vv = np.where(there[:, None], v[at, keys % page, h], 0.0) if most else np.zeros((0, dim))
+            for i in range(fresh):
+                p, row = int(lengths[s]) - fresh + i, starts[s] + i
+                j = keys[:max(p + 1, 0)]
+                if window:
+                    j = j[(j > p - window) | (j < sinks)]
+                rows = (row, slice(h * group, (h + 1) * group))
+                if not len(j):
+                    out[rows] = 0.0
                     continue
-                w = np.exp(logits - logits.max())
-                w /= w.sum()
-                out[row, h] = w @ vv
-                sizes = w @ np.abs(vv)
-                off = scale * (np.abs(kk) @ np.abs(q[row, h])).max()
-                bound[row, h] = (U16 * (np.abs(out[row, h]) * (1 + U16) + sizes)
-                                 + U32 * (2 * (dim + 16) * off + len(j) / 8 + 96) * sizes)
+                of_j = slice(0, len(j)) if len(j) == j[-1] + 1 else j  # no copy where nothing is left out
+                kj, vj = kk[of_j], vv[of_j]
+                logits = scale * (q[rows] @ kj.T)
+                top = logits.max(1, keepdims=True)
+                w = np.exp(logits - np.where(top == -np.inf, 0.0, top))
+                total = w.sum(1, keepdims=True)
+                w /= np.where(total == 0.0, 1.0, total)
+                o = w @ vj
+                sizes = w @ np.abs(vj)
+                # sum w |v - out| by Cauchy's inequality: no term for each key, element and row
+                spread = np.sqrt(np.maximum(w @ (vj * vj) - o * o * (2 - w.sum(1, keepdims=True)), 0.0))
+                off = scale * (np.abs(q[rows]) @ np.abs(kj).T).max(1, keepdims=True)
+                out[rows] = o
+                bound[rows] = (U16 * (np.abs(o) * (1 + U16) + (1 + 2 * U16) * np.minimum(spread, sizes + np.abs(o)))
+                               + U32 * (2 * (dim + 16) * off + len(j) / 8 + 96) * sizes)
+                dead = np.nonzero(total[:, 0] == 0.0)[0]  # every logit -infinity
+                out[row, h * group + dead], bound[row, h * group + dead] = 0.0, 0.0
     return out, bound

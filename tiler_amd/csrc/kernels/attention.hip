@@ -9,7 +9,8 @@
 // exchange across lanes a step, and its weights are, as they lie, the right
 // operand of O^T = V^T P^T: the matrix unit sums over the keys in whatever order
 // both operands name them.  The weights are rounded to bf16, the matrix unit's
-// operand type; their sum is taken before that, in binary32.
+// operand type; their sum, in binary32, is of the rounded ones, so that the
+// rounding errors of equal weights cancel.
 //
 // The query heads that share a key/value head are rows of one tile (row =
 // token * group + head of the group), so the cache is read once for all.
@@ -25,7 +26,6 @@
 #include "row_pieces.h"
 
 namespace tiler_attention {
-
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -139,29 +139,32 @@ __device__ __forceinline__ uint32_t value_piece(uint32_t key, uint32_t piece) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: a tile of 16 rows, four waves that each take every fourth step of
-// 32 keys on their own (keys to registers, values to LDS, one step ahead), and a
-// join of the waves at the end.  A decode step is bound by the cache's bytes.
-template <int NC>
+// Few rows: a tile of 16 rows, four waves that take the steps of 32 keys in turn,
+// each on its own (keys to registers, values to LDS, one step ahead of the
+// products, no barrier), and a join of the waves at the end.  A decode step is
+// bound by the cache's bytes, a short one by the way to the first of them.
+template <int NC, int WAVES>
 struct FewSpace {
   static constexpr int D = 32 * NC;
-  static constexpr uint32_t kRow = D * 2, kStage = 32 * kRow, kWaves = 4;
+  static constexpr uint32_t kRow = D * 2, kStage = 32 * kRow;
   union {
-    uint8_t stage[kWaves][2][kStage];
-    struct {
-      float o[kWaves][16][D + 4];
-    } join;
+    uint8_t stage[WAVES][2][kStage];
+    float o[WAVES][16][D + 4];
   };
-  float m[kWaves][16], l[kWaves][16];
+  float m[WAVES][16], l[WAVES][16];
 };
 
-template <int NC>
-__device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t* __restrict__ q, const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
-                                    const int32_t* __restrict__ table, const int32_t* __restrict__ starts, const int32_t* __restrict__ lengths, uint16_t* __restrict__ out,
-                                    float* __restrict__ part_o, tiler::f32x2_pair* __restrict__ part_ml, FewSpace<NC>& space) {
-  using Space = FewSpace<NC>;
+template <int NC, int WAVES>
+__device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t* __restrict__ q, const uint8_t* __restrict__ k,
+                                    const uint8_t* __restrict__ v, const int32_t* __restrict__ table,
+                                    const int32_t* __restrict__ starts, const int32_t* __restrict__ lengths,
+                                    uint16_t* __restrict__ out, float* __restrict__ part_o,
+                                    tiler::f32x2_pair* __restrict__ part_ml, FewSpace<NC, WAVES>& space) {
+  using Space = FewSpace<NC, WAVES>;
   constexpr int D = Space::D, NB = 2 * NC;  // blocks of 16 elements
-  constexpr uint32_t kPieces = D / 8;
+  constexpr uint32_t kPieces = D / 8, kValueLoads = Space::kStage / 1024u;
+  constexpr int kLoads = kValueLoads + 2 * NC + 1;  // of a step, with the next one's entry
+  static_assert(kLoads < 64, "a step's loads fit the wait counter");
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t col = lane & 15u, g = lane >> 4;
   const uint32_t split = blockIdx.x / a.kv_heads % a.splits, head = blockIdx.x % a.kv_heads;
@@ -170,6 +173,7 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
   const uint32_t rows = seq.fresh * a.group;
   const int32_t* const pages = table + (uint64_t)s * a.width;
   const uint32_t real_pieces = a.head_dim / 8u;
+  const uint64_t zero = zero_row();
   for (uint32_t row0 = 0; row0 < rows; row0 += 16u) {
     const uint32_t row = row0 + col, last = row0 + 15u < rows - 1u ? row0 + 15u : rows - 1u;
     const uint32_t token = divide(a.groups, row < rows ? row : rows - 1u);
@@ -177,30 +181,16 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
     const int32_t p = seq.kept + (int32_t)token;
     const int32_t p_first = seq.kept + (int32_t)divide(a.groups, row0), p_last = seq.kept + (int32_t)divide(a.groups, last);
     const Keys<32> keys(a, p_first, p_last);
-    u32x4 qf[NC];
-    {
-      const uint16_t* at = q + (uint64_t)(seq.first + token) * a.q_stride + (uint64_t)(head * a.group + in_group) * a.head_dim;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        qf[c] = 4u * c + g < real_pieces ? *reinterpret_cast<const u32x4_any*>(at + 32 * c + 8 * g) : u32x4{0, 0, 0, 0};
-    }
-    const uint32_t begin = (uint32_t)((uint64_t)keys.steps * split / a.splits);
+    const uint32_t begin = (uint32_t)((uint64_t)keys.steps * split / a.splits) + wave;
     const uint32_t end = (uint32_t)((uint64_t)keys.steps * (split + 1u) / a.splits);
-    f32x4 o[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) o[i] = f32x4{0, 0, 0, 0};
-    float m = kHidden, l = 0.0f;
-    u32x4 kf[2][NC];
     const Sight sight(a, keys.high, p);
     const int32_t sinks = a.sinks < 0x7fffffffu ? (int32_t)a.sinks : 0x7fffffff;
-    const uint64_t zero = zero_row();
-    int32_t entry = -1;
     auto look_up = [&](uint32_t t) {
       const uint32_t key = keys.base(t) + (lane & 31u);
-      entry = pages[((t < end) & keys.read(key)) ? divide(a.page, key) : 0u];
+      return pages[((t < end) & keys.read(key)) ? divide(a.page, key) : 0u];
     };
-    // Step t's keys into kf, its values on their way to the stage.
-    auto request = [&](uint32_t t, uint32_t stage) {
+    // Step t's values on their way to the stage, its keys to kf.
+    auto request = [&](uint32_t t, int32_t entry, uint8_t* stage, u32x4 (&kf)[2][NC]) {
       const uint32_t key = keys.base(t) + (lane & 31u);
       const int64_t off = row_offset(a, keys.read(key), entry, key, head);
       auto of = [&](uint32_t r) {  // row r's offset
@@ -209,10 +199,10 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
         return (int64_t)((uint64_t)hi << 32 | lo);
       };
 #pragma unroll
-      for (uint32_t i = 0; i < Space::kStage / 1024u; ++i) {
+      for (uint32_t i = 0; i < kValueLoads; ++i) {
         const uint32_t id = i * 64u + lane, r = id / kPieces, piece = value_piece<D>(r, id % kPieces);
         const int64_t at = of(r);
-        load_to_lds(at >= 0 && piece < real_pieces ? (uint64_t)v + at + piece * 16u : zero, space.stage[wave][stage] + i * 1024u);
+        load_to_lds(at >= 0 && piece < real_pieces ? (uint64_t)v + at + piece * 16u : zero, stage + i * 1024u);
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -224,13 +214,37 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
         }
       }
     };
-    for (uint32_t t = begin + wave; t < end; t += Space::kWaves) {
-      look_up(t);
-      __builtin_amdgcn_s_waitcnt(kWaitLds);  // the stage is read
-      asm volatile("" ::: "memory");
-      request(t, 0);
-      __builtin_amdgcn_s_waitcnt(kWaitLoads);
-      asm volatile("" ::: "memory");
+    u32x4 even[2][NC], odd[2][NC], qf[NC];
+    int32_t entry = -1;
+    if (begin < end) {
+      entry = look_up(begin);
+      const int32_t next = look_up(begin + WAVES);
+      request(begin, entry, space.stage[wave][0], even);
+      entry = next;
+    }
+    {
+      const uint16_t* at = q + (uint64_t)(seq.first + token) * a.q_stride + (uint64_t)(head * a.group + in_group) * a.head_dim;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        qf[c] = 4u * c + g < real_pieces ? *reinterpret_cast<const u32x4_any*>(at + 32 * c + 8 * g) : u32x4{0, 0, 0, 0};
+    }
+    f32x4 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o[i] = f32x4{0, 0, 0, 0};
+    float m = kHidden, l = 0.0f;
+    // Step t with the keys in kf, the next one's into next.
+    auto step = [&](uint32_t t, uint32_t at, const u32x4 (&kf)[2][NC], u32x4 (&next)[2][NC]) {
+      if (t + WAVES < end) {
+        __builtin_amdgcn_s_waitcnt(kWaitLds);  // the stage is read
+        asm volatile("" ::: "memory");
+        request(t + WAVES, entry, space.stage[wave][at ^ 1u], next);
+        entry = look_up(t + 2 * WAVES);
+        asm volatile("" ::: "memory");  // all of them requested: the wait counts them
+        __builtin_amdgcn_s_waitcnt((kLoads & 15) | (kLoads >> 4) << 14 | 0x0F70);
+      } else {
+        __builtin_amdgcn_s_waitcnt(kWaitLoads);
+      }
+      asm volatile("" ::: "memory");  // step t's values have landed
       f32x4 sc[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -262,12 +276,12 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
         float w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[r] = exp2_fast(__builtin_fmaf(sc[b][r], a.scale, shift));
-        sum += (w[0] + w[1]) + (w[2] + w[3]);
         pf[2 * b] = narrow2(w[0], w[1]);
         pf[2 * b + 1] = narrow2(w[2], w[3]);
+        sum = add_pair(pf[2 * b + 1], add_pair(pf[2 * b], sum));
       }
       l = __builtin_fmaf(l, alpha, sum);
-      const uint8_t* const stage = space.stage[wave][0];
+      const uint8_t* const stage = space.stage[wave][at];
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         o[i] *= alpha;
@@ -275,33 +289,37 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const uint32_t key = 16u * b + 4u * g + (col >> 2);
-          const uint8_t* at = stage + key * Space::kRow + value_piece<D>(key, 2u * i + ((col & 3u) >> 1)) * 16u + (col & 1u) * 8u;
-          h[b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+          const uint8_t* from = stage + key * Space::kRow + value_piece<D>(key, 2u * i + ((col & 3u) >> 1)) * 16u + (col & 1u) * 8u;
+          h[b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)from));
         }
         o[i] = mfma16(u32x4{h[0].x, h[0].y, h[1].x, h[1].y}, pf, o[i]);
       }
+    };
+    for (uint32_t t = begin; t < end; t += 2 * WAVES) {
+      step(t, 0, even, odd);
+      if (t + WAVES < end) step(t + WAVES, 1, odd, even);
     }
-    // the four lanes of a row hold its sum in parts, the four waves its keys
+    // the four lanes of a row hold its sum in parts, the waves its keys
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     __syncthreads();  // the stages are read
     if (g == 0) space.m[wave][col] = m, space.l[wave][col] = l;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4*>(&space.join.o[wave][col][16 * i + 4 * g]) = o[i];
+    for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4*>(&space.o[wave][col][16 * i + 4 * g]) = o[i];
     __syncthreads();
-    for (uint32_t id = threadIdx.x; id < 16u * (D / 4); id += 256u) {
+    for (uint32_t id = threadIdx.x; id < 16u * (D / 4); id += 64u * WAVES) {
       const uint32_t r = id / (D / 4), d = id % (D / 4) * 4u, flat = row0 + r;
       if (flat >= rows || d >= a.head_dim) continue;
       float top = kHidden, total = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, space.m[w][r]);
+      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, space.m[w][r]);
       const float shift = top == kHidden ? 0.0f : -top * a.scale;
       f32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float weight = exp2_fast(__builtin_fmaf(space.m[w][r], a.scale, shift));
         total += weight * space.l[w][r];
-        sum += weight * *reinterpret_cast<const f32x4*>(&space.join.o[w][r][d]);
+        sum += weight * *reinterpret_cast<const f32x4*>(&space.o[w][r][d]);
       }
       const uint32_t t = divide(a.groups, flat), h = head * a.group + (flat - t * a.group);
       const uint64_t token_row = seq.first + t;
@@ -467,6 +485,7 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
     request(r, values_from, value_in, to + (2u + buffer) * TileSpace<NS>::kOperand);
   };
   auto landed = [&] {  // everything this wave requested; behind the barrier, every wave's
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(kWaitAll);
     asm volatile("s_barrier" ::: "memory");
   };
@@ -691,52 +710,57 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   }
 }
 
-// A row's splits joined, in order: a wave a row.
-__device__ __forceinline__ void join(const TilerAttentionShape& a, const int32_t* starts, const float* part_o,
-                                     const tiler::f32x2_pair* part_ml, uint16_t* out) {
-  const uint32_t lane = threadIdx.x & 63u, heads = a.kv_heads * a.group;
+// The parts of the keys joined, in order, four elements of a row a thread.
+__device__ __forceinline__ void join(const TilerAttentionShape& a, const int32_t* __restrict__ starts,
+                                     const float* __restrict__ part_o, const tiler::f32x2_pair* __restrict__ part_ml,
+                                     uint16_t* __restrict__ out) {
+  const uint32_t heads = a.kv_heads * a.group, quads = a.head_dim / 4u;
   const int32_t said = starts[a.sequences];
-  const uint64_t tokens = said < 0 ? 0u : (uint32_t)said < a.tokens ? (uint32_t)said : a.tokens;
-  for (uint64_t row = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6); row < tokens * heads; row += (uint64_t)gridDim.x * 4u) {
-    const tiler::f32x2_pair* ml = part_ml + row * a.splits;
+  const uint32_t tokens = said < 0 ? 0u : (uint32_t)said < a.tokens ? (uint32_t)said : a.tokens;
+  const uint64_t all = (uint64_t)tokens * heads * quads;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
+    const uint32_t row = (uint32_t)(i / quads), d = (uint32_t)(i - (uint64_t)row * quads) * 4u;
+    const tiler::f32x2_pair* ml = part_ml + (uint64_t)row * a.splits;
+    const float* const from = part_o + (uint64_t)row * a.splits * a.head_dim + d;
     float top = kHidden, total = 0.0f;
+#pragma unroll 4
     for (uint32_t z = 0; z < a.splits; ++z) top = fmaxf(top, ml[z].x);
     const float shift = top == kHidden ? 0.0f : -top * a.scale;
-    for (uint32_t z = 0; z < a.splits; ++z) total += exp2_fast(__builtin_fmaf(ml[z].x, a.scale, shift)) * ml[z].y;
-    const float by = total == 0.0f ? 0.0f : 1.0f / total;
-    const uint64_t token = row / heads, h = row % heads;
-    for (uint32_t d = lane * 4u; d < a.head_dim; d += 256u) {
-      f32x4 sum = {0, 0, 0, 0};
-      for (uint32_t z = 0; z < a.splits; ++z) {
-        const float weight = exp2_fast(__builtin_fmaf(ml[z].x, a.scale, shift));
-        sum += weight * *reinterpret_cast<const f32x4*>(part_o + (row * a.splits + z) * a.head_dim + d);
-      }
-      u32x2 y = {narrow2(sum[0] * by, sum[1] * by), narrow2(sum[2] * by, sum[3] * by)};
-      *reinterpret_cast<u32x2_any*>(out + token * a.out_stride + h * a.head_dim + d) = y;
+    f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t z = 0; z < a.splits; ++z) {
+      const tiler::f32x2_pair at = ml[z];
+      const float weight = exp2_fast(__builtin_fmaf(at.x, a.scale, shift));
+      total += weight * at.y;
+      sum += weight * __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(from + z * a.head_dim));
     }
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    const uint32_t token = row / heads, h = row - token * heads;
+    const u32x2 y = {narrow2(sum[0] * by, sum[1] * by), narrow2(sum[2] * by, sum[3] * by)};
+    *reinterpret_cast<u32x2_any*>(out + (uint64_t)token * a.out_stride + (uint64_t)h * a.head_dim + d) = y;
   }
 }
 
 }  // namespace tiler_attention
 
-#define TILER_ATTENTION_FEW(NAME, NC)                                                                               \
-  extern "C" __global__ void __launch_bounds__(256) NAME(                                                           \
+#define TILER_ATTENTION_FEW(NAME, NC, WAVES)                                                                        \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(                                                    \
       TilerAttentionShape a, const uint16_t* q, const uint8_t* k, const uint8_t* v, const int32_t* table,           \
-      const int32_t* starts, const int32_t* lengths, uint16_t* out, float* part_o, tiler::f32x2_pair* part_ml) {              \
-    __shared__ __attribute__((aligned(16))) tiler_attention::FewSpace<NC> space;                                    \
-    tiler_attention::few<NC>(a, q, k, v, table, starts, lengths, out, part_o, part_ml, space);                      \
+      const int32_t* starts, const int32_t* lengths, uint16_t* out, float* part_o, tiler::f32x2_pair* part_ml) {    \
+    __shared__ __attribute__((aligned(16))) tiler_attention::FewSpace<NC, WAVES> space;                             \
+    tiler_attention::few<NC, WAVES>(a, q, k, v, table, starts, lengths, out, part_o, part_ml, space);               \
   }
-TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few64, 2)
-TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few128, 4)
-TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few256, 8)
+TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few64, 2, 4)
+TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few128, 4, 4)
+TILER_ATTENTION_FEW(tiler_paged_attention_bf16_few256, 8, 4)
 #undef TILER_ATTENTION_FEW
 
 #define TILER_ATTENTION_TILE(NAME, NS, WAVES, EACH)                                                                 \
-  extern "C" __global__ void __launch_bounds__(64 * WAVES, EACH) NAME(                                                    \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, EACH) NAME(                                              \
       TilerAttentionShape a, const uint16_t* q, const uint8_t* k, const uint8_t* v, const int32_t* table,           \
       const int32_t* starts, const int32_t* lengths, uint16_t* out, float* part_o, tiler::f32x2_pair* part_ml) {    \
     __shared__ __attribute__((aligned(16))) tiler_attention::TileSpace<NS> space;                                   \
-    tiler_attention::tile<NS, WAVES>(a, q, k, v, table, starts, lengths, out, part_o, part_ml, space);                 \
+    tiler_attention::tile<NS, WAVES>(a, q, k, v, table, starts, lengths, out, part_o, part_ml, space);              \
   }
 TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t128_d64, 2, 4, 2)
 TILER_ATTENTION_TILE(tiler_paged_attention_bf16_t128_d96, 3, 4, 2)

@@ -295,6 +295,67 @@ tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint
   return TILER_HIP_OK;
 }
 
+namespace {
+
+// A form of the attention's tiles: rows, the head size it is built for, the tiles of
+// a batch (at most: each sequence's last one may be cut) and the parts of the keys.
+struct AttentionForm {
+  uint32_t rows, dim;
+  uint64_t tiles, splits;
+};
+
+// us a step of 64 keys takes where a CU has one workgroup, and where it has two
+// (128 rows; LDS holds one from heads of more than 128 on), or eight waves of 256 rows:
+// 512, 4096 and 8192 rows a head over 8000 keys and more, pages of 64.
+struct StepTime {
+  uint32_t dim;
+  double one, two, eight_alone, eight;
+};
+constexpr StepTime kStepTimes[] = {
+    {64, 0.93, 1.30, 1.10, 1.25}, {96, 1.10, 1.66, 1.33, 1.45}, {128, 1.25, 2.00, 1.55, 1.80},
+    {192, 2.05, 0, 0, 0},         {256, 2.70, 0, 0, 0},
+};
+
+AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequences, uint64_t fresh, uint32_t heads,
+                               uint32_t group, uint32_t head_dim, uint64_t longest) {
+  const uint64_t cus = t.compute_units, rows = tokens * group;
+  if (fresh * group <= 16) {
+    // Two workgroups to a CU, 256 keys at least to a part: us, 16 sequences of up to 1000
+    // keys, 8 heads, whole / in two / four / eight parts 18.9 / 16.6 / 14.3 / 15.8; 8 of up
+    // to 32000, in four / eight / sixteen 165 / 148 / 151.
+    uint64_t splits = ceil_div(2 * cus, mul_sat(sequences, heads));
+    if (splits > ceil_div(longest, 256)) splits = ceil_div(longest, 256);
+    return {16, head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u, sequences, splits ? splits : 1};
+  }
+  // The least of an estimate: the steps of a part (and four for its start and end) in
+  // as many rounds as the workgroups take, the parts' results written and joined.  us,
+  // 512 tokens of 32 and 8 heads of 128 over 8512 keys: 128 rows whole 169, in two / three /
+  // four / six parts 96 / 93 / 85 / 94; 256 rows in four 81.  Two prompts of 4096 tokens: 256
+  // rows 282, 128 rows 293.
+  const StepTime* c = kStepTimes;
+  while (c->dim < head_dim) ++c;
+  AttentionForm best{};
+  double least = 0;
+  for (const uint32_t tile : {128u, 256u}) {
+    if (tile == 256 && head_dim > 128) continue;
+    const double one = tile == 256 ? c->eight_alone : c->one, two = tile == 256 ? c->eight : c->two > 0 ? c->two : c->one;
+    const double slots = (double)cus * (tile == 128 && c->two > 0 ? 2 : 1);
+    const double work = ((double)ceil_div(rows, tile) + 0.5 * (double)(sequences - 1)) * heads;
+    const double steps = (double)ceil_div(longest, 64) + tile / 64.0 / group;
+    for (uint64_t splits = 1; splits <= 16 && (splits == 1 || longest >= 256 * splits); ++splits) {
+      const double groups = work * (double)splits, rounds = groups / slots;
+      double us = rounds > 2 ? (rounds + 0.3) * two : std::floor(rounds) * two;
+      if (const double rest = groups - std::floor(rounds) * slots; rounds <= 2 && rest > 0) us += rest <= (double)cus ? one : two;
+      us *= steps / (double)splits + 4;
+      if (splits > 1) us += 5 + (double)rows * heads * (double)splits * head_dim * 1.2e-6;
+      if (!best.rows || us < least) best = {tile, c->dim, rows / tile + sequences, splits}, least = us;
+    }
+  }
+  return best;
+}
+
+}  // namespace
+
 // Slots: q, k, v, [table,] starts, lengths, out, [partial results, their maxima
 // and sums: scratch].
 tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_attention_shape& a,
@@ -321,10 +382,13 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   const uint32_t starts = p.slot(4 * (a.sequences + 1), kSlotInput), lengths = p.slot(4 * a.sequences, kSlotInput);
   const uint32_t out = p.slot(2 * span(a.tokens, a.out_stride, row), kSlotOutput);
   if (a.sequences == 0 || a.tokens == 0) return TILER_HIP_OK;
+  // an axis of one has no stride; a page's tokens are stepped through by it all the same
+  const uint64_t page_stride = cache.pages > 1 ? cache.page_stride : 0, head_stride = cache.heads > 1 ? cache.head_stride : 0;
+  const uint64_t token_stride = cache.page > 1 ? cache.token_stride : 8;
   // the kernels' offsets inside the cache: 32 bits times 32 bits, and 32 inside a page
-  if ((cache.pages > 1 && cache.page_stride > 0xffffffffull) || mul_sat(cache.page, cache.token_stride) > 0xffffffffull)
+  if (page_stride > 0xffffffffull || mul_sat(cache.page, token_stride) > 0xffffffffull)
     return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: a page of 2^32 elements and more");
-  if ((cache.page_stride | cache.token_stride | cache.head_stride) % 8 || !aligned16(addr[k]) || !aligned16(addr[v]))
+  if ((page_stride | token_stride | head_stride) % 8 || !aligned16(addr[k]) || !aligned16(addr[v]))
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "the cache's rows start on 16 bytes");
   TilerAttentionShape s{};
   s.tokens = (uint32_t)a.tokens;
@@ -341,26 +405,15 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   s.groups = divisor_of(s.group);
   s.q_stride = a.q_stride;
   s.out_stride = a.out_stride;
-  s.page_stride = (uint32_t)cache.page_stride;
-  s.token_stride = (uint32_t)cache.token_stride;
-  s.head_stride = cache.head_stride;
+  s.page_stride = (uint32_t)page_stride;
+  s.token_stride = (uint32_t)token_stride;
+  s.head_stride = head_stride;
   const uint64_t room = a.table_width * cache.page;
   uint64_t longest = a.max_length && a.max_length < room ? a.max_length : room;
   if (a.window && longest > (uint64_t)a.window + a.sinks) longest = (uint64_t)a.window + a.sinks;
   const uint64_t fresh = a.max_fresh && a.max_fresh < a.tokens ? a.max_fresh : a.tokens;
-  const uint32_t dim = s.head_dim;
-  uint64_t tile_rows = 16;
-  if (fresh * s.group > 16) {
-    tile_rows = 128;
-    // 256 rows (eight waves share the keys) where such tiles are two to a CU
-    if (dim <= 128 && mul_sat(a.tokens * s.group / 256, s.kv_heads) >= 2ull * t.compute_units) tile_rows = 256;
-  }
-  // split the keys where the tiles would leave CUs idle, 512 keys at least to a part
-  const uint64_t tiles = tile_rows == 16 ? a.sequences : a.tokens * s.group / tile_rows + a.sequences;
-  const uint64_t alone = mul_sat(tiles, s.kv_heads);
-  uint64_t splits = ceil_div(2ull * t.compute_units, alone);
-  if (splits > ceil_div(longest, 512)) splits = ceil_div(longest, 512);
-  if (splits < 1) splits = 1;
+  const AttentionForm f = choose_attention(t, a.tokens, a.sequences, fresh, cache.heads, s.group, s.head_dim, longest);
+  const uint64_t splits = f.splits, alone = mul_sat(f.tiles, s.kv_heads);
   s.splits = (uint32_t)splits;
   if (mul_sat(alone, splits) > 0xffffffffull / 512)
     return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: more workgroups than a launch holds");
@@ -368,20 +421,16 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   const uint32_t part = splits > 1 ? p.slot(4 * mul_sat(rows * splits, s.head_dim), kSlotScratch) : 0;
   const uint32_t ml = splits > 1 ? p.slot(8 * rows * splits, kSlotScratch) : 0;
   char name[64];
-  if (tile_rows == 16)
-    std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_few%u", dim <= 64 ? 64 : dim <= 128 ? 128 : 256);
-  else
-    std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_t%u_d%u", (uint32_t)tile_rows,
-                  dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256);
-  const uint32_t block = tile_rows == 256 ? 512 : 256;
-  Launch& l = p.add(name, (uint32_t)(alone * splits), 1, block).blob(&s, sizeof(s), 8).ptr(q).ptr(k).ptr(v);
+  if (f.rows == 16) std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_few%u", f.dim);
+  else std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_t%u_d%u", f.rows, f.dim);
+  Launch& l = p.add(name, (uint32_t)(alone * splits), 1, f.rows == 256 ? 512 : 256).blob(&s, sizeof(s), 8).ptr(q).ptr(k).ptr(v);
   slot_or_null(l, table, at);
   l.ptr(starts).ptr(lengths).ptr(out);
   slot_or_null(l, splits > 1, part);
   slot_or_null(l, splits > 1, ml);
   if (splits > 1) {
-    const uint64_t groups = ceil_div(rows, 4);
-    p.add("tiler_paged_attention_bf16_join", (uint32_t)(groups < 8192 ? groups : 8192), 1, 256)
+    const uint64_t groups = ceil_div(rows * (s.head_dim / 4), 256);
+    p.add("tiler_paged_attention_bf16_join", (uint32_t)(groups < 16384 ? groups : 16384), 1, 256)
         .blob(&s, sizeof(s), 8).ptr(starts).ptr(part).ptr(ml).ptr(out);
   }
   return TILER_HIP_OK;
