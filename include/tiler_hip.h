@@ -877,7 +877,8 @@ tiler_hip_status tiler_hip_contract_i8(tiler_hip_context *ctx, const int8_t *a, 
  * head h starts at element n * page_stride + t * token_stride + h * head_stride
  * of k and of v (bf16, head_dim elements).  Slot n * page + t names the token; at
  * most 2^31 - 1 slots.  Any strides under which no two rows overlap: [pages, page,
- * heads, head_dim] and [pages, heads, page, head_dim] are the usual ones. */
+ * heads, head_dim] and [pages, heads, page, head_dim] are the usual ones;
+ * an axis of one has no stride (any value). */
 typedef struct {
     void *k;
     void *v;
@@ -991,7 +992,7 @@ typedef struct {
  * j < sinks:
  *   out = sum_j e^(scale q k_j) v_j / sum_j e^(scale q k_j)
  * q, out bf16 [tokens, q_heads, head_dim]; sums, maxima and the softmax in binary32,
- * its weights rounded to bf16 for the product with v.  Token j of sequence s lies
+ * its weights rounded to bf16 for the product with v and their sum alike.  Token j of sequence s lies
  * in page table[s][j / page]; an entry that names no page of the cache reads as
  * zeros, and keys past the table's width are not seen.  A row that sees no key, or
  * none with a logit above -infinity, is zeros.  Rows behind starts[sequences] are
@@ -1000,7 +1001,9 @@ typedef struct {
  * (no row reads what none of its tile's sees).  starts and lengths out of order or
  * range touch nothing outside the operands.
  * head_dim a multiple of 8 up to 256; the cache's rows start on 16 bytes
- * (TILER_HIP_REFUSE_UNSUPPORTED else); q and out at any alignment. */
+ * (TILER_HIP_REFUSE_UNSUPPORTED else); q and out at any alignment.  A page's
+ * tokens span fewer than 2^32 elements, and so does the step from page to page
+ * (TILER_HIP_REFUSE_CAPACITY else). */
 tiler_hip_status tiler_hip_paged_attention_bf16(tiler_hip_context *ctx,
                                                 const tiler_hip_attention_shape *shape, const uint16_t *q,
                                                 const tiler_hip_paged_cache *cache, const int32_t *table,
@@ -1062,6 +1065,17 @@ tiler_hip_status tiler_hip_paged_attention_bf16_workspace(const tiler_hip_contex
 #define TILER_HIP_PROGRAM_GATED_CONTRACTION_BACKWARD 16 /* bf16, extents {m, n, k}; TILER_HIP_GATED_{DX,DW} */
 #define TILER_HIP_PROGRAM_QUANTIZE_ROWS_I8 17    /* dtype: x's; extents {rows, extent}; variant 0 */
 #define TILER_HIP_PROGRAM_CONTRACTION_I8 18      /* dtype: the result's; extents {m, n, k}; variant 0 */
+/* The attention sublayer's (likewise).  A region's results are its own, so the
+ * store into a cache and the page tables, which update operands in place, are
+ * direct calls. */
+#define TILER_HIP_PROGRAM_NORM_ROTATE 19          /* extents {tokens, q heads, kv heads, head_dim, rotary},
+                                                     strides {q, k, q_out, k_out}, grouping {pairing}, scalars
+                                                     {eps bits}; TILER_HIP_ROTATE_{WQ,WK,K_OUT} */
+#define TILER_HIP_PROGRAM_NORM_ROTATE_BACKWARD 20 /* the same; TILER_HIP_ROTATE_{WQ,WK,DQ,DK,DWQ,DWK} */
+#define TILER_HIP_PROGRAM_PAGED_ATTENTION 21      /* bf16, ALIGNED16; extents {tokens, sequences, table width,
+                                                     pages, page, kv heads, q heads, head_dim}, strides {q, out,
+                                                     page, token, head}, grouping {window, sinks, most new tokens
+                                                     of a sequence or 0}, scalars {scale bits}; variant 0 */
 #define TILER_HIP_NORM_WEIGHT 1u
 #define TILER_HIP_NORM_BIAS 2u
 #define TILER_HIP_NORM_STATISTICS 4u

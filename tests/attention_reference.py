@@ -126,6 +126,7 @@ def paged_attention(q, k, v, table, starts, lengths, scale, window, sinks, out):
         for h in range(kv_heads):
             kk = np.where(there[:, None], k[at, keys % page, h], 0.0) if most else np.zeros((0, dim))
             vv = np.where(there[:, None], v[at, keys % page, h], 0.0) if most else np.zeros((0, dim))
+            k_size, v_size, v_square = np.abs(kk), np.abs(vv), vv * vv
             for i in range(fresh):
                 p, row = int(lengths[s]) - fresh + i, starts[s] + i
                 j = keys[:max(p + 1, 0)]
@@ -143,10 +144,10 @@ def paged_attention(q, k, v, table, starts, lengths, scale, window, sinks, out):
                 total = w.sum(1, keepdims=True)
                 w /= np.where(total == 0.0, 1.0, total)
                 o = w @ vj
-                sizes = w @ np.abs(vj)
+                sizes = w @ v_size[of_j]
                 # sum w |v - out| by Cauchy's inequality: no term for each key, element and row
-                spread = np.sqrt(np.maximum(w @ (vj * vj) - o * o * (2 - w.sum(1, keepdims=True)), 0.0))
-                off = scale * (np.abs(q[rows]) @ np.abs(kj).T).max(1, keepdims=True)
+                spread = np.sqrt(np.maximum(w @ v_square[of_j] - o * o * (2 - w.sum(1, keepdims=True)), 0.0))
+                off = scale * (np.abs(q[rows]) @ k_size[of_j].T).max(1, keepdims=True)
                 out[rows] = o
                 bound[rows] = (U16 * (np.abs(o) * (1 + U16) + (1 + 2 * U16) * np.minimum(spread, sizes + np.abs(o)))
                                + U32 * (2 * (dim + 16) * off + len(j) / 8 + 96) * sizes)

@@ -11,6 +11,9 @@ import pytest
 import attention_reference as ref
 import test_abi_layout
 from tiler_amd import _lib as L
+from tiler_amd import families
+from tiler_amd.realize import propose, realize
+from tiler_amd.runtime import Refusal
 
 
 def test_struct_layouts(tmp_path, monkeypatch):
@@ -217,3 +220,158 @@ def test_oracle_of_page_slots_on_a_batch_written_out():
     assert positions.tolist() == [5, 6, 8, 9, 10, 11, 12, 0]
     assert slots.tolist() == [9, 10, 28, 29, 30, 31, -1, -1]  # position 12 lies past the table's width
     assert taken == 1
+
+
+# -- the recognizer ---------------------------------------------------------------
+RE = L.PERMITS_REASSOCIATION
+EPS = 0x358637BD
+
+
+def bits(x):
+    return int(np.float32(x).view(np.uint32))
+
+
+def rotate_region(backward=False, extents=(5, 8, 2, 64, 64), variant=0, dtype=L.BF16, pairing=0, eps=EPS, **kw):
+    q, k = extents[1] * extents[3], extents[2] * extents[3]
+    kw = {"permissions": RE, "strides": (q, k, q, k), "grouping": (pairing,), "scalars": (eps,), **kw}
+    return realize(L.PROGRAM_NORM_ROTATE_BACKWARD if backward else L.PROGRAM_NORM_ROTATE, extents, dtype=dtype,
+                   variant=variant, **kw)
+
+
+def attention_region(tokens=4, sequences=4, width=5, pages=10, page=16, kv_heads=2, heads=8, dim=64, window=0, sinks=0,
+                     fresh=0, scale=0.125, **kw):
+    row = kv_heads * dim
+    kw = {"permissions": RE, "dtype": L.BF16, "strides": (heads * dim, heads * dim, page * row, row, dim), **kw}
+    return realize(L.PROGRAM_PAGED_ATTENTION, (tokens, sequences, width, pages, page, kv_heads, heads, dim),
+                   grouping=(window, sinks, fresh), scalars=(bits(scale),), **kw)
+
+
+def counted(rz):
+    roles = [role for role, _ in rz.slots]
+    return tuple(roles.count(r) for r in (L.SLOT_INPUT, L.SLOT_OUTPUT, L.SLOT_SCRATCH))
+
+
+ALL_GRADS = L.ROTATE_DQ | L.ROTATE_DK | L.ROTATE_DWQ | L.ROTATE_DWK
+
+
+@pytest.mark.parametrize("rz,counts", [
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT), (4, 2, 0)),
+    (lambda: rotate_region(variant=L.ROTATE_WQ | L.ROTATE_WK | L.ROTATE_K_OUT), (6, 2, 0)),
+    (lambda: rotate_region(extents=(5, 8, 0, 64, 0)), (1, 1, 0)),
+    (lambda: rotate_region(True, variant=L.ROTATE_WQ | L.ROTATE_WK | ALL_GRADS), (8, 4, 2)),
+    (lambda: rotate_region(True, variant=L.ROTATE_DQ, eps=0), (3, 1, 0)),
+    (lambda: rotate_region(True, variant=L.ROTATE_DK | L.ROTATE_DWK), (4, 2, 1)),
+    (lambda: attention_region(), (6, 1, 0)),
+    (lambda: attention_region(width=1000, tokens=1, sequences=1), (6, 1, 2)),
+    (lambda: attention_region(width=0), (5, 1, 0)),
+])
+def test_slots(rz, counts):
+    rz = rz()
+    assert counted(rz) == counts and rz.symbols
+    for i, (role, _) in enumerate(rz.slots):
+        assert rz.slot_alignment(i) == 16
+
+
+@pytest.mark.parametrize("rz,status", [
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT, permissions=0), L.REFUSE_UNSUPPORTED),
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT, dtype=2), L.REFUSE_UNSUPPORTED),
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT, input_subnormals=L.SUBNORMALS_FLUSH_SIGN), L.REFUSE_UNSUPPORTED),
+    (lambda: rotate_region(variant=0), L.REFUSE_INVALID_ARGUMENT),  # the keys go nowhere
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT | L.ROTATE_DQ), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT | L.ROTATE_WQ, eps=0), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT, pairing=2), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT, pairing=1 << 32), L.REFUSE_CAPACITY),
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT, extents=(5, (1 << 32) + 8, 2, 64, 64)), L.REFUSE_CAPACITY),
+    (lambda: rotate_region(True, variant=L.ROTATE_K_OUT), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: rotate_region(True, variant=L.ROTATE_DWQ, eps=0), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: rotate_region(True, variant=L.ROTATE_DQ, permissions=0), L.REFUSE_UNSUPPORTED),
+    (lambda: attention_region(permissions=0), L.REFUSE_UNSUPPORTED),
+    (lambda: attention_region(dtype=L.F32), L.REFUSE_UNSUPPORTED),
+    (lambda: attention_region(variant=1), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: attention_region(window=1 << 32), L.REFUSE_CAPACITY),
+    (lambda: attention_region(page=1 << 32), L.REFUSE_CAPACITY),
+    (lambda: attention_region(scale=0.0), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: attention_region(heads=7), L.REFUSE_INVALID_ARGUMENT),
+    (lambda: attention_region(flags=0), L.REFUSE_UNSUPPORTED),  # the cache's rows start on 16 bytes
+    (lambda: attention_region(strides=(512, 512, 1 << 33, 128, 64)), L.REFUSE_CAPACITY),
+    (lambda: attention_region(pages=1, strides=(512, 512, 1 << 33, 128, 64)), None),  # one page has no next one
+    (lambda: attention_region(pages=1, strides=(512, 512, 7, 128, 64)), None),
+    (lambda: attention_region(kv_heads=1, strides=(512, 512, 1024, 64, 3)), None),
+    (lambda: attention_region(page=1, strides=(512, 512, 128, 5, 64)), None),
+    (lambda: attention_region(pages=1, page=1 << 26, width=1, strides=(512, 512, 0, 128, 64)), L.REFUSE_CAPACITY),
+])
+def test_refused_regions(rz, status):
+    if status is None:
+        assert rz().symbols
+        return
+    with pytest.raises(Refusal) as e:
+        rz()
+    assert e.value.status == status, str(e.value)
+
+
+def test_proposals():
+    for rz, program, kw in ((rotate_region(variant=L.ROTATE_K_OUT), L.PROGRAM_NORM_ROTATE,
+                             dict(extents=(5, 8, 2, 64, 64), variant=L.ROTATE_K_OUT, strides=(512, 128, 512, 128),
+                                  scalars=(EPS,), dtype=L.BF16)),
+                            (attention_region(), L.PROGRAM_PAGED_ATTENTION,
+                             dict(extents=(4, 4, 5, 10, 16, 2, 8, 64), strides=(512, 512, 16 * 128, 128, 64),
+                                  scalars=(bits(0.125),), dtype=L.BF16))):
+        offer = propose(program, permissions=RE, **kw)
+        assert offer.proposals[offer.chosen].symbols == rz.symbols
+        strict = propose(program, **kw)
+        assert not strict.proposals and strict.declined
+
+
+@pytest.mark.parametrize("kw,symbol", [
+    (dict(dim=64, eps=EPS), "tiler_norm_rotate_bf16_h4"), (dict(dim=128, pairing=1), "tiler_norm_rotate_bf16_n8"),
+    (dict(dim=256), "tiler_norm_rotate_bf16_h16"), (dict(dim=512), "tiler_norm_rotate_bf16_h32"),
+    (dict(dim=1024), "tiler_norm_rotate_bf16_h64"), (dict(dim=90, rotary=34), "tiler_norm_rotate_bf16_any"),
+    (dict(dim=128, dtype=L.F32), "tiler_norm_rotate_f32_h16"), (dict(dim=1024, dtype=L.F32), "tiler_norm_rotate_f32_any"),
+    (dict(dim=64, rotary=24), "tiler_norm_rotate_bf16_any")])
+def test_rotation_forms(kw, symbol):
+    kw = dict(kw)
+    dim = kw.pop("dim")
+    rotary = kw.pop("rotary", dim)
+    assert rotate_region(extents=(5, 8, 2, dim, rotary), variant=L.ROTATE_K_OUT, **kw).symbols == [symbol]
+
+
+@pytest.mark.parametrize("kw,symbols", [
+    (dict(tokens=4, fresh=1), ["few64"]),
+    (dict(tokens=4, fresh=1, dim=72), ["few128"]),
+    (dict(tokens=4, fresh=1, dim=136), ["few256"]),
+    (dict(tokens=1, sequences=1, width=1000), ["few64", "join"]),
+    (dict(tokens=40, sequences=1), ["t128_d64"]),
+    (dict(tokens=40, sequences=1, dim=72), ["t128_d96"]),
+    (dict(tokens=40, sequences=1, dim=104), ["t128_d128"]),
+    (dict(tokens=40, sequences=1, dim=136), ["t128_d192"]),
+    (dict(tokens=40, sequences=1, dim=200), ["t128_d256"]),
+    (dict(tokens=40, sequences=1, width=1000), ["t128_d64", "join"]),
+    (dict(tokens=1 << 14, sequences=1, width=1 << 10), ["t256_d64"]),
+    (dict(tokens=1 << 14, sequences=1, width=1 << 10, dim=256), ["t128_d256"]),
+])
+def test_attention_forms(kw, symbols):
+    assert attention_region(**kw).symbols == ["tiler_paged_attention_bf16_" + s for s in symbols]
+
+
+# -- the host functions' checks ------------------------------------------------------
+def test_host_functions_refuse():
+    q, k = np.zeros((3, 4, 64), np.uint16), np.zeros((3, 2, 64), np.uint16)
+    at, f = np.zeros(3, np.int32), np.ones(32)
+    cache, table, starts, lengths = (np.zeros((6, 4, 2, 64), np.uint16), np.zeros((2, 3), np.int32), np.zeros(3, np.int32),
+                                     np.zeros(2, np.int32))
+    for call, status in (
+            (lambda: families.page_slots([1], [1, 2], 4, [0], np.zeros((1, 2))), L.REFUSE_INVALID_ARGUMENT),
+            (lambda: families.page_slots([1], [1], 4, [0], np.zeros((2, 2))), L.REFUSE_INVALID_ARGUMENT),
+            (lambda: families.norm_rotate(q, k[:, :, :32], None, None, at, f, 64), L.REFUSE_UNSUPPORTED),
+            (lambda: families.norm_rotate(q, k.astype(np.float32), None, None, at, f, 64), L.REFUSE_UNSUPPORTED),
+            (lambda: families.norm_rotate(q, k, None, None, at, f, 64, "pairs"), L.REFUSE_UNSUPPORTED),
+            (lambda: families.norm_rotate(q, k, None, None, at[:2], f, 64), L.REFUSE_INVALID_ARGUMENT),
+            (lambda: families.norm_rotate(q, k, None, None, at, f[:4], 64), L.REFUSE_INVALID_ARGUMENT),
+            (lambda: families.norm_rotate(q, k, np.zeros(8, np.uint16), None, at, f, 64), L.REFUSE_INVALID_ARGUMENT),
+            (lambda: families.norm_rotate_backward(q, q, q, k, None, None, at, f, 64), L.REFUSE_INVALID_ARGUMENT),
+            (lambda: families.paged_attention_bf16(q[0], cache, cache, table, starts, lengths, 1.0), L.REFUSE_UNSUPPORTED),
+            (lambda: families.paged_attention_bf16(q, cache, cache[:5], table, starts, lengths, 1.0), L.REFUSE_INVALID_ARGUMENT),
+            (lambda: families.paged_attention_bf16(q, cache, cache, table, starts[:2], lengths, 1.0), L.REFUSE_INVALID_ARGUMENT)):
+        with pytest.raises(Refusal) as e:
+            call()
+        assert e.value.status == status, str(e.value)

@@ -70,6 +70,9 @@ PROGRAM_GATED_CONTRACTION = 15
 PROGRAM_GATED_CONTRACTION_BACKWARD = 16
 PROGRAM_QUANTIZE_ROWS_I8 = 17
 PROGRAM_CONTRACTION_I8 = 18
+PROGRAM_NORM_ROTATE = 19
+PROGRAM_NORM_ROTATE_BACKWARD = 20
+PROGRAM_PAGED_ATTENTION = 21
 
 NORM_WEIGHT = 1
 NORM_BIAS = 2

@@ -2727,6 +2727,49 @@ static tiler_hip_status plan_region(const tiler_hip_context* ctx, const tiler_hi
       st = r->variant ? p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "contract_i8 variant")
                       : tiler_rt::plan_contract_i8(t, r->dtype, e[0], e[1], e[2], addr, p);
       break;
+    case TILER_HIP_PROGRAM_NORM_ROTATE:
+    case TILER_HIP_PROGRAM_NORM_ROTATE_BACKWARD: {
+      tiler_hip_head_layout h{};
+      const uint64_t* sizes[] = {&e[1], &e[2], &e[3], &e[4], &r->grouping[0]};
+      uint32_t* fields[] = {&h.q_heads, &h.kv_heads, &h.head_dim, &h.rotary, &h.pairing};
+      bool fit = true;
+      for (int i = 0; i < 5; ++i) {
+        fit = fit && *sizes[i] <= UINT32_MAX;
+        *fields[i] = (uint32_t)*sizes[i];
+      }
+      h.tokens = e[0];
+      h.q_stride = r->strides[0], h.k_stride = r->strides[1];
+      h.q_out_stride = r->strides[2], h.k_out_stride = r->strides[3];
+      h.eps_bits = r->scalars[0];
+      if (!fit) st = p.refuse(TILER_HIP_REFUSE_CAPACITY, "head layout: sizes of 2^32 and more");
+      else if (!c.reassociate) st = needs_reassociation("the head norm's sums");
+      else if (r->program == TILER_HIP_PROGRAM_NORM_ROTATE)
+        st = tiler_rt::plan_norm_rotate(t, r->dtype, r->variant, h, nullptr, addr, p);
+      else st = tiler_rt::plan_norm_rotate_backward(t, r->dtype, r->variant, h, addr, p);
+      break;
+    }
+    case TILER_HIP_PROGRAM_PAGED_ATTENTION: {
+      tiler_hip_attention_shape a{};
+      tiler_hip_paged_cache cache{};
+      const uint64_t* sizes[] = {&e[4], &e[5], &e[6], &e[7], &r->grouping[0], &r->grouping[1]};
+      uint32_t* fields[] = {&cache.page, &cache.heads, &a.q_heads, &cache.head_dim, &a.window, &a.sinks};
+      bool fit = true;
+      for (int i = 0; i < 6; ++i) {
+        fit = fit && *sizes[i] <= UINT32_MAX;
+        *fields[i] = (uint32_t)*sizes[i];
+      }
+      a.tokens = e[0], a.sequences = e[1], a.table_width = e[2], a.max_fresh = r->grouping[2];
+      a.q_stride = r->strides[0], a.out_stride = r->strides[1];
+      std::memcpy(&a.scale, &r->scalars[0], 4);
+      cache.pages = e[3];
+      cache.page_stride = r->strides[2], cache.token_stride = r->strides[3], cache.head_stride = r->strides[4];
+      if (r->dtype != TILER_HIP_BF16) st = p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "paged attention is a bf16 family");
+      else if (r->variant) st = p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "paged attention variant");
+      else if (!fit) st = p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: sizes of 2^32 and more");
+      else if (!c.reassociate) st = needs_reassociation("paged attention");
+      else st = tiler_rt::plan_paged_attention_bf16(t, a, cache, addr, p);
+      break;
+    }
     default:
       st = p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "no realization for this scalar program");
   }

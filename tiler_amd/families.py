@@ -360,9 +360,102 @@ def contract_i8(a, b, a_scales, b_scales, out_dtype=np.float32, ctx=None):
     return _run(ctx, operands, [(out_dtype, (m, n))], lambda c, i, o: c.contract_i8(*i, m, n, k, code, *o))[0]
 
 
+# --- the attention sublayer (no reference counterpart) --------------------------
+
+def _lists(values):
+    return [np.ascontiguousarray(v, dtype=np.int32).reshape(-1) for v in values]
+
+
+def page_slots(kept, fresh, page: int, free_pages, table, tokens: int | None = None, ctx=None):
+    """(table, starts, lengths, positions, slots, taken) of a batch whose
+    sequences hold `kept` tokens and get `fresh` more; table [sequences, width]
+    names the kept tokens' pages, and the new pages come from free_pages.
+    `tokens`: rows of the batch (default: the sum of fresh)."""
+    kept, fresh, free = _lists((kept, fresh, free_pages))
+    table = np.ascontiguousarray(table, dtype=np.int32)
+    if table.ndim != 2 or not len(kept) == len(fresh) == len(table):
+        raise Refusal(L.REFUSE_INVALID_ARGUMENT, "page_slots", "a length of each kind and a row of the table for each sequence")
+    if tokens is None:
+        tokens = int(np.maximum(fresh, 0).sum(dtype=np.int64))
+    n, i32 = len(kept), np.int32
+
+    def launch(c, i, o):
+        if table.size:
+            c.copy(o[0], i[3], table.nbytes)
+        c.page_slots(i[0], i[1], n, page, i[2], len(free), o[0], table.shape[1], tokens, *o[1:])
+
+    return tuple(_run(ctx, [kept, fresh, free, table],
+                      [(i32, table.shape), (i32, (n + 1,)), (i32, (n,)), (i32, (tokens,)), (i32, (tokens,)), (i32, (1,))], launch))
+
+
+def _heads(q, k, rotary, pairing, eps_bits, frequencies, positions, what: str):
+    q, k = np.ascontiguousarray(q), np.ascontiguousarray(k)
+    if q.ndim != 3 or k.ndim != 3 or q.dtype != k.dtype or q.dtype not in (np.float32, np.uint16) or \
+            q.shape[::2] != k.shape[::2] or pairing not in ("halves", "neighbours"):
+        raise Refusal(L.REFUSE_UNSUPPORTED, what,
+                      "q and k [tokens, heads, head_dim], float32 or uint16 (bf16 patterns), pairs as halves or neighbours")
+    (tokens, q_heads, dim), kv_heads = q.shape, k.shape[1]
+    positions = _operand(positions, np.int32, (tokens,), what)
+    frequencies = _operand(frequencies, np.float64, (rotary // 2,), what)
+    layout = L.HeadLayout(tokens=tokens, q_heads=q_heads, kv_heads=kv_heads, head_dim=dim, rotary=rotary,
+                          pairing=L.ROTATE_HALVES if pairing == "halves" else L.ROTATE_NEIGHBOURS, eps_bits=eps_bits,
+                          q_stride=q_heads * dim, k_stride=kv_heads * dim, q_out_stride=q_heads * dim, k_out_stride=kv_heads * dim)
+    return q, k, layout, L.F32 if q.dtype == np.float32 else L.BF16, [positions, frequencies]
+
+
+def norm_rotate(q, k, wq, wk, positions, frequencies, rotary: int, pairing: str = "halves", eps_bits: int = 0x358637BD, ctx=None):
+    """(q_out, k_out): each head normed (eps_bits 0: not) and its first `rotary`
+    elements turned by positions [tokens] times frequencies [rotary / 2]; wq and
+    wk [head_dim] or None."""
+    q, k, layout, code, turn = _heads(q, k, rotary, pairing, eps_bits, frequencies, positions, "norm_rotate")
+    w = [None if v is None else _operand(v, q.dtype, q.shape[2:], "norm_rotate") for v in (wq, wk)]
+    return tuple(_run(ctx, [q, k, *w, *turn], [(q.dtype, q.shape), (k.dtype, k.shape)],
+                      lambda c, i, o: c.norm_rotate(code, layout, i[0], i[1], None, *i[2:], *o)))
+
+
+def norm_rotate_backward(dq_out, dk_out, q, k, wq, wk, positions, frequencies, rotary: int, pairing: str = "halves",
+                         eps_bits: int = 0x358637BD, ctx=None):
+    """(dq, dk, dwq, dwk) of norm_rotate; without a norm dwq and dwk are None."""
+    what = "norm_rotate_backward"
+    q, k, layout, code, turn = _heads(q, k, rotary, pairing, eps_bits, frequencies, positions, what)
+    dy = [_operand(d, x.dtype, x.shape, what) for d, x in ((dq_out, q), (dk_out, k))]
+    w = [None if v is None else _operand(v, q.dtype, q.shape[2:], what) for v in (wq, wk)]
+    outputs = [(q.dtype, q.shape), (k.dtype, k.shape)] + ([(q.dtype, q.shape[2:])] * 2 if eps_bits else [])
+    got = _run(ctx, [*dy, q, k, *w, *turn], outputs,
+               lambda c, i, o: c.norm_rotate_backward(code, layout, *i, *o))
+    return tuple(got) if eps_bits else (*got, None, None)
+
+
+def paged_attention_bf16(q, k_cache, v_cache, table, starts, lengths, scale: float, window: int = 0, sinks: int = 0, ctx=None):
+    """out [tokens, heads, head_dim]: the attention of q's rows over the cache
+    [pages, page, kv_heads, head_dim] (bf16 patterns); rows of no sequence are 0."""
+    what = "paged_attention_bf16"
+    q, k_cache, v_cache = (np.ascontiguousarray(a) for a in (q, k_cache, v_cache))
+    table = np.ascontiguousarray(table, dtype=np.int32)
+    if q.ndim != 3 or k_cache.ndim != 4 or table.ndim != 2 or q.dtype != np.uint16 or q.shape[2] != k_cache.shape[3]:
+        raise Refusal(L.REFUSE_UNSUPPORTED, what, "q [tokens, heads, head_dim] and the cache [pages, page, heads, head_dim], uint16")
+    k_cache, v_cache = (_operand(a, np.uint16, k_cache.shape, what) for a in (k_cache, v_cache))
+    starts = _operand(starts, np.int32, (len(table) + 1,), what)
+    lengths = _operand(lengths, np.int32, (len(table),), what)
+    (tokens, heads, dim), (pages, page, kv_heads, _) = q.shape, k_cache.shape
+    shape = L.AttentionShape(tokens=tokens, sequences=len(table), q_heads=heads, scale=scale, q_stride=heads * dim,
+                             out_stride=heads * dim, table_width=table.shape[1], window=window, sinks=sinks,
+                             max_fresh=max(int(np.diff(starts).max(initial=0)), 0), max_length=max(int(lengths.max(initial=0)), 0))
+
+    def launch(c, i, o):
+        cache = L.PagedCache(k=i[1].ptr, v=i[2].ptr, pages=pages, page=page, heads=kv_heads, head_dim=dim,
+                             page_stride=page * kv_heads * dim, token_stride=kv_heads * dim, head_stride=dim)
+        if q.size:
+            c.copy(o[0], i[6], q.nbytes)
+        c.paged_attention_bf16(shape, i[0], cache, *i[3:6], o[0])
+
+    return _run(ctx, [q, k_cache, v_cache, table, starts, lengths, np.zeros_like(q)], [(np.uint16, q.shape)], launch)[0]
+
+
 __all__ = [
     "strict_sum", "strict_partitioned_sum", "cooperative_grouped_sum", "tree_sum",
     "rms_norm_f32", "rms_norm_bf16", "softmax_f32", "silu_f32", "gather",
     "contract_strict_f32", "contract_bf16", "dequantize_u4", "layer_norm", "layer_norm_backward", "gated_contract_bf16",
-    "gated_contract_bf16_backward", "quantize_rows_i8", "contract_i8", "default_context", "GatherIndexOutOfBounds",
+    "gated_contract_bf16_backward", "quantize_rows_i8", "contract_i8", "page_slots", "norm_rotate", "norm_rotate_backward",
+    "paged_attention_bf16", "default_context", "GatherIndexOutOfBounds",
 ]

@@ -60,14 +60,15 @@ class Realization:
 
     def slot_alignment(self, slot: int) -> int:
         """What slot `slot`'s address has to be a multiple of.  The scratch of
-        the feed-forward sublayer's gradients is moved in aligned 16-byte
-        pieces, however the operands lie."""
+        the feed-forward sublayer's gradients and of the attention sublayer is
+        moved in aligned 16-byte pieces, however the operands lie."""
         if self.slots[slot][0] == L.SLOT_SCRATCH and self.program in _ALIGNED_SCRATCH:
             return 16
         return self.alignment
 
 
-_ALIGNED_SCRATCH = (L.PROGRAM_LAYER_NORM_BACKWARD, L.PROGRAM_GATED_CONTRACTION_BACKWARD)
+_ALIGNED_SCRATCH = (L.PROGRAM_LAYER_NORM_BACKWARD, L.PROGRAM_GATED_CONTRACTION_BACKWARD,
+                    L.PROGRAM_NORM_ROTATE_BACKWARD, L.PROGRAM_PAGED_ATTENTION)
 
 
 def _entry_info(index: int):
