@@ -1193,7 +1193,8 @@ typedef struct {
 
 /* Forms a region may name (tiler_hip_region.form).  The contraction forms
  * apply to td,od->to bf16 under PERMITS_REASSOCIATION; the softmax forms to
- * rows of more than four 8192-element segments under PERMITS_REASSOCIATION. */
+ * rows of more than four 8192-element segments under PERMITS_REASSOCIATION;
+ * the attention forms to any batch. */
 #define TILER_HIP_FORM_AUTO 0u
 #define TILER_HIP_FORM_CONTRACT_SKINNY 1u     /* m <= 64: B streamed once, 16 columns per workgroup */
 #define TILER_HIP_FORM_CONTRACT_STAGED_256 2u /* 256x256 tiles, 16 waves, LDS-DMA double buffer */
@@ -1201,6 +1202,9 @@ typedef struct {
 #define TILER_HIP_FORM_CONTRACT_GENERAL_128 4u /* register-staged 128x128 tiles, any n and k */
 #define TILER_HIP_FORM_SOFTMAX_SPLIT 5u       /* three launches over segment partials in scratch */
 #define TILER_HIP_FORM_SOFTMAX_ROW_SYNC 6u    /* one row-synchronized launch (at most two workgroups per CU) */
+#define TILER_HIP_FORM_ATTENTION_FEW 7u       /* 16 rows a sequence at a time, its keys shared out to waves */
+#define TILER_HIP_FORM_ATTENTION_TILE_128 8u  /* tiles of 128 rows, four waves */
+#define TILER_HIP_FORM_ATTENTION_TILE_256 9u  /* tiles of 256 rows, eight waves; heads of up to 128 */
 
 /* Storage slot roles.  Slot order per program:
  *   expression  the inputs in access order, y, program (a constant slot)

@@ -287,6 +287,10 @@ def test_slots(rz, counts):
     (lambda: rotate_region(True, variant=L.ROTATE_DQ, permissions=0), L.REFUSE_UNSUPPORTED),
     (lambda: attention_region(permissions=0), L.REFUSE_UNSUPPORTED),
     (lambda: attention_region(dtype=L.F32), L.REFUSE_UNSUPPORTED),
+    (lambda: attention_region(form=L.FORM_CONTRACT_SKINNY), L.REFUSE_UNSUPPORTED),
+    (lambda: attention_region(form=10), L.REFUSE_UNSUPPORTED),
+    (lambda: attention_region(dim=136, form=L.FORM_ATTENTION_TILE_256), L.REFUSE_UNSUPPORTED),
+    (lambda: rotate_region(variant=L.ROTATE_K_OUT, form=L.FORM_ATTENTION_FEW), L.REFUSE_UNSUPPORTED),
     (lambda: attention_region(variant=1), L.REFUSE_INVALID_ARGUMENT),
     (lambda: attention_region(window=1 << 32), L.REFUSE_CAPACITY),
     (lambda: attention_region(page=1 << 32), L.REFUSE_CAPACITY),

@@ -251,29 +251,44 @@ def test_two_streams(ctx):
 
 
 # -- tiles of 256 rows, and forms at their edges ----------------------------------
-LARGE = [  # dim, heads, kv_heads, lengths, page, window, sinks
-    *((dim, 128, 8, [(90, 170), (0, 5), (300, 0), (7, 93)], 24, window, sinks)
-      for dim in (64, 80, 96, 104, 128) for window, sinks in ((0, 0), (100, 5))),
-    (64, 2, 1, [(6000, 2048)], 64, 0, 0), (128, 4, 1, [(1000, 1300), (0, 700), (10, 48)], 64, 0, 0),
-    (96, 4, 1, [(1000, 1300), (0, 700), (10, 48)], 64, 1900, 100),
-]
-
-
-def form_of(b):
-    """Symbols of the program that a batch is run by."""
+def region_of(b):
+    """A batch's program and extents, and what else names its region."""
     row = b.kv_heads * b.dim
-    return realize(L.PROGRAM_PAGED_ATTENTION, (b.tokens, len(b.lengths), b.width, b.pages, b.page, b.kv_heads, b.heads, b.dim),
-                   dtype=L.BF16, strides=(b.q_stride, b.out_stride, b.page * row, row, b.dim), permissions=RE,
-                   grouping=(b.window, b.sinks, max(b.fresh)), scalars=(int(np.float32(b.scale).view(np.uint32)),)).symbols
+    return ((L.PROGRAM_PAGED_ATTENTION, (b.tokens, len(b.lengths), b.width, b.pages, b.page, b.kv_heads, b.heads, b.dim)),
+            dict(dtype=L.BF16, strides=(b.q_stride, b.out_stride, b.page * row, row, b.dim), permissions=RE,
+                 grouping=(b.window, b.sinks, max(b.fresh)), scalars=(int(np.float32(b.scale).view(np.uint32)),)))
 
 
-@pytest.mark.parametrize("dim,heads,kv_heads,lengths,page,window,sinks", LARGE)
-def test_tiles_of_256_rows(ctx, dim, heads, kv_heads, lengths, page, window, sinks):
-    """Rows enough for them: sequences that end inside tiles, some of few tokens or
-    none, whole and in parts of the keys."""
+@pytest.mark.parametrize("dim", [8, 64, 80, 96, 104, 128, 160, 256])
+@pytest.mark.parametrize("heads,kv_heads,lengths,page,window,sinks", [
+    (6, 2, [(90, 170), (0, 5), (300, 0), (7, 93)], 24, 0, 0), (28, 4, [(90, 17), (700, 5), (2, 60)], 24, 100, 5),
+    (3, 1, [(1500, 260), (0, 3), (1100, 90)], 64, 900, 70), (4, 2, [(40, 1), (2000, 1), (0, 1), (31, 2)], 16, 0, 0)])
+def test_every_form(ctx, dim, heads, kv_heads, lengths, page, window, sinks):
+    """The same batch in every form that is offered for it, parts of the keys among them."""
     b = Batch(lengths, heads, kv_heads, dim, page=page, pad=3, gap=4, window=window, sinks=sinks, seed=dim)
-    assert "_t256_" in form_of(b)[0]
-    b.check(ctx, max_length=0)
+    want, bound = b.want()
+    q, k, v, table, starts, lens, out = b.upload(ctx)
+    region, kw = region_of(b)
+    offer = propose(*region, ctx=ctx, **kw)
+    assert [p.symbols[0].rstrip("0123456789") for p in offer.proposals] == [
+        "tiler_paged_attention_bf16_" + f for f in ("few", "t128_d", "t256_d")[:2 if dim > 128 else 3]]
+    for p in offer.proposals:
+        out.upload(np.full((b.tokens, b.out_stride), 0x40A8, np.uint16))
+        routed(ctx, p.realize(ctx), [q, k, v, table, starts, lens], [out])
+        got = widen(out.download(np.uint16, (b.tokens, b.out_stride)))
+        off = np.abs(got[:, :heads * dim].reshape(want.shape) - want)
+        assert (off <= bound).all(), f"{p.symbols}: worst {np.nanmax(off / np.maximum(bound, 1e-30))} of the bound"
+        assert (got[:, heads * dim:] == 5.25).all(), p.symbols
+    b.free()
+
+
+def test_rows_for_tiles_of_256(ctx):
+    """Work enough that they are chosen, whole and in parts of the keys."""
+    for lengths, heads, kv_heads, window in (([(0, 4096), (0, 4096)], 16, 1, 64), ([(3000, 300)], 32, 8, 0)):
+        b = Batch(lengths, heads, kv_heads, 96 if window else 128, page=64, window=window, sinks=2 if window else 0, seed=1)
+        region, kw = region_of(b)
+        assert "_t256_" in realize(*region, ctx=ctx, **kw).symbols[0]
+        b.check(ctx, max_length=0)
 
 
 def test_one_token_to_a_page_and_axes_of_one(ctx):
@@ -385,10 +400,9 @@ def test_routed_attention(ctx, lengths, heads, kv_heads, dim, window, sinks):
     b = Batch(lengths, heads, kv_heads, dim, window=window, sinks=sinks, seed=dim)
     want = b.run(ctx, max_length=0)
     q, k, v, table, starts, lens, out = b.upload(ctx)
-    row = kv_heads * dim
-    for rz in realizations(ctx, L.PROGRAM_PAGED_ATTENTION, (b.tokens, len(lengths), b.width, b.pages, b.page, kv_heads, heads, dim),
-                           dtype=L.BF16, strides=(b.q_stride, b.out_stride, b.page * row, row, dim),
-                           grouping=(window, sinks, max(b.fresh)), scalars=(int(np.float32(b.scale).view(np.uint32)),)):
+    region, kw = region_of(b)
+    offer = propose(*region, ctx=ctx, **kw)
+    for rz in (realize(*region, ctx=ctx, **kw), offer.proposals[offer.chosen].realize(ctx)):
         out.upload(np.zeros((b.tokens, b.out_stride), np.uint16))
         routed(ctx, rz, [q, k, v, table, starts, lens], [out])
         np.testing.assert_array_equal(out.download(np.uint16, want.shape), want)

@@ -123,6 +123,9 @@ FORM_CONTRACT_STAGED_128 = 3
 FORM_CONTRACT_GENERAL_128 = 4
 FORM_SOFTMAX_SPLIT = 5
 FORM_SOFTMAX_ROW_SYNC = 6
+FORM_ATTENTION_FEW = 7
+FORM_ATTENTION_TILE_128 = 8
+FORM_ATTENTION_TILE_256 = 9
 
 MAX_PROPOSALS = 6
 DECLINE_NUMERICAL_PERMISSION_REFUSED = 1

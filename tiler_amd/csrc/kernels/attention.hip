@@ -78,10 +78,12 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 struct Sequence {
   uint32_t first, fresh;  // its rows of q and out
   int32_t kept;           // position of its first new token (below zero: the list says fewer tokens than are new)
-  __device__ __forceinline__ Sequence(const TilerAttentionShape& a, const int32_t* starts, const int32_t* lengths, uint32_t s) {
+  __device__ __forceinline__ Sequence(const TilerAttentionShape& a, const int32_t* starts, const int32_t* lengths, uint32_t s)
+      : Sequence(a, starts[s], starts[s + 1], lengths[s]) {}
+  __device__ __forceinline__ Sequence(const TilerAttentionShape& a, int32_t start, int32_t next, int32_t length) {
     const int32_t most = (int32_t)a.tokens;
     auto cut = [&](int32_t v) { return v < 0 ? 0 : v > most ? most : v; };
-    const int32_t b = cut(starts[s]), e = cut(starts[s + 1]), length = lengths[s];
+    const int32_t b = cut(start), e = cut(next);
     first = (uint32_t)b;
     fresh = e > b ? (uint32_t)(e - b) : 0u;
     kept = (length < 0 ? 0 : length) - (int32_t)fresh;
@@ -378,25 +380,28 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   const uint32_t head = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads % a.splits;
   const uint32_t at_tile = gridDim.x / (a.kv_heads * a.splits) - 1u - blockIdx.x / (a.kv_heads * a.splits);
   // Sequence s has the tiles from starts[s] * group / kRows + s on: as many as its
-  // rows need, or one more.
-  uint32_t s = 0, tile_in = 0;
-  {
-    uint32_t before = 0, at = 0;
-    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64u) {
-      const uint32_t n = s0 + lane;
-      int32_t start = n < a.sequences ? starts[n] : 0;
-      start = start < 0 ? 0 : start > (int32_t)a.tokens ? (int32_t)a.tokens : start;
-      const uint32_t from = (uint32_t)start * a.group / kRows + n;
-      const uint64_t mask = __ballot(n < a.sequences && from <= at_tile);
-      if (mask) at = __builtin_amdgcn_readlane(from, 63 - __builtin_clzll(mask));
-      before += __popcll(mask);
-      if (mask != ~0ull) break;
+  // rows need, or one more.  Its lists' entries come along with the search.
+  uint32_t before = 0, tile_in = 0;
+  int32_t start = 0, next = 0, length = 0;
+  for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64u) {
+    const uint32_t n = s0 + lane, at = n < a.sequences ? n : a.sequences - 1u;
+    const int32_t starts_here = starts[at], next_here = starts[at + 1u], length_here = lengths[at];
+    const int32_t cut = starts_here < 0 ? 0 : starts_here > (int32_t)a.tokens ? (int32_t)a.tokens : starts_here;
+    const uint32_t from = (uint32_t)cut * a.group / kRows + n;
+    const uint64_t mask = __ballot(n < a.sequences && from <= at_tile);
+    if (mask) {
+      const int last = 63 - __builtin_clzll(mask);
+      tile_in = at_tile - (uint32_t)__builtin_amdgcn_readlane(from, last);
+      start = __builtin_amdgcn_readlane(starts_here, last);
+      next = __builtin_amdgcn_readlane(next_here, last);
+      length = __builtin_amdgcn_readlane(length_here, last);
     }
-    if (before == 0) return;
-    s = before - 1u;
-    tile_in = at_tile - at;
+    before += __popcll(mask);
+    if (mask != ~0ull) break;
   }
-  const Sequence seq(a, starts, lengths, s);
+  if (before == 0) return;
+  const uint32_t s = before - 1u;
+  const Sequence seq(a, start, next, length);
   const uint32_t rows = seq.fresh * a.group, row0 = tile_in * kRows;
   if (row0 >= rows) return;
   const int32_t* const pages = table + (uint64_t)s * a.width;

@@ -123,8 +123,8 @@ __device__ __forceinline__ void rotate_any(const TilerHeads& a, const T* q, cons
   }
 }
 
-// Its gradients, in the same manner; blockIdx.y: the queries' (0) or the keys'.
-// A lane adds up its own elements of dw in LDS, its wave's share, and the
+// Its gradients, in the same manner; the first q_groups workgroups take the
+// queries', the others the keys'.  A lane adds up its own elements of dw in LDS, its wave's share, and the
 // workgroup writes one row of partial sums.
 template <typename T>
 __device__ __forceinline__ void rotate_grad_any(const TilerHeads& a, const T* dq_out, const T* dk_out, const T* q,
@@ -133,15 +133,16 @@ __device__ __forceinline__ void rotate_grad_any(const TilerHeads& a, const T* dq
   __shared__ tiler::f32x2_pair turns[kMostPairs];
   __shared__ float sums[4][2 * kMostPairs];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, pairs = a.rotary / 2u;
-  const bool is_q = blockIdx.y == 0;
+  const bool is_q = blockIdx.x < a.q_groups;
+  const uint32_t block = is_q ? blockIdx.x : blockIdx.x - a.q_groups, blocks = is_q ? a.q_groups : gridDim.x - a.q_groups;
   const uint32_t heads = is_q ? a.q_heads : a.kv_heads;
   const uint64_t x_stride = is_q ? a.q_stride : a.k_stride, dy_stride = is_q ? a.q_out_stride : a.k_out_stride;
   const T *const xs = is_q ? q : k, *const dys = is_q ? dq_out : dk_out, *const w = is_q ? wq : wk;
   T* const dxs = is_q ? dq : dk;
   float* const partials = is_q ? partials_q : partials_k;
   if (!dxs && !partials) return;
-  for (uint32_t i = threadIdx.x; i < 4u * 2u * kMostPairs; i += 256u) (&sums[0][0])[i] = 0.0f;
-  for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+  for (uint32_t i = lane; i < a.head_dim; i += 64u) sums[wave][i] = 0.0f;
+  for (uint64_t token = block; token < a.tokens; token += blocks) {
     __syncthreads();
     for (uint32_t p = threadIdx.x; p < pairs; p += 256u) turns[p] = turn_of((double)positions[token] * frequencies[p]);
     __syncthreads();
@@ -183,7 +184,7 @@ __device__ __forceinline__ void rotate_grad_any(const TilerHeads& a, const T* dq
   if (!partials) return;
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < a.head_dim; i += 256u)
-    partials[(uint64_t)blockIdx.x * a.head_dim + i] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+    partials[(uint64_t)block * a.head_dim + i] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 }
 
 // Heads in registers: a unit is two 16-byte pieces of a head, a lane's, and L lanes
@@ -441,24 +442,26 @@ __device__ __forceinline__ void rotate_grad_units(const TilerHeads& a, const T* 
   }
 }
 
-// dw from the rows of partial sums: 64 elements a workgroup, sixteen waves that
-// each add every sixteenth row.  blockIdx.y: the queries' (0) or the keys'.
+// dw from the rows of partial sums: sixteen elements a workgroup, whose 64 groups
+// of sixteen lanes each add every 64th row.  blockIdx.y: the queries' (0) or the keys'.
 template <typename T>
 __device__ __forceinline__ void rotate_sums(const float* partials_q, const float* partials_k, uint32_t count_q,
                                             uint32_t count_k, uint32_t head_dim, T* dwq, T* dwk) {
-  __shared__ float waves[16][64];
+  __shared__ float waves[16][16];
   const float* const partials = blockIdx.y ? partials_k : partials_q;
   const uint32_t count = blockIdx.y ? count_k : count_q;
   T* const dw = blockIdx.y ? dwk : dwq;
   if (!dw) return;
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i = blockIdx.x * 64u + lane;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i = blockIdx.x * 16u + (lane & 15u);
   float s = 0.0f;
   if (i < head_dim)
 #pragma unroll 8
-    for (uint32_t p = wave; p < count; p += 16u) s += partials[(uint64_t)p * head_dim + i];
-  waves[wave][lane] = s;
+    for (uint32_t p = threadIdx.x >> 4; p < count; p += 64u) s += partials[(uint64_t)p * head_dim + i];
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
+  if (lane < 16u) waves[wave][lane] = s;
   __syncthreads();
-  if (wave == 0 && i < head_dim) {
+  if (threadIdx.x < 16u && i < head_dim) {
 #pragma unroll
     for (int n = 1; n < 16; ++n) s += waves[n][lane];
     dw[i] = narrowed<T>(s);

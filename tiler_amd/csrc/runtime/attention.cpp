@@ -252,24 +252,26 @@ tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint
   char name[64];
   const bool sum_q = of_q && dwq && h.tokens, sum_k = of_k && dwk && h.tokens;
   uint32_t partials_q = 0, partials_k = 0;
-  // each workgroup leaves one row of partial sums
+  // Each workgroup leaves one row of partial sums.  In units, four to a CU, by the
+  // heads' shares; the form of any size, whose four waves take a head each, as many
+  // as LDS holds, by the rounds of heads: a token's way through it is latency (1237
+  // tokens of 7 and 1 heads, us: half as many 14.4).
   const uint32_t lanes = unit_lanes(dtype, h);
   a.each = lanes ? tokens_each(t, h) : 1;
-  const uint64_t most = 4ull * t.compute_units, all = ceil_div(h.tokens, a.each);
-  uint32_t count_q = (uint32_t)(all < most / 2 ? all : most / 2), count_k = count_q;
-  if (lanes) {  // the workgroups by the heads' shares
-    const double share = of_q && of_k ? (double)h.q_heads / ((double)h.q_heads + h.kv_heads) : 1.0;
-    const uint64_t q_most = (uint64_t)(share * (double)most), k_most = of_q ? most - q_most : most;
-    count_q = of_q ? (uint32_t)(all < q_most ? all : q_most ? q_most : 1) : 0;
-    count_k = of_k ? (uint32_t)(all < k_most ? all : k_most ? k_most : 1) : 0;
-    a.q_groups = count_q;
-  }
+  const uint64_t most = (lanes ? 4ull : 8ull) * t.compute_units, all = ceil_div(h.tokens, a.each);
+  const double of_each_q = lanes ? h.q_heads : (double)ceil_div(h.q_heads, 4);
+  const double of_each_k = lanes ? h.kv_heads : (double)ceil_div(h.kv_heads, 4);
+  const double share = of_q && of_k ? of_each_q / (of_each_q + of_each_k) : 1.0;
+  const uint64_t q_most = (uint64_t)(share * (double)most), k_most = of_q ? most - q_most : most;
+  const uint32_t count_q = of_q ? (uint32_t)(all < q_most ? all : q_most ? q_most : 1) : 0;
+  const uint32_t count_k = of_k ? (uint32_t)(all < k_most ? all : k_most ? k_most : 1) : 0;
+  a.q_groups = count_q;
   if (sum_q) partials_q = p.slot(4ull * count_q * h.head_dim, kSlotScratch);
   if (sum_k) partials_k = p.slot(4ull * count_k * h.head_dim, kSlotScratch);
   if (h.tokens && (of_q || of_k)) {
     if (lanes) std::snprintf(name, sizeof(name), "tiler_norm_rotate_grad_%s_%c%u", type_name(dtype), a.neighbours ? 'n' : 'h', lanes);
     else std::snprintf(name, sizeof(name), "tiler_norm_rotate_grad_%s_any", type_name(dtype));
-    Launch& l = (lanes ? p.add(name, count_q + count_k, 1, 256) : p.add(name, count_q, 2, 256)).blob(&a, sizeof(a), 8);
+    Launch& l = p.add(name, count_q + count_k, 1, 256).blob(&a, sizeof(a), 8);
     slot_or_null(l, of_q, dq_out);
     slot_or_null(l, of_k, dk_out);
     slot_or_null(l, of_q && a.norm, q);
@@ -285,7 +287,7 @@ tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint
   }
   if (dwq || dwk) {  // no tokens or no heads: zeros
     std::snprintf(name, sizeof(name), "tiler_norm_rotate_sum_%s", type_name(dtype));
-    Launch& l = p.add(name, (uint32_t)ceil_div(h.head_dim, 64), 2, 1024);
+    Launch& l = p.add(name, (uint32_t)ceil_div(h.head_dim, 16), 2, 1024);
     slot_or_null(l, sum_q, partials_q);
     slot_or_null(l, sum_k, partials_k);
     l.u32(sum_q ? count_q : 0).u32(sum_k ? count_k : 0).u32(h.head_dim);
@@ -317,37 +319,57 @@ constexpr StepTime kStepTimes[] = {
 };
 
 AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequences, uint64_t fresh, uint32_t heads,
-                               uint32_t group, uint32_t head_dim, uint64_t longest) {
+                               uint32_t group, uint32_t head_dim, uint64_t longest, uint64_t window, uint32_t form) {
   const uint64_t cus = t.compute_units, rows = tokens * group;
-  if (fresh * group <= 16) {
-    // Two workgroups to a CU, 256 keys at least to a part: us, 16 sequences of up to 1000
-    // keys, 8 heads, whole / in two / four / eight parts 18.9 / 16.6 / 14.3 / 15.8; 8 of up
-    // to 32000, in four / eight / sixteen 165 / 148 / 151.
+  if (form == TILER_HIP_FORM_AUTO ? fresh * group <= 16 : form == TILER_HIP_FORM_ATTENTION_FEW) {
+    // One turn of 16 rows (32 rows, two turns, us: 90, in tiles of 128 rows 58; 16 rows 25.2
+    // and 24.8; 2 rows 14.5 and 14.8; 4 rows over 32000 keys 164 and 167).  Two workgroups
+    // to a CU, 256 keys at least to a part: 16 sequences of up to 1000 keys, 8 heads, whole /
+    // in two / four / eight parts 19.1 / 16.0 / 14.5 / 16.2; 8 of up to 32000, in two / four /
+    // eight / sixteen 232 / 160 / 164 / 164.
+    const uint64_t seen = window && longest > window ? window : longest;
     uint64_t splits = ceil_div(2 * cus, mul_sat(sequences, heads));
-    if (splits > ceil_div(longest, 256)) splits = ceil_div(longest, 256);
+    if (splits > ceil_div(seen, 256)) splits = ceil_div(seen, 256);
     return {16, head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u, sequences, splits ? splits : 1};
   }
-  // The least of an estimate: the steps of a part (and four for its start and end) in
-  // as many rounds as the workgroups take, the parts' results written and joined.  us,
-  // 512 tokens of 32 and 8 heads of 128 over 8512 keys: 128 rows whole 169, in two / three /
-  // four / six parts 96 / 93 / 85 / 94; 256 rows in four 81.  Two prompts of 4096 tokens: 256
-  // rows 282, 128 rows 293.
+  // The least of an estimate: a part's steps, and two for its start and end, in the
+  // rounds that its workgroups take; past the first round the average length counts,
+  // and a tail, of the longest less what a prompt's rows, the last ones first, level out.
+  // A lone sequence's average is its middle row's; that of several, of which nothing but
+  // the longest is known, half of that.  Parts cost a launch and their results' way out
+  // and back.  The constants are the least regret (under 1 % on average) over 18
+  // batches measured in both tiles and 1 to 16 parts.
+  // us, 512 tokens of 32 and 8 heads of 128 over 8512 keys: 128 rows whole 169, in two /
+  // three / four / six parts 96 / 93 / 85 / 94; 256 rows in four 81.  Two prompts of 4096:
+  // 256 rows 282, 128 rows 293.  24 sequences of up to 150 tokens over up to 3000 keys, 35
+  // and 5 heads of 80: 128 rows whole, in two / three / four / six 69 / 62 / 60 / 61 / 75.
   const StepTime* c = kStepTimes;
   while (c->dim < head_dim) ++c;
   AttentionForm best{};
   double least = 0;
   for (const uint32_t tile : {128u, 256u}) {
     if (tile == 256 && head_dim > 128) continue;
+    if (form != TILER_HIP_FORM_AUTO && (tile == 256) != (form == TILER_HIP_FORM_ATTENTION_TILE_256)) continue;
     const double one = tile == 256 ? c->eight_alone : c->one, two = tile == 256 ? c->eight : c->two > 0 ? c->two : c->one;
     const double slots = (double)cus * (tile == 128 && c->two > 0 ? 2 : 1);
-    const double work = ((double)ceil_div(rows, tile) + 0.5 * (double)(sequences - 1)) * heads;
-    const double steps = (double)ceil_div(longest, 64) + tile / 64.0 / group;
-    for (uint64_t splits = 1; splits <= 16 && (splits == 1 || longest >= 256 * splits); ++splits) {
-      const double groups = work * (double)splits, rounds = groups / slots;
-      double us = rounds > 2 ? (rounds + 0.3) * two : std::floor(rounds) * two;
-      if (const double rest = groups - std::floor(rounds) * slots; rounds <= 2 && rest > 0) us += rest <= (double)cus ? one : two;
-      us *= steps / (double)splits + 4;
-      if (splits > 1) us += 5 + (double)rows * heads * (double)splits * head_dim * 1.2e-6;
+    const double each = (double)sequences * (double)ceil_div(fresh * group, tile);
+    double tiles = (double)ceil_div(rows, tile) + 0.3 * (double)(sequences - 1);
+    if (tokens == sequences * fresh || tiles > each) tiles = each;
+    double most = (double)longest, average = most - 0.5 * (double)(fresh < longest ? fresh : longest);
+    if (sequences > 1 && average > 0.5 * most) average = 0.5 * most;
+    const double shared = window && most > (double)window ? (double)window : most;  // by the parts
+    if (const double seen = (double)window + tile / (double)group; window && most > seen) {
+      most = seen;
+      average = average < seen ? average : seen;
+    }
+    const double leveled = (double)fresh < most ? (double)fresh : most;
+    for (uint64_t splits = 1; splits <= 64 && (splits == 1 || shared >= 256.0 * (double)splits); splits += 1 + splits / 8) {
+      const double groups = tiles * heads * (double)splits, by = 64.0 * (double)splits;
+      const double beside_us = 0.8 * (most / by + 2) * two;
+      double us = (most / by + 2) * one;
+      if (groups > slots) us = groups / slots * (average / by + 2) * two + 0.5 * ((most - 0.6 * leveled) / by + 2) * one;
+      else if (groups > (double)cus && beside_us > us) us = beside_us;
+      if (splits > 1) us += 4 + (double)rows * heads * (double)splits * head_dim * 2e-6;
       if (!best.rows || us < least) best = {tile, c->dim, rows / tile + sequences, splits}, least = us;
     }
   }
@@ -359,7 +381,8 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
 // Slots: q, k, v, [table,] starts, lengths, out, [partial results, their maxima
 // and sums: scratch].
 tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_attention_shape& a,
-                                           const tiler_hip_paged_cache& cache, const uintptr_t* addr, Program& p) {
+                                           const tiler_hip_paged_cache& cache, const uintptr_t* addr, Program& p,
+                                           uint32_t form) {
   uint64_t cached = 0;
   if (tiler_hip_status st = check_cache(cache, p, cached); st != TILER_HIP_OK) return st;
   if (a.reserved) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "attention shape: reserved is not 0");
@@ -369,6 +392,10 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "heads of 8 to 256 elements, a multiple of 8");
   if (!(a.scale > 0.0f) || !std::isfinite(a.scale))
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (form != TILER_HIP_FORM_AUTO && (form < TILER_HIP_FORM_ATTENTION_FEW || form > TILER_HIP_FORM_ATTENTION_TILE_256))
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "form: not one of attention's");
+  if (form == TILER_HIP_FORM_ATTENTION_TILE_256 && cache.head_dim > 128)
+    return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "head-size: tiles of 256 rows hold heads of up to 128 elements");
   const uint64_t row = (uint64_t)a.q_heads * cache.head_dim;
   if (a.tokens > 1 && (a.q_stride < row || a.out_stride < row))
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
@@ -410,9 +437,9 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   s.head_stride = head_stride;
   const uint64_t room = a.table_width * cache.page;
   uint64_t longest = a.max_length && a.max_length < room ? a.max_length : room;
-  if (a.window && longest > (uint64_t)a.window + a.sinks) longest = (uint64_t)a.window + a.sinks;
+  const uint64_t window = a.window ? (uint64_t)a.window + a.sinks : 0;
   const uint64_t fresh = a.max_fresh && a.max_fresh < a.tokens ? a.max_fresh : a.tokens;
-  const AttentionForm f = choose_attention(t, a.tokens, a.sequences, fresh, cache.heads, s.group, s.head_dim, longest);
+  const AttentionForm f = choose_attention(t, a.tokens, a.sequences, fresh, cache.heads, s.group, s.head_dim, longest, window, form);
   const uint64_t splits = f.splits, alone = mul_sat(f.tiles, s.kv_heads);
   s.splits = (uint32_t)splits;
   if (mul_sat(alone, splits) > 0xffffffffull / 512)

@@ -253,6 +253,7 @@ tiler_hip_status plan_norm_rotate(const Target& t, uint32_t dtype, uint32_t part
 tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint32_t parts,
                                            const tiler_hip_head_layout& h, const uintptr_t* addr, Program& p);
 tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_attention_shape& a,
-                                           const tiler_hip_paged_cache& cache, const uintptr_t* addr, Program& p);
+                                           const tiler_hip_paged_cache& cache, const uintptr_t* addr, Program& p,
+                                           uint32_t form = TILER_HIP_FORM_AUTO);
 
 }  // namespace tiler_rt

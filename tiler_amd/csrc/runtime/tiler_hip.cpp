@@ -2536,6 +2536,7 @@ static tiler_hip_status plan_region(const tiler_hip_context* ctx, const tiler_hi
                     "a flushing subnormal mode is not realized for this program (the device preserves subnormals)");
   // Forms belong to the softmax and the td,od->to bf16 contraction.
   if (r->form != TILER_HIP_FORM_AUTO && r->program != TILER_HIP_PROGRAM_SOFTMAX &&
+      r->program != TILER_HIP_PROGRAM_PAGED_ATTENTION &&
       !(r->program == TILER_HIP_PROGRAM_CONTRACTION && !r->structure && r->dtype == TILER_HIP_BF16))
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "form: this program has one form");
   // A live extent belongs to the contraction (LiveContraction, schedule/model.rs:1429-1450).
@@ -2767,7 +2768,7 @@ static tiler_hip_status plan_region(const tiler_hip_context* ctx, const tiler_hi
       else if (r->variant) st = p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "paged attention variant");
       else if (!fit) st = p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: sizes of 2^32 and more");
       else if (!c.reassociate) st = needs_reassociation("paged attention");
-      else st = tiler_rt::plan_paged_attention_bf16(t, a, cache, addr, p);
+      else st = tiler_rt::plan_paged_attention_bf16(t, a, cache, addr, p, r->form);
       break;
     }
     default:
@@ -3099,6 +3100,25 @@ tiler_hip_status tiler_hip_propose(const tiler_hip_context* ctx, const tiler_hip
         const int i = regrouping(f.strategy, v, extent, false);
         if (i >= 0 && auto_ok && autop.nlaunches && out->proposals[i].dispatch_count == autop.nlaunches &&
             std::strcmp(out->proposals[i].symbols[0], autop.launches[0].symbol) == 0)
+          chosen = i;
+      }
+      break;
+    }
+    case TILER_HIP_PROGRAM_PAGED_ATTENTION: {
+      static const struct {
+        const char* strategy;
+        uint32_t form;
+      } forms[] = {{"gfx950.attention.few-rows", TILER_HIP_FORM_ATTENTION_FEW},
+                   {"gfx950.attention.tiles-128", TILER_HIP_FORM_ATTENTION_TILE_128},
+                   {"gfx950.attention.tiles-256", TILER_HIP_FORM_ATTENTION_TILE_256}};
+      tiler_rt::Program autop;
+      const bool auto_ok = reassociate && plan_region(ctx, &base, autop) == TILER_HIP_OK;
+      for (const auto& f : forms) {
+        tiler_hip_region v = base;
+        v.form = f.form;
+        const int i = regrouping(f.strategy, v, e[7], false);
+        if (i >= 0 && auto_ok &&
+            (!autop.nlaunches || std::strcmp(out->proposals[i].symbols[0], autop.launches[0].symbol) == 0))
           chosen = i;
       }
       break;
