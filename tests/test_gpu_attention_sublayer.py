@@ -282,6 +282,29 @@ def test_every_form(ctx, dim, heads, kv_heads, lengths, page, window, sinks):
     b.free()
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("of", ["keys", "values"])
+def test_nan_reaches_the_rows_that_see_it(ctx, dim, of):
+    """In every form, the keys in parts: a row of nothing else but one, rows of many
+    others; the rows before it keep out of it where a key is meant."""
+    b = Batch([(1900, 40), (0, 3)], 4, 2, dim, page=16, seed=dim, width=130)
+    want, bound = b.want()
+    for s, j in ((0, 1920), (1, 0)):
+        up = b.k_up if of == "keys" else b.v_up
+        up[b.table[s, j // 16], j % 16] = 0x7FC0
+    q, k, v, table, starts, lens, out = b.upload(ctx)
+    region, kw = region_of(b)
+    for p in propose(*region, ctx=ctx, **kw).proposals:
+        assert len(p.symbols) == 2  # joined
+        routed(ctx, p.realize(ctx), [q, k, v, table, starts, lens], [out])
+        got = widen(out.download(np.uint16, (b.tokens, b.out_stride))).reshape(want.shape)
+        sees = np.r_[20:40, 40:43]
+        assert np.isnan(got[sees]).all(), p.symbols
+        if of == "keys":
+            assert (np.abs(got[:20] - want[:20]) <= bound[:20]).all(), p.symbols
+    b.free()
+
+
 def test_rows_for_tiles_of_256(ctx):
     """Work enough that they are chosen, whole and in parts of the keys."""
     for lengths, heads, kv_heads, window in (([(0, 4096), (0, 4096)], 16, 1, 64), ([(3000, 300)], 32, 8, 0)):

@@ -715,32 +715,53 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   }
 }
 
-// The parts of the keys joined, in order, four elements of a row a thread.
+// The parts of the keys joined, in order, four elements of a row a thread and four
+// parts at a time: their sums and results are read at once, ahead of the maximum that
+// weighs them and of the list that says which rows are any sequence's.
 __device__ __forceinline__ void join(const TilerAttentionShape& a, const int32_t* __restrict__ starts,
                                      const float* __restrict__ part_o, const tiler::f32x2_pair* __restrict__ part_ml,
                                      uint16_t* __restrict__ out) {
   const uint32_t heads = a.kv_heads * a.group, quads = a.head_dim / 4u;
   const int32_t said = starts[a.sequences];
-  const uint32_t tokens = said < 0 ? 0u : (uint32_t)said < a.tokens ? (uint32_t)said : a.tokens;
-  const uint64_t all = (uint64_t)tokens * heads * quads;
+  const uint64_t all = (uint64_t)a.tokens * heads * quads;
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
     const uint32_t row = (uint32_t)(i / quads), d = (uint32_t)(i - (uint64_t)row * quads) * 4u;
     const tiler::f32x2_pair* ml = part_ml + (uint64_t)row * a.splits;
     const float* const from = part_o + (uint64_t)row * a.splits * a.head_dim + d;
-    float top = kHidden, total = 0.0f;
-#pragma unroll 4
-    for (uint32_t z = 0; z < a.splits; ++z) top = fmaxf(top, ml[z].x);
-    const float shift = top == kHidden ? 0.0f : -top * a.scale;
+    float m = kHidden, total = 0.0f;
     f32x4 sum = {0, 0, 0, 0};
-#pragma unroll 4
-    for (uint32_t z = 0; z < a.splits; ++z) {
-      const tiler::f32x2_pair at = ml[z];
-      const float weight = exp2_fast(__builtin_fmaf(at.x, a.scale, shift));
-      total += weight * at.y;
-      sum += weight * __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(from + z * a.head_dim));
+    for (uint32_t z0 = 0; z0 < a.splits; z0 += 4u) {
+      tiler::f32x2_pair of[4];
+      f32x4 o[4];
+#pragma unroll
+      for (uint32_t z = 0; z < 4u; ++z) {
+        const uint32_t at = z0 + z < a.splits ? z0 + z : a.splits - 1u;
+        of[z] = ml[at];
+        o[z] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(from + (uint64_t)at * a.head_dim));
+      }
+      float top = m;
+#pragma unroll
+      for (uint32_t z = 0; z < 4u; ++z) {
+        const bool there = z0 + z < a.splits;
+        of[z] = there ? of[z] : tiler::f32x2_pair{kHidden, 0.0f};
+        o[z] = there ? o[z] : f32x4{0, 0, 0, 0};
+        top = fmaxf(top, of[z].x);
+      }
+      const float shift = top == kHidden ? 0.0f : -top * a.scale;
+      const float before = exp2_fast(__builtin_fmaf(m, a.scale, shift));
+      m = top;
+      total *= before;
+      sum *= before;
+#pragma unroll
+      for (uint32_t z = 0; z < 4u; ++z) {
+        const float weight = exp2_fast(__builtin_fmaf(of[z].x, a.scale, shift));
+        total += weight * of[z].y;
+        sum += weight * o[z];
+      }
     }
     const float by = total == 0.0f ? 0.0f : 1.0f / total;
     const uint32_t token = row / heads, h = row - token * heads;
+    if ((int32_t)token >= said) continue;
     const u32x2 y = {narrow2(sum[0] * by, sum[1] * by), narrow2(sum[2] * by, sum[3] * by)};
     *reinterpret_cast<u32x2_any*>(out + (uint64_t)token * a.out_stride + (uint64_t)h * a.head_dim + d) = y;
   }
