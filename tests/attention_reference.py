@@ -136,7 +136,7 @@ def paged_attention(q, k, v, table, starts, lengths, scale, window, sinks, out):
                 if not len(j):
                     out[rows] = 0.0
                     continue
-                of_j = slice(0, len(j)) if len(j) == j[-1] + 1 else j  # no copy where nothing is left out
+                of_j = slice(j[0], j[-1] + 1) if len(j) == j[-1] - j[0] + 1 else j  # no copy where nothing lies between
                 kj, vj = kk[of_j], vv[of_j]
                 logits = scale * (q[rows] @ kj.T)
                 top = logits.max(1, keepdims=True)

@@ -305,6 +305,31 @@ def test_nan_reaches_the_rows_that_see_it(ctx, dim, of):
     b.free()
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads,lengths,window,sinks", [
+    (64, 64, 8, [(900, 275), (3000, 257), (0, 275), (400, 265)], 1030, 3), (256, 64, 8, [(2200, 273), (90, 273)], 1100, 0),
+    (96, 192, 8, [(2000, 350)], 800, 30), (128, 192, 8, [(10, 175), (3000, 172), (9, 3)], 1100, 0)])
+def test_a_last_round_in_parts(ctx, dim, heads, kv_heads, lengths, window, sinks):
+    """Equal tiles a few more than fill the CUs: whole ones, then parts of the others;
+    sequences that end inside tiles of either kind."""
+    b = Batch(lengths, heads, kv_heads, dim, page=32, window=window, sinks=sinks, pad=5, gap=2, seed=dim)
+    want, bound = b.want()
+    q, k, v, table, starts, lens, out = b.upload(ctx)
+    region, kw = region_of(b)
+    joins = []
+    for p in propose(*region, ctx=ctx, **kw).proposals[1:]:
+        joins += p.symbols[1:]
+        out.upload(np.full((b.tokens, b.out_stride), 0x40A8, np.uint16))
+        for _ in range(2):
+            routed(ctx, p.realize(ctx), [q, k, v, table, starts, lens], [out])
+            got = widen(out.download(np.uint16, (b.tokens, b.out_stride)))
+            off = np.abs(got[:, :heads * dim].reshape(want.shape) - want)
+            assert (off <= bound).all(), f"{p.symbols}: worst {np.nanmax(off / np.maximum(bound, 1e-30))} of the bound"
+            assert (got[:, heads * dim:] == 5.25).all(), p.symbols
+    assert any("_join_t" in j for j in joins)
+    b.check(ctx)
+    b.free()
+
+
 def test_rows_for_tiles_of_256(ctx):
     """Work enough that they are chosen, whole and in parts of the keys."""
     for lengths, heads, kv_heads, window in (([(0, 4096), (0, 4096)], 16, 1, 64), ([(3000, 300)], 32, 8, 0)):

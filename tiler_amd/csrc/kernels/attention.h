@@ -17,7 +17,7 @@ struct TilerAttentionShape {
   float scale;                                  // of the logits, times log2(e)
   TilerDivisor page, groups;
   uint32_t page_stride, token_stride;           // of the cache, elements; a page's tokens span less than 2^32
-  uint32_t reserved;
+  uint32_t whole;                               // of the tiles: the first workgroups, which take all keys; the others' keys are split
   uint64_t q_stride, out_stride;                // elements from token to token
   uint64_t head_stride;
 };

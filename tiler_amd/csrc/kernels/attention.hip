@@ -90,6 +90,54 @@ struct Sequence {
   }
 };
 
+// Which rows a tile of kRows has.  Sequence s has the tiles from starts[s] * group /
+// kRows + s on: as many as its rows need, or one more.  Its lists' entries come
+// along with the search.
+template <uint32_t kRows>
+struct Tile {
+  uint32_t before = 0, in = 0;  // sequence s = before - 1 (0: none), and its tile
+  int32_t start = 0, next = 0, length = 0;
+  __device__ __forceinline__ Tile(const TilerAttentionShape& a, const int32_t* starts, const int32_t* lengths, uint32_t tile) {
+    const uint32_t lane = threadIdx.x & 63u;
+    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64u) {
+      const uint32_t n = s0 + lane, at = n < a.sequences ? n : a.sequences - 1u;
+      const int32_t starts_here = starts[at], next_here = starts[at + 1u], length_here = lengths[at];
+      const int32_t cut = starts_here < 0 ? 0 : starts_here > (int32_t)a.tokens ? (int32_t)a.tokens : starts_here;
+      const uint32_t from = (uint32_t)cut * a.group / kRows + n;
+      const uint64_t mask = __ballot(n < a.sequences && from <= tile);
+      if (mask) {
+        const int last = 63 - __builtin_clzll(mask);
+        in = tile - (uint32_t)__builtin_amdgcn_readlane(from, last);
+        start = __builtin_amdgcn_readlane(starts_here, last);
+        next = __builtin_amdgcn_readlane(next_here, last);
+        length = __builtin_amdgcn_readlane(length_here, last);
+      }
+      before += __popcll(mask);
+      if (mask != ~0ull) break;
+    }
+  }
+};
+
+// What a workgroup of the tiles does: with `whole` zero, every tile's keys in `splits`
+// parts, a tile's and head's parts one after another; else the first `whole` tiles (times
+// heads) whole, and the others' keys in parts, every first part before every second.
+// Either way a head's workgroups are a multiple of the heads apart, on as few XCDs as can be.
+struct Work {
+  uint32_t head, tile, split = 0, splits = 1, part = 0;  // part: the split tile's number among them
+  __device__ __forceinline__ Work(const TilerAttentionShape& a, uint32_t block, uint32_t rest) {
+    uint32_t at = block;
+    if (block >= a.whole) {
+      const uint32_t in = block - a.whole;
+      splits = a.splits;
+      split = a.whole ? in / rest : in / a.kv_heads % splits;
+      part = a.whole ? in % rest : in / (a.kv_heads * splits) * a.kv_heads + in % a.kv_heads;
+      at = a.whole + part;
+    }
+    head = at % a.kv_heads;
+    tile = (a.whole + rest) / a.kv_heads - 1u - at / a.kv_heads;
+  }
+};
+
 // The keys a run of rows sees, in steps of `kStep`: first the steps of the
 // sinks before the window, then those from the window's first key on.
 template <uint32_t kStep>
@@ -377,39 +425,20 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   constexpr int NC = 2 * NS;  // depth steps of 16 elements
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t col = lane & 31u, h = lane >> 5;
-  const uint32_t head = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads % a.splits;
-  const uint32_t at_tile = gridDim.x / (a.kv_heads * a.splits) - 1u - blockIdx.x / (a.kv_heads * a.splits);
-  // Sequence s has the tiles from starts[s] * group / kRows + s on: as many as its
-  // rows need, or one more.  Its lists' entries come along with the search.
-  uint32_t before = 0, tile_in = 0;
-  int32_t start = 0, next = 0, length = 0;
-  for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64u) {
-    const uint32_t n = s0 + lane, at = n < a.sequences ? n : a.sequences - 1u;
-    const int32_t starts_here = starts[at], next_here = starts[at + 1u], length_here = lengths[at];
-    const int32_t cut = starts_here < 0 ? 0 : starts_here > (int32_t)a.tokens ? (int32_t)a.tokens : starts_here;
-    const uint32_t from = (uint32_t)cut * a.group / kRows + n;
-    const uint64_t mask = __ballot(n < a.sequences && from <= at_tile);
-    if (mask) {
-      const int last = 63 - __builtin_clzll(mask);
-      tile_in = at_tile - (uint32_t)__builtin_amdgcn_readlane(from, last);
-      start = __builtin_amdgcn_readlane(starts_here, last);
-      next = __builtin_amdgcn_readlane(next_here, last);
-      length = __builtin_amdgcn_readlane(length_here, last);
-    }
-    before += __popcll(mask);
-    if (mask != ~0ull) break;
-  }
-  if (before == 0) return;
-  const uint32_t s = before - 1u;
-  const Sequence seq(a, start, next, length);
+  const Work work(a, blockIdx.x, (gridDim.x - a.whole) / a.splits);
+  const uint32_t head = work.head, split = work.split, splits = work.splits;
+  const Tile<kRows> place(a, starts, lengths, work.tile);
+  if (place.before == 0) return;
+  const uint32_t s = place.before - 1u, tile_in = place.in;
+  const Sequence seq(a, place.start, place.next, place.length);
   const uint32_t rows = seq.fresh * a.group, row0 = tile_in * kRows;
   if (row0 >= rows) return;
   const int32_t* const pages = table + (uint64_t)s * a.width;
   const uint32_t real_pieces = a.head_dim / 8u;
   auto position = [&](uint32_t row) { return seq.kept + (int32_t)divide(a.groups, row < rows ? row : rows - 1u); };
   const Keys<64> keys(a, position(row0), position(row0 + kRows - 1u));
-  const uint32_t begin = (uint32_t)((uint64_t)keys.steps * split / a.splits);
-  const uint32_t end = (uint32_t)((uint64_t)keys.steps * (split + 1u) / a.splits);
+  const uint32_t begin = (uint32_t)((uint64_t)keys.steps * split / splits);
+  const uint32_t end = (uint32_t)((uint64_t)keys.steps * (split + 1u) / splits);
   const uint32_t wave_row = row0 + wave * 32u;
   const bool works = wave_row < rows;
   const int32_t p_first = position(wave_row), p_last = position(wave_row + 31u);
@@ -691,8 +720,8 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
   const float total = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
   const uint64_t token_row = seq.first + token;
-  if (a.splits > 1u) {
-    const uint64_t at = (token_row * (a.kv_heads * a.group) + hq) * a.splits + split;
+  if (splits > 1u) {
+    const uint64_t at = (a.whole ? (uint64_t)work.part * kRows + (row - row0) : token_row * (a.kv_heads * a.group) + hq) * splits + split;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
@@ -715,9 +744,46 @@ __device__ __forceinline__ void tile(const TilerAttentionShape& a, const uint16_
   }
 }
 
-// The parts of the keys joined, in order, four elements of a row a thread and four
-// parts at a time: their sums and results are read at once, ahead of the maximum that
-// weighs them and of the list that says which rows are any sequence's.
+// Four elements of a row from its parts, in order, four parts at a time: their sums
+// and results are read at once, ahead of the maximum that weighs them.
+__device__ __forceinline__ u32x2 joined(const TilerAttentionShape& a, const tiler::f32x2_pair* ml, const float* from) {
+  float m = kHidden, total = 0.0f;
+  f32x4 sum = {0, 0, 0, 0};
+  for (uint32_t z0 = 0; z0 < a.splits; z0 += 4u) {
+    tiler::f32x2_pair of[4];
+    f32x4 o[4];
+#pragma unroll
+    for (uint32_t z = 0; z < 4u; ++z) {
+      const uint32_t at = z0 + z < a.splits ? z0 + z : a.splits - 1u;
+      of[z] = ml[at];
+      o[z] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(from + (uint64_t)at * a.head_dim));
+    }
+    float top = m;
+#pragma unroll
+    for (uint32_t z = 0; z < 4u; ++z) {
+      const bool there = z0 + z < a.splits;
+      of[z] = there ? of[z] : tiler::f32x2_pair{kHidden, 0.0f};
+      o[z] = there ? o[z] : f32x4{0, 0, 0, 0};
+      top = fmaxf(top, of[z].x);
+    }
+    const float shift = top == kHidden ? 0.0f : -top * a.scale;
+    const float before = exp2_fast(__builtin_fmaf(m, a.scale, shift));
+    m = top;
+    total *= before;
+    sum *= before;
+#pragma unroll
+    for (uint32_t z = 0; z < 4u; ++z) {
+      const float weight = exp2_fast(__builtin_fmaf(of[z].x, a.scale, shift));
+      total += weight * of[z].y;
+      sum += weight * o[z];
+    }
+  }
+  const float by = total == 0.0f ? 0.0f : 1.0f / total;
+  return u32x2{narrow2(sum[0] * by, sum[1] * by), narrow2(sum[2] * by, sum[3] * by)};
+}
+
+// All rows' parts, four elements a thread, read ahead of the list that says which rows
+// are any sequence's.
 __device__ __forceinline__ void join(const TilerAttentionShape& a, const int32_t* __restrict__ starts,
                                      const float* __restrict__ part_o, const tiler::f32x2_pair* __restrict__ part_ml,
                                      uint16_t* __restrict__ out) {
@@ -726,44 +792,31 @@ __device__ __forceinline__ void join(const TilerAttentionShape& a, const int32_t
   const uint64_t all = (uint64_t)a.tokens * heads * quads;
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
     const uint32_t row = (uint32_t)(i / quads), d = (uint32_t)(i - (uint64_t)row * quads) * 4u;
-    const tiler::f32x2_pair* ml = part_ml + (uint64_t)row * a.splits;
-    const float* const from = part_o + (uint64_t)row * a.splits * a.head_dim + d;
-    float m = kHidden, total = 0.0f;
-    f32x4 sum = {0, 0, 0, 0};
-    for (uint32_t z0 = 0; z0 < a.splits; z0 += 4u) {
-      tiler::f32x2_pair of[4];
-      f32x4 o[4];
-#pragma unroll
-      for (uint32_t z = 0; z < 4u; ++z) {
-        const uint32_t at = z0 + z < a.splits ? z0 + z : a.splits - 1u;
-        of[z] = ml[at];
-        o[z] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(from + (uint64_t)at * a.head_dim));
-      }
-      float top = m;
-#pragma unroll
-      for (uint32_t z = 0; z < 4u; ++z) {
-        const bool there = z0 + z < a.splits;
-        of[z] = there ? of[z] : tiler::f32x2_pair{kHidden, 0.0f};
-        o[z] = there ? o[z] : f32x4{0, 0, 0, 0};
-        top = fmaxf(top, of[z].x);
-      }
-      const float shift = top == kHidden ? 0.0f : -top * a.scale;
-      const float before = exp2_fast(__builtin_fmaf(m, a.scale, shift));
-      m = top;
-      total *= before;
-      sum *= before;
-#pragma unroll
-      for (uint32_t z = 0; z < 4u; ++z) {
-        const float weight = exp2_fast(__builtin_fmaf(of[z].x, a.scale, shift));
-        total += weight * of[z].y;
-        sum += weight * o[z];
-      }
-    }
-    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    const uint64_t at = (uint64_t)row * a.splits;
+    const u32x2 y = joined(a, part_ml + at, part_o + at * a.head_dim + d);
     const uint32_t token = row / heads, h = row - token * heads;
     if ((int32_t)token >= said) continue;
-    const u32x2 y = {narrow2(sum[0] * by, sum[1] * by), narrow2(sum[2] * by, sum[3] * by)};
     *reinterpret_cast<u32x2_any*>(out + (uint64_t)token * a.out_stride + (uint64_t)h * a.head_dim + d) = y;
+  }
+}
+
+// The split tiles' behind the whole ones: a workgroup takes 32 rows of one.
+template <uint32_t kRows>
+__device__ __forceinline__ void join_tail(const TilerAttentionShape& a, const int32_t* __restrict__ starts,
+                                          const int32_t* __restrict__ lengths, const float* __restrict__ part_o,
+                                          const tiler::f32x2_pair* __restrict__ part_ml, uint16_t* __restrict__ out) {
+  const Work work(a, a.whole + blockIdx.x, gridDim.x);
+  const Tile<kRows> place(a, starts, lengths, work.tile);
+  if (place.before == 0) return;
+  const Sequence seq(a, place.start, place.next, place.length);
+  const uint32_t rows = seq.fresh * a.group, quads = a.head_dim / 4u;
+  for (uint32_t i = threadIdx.x; i < 32u * quads; i += 256u) {
+    const uint32_t in = blockIdx.y * 32u + i / quads, d = i % quads * 4u, row = place.in * kRows + in;
+    if (row >= rows) return;
+    const uint64_t at = ((uint64_t)work.part * kRows + in) * a.splits;
+    const u32x2 y = joined(a, part_ml + at, part_o + at * a.head_dim + d);
+    const uint32_t token = divide(a.groups, row), h = work.head * a.group + (row - token * a.group);
+    *reinterpret_cast<u32x2_any*>(out + (uint64_t)(seq.first + token) * a.out_stride + (uint64_t)h * a.head_dim + d) = y;
   }
 }
 
@@ -802,4 +855,14 @@ extern "C" __global__ void __launch_bounds__(256)
     tiler_paged_attention_bf16_join(TilerAttentionShape a, const int32_t* starts, const float* part_o,
                                     const tiler::f32x2_pair* part_ml, uint16_t* out) {
   tiler_attention::join(a, starts, part_o, part_ml, out);
+}
+extern "C" __global__ void __launch_bounds__(256)
+    tiler_paged_attention_bf16_join_t128(TilerAttentionShape a, const int32_t* starts, const int32_t* lengths, const float* part_o,
+                                         const tiler::f32x2_pair* part_ml, uint16_t* out) {
+  tiler_attention::join_tail<128>(a, starts, lengths, part_o, part_ml, out);
+}
+extern "C" __global__ void __launch_bounds__(256)
+    tiler_paged_attention_bf16_join_t256(TilerAttentionShape a, const int32_t* starts, const int32_t* lengths, const float* part_o,
+                                         const tiler::f32x2_pair* part_ml, uint16_t* out) {
+  tiler_attention::join_tail<256>(a, starts, lengths, part_o, part_ml, out);
 }

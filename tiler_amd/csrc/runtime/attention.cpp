@@ -304,6 +304,7 @@ namespace {
 struct AttentionForm {
   uint32_t rows, dim;
   uint64_t tiles, splits;
+  uint64_t whole;  // of the tiles times heads: those that are not split (0: all are)
 };
 
 // us a step of 64 keys takes where a CU has one workgroup, and where it has two
@@ -330,7 +331,7 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
     const uint64_t seen = window && longest > window ? window : longest;
     uint64_t splits = ceil_div(2 * cus, mul_sat(sequences, heads));
     if (splits > ceil_div(seen, 256)) splits = ceil_div(seen, 256);
-    return {16, head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u, sequences, splits ? splits : 1};
+    return {16, head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u, sequences, splits ? splits : 1, 0};
   }
   // The least of an estimate: a part's steps, and two for its start and end, in the
   // rounds that its workgroups take; past the first round the average length counts,
@@ -370,7 +371,24 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
       if (groups > slots) us = groups / slots * (average / by + 2) * two + 0.5 * ((most - 0.6 * leveled) / by + 2) * one;
       else if (groups > (double)cus && beside_us > us) us = beside_us;
       if (splits > 1) us += 4 + (double)rows * heads * (double)splits * head_dim * 2e-6;
-      if (!best.rows || us < least) best = {tile, c->dim, rows / tile + sequences, splits}, least = us;
+      if (splits == 1 && groups > slots && average > 0.9 * most) continue;  // below
+      if (!best.rows || us < least) best = {tile, c->dim, rows / tile + sequences, splits, 0}, least = us;
+    }
+    // Equal tiles of more than one round take whole rounds; a last one that fills the CUs
+    // badly is split over them.
+    if (const double groups = tiles * heads; groups > slots && average > 0.9 * most) {
+      const double rounds = std::floor(groups / slots), rest = groups - rounds * slots;
+      const double first_us = rounds * (most / 64 + 2) * two;
+      double us = first_us;
+      if (rest > 0) us += rest <= (double)cus ? (most / 64 + 2) * one : 0.8 * (most / 64 + 2) * two;
+      if (!best.rows || us < least) best = {tile, c->dim, rows / tile + sequences, 1, 0}, least = us;
+      double parts = rest > 0 ? std::floor(slots / rest) : 1;
+      if (parts > std::floor(shared / 256)) parts = std::floor(shared / 256);
+      us = first_us + (most / 64 / parts + 2) * (rest * parts > (double)cus ? 0.8 * two : one) + 4 +
+           rest * tile * parts * head_dim * 2e-6;
+      const uint64_t whole = (uint64_t)(rounds * slots) / heads * heads;
+      if (parts >= 2 && whole && us < least)
+        best = {tile, c->dim, rows / tile + sequences, (uint64_t)parts, whole}, least = us;
     }
   }
   return best;
@@ -441,21 +459,26 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   const uint64_t fresh = a.max_fresh && a.max_fresh < a.tokens ? a.max_fresh : a.tokens;
   const AttentionForm f = choose_attention(t, a.tokens, a.sequences, fresh, cache.heads, s.group, s.head_dim, longest, window, form);
   const uint64_t splits = f.splits, alone = mul_sat(f.tiles, s.kv_heads);
+  const uint64_t whole = f.whole < alone ? f.whole : 0, split = alone - whole;  // tiles times heads
   s.splits = (uint32_t)splits;
+  s.whole = (uint32_t)whole;
   if (mul_sat(alone, splits) > 0xffffffffull / 512)
     return p.refuse(TILER_HIP_REFUSE_CAPACITY, "paged attention: more workgroups than a launch holds");
-  const uint64_t rows = a.tokens * a.q_heads;
-  const uint32_t part = splits > 1 ? p.slot(4 * mul_sat(rows * splits, s.head_dim), kSlotScratch) : 0;
-  const uint32_t ml = splits > 1 ? p.slot(8 * rows * splits, kSlotScratch) : 0;
+  const uint64_t rows = a.tokens * a.q_heads, part_rows = (whole ? split * f.rows : rows) * splits;
+  const uint32_t part = splits > 1 ? p.slot(4 * mul_sat(part_rows, s.head_dim), kSlotScratch) : 0;
+  const uint32_t ml = splits > 1 ? p.slot(8 * part_rows, kSlotScratch) : 0;
   char name[64];
   if (f.rows == 16) std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_few%u", f.dim);
   else std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_t%u_d%u", f.rows, f.dim);
-  Launch& l = p.add(name, (uint32_t)(alone * splits), 1, f.rows == 256 ? 512 : 256).blob(&s, sizeof(s), 8).ptr(q).ptr(k).ptr(v);
+  Launch& l = p.add(name, (uint32_t)(whole + split * splits), 1, f.rows == 256 ? 512 : 256).blob(&s, sizeof(s), 8).ptr(q).ptr(k).ptr(v);
   slot_or_null(l, table, at);
   l.ptr(starts).ptr(lengths).ptr(out);
   slot_or_null(l, splits > 1, part);
   slot_or_null(l, splits > 1, ml);
-  if (splits > 1) {
+  if (splits > 1 && whole) {
+    std::snprintf(name, sizeof(name), "tiler_paged_attention_bf16_join_t%u", f.rows);
+    p.add(name, (uint32_t)split, f.rows / 32, 256).blob(&s, sizeof(s), 8).ptr(starts).ptr(lengths).ptr(part).ptr(ml).ptr(out);
+  } else if (splits > 1) {
     const uint64_t groups = ceil_div(rows * (s.head_dim / 4), 256);
     p.add("tiler_paged_attention_bf16_join", (uint32_t)(groups < 16384 ? groups : 16384), 1, 256)
         .blob(&s, sizeof(s), 8).ptr(starts).ptr(part).ptr(ml).ptr(out);

@@ -431,6 +431,8 @@ const EntryRow kEntries[] = {
     {"tiler_paged_attention_bf16_t256_d96", "paged-attention-bf16", 9},
     {"tiler_paged_attention_bf16_t256_d128", "paged-attention-bf16", 9},
     {"tiler_paged_attention_bf16_join", "paged-attention-bf16", 4},
+    {"tiler_paged_attention_bf16_join_t128", "paged-attention-bf16", 5},
+    {"tiler_paged_attention_bf16_join_t256", "paged-attention-bf16", 5},
 };
 constexpr uint32_t kEntryCount = sizeof(kEntries) / sizeof(kEntries[0]);
 
