@@ -286,10 +286,21 @@ __device__ __forceinline__ float group_sum(float v) {
 
 constexpr uint32_t kTurnPairs = 2048;  // angles a workgroup holds: of 8 tokens of 256 pairs, say
 
-// The workgroup's tokens are `each` at a time; its tasks, heads of them, go round the
-// groups of L lanes.  HBM bounds it: 8192 tokens of 32 and 8 heads of 128 bf16 take 28 us
-// traced (6.0 TB/s), 173 in the form of any size; their gradients 46 (5.5 TB/s) and 5 for
-// the sum of the partials, 334 in the form of any size.
+// Head n of a token: of its queries, its keys or its values.
+template <typename T>
+__device__ __forceinline__ const T* head_at(const TilerHeads& a, const T* q, const T* k, const T* v, uint64_t token, uint32_t n) {
+  if (n < a.q_heads) return q + token * a.q_stride + (uint64_t)n * a.head_dim;
+  n -= a.q_heads;
+  if (n < a.kv_heads) return k + token * a.k_stride + (uint64_t)n * a.head_dim;
+  return v + token * a.v_stride + (uint64_t)(n - a.kv_heads) * a.head_dim;
+}
+
+// The workgroup's tokens are `each` at a time; their tasks, heads, go round the groups
+// of L lanes of the blockIdx.y workgroups that share them (few tokens: one task a group).
+// A task's head is read ahead, the first one before the angles.  HBM bounds it: 8192
+// tokens of 32 and 8 heads of 128 bf16 take 28 us traced (6.0 TB/s), 173 in the form of any
+// size; their gradients 46 (5.5 TB/s) and 5 for the sum of the partials, 334 in the form of
+// any size.
 template <typename T, int L, bool kNeighbours>
 __device__ __forceinline__ void rotate_units(const TilerHeads& a, const T* __restrict__ q, const T* __restrict__ k,
                                              const T* __restrict__ v, const T* __restrict__ wq, const T* __restrict__ wk,
@@ -299,7 +310,7 @@ __device__ __forceinline__ void rotate_units(const TilerHeads& a, const T* __res
   constexpr int V = tiler_rows::kVec<T>;
   constexpr uint32_t kGroups = 256 / L;
   __shared__ __attribute__((aligned(16))) tiler::f32x2_pair turns[kTurnPairs];
-  const uint32_t group = threadIdx.x / L, pairs = a.rotary / 2u, each = a.each;
+  const uint32_t group = blockIdx.y * kGroups + threadIdx.x / L, step = gridDim.y * kGroups, pairs = a.rotary / 2u, each = a.each;
   const uint32_t heads = a.q_heads + a.kv_heads + (v ? a.kv_heads : 0u);
   const Unit<T, kNeighbours> unit(a, threadIdx.x % L);
   Pieces<T> of_q, of_k;
@@ -307,19 +318,25 @@ __device__ __forceinline__ void rotate_units(const TilerHeads& a, const T* __res
   if (wk) of_k.load(wk, unit);
   for (uint64_t token0 = (uint64_t)blockIdx.x * each; token0 < a.tokens; token0 += (uint64_t)gridDim.x * each) {
     const uint32_t count = a.tokens - token0 < each ? (uint32_t)(a.tokens - token0) : each;
+    uint32_t in = group / heads, n = group - in * heads;  // the task's token, and its head
+    Pieces<T> ahead{};
+    if (in < count) ahead.load(head_at(a, q, k, v, token0 + in, n), unit);
     if (token0 != (uint64_t)blockIdx.x * each) __syncthreads();  // the turns before are read
     for (uint32_t i = threadIdx.x; i < count * pairs; i += 256u) {
       const uint32_t t = i / pairs;
       turns[i] = turn_of((double)positions[token0 + t] * frequencies[i - t * pairs]);
     }
     __syncthreads();
-    uint32_t in = group / heads, n = group - in * heads;  // the task's token, and its head
     while (in < count) {
       const uint64_t token = token0 + in;
+      const uint32_t of = in;
       const bool is_q = n < a.q_heads, is_k = !is_q && n < a.q_heads + a.kv_heads;
       const uint32_t head = is_q ? n : is_k ? n - a.q_heads : n - a.q_heads - a.kv_heads;
-      Pieces<T> x;
-      x.load((is_q ? q + token * a.q_stride : is_k ? k + token * a.k_stride : v + token * a.v_stride) + (uint64_t)head * a.head_dim, unit);
+      Pieces<T> x = ahead;
+      const int64_t slot = slots && !is_q ? slots[token] : -1;
+      n += step;
+      while (n >= heads) n -= heads, ++in;
+      if (in < count) ahead.load(head_at(a, q, k, v, token0 + in, n), unit);
       if (is_q || is_k) {
         float u[2 * V];
         x.widen(u);
@@ -337,20 +354,15 @@ __device__ __forceinline__ void rotate_units(const TilerHeads& a, const T* __res
 #pragma unroll
           for (int e = 0; e < 2 * V; ++e) u[e] = weighted ? u[e] * r * w[e] : u[e] * r;
         }
-        if (unit.rotated) turn<V, kNeighbours>(u, turns + in * pairs + unit.pair, false);
+        if (unit.rotated) turn<V, kNeighbours>(u, turns + of * pairs + unit.pair, false);
         x.narrow(u);
       }
       if (is_q) x.store(q_out + token * a.q_out_stride + (uint64_t)head * a.head_dim, unit);
       if (is_k && k_out) x.store(k_out + token * a.k_out_stride + (uint64_t)head * a.head_dim, unit);
-      if (!is_q && slots) {
-        const int64_t slot = slots[token];
-        if (slot >= 0 && (uint64_t)slot < a.slots) {
-          const uint32_t page = (uint32_t)slot / a.page, place = (uint32_t)slot - page * a.page;
-          x.store((is_k ? k_cache : v_cache) + (uint64_t)page * a.page_stride + (uint64_t)place * a.token_stride + (uint64_t)head * a.head_stride, unit);
-        }
+      if (slot >= 0 && (uint64_t)slot < a.slots) {
+        const uint32_t page = (uint32_t)slot / a.page, place = (uint32_t)slot - page * a.page;
+        x.store((is_k ? k_cache : v_cache) + (uint64_t)page * a.page_stride + (uint64_t)place * a.token_stride + (uint64_t)head * a.head_stride, unit);
       }
-      n += kGroups;
-      while (n >= heads) n -= heads, ++in;
     }
   }
 }

@@ -30,6 +30,10 @@ __device__ __forceinline__ void block_sums(int64_t& a, int64_t& b, int64_t (&wav
   for (uint32_t w = 0; w < wave; ++w) a += waves[0][w], b += waves[1][w];
 }
 
+// n / d for n from 0 on: in 32 bits where n fits, as it nearly always does.
+__device__ __forceinline__ int64_t divided(int64_t n, uint32_t d) {
+  return (uint64_t)n >> 32 ? n / d : (int64_t)((uint32_t)n / d);
+}
 __device__ __forceinline__ int32_t saturated(int64_t v) { return v > 0x7fffffff ? 0x7fffffff : (int32_t)v; }
 
 }  // namespace tiler_slots
@@ -51,7 +55,7 @@ extern "C" __global__ void __launch_bounds__(1024)
     const bool is = s < a.sequences;
     const int32_t kept = is ? max(kept_of[s], 0) : 0, fresh = is ? max(fresh_of[s], 0) : 0;
     const int64_t length = (int64_t)kept + fresh;
-    const int64_t have = ((int64_t)kept + a.page - 1) / a.page, need = (length + a.page - 1) / a.page;
+    const int64_t have = divided((int64_t)kept + a.page - 1, a.page), need = divided(length + a.page - 1, a.page);
     const int64_t most = need < (int64_t)a.width ? need : (int64_t)a.width, fresh_pages = most > have ? most - have : 0;
     int64_t end = fresh, page_end = fresh_pages;
     block_sums(end, page_end, waves);
@@ -75,8 +79,8 @@ extern "C" __global__ void __launch_bounds__(1024)
         else low = mid + 1u;
       }
       const int64_t position = (int64_t)kept_at[low] + ((int64_t)t - (ends[low] - fresh_at[low]));
-      const int64_t j = position / a.page, in = position - j * a.page;
-      const int64_t opened = ((int64_t)kept_at[low] + a.page - 1) / a.page;
+      const int64_t j = divided(position, a.page), in = position - j * a.page;
+      const int64_t opened = divided((int64_t)kept_at[low] + a.page - 1, a.page);
       int32_t entry = -1;
       if (j < (int64_t)a.width) {
         int32_t* const at = table + (s0 + low) * a.width + j;

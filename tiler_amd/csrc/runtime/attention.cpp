@@ -205,7 +205,14 @@ tiler_hip_status plan_norm_rotate(const Target& t, uint32_t dtype, uint32_t part
   const uint32_t groups = (uint32_t)(all < (1u << 20) ? all : 1u << 20);
   if (lanes) std::snprintf(name, sizeof(name), "tiler_norm_rotate_%s_%c%u", type_name(dtype), a.neighbours ? 'n' : 'h', lanes);
   else std::snprintf(name, sizeof(name), "tiler_norm_rotate_%s_any", type_name(dtype));
-  Launch& l = p.add(name, groups, 1, 256).blob(&a, sizeof(a), 8);
+  // few tokens: workgroups that share one's heads, one a group of lanes, up to two a CU
+  uint64_t share = 1;
+  if (lanes && groups < 2 * t.compute_units) {
+    const uint64_t heads = (uint64_t)h.q_heads + h.kv_heads + (cache ? h.kv_heads : 0);
+    share = ceil_div(a.each * heads * lanes, 256);
+    if (share > 2 * t.compute_units / groups) share = 2 * t.compute_units / groups;
+  }
+  Launch& l = p.add(name, groups, (uint32_t)share, 256).blob(&a, sizeof(a), 8);
   slot_or_null(l, has_q, q);
   slot_or_null(l, has_k, k);
   slot_or_null(l, cache, v);
