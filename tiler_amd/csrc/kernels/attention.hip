@@ -191,8 +191,12 @@ __device__ __forceinline__ uint32_t value_piece(uint32_t key, uint32_t piece) {
 // ---------------------------------------------------------------------------
 // Few rows: a tile of 16 rows, four waves that take the steps of 32 keys in turn,
 // each on its own (keys to registers, values to LDS, one step ahead of the
-// products, no barrier), and a join of the waves at the end.  A decode step is
-// bound by the cache's bytes, a short one by the way to the first of them.
+// products, no barrier), and a join of the waves at the end.  16 rows fill the smaller
+// matrix instruction; eight waves and no parts to join afterwards are slower (15.4 us
+// against 14.3).  A long decode step is bound by the cache's bytes: 8 sequences of 20000 to
+// 32000 tokens, 8 heads of 128, 148 us (5.6 TB/s; 164 when each step waits for its
+// loads).  A short one is bound by five trips to memory in a row (arguments, lists, table,
+// keys, results): 16 sequences of 100 to 1000 tokens 11 us traced and 3 for the join.
 template <int NC, int WAVES>
 struct FewSpace {
   static constexpr int D = 32 * NC;
@@ -401,6 +405,17 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
 //
 // The running maximum moves only where a logit passes it by kSlack (a factor of
 // 2^8 in the weights, far inside binary32 and bf16): most steps rescale nothing.
+//
+// Heads of 128 are bound by the matrix pipe under the card's power limit: two prompts
+// of 4096 tokens, 32 heads on 8, 283 us or 972 TFLOP/s, four fifths of a library product
+// of 8192^3 (1209); the products alone, without the softmax, take 221.  512 tokens over
+// 8512 keys: 73 us and 7 for the join.  Heads of 64 have half the products for the same
+// exponentials, and the vector pipe bounds them: 826 TFLOP/s on full CUs (heads of 96,
+// 970).  Heads of 192 and 256 leave a CU one workgroup; at 256 some 160 bytes a lane do
+// not fit the 512 registers (795 TFLOP/s).
+// Slower, us on the prompts: 64 rows a wave 356; three or four steps in LDS with the
+// table's entries brought along 300; table lookups dealt out among the products 300; the
+// keys' products before the values' (registers spill), and so two steps unrolled.
 constexpr float kSlack = 8.0f;
 
 template <int I, int N, typename F>

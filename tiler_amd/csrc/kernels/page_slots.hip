@@ -7,7 +7,8 @@
 // (a few KB from L2).  A token's sequence is found among the block's sums in LDS.
 // The token that opens a page enters the page into the table; pages before that
 // are read from it, new ones computed from the list, so no workgroup reads what
-// another writes.
+// another writes.  Latency bounds it: 64 sequences of a token each 4.6 us traced, 512
+// of up to 130 tokens 6.2, and a launch from the host takes 4.4.
 #pragma once
 
 #include "common.h"
