@@ -975,7 +975,7 @@ typedef struct {
     uint64_t tokens;
     uint64_t sequences;
     uint32_t q_heads;       /* a multiple of the cache's heads: q head n reads key/value head n / (q_heads / heads) */
-    float scale;            /* of the logits; positive and finite */
+    float scale;            /* of the logits; positive, and finite times log2(e) */
     uint64_t q_stride;      /* from token to token of q and of out, elements; heads one after another */
     uint64_t out_stride;
     uint64_t table_width;   /* pages a row of the table */

@@ -53,6 +53,7 @@ def attention(s, c):
     (shape(scale=-1.0), cache(), L.REFUSE_INVALID_ARGUMENT),
     (shape(scale=float("nan")), cache(), L.REFUSE_INVALID_ARGUMENT),
     (shape(scale=float("inf")), cache(), L.REFUSE_INVALID_ARGUMENT),
+    (shape(scale=3e38), cache(), L.REFUSE_INVALID_ARGUMENT),  # not finite in steps of log2
     (shape(q_stride=511), cache(), L.REFUSE_INVALID_ARGUMENT),
     (shape(out_stride=511), cache(), L.REFUSE_INVALID_ARGUMENT),
     (shape(q_stride=0, out_stride=0, tokens=1), cache(), L.OK),  # one token has no next one

@@ -282,6 +282,24 @@ def test_every_form(ctx, dim, heads, kv_heads, lengths, page, window, sinks):
     b.free()
 
 
+def test_rows_before_the_first_sequence(ctx):
+    """starts[0] above zero: the rows before it are no sequence's and stay, in every form
+    and where parts are joined."""
+    for lengths in ([(1900, 40), (0, 3)], [(20, 9), (70, 1)]):
+        b = Batch(lengths, 4, 2, 64, page=16, seed=3, width=130, pad=9)
+        b.starts = b.starts + 5
+        want, bound = b.want()
+        q, k, v, table, starts, lens, out = b.upload(ctx)
+        region, kw = region_of(b)
+        for p in propose(*region, ctx=ctx, **kw).proposals:
+            out.upload(np.full((b.tokens, b.out_stride), 0x40A8, np.uint16))
+            routed(ctx, p.realize(ctx), [q, k, v, table, starts, lens], [out])
+            got = widen(out.download(np.uint16, (b.tokens, b.out_stride))).reshape(want.shape)
+            assert (np.abs(got - want) <= bound).all(), p.symbols
+            assert (got[:5] == 5.25).all() and (got[b.starts[-1]:] == 5.25).all(), p.symbols
+        b.free()
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("of", ["keys", "values"])
 def test_nan_reaches_the_rows_that_see_it(ctx, dim, of):

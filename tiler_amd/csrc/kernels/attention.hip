@@ -803,14 +803,14 @@ __device__ __forceinline__ void join(const TilerAttentionShape& a, const int32_t
                                      const float* __restrict__ part_o, const tiler::f32x2_pair* __restrict__ part_ml,
                                      uint16_t* __restrict__ out) {
   const uint32_t heads = a.kv_heads * a.group, quads = a.head_dim / 4u;
-  const int32_t said = starts[a.sequences];
+  const int32_t first = starts[0], said = starts[a.sequences];
   const uint64_t all = (uint64_t)a.tokens * heads * quads;
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
     const uint32_t row = (uint32_t)(i / quads), d = (uint32_t)(i - (uint64_t)row * quads) * 4u;
     const uint64_t at = (uint64_t)row * a.splits;
     const u32x2 y = joined(a, part_ml + at, part_o + at * a.head_dim + d);
     const uint32_t token = row / heads, h = row - token * heads;
-    if ((int32_t)token >= said) continue;
+    if ((int32_t)token < first || (int32_t)token >= said) continue;
     *reinterpret_cast<u32x2_any*>(out + (uint64_t)token * a.out_stride + (uint64_t)h * a.head_dim + d) = y;
   }
 }

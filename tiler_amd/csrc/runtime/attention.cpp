@@ -416,7 +416,8 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "query heads: a multiple of the cache's heads");
   if (cache.head_dim % 8 || cache.head_dim > 256)
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "heads of 8 to 256 elements, a multiple of 8");
-  if (!(a.scale > 0.0f) || !std::isfinite(a.scale))
+  const float scale = (float)((double)a.scale * 1.4426950408889634074);  // of powers of two
+  if (!(a.scale > 0.0f) || !std::isfinite(scale))
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "scale must be positive and finite");
   if (form != TILER_HIP_FORM_AUTO && (form < TILER_HIP_FORM_ATTENTION_FEW || form > TILER_HIP_FORM_ATTENTION_TILE_256))
     return p.refuse(TILER_HIP_REFUSE_UNSUPPORTED, "form: not one of attention's");
@@ -453,7 +454,7 @@ tiler_hip_status plan_paged_attention_bf16(const Target& t, const tiler_hip_atte
   s.width = (uint32_t)a.table_width;
   s.window = a.window;
   s.sinks = a.sinks;
-  s.scale = (float)((double)a.scale * 1.4426950408889634074);
+  s.scale = scale;
   s.page = divisor_of(cache.page);
   s.groups = divisor_of(s.group);
   s.q_stride = a.q_stride;
