@@ -992,14 +992,15 @@ typedef struct {
  * j < sinks:
  *   out = sum_j e^(scale q k_j) v_j / sum_j e^(scale q k_j)
  * q, out bf16 [tokens, q_heads, head_dim]; sums, maxima and the softmax in binary32,
- * its weights rounded to bf16 for the product with v and their sum alike.  Token j of sequence s lies
- * in page table[s][j / page]; an entry that names no page of the cache reads as
- * zeros, and keys past the table's width are not seen.  A row that sees no key, or
- * none with a logit above -infinity, is zeros.  Rows behind starts[sequences] are
- * left as they are.  A NaN or an infinity in a key or value reaches the rows that
- * see it; in a value also rows of its sequence that share a tile with one of those
- * (no row reads what none of its tile's sees).  starts and lengths out of order or
- * range touch nothing outside the operands.
+ * its weights rounded to bf16 for the product with v and their sum alike.  Token j
+ * of sequence s lies in page table[s][j / page]; an entry that names no page of the
+ * cache reads as zeros, and keys past the table's width are not seen.  A row that
+ * sees no key, or none with a logit above -infinity, is zeros.  Rows of no sequence
+ * (before starts[0], behind starts[sequences]) are left as they are.  A NaN or an
+ * infinity in a key or value reaches the rows that see it; in a value also rows of
+ * its sequence that share a tile with one of those (no row reads what none of its
+ * tile's sees).  starts and lengths out of order or range touch nothing outside the
+ * operands.
  * head_dim a multiple of 8 up to 256; the cache's rows start on 16 bytes
  * (TILER_HIP_REFUSE_UNSUPPORTED else); q and out at any alignment.  A page's
  * tokens span fewer than 2^32 elements, and so does the step from page to page
