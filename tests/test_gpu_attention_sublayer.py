@@ -11,6 +11,7 @@ import attention_reference as ref
 import oracle
 import tiler_amd
 from attention_reference import U16
+from test_gpu_norm_rotate import Case, backward, forward
 from test_gpu_paged_attention import Batch, bf16, widen
 from tiler_amd import _lib as L
 from tiler_amd import families
@@ -145,6 +146,41 @@ def test_served_sequences(ctx, heads, kv_heads, dim, page, window, sinks):
         ctx.synchronize()
         s.check()
     s.close()
+
+
+def test_a_large_step(ctx):
+    """Tokens enough that a workgroup takes several at a time."""
+    s = Server(ctx, 4, 4, 2, 64, 16, 200, 90, 2100, seed=6)
+    for fresh in ([1050, 3, 0, 1040], [1, 60, 900, 0]):
+        s.load(fresh)
+        s.step()
+        ctx.synchronize()
+        s.check()
+    s.close()
+
+
+@pytest.mark.parametrize("tokens", [1025, 2051, 4100])
+def test_rotation_of_several_tokens_a_workgroup(ctx, tokens):
+    for dim, rotary, pairing, dtype in ((64, 64, "halves", L.BF16), (40, 16, "neighbours", L.F32), (22, 6, "halves", L.BF16)):
+        forward(ctx, Case(tokens, 3, 1, dim, rotary, pairing, True, dtype, seed=tokens))
+        backward(ctx, Case(tokens, 3, 1, dim, rotary, pairing, True, dtype, seed=tokens))
+
+
+@pytest.mark.parametrize("sequences", [64, 65, 200])
+def test_many_sequences_in_every_form(ctx, sequences):
+    """More than a wave's worth of them, many of no new tokens: each tile finds its own."""
+    rng = np.random.default_rng(sequences)
+    lengths = [(int(k), int(f)) for k, f in zip(rng.integers(0, 90, sequences), rng.integers(-8, 9, sequences).clip(0))]
+    b = Batch(lengths, 6, 2, 64, page=8, pad=4, seed=sequences)
+    want, bound = b.want()
+    q, k, v, table, starts, lens, out = b.upload(ctx)
+    region, kw = region_of(b)
+    for p in propose(*region, ctx=ctx, **kw).proposals:
+        out.upload(np.full((b.tokens, b.out_stride), 0x40A8, np.uint16))
+        routed(ctx, p.realize(ctx), [q, k, v, table, starts, lens], [out])
+        got = widen(out.download(np.uint16, (b.tokens, b.out_stride))).reshape(want.shape)
+        assert (np.abs(got - want) <= bound).all(), p.symbols
+    b.free()
 
 
 @pytest.mark.parametrize("rows,fresh,kept,most,longest", [
@@ -325,7 +361,7 @@ def test_nan_reaches_the_rows_that_see_it(ctx, dim, of):
 
 @pytest.mark.parametrize("dim,heads,kv_heads,lengths,window,sinks", [
     (64, 64, 8, [(900, 275), (3000, 257), (0, 275), (400, 265)], 1030, 3), (256, 64, 8, [(2200, 273), (90, 273)], 1100, 0),
-    (96, 192, 8, [(2000, 350)], 800, 30), (128, 192, 8, [(10, 175), (3000, 172), (9, 3)], 1100, 0)])
+    (64, 70, 7, [(900, 275), (3000, 257), (0, 275), (400, 265)], 1030, 0), (96, 192, 8, [(2000, 350)], 800, 30), (128, 192, 8, [(10, 175), (3000, 172), (9, 3)], 1100, 0)])
 def test_a_last_round_in_parts(ctx, dim, heads, kv_heads, lengths, window, sinks):
     """Equal tiles a few more than fill the CUs: whole ones, then parts of the others;
     sequences that end inside tiles of either kind."""
