@@ -339,6 +339,10 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
     const uint64_t seen = window && longest > window ? window : longest;
     uint64_t splits = ceil_div(2 * cus, mul_sat(sequences, heads));
     if (splits > ceil_div(seen, 256)) splits = ceil_div(seen, 256);
+    // A part's time falls with their number and the join's grows with it: one sequence of
+    // 130000 keys, one key/value head, in 64 / 128 / 256 / 512 parts 43 / 37 / 49 / 78 us.
+    const uint64_t most = (uint64_t)std::sqrt((double)seen / 8.0);
+    if (splits > most) splits = most;
     return {16, head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u, sequences, splits ? splits : 1, 0};
   }
   // The least of an estimate: a part's steps, and two for its start and end, in the
