@@ -1,0 +1,46 @@
+"""The attention sublayer's requests at their ends, without a GPU: what the
+workspace queries and the recognizer answer for the largest, the widest and the
+unusual."""
+from __future__ import annotations
+
+import pytest
+
+from test_attention import attention, cache, shape
+from tiler_amd import _lib as L
+
+
+def need(tokens, sequences, heads, kv_heads, dim, **kw):
+    row = kv_heads * dim
+    status, n = attention(shape(tokens=tokens, sequences=sequences, q_heads=heads, q_stride=heads * dim, out_stride=heads * dim,
+                                table_width=64, **kw),
+                          cache(page=1024, heads=kv_heads, head_dim=dim, page_stride=1024 * row, token_stride=row, head_stride=dim))
+    assert status == L.OK
+    return n
+
+
+def most(tokens, heads, dim):
+    """Bytes that parts may take: eight of every row or 256 MB, or two rounds of workgroups
+    (512 of 128 rows, 256 from heads of more than 128 on) of the tiles behind whole ones."""
+    part = 4 * dim + 8  # results, maximum and sum in binary32
+    return max(8 * tokens * heads * part, 256 << 20, 2 * 512 * 128 * part) + 512
+
+
+@pytest.mark.parametrize("tokens,sequences,heads,kv_heads,dim,window,fresh", [
+    (814, 128, 32, 8, 256, 32768, 7), (6629, 256, 8, 8, 128, 16384, 0), (814, 128, 32, 8, 256, 32768, 0),
+    (30000, 1000, 16, 8, 64, 32768, 0), (3000, 1000, 8, 8, 128, 4096, 0)])
+def test_workspace_of_many_windowed_sequences(tokens, sequences, heads, kv_heads, dim, window, fresh):
+    assert need(tokens, sequences, heads, kv_heads, dim, window=window, max_fresh=fresh) <= most(tokens, heads, dim)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (8, 8, 128), (32, 8, 256), (16, 1, 64), (64, 8, 64), (40, 1, 8)])
+def test_workspace_is_bounded(heads, kv_heads, dim):
+    for sequences in (1, 2, 7, 24, 128, 256, 1000):
+        for each in (1, 3, 7, 30, 100, 512, 2048):
+            for tokens in {sequences * each, sequences * each * 3 // 5 + 1, sequences * each * 9}:
+                if tokens > 40000:
+                    continue
+                for window in (0, 300, 4096, 32768):
+                    for longest in (500, 8000, 65536):
+                        for fresh in (min(each, tokens), 0):
+                            n = need(tokens, sequences, heads, kv_heads, dim, window=window, max_fresh=fresh, max_length=longest)
+                            assert n <= most(tokens, heads, dim), (tokens, sequences, window, longest, fresh)

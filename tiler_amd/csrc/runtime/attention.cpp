@@ -3,6 +3,7 @@
 // cache.
 #include "../kernels/attention.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 
@@ -330,6 +331,9 @@ constexpr StepTime kStepTimes[] = {
 AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequences, uint64_t fresh, uint32_t heads,
                                uint32_t group, uint32_t head_dim, uint64_t longest, uint64_t window, uint32_t form) {
   const uint64_t cus = t.compute_units, rows = tokens * group;
+  // Parts of all rows, results in binary32: eight (16 times the output) at most, or
+  // 256 MB of them.
+  const uint64_t most_parts = std::max<uint64_t>(8, (256ull << 20) / (rows * heads * (head_dim * 4 + 8)));
   if (form == TILER_HIP_FORM_AUTO ? fresh * group <= 16 : form == TILER_HIP_FORM_ATTENTION_FEW) {
     // One turn of 16 rows (32 rows, two turns, us: 90, in tiles of 128 rows 58; 16 rows 25.2
     // and 24.8; 2 rows 14.5 and 14.8; 4 rows over 32000 keys 164 and 167).  Two workgroups
@@ -343,6 +347,7 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
     // 130000 keys, one key/value head, in 64 / 128 / 256 / 512 parts 43 / 37 / 49 / 78 us.
     const uint64_t most = (uint64_t)std::sqrt((double)seen / 8.0);
     if (splits > most) splits = most;
+    if (splits > most_parts) splits = most_parts;
     return {16, head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u, sequences, splits ? splits : 1, 0};
   }
   // The least of an estimate: a part's steps, and two for its start and end, in the
@@ -368,6 +373,8 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
     const double each = (double)sequences * (double)ceil_div(fresh * group, tile);
     double tiles = (double)ceil_div(rows, tile) + 0.3 * (double)(sequences - 1);
     if (tokens == sequences * fresh || tiles > each) tiles = each;
+    // no two sequences share a tile
+    const double own = (double)(sequences < tokens ? sequences : tokens), equal = (tiles > own ? tiles : own) * heads;
     double most = (double)longest, average = most - 0.5 * (double)(fresh < longest ? fresh : longest);
     if (sequences > 1 && average > 0.5 * most) average = 0.5 * most;
     const double shared = window && most > (double)window ? (double)window : most;  // by the parts
@@ -376,29 +383,33 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
       average = average < seen ? average : seen;
     }
     const double leveled = (double)fresh < most ? (double)fresh : most;
-    for (uint64_t splits = 1; splits <= 64 && (splits == 1 || shared >= 256.0 * (double)splits); splits += 1 + splits / 8) {
+    for (uint64_t splits = 1; splits <= 64 && splits <= most_parts && (splits == 1 || shared >= 256.0 * (double)splits); splits += 1 + splits / 8) {
       const double groups = tiles * heads * (double)splits, by = 64.0 * (double)splits;
       const double beside_us = 0.8 * (most / by + 2) * two;
       double us = (most / by + 2) * one;
       if (groups > slots) us = groups / slots * (average / by + 2) * two + 0.5 * ((most - 0.6 * leveled) / by + 2) * one;
       else if (groups > (double)cus && beside_us > us) us = beside_us;
       if (splits > 1) us += 4 + (double)rows * heads * (double)splits * head_dim * 2e-6;
-      if (splits == 1 && groups > slots && average > 0.9 * most) continue;  // below
+      if (splits == 1 && equal > slots && average > 0.9 * most) continue;  // below
       if (!best.rows || us < least) best = {tile, c->dim, rows / tile + sequences, splits, 0}, least = us;
     }
     // Equal tiles of more than one round take whole rounds; a last one that fills the CUs
-    // badly is split over them.
-    if (const double groups = tiles * heads; groups > slots && average > 0.9 * most) {
-      const double rounds = std::floor(groups / slots), rest = groups - rounds * slots;
+    // badly is split over them.  What is split is every tile that there may be behind the
+    // whole ones, most of them empty where sequences are many: their parts, and with them
+    // the scratch, are held to two rounds (67 MB on 256 CUs).
+    if (equal > slots && average > 0.9 * most) {
+      const double rounds = std::floor(equal / slots), rest = equal - rounds * slots;
       const double first_us = rounds * (most / 64 + 2) * two;
       double us = first_us;
       if (rest > 0) us += rest <= (double)cus ? (most / 64 + 2) * one : 0.8 * (most / 64 + 2) * two;
       if (!best.rows || us < least) best = {tile, c->dim, rows / tile + sequences, 1, 0}, least = us;
-      double parts = rest > 0 ? std::floor(slots / rest) : 1;
+      const uint64_t whole = (uint64_t)(rounds * slots) / heads * heads, all = (rows / tile + sequences) * heads;
+      double parts = rest > 0 ? std::floor(slots / std::ceil(rest)) : 1;
       if (parts > std::floor(shared / 256)) parts = std::floor(shared / 256);
+      const double places = whole < all ? std::floor(2 * slots / (double)(all - whole)) : 1;
+      if (parts > places) parts = places;
       us = first_us + (most / 64 / parts + 2) * (rest * parts > (double)cus ? 0.8 * two : one) + 4 +
            rest * tile * parts * head_dim * 2e-6;
-      const uint64_t whole = (uint64_t)(rounds * slots) / heads * heads;
       if (parts >= 2 && whole && us < least)
         best = {tile, c->dim, rows / tile + sequences, (uint64_t)parts, whole}, least = us;
     }
