@@ -3,9 +3,11 @@ workspace queries and the recognizer answer for the largest, the widest and the
 unusual."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 
-from test_attention import attention, cache, shape
+from test_attention import ALL_GRADS, attention, cache, rotate_region, shape
 from tiler_amd import _lib as L
 
 
@@ -44,3 +46,22 @@ def test_workspace_is_bounded(heads, kv_heads, dim):
                         for fresh in (min(each, tokens), 0):
                             n = need(tokens, sequences, heads, kv_heads, dim, window=window, max_fresh=fresh, max_length=longest)
                             assert n <= most(tokens, heads, dim), (tokens, sequences, window, longest, fresh)
+
+
+def test_every_rotation_kernel_is_tested():
+    """The heads that the GPU tests run reach each kernel that a request can be sent to."""
+    from test_gpu_attention_ends import WIDE_FORMS
+    from test_gpu_norm_rotate import FORMS
+
+    reached = set()
+    for heads, kv_heads, dim, rotary in FORMS + WIDE_FORMS:
+        for dtype in (L.BF16, L.F32):
+            for pairing in (L.ROTATE_HALVES, L.ROTATE_NEIGHBOURS):
+                kw = dict(extents=(5, heads, kv_heads, dim, rotary), dtype=dtype, pairing=pairing)
+                reached.update(rotate_region(variant=L.ROTATE_K_OUT, **kw).symbols)
+                reached.update(rotate_region(True, variant=ALL_GRADS, **kw).symbols)
+    info, registered, i = L.EntryInfo(), set(), 0
+    while L.lib().tiler_hip_payload_entry(i, ctypes.byref(info)) == L.OK:
+        registered.add(info.symbol.decode())
+        i += 1
+    assert reached == {s for s in registered if s.startswith("tiler_norm_rotate")}
