@@ -1,11 +1,17 @@
-"""The attention sublayer's calls at their ends: heads of every register form."""
+"""The attention sublayer's calls at their ends: heads of every register form,
+lists that break their contract between guarded operands, many windowed
+sequences."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
 import test_gpu_norm_rotate as rotation
+from test_gpu_attention_sublayer import region_of, routed
 from test_gpu_norm_rotate import Case, backward, forward
+from test_gpu_paged_attention import Batch, widen
 from tiler_amd import _lib as L
+from tiler_amd.realize import propose, realize, route
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +32,99 @@ def test_wide_heads(ctx, heads, kv_heads, dim, rotary, pairing, dtype):
 @pytest.mark.parametrize("heads,kv_heads,dim,rotary", WIDE_FORMS[::2])
 def test_store_of_wide_heads(ctx, heads, kv_heads, dim, rotary, layout):
     rotation.test_store(ctx, heads, kv_heads, dim, rotary, 5, layout)
+
+
+MARGIN = 4096
+
+
+class Guarded:
+    """Storage between two margins of bytes that nothing may touch."""
+
+    def __init__(self, ctx, nbytes, fill=0xA5):
+        self.nbytes, self.fill = nbytes, fill
+        self.whole = ctx.to_device(np.full(nbytes + 2 * MARGIN, fill, np.uint8))
+        self.at = self.whole.offset(MARGIN)
+
+    def reset(self):
+        self.whole.upload(np.full(self.whole.nbytes, self.fill, np.uint8))
+
+    def inside(self):
+        """The bytes between the margins, which are as they were."""
+        got = self.whole.download(np.uint8, (self.whole.nbytes,))
+        assert (got[:MARGIN] == self.fill).all() and (got[MARGIN + self.nbytes:] == self.fill).all()
+        return got[MARGIN:MARGIN + self.nbytes]
+
+
+def broken_lists(rng, sequences, tokens):
+    top, low = 2 ** 31 - 1, -2 ** 31
+    down = np.linspace(tokens, 0, sequences + 1).astype(np.int64)
+    yield down, rng.integers(0, 400, sequences)
+    yield np.where(np.arange(sequences + 1) % 2, top, low), np.where(np.arange(sequences) % 2, low, top)
+    yield np.r_[0, -5, np.full(sequences - 1, tokens)], np.full(sequences, top)
+    yield np.r_[np.zeros(sequences, np.int64), top], np.r_[np.full(sequences - 1, -1), 4000]
+    for _ in range(2):
+        yield rng.integers(-10, tokens + 10, sequences + 1), rng.integers(-10, 4000, sequences)
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,lengths,window,sinks", [
+    (64, 4, 2, [(40, 3), (10, 50), (3, 20)], 0, 0), (128, 64, 4, [(40, 30), (1900, 50), (3, 20)], 0, 0),
+    (256, 8, 2, [(2000, 1), (10, 1), (3, 1)], 0, 0), (64, 4, 2, [(2000, 9), (10, 1), (3, 90)], 70, 5),
+    (64, 64, 8, [(900, 275), (3000, 257), (0, 275), (400, 265)], 1030, 3)])
+def test_broken_lists_stay_inside(ctx, dim, heads, kv_heads, lengths, window, sinks):
+    """starts and lengths out of order and range, in every form: nothing beside out's rows
+    and the scratch is written, nothing of the inputs."""
+    b = Batch(lengths, heads, kv_heads, dim, page=32, window=window, sinks=sinks, pad=4, gap=2, seed=dim)
+    rng = np.random.default_rng(dim)
+    row, joins = heads * dim, []
+    for starts, lens in broken_lists(rng, len(lengths), b.tokens):
+        b.starts, b.lengths = starts.astype(np.int32), lens.astype(np.int32)
+        bufs = b.upload(ctx)
+        inputs, before = bufs[:6], [x.download(np.uint8, (x.nbytes,)) for x in bufs[:6]]
+        region, kw = region_of(b)
+        for p in propose(*region, ctx=ctx, **kw).proposals:
+            rz = p.realize(ctx)
+            joins += p.symbols[1:]
+            out, scratch = Guarded(ctx, b.tokens * b.out_stride * 2, 0x40), []
+            for role, nbytes in rz.slots:
+                if role == L.SLOT_SCRATCH:
+                    scratch.append(Guarded(ctx, nbytes))
+            print(p.symbols, starts, lens, flush=True)
+            routed_with(ctx, rz, inputs, out.at, [s.at for s in scratch])
+            rows = out.inside().view(np.uint16).reshape(b.tokens, b.out_stride)
+            assert (rows[:, row:] == 0x4040).all(), p.symbols
+            for s in scratch:
+                s.inside()
+                s.whole.free()
+            out.whole.free()
+            for x, was in zip(inputs, before):
+                np.testing.assert_array_equal(x.download(np.uint8, was.shape), was, str(p.symbols))
+        b.free()
+    assert window < 1000 or any("_join_t" in j for j in joins)
+
+
+def routed_with(ctx, rz, inputs, out, scratch):
+    ins, spare = iter(inputs), iter(scratch)
+    storage = [next(ins) if role == L.SLOT_INPUT else out if role == L.SLOT_OUTPUT else next(spare) for role, _ in rz.slots]
+    route(ctx, rz, storage)
+    ctx.synchronize()
+
+
+def test_many_windowed_sequences(ctx):
+    """Equal tiles of one sequence each, one round and a few more: those in parts, most of
+    which have no rows."""
+    rng = np.random.default_rng(0)
+    lengths = [(int(k), int(f)) for k, f in zip(rng.integers(1300, 1400, 33), rng.integers(26, 32, 33))]
+    b = Batch(lengths, 64, 8, 16, page=64, window=600, sinks=3, pad=40, gap=4, seed=33)
+    want, bound = b.want()
+    q, k, v, table, starts, lens, out = b.upload(ctx)
+    region, kw = region_of(b)
+    offered = [p for p in propose(*region, ctx=ctx, **kw).proposals if any("_join_t" in s for s in p.symbols)]
+    assert offered
+    for rz in [realize(*region, ctx=ctx, **kw)] + [p.realize(ctx) for p in offered]:
+        out.upload(np.full((b.tokens, b.out_stride), 0x40A8, np.uint16))
+        routed(ctx, rz, [q, k, v, table, starts, lens], [out])
+        got = widen(out.download(np.uint16, (b.tokens, b.out_stride)))
+        assert (np.abs(got[:, :1024].reshape(want.shape) - want) <= bound).all(), rz.symbols
+        assert (got[:, 1024:] == 5.25).all()
+    b.free()
+    b.check(ctx)
