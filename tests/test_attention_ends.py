@@ -9,6 +9,8 @@ import pytest
 
 from test_attention import ALL_GRADS, attention, cache, rotate_region, shape
 from tiler_amd import _lib as L
+from tiler_amd.realize import propose
+from tiler_amd.runtime import Refusal
 
 
 def need(tokens, sequences, heads, kv_heads, dim, **kw):
@@ -65,3 +67,19 @@ def test_every_rotation_kernel_is_tested():
         registered.add(info.symbol.decode())
         i += 1
     assert reached == {s for s in registered if s.startswith("tiler_norm_rotate")}
+
+
+@pytest.mark.parametrize("pairing", [L.ROTATE_HALVES, L.ROTATE_NEIGHBOURS])
+@pytest.mark.parametrize("dtype", [L.BF16, L.F32])
+def test_rotation_without_a_norm_under_the_strict_contract(dtype, pairing):
+    """Without a norm nothing is summed: no order to permit."""
+    kw = dict(dtype=dtype, pairing=pairing, eps=0)
+    for backward, variant in ((False, L.ROTATE_K_OUT), (True, L.ROTATE_DQ | L.ROTATE_DK), (True, L.ROTATE_DK)):
+        strict = rotate_region(backward, variant=variant, permissions=0, **kw)
+        assert strict.symbols and strict.symbols == rotate_region(backward, variant=variant, **kw).symbols
+        with pytest.raises(Refusal) as e:
+            rotate_region(backward, variant=variant, permissions=0, dtype=dtype, pairing=pairing)
+        assert e.value.status == L.REFUSE_UNSUPPORTED
+    offer = propose(L.PROGRAM_NORM_ROTATE, (5, 8, 2, 64, 64), dtype=dtype, variant=L.ROTATE_K_OUT, strides=(512, 128, 512, 128),
+                    grouping=(pairing,))
+    assert len(offer.proposals) == 1 and not offer.declined

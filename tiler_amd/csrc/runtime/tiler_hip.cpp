@@ -2745,7 +2745,7 @@ static tiler_hip_status plan_region(const tiler_hip_context* ctx, const tiler_hi
       h.q_out_stride = r->strides[2], h.k_out_stride = r->strides[3];
       h.eps_bits = r->scalars[0];
       if (!fit) st = p.refuse(TILER_HIP_REFUSE_CAPACITY, "head layout: sizes of 2^32 and more");
-      else if (!c.reassociate) st = needs_reassociation("the head norm's sums");
+      else if (h.eps_bits && !c.reassociate) st = needs_reassociation("the head norm's sums");
       else if (r->program == TILER_HIP_PROGRAM_NORM_ROTATE)
         st = tiler_rt::plan_norm_rotate(t, r->dtype, r->variant, h, nullptr, addr, p);
       else st = tiler_rt::plan_norm_rotate_backward(t, r->dtype, r->variant, h, addr, p);
