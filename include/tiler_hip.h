@@ -1076,7 +1076,8 @@ tiler_hip_status tiler_hip_paged_attention_bf16_workspace(const tiler_hip_contex
 #define TILER_HIP_PROGRAM_PAGED_ATTENTION 21      /* bf16, ALIGNED16; extents {tokens, sequences, table width,
                                                      pages, page, kv heads, q heads, head_dim}, strides {q, out,
                                                      page, token, head}, grouping {window, sinks, most new tokens
-                                                     of a sequence or 0}, scalars {scale bits}; variant 0 */
+                                                     of a sequence or 0}, scalars {scale bits, most tokens of a
+                                                     sequence or 0}; variant 0 */
 #define TILER_HIP_NORM_WEIGHT 1u
 #define TILER_HIP_NORM_BIAS 2u
 #define TILER_HIP_NORM_STATISTICS 4u

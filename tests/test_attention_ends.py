@@ -7,9 +7,9 @@ import ctypes
 
 import pytest
 
-from test_attention import ALL_GRADS, attention, cache, rotate_region, shape
+from test_attention import ALL_GRADS, RE, attention, bits, cache, rotate_region, shape
 from tiler_amd import _lib as L
-from tiler_amd.realize import propose
+from tiler_amd.realize import propose, realize
 from tiler_amd.runtime import Refusal
 
 
@@ -83,3 +83,19 @@ def test_rotation_without_a_norm_under_the_strict_contract(dtype, pairing):
     offer = propose(L.PROGRAM_NORM_ROTATE, (5, 8, 2, 64, 64), dtype=dtype, variant=L.ROTATE_K_OUT, strides=(512, 128, 512, 128),
                     grouping=(pairing,))
     assert len(offer.proposals) == 1 and not offer.declined
+
+
+def test_a_region_says_its_longest_sequence():
+    """The parts of the keys go by the longest sequence, as the direct call's do by
+    max_length, not by the table's room."""
+    def region(longest):
+        return realize(L.PROGRAM_PAGED_ATTENTION, (1, 1, 1000, 10, 16, 2, 8, 64), dtype=L.BF16, permissions=RE,
+                       strides=(512, 512, 16 * 128, 128, 64), grouping=(0, 0, 1), scalars=(bits(0.125), longest))
+
+    def direct(longest):
+        return attention(shape(tokens=1, sequences=1, table_width=1000, max_fresh=1, max_length=longest), cache())[1]
+
+    for longest in (0, 100, 600, 5000, 15999, 16000, 1 << 31):
+        scratch = sum(-(-n // 256) * 256 for role, n in region(longest).slots if role == L.SLOT_SCRATCH)
+        assert scratch == direct(longest), longest
+    assert len(region(100).symbols) == 1 and len(region(0).symbols) == 2

@@ -128,3 +128,19 @@ def test_many_windowed_sequences(ctx):
         assert (got[:, 1024:] == 5.25).all()
     b.free()
     b.check(ctx)
+
+
+def test_routed_by_its_longest_sequence(ctx):
+    """A region that names its longest sequence runs what the direct call with that hint
+    runs, bit for bit, in a table with room for far more."""
+    for lengths in ([(3000, 1), (20, 1)], [(900, 40), (3, 2)]):
+        b = Batch(lengths, 8, 2, 64, width=1500, seed=7)
+        want = b.run(ctx)
+        q, k, v, table, starts, lens, out = b.upload(ctx)
+        region, kw = region_of(b)
+        kw["scalars"] += (int(b.lengths.max()),)
+        out.upload(np.zeros((b.tokens, b.out_stride), np.uint16))
+        routed(ctx, realize(*region, ctx=ctx, **kw), [q, k, v, table, starts, lens], [out])
+        np.testing.assert_array_equal(out.download(np.uint16, want.shape), want)
+        b.free()
+        b.check(ctx)

@@ -2762,6 +2762,7 @@ static tiler_hip_status plan_region(const tiler_hip_context* ctx, const tiler_hi
         *fields[i] = (uint32_t)*sizes[i];
       }
       a.tokens = e[0], a.sequences = e[1], a.table_width = e[2], a.max_fresh = r->grouping[2];
+      a.max_length = r->scalars[1];
       a.q_stride = r->strides[0], a.out_stride = r->strides[1];
       std::memcpy(&a.scale, &r->scalars[0], 4);
       cache.pages = e[3];
