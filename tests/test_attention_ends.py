@@ -5,10 +5,12 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 
 from test_attention import ALL_GRADS, RE, attention, bits, cache, rotate_region, shape
 from tiler_amd import _lib as L
+from tiler_amd import families
 from tiler_amd.realize import propose, realize
 from tiler_amd.runtime import Refusal
 
@@ -99,3 +101,33 @@ def test_a_region_says_its_longest_sequence():
         scratch = sum(-(-n // 256) * 256 for role, n in region(longest).slots if role == L.SLOT_SCRATCH)
         assert scratch == direct(longest), longest
     assert len(region(100).symbols) == 1 and len(region(0).symbols) == 2
+
+
+def test_host_functions_keep_their_numbers():
+    """Numbers that do not fit what the call takes are refused, not cut: a window of -1
+    would be one of 2^32 - 1, a length of 2^31 one of nothing."""
+    q, k = np.zeros((3, 4, 64), np.uint16), np.zeros((3, 2, 64), np.uint16)
+    at, f = np.zeros(3, np.int32), np.ones(32)
+    pages, table, starts, lengths = (np.zeros((6, 4, 2, 64), np.uint16), np.zeros((2, 3), np.int32), np.zeros(3, np.int32),
+                                     np.zeros(2, np.int32))
+    wide, none = np.array([1 << 31]), np.zeros((1, 2), np.int32)
+    for call in (
+            lambda: families.paged_attention_bf16(q, pages, pages, table, starts, lengths, 1.0, window=-1),
+            lambda: families.paged_attention_bf16(q, pages, pages, table, starts, lengths, 1.0, window=1 << 32),
+            lambda: families.paged_attention_bf16(q, pages, pages, table, starts, lengths, 1.0, window=4, sinks=-1),
+            lambda: families.paged_attention_bf16(q, pages, pages, table + 0.5, starts, lengths, 1.0),
+            lambda: families.paged_attention_bf16(q, pages, pages, table.astype(np.int64) + (1 << 32), starts, lengths, 1.0),
+            lambda: families.page_slots(wide, [1], 4, [0], none),
+            lambda: families.page_slots([1], wide, 4, [0], none),
+            lambda: families.page_slots([1.5], [1], 4, [0], none),
+            lambda: families.page_slots([float("nan")], [1], 4, [0], none),
+            lambda: families.page_slots([1], [1], 4, wide, none),
+            lambda: families.page_slots([1], [1], 4, [0], none.astype(np.int64) + (1 << 33)),
+            lambda: families.page_slots([1], [1], 4, ["a"], none),
+            lambda: families.page_slots([1], [1], -4, [0], none),
+            lambda: families.page_slots([1], [1], 4, [0], none, tokens=-1),
+            lambda: families.norm_rotate(q, k, None, None, at, f, 64, eps_bits=1 << 32),
+            lambda: families.norm_rotate(q, k, None, None, at, f, -64)):
+        with pytest.raises(Refusal) as e:
+            call()
+        assert e.value.status == L.REFUSE_INVALID_ARGUMENT, str(e.value)

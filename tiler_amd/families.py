@@ -362,8 +362,21 @@ def contract_i8(a, b, a_scales, b_scales, out_dtype=np.float32, ctx=None):
 
 # --- the attention sublayer (no reference counterpart) --------------------------
 
-def _lists(values):
-    return [np.ascontiguousarray(v, dtype=np.int32).reshape(-1) for v in values]
+def _int32(values, what: str):
+    """Whole numbers as i32; refused where that would change one."""
+    a = np.asarray(values)
+    with np.errstate(invalid="ignore"):
+        b = np.ascontiguousarray(a.astype(np.int32)) if a.dtype.kind in "biuf" else None
+    if b is None or not np.array_equal(a, b):
+        raise Refusal(L.REFUSE_INVALID_ARGUMENT, what, "a list holds more than whole numbers of 32 bits")
+    return b
+
+
+def _counts(what: str, **values):
+    """Sizes that are passed on as unsigned numbers of 32 bits."""
+    for name, v in values.items():
+        if not 0 <= v < 1 << 32:
+            raise Refusal(L.REFUSE_INVALID_ARGUMENT, what, f"{name} is {v}")
 
 
 def page_slots(kept, fresh, page: int, free_pages, table, tokens: int | None = None, ctx=None):
@@ -371,12 +384,13 @@ def page_slots(kept, fresh, page: int, free_pages, table, tokens: int | None = N
     sequences hold `kept` tokens and get `fresh` more; table [sequences, width]
     names the kept tokens' pages, and the new pages come from free_pages.
     `tokens`: rows of the batch (default: the sum of fresh)."""
-    kept, fresh, free = _lists((kept, fresh, free_pages))
-    table = np.ascontiguousarray(table, dtype=np.int32)
+    kept, fresh, free = (_int32(v, "page_slots").reshape(-1) for v in (kept, fresh, free_pages))
+    table = _int32(table, "page_slots")
     if table.ndim != 2 or not len(kept) == len(fresh) == len(table):
         raise Refusal(L.REFUSE_INVALID_ARGUMENT, "page_slots", "a length of each kind and a row of the table for each sequence")
     if tokens is None:
         tokens = int(np.maximum(fresh, 0).sum(dtype=np.int64))
+    _counts("page_slots", page=page, tokens=tokens)
     n, i32 = len(kept), np.int32
 
     def launch(c, i, o):
@@ -395,6 +409,7 @@ def _heads(q, k, rotary, pairing, eps_bits, frequencies, positions, what: str):
         raise Refusal(L.REFUSE_UNSUPPORTED, what,
                       "q and k [tokens, heads, head_dim], float32 or uint16 (bf16 patterns), pairs as halves or neighbours")
     (tokens, q_heads, dim), kv_heads = q.shape, k.shape[1]
+    _counts(what, rotary=rotary, eps_bits=eps_bits)
     positions = _operand(positions, np.int32, (tokens,), what)
     frequencies = _operand(frequencies, np.float64, (rotary // 2,), what)
     layout = L.HeadLayout(tokens=tokens, q_heads=q_heads, kv_heads=kv_heads, head_dim=dim, rotary=rotary,
@@ -431,7 +446,8 @@ def paged_attention_bf16(q, k_cache, v_cache, table, starts, lengths, scale: flo
     [pages, page, kv_heads, head_dim] (bf16 patterns); rows of no sequence are 0."""
     what = "paged_attention_bf16"
     q, k_cache, v_cache = (np.ascontiguousarray(a) for a in (q, k_cache, v_cache))
-    table = np.ascontiguousarray(table, dtype=np.int32)
+    table = _int32(table, what)
+    _counts(what, window=window, sinks=sinks)
     if q.ndim != 3 or k_cache.ndim != 4 or table.ndim != 2 or q.dtype != np.uint16 or q.shape[2] != k_cache.shape[3]:
         raise Refusal(L.REFUSE_UNSUPPORTED, what, "q [tokens, heads, head_dim] and the cache [pages, page, heads, head_dim], uint16")
     k_cache, v_cache = (_operand(a, np.uint16, k_cache.shape, what) for a in (k_cache, v_cache))
