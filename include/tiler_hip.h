@@ -940,8 +940,8 @@ typedef struct {
  *   u = x w / sqrt(mean(x^2) + eps)
  *   y_i = u_i cos a - u_j sin a, y_j = u_j cos a + u_i sin a   for each pair (i, j)
  * with a = positions[token] * frequencies[pair], a product in 64 bits (frequencies
- * are f64 [rotary / 2], radians a position), cos and sin to binary32; elements
- * behind `rotary` are u.  dtype TILER_HIP_F32 or TILER_HIP_BF16 (binary32
+ * are f64 [rotary / 2], radians a position) below 2^62, cos and sin to binary32;
+ * elements behind `rotary` are u.  dtype TILER_HIP_F32 or TILER_HIP_BF16 (binary32
  * arithmetic on exactly widened operands, one narrowing of y).  wq and wk [head_dim]
  * or NULL (ones).  A head whose sum of squares passes binary32's range is not
  * normed (zeros); a NaN or an infinity in a head gives NaNs there.

@@ -144,3 +144,15 @@ def test_routed_by_its_longest_sequence(ctx):
         np.testing.assert_array_equal(out.download(np.uint16, want.shape), want)
         b.free()
         b.check(ctx)
+
+
+@pytest.mark.parametrize("dim", [64, 22])  # in registers, and the form of any size
+def test_far_angles(ctx, dim):
+    """Angles up to 2^61 keep binary32's digits: the product of position and frequency is
+    the same 64 bits here and there."""
+    for scale in (2.0 ** 10, 2.0 ** 20, 2.0 ** 22, 2.0 ** 25, 2.0 ** 30):
+        c = Case(200, 2, 1, dim, dim, "halves", False, L.F32, far=2 ** 31 - 1, seed=dim)
+        c.positions[:4] = [2 ** 31 - 1, 2 ** 24 + 1, 0, -(2 ** 31)]
+        c.frequencies = c.frequencies * scale
+        forward(ctx, c)
+        backward(ctx, c)

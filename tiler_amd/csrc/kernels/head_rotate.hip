@@ -17,13 +17,21 @@
 
 namespace tiler_heads {
 
-// (cos, sin) of an angle.  Its quarter turns come off in 64 bits, by pi / 2 in two
-// parts (a fused product is exact before its one rounding); the series for what
+// (cos, sin) of an angle below 2^62.  Its quarter turns come off in 64 bits, by pi / 2
+// in two parts (a fused product is exact before its one rounding), and once more from an
+// angle beyond 2^40, whose quotient may itself be off by turns.  The series for what
 // remains, |r| <= pi / 4, go to r^9 and r^10 and leave out less than 3e-8 of it.
 __device__ __forceinline__ tiler::f32x2_pair turn_of(double angle) {
   const double quarters = __builtin_rint(angle * 0.63661977236758134308);
   double left = __builtin_fma(-quarters, 1.57079632679489655800, angle);
   left = __builtin_fma(-quarters, 6.12323399573676603587e-17, left);
+  uint32_t turn = (uint32_t)(long long)quarters;
+  if (__builtin_fabs(angle) > 0x1p40) {
+    const double more = __builtin_rint(left * 0.63661977236758134308);
+    left = __builtin_fma(-more, 1.57079632679489655800, left);
+    left = __builtin_fma(-more, 6.12323399573676603587e-17, left);
+    turn += (uint32_t)(int)more;
+  }
   const float r = (float)left, r2 = r * r;
   float s = __builtin_fmaf(r2, 1.0f / 362880.0f, -1.0f / 5040.0f);
   s = __builtin_fmaf(r2, s, 1.0f / 120.0f);
@@ -34,7 +42,7 @@ __device__ __forceinline__ tiler::f32x2_pair turn_of(double angle) {
   c = __builtin_fmaf(r2, c, 1.0f / 24.0f);
   c = __builtin_fmaf(r2, c, -0.5f);
   c = __builtin_fmaf(r2, c, 1.0f);
-  const uint32_t turn = (uint32_t)(long long)quarters & 3u;
+  turn &= 3u;
   const float a = turn & 1u ? s : c, b = turn & 1u ? c : s;
   return tiler::f32x2_pair{turn == 1u || turn == 2u ? -a : a, turn >= 2u ? -b : b};
 }
