@@ -131,3 +131,23 @@ def test_host_functions_keep_their_numbers():
         with pytest.raises(Refusal) as e:
             call()
         assert e.value.status == L.REFUSE_INVALID_ARGUMENT, str(e.value)
+
+
+def test_gradients_of_one_side_ask_nothing_of_the_other():
+    """Without dk and dwk (dq and dwq) the strides of the keys (queries) do not matter."""
+    for norm in (0x358637BD, 0):
+        for variant, strides in ((L.ROTATE_DQ, (512, 0, 512, 0)), (L.ROTATE_DK, (0, 128, 0, 128))):
+            assert rotate_region(True, variant=variant, strides=strides, eps=norm).symbols
+            for i in (0, 1, 2, 3):
+                if strides[i]:
+                    cut = tuple(s - (n == i) for n, s in enumerate(strides))
+                    with pytest.raises(Refusal) as e:
+                        rotate_region(True, variant=variant, strides=cut, eps=norm)
+                    assert e.value.status == L.REFUSE_INVALID_ARGUMENT
+    for variant in (L.ROTATE_DQ | L.ROTATE_DK, L.ROTATE_DQ | L.ROTATE_DWK):
+        for strides in ((511, 128, 512, 128), (512, 127, 512, 128), (512, 128, 511, 128), (512, 128, 512, 127)):
+            with pytest.raises(Refusal):
+                rotate_region(True, variant=variant, strides=strides)
+    for strides in ((511, 128, 512, 128), (512, 127, 512, 128)):
+        with pytest.raises(Refusal):
+            rotate_region(variant=L.ROTATE_K_OUT, strides=strides)

@@ -83,9 +83,6 @@ tiler_hip_status check_heads(uint32_t dtype, uint32_t parts, const tiler_hip_hea
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "weights without a norm");
   if (h.q_heads > (1u << 20) || h.kv_heads > (1u << 20))
     return p.refuse(TILER_HIP_REFUSE_CAPACITY, "more than 2^20 heads");
-  const uint64_t q_row = (uint64_t)h.q_heads * h.head_dim, k_row = (uint64_t)h.kv_heads * h.head_dim;
-  if (h.tokens > 1 && (h.q_stride < q_row || h.k_stride < k_row))
-    return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
   if (h.tokens > (1ull << 40) || h.q_stride > (1ull << 40) || h.k_stride > (1ull << 40) || h.v_stride > (1ull << 40) ||
       h.q_out_stride > (1ull << 40) || h.k_out_stride > (1ull << 40) ||
       mul_sat(h.tokens, h.q_stride + h.k_stride + h.v_stride + h.q_out_stride + h.k_out_stride) > (1ull << 60))
@@ -171,7 +168,8 @@ tiler_hip_status plan_norm_rotate(const Target& t, uint32_t dtype, uint32_t part
   const bool has_q = h.q_heads, has_k = h.kv_heads, k_out = parts & TILER_HIP_ROTATE_K_OUT;
   const uint64_t elem = dtype == TILER_HIP_BF16 ? 2 : 4;
   const uint64_t q_row = (uint64_t)h.q_heads * h.head_dim, k_row = (uint64_t)h.kv_heads * h.head_dim;
-  if (h.tokens > 1 && (h.q_out_stride < q_row || (k_out && h.k_out_stride < k_row) || (cache && h.v_stride < k_row)))
+  if (h.tokens > 1 && (h.q_stride < q_row || h.k_stride < k_row || h.q_out_stride < q_row ||
+                       (k_out && h.k_out_stride < k_row) || (cache && h.v_stride < k_row)))
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
   if (has_k && !k_out && !cache) return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "the keys go nowhere");
   uint64_t cached = 0;
@@ -244,7 +242,8 @@ tiler_hip_status plan_norm_rotate_backward(const Target& t, uint32_t dtype, uint
   const bool of_q = (dq || dwq) && h.q_heads, of_k = (dk || dwk) && h.kv_heads;
   const uint64_t elem = dtype == TILER_HIP_BF16 ? 2 : 4;
   const uint64_t q_row = (uint64_t)h.q_heads * h.head_dim, k_row = (uint64_t)h.kv_heads * h.head_dim;
-  if (h.tokens > 1 && ((of_q && h.q_out_stride < q_row) || (of_k && h.k_out_stride < k_row)))
+  if (h.tokens > 1 && ((of_q && (h.q_stride < q_row || h.q_out_stride < q_row)) ||
+                       (of_k && (h.k_stride < k_row || h.k_out_stride < k_row))))
     return p.refuse(TILER_HIP_REFUSE_INVALID_ARGUMENT, "rows of heads overlap");
   auto given = [&](bool there, uint64_t bytes, uint32_t role) { return there ? p.slot(bytes, role) : 0; };
   const uint32_t dq_out = given(of_q, mul_sat(span(h.tokens, h.q_out_stride, q_row), elem), kSlotInput);
