@@ -12,6 +12,7 @@ from test_gpu_norm_rotate import Case, backward, forward
 from test_gpu_paged_attention import Batch, widen
 from tiler_amd import _lib as L
 from tiler_amd.realize import propose, realize, route
+from tiler_amd.runtime import Refusal
 
 pytestmark = pytest.mark.gpu
 
@@ -156,3 +157,25 @@ def test_far_angles(ctx, dim):
         c.frequencies = c.frequencies * scale
         forward(ctx, c)
         backward(ctx, c)
+
+
+def test_a_cache_without_pages(ctx):
+    """As in attention, one without pages has no address; no slot names it."""
+    c = Case(5, 4, 2, 64, 64, "halves", True, L.BF16, seed=1)
+    wq, wk = c.upload(ctx)
+    out, slots = ctx.alloc(5 * 4 * 64 * 2), ctx.to_device(np.array([-1, 0, 7, -1, 2 ** 31 - 1], np.int32))
+    empty = L.PagedCache(k=None, v=None, pages=0, page=16, heads=2, head_dim=64, page_stride=2048, token_stride=128, head_stride=64)
+    ctx.norm_rotate(c.dtype, c.layout(), c.d_row.ptr, c.d_row.ptr + c.part("k")[1], c.d_row.ptr + c.part("v")[1], wq, wk, c.d_pos,
+                    c.d_freq, out, None, empty, slots)
+    ctx.synchronize()
+    want, bound = c.want("q")
+    rotation.close(rotation.values(out.download(np.uint16, want.shape), L.BF16), want, bound, L.BF16, "q")
+    some = L.PagedCache.from_buffer_copy(empty)
+    some.pages = 1
+    with pytest.raises(Refusal) as e:
+        ctx.norm_rotate(c.dtype, c.layout(), c.d_row.ptr, c.d_row.ptr + c.part("k")[1], c.d_row.ptr + c.part("v")[1], wq, wk,
+                        c.d_pos, c.d_freq, out, None, some, slots)
+    assert e.value.status == L.REFUSE_INVALID_ARGUMENT
+    for b in (out, slots):
+        b.free()
+    c.free()

@@ -2271,8 +2271,8 @@ tiler_hip_status tiler_hip_norm_rotate(tiler_hip_context* ctx, uint32_t dtype, c
   if (heads->q_heads) list.add(q_out);
   list.add_given(k_out);
   if (cache) {
-    list.add(cache->k);
-    list.add(cache->v);
+    list.add(cache->k, cache->pages != 0);
+    list.add(cache->v, cache->pages != 0);
     list.add(slots);
   }
   const uint32_t parts = (wq ? TILER_HIP_ROTATE_WQ : 0u) | (wk ? TILER_HIP_ROTATE_WK : 0u) |
