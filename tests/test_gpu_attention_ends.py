@@ -179,3 +179,90 @@ def test_a_cache_without_pages(ctx):
     for b in (out, slots):
         b.free()
     c.free()
+
+
+@pytest.mark.parametrize("window,sinks", [(1 << 31, 0), (2 ** 32 - 1, 2 ** 32 - 1), (2 ** 31 - 1, 5), (40, 2 ** 32 - 1)])
+def test_windows_and_sinks_past_every_length(ctx, window, sinks):
+    """Each sees all that is before it: the results of no window."""
+    b = Batch([(300, 1), (90, 40), (0, 3), (1500, 2)], 4, 2, 64, seed=3)
+    want, bound = b.want()
+    b.window, b.sinks = window, sinks
+    q, k, v, table, starts, lens, out = b.upload(ctx)
+    region, kw = region_of(b)
+    for p in propose(*region, ctx=ctx, **kw).proposals:
+        out.upload(np.full((b.tokens, b.out_stride), 0x40A8, np.uint16))
+        routed(ctx, p.realize(ctx), [q, k, v, table, starts, lens], [out])
+        got = widen(out.download(np.uint16, (b.tokens, b.out_stride))).reshape(want.shape)
+        assert (np.abs(got - want) <= bound).all(), p.symbols
+    b.free()
+
+
+@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("length", [2 ** 31 - 1024 - 700, 2 ** 31 - 1024, 2 ** 31 - 1024 + 20, 2 ** 31 - 1])
+def test_positions_next_to_2_to_31(ctx, length, fresh):
+    """A window at the end of the longest table, first tokens visible: what a short sequence
+    of the same first and last pages gives.  Keys past the table are not seen."""
+    page, width, near, window, sinks = 1024, 2 ** 21 - 1, 8, 1500, 70
+    moved = (width - near) * page  # tokens between the pages that either sequence has
+    b = Batch([(length - moved - fresh, fresh), (30, 2)], 6, 2, 64, page=page, window=window, sinks=sinks, seed=5, width=near)
+    want, bound = b.want()
+    q, k, v, _, starts, _, out = b.upload(ctx)
+    table = np.full((2, width), -1, np.int32)
+    table[0, 0], table[0, width - near + 1:] = b.table[0, 0], b.table[0, 1:]
+    table[1, :near] = b.table[1]
+    b.lengths[0], b.width = length, width
+    wide, lens = ctx.to_device(table), ctx.to_device(b.lengths)
+    region, kw = region_of(b)
+    for p in propose(*region, ctx=ctx, **kw).proposals:
+        out.upload(np.full((b.tokens, b.out_stride), 0x40A8, np.uint16))
+        routed(ctx, p.realize(ctx), [q, k, v, wide, starts, lens], [out])
+        got = widen(out.download(np.uint16, (b.tokens, b.out_stride))).reshape(want.shape)
+        assert (np.abs(got - want) <= bound).all(), p.symbols
+    for x in (wide, lens):
+        x.free()
+    b.free()
+
+
+@pytest.mark.parametrize("dim,rotary,dtype", [(128, 128, L.BF16), (90, 34, L.F32)])
+def test_captured_gradients(ctx, dim, rotary, dtype):
+    """The rotation and its gradients in a graph, replayed on other inputs between eager
+    calls, a workspace of its own; without one the capture is refused."""
+    c = Case(300, 5, 2, dim, rotary, "halves", True, dtype, seed=1)
+    wq, wk = c.upload(ctx)
+    heads, store = c.layout(), np.uint16 if dtype == L.BF16 else np.float32
+    need = ctx.norm_rotate_backward_workspace(dtype, heads)
+    shapes = [(300, 5, dim), (300, 2, dim), (300, c.stride), (300, c.stride), (dim,), (dim,)]
+    # of the graph and of the eager calls: rotated queries and keys (which are their own gradients), dq and dk, dwq, dwk
+    sides = [[ctx.alloc(int(np.prod(s)) * c.elem) for s in shapes] + [ctx.alloc(need)] for _ in range(2)]
+    for side in sides:
+        for x, s in zip(side, shapes):
+            x.upload(np.zeros(s, store))
+
+    def step(side):
+        q, k, dq, dk, dwq, dwk, space = side
+        ctx.norm_rotate(dtype, heads, c.d_row.ptr, c.d_row.ptr + c.part("k")[1], None, wq, wk, c.d_pos, c.d_freq, q, k)
+        ctx.norm_rotate_backward(dtype, heads, q, k, c.d_row.ptr, c.d_row.ptr + c.part("k")[1], wq, wk, c.d_pos, c.d_freq,
+                                 dq, dk, dwq, dwk, workspace=space, workspace_bytes=need)
+
+    ctx.capture_begin()
+    step(sides[0])
+    with pytest.raises(Refusal) as e:
+        ctx.norm_rotate_backward(dtype, heads, *sides[0][:2], c.d_row.ptr, c.d_row.ptr + c.part("k")[1], wq, wk, c.d_pos,
+                                 c.d_freq, *sides[0][2:6])
+    graph = ctx.capture_end()
+    assert e.value.status == L.REFUSE_CAPACITY
+    for i in range(4):
+        rng = np.random.default_rng(i)
+        c.d_row.upload(rotation.stored(rng.standard_normal((300, c.stride)), dtype)[0])
+        c.d_pos.upload(rng.integers(0, 10 ** 6, 300).astype(np.int32))
+        ctx.graph_launch(graph)
+        ctx.synchronize()
+        step(sides[1])
+        ctx.synchronize()
+        for a, b, s in zip(*sides, shapes):
+            np.testing.assert_array_equal(a.download(store, s), b.download(store, s), str(i))
+    ctx.graph_destroy(graph)
+    for side in sides:
+        for x in side:
+            x.free()
+    c.free()
