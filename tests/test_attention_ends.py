@@ -4,6 +4,9 @@ unusual."""
 from __future__ import annotations
 
 import ctypes
+import os
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -13,6 +16,8 @@ from tiler_amd import _lib as L
 from tiler_amd import families
 from tiler_amd.realize import propose, realize
 from tiler_amd.runtime import Refusal
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def need(tokens, sequences, heads, kv_heads, dim, **kw):
@@ -151,3 +156,19 @@ def test_gradients_of_one_side_ask_nothing_of_the_other():
     for strides in ((511, 128, 512, 128), (512, 127, 512, 128)):
         with pytest.raises(Refusal):
             rotate_region(variant=L.ROTATE_K_OUT, strides=strides)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_planners_are_sanitizer_clean(tmp_path):
+    """tests/native/attention_planner_sanitize.cpp: 400000 requests, ordinary and extreme,
+    under the address and undefined-behaviour sanitizers; grids, parts, tiles and scratch of
+    each plan are what the kernels take them for."""
+    exe, runtime = tmp_path / "attention_planner_sanitize", os.path.join(ROOT, "tiler_amd", "csrc", "runtime")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined,float-cast-overflow,float-divide-by-zero",
+                    "-fno-sanitize-recover=all", f"-I{os.path.join(ROOT, 'include')}", f"-I{runtime}",
+                    os.path.join(ROOT, "tests", "native", "attention_planner_sanitize.cpp"),
+                    os.path.join(runtime, "attention.cpp"), os.path.join(runtime, "program.cpp"), "-o", str(exe)],
+                   check=True, capture_output=True, text=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "attention-planner-sanitize ok" in r.stdout and "runtime error" not in r.stderr

@@ -407,10 +407,10 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
       if (parts > std::floor(shared / 256)) parts = std::floor(shared / 256);
       const double places = whole < all ? std::floor(2 * slots / (double)(all - whole)) : 1;
       if (parts > places) parts = places;
+      if (parts < 2 || !whole) continue;
       us = first_us + (most / 64 / parts + 2) * (rest * parts > (double)cus ? 0.8 * two : one) + 4 +
            rest * tile * parts * head_dim * 2e-6;
-      if (parts >= 2 && whole && us < least)
-        best = {tile, c->dim, rows / tile + sequences, (uint64_t)parts, whole}, least = us;
+      if (us < least) best = {tile, c->dim, rows / tile + sequences, (uint64_t)parts, whole}, least = us;
     }
   }
   return best;
