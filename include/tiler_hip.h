@@ -868,9 +868,9 @@ tiler_hip_status tiler_hip_contract_i8(tiler_hip_context *ctx, const int8_t *a, 
  *   tiler_hip_norm_rotate           queries and keys normed and rotated, keys and
  *                                   values stored there
  *   tiler_hip_paged_attention_bf16  the new tokens' attention over the cache
- * Every call is deterministic, launches on `stream` and may be captured into a
- * graph; lengths and tables are read on the device, so that a graph replays with
- * other ones.  Workspaces as for the feed-forward sublayer.  Outputs overlap
+ * Every call is deterministic (but for two tokens of one slot), launches on `stream`
+ * and may be captured into a graph; lengths and tables are read on the device, so
+ * that a graph replays with other ones.  Workspaces as for the feed-forward sublayer.  Outputs overlap
  * neither the inputs nor one another, except that a cache is updated in place. */
 
 /* A cache of keys and values in pages of `page` tokens each: token t of page n,
@@ -944,11 +944,12 @@ typedef struct {
  * elements behind `rotary` are u.  dtype TILER_HIP_F32 or TILER_HIP_BF16 (binary32
  * arithmetic on exactly widened operands, one narrowing of y).  wq and wk [head_dim]
  * or NULL (ones).  A head whose sum of squares passes binary32's range is not
- * normed (zeros); a NaN or an infinity in a head gives NaNs there.
+ * normed (zeros), one whose squares fall below it is only by eps; a NaN or an
+ * infinity in a head gives NaNs there.
  * The queries go to q_out; the keys to k_out, and with a cache (bf16) the keys and
  * the values of v to the slots that slots[token] names: a slot outside the cache
- * (-1) stores nothing, two tokens with one slot leave either.  v, cache and slots
- * go together; k_out may be NULL with them. */
+ * (-1) stores nothing; two tokens with one slot leave a mixture, each element of
+ * either.  v, cache and slots go together; k_out may be NULL with them. */
 tiler_hip_status tiler_hip_norm_rotate(tiler_hip_context *ctx, uint32_t dtype,
                                        const tiler_hip_head_layout *heads, const void *q, const void *k,
                                        const void *v, const void *wq, const void *wk,
@@ -982,7 +983,9 @@ typedef struct {
     uint32_t window;        /* keys a query sees, its own among them; 0: all before it */
     uint32_t sinks;         /* first tokens of a sequence that stay visible under a window */
     uint64_t max_fresh;     /* the most new tokens of a sequence, and the most tokens of one with them: */
-    uint64_t max_length;    /* what the work is cut by (0: unknown); results do not depend on their being right */
+    uint64_t max_length;    /* what the work is cut by (0: unknown).  They need not be right: other hints, other
+                               orders of summation and the same results but for the rounding; the same hints,
+                               the same bits */
     uint64_t reserved;      /* 0 */
 } tiler_hip_attention_shape;
 
@@ -1003,8 +1006,11 @@ typedef struct {
  * operands.
  * head_dim a multiple of 8 up to 256; the cache's rows start on 16 bytes
  * (TILER_HIP_REFUSE_UNSUPPORTED else); q and out at any alignment.  A page's
- * tokens span fewer than 2^32 elements, and so does the step from page to page
- * (TILER_HIP_REFUSE_CAPACITY else). */
+ * tokens span fewer than 2^32 elements, and so does the step from page to page; a
+ * launch has fewer than 2^23 workgroups (sequences, or tiles of their rows, times
+ * key/value heads and parts; TILER_HIP_REFUSE_CAPACITY else).  The workspace holds
+ * the parts' results and sums: 16 times the output and 64 bytes a row at most, or
+ * 256 MB. */
 tiler_hip_status tiler_hip_paged_attention_bf16(tiler_hip_context *ctx,
                                                 const tiler_hip_attention_shape *shape, const uint16_t *q,
                                                 const tiler_hip_paged_cache *cache, const int32_t *table,

@@ -172,3 +172,20 @@ def test_planners_are_sanitizer_clean(tmp_path):
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
     assert "attention-planner-sanitize ok" in r.stdout and "runtime error" not in r.stderr
+
+
+@pytest.mark.parametrize("sequences,kv_heads,keys,parts", [
+    (1, 1, 2000, 8), (1, 1, 4000, 16), (1, 1, 8000, 31), (1, 1, 32000, 63), (1, 2, 32000, 63), (1, 1, 60000, 86), (1, 8, 32000, 63),
+    (1, 8, 60000, 64), (8, 8, 32000, 8), (16, 8, 1000, 4), (64, 8, 32000, 1)])
+def test_parts_of_few_rows(sequences, kv_heads, keys, parts):
+    """256 keys to a part at least, sqrt(keys / 8) parts at most, and the CUs' share."""
+    for group, dim in ((1, 64), (4, 128), (4, 256)):
+        n = need(sequences, sequences, group * kv_heads, kv_heads, dim, max_fresh=1, max_length=keys)
+        rows = sequences * group * kv_heads
+        up = lambda b: -(-b // 256) * 256
+        assert n == (up(4 * dim * rows * parts) + up(8 * rows * parts) if parts > 1 else 0)
+
+
+def test_more_workgroups_than_a_launch_has():
+    for sequences, status in (((1 << 22) - 1, L.OK), (1 << 22, L.REFUSE_CAPACITY), (1 << 23, L.REFUSE_CAPACITY)):
+        assert attention(shape(tokens=sequences, sequences=sequences, max_fresh=1), cache())[0] == status

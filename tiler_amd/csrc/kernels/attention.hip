@@ -407,12 +407,13 @@ __device__ __forceinline__ void few(const TilerAttentionShape& a, const uint16_t
 // 2^8 in the weights, far inside binary32 and bf16): most steps rescale nothing.
 //
 // Heads of 128 are bound by the matrix pipe under the card's power limit: two prompts
-// of 4096 tokens, 32 heads on 8, 283 us or 972 TFLOP/s, four fifths of a library product
-// of 8192^3 (1209); the products alone, without the softmax, take 221.  512 tokens over
-// 8512 keys: 73 us and 7 for the join.  Heads of 64 have half the products for the same
-// exponentials, and the vector pipe bounds them: 826 TFLOP/s on full CUs (heads of 96,
-// 970).  Heads of 192 and 256 leave a CU one workgroup; at 256 some 160 bytes a lane do
-// not fit the 512 registers (795 TFLOP/s).
+// of 4096 tokens, 32 heads on 8, 283 to 295 us from card to card or 930 to 972 TFLOP/s,
+// four fifths of a library product of 8192^3 (1209); the products alone, without the
+// softmax, take 221.  512 tokens over 8512 keys: 73 to 81 us and 7 for the join.  Heads of
+// 64 have half the products for the same exponentials, and the vector pipe bounds them:
+// 700 TFLOP/s on the same prompts (heads of 96, 879).  Heads of 192 and 256 leave a CU one
+// workgroup (674 and 655 TFLOP/s); at 256 some 160 bytes a lane do not fit the 512
+// registers.
 // Slower, us on the prompts: 64 rows a wave 356; three or four steps in LDS with the
 // table's entries brought along 300; table lookups dealt out among the products 300; the
 // keys' products before the values' (registers spill), and so two steps unrolled.

@@ -71,7 +71,9 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // Any head size, rotation and alignment: a workgroup a token, a wave a head, an
-// element a load; the head is read twice.
+// element a load; the head is read twice.  Latency bounds it: 8192 tokens of 32 and 8
+// heads of 80, 20 elements rotated, 164 us and 301 for the gradients (32 rotated, in
+// units, 27 and 44).
 template <typename T>
 __device__ __forceinline__ void rotate_any(const TilerHeads& a, const T* q, const T* k, const T* v, const T* wq,
                                            const T* wk, const int32_t* positions, const double* frequencies, T* q_out,
@@ -292,7 +294,7 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-constexpr uint32_t kTurnPairs = 2048;  // angles a workgroup holds: of 8 tokens of 256 pairs, say
+constexpr uint32_t kTurnPairs = 2048;  // angles a workgroup holds: of 4 tokens of 512 pairs
 
 // Head n of a token: of its queries, its keys or its values.
 template <typename T>
@@ -306,9 +308,10 @@ __device__ __forceinline__ const T* head_at(const TilerHeads& a, const T* q, con
 // The workgroup's tokens are `each` at a time; their tasks, heads, go round the groups
 // of L lanes of the blockIdx.y workgroups that share them (few tokens: one task a group).
 // A task's head is read ahead, the first one before the angles.  HBM bounds it: 8192
-// tokens of 32 and 8 heads of 128 bf16 take 28 us traced (6.0 TB/s), 173 in the form of any
-// size; their gradients 46 (5.5 TB/s) and 5 for the sum of the partials, 334 in the form of
-// any size.
+// tokens of 32 and 8 heads of 128 bf16 take 35 us on changing inputs (4.8 TB/s; f32 70),
+// 173 in the form of any size; their gradients 56 (4.5 TB/s) and 5 for the sum of the
+// partials (f32 107 in all), 334 in the form of any size; 4096 tokens and their values
+// stored 24 (4.3 TB/s).  Inputs that lie in the last cache take 28 and 45.
 template <typename T, int L, bool kNeighbours>
 __device__ __forceinline__ void rotate_units(const TilerHeads& a, const T* __restrict__ q, const T* __restrict__ k,
                                              const T* __restrict__ v, const T* __restrict__ wq, const T* __restrict__ wk,

@@ -331,7 +331,7 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
                                uint32_t group, uint32_t head_dim, uint64_t longest, uint64_t window, uint32_t form) {
   const uint64_t cus = t.compute_units, rows = tokens * group;
   // Parts of all rows, results in binary32: eight (16 times the output) at most, or
-  // 256 MB of them.
+  // 256 MB of them, which eight rounds of full tiles leave (256 CUs).
   const uint64_t most_parts = std::max<uint64_t>(8, (256ull << 20) / (rows * heads * (head_dim * 4 + 8)));
   if (form == TILER_HIP_FORM_AUTO ? fresh * group <= 16 : form == TILER_HIP_FORM_ATTENTION_FEW) {
     // One turn of 16 rows (32 rows, two turns, us: 90, in tiles of 128 rows 58; 16 rows 25.2
@@ -342,8 +342,11 @@ AttentionForm choose_attention(const Target& t, uint64_t tokens, uint64_t sequen
     const uint64_t seen = window && longest > window ? window : longest;
     uint64_t splits = ceil_div(2 * cus, mul_sat(sequences, heads));
     if (splits > ceil_div(seen, 256)) splits = ceil_div(seen, 256);
-    // A part's time falls with their number and the join's grows with it: one sequence of
-    // 130000 keys, one key/value head, in 64 / 128 / 256 / 512 parts 43 / 37 / 49 / 78 us.
+    // A part's time falls with their number and the join's grows with it, us for one
+    // sequence on one key/value head of 128 in half / as many / twice / four times as
+    // many parts: 8000 keys (31) 18.5 / 17.0 / 18.4 / 24.6, 32000 (63) 29.3 / 24.7 / 29.0 /
+    // 42.9, 130000 (127) 49.7 / 42.3 / 53.4 / 84; 32000 and 130000 on two heads 30.6 / 25.6
+    // / 31.6 and 52.3 / 49.8 / 63.7, on eight (the CUs' share) 38.0 / 40.3 and 105 / 110.
     const uint64_t most = (uint64_t)std::sqrt((double)seen / 8.0);
     if (splits > most) splits = most;
     if (splits > most_parts) splits = most_parts;
