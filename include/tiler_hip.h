@@ -944,7 +944,7 @@ typedef struct {
  * elements behind `rotary` are u.  dtype TILER_HIP_F32 or TILER_HIP_BF16 (binary32
  * arithmetic on exactly widened operands, one narrowing of y).  wq and wk [head_dim]
  * or NULL (ones).  A head whose sum of squares passes binary32's range is not
- * normed (zeros), one whose squares fall below it is only by eps; a NaN or an
+ * normed (zeros), one whose squares fall below it is by eps alone; a NaN or an
  * infinity in a head gives NaNs there.
  * The queries go to q_out; the keys to k_out, and with a cache (bf16) the keys and
  * the values of v to the slots that slots[token] names: a slot outside the cache
@@ -995,7 +995,8 @@ typedef struct {
  * j < sinks:
  *   out = sum_j e^(scale q k_j) v_j / sum_j e^(scale q k_j)
  * q, out bf16 [tokens, q_heads, head_dim]; sums, maxima and the softmax in binary32,
- * its weights rounded to bf16 for the product with v and their sum alike.  Token j
+ * its weights rounded to bf16 for the product with v and their sum alike; scaled
+ * logits are taken to lie in binary32's range.  Token j
  * of sequence s lies in page table[s][j / page]; an entry that names no page of the
  * cache reads as zeros, and keys past the table's width are not seen.  A row that
  * sees no key, or none with a logit above -infinity, is zeros.  Rows of no sequence
